@@ -75,14 +75,18 @@ ACL_FUNC_VISIBILITY int32_t gmmB200StreamIsCapturing(aclrtStream stream);
  *   MOE_INIT_ROUTING_V3: x, expertIdx, scale, offset, expandedX, expandedRowIdx, expertTokensCountOrCumsum, expandedScale;
  *              activeNum, expertCapacity, expertNum, dropPadMode, expertTokensNumType, expertTokensNumFlag, quantMode,
  *              rowIdxType, activeExpertRange array
+ *   ADD_RMS_NORM_QUANT: x, residual, gamma, smooth, q, scale, residualOut, normedOut; eps (float)
+ *   ROUTE_TOP_K: logits, bias, tokenMask, weights, ids; scoring, nGroup, topkGroup, groupScore, renormalize, scale (float)
+ *   ADAPTER_ADD: base, x, xScale, a, b, adapterIds, scaling, out
  * If the workspace is too small, or a pooled one and the stream is being captured, the first phase's executor comes back (stage
  * PLANNED): the caller allocates result->workspaceSize bytes and makes the operator's second-phase call, or destroys the executor.  Otherwise stage says
  * how far the call came when its status is not ACLNN_SUCCESS. */
 enum {
     GMM_B200_OP_GMM_V4 = 0, GMM_B200_OP_GMM_V5 = 1, GMM_B200_OP_GMM_WEIGHT_NZ = 2, GMM_B200_OP_SWIGLU_QUANT = 3,
     GMM_B200_OP_SWIGLU_QUANT_WEIGHT_NZ = 4, GMM_B200_OP_FINALIZE_ROUTING = 5, GMM_B200_OP_FINALIZE_ROUTING_V2 = 6,
-    GMM_B200_OP_MOE_INIT_ROUTING_V3 = 7,
-    GMM_B200_OP_POOLED = 0x100   /* added to the operator: `workspace` comes from a pool and is not used if `stream` is being captured */
+    GMM_B200_OP_MOE_INIT_ROUTING_V3 = 7, GMM_B200_OP_ADD_RMS_NORM_QUANT = 8, GMM_B200_OP_ROUTE_TOP_K = 9, GMM_B200_OP_ADAPTER_ADD = 10,
+    GMM_B200_OP_POOLED = 0x100,   /* added to the operator: `workspace` comes from a pool and is not used if `stream` is being captured */
+    GMM_B200_OP_PLAN_ONLY = 0x200 /* added to the operator: the first phase alone (stage PLANNED), whatever workspace is there */
 };
 enum { GMM_B200_STAGE_PLAN = 0, GMM_B200_STAGE_OPTIONS = 1, GMM_B200_STAGE_PLANNED = 2, GMM_B200_STAGE_RUN = 3 };
 typedef struct gmmB200CallResult {
@@ -119,6 +123,62 @@ ACL_FUNC_VISIBILITY aclnnStatus gmmB200GroupedMatmulW8A8(const void *x, const vo
                                                         void *const *outPeers, int32_t numPeers, int64_t outRows, void *y, int32_t yDtype,
                                                         void *workspace, uint64_t workspaceSize, aclrtStream stream,
                                                         const gmmB200LaunchOptions *options);
+
+/* Three operators that stand around the expert FFN in a mixture-of-experts block, in the two-phase form of the aclnn operators (checks
+ * and executor in the first call, which never touches the device; the second enqueues on `stream` and uses the executor up).  Absent
+ * optional tensors are null.  Views whose rows are dense are read and written where they are, others through copies in the
+ * workspace.  Lengths of zero are valid where stated and do nothing. */
+
+/* The norm in front of the experts, with the int8 rows and per-token scales that the W8A8 operators take:
+ *   h = x + residual (fp32);  r = 1 / sqrt(mean(h^2) + eps);  u = h * gamma * smooth;  step = max|u| / 127
+ *   q = rint(u / step) within [-127, 127] (0 where step is 0 or not finite);  scale = step * r
+ *   residualOut = h, normedOut = h * r * gamma, both rounded to x's type
+ * q * scale is the normed row (times smooth) in 8 bits: r belongs to the whole row and cancels in u / step.  A row that holds an
+ * infinity or a NaN gets a scale of NaN.
+ *   x, residual       [rows, h] fp32 / fp16 / bf16, h in [1, 65535], rows may be 0; residual optional
+ *   gamma             [h] x's type or fp32;   smooth  fp32 [h], optional
+ *   q                 int8 [rows, h];   scale  fp32 [rows]
+ *   residualOut       [rows, h] x's type, optional, needs residual; may be x or residual itself
+ *   normedOut         [rows, h] x's type, optional; may be x itself if residualOut is not
+ *   eps               positive and finite */
+ACL_FUNC_VISIBILITY aclnnStatus gmmB200AddRmsNormQuantGetWorkspaceSize(
+    const aclTensor *x, const aclTensor *residualOptional, const aclTensor *gamma, const aclTensor *smoothOptional, float eps,
+    aclTensor *q, aclTensor *scale, aclTensor *residualOutOptional, aclTensor *normedOutOptional, uint64_t *workspaceSize,
+    aclOpExecutor **executor);
+ACL_FUNC_VISIBILITY aclnnStatus gmmB200AddRmsNormQuant(void *workspace, uint64_t workspaceSize, aclOpExecutor *executor,
+                                                      aclrtStream stream);
+
+/* The choice of experts, in front of aclnnMoeInitRoutingV3 (ids, int32) or of the expert-parallel layer (int64):
+ *   score s = sigmoid(logit) or softmax(logits); choice c = s + bias.  Without bias, and unless groups are ranked by two sums, the
+ *   choice goes by the logits themselves, which order alike.  An expert whose logit or choice is NaN or minus infinity is not there.
+ *   nGroup > 1: only the topkGroup best groups of experts / nGroup consecutive experts stay; a group's rank is its largest choice or
+ *   the sum of its two largest (of those that are there).
+ *   ids = the top_k largest choices that stay, largest first, ties to the lowest id; weights = their scores, divided by their sum with
+ *   `renormalize`, times `scale`.  Slots for which no expert is left, and rows whose tokenMask is 0, get id -1 and weight 0 (a negative
+ *   id is no pair to the routing operators).
+ *   logits            fp32 / fp16 / bf16 [rows, experts], experts in [1, 1024], rows may be 0
+ *   bias              fp32 [experts], optional;   tokenMask  int8 or bool [rows], optional
+ *   scoring           0 softmax, 1 sigmoid;   groupScore  0 largest, 1 sum of the two largest
+ *   nGroup            divides experts, at most 32;   topkGroup  in [1, nGroup]
+ *   weights           fp32 [rows, top_k], top_k in [1, 32] and at most topkGroup * experts / nGroup;   ids  int32 or int64, same shape */
+ACL_FUNC_VISIBILITY aclnnStatus gmmB200RouteTopKGetWorkspaceSize(
+    const aclTensor *logits, const aclTensor *biasOptional, const aclTensor *tokenMaskOptional, int64_t scoring, int64_t nGroup,
+    int64_t topkGroup, int64_t groupScore, bool renormalize, float scale, aclTensor *weights, aclTensor *ids, uint64_t *workspaceSize,
+    aclOpExecutor **executor);
+ACL_FUNC_VISIBILITY aclnnStatus gmmB200RouteTopK(void *workspace, uint64_t workspaceSize, aclOpExecutor *executor, aclrtStream stream);
+
+/* Low-rank adapters of many requests on top of a projection that they share:
+ *   out[t] = base[t] + scaling[i] * (x[t] a[i]^T) b[i]^T with i = adapterIds[t]; out[t] = base[t] where i names no adapter
+ *   (negative, or at least `adapters`).  Sums are fp32, the result is rounded once.
+ *   base, out         [rows, n] fp16 / bf16; out may be base itself;   rows may be 0
+ *   x                 [rows, k] base's type, or int8 with xScale (fp32 [rows]): the rows of the W8A8 operators
+ *   a                 [adapters, rank, k], b [adapters, n, rank], both base's type; rank in [1, 128]; k, n in [1, 65535]
+ *   adapterIds        int32 [rows];   scaling  fp32 [adapters], optional (1 without it)
+ * Tokens may come in any order; those of one adapter share its weights. */
+ACL_FUNC_VISIBILITY aclnnStatus gmmB200AdapterAddGetWorkspaceSize(
+    const aclTensor *base, const aclTensor *x, const aclTensor *xScaleOptional, const aclTensor *a, const aclTensor *b,
+    const aclTensor *adapterIds, const aclTensor *scalingOptional, aclTensor *out, uint64_t *workspaceSize, aclOpExecutor **executor);
+ACL_FUNC_VISIBILITY aclnnStatus gmmB200AdapterAdd(void *workspace, uint64_t workspaceSize, aclOpExecutor *executor, aclrtStream stream);
 
 /* Buffers that other GPUs of the node can write into (CUDA IPC).  PeerAlloc/PeerFree own device memory of the calling
  * process; PeerExport fills a 64-byte handle that another process passes to PeerImport to obtain a device pointer to the

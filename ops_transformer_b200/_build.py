@@ -16,8 +16,9 @@ LIB_PATH = os.path.join(PKG_DIR, "libgmm_b200.so")
 DESCRIBE_PATH = os.path.join(PKG_DIR, "_describe.so")
 DESCRIBE_SOURCE = os.path.join(CSRC, "describe.cpp")
 
-SOURCES = ["gmm_sm100.cu", "gmm_simt.cu", "gmm_noalloc.cu", "ep_peer.cu", "moe_init_routing.cu", "view_copy.cu", "acl_shim.cpp", "op_api.cpp"]
-HEADERS = ["gmm_common.h", "acl_shim.h"]
+SOURCES = ["gmm_sm100.cu", "gmm_simt.cu", "gmm_noalloc.cu", "ep_peer.cu", "moe_init_routing.cu", "norm_quant.cu", "route_top_k.cu",
+           "adapter_add.cu", "view_copy.cu", "acl_shim.cpp", "op_api.cpp", "block_ops.cpp"]
+HEADERS = ["gmm_common.h", "acl_shim.h", "op_api.h"]
 
 # -fmad=false: the epilogues reproduce the reference's separately rounded fp32 steps, so the compiler must not
 # fuse a multiply and an add.  No fast-math.

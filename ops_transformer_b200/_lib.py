@@ -37,6 +37,8 @@ EXPORTED_SYMBOLS = [
     "gmmB200GroupedMatmulSwigluQuantWorkspaceSize", "gmmB200GroupedMatmulSwigluQuant",
     "gmmB200NoAllocScratchBytes", "gmmB200GroupedMatmulSwigluQuantNoAlloc", "gmmB200NoAllocCheckStatus",
     "gmmB200PeerAlloc", "gmmB200PeerFree", "gmmB200PeerExport", "gmmB200PeerImport", "gmmB200PeerRelease", "gmmB200EpDispatch", "gmmB200EpCount", "gmmB200EpRoute", "gmmB200EpInverseMap", "gmmB200EpCombine",
+    "gmmB200AddRmsNormQuantGetWorkspaceSize", "gmmB200AddRmsNormQuant", "gmmB200RouteTopKGetWorkspaceSize", "gmmB200RouteTopK",
+    "gmmB200AdapterAddGetWorkspaceSize", "gmmB200AdapterAdd",
 ]
 
 
@@ -55,7 +57,8 @@ class CallResult(C.Structure):
 
 
 OP_GMM, OP_SWIGLU_QUANT, OP_FINALIZE_ROUTING, OP_MOE_INIT_ROUTING = {"V4": 0, "V5": 1, "WeightNz": 2}, {"": 3, "WeightNZ": 4}, {"": 5, "V2": 6}, 7
-OP_POOLED = 0x100
+OP_ADD_RMS_NORM_QUANT, OP_ROUTE_TOP_K, OP_ADAPTER_ADD = 8, 9, 10
+OP_POOLED, OP_PLAN_ONLY = 0x100, 0x200
 STAGE_PLAN, STAGE_OPTIONS, STAGE_PLANNED, STAGE_RUN = range(4)
 
 
@@ -119,6 +122,12 @@ def _load():
     L.gmmB200EpRoute.argtypes = [p, p, p, i64, i32, i32, i32, i32, i64, i64, i64, p, p, p, p, p, p, p]
     L.gmmB200EpInverseMap.argtypes = [p, p, i64, i64, i64, p, p, p]
     L.gmmB200EpCombine.argtypes = [p, p, p, p, i64, i32, i64, i64, p]
+    L.gmmB200AddRmsNormQuantGetWorkspaceSize.argtypes = [p] * 4 + [f32] + [p] * 4 + [C.POINTER(u64), C.POINTER(p)]
+    L.gmmB200AddRmsNormQuant.argtypes = [p, u64, p, p]
+    L.gmmB200RouteTopKGetWorkspaceSize.argtypes = [p] * 3 + [i64] * 4 + [b8, f32, p, p, C.POINTER(u64), C.POINTER(p)]
+    L.gmmB200RouteTopK.argtypes = [p, u64, p, p]
+    L.gmmB200AdapterAddGetWorkspaceSize.argtypes = [p] * 8 + [C.POINTER(u64), C.POINTER(p)]
+    L.gmmB200AdapterAdd.argtypes = [p, u64, p, p]
     L.gmmB200NoAllocScratchBytes.restype = u64
     L.gmmB200GroupedMatmulSwigluQuantNoAlloc.argtypes = [p, p, p, i32, p, p, i64, i64, i64, i64, i64, p, p, p]
     L.gmmB200NoAllocCheckStatus.argtypes = [p, C.POINTER(i32)]

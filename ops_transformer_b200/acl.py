@@ -11,6 +11,7 @@ from __future__ import annotations
 import array
 import contextlib
 import ctypes as C
+import functools
 import struct
 import threading
 from typing import Optional, Sequence
@@ -423,3 +424,92 @@ def moe_init_routing_v3(x: torch.Tensor, expert_idx: torch.Tensor, *, expert_num
                                row_idx_type, _ints(active_expert_range))
     _call(_lib.OP_MOE_INIT_ROUTING, "aclnnMoeInitRoutingV3", words, x.device, workspace, stream, None)
     return ex, ri, cnt, es
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# Operators around the expert FFN (include/gmm_b200.h)
+# ---------------------------------------------------------------------------------------------------------------------
+
+@functools.lru_cache(maxsize=64)
+def _float_bits(v: float) -> int:
+    return struct.unpack("<I", struct.pack("<f", v))[0]
+
+
+def _block_call(op: int, name: str, words: bytes, tensors, workspace: Optional[torch.Tensor], stream,
+                options: Optional[LaunchOptions] = None) -> Optional[torch.Tensor]:
+    """``_call`` for operators whose tensors all have to be on the first one's GPU.  Elsewhere the arguments are checked and the call is
+    refused: these operators may need no workspace, whose place would tell."""
+    device = tensors[0].device
+    if device.type != "cuda" or any(t is not None and t.device != device for t in tensors):
+        res = _lib.CallResult()
+        rc = _lib.lib().gmmB200Call(op | _lib.OP_PLAN_ONLY, words, len(words) // 8, None, 0, None, None, C.byref(res))
+        if rc != ACLNN_SUCCESS:
+            raise AclnnError(rc, name + "GetWorkspaceSize")
+        _lib.lib().aclDestroyAclOpExecutor(C.c_void_p(res.executor))
+        raise ValueError(f"{name}: all tensors must be on one CUDA device")
+    return _call(op, name, words, device, workspace, stream, options)
+
+
+def add_rms_norm_quant(x: torch.Tensor, gamma: torch.Tensor, *, residual: Optional[torch.Tensor] = None,
+                       smooth: Optional[torch.Tensor] = None, eps: float = 1e-6, normed: bool = False,
+                       q: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None,
+                       residual_out: Optional[torch.Tensor] = None, normed_out: Optional[torch.Tensor] = None, stream=None,
+                       workspace: Optional[torch.Tensor] = None):
+    """(q int8 [rows, h], scale fp32 [rows], residual_out, normed_out): the norm of ``h = x + residual`` in 8 bits with per-token scales,
+    as the W8A8 operators take their rows, ``h`` itself (None without a residual) and, with ``normed`` or a ``normed_out`` to write to,
+    the normed rows in x's type.  ``smooth`` (fp32 [h]) multiplies what is quantised, not ``normed_out``.  ``residual_out`` may be
+    ``residual`` or ``x``.  gmmB200AddRmsNormQuant (include/gmm_b200.h) has the formulas."""
+    if q is None:
+        q = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
+    if scale is None:
+        scale = x.new_empty(x.shape[:1], dtype=torch.float32)
+    if residual_out is None and residual is not None:
+        residual_out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    if normed_out is None and normed:
+        normed_out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    words = _lib.describe_call("tttttttti", x, residual, gamma, smooth, q, scale, residual_out, normed_out, _float_bits(eps))
+    _block_call(_lib.OP_ADD_RMS_NORM_QUANT, "gmmB200AddRmsNormQuant", words, (x, residual, gamma, smooth, q, scale, residual_out, normed_out),
+                workspace, stream)
+    return q, scale, residual_out, normed_out
+
+
+_SCORING = {"softmax": 0, "sigmoid": 1}
+_GROUP_SCORE = {"max": 0, "top2": 1}
+
+
+def route_top_k(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", bias: Optional[torch.Tensor] = None, n_group: int = 1,
+                topk_group: int = 1, group_score: str = "max", renormalize: bool = True, scale: float = 1.0,
+                token_mask: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None, ids: Optional[torch.Tensor] = None,
+                ids_dtype: torch.dtype = torch.int32, stream=None, workspace: Optional[torch.Tensor] = None):
+    """(weights fp32 [rows, top_k], ids [rows, top_k]): the experts of every row, largest choice first, ties to the lowest id.
+    ``scoring`` "softmax" or "sigmoid"; ``bias`` (fp32 [experts]) is added for the choice and is no part of the weights; with ``n_group``
+    only the ``topk_group`` best groups stay, ranked by their largest choice ("max") or the sum of the two largest ("top2").
+    ``token_mask`` (bool or int8 [rows]): rows without a token.  Slots without an expert have id -1 and weight 0.  ``ids_dtype`` int32 is
+    what ``moe_init_routing_v3`` takes, int64 the expert-parallel layer.  gmmB200RouteTopK (include/gmm_b200.h) has the rules."""
+    if scoring not in _SCORING or group_score not in _GROUP_SCORE:
+        raise ValueError(f"unknown scoring {scoring!r} or group_score {group_score!r}")
+    shape = (logits.shape[0], top_k)
+    if weights is None:
+        weights = logits.new_empty(shape, dtype=torch.float32)
+    if ids is None:
+        ids = logits.new_empty(shape, dtype=ids_dtype)
+    if token_mask is not None and token_mask.dtype == torch.bool:
+        token_mask = token_mask.view(torch.int8)
+    words = _lib.describe_call("tttttiiiiii", logits, bias, token_mask, weights, ids, _SCORING[scoring], n_group, topk_group,
+                               _GROUP_SCORE[group_score], 1 if renormalize else 0, _float_bits(scale))
+    _block_call(_lib.OP_ROUTE_TOP_K, "gmmB200RouteTopK", words, (logits, bias, token_mask, weights, ids), workspace, stream)
+    return weights, ids
+
+
+def adapter_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter_ids: torch.Tensor, *,
+                x_scale: Optional[torch.Tensor] = None, scaling: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                stream=None, workspace: Optional[torch.Tensor] = None):
+    """out [rows, n] = base + scaling[i] * (x a[i]^T) b[i]^T with the adapter i = adapter_ids[row] of every row (int32, negative: none):
+    low-rank adapters of many requests beside one shared projection, whose result is ``base``.  ``x`` has base's type or is int8 with
+    ``x_scale`` (fp32 [rows]); a [adapters, rank, k], b [adapters, n, rank].  ``out`` may be ``base``.  gmmB200AdapterAdd
+    (include/gmm_b200.h)."""
+    if out is None:
+        out = torch.empty_like(base, memory_format=torch.contiguous_format)
+    words = _lib.describe_call("tttttttt", base, x, x_scale, a, b, adapter_ids, scaling, out)
+    _block_call(_lib.OP_ADAPTER_ADD, "gmmB200AdapterAdd", words, (base, x, x_scale, a, b, adapter_ids, scaling, out), workspace, stream)
+    return out

@@ -46,13 +46,16 @@ struct aclIntArray {
 };
 
 struct aclOpExecutor {
-    enum Kind { kNoop = 0, kGmm = 1, kInitRouting = 2 } kind = kNoop;
+    enum Kind { kNoop = 0, kGmm = 1, kInitRouting = 2, kNormQuant = 3, kRouteTopK = 4, kAdapterAdd = 5 } kind = kNoop;
     uint32_t magic = 0xac10e8ecu;
     bool consumed = false;
     const char *op_name = "";
     gmm::Problem problem;
     gmm::Plan plan;
     gmm::InitRoutingProblem routing;
+    gmm::NormQuantProblem norm;
+    gmm::RouteTopKProblem route;
+    gmm::AdapterProblem adapter;
     std::vector<gmm::StagedView> staged;   // non-contiguous views with a contiguous copy in the workspace tail
     size_t staged_bytes = 0;
 };

@@ -109,6 +109,60 @@ struct InitRoutingProblem {
 size_t init_routing_workspace_bytes(const InitRoutingProblem &r);
 cudaError_t init_routing_launch(const InitRoutingProblem &r, void *workspace, size_t workspace_bytes, cudaStream_t stream);
 
+// add_rms_norm_quant (norm_quant.cu).  Row strides are in elements; a missing tensor is null.
+struct NormQuantProblem {
+    const void *x = nullptr, *residual = nullptr;   // [rows, h]
+    const void *gamma = nullptr;                    // [h], dtype or fp32
+    const float *smooth = nullptr;                  // [h]
+    int8_t *q = nullptr;                            // [rows, h]
+    float *scale = nullptr;                         // [rows]
+    void *residual_out = nullptr, *normed_out = nullptr;
+    int64_t rows = 0, h = 0;
+    int64_t ld_x = 0, ld_residual = 0, ld_q = 0, ld_residual_out = 0, ld_normed = 0;
+    int dtype = kBF16, gamma_dtype = kBF16;
+    float eps = 0.0f;
+};
+cudaError_t norm_quant_launch(const NormQuantProblem &p, cudaStream_t stream);
+
+// route_top_k (route_top_k.cu).
+enum : int { kScoreSoftmax = 0, kScoreSigmoid = 1 };
+enum : int { kGroupMax = 0, kGroupTop2 = 1 };
+struct RouteTopKProblem {
+    const void *logits = nullptr;       // [rows, experts] f32 / f16 / bf16
+    int dtype = kF32;
+    int64_t ld = 0;                     // its row stride in elements
+    const float *bias = nullptr;        // [experts], optional
+    const int8_t *token_mask = nullptr; // [rows], optional: 0 = a row without a token
+    int64_t rows = 0;
+    int experts = 0, top_k = 0;
+    int scoring = kScoreSoftmax, group_score = kGroupMax;
+    int n_group = 1, topk_group = 1;
+    bool renormalize = false;
+    float scale = 1.0f;
+    float *weights = nullptr;           // [rows, top_k]
+    void *ids = nullptr;                // [rows, top_k] int32 or int64
+    bool ids_i64 = false;
+};
+cudaError_t route_top_k_launch(const RouteTopKProblem &p, cudaStream_t stream);
+
+// adapter_add (adapter_add.cu).
+struct AdapterProblem {
+    const void *base = nullptr;         // [rows, n] f16 / bf16
+    const void *x = nullptr;            // [rows, k] dtype, or int8 with x_scale
+    const float *x_scale = nullptr;     // [rows]
+    const void *a = nullptr;            // [adapters, rank, k] dtype
+    const void *b = nullptr;            // [adapters, n, rank] dtype
+    const int *ids = nullptr;           // [rows]; outside [0, adapters): none
+    const float *scaling = nullptr;     // [adapters], optional
+    void *out = nullptr;                // [rows, n], may be base
+    int64_t rows = 0, k = 0, n = 0, adapters = 0, rank = 0;
+    int64_t ld_base = 0, ld_x = 0, ld_out = 0;
+    int dtype = kBF16;
+    bool x_i8 = false;
+};
+size_t adapter_workspace_bytes(const AdapterProblem &p);
+cudaError_t adapter_launch(const AdapterProblem &p, void *workspace, size_t workspace_bytes, cudaStream_t stream);
+
 // A non-contiguous tensor view whose contiguous copy lives in the workspace (view_copy.cu).
 struct StagedView {
     std::vector<int64_t> dims, strides;  // strides in elements

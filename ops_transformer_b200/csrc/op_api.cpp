@@ -10,13 +10,11 @@
 //       CheckNotNull :75-105, CheckInputOutDims_A8W8 :108-125, CheckInputOutShape_A8W8 :149-213, CheckDtypeValid :304-324
 // restricted to the int8 x int8 path.  The first phase is host only and never reads group_list; the second
 // phase enqueues on the caller's CUDA stream and returns.
-#include <nvtx3/nvToolsExt.h>
-
 #include <cstdlib>
 #include <cstring>
 #include <type_traits>
 
-#include "acl_shim.h"
+#include "op_api.h"
 #include "aclnnop/aclnn_grouped_matmul_finalize_routing_weight_nz.h"
 #include "aclnnop/aclnn_grouped_matmul_swiglu_quant.h"
 #include "aclnnop/aclnn_grouped_matmul_swiglu_quant_weight_nz.h"
@@ -27,23 +25,12 @@
 #include "gmm_b200.h"
 
 namespace gmm {
-void register_executor(aclOpExecutor *e);
-bool claim_executor(aclOpExecutor *e);
-bool executor_is_live(aclOpExecutor *e);
-
 namespace {
 
 constexpr int64_t kMaxGroupListLen = 1024;   // MAX_GROUP_LIST_SIZE_TENSOR, aclnn_grouped_matmul.cpp:52
 constexpr int64_t kMaxInnerAxis = 65535;     // aclnn_grouped_matmul.cpp:53
 constexpr int64_t kSwigluNLimit = 10240;     // N_LIMIT, aclnn_grouped_matmul_swiglu_quant.cpp:39
 constexpr int64_t kSwigluKLimit = 65536;     // K_LIMIT_A8W8, :37
-
-#define GMM_REQUIRE(cond, code, ...)                   \
-    do {                                               \
-        if (!(cond)) return fail((code), __VA_ARGS__); \
-    } while (0)
-
-bool is_private_format(aclFormat f) { return f == ACL_FORMAT_FRACTAL_NZ || f == ACL_FORMAT_FRACTAL_Z || f == ACL_FORMAT_NC1HWC0; }
 
 // Same test as IsTransposeLastTwoDims (gmm/grouped_matmul/op_host/op_api/aclnn_grouped_matmul_util.cpp:16-33).
 bool is_transposed_last_two(const aclTensor *t)
@@ -61,60 +48,6 @@ bool is_transposed_last_two(const aclTensor *t)
     }
     return false;
 }
-
-aclOpExecutor *new_executor(const char *name)
-{
-    aclOpExecutor *e = new (std::nothrow) aclOpExecutor();
-    if (e) e->op_name = name;
-    return e;
-}
-
-// Address the operator will use for tensor `t`: the tensor's own memory when it is contiguous; otherwise a contiguous
-// copy in the workspace tail, filled before the launch (and, for an output, copied back afterwards).  The address of a
-// copy is only known in the second phase: until then `*field` holds an aligned stand-in.
-template <typename P>
-void bind_tensor(aclOpExecutor *e, const aclTensor *t, P *field, bool is_output, bool contiguous_enough = false)
-{
-    if (!t) { *field = nullptr; return; }
-    if (t->contiguous() || contiguous_enough) { *field = (P)tensor_ptr(t); return; }
-    StagedView v;
-    v.dims = t->view_dims;
-    v.strides = t->strides;
-    v.elem = (int)dtype_size(t->dtype);
-    v.data = tensor_ptr(t);
-    v.ws_off = e->staged_bytes;
-    v.is_output = is_output;
-    v.field = (void **)field;  // the field is a pointer of some type; only its value is replaced
-    e->staged_bytes += ((size_t)t->numel() * v.elem + 255) / 256 * 256;
-    e->staged.push_back(v);
-    *field = (P)(uintptr_t)4096;
-}
-
-// Env-gated profiler ranges around both phases of every entry point (GMM_B200_NVTX=1), the counterpart of the
-// reference's L2_DFX_PHASE_1 / L2_DFX_PHASE_2 (gmm/grouped_matmul/op_host/op_api/aclnn_grouped_matmul.cpp:2005, 2151).
-// NVTX is header only and does nothing unless a tool is attached.
-bool nvtx_enabled()
-{
-    static const bool on = [] {
-        const char *e = std::getenv("GMM_B200_NVTX");
-        return e && e[0] && e[0] != '0';
-    }();
-    return on;
-}
-struct PhaseRange {
-    bool on;
-    PhaseRange(const char *op, int phase) : on(nvtx_enabled())
-    {
-        if (!on) return;
-        char name[160];
-        std::snprintf(name, sizeof(name), "%s phase %d", op, phase);
-        nvtxRangePushA(name);
-    }
-    ~PhaseRange()
-    {
-        if (on) nvtxRangePop();
-    }
-};
 
 // Public options -> internal form.  Fields beyond the caller's structSize read as zero.
 aclnnStatus convert_options(const gmmB200LaunchOptions *o, LaunchOptions *out)
@@ -135,15 +68,6 @@ aclnnStatus convert_options(const gmmB200LaunchOptions *o, LaunchOptions *out)
     out->ev_stop = static_cast<cudaEvent_t>(full.stopEvent);
     out->wait_limit_cycles = full.waitLimitCycles;
     out->test_skip_k_blocks = full.testSkipKBlocks;
-    return ACLNN_SUCCESS;
-}
-
-aclnnStatus finish_phase1(aclOpExecutor *e, uint64_t *workspaceSize, aclOpExecutor **executor)
-{
-    // kInitRouting stores its size in plan.ws_bytes too
-    *workspaceSize = e->kind == aclOpExecutor::kNoop ? 0 : e->plan.ws_bytes + e->staged_bytes;
-    register_executor(e);
-    *executor = e;
     return ACLNN_SUCCESS;
 }
 
@@ -177,10 +101,13 @@ aclnnStatus run_executor(const char *op_name, void *workspace, uint64_t workspac
             }
             if (executor->kind == aclOpExecutor::kGmm && executor->plan.path == kPathSm100 && !sm100_shape_ok(executor->problem))
                 executor->plan.path = kPathSimt;      // a workspace that is not 16-byte aligned cannot feed TMA
-            if (ce == cudaSuccess)
-                ce = executor->kind == aclOpExecutor::kInitRouting
-                         ? init_routing_launch(executor->routing, workspace, executor->plan.ws_bytes, cs)
-                         : launch(executor->problem, executor->plan, workspace, executor->plan.ws_bytes, cs);
+            if (ce == cudaSuccess) switch (executor->kind) {
+                case aclOpExecutor::kInitRouting: ce = init_routing_launch(executor->routing, workspace, executor->plan.ws_bytes, cs); break;
+                case aclOpExecutor::kNormQuant: ce = norm_quant_launch(executor->norm, cs); break;
+                case aclOpExecutor::kRouteTopK: ce = route_top_k_launch(executor->route, cs); break;
+                case aclOpExecutor::kAdapterAdd: ce = adapter_launch(executor->adapter, workspace, executor->plan.ws_bytes, cs); break;
+                default: ce = launch(executor->problem, executor->plan, workspace, executor->plan.ws_bytes, cs);
+            }
             for (StagedView &v : executor->staged)
                 if (v.is_output && ce == cudaSuccess) ce = view_copy_launch(v, tail + v.ws_off, false, cs);
             if (ce != cudaSuccess)
@@ -1259,6 +1186,34 @@ aclnnStatus plan_packed(int32_t op, WordReader &r, uint64_t *size, aclOpExecutor
                                                          num_type, num_flag, quant, range.get(), row_type, ex_out.get(), row_idx.get(),
                                                          counts.get(), ex_scale.get(), size, ex);
         }
+        case GMM_B200_OP_ADD_RMS_NORM_QUANT: {
+            PackedTensor x, residual, gamma, smooth, q, scale, residual_out, normed;
+            for (PackedTensor *t : {&x, &residual, &gamma, &smooth, &q, &scale, &residual_out, &normed}) t->read(r);
+            const float eps = float_of_bits(r.next());
+            if (!r.all_read()) return malformed();
+            *run = gmmB200AddRmsNormQuant;
+            return gmmB200AddRmsNormQuantGetWorkspaceSize(x.get(), residual.get(), gamma.get(), smooth.get(), eps, q.out(), scale.out(),
+                                                          residual_out.out(), normed.out(), size, ex);
+        }
+        case GMM_B200_OP_ROUTE_TOP_K: {
+            PackedTensor logits, bias, mask, weights, ids;
+            for (PackedTensor *t : {&logits, &bias, &mask, &weights, &ids}) t->read(r);
+            const int64_t scoring = r.next(), n_group = r.next(), topk_group = r.next(), group_score = r.next();
+            const bool renormalize = r.next() != 0;
+            const float scale = float_of_bits(r.next());
+            if (!r.all_read()) return malformed();
+            *run = gmmB200RouteTopK;
+            return gmmB200RouteTopKGetWorkspaceSize(logits.get(), bias.get(), mask.get(), scoring, n_group, topk_group, group_score,
+                                                    renormalize, scale, weights.out(), ids.out(), size, ex);
+        }
+        case GMM_B200_OP_ADAPTER_ADD: {
+            PackedTensor base, x, x_scale, a, b, ids, scaling, out;
+            for (PackedTensor *t : {&base, &x, &x_scale, &a, &b, &ids, &scaling, &out}) t->read(r);
+            if (!r.all_read()) return malformed();
+            *run = gmmB200AdapterAdd;
+            return gmmB200AdapterAddGetWorkspaceSize(base.get(), x.get(), x_scale.get(), a.get(), b.get(), ids.get(), scaling.get(), out.out(),
+                                                     size, ex);
+        }
         default: return fail(ACLNN_ERR_PARAM_INVALID, "gmmB200Call: unknown operator %d.", op);
     }
 }
@@ -1277,7 +1232,7 @@ aclnnStatus gmmB200Call(int32_t op, const int64_t *words, uint64_t count, void *
     uint64_t need = 0;
     aclOpExecutor *ex = nullptr;
     RunFn run = nullptr;
-    aclnnStatus rc = plan_packed(op & ~GMM_B200_OP_POOLED, r, &need, &ex, &run);
+    aclnnStatus rc = plan_packed(op & ~(GMM_B200_OP_POOLED | GMM_B200_OP_PLAN_ONLY), r, &need, &ex, &run);
     if (rc != ACLNN_SUCCESS) return rc;
     result->workspaceSize = need;
     if (options) {
@@ -1288,7 +1243,7 @@ aclnnStatus gmmB200Call(int32_t op, const int64_t *words, uint64_t count, void *
             return rc;
         }
     }
-    if (need > workspaceBytes || (need && (op & GMM_B200_OP_POOLED) && gmmB200StreamIsCapturing(stream))) {  // the caller finds more and runs the second phase itself
+    if ((op & GMM_B200_OP_PLAN_ONLY) || need > workspaceBytes || (need && (op & GMM_B200_OP_POOLED) && gmmB200StreamIsCapturing(stream))) {  // the caller finds more and runs the second phase itself
         result->stage = GMM_B200_STAGE_PLANNED;
         result->executor = ex;
         return ACLNN_SUCCESS;
