@@ -172,7 +172,8 @@ ACL_FUNC_VISIBILITY aclnnStatus gmmB200RouteTopK(void *workspace, uint64_t works
  *   (negative, or at least `adapters`).  Sums are fp32, the result is rounded once.
  *   base, out         [rows, n] fp16 / bf16; out may be base itself;   rows may be 0
  *   x                 [rows, k] base's type, or int8 with xScale (fp32 [rows]): the rows of the W8A8 operators
- *   a                 [adapters, rank, k], b [adapters, n, rank], both base's type; rank in [1, 128]; k, n in [1, 65535]
+ *   a                 [adapters, rank, k], b [adapters, n, rank], both base's type; adapters in [1, 16384], rank in [1, 128], k and n in
+ *                     [1, 65535]
  *   adapterIds        int32 [rows];   scaling  fp32 [adapters], optional (1 without it)
  * Tokens may come in any order; those of one adapter share its weights. */
 ACL_FUNC_VISIBILITY aclnnStatus gmmB200AdapterAddGetWorkspaceSize(

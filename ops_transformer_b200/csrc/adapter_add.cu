@@ -2,98 +2,789 @@
 //
 //   out[t] = base[t] + scaling[i] * (x[t] a[i]^T) b[i]^T,  i = ids[t]
 //
-// Two kernels: v[t] = scaling * x[t] a[i]^T in fp32 (workspace), then out[t] = base[t] + v[t] b[i]^T, rounded once.
+// The tokens of one adapter are gathered into tiles, and two kernels run over them:
+//   shrink - v[t] = scaling * x[t] a[i]^T in fp32, K split over CTAs, one partial sum each (workspace)
+//   expand - out[t] = base[t] + v[t] b[i]^T: the partial sums are added in a fixed order, the result is rounded once
+// Both products run on the tensor cores (tcgen05, fp32 accumulators in tensor memory) although few operations come with every byte:
+// they then cost no issue slots beside the loads.  The tokens are rows of the first product and columns of the second, so that tiles of
+// 16 tokens (few tokens) and of 64 share the code and the channels of a result row lie in neighbouring lanes.
+// v enters the second product as two 16-bit parts, v = hi + lo: one alone would add an error of 2^-9 (bf16) of v, as large as the
+// rounding of the result.  fp16 has no range to spare, so there every token's v is scaled by a power of two to below 2.
+// The operands are fetched with 16-byte asynchronous copies (8, 4 or 2 bytes where rows start on no such boundary), straight into the
+// 128-byte-swizzled layout that the tensor cores read; a row's tail is zero filled.
+//
+// Which tokens share an adapter is found on the device.  Up to kSelfPlan tokens every CTA ranks the tokens among those of their
+// adapter itself, beside its first loads; beyond, a one-CTA kernel counts and sorts them.  The order within an adapter does not matter:
+// every row's arithmetic is its own.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "gmm_common.h"
 
 namespace gmm {
 namespace {
 
+constexpr int kBlockK = 64;          // elements of a row per K block: 128 bytes, one swizzled row
+constexpr int kChunkN = 128;         // channels per step of the second product
+constexpr int kSelfPlan = 256;       // most tokens for which every CTA finds its tile itself
+constexpr int kPlanThreads = 1024;
+constexpr int kShrinkThreads = 128, kExpandThreads = 256;
+constexpr int kShrinkStages = 4, kExpandStages = 2;
+constexpr long long kWaitLimitCycles = 1ll << 31;   // about a second
+
 struct AdapterParams {
     const void *base, *x, *a, *b;
     const float *x_scale, *scaling;
     const int *ids;
     void *out;
-    float *v;                       // [rows, rank]
     long long ld_base, ld_x, ld_out;
     int rows, k, n, adapters, rank;
+    int rank_pad;                   // rank, rounded up to the tensor cores' K step of 16
+    int grain_x, grain_a, grain_b, grain_base;   // bytes of a copy
+    int ksplit, nsplit;
+    int *status;                    // [4]
+    int *n_tiles;
+    int4 *tiles;                    // adapter (-1: none), first entry in `order`, tokens
+    int *order;                     // [rows] tokens grouped by adapter
+    float *v;                       // [ksplit, rows, rank_pad]
 };
 
-__device__ __forceinline__ float to_float(int8_t v) { return (float)v; }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void pdl_release() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count)
+{
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// Bounded wait for the tensor cores.  When it runs out the status says so and later waits of the CTA return at once.
+__device__ __noinline__ void mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int *gave_up, int *status, int role)
+{
+    const long long t0 = clock64();
+    while (!mbar_try(bar, parity)) {
+        if (*gave_up) return;
+        if (clock64() - t0 > kWaitLimitCycles) {
+            *gave_up = 1;
+            if (atomicCAS(status, kStatusOk, kStatusWaitTimeout) == kStatusOk) {
+                status[1] = (int)(blockIdx.y * gridDim.x + blockIdx.x);
+                status[2] = role;
+                status[3] = (int)parity;
+            }
+            return;
+        }
+    }
+}
+__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatile int *gave_up, int *status, int role)
+{
+    if (!mbar_try(bar, parity)) mbar_wait_slow(bar, parity, gave_up, status, role);
+}
+
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tmem_alloc(uint32_t *dst, uint32_t cols)
+{
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t cols)
+{
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint32_t bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// K-major operand in rows of 128 bytes with the 128-byte swizzle, 8 rows (1024 bytes) a group.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t saddr)
+{
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | (uint64_t)2 << 61;
+}
+// fp32 accumulators, both operands K-major and of type T, M = 128.
+template <typename T>
+__device__ __forceinline__ uint32_t instr_desc(int n)
+{
+    constexpr uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    return 1u << 4 | type << 7 | type << 10 | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
+}
+
+template <int BYTES>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void *src, int valid)
+{
+    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(valid), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// One copy of GRAIN bytes, of which `valid` are read and the rest is zero.
+template <int GRAIN>
+__device__ __forceinline__ void copy_grain(uint32_t dst, const char *src, int valid)
+{
+    if (GRAIN >= 4) {
+        cp_async<GRAIN>(dst, src, valid);
+    } else if (GRAIN == 2) {
+        const uint16_t v = valid > 0 ? *reinterpret_cast<const uint16_t *>(src) : (uint16_t)0;
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst), "h"(v) : "memory");
+    } else {
+        const uint16_t v = valid > 0 ? *reinterpret_cast<const uint8_t *>(src) : (uint16_t)0;
+        asm volatile("st.shared.u8 [%0], %1;" ::"r"(dst), "h"(v) : "memory");
+    }
+}
+
+// Offset of byte `b` of row `r` in a tile of 128-byte rows with the 128-byte swizzle.
+__device__ __forceinline__ uint32_t swizzled(int r, int b) { return (uint32_t)(r * 128 + ((((b >> 4) ^ r) & 7) << 4) + (b & 15)); }
+
+// Rows of `width` bytes (a power of two up to 256) into shared memory, `valid` bytes of each read; row r comes from src(r).
+// SWIZZLE: into 128-byte swizzled rows (width <= 128), else rows `width` bytes apart.
+template <int GRAIN, bool SWIZZLE, int THREADS, typename Src>
+__device__ __forceinline__ void copy_rows_grain(uint32_t dst, int rows, int width, int valid, Src src)
+{
+    const int shift = 31 - __clz(width / GRAIN);
+    for (int i = threadIdx.x; i < rows << shift; i += THREADS) {
+        const int r = i >> shift, b = (i & ((1 << shift) - 1)) * GRAIN;
+        const int have = min(max(valid - b, 0), GRAIN);
+        const char *row = src(r);
+        copy_grain<GRAIN>(dst + (SWIZZLE ? swizzled(r, b) : (uint32_t)(r * width + b)), have > 0 ? row + b : row, have);
+    }
+}
+template <bool SWIZZLE, int THREADS, typename Src>
+__device__ __forceinline__ void copy_rows(int grain, uint32_t dst, int rows, int width, int valid, Src src)
+{
+    if (grain == 16) copy_rows_grain<16, SWIZZLE, THREADS>(dst, rows, width, valid, src);
+    else if (grain == 8) copy_rows_grain<8, SWIZZLE, THREADS>(dst, rows, width, valid, src);
+    else if (grain == 4) copy_rows_grain<4, SWIZZLE, THREADS>(dst, rows, width, valid, src);
+    else if (grain == 2) copy_rows_grain<2, SWIZZLE, THREADS>(dst, rows, width, valid, src);
+    else copy_rows_grain<1, SWIZZLE, THREADS>(dst, rows, width, valid, src);
+}
+
 template <typename T> __device__ __forceinline__ T from_float(float v);
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-// One warp per (row, rank component).
-template <typename T, typename X>
-__global__ void __launch_bounds__(128) adapter_shrink_kernel(const AdapterParams p)
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b)
 {
-    const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (at >= (long long)p.rows * p.rank) return;
-    const int row = (int)(at / p.rank), j = (int)(at % p.rank);
-    const int i = p.ids[row];
-    if (i < 0 || i >= p.adapters) return;
-    const X *x = reinterpret_cast<const X *>(p.x) + row * p.ld_x;
-    const T *a = reinterpret_cast<const T *>(p.a) + ((long long)i * p.rank + j) * p.k;
-    float sum = 0.0f;
-    for (int c = lane; c < p.k; c += 32) sum = __fmaf_rn(to_float(x[c]), to_float(a[c]), sum);
+    const T lo = from_float<T>(a), hi = from_float<T>(b);
+    return (uint32_t)*reinterpret_cast<const uint16_t *>(&lo) | (uint32_t)*reinterpret_cast<const uint16_t *>(&hi) << 16;
+}
+
+// The int8 elements that this thread copied to `raw` (rows of 64), as T in the swizzled tile: exact in both types.
+template <typename T, int GRAIN, int THREADS>
+__device__ __forceinline__ void widen_rows_grain(uint32_t raw, uint32_t dst, int rows)
+{
+    constexpr int PER_ROW = 64 / GRAIN;
+    for (int i = threadIdx.x; i < rows * PER_ROW; i += THREADS) {
+        const int r = i / PER_ROW, c = (i % PER_ROW) * GRAIN;
+        if (GRAIN == 1) {
+            uint16_t q;
+            asm volatile("ld.shared.u8 %0, [%1];" : "=h"(q) : "r"(raw + r * 64 + c) : "memory");
+            const T f = from_float<T>((float)(int8_t)q);
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + swizzled(r, 2 * c)), "h"(*reinterpret_cast<const uint16_t *>(&f)) : "memory");
+        } else {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) {
-        if (p.x_scale) sum = __fmul_rn(sum, p.x_scale[row]);
-        if (p.scaling) sum = __fmul_rn(sum, p.scaling[i]);
-        p.v[at] = sum;
+            for (int e = 0; e < GRAIN; e += 4) {
+                int q;
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(q) : "r"(raw + r * 64 + c + e) : "memory");
+                const uint32_t lo = pack2<T>((float)(int8_t)q, (float)(int8_t)(q >> 8));
+                const uint32_t hi = pack2<T>((float)(int8_t)(q >> 16), (float)(q >> 24));
+                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(dst + swizzled(r, 2 * (c + e))), "r"(lo), "r"(hi) : "memory");
+            }
+        }
+    }
+}
+template <typename T, int THREADS>
+__device__ __forceinline__ void widen_rows(int grain, uint32_t raw, uint32_t dst, int rows)
+{
+    if (grain == 16) widen_rows_grain<T, 16, THREADS>(raw, dst, rows);
+    else if (grain == 8) widen_rows_grain<T, 8, THREADS>(raw, dst, rows);
+    else if (grain == 4) widen_rows_grain<T, 4, THREADS>(raw, dst, rows);
+    else widen_rows_grain<T, 1, THREADS>(raw, dst, rows);
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// Which tokens make a tile
+// ---------------------------------------------------------------------------------------------------------
+
+struct Tile {
+    int adapter, count;   // adapter -1: tokens without one; count 0: there is no such tile
+};
+
+__device__ __forceinline__ int adapter_of(const AdapterParams &p, int t)
+{
+    const int i = __ldg(p.ids + t);
+    return i >= 0 && i < p.adapters ? i : -1;
+}
+
+// Tile number blockIdx.x of at most TN tokens each, found by every CTA for itself; rows[slot] = token.  A token whose rank among the
+// tokens of its adapter is a multiple of TN begins a tile, and tiles are numbered by their first tokens.
+struct SelfPlan {
+    int ids[kSelfPlan];
+    int leaders[kSelfPlan / 32];
+    int adapter, from, count;
+};
+template <int TN, int THREADS>
+__device__ __forceinline__ Tile self_plan(const AdapterParams &p, SelfPlan &s, int *rows)
+{
+    constexpr int PER = kSelfPlan / THREADS;
+    const int tid = threadIdx.x;
+    for (int t = tid; t < kSelfPlan; t += THREADS) s.ids[t] = t < p.rows ? adapter_of(p, t) : -2;
+    if (tid == 0) { s.count = 0; s.from = -1; s.adapter = -1; }
+    __syncthreads();
+    int rank[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int t = j * THREADS + tid, id = s.ids[t];
+        int r = 0;
+        for (int o = 0; o < p.rows; o += 4) {
+            const int4 q = *reinterpret_cast<const int4 *>(&s.ids[o]);
+            r += (q.x == id && o < t) + (q.y == id && o + 1 < t) + (q.z == id && o + 2 < t) + (q.w == id && o + 3 < t);
+        }
+        rank[j] = r;
+        const unsigned b = __ballot_sync(0xffffffffu, id != -2 && r % TN == 0);
+        if ((tid & 31) == 0) s.leaders[t >> 5] = (int)b;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int t = j * THREADS + tid;
+        int before = 0;
+        for (int w = 0; w < (t >> 5); ++w) before += __popc(s.leaders[w]);
+        const unsigned mine = (unsigned)s.leaders[t >> 5];
+        before += __popc(mine & ((1u << (t & 31)) - 1u));
+        if ((mine >> (t & 31) & 1u) && before == (int)blockIdx.x) { s.adapter = s.ids[t]; s.from = rank[j]; }
+    }
+    __syncthreads();
+    if (s.from < 0) return Tile{-1, 0};
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int t = j * THREADS + tid;
+        if (s.ids[t] == s.adapter && rank[j] >= s.from && rank[j] < s.from + TN) {
+            rows[rank[j] - s.from] = t;
+            atomicAdd(&s.count, 1);
+        }
+    }
+    __syncthreads();
+    return Tile{s.adapter, s.count};
+}
+
+// The same from the plan in the workspace.
+__device__ __forceinline__ Tile read_plan(const AdapterParams &p, int threads, int *rows)
+{
+    if ((int)blockIdx.x >= __ldcg(p.n_tiles)) return Tile{-1, 0};
+    const int4 t = __ldcg(p.tiles + blockIdx.x);
+    for (int i = threadIdx.x; i < t.z; i += threads) rows[i] = __ldcg(p.order + t.y + i);
+    __syncthreads();
+    return Tile{t.x, t.z};
+}
+
+// One CTA: counts the tokens of every adapter (the last counter: none), lays the tiles out and sorts the tokens.
+__global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(const AdapterParams p, int tile_tokens)
+{
+    extern __shared__ int counts[];          // [adapters + 1] tokens, then the next place in `order`
+    __shared__ int2 carry, warp_sum[32];
+    const int tid = threadIdx.x, lane = tid & 31, n = p.adapters + 1;
+    pdl_release();
+    for (int i = tid; i < n; i += kPlanThreads) counts[i] = 0;
+    if (tid == 0) carry = make_int2(0, 0);
+    if (tid < 4) p.status[tid] = 0;
+    __syncthreads();
+    for (int t0 = 0; t0 < p.rows; t0 += kPlanThreads) {
+        const int t = t0 + tid, id = t < p.rows ? adapter_of(p, t) : -2;
+        const unsigned same = __match_any_sync(0xffffffffu, id);
+        if (id != -2 && lane == __ffs(same) - 1) atomicAdd(&counts[id < 0 ? p.adapters : id], __popc(same));
+    }
+    __syncthreads();
+    // running totals of tokens and tiles over the adapters
+    for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+        const int i = i0 + tid, c = i < n ? counts[i] : 0, tiles = (c + tile_tokens - 1) / tile_tokens;
+        int2 s = make_int2(c, tiles);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int a = __shfl_up_sync(0xffffffffu, s.x, o), b = __shfl_up_sync(0xffffffffu, s.y, o);
+            if (lane >= o) { s.x += a; s.y += b; }
+        }
+        if (lane == 31) warp_sum[tid >> 5] = s;
+        __syncthreads();
+        if (tid < 32) {
+            int2 w = warp_sum[tid];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int a = __shfl_up_sync(0xffffffffu, w.x, o), b = __shfl_up_sync(0xffffffffu, w.y, o);
+                if (lane >= o) { w.x += a; w.y += b; }
+            }
+            warp_sum[tid] = w;
+        }
+        __syncthreads();
+        const int2 before = tid >= 32 ? warp_sum[(tid >> 5) - 1] : make_int2(0, 0);
+        const int start = carry.x + before.x + s.x - c, first = carry.y + before.y + s.y - tiles;
+        if (i < n) {
+            counts[i] = start;
+            for (int q = 0; q < tiles; ++q)
+                p.tiles[first + q] = make_int4(i < p.adapters ? i : -1, start + q * tile_tokens, min(tile_tokens, c - q * tile_tokens), 0);
+        }
+        __syncthreads();
+        if (tid == kPlanThreads - 1) carry = make_int2(carry.x + warp_sum[31].x, carry.y + warp_sum[31].y);
+        __syncthreads();
+    }
+    if (tid == 0) *p.n_tiles = carry.y;
+    for (int t0 = 0; t0 < p.rows; t0 += kPlanThreads) {
+        const int t = t0 + tid, id = t < p.rows ? adapter_of(p, t) : -2;
+        const unsigned same = __match_any_sync(0xffffffffu, id);
+        const int leader = __ffs(same) - 1;
+        int at = 0;
+        if (id != -2 && lane == leader) at = atomicAdd(&counts[id < 0 ? p.adapters : id], __popc(same));
+        at = __shfl_sync(0xffffffffu, at, leader);
+        if (id != -2) p.order[at + __popc(same & ((1u << lane) - 1u))] = t;
     }
 }
 
-// One CTA per row and 128 columns.
-template <typename T>
-__global__ void __launch_bounds__(128) adapter_expand_kernel(const AdapterParams p)
+// ---------------------------------------------------------------------------------------------------------
+// v = scaling * x a^T
+// ---------------------------------------------------------------------------------------------------------
+
+__host__ __device__ constexpr int align_up(int v, int a) { return (v + a - 1) / a * a; }
+__host__ __device__ inline int tmem_cols(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : 128; }
+// Bytes of a stage: the tokens' rows and the weights' (and the int8 rows as they come).
+__host__ __device__ inline int shrink_stage(int tn, int rank_pad, bool i8) { return (tn + rank_pad) * 128 + (i8 ? tn * 64 : 0); }
+// The first product reads 128 rows from the start of the tokens' tile, however few there are: what lies behind it decides nothing
+// but results that are not read.  The last stage needs that much room behind it.
+inline int shrink_smem(int tn, int rank_pad, bool i8) { return 1024 + kShrinkStages * align_up(shrink_stage(tn, rank_pad, i8), 1024) + 128 * 128; }
+
+// Grid: (tiles, ksplit).  CTA y takes the K blocks [y * blocks / ksplit, (y + 1) * blocks / ksplit).
+template <typename T, bool I8, int TN, bool SELF>
+__global__ void __launch_bounds__(kShrinkThreads) adapter_shrink_kernel(const AdapterParams p)
 {
-    const int row = blockIdx.x, c = blockIdx.y * 128 + threadIdx.x;
-    if (c >= p.n) return;
-    const int i = p.ids[row];
-    float sum = to_float(reinterpret_cast<const T *>(p.base)[row * p.ld_base + c]);
-    if (i >= 0 && i < p.adapters) {
-        const T *b = reinterpret_cast<const T *>(p.b) + ((long long)i * p.n + c) * p.rank;
-        const float *v = p.v + (long long)row * p.rank;
-        float delta = 0.0f;
-        for (int j = 0; j < p.rank; ++j) delta = __fmaf_rn(v[j], to_float(b[j]), delta);
-        sum = __fadd_rn(sum, delta);
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ alignas(16) SelfPlan plan;
+    __shared__ alignas(8) uint64_t bars[kShrinkStages];
+    __shared__ uint32_t tmem_base;
+    __shared__ int gave_up;
+    __shared__ int rows[TN];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t cols = tmem_cols(p.rank_pad);
+    if (warp == 0) tmem_alloc(&tmem_base, cols);
+    if (tid == 0) {
+        for (int i = 0; i < kShrinkStages; ++i) mbar_init(smem_u32(&bars[i]), 1);
+        gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (SELF && blockIdx.x == 0 && blockIdx.y == 0)   // long before a wait can run out and record it
+            for (int i = 0; i < 4; ++i) p.status[i] = 0;
     }
-    reinterpret_cast<T *>(p.out)[row * p.ld_out + c] = from_float<T>(sum);
+    tc_fence_before();
+    if (!SELF) pdl_wait();
+    // Only now: the next kernel's CTAs wait for this grid with tensor memory in their hands, so every CTA of this one has its own first.
+    __syncthreads();
+    pdl_release();
+    tc_fence_after();
+    const Tile tile = SELF ? self_plan<TN, kShrinkThreads>(p, plan, rows) : read_plan(p, kShrinkThreads, rows);
+    const int blocks = (p.k + kBlockK - 1) / kBlockK;
+    const int kb0 = (int)((long long)blockIdx.y * blocks / p.ksplit), kb1 = (int)((long long)(blockIdx.y + 1) * blocks / p.ksplit);
+    if (tile.count > 0 && tile.adapter >= 0 && kb0 < kb1) {
+        const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+        const uint32_t stage_bytes = align_up(shrink_stage(TN, p.rank_pad, I8), 1024);
+        constexpr int XB = I8 ? 1 : 2;
+        const char *x = reinterpret_cast<const char *>(p.x);
+        const char *a = reinterpret_cast<const char *>(p.a) + (long long)tile.adapter * p.rank * p.k * 2;
+        const auto load = [&](int kb) {
+            const uint32_t s = smem0 + (uint32_t)((kb - kb0) % kShrinkStages) * stage_bytes;
+            const int have = min(kBlockK, p.k - kb * kBlockK);
+            copy_rows<true, kShrinkThreads>(p.grain_a, s + TN * 128, p.rank, 128, have * 2,
+                                            [&](int r) { return a + ((long long)r * p.k + (long long)kb * kBlockK) * 2; });
+            const auto x_row = [&](int r) { return x + ((long long)rows[r] * p.ld_x + (long long)kb * kBlockK) * XB; };
+            if (I8) copy_rows<false, kShrinkThreads>(p.grain_x, s + (TN + p.rank_pad) * 128, tile.count, 64, have, x_row);
+            else copy_rows<true, kShrinkThreads>(p.grain_x, s, tile.count, 128, have * 2, x_row);
+        };
+        for (int i = 0; i < kShrinkStages - 1; ++i) {
+            if (kb0 + i < kb1) load(kb0 + i);
+            cp_commit();
+        }
+        const uint32_t idesc = instr_desc<T>(p.rank_pad);
+        for (int kb = kb0; kb < kb1; ++kb) {
+            const int i = kb - kb0, stage = i % kShrinkStages;
+            const uint32_t s = smem0 + (uint32_t)stage * stage_bytes;
+            cp_wait<kShrinkStages - 2>();
+            if (I8) widen_rows<T, kShrinkThreads>(p.grain_x, s + (TN + p.rank_pad) * 128, s, tile.count);
+            fence_async_proxy();
+            __syncthreads();
+            if (tid == 0) {
+                tc_fence_after();
+                const uint64_t xd = operand_desc(s), ad = operand_desc(s + TN * 128);
+                const int steps = (min(kBlockK, p.k - kb * kBlockK) + 15) / 16;
+                for (int j = 0; j < steps; ++j) umma_f16(tmem_base, xd + j * 2, ad + j * 2, idesc, (i | j) != 0);
+                umma_commit(smem_u32(&bars[stage]));
+            }
+            // the stage that the block before this one was read from takes the next block
+            if (kb + kShrinkStages - 1 < kb1) {
+                if (i > 0) mbar_wait(smem_u32(&bars[(i - 1) % kShrinkStages]), ((i - 1) / kShrinkStages) & 1, &gave_up, p.status, 900);
+                load(kb + kShrinkStages - 1);
+            }
+            cp_commit();
+        }
+        const int last = kb1 - 1 - kb0;
+        mbar_wait(smem_u32(&bars[last % kShrinkStages]), (last / kShrinkStages) & 1, &gave_up, p.status, 901);
+        tc_fence_after();
+        const int slot = warp * 32 + lane;
+        if (warp * 32 < TN) {
+            const bool live = slot < tile.count;
+            const int row = live ? rows[slot] : 0;
+            float f = p.scaling ? __ldg(p.scaling + tile.adapter) : 1.0f;
+            if (I8 && live) f = __fmul_rn(f, __ldg(p.x_scale + row));
+            float4 *v = reinterpret_cast<float4 *>(p.v + ((long long)blockIdx.y * p.rows + row) * p.rank_pad);
+            for (int c = 0; c < p.rank_pad; c += 16) {
+                uint32_t d[16];
+                tmem_ld16(tmem_base + ((uint32_t)(warp * 32) << 16) + (uint32_t)c, d);
+                tmem_ld_wait();
+                if (live) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        v[(c + e) / 4] = make_float4(__fmul_rn(__uint_as_float(d[e]), f), __fmul_rn(__uint_as_float(d[e + 1]), f),
+                                                     __fmul_rn(__uint_as_float(d[e + 2]), f), __fmul_rn(__uint_as_float(d[e + 3]), f));
+                }
+            }
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == 0) tmem_dealloc(tmem_base, cols);
 }
 
-template <typename T>
-cudaError_t launch_typed(const AdapterParams &p, bool x_i8, cudaStream_t stream)
+// ---------------------------------------------------------------------------------------------------------
+// out = base + v b^T
+// ---------------------------------------------------------------------------------------------------------
+
+__host__ __device__ inline int rank_atoms(int rank_pad) { return rank_pad > 64 ? 2 : 1; }
+__host__ __device__ inline int expand_stage(int tn, int rank_pad) { return rank_atoms(rank_pad) * kChunkN * 128 + tn * kChunkN * 2; }
+inline int expand_smem(int tn, int rank_pad) { return 1024 + rank_atoms(rank_pad) * tn * 256 + kExpandStages * expand_stage(tn, rank_pad); }
+
+// Grid: (tiles, nsplit).  CTA y takes the channel chunks [y * chunks / nsplit, (y + 1) * chunks / nsplit).
+template <typename T, int TN, bool SELF>
+__global__ void __launch_bounds__(kExpandThreads) adapter_expand_kernel(const AdapterParams p)
 {
-    const long long dots = (long long)p.rows * p.rank;
-    if (x_i8) adapter_shrink_kernel<T, int8_t><<<(unsigned)((dots + 3) / 4), 128, 0, stream>>>(p);
-    else adapter_shrink_kernel<T, T><<<(unsigned)((dots + 3) / 4), 128, 0, stream>>>(p);
-    adapter_expand_kernel<T><<<dim3((unsigned)p.rows, (unsigned)((p.n + 127) / 128)), 128, 0, stream>>>(p);
-    return cudaGetLastError();
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ alignas(16) SelfPlan plan;
+    __shared__ alignas(8) uint64_t bar;
+    __shared__ uint32_t tmem_base;
+    __shared__ int gave_up;
+    __shared__ int rows[TN];
+    __shared__ float unscale[TN];          // fp16: the power of two that v was divided by
+    constexpr bool F16 = std::is_same<T, __half>::value;
+    constexpr uint32_t COLS = TN <= 32 ? 32 : TN;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (warp == 0) tmem_alloc(&tmem_base, COLS);
+    if (tid == 0) {
+        mbar_init(smem_u32(&bar), 1);
+        gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const Tile tile = SELF ? self_plan<TN, kExpandThreads>(p, plan, rows) : read_plan(p, kExpandThreads, rows);
+    const int chunks = (p.n + kChunkN - 1) / kChunkN;
+    const int c0 = (int)((long long)blockIdx.y * chunks / p.nsplit), c1 = (int)((long long)(blockIdx.y + 1) * chunks / p.nsplit);
+    const T *base = reinterpret_cast<const T *>(p.base);
+    T *out = reinterpret_cast<T *>(p.out);
+    if (tile.count > 0 && tile.adapter < 0) {
+        if (p.out != p.base) {
+            pdl_wait();
+            const int n0 = c0 * kChunkN, width = min(c1 * kChunkN, p.n) - n0;
+            for (int r = 0; r < tile.count; ++r)
+                for (int c = tid; c < width; c += kExpandThreads)
+                    out[(long long)rows[r] * p.ld_out + n0 + c] = base[(long long)rows[r] * p.ld_base + n0 + c];
+        }
+    } else if (tile.count > 0 && c0 < c1) {
+        const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+        const int atoms = rank_atoms(p.rank_pad);
+        const uint32_t v_hi = smem0, v_lo = v_hi + (uint32_t)(atoms * TN * 128), stage0 = v_lo + (uint32_t)(atoms * TN * 128);
+        const uint32_t stage_bytes = expand_stage(TN, p.rank_pad), base_at = (uint32_t)(atoms * kChunkN * 128);
+        const char *b = reinterpret_cast<const char *>(p.b) + (long long)tile.adapter * p.n * p.rank * 2;
+        const auto load = [&](int c) {
+            const uint32_t s = stage0 + (uint32_t)((c - c0) % kExpandStages) * stage_bytes;
+            const int n0 = c * kChunkN, channels = min(kChunkN, p.n - n0);
+            for (int at = 0; at < atoms; ++at) {
+                const int left = p.rank_pad - at * 64;                       // a whole number of K steps, zero beyond the rank
+                const int width = left > 32 ? 128 : left > 16 ? 64 : 32;
+                copy_rows<true, kExpandThreads>(p.grain_b, s + (uint32_t)at * kChunkN * 128, channels, width, (p.rank - at * 64) * 2,
+                                                [&](int r) { return b + ((long long)(n0 + r) * p.rank + at * 64) * 2; });
+            }
+            copy_rows<false, kExpandThreads>(p.grain_base, s + base_at, tile.count, kChunkN * 2, channels * 2,
+                                             [&](int r) { return reinterpret_cast<const char *>(base + (long long)rows[r] * p.ld_base + n0); });
+        };
+        for (int i = 0; i < kExpandStages; ++i) {
+            if (c0 + i < c1) load(c0 + i);
+            cp_commit();
+        }
+        pdl_wait();   // the partial sums are complete
+        {
+            constexpr int LANES = kExpandThreads / TN;    // per token
+            const int slot = tid / LANES, part = tid % LANES;
+            const bool live = slot < tile.count;
+            const int row = live ? rows[slot] : 0;
+            const auto sum8 = [&](int j, float (&f)[8]) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = 0.0f;
+                if (!live) return;
+                for (int s = 0; s < p.ksplit; ++s) {
+                    const float4 *v = reinterpret_cast<const float4 *>(p.v + ((long long)s * p.rows + row) * p.rank_pad + j);
+                    const float4 q = __ldcg(v), w = __ldcg(v + 1);
+                    f[0] += q.x; f[1] += q.y; f[2] += q.z; f[3] += q.w; f[4] += w.x; f[5] += w.y; f[6] += w.z; f[7] += w.w;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (j + e >= p.rank) f[e] = 0.0f;
+            };
+            float down = 1.0f;
+            if (F16) {
+                uint32_t m = 0;
+                for (int j = part * 8; j < p.rank_pad; j += LANES * 8) {
+                    float f[8];
+                    sum8(j, f);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(f[e]) & 0x7fffffffu);
+                }
+#pragma unroll
+                for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                // 2^-e for a largest value in [2^e, 2^(e+1)); none for zero, for what no power of two can help, and at the ends of fp32
+                const int e = (int)(m >> 23) - 127;
+                const bool shift = m != 0 && e > -120 && e < 120;
+                down = shift ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.0f;
+                if (part == 0) unscale[slot] = shift ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.0f;
+            }
+            for (int j = part * 8; j < p.rank_pad; j += LANES * 8) {
+                float f[8], g[8];
+                sum8(j, f);
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    f[e] = __fmul_rn(f[e], down);
+                    g[e] = __fsub_rn(f[e], to_float(from_float<T>(f[e])));
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    hi[e] = pack2<T>(f[2 * e], f[2 * e + 1]);
+                    lo[e] = pack2<T>(g[2 * e], g[2 * e + 1]);
+                }
+                const uint32_t at = (uint32_t)(j / 64 * TN * 128) + swizzled(slot, (j % 64) * 2);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(v_hi + at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(v_lo + at), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
+            }
+        }
+        const uint32_t idesc = instr_desc<T>(TN);
+        for (int c = c0; c < c1; ++c) {
+            const int i = c - c0;
+            const uint32_t s = stage0 + (uint32_t)(i % kExpandStages) * stage_bytes;
+            cp_wait<kExpandStages - 1>();
+            fence_async_proxy();
+            __syncthreads();
+            if (tid == 0) {
+                tc_fence_after();
+                uint32_t more = 0;
+                for (int j = 0; j < p.rank_pad / 16; ++j) {
+                    const uint64_t bd = operand_desc(s + (uint32_t)(j / 4) * kChunkN * 128) + (j % 4) * 2;
+                    umma_f16(tmem_base, bd, operand_desc(v_hi + (uint32_t)(j / 4) * TN * 128) + (j % 4) * 2, idesc, more);
+                    more = 1;
+                    umma_f16(tmem_base, bd, operand_desc(v_lo + (uint32_t)(j / 4) * TN * 128) + (j % 4) * 2, idesc, more);
+                }
+                umma_commit(smem_u32(&bar));
+            }
+            mbar_wait(smem_u32(&bar), i & 1, &gave_up, p.status, 910);
+            tc_fence_after();
+            // warp w: channels 32 (w % 4) + lane, half of the tokens
+            const int q = warp & 3, ch = q * 32 + lane, n = c * kChunkN + ch;
+            constexpr int HALF = TN / 2;
+            const int first = (warp >> 2) * HALF;
+            for (int t0 = first; t0 < min(first + HALF, tile.count); t0 += 8) {
+                uint32_t d[8];
+                tmem_ld8(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)t0, d);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int slot = t0 + e;
+                    if (slot < tile.count && n < p.n) {
+                        uint16_t raw;
+                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(raw) : "r"(s + base_at + (uint32_t)(slot * kChunkN * 2 + ch * 2)) : "memory");
+                        float f = __uint_as_float(d[e]);
+                        if (F16) f = __fmul_rn(f, unscale[slot]);
+                        out[(long long)rows[slot] * p.ld_out + n] = from_float<T>(__fadd_rn(to_float(*reinterpret_cast<const T *>(&raw)), f));
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncthreads();
+            if (c + kExpandStages < c1) load(c + kExpandStages);
+            cp_commit();
+        }
+        cp_wait<0>();
+    }
+    pdl_wait();   // this grid must not end before the kernels in front of it: the stream goes on behind it alone
+    __syncthreads();
+    if (warp == 0) tmem_dealloc(tmem_base, COLS);
+}
+
+// ---------------------------------------------------------------------------------------------------------
+
+template <typename... KArgs>
+cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, int threads, int smem, cudaStream_t stream, bool dependent, KArgs... args)
+{
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = dependent ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+constexpr size_t align256(size_t v) { return (v + 255) / 256 * 256; }
+
+struct Shape {
+    int tile_tokens, tiles, ksplit, nsplit, rank_pad;
+    bool self;
+};
+
+// Tiles of 16 tokens while every CTA plans for itself, of 64 beyond.  `tiles` is the most there can be: full ones, and one that is not for
+// every adapter and for none.  K and N are split so that about two CTAs find a place on every SM, but no CTA gets less than two K blocks.
+Shape shape_of(const AdapterProblem &p)
+{
+    Shape s;
+    s.self = p.rows <= kSelfPlan;
+    s.tile_tokens = s.self ? 16 : 64;
+    const long long partial = p.adapters + 1 < p.rows ? p.adapters + 1 : p.rows;
+    s.tiles = (int)(p.rows / s.tile_tokens + partial);
+    if (s.tiles > p.rows) s.tiles = (int)p.rows;
+    s.rank_pad = align_up((int)p.rank, 16);
+    const int want = (2 * 148 + s.tiles - 1) / s.tiles;
+    const int blocks = (int)((p.k + kBlockK - 1) / kBlockK), chunks = (int)((p.n + kChunkN - 1) / kChunkN);
+    s.ksplit = want < blocks / 2 ? want : blocks / 2;
+    if (s.ksplit > 16) s.ksplit = 16;
+    if (s.ksplit < 1) s.ksplit = 1;
+    s.nsplit = 2 * want < chunks ? 2 * want : chunks;
+    return s;
+}
+
+int grain_of(const void *base, long long pitch_bytes, int smallest)
+{
+    const uintptr_t v = (uintptr_t)base | (uintptr_t)pitch_bytes;
+    return v % 16 == 0 ? 16 : v % 8 == 0 ? 8 : v % 4 == 0 ? 4 : smallest;
+}
+
+template <typename T, bool I8, int TN, bool SELF>
+cudaError_t launch_tiles(const AdapterParams &p, const Shape &s, cudaStream_t stream)
+{
+    cudaError_t e = cudaSuccess;
+    if (!SELF) {
+        e = launch_kernel(adapter_plan_kernel, dim3(1), kPlanThreads, (p.adapters + 1) * 4, stream, false, p, s.tile_tokens);
+        if (e != cudaSuccess) return e;
+    }
+    e = launch_kernel(adapter_shrink_kernel<T, I8, TN, SELF>, dim3((unsigned)s.tiles, (unsigned)s.ksplit), kShrinkThreads,
+                      shrink_smem(TN, s.rank_pad, I8), stream, !SELF, p);
+    if (e != cudaSuccess) return e;
+    return launch_kernel(adapter_expand_kernel<T, TN, SELF>, dim3((unsigned)s.tiles, (unsigned)s.nsplit), kExpandThreads,
+                         expand_smem(TN, s.rank_pad), stream, true, p);
+}
+
+template <typename T, bool I8>
+cudaError_t launch_typed(const AdapterParams &p, const Shape &s, cudaStream_t stream)
+{
+    return s.self ? launch_tiles<T, I8, 16, true>(p, s, stream) : launch_tiles<T, I8, 64, false>(p, s, stream);
 }
 
 }  // namespace
 
-size_t adapter_workspace_bytes(const AdapterProblem &p) { return 256 + ((size_t)p.rows * p.rank * 4 + 255) / 256 * 256; }
+size_t adapter_workspace_bytes(const AdapterProblem &p)
+{
+    const Shape s = shape_of(p);
+    return 256 + (s.self ? 0 : 256 + align256((size_t)s.tiles * sizeof(int4)) + align256((size_t)p.rows * 4)) +
+           align256((size_t)s.ksplit * (size_t)p.rows * (size_t)s.rank_pad * 4);
+}
 
 cudaError_t adapter_launch(const AdapterProblem &a, void *workspace, size_t workspace_bytes, cudaStream_t stream)
 {
     if (a.rows <= 0) return cudaSuccess;
-    if (!workspace || workspace_bytes < adapter_workspace_bytes(a)) return cudaErrorInvalidValue;
+    if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < adapter_workspace_bytes(a)) return cudaErrorInvalidValue;
+    const Shape s = shape_of(a);
     AdapterParams p;
     p.base = a.base; p.x = a.x; p.a = a.a; p.b = a.b;
     p.x_scale = a.x_scale; p.scaling = a.scaling; p.ids = a.ids; p.out = a.out;
-    p.v = reinterpret_cast<float *>(static_cast<char *>(workspace) + 256);
     p.ld_base = a.ld_base; p.ld_x = a.ld_x; p.ld_out = a.ld_out;
     p.rows = (int)a.rows; p.k = (int)a.k; p.n = (int)a.n; p.adapters = (int)a.adapters; p.rank = (int)a.rank;
-    return a.dtype == kF16 ? launch_typed<__half>(p, a.x_i8, stream) : launch_typed<__nv_bfloat16>(p, a.x_i8, stream);
+    p.rank_pad = s.rank_pad;
+    const int xb = a.x_i8 ? 1 : 2;
+    p.grain_x = grain_of(a.x, a.ld_x * xb, xb);
+    p.grain_a = grain_of(a.a, a.k * 2, 2);
+    p.grain_b = grain_of(a.b, a.rank * 2, 2);
+    p.grain_base = grain_of(a.base, a.ld_base * 2, 2);
+    p.ksplit = s.ksplit; p.nsplit = s.nsplit;
+    char *ws = static_cast<char *>(workspace);
+    p.status = reinterpret_cast<int *>(ws);
+    ws += 256;
+    p.n_tiles = nullptr; p.tiles = nullptr; p.order = nullptr;
+    if (!s.self) {
+        p.n_tiles = reinterpret_cast<int *>(ws); ws += 256;
+        p.tiles = reinterpret_cast<int4 *>(ws); ws += align256((size_t)s.tiles * sizeof(int4));
+        p.order = reinterpret_cast<int *>(ws); ws += align256((size_t)a.rows * 4);
+    }
+    p.v = reinterpret_cast<float *>(ws);
+    if (a.dtype == kF16) return a.x_i8 ? launch_typed<__half, true>(p, s, stream) : launch_typed<__half, false>(p, s, stream);
+    return a.x_i8 ? launch_typed<__nv_bfloat16, true>(p, s, stream) : launch_typed<__nv_bfloat16, false>(p, s, stream);
 }
 
 }  // namespace gmm

@@ -165,7 +165,7 @@ aclnnStatus adapter_phase1(const aclTensor *base, const aclTensor *x, const aclT
     GMM_REQUIRE(rows >= 0 && rows <= kMaxRows, ACLNN_ERR_PARAM_INVALID, "base must not have more than %lld rows.", (long long)kMaxRows);
     GMM_REQUIRE(n >= 1 && n <= kMaxAxis && k >= 1 && k <= kMaxAxis, ACLNN_ERR_PARAM_INVALID, "k and n must be in [1, %lld].", (long long)kMaxAxis);
     GMM_REQUIRE(rank >= 1 && rank <= 128, ACLNN_ERR_PARAM_INVALID, "rank must be in [1, 128], but is %lld.", (long long)rank);
-    GMM_REQUIRE(adapters >= 1 && adapters <= 65535, ACLNN_ERR_PARAM_INVALID, "a must hold 1 to 65535 adapters, but holds %lld.", (long long)adapters);
+    GMM_REQUIRE(adapters >= 1 && adapters <= 16384, ACLNN_ERR_PARAM_INVALID, "a must hold 1 to 16384 adapters, but holds %lld.", (long long)adapters);
     REQUIRE_SHAPE2(x, rows, k);
     GMM_REQUIRE(x->dtype == base->dtype || x->dtype == ACL_INT8, ACLNN_ERR_PARAM_INVALID, "x dtype must be base's or int8.");
     GMM_REQUIRE(x->dtype != ACL_INT8 || xScale, ACLNN_ERR_PARAM_NULLPTR, "an int8 x needs xScale.");
