@@ -42,7 +42,7 @@ struct AdapterParams {
     long long ld_base, ld_x, ld_out;
     int rows, k, n, adapters, rank;
     int rank_pad;                   // rank, rounded up to the tensor cores' K step of 16
-    int grain_x, grain_a, grain_b, grain_base;   // bytes of a copy
+    int grain_x, grain_a, grain_b, grain_base, grain_out;   // bytes of a copy
     int ksplit, nsplit;
     int *status;                    // [4]
     int *n_tiles;
@@ -285,7 +285,7 @@ __device__ __forceinline__ Tile self_plan(const AdapterParams &p, SelfPlan &s, i
     for (int j = 0; j < PER; ++j) {
         const int t = j * THREADS + tid, id = s.ids[t];
         int r = 0;
-        for (int o = 0; o < p.rows; o += 4) {
+        for (int o = 0; j * THREADS < p.rows && o < p.rows; o += 4) {
             const int4 q = *reinterpret_cast<const int4 *>(&s.ids[o]);
             r += (q.x == id && o < t) + (q.y == id && o + 1 < t) + (q.z == id && o + 2 < t) + (q.w == id && o + 3 < t);
         }
@@ -401,7 +401,9 @@ __host__ __device__ inline int shrink_stage(int tn, int rank_pad, bool i8) { ret
 inline int shrink_smem(int tn, int rank_pad, bool i8) { return 1024 + kShrinkStages * align_up(shrink_stage(tn, rank_pad, i8), 1024) + 128 * 128; }
 
 // Grid: (tiles, ksplit).  CTA y takes the K blocks [y * blocks / ksplit, (y + 1) * blocks / ksplit).
-template <typename T, bool I8, int TN, bool SELF>
+// FAST: rows of x and a start on 16-byte boundaries.  A thread then copies the same 16 bytes of every K block, whose addresses it works
+// out once; with the addresses of every copy worked out anew the kernel was bound by its instructions.
+template <typename T, bool I8, int TN, bool SELF, bool FAST>
 __global__ void __launch_bounds__(kShrinkThreads) adapter_shrink_kernel(const AdapterParams p)
 {
     extern __shared__ uint8_t smem_raw[];
@@ -435,9 +437,39 @@ __global__ void __launch_bounds__(kShrinkThreads) adapter_shrink_kernel(const Ad
         constexpr int XB = I8 ? 1 : 2;
         const char *x = reinterpret_cast<const char *>(p.x);
         const char *a = reinterpret_cast<const char *>(p.a) + (long long)tile.adapter * p.rank * p.k * 2;
+        constexpr int XC = I8 ? 4 : 8;                        // copies per token row of a K block
+        constexpr int NX = (TN * XC + kShrinkThreads - 1) / kShrinkThreads, NA = 128 * 8 / kShrinkThreads;
+        const char *x_at[NX];
+        const int xc = tid % XC, ac = tid % 8;
+        const char *a_at = a + (long long)(tid / 8) * p.k * 2 + ac * 16;
+        const int a_step = (kShrinkThreads / 8) * p.k * 2;
+        if (FAST) {
+#pragma unroll
+            for (int i = 0; i < NX; ++i) {
+                const int r = tid / XC + i * (kShrinkThreads / XC);
+                x_at[i] = r < tile.count ? x + (long long)rows[r] * p.ld_x * XB + xc * 16 : nullptr;
+            }
+        }
         const auto load = [&](int kb) {
             const uint32_t s = smem0 + (uint32_t)((kb - kb0) % kShrinkStages) * stage_bytes;
             const int have = min(kBlockK, p.k - kb * kBlockK);
+            if (FAST) {
+                const int ax = min(max(have * XB - xc * 16, 0), 16), aa = min(max(have * 2 - ac * 16, 0), 16);
+                // a copy of no bytes names the row's start: its own place may lie beyond the tensor
+                const long long xo = ax > 0 ? (long long)kb * kBlockK * XB : -(long long)xc * 16;
+                const long long ao = aa > 0 ? (long long)kb * kBlockK * 2 : -(long long)ac * 16;
+#pragma unroll
+                for (int i = 0; i < NX; ++i) {
+                    const int r = tid / XC + i * (kShrinkThreads / XC);
+                    if (x_at[i]) cp_async<16>(I8 ? s + (TN + p.rank_pad) * 128 + r * 64 + xc * 16 : s + swizzled(r, xc * 16), x_at[i] + xo, ax);
+                }
+#pragma unroll
+                for (int i = 0; i < NA; ++i) {
+                    const int r = tid / 8 + i * (kShrinkThreads / 8);
+                    if (r < p.rank) cp_async<16>(s + TN * 128 + swizzled(r, ac * 16), a_at + (long long)i * a_step + ao, aa);
+                }
+                return;
+            }
             copy_rows<true, kShrinkThreads>(p.grain_a, s + TN * 128, p.rank, 128, have * 2,
                                             [&](int r) { return a + ((long long)r * p.k + (long long)kb * kBlockK) * 2; });
             const auto x_row = [&](int r) { return x + ((long long)rows[r] * p.ld_x + (long long)kb * kBlockK) * XB; };
@@ -453,7 +485,8 @@ __global__ void __launch_bounds__(kShrinkThreads) adapter_shrink_kernel(const Ad
             const int i = kb - kb0, stage = i % kShrinkStages;
             const uint32_t s = smem0 + (uint32_t)stage * stage_bytes;
             cp_wait<kShrinkStages - 2>();
-            if (I8) widen_rows<T, kShrinkThreads>(p.grain_x, s + (TN + p.rank_pad) * 128, s, tile.count);
+            if (I8 && FAST) widen_rows_grain<T, 16, kShrinkThreads>(s + (TN + p.rank_pad) * 128, s, tile.count);
+            else if (I8) widen_rows<T, kShrinkThreads>(p.grain_x, s + (TN + p.rank_pad) * 128, s, tile.count);
             fence_async_proxy();
             __syncthreads();
             if (tid == 0) {
@@ -507,7 +540,9 @@ __host__ __device__ inline int expand_stage(int tn, int rank_pad) { return rank_
 inline int expand_smem(int tn, int rank_pad) { return 1024 + rank_atoms(rank_pad) * tn * 256 + kExpandStages * expand_stage(tn, rank_pad); }
 
 // Grid: (tiles, nsplit).  CTA y takes the channel chunks [y * chunks / nsplit, (y + 1) * chunks / nsplit).
-template <typename T, int TN, bool SELF>
+// GB: 16 or 8 bytes of b a copy, with rows of base and out on 16-byte boundaries; addresses are worked out once, and results go back
+// through the chunk's base rows in shared memory, from which they are stored 16 bytes at a time.  0: any strides.
+template <typename T, int TN, bool SELF, int GB>
 __global__ void __launch_bounds__(kExpandThreads) adapter_expand_kernel(const AdapterParams p)
 {
     extern __shared__ uint8_t smem_raw[];
@@ -548,9 +583,42 @@ __global__ void __launch_bounds__(kExpandThreads) adapter_expand_kernel(const Ad
         const uint32_t v_hi = smem0, v_lo = v_hi + (uint32_t)(atoms * TN * 128), stage0 = v_lo + (uint32_t)(atoms * TN * 128);
         const uint32_t stage_bytes = expand_stage(TN, p.rank_pad), base_at = (uint32_t)(atoms * kChunkN * 128);
         const char *b = reinterpret_cast<const char *>(p.b) + (long long)tile.adapter * p.n * p.rank * 2;
+        // b: the copies of a chunk, offset in its rows << 8 | bytes, and place in the tile
+        constexpr int NB = GB ? 256 / (2 * GB) : 1, NR = TN * 16 / kExpandThreads;
+        const int per_row = GB ? p.rank_pad * 2 / (GB ? GB : 1) : 1, nb = per_row * kChunkN / kExpandThreads;
+        uint32_t b_from[NB], b_to[NB];
+        long long base_at_row[NR], out_at_row[NR];
+        const int rc = (tid % 16) * 8;
+        if (GB) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                const int idx = tid + i * kExpandThreads, r = idx / per_row, byte = (idx - r * per_row) * GB;
+                const int valid = min(max(p.rank * 2 - byte, 0), GB);
+                b_from[i] = (uint32_t)(r * p.rank * 2 + (valid ? byte : 0)) << 8 | (uint32_t)valid;
+                b_to[i] = (uint32_t)(byte / 128 * kChunkN * 128) + swizzled(r, byte % 128);
+            }
+#pragma unroll
+            for (int i = 0; i < NR; ++i) {
+                const int r = tid / 16 + i * 16;
+                base_at_row[i] = r < tile.count ? (long long)rows[r] * p.ld_base + rc : -1;
+                out_at_row[i] = r < tile.count ? (long long)rows[r] * p.ld_out + rc : -1;
+            }
+        }
         const auto load = [&](int c) {
             const uint32_t s = stage0 + (uint32_t)((c - c0) % kExpandStages) * stage_bytes;
             const int n0 = c * kChunkN, channels = min(kChunkN, p.n - n0);
+            if (GB) {
+                const char *from = b + (long long)n0 * p.rank * 2;
+                const uint32_t end = (uint32_t)(channels * p.rank * 2);
+#pragma unroll
+                for (int i = 0; i < NB; ++i)
+                    if (i < nb && b_from[i] >> 8 < end) cp_async<GB ? GB : 16>(s + b_to[i], from + (b_from[i] >> 8), (int)(b_from[i] & 255u));
+#pragma unroll
+                for (int i = 0; i < NR; ++i)
+                    if (base_at_row[i] >= 0 && rc < channels)
+                        cp_async<16>(s + base_at + (uint32_t)((tid + i * kExpandThreads) * 16), base + base_at_row[i] + n0, 16);
+                return;
+            }
             for (int at = 0; at < atoms; ++at) {
                 const int left = p.rank_pad - at * 64;                       // a whole number of K steps, zero beyond the rank
                 const int width = left > 32 ? 128 : left > 16 ? 64 : 32;
@@ -570,28 +638,48 @@ __global__ void __launch_bounds__(kExpandThreads) adapter_expand_kernel(const Ad
             const int slot = tid / LANES, part = tid % LANES;
             const bool live = slot < tile.count;
             const int row = live ? rows[slot] : 0;
-            const auto sum8 = [&](int j, float (&f)[8]) {
+            constexpr int CH = 16 / LANES;                // 8 components of v each, LANES apart
+            float f[CH][8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = 0.0f;
-                if (!live) return;
-                for (int s = 0; s < p.ksplit; ++s) {
-                    const float4 *v = reinterpret_cast<const float4 *>(p.v + ((long long)s * p.rows + row) * p.rank_pad + j);
-                    const float4 q = __ldcg(v), w = __ldcg(v + 1);
-                    f[0] += q.x; f[1] += q.y; f[2] += q.z; f[3] += q.w; f[4] += w.x; f[5] += w.y; f[6] += w.z; f[7] += w.w;
+            for (int h = 0; h < CH; ++h)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[h][e] = 0.0f;
+            const float4 *v = reinterpret_cast<const float4 *>(p.v + (long long)row * p.rank_pad);
+            const long long split = (long long)p.rows * p.rank_pad / 4;
+            if (live) {
+                constexpr int AHEAD = CH == 1 ? 8 : 4;    // partial sums that are fetched together
+                for (int s0 = 0; s0 < p.ksplit; s0 += AHEAD) {
+#pragma unroll
+                    for (int h = 0; h < CH; ++h) {
+                        const int j = (part + h * LANES) * 8;
+                        if (j >= p.rank_pad) break;
+                        float4 q[AHEAD][2];
+#pragma unroll
+                        for (int s = 0; s < AHEAD; ++s) {
+                            const bool there = s0 + s < p.ksplit;
+                            q[s][0] = there ? __ldcg(v + (s0 + s) * split + j / 4) : make_float4(0, 0, 0, 0);
+                            q[s][1] = there ? __ldcg(v + (s0 + s) * split + j / 4 + 1) : make_float4(0, 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int s = 0; s < AHEAD; ++s) {
+                            f[h][0] += q[s][0].x; f[h][1] += q[s][0].y; f[h][2] += q[s][0].z; f[h][3] += q[s][0].w;
+                            f[h][4] += q[s][1].x; f[h][5] += q[s][1].y; f[h][6] += q[s][1].z; f[h][7] += q[s][1].w;
+                        }
+                    }
                 }
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (j + e >= p.rank) f[e] = 0.0f;
-            };
+                for (int h = 0; h < CH; ++h)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if ((part + h * LANES) * 8 + e >= p.rank) f[h][e] = 0.0f;
+            }
             float down = 1.0f;
             if (F16) {
                 uint32_t m = 0;
-                for (int j = part * 8; j < p.rank_pad; j += LANES * 8) {
-                    float f[8];
-                    sum8(j, f);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(f[e]) & 0x7fffffffu);
-                }
+                for (int h = 0; h < CH; ++h)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(f[h][e]) & 0x7fffffffu);
 #pragma unroll
                 for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
                 // 2^-e for a largest value in [2^e, 2^(e+1)); none for zero, for what no power of two can help, and at the ends of fp32
@@ -600,18 +688,20 @@ __global__ void __launch_bounds__(kExpandThreads) adapter_expand_kernel(const Ad
                 down = shift ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.0f;
                 if (part == 0) unscale[slot] = shift ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.0f;
             }
-            for (int j = part * 8; j < p.rank_pad; j += LANES * 8) {
-                float f[8], g[8];
-                sum8(j, f);
+#pragma unroll
+            for (int h = 0; h < CH; ++h) {
+                const int j = (part + h * LANES) * 8;
+                if (j >= p.rank_pad) break;
+                float g[8];
                 uint32_t hi[4], lo[4];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    f[e] = __fmul_rn(f[e], down);
-                    g[e] = __fsub_rn(f[e], to_float(from_float<T>(f[e])));
+                    f[h][e] = __fmul_rn(f[h][e], down);
+                    g[e] = __fsub_rn(f[h][e], to_float(from_float<T>(f[h][e])));
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    hi[e] = pack2<T>(f[2 * e], f[2 * e + 1]);
+                    hi[e] = pack2<T>(f[h][2 * e], f[h][2 * e + 1]);
                     lo[e] = pack2<T>(g[2 * e], g[2 * e + 1]);
                 }
                 const uint32_t at = (uint32_t)(j / 64 * TN * 128) + swizzled(slot, (j % 64) * 2);
@@ -646,21 +736,34 @@ __global__ void __launch_bounds__(kExpandThreads) adapter_expand_kernel(const Ad
             for (int t0 = first; t0 < min(first + HALF, tile.count); t0 += 8) {
                 uint32_t d[8];
                 tmem_ld8(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)t0, d);
+                const uint32_t at = s + base_at + (uint32_t)(t0 * kChunkN * 2 + ch * 2);
+                uint16_t raw[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) asm volatile("ld.shared.u16 %0, [%1];" : "=h"(raw[e]) : "r"(at + e * kChunkN * 2) : "memory");
                 tmem_ld_wait();
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const int slot = t0 + e;
-                    if (slot < tile.count && n < p.n) {
-                        uint16_t raw;
-                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(raw) : "r"(s + base_at + (uint32_t)(slot * kChunkN * 2 + ch * 2)) : "memory");
-                        float f = __uint_as_float(d[e]);
-                        if (F16) f = __fmul_rn(f, unscale[slot]);
-                        out[(long long)rows[slot] * p.ld_out + n] = from_float<T>(__fadd_rn(to_float(*reinterpret_cast<const T *>(&raw)), f));
-                    }
+                    const int slot = t0 + e;   // beyond the tile's tokens: values of no meaning that are not stored
+                    float f = __uint_as_float(d[e]);
+                    if (F16) f = __fmul_rn(f, unscale[slot]);
+                    const T o = from_float<T>(__fadd_rn(to_float(*reinterpret_cast<const T *>(&raw[e])), f));
+                    if (GB) asm volatile("st.shared.u16 [%0], %1;" ::"r"(at + e * kChunkN * 2), "h"(*reinterpret_cast<const uint16_t *>(&o)) : "memory");
+                    else if (slot < tile.count && n < p.n) out[(long long)rows[slot] * p.ld_out + n] = o;
                 }
             }
             tc_fence_before();
             __syncthreads();
+            if (GB) {   // a thread stores the 16 bytes whose place it then fills again
+#pragma unroll
+                for (int i = 0; i < NR; ++i) {
+                    if (out_at_row[i] >= 0 && c * kChunkN + rc < p.n) {
+                        uint4 o;
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(o.x), "=r"(o.y), "=r"(o.z), "=r"(o.w)
+                                     : "r"(s + base_at + (uint32_t)((tid + i * kExpandThreads) * 16)) : "memory");
+                        *reinterpret_cast<uint4 *>(out + out_at_row[i] + c * kChunkN) = o;
+                    }
+                }
+            }
             if (c + kExpandStages < c1) load(c + kExpandStages);
             cp_commit();
         }
@@ -701,7 +804,8 @@ struct Shape {
 };
 
 // Tiles of 16 tokens while every CTA plans for itself, of 64 beyond.  `tiles` is the most there can be: full ones, and one that is not for
-// every adapter and for none.  K and N are split so that about two CTAs find a place on every SM, but no CTA gets less than two K blocks.
+// every adapter and for none.  K and N are split so that the CTAs find a place on the SMs together (about five of the small ones fit an SM,
+// two of the large), but no CTA gets less than two K blocks.
 Shape shape_of(const AdapterProblem &p)
 {
     Shape s;
@@ -711,12 +815,13 @@ Shape shape_of(const AdapterProblem &p)
     s.tiles = (int)(p.rows / s.tile_tokens + partial);
     if (s.tiles > p.rows) s.tiles = (int)p.rows;
     s.rank_pad = align_up((int)p.rank, 16);
-    const int want = (2 * 148 + s.tiles - 1) / s.tiles;
+    const int want = (s.self ? 4 : 2) * 148 / s.tiles;
     const int blocks = (int)((p.k + kBlockK - 1) / kBlockK), chunks = (int)((p.n + kChunkN - 1) / kChunkN);
     s.ksplit = want < blocks / 2 ? want : blocks / 2;
     if (s.ksplit > 16) s.ksplit = 16;
     if (s.ksplit < 1) s.ksplit = 1;
-    s.nsplit = 2 * want < chunks ? 2 * want : chunks;
+    s.nsplit = want < chunks ? want : chunks;
+    if (s.nsplit < 1) s.nsplit = 1;
     return s;
 }
 
@@ -734,11 +839,13 @@ cudaError_t launch_tiles(const AdapterParams &p, const Shape &s, cudaStream_t st
         e = launch_kernel(adapter_plan_kernel, dim3(1), kPlanThreads, (p.adapters + 1) * 4, stream, false, p, s.tile_tokens);
         if (e != cudaSuccess) return e;
     }
-    e = launch_kernel(adapter_shrink_kernel<T, I8, TN, SELF>, dim3((unsigned)s.tiles, (unsigned)s.ksplit), kShrinkThreads,
-                      shrink_smem(TN, s.rank_pad, I8), stream, !SELF, p);
+    const auto shrink = p.grain_x == 16 && p.grain_a == 16 ? adapter_shrink_kernel<T, I8, TN, SELF, true> : adapter_shrink_kernel<T, I8, TN, SELF, false>;
+    e = launch_kernel(shrink, dim3((unsigned)s.tiles, (unsigned)s.ksplit), kShrinkThreads, shrink_smem(TN, s.rank_pad, I8), stream, !SELF, p);
     if (e != cudaSuccess) return e;
-    return launch_kernel(adapter_expand_kernel<T, TN, SELF>, dim3((unsigned)s.tiles, (unsigned)s.nsplit), kExpandThreads,
-                         expand_smem(TN, s.rank_pad), stream, true, p);
+    const bool rows16 = p.grain_base == 16 && p.grain_out == 16 && p.n % 8 == 0;
+    const auto expand = rows16 && p.grain_b == 16 ? adapter_expand_kernel<T, TN, SELF, 16>
+                        : rows16 && p.grain_b == 8 ? adapter_expand_kernel<T, TN, SELF, 8> : adapter_expand_kernel<T, TN, SELF, 0>;
+    return launch_kernel(expand, dim3((unsigned)s.tiles, (unsigned)s.nsplit), kExpandThreads, expand_smem(TN, s.rank_pad), stream, true, p);
 }
 
 template <typename T, bool I8>
@@ -772,6 +879,7 @@ cudaError_t adapter_launch(const AdapterProblem &a, void *workspace, size_t work
     p.grain_a = grain_of(a.a, a.k * 2, 2);
     p.grain_b = grain_of(a.b, a.rank * 2, 2);
     p.grain_base = grain_of(a.base, a.ld_base * 2, 2);
+    p.grain_out = grain_of(a.out, a.ld_out * 2, 2);
     p.ksplit = s.ksplit; p.nsplit = s.nsplit;
     char *ws = static_cast<char *>(workspace);
     p.status = reinterpret_cast<int *>(ws);
