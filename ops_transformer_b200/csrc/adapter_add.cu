@@ -573,9 +573,25 @@ __global__ void __launch_bounds__(kExpandThreads) adapter_expand_kernel(const Ad
         if (p.out != p.base) {
             pdl_wait();
             const int n0 = c0 * kChunkN, width = min(c1 * kChunkN, p.n) - n0;
-            for (int r = 0; r < tile.count; ++r)
-                for (int c = tid; c < width; c += kExpandThreads)
-                    out[(long long)rows[r] * p.ld_out + n0 + c] = base[(long long)rows[r] * p.ld_base + n0 + c];
+            constexpr int V = GB ? 8 : 1, AHEAD = 4;     // elements a copy, copies in flight
+            using Copy = typename std::conditional<GB != 0, uint4, uint16_t>::type;
+            const int across = (width + V - 1) / V, total = across * tile.count;   // at most 64 rows of 65535
+            for (int i0 = tid; i0 < total; i0 += kExpandThreads * AHEAD) {
+                Copy v[AHEAD];
+                T *to[AHEAD];
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) {
+                    const int i = i0 + j * kExpandThreads, r = i / across, c = n0 + (i - r * across) * V;
+                    to[j] = nullptr;
+                    if (i < total) {
+                        v[j] = *reinterpret_cast<const Copy *>(base + (long long)rows[r] * p.ld_base + c);
+                        to[j] = out + (long long)rows[r] * p.ld_out + c;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j)
+                    if (to[j]) *reinterpret_cast<Copy *>(to[j]) = v[j];
+            }
         }
     } else if (tile.count > 0 && c0 < c1) {
         const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
