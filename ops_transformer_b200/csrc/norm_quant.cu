@@ -13,6 +13,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "gmm_common.h"
 
 namespace gmm {
@@ -38,141 +40,353 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// N elements at once: one load or store of N * sizeof(T) bytes, which p is aligned to.
-template <typename T, int N>
-struct alignas(sizeof(T) * N) Pack { T v[N]; };
-
-template <typename T, int N>
-__device__ __forceinline__ void load_floats(const void *base, long long at, float (&f)[N])
+// 16 bytes of T as floats, and back with one rounding each.
+template <typename T> __device__ __forceinline__ void unpack(const uint4 &u, float *f);
+template <> __device__ __forceinline__ void unpack<float>(const uint4 &u, float *f)
 {
-    const Pack<T, N> p = *reinterpret_cast<const Pack<T, N> *>(reinterpret_cast<const T *>(base) + at);
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = to_float<T>(p.v[i]);
+    f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
 }
-template <typename T, int N>
-__device__ __forceinline__ void store_floats(void *base, long long at, const float (&f)[N])
+template <> __device__ __forceinline__ void unpack<__half>(const uint4 &u, float *f)
 {
-    Pack<T, N> p;
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int i = 0; i < N; ++i) p.v[i] = from_float<T>(f[i]);
-    *reinterpret_cast<Pack<T, N> *>(reinterpret_cast<T *>(base) + at) = p;
+    for (int i = 0; i < 4; ++i) {
+        const float2 t = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        f[2 * i] = t.x; f[2 * i + 1] = t.y;
+    }
+}
+template <> __device__ __forceinline__ void unpack<__nv_bfloat16>(const uint4 &u, float *f)
+{
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+template <typename T> __device__ __forceinline__ uint4 pack(const float *f);
+template <> __device__ __forceinline__ uint4 pack<float>(const float *f)
+{
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+}
+template <> __device__ __forceinline__ uint4 pack<__half>(const float *f)
+{
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 t = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t *>(&t);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <> __device__ __forceinline__ uint4 pack<__nv_bfloat16>(const float *f)
+{
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t *>(&t);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Sum of `sum` and largest of `mag` (bits of magnitudes: as unsigned numbers they order like them, and a NaN is the largest of all,
-// so that it is not passed over) of the block, in every thread.
-template <int THREADS>
-__device__ __forceinline__ void block_reduce(float &sum, uint32_t &mag, float2 *red)
+// Largest magnitude; a NaN is larger than all numbers, so that it is not passed over.
+__device__ __forceinline__ float max_mag(float m, float v)
 {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(v)));
+    return r;
+}
+
+// Sum of `sum` and largest of `mag` over the block, in every thread; at most 32 warps.  The magnitudes are compared as unsigned
+// numbers, which order like them (NaN last).
+__device__ __forceinline__ void block_reduce(float &sum, float &mag, float2 *red)
+{
+    uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(mag) & 0x7fffffffu);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    mag = __reduce_max_sync(0xffffffffu, mag);
-    if (THREADS == 32) return;
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = make_float2(sum, __uint_as_float(mag));
-    __syncthreads();
-    constexpr int W = THREADS / 32;
-    const float2 v = red[(threadIdx.x & 31) % W];
-    sum = v.x;
-    mag = __float_as_uint(v.y);
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    if (warps > 1) {
+        if (lane == 0) red[threadIdx.x >> 5] = make_float2(sum, __uint_as_float(m));
+        __syncthreads();
+        const float2 v = lane < warps ? red[lane] : make_float2(0.0f, 0.0f);
+        sum = v.x;
+        m = __reduce_max_sync(0xffffffffu, __float_as_uint(v.y));
 #pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    mag = __reduce_max_sync(0xffffffffu, mag);
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+    mag = __uint_as_float(m);
 }
 
-// rint(u / step), 0 where there is no step to divide by.
-__device__ __forceinline__ int quantise(float u, float step)
+// How a row is divided by its step.  rcp: the correctly rounded reciprocal where the quotient can be formed with it, else 0.
+struct Quantiser {
+    float step, rcp;
+    __device__ __forceinline__ void set(float s)
+    {
+        step = s;
+        rcp = s > 1e-30f && s < 1e30f ? __frcp_rn(s) : 0.0f;
+    }
+    __device__ __forceinline__ uint32_t one(float u) const
+    {
+        if (!(step > 0.0f && step < __int_as_float(0x7f800000))) return 0u;
+        return (uint32_t)max(-127, min(127, __float2int_rn(__fdiv_rn(u, step))));
+    }
+    // rint(u / step) of two values, in the low bytes.  q = u * rcp, twice q += (u - q * step) * rcp: after the first correction q is a
+    // faithful rounding of the quotient, and with an exact residual and a correctly rounded reciprocal the second one yields the
+    // correctly rounded quotient (Markstein's theorem), at most 127 in magnitude.  Adding 1.5 * 2^23 rounds it to an integer, ties to
+    // even, in the low bits.
+    __device__ __forceinline__ void two(f32x2 u, uint32_t &a, uint32_t &b) const
+    {
+        const f32x2 r = pair2(rcp, rcp), ns = pair2(-step, -step);
+        f32x2 q = mul2(u, r);
+        q = fma2(fma2(q, ns, u), r, q);
+        q = fma2(fma2(q, ns, u), r, q);
+        q = fma2(q, pair2(1.0f, 1.0f), pair2(12582912.0f, 12582912.0f));
+        a = (uint32_t)q;
+        b = (uint32_t)(q >> 32);
+    }
+    __device__ __forceinline__ uint32_t four(const float *u) const
+    {
+        uint32_t a, b, c, d;
+        if (rcp != 0.0f) {
+            two(pair2(u[0], u[1]), a, b);
+            two(pair2(u[2], u[3]), c, d);
+        } else {
+            a = one(u[0]); b = one(u[1]); c = one(u[2]); d = one(u[3]);
+        }
+        return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+    }
+};
+
+__device__ __forceinline__ float rms_scale(float sum, const NormParams &p)
 {
-    if (!(step > 0.0f && step < __int_as_float(0x7f800000))) return 0;
-    return max(-127, min(127, __float2int_rn(__fdiv_rn(u, step))));
+    return __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, (float)p.h), p.eps)));
 }
 
-// One CTA per row.  A thread holds NCH packs of V elements, THREADS packs apart; REG: the row fits, else it is read again.
-template <typename T, typename G, int V, int NCH, int THREADS>
-__global__ void __launch_bounds__(THREADS) norm_quant_kernel(const NormParams p)
+// V elements from `at` on, which stands anywhere: 16-bit weights out of two aligned packs where these lie inside, else one by one.
+template <typename G, int V>
+__device__ __forceinline__ void load_anywhere(const G *g, int at, int h, float *f)
 {
-    __shared__ float2 red[THREADS / 32];
+    if (sizeof(G) == 2 && at >= 0) {
+        const int lo = at & ~7, shift = at & 7;
+        if (lo + 16 <= h) {
+            const uint4 a = __ldg(reinterpret_cast<const uint4 *>(g + lo)), b = __ldg(reinterpret_cast<const uint4 *>(g + lo + 8));
+            uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            if (shift & 4) { w[0] = w[2]; w[1] = w[3]; w[2] = w[4]; w[3] = w[5]; w[4] = w[6]; w[5] = w[7]; }
+            if (shift & 2) { w[0] = w[1]; w[1] = w[2]; w[2] = w[3]; w[3] = w[4]; w[4] = w[5]; }
+            const uint32_t bits = (shift & 1) * 16;
+            const uint4 u = make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                                       __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+            if (sizeof(G) == 2 && V == 8) unpack<G>(u, f);
+            return;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = at + e >= 0 && at + e < h ? to_float<G>(g[at + e]) : 0.0f;
+}
+template <int N>
+__device__ __forceinline__ void load_floats(const float *g, float *f)
+{
+#pragma unroll
+    for (int e = 0; e < N; e += 4) {
+        const float4 v = __ldg(reinterpret_cast<const float4 *>(g + e));
+        f[e] = v.x; f[e + 1] = v.y; f[e + 2] = v.z; f[e + 3] = v.w;
+    }
+}
+
+// One CTA per row; a thread holds NCH packs of 16 bytes, blockDim.x apart, as fp32 sums h between the reduction and the stores (rows
+// that do not fit are read again).  WHOLE: rows start on packs.  Else every row starts `lead` elements into one, the same in all tensors
+// (their rows are equally far apart, counted in elements modulo a pack), and only its first and last pack are handled one element at a
+// time.
+template <typename T, typename G, int NCH, bool WHOLE, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) norm_quant_kernel(const NormParams p)
+{
+    constexpr int V = 16 / (int)sizeof(T);
+    __shared__ float2 red[32];
     const long long row = blockIdx.x;
-    const int packs = p.h / V;
+    const int lead = WHOLE ? 0 : (int)((row * p.ld_x) & (V - 1));
+    const int packs = (lead + p.h + V - 1) / V, threads = blockDim.x;
+    const T *x = reinterpret_cast<const T *>(p.x) + row * p.ld_x - lead;
+    const T *residual = reinterpret_cast<const T *>(p.residual) + row * p.ld_residual - lead;
+    const G *gamma = reinterpret_cast<const G *>(p.gamma);
+    const auto full = [&](int c) { return WHOLE || (c * V >= lead && (c + 1) * V <= lead + p.h); };
+    const auto load_pack = [&](const T *from, int c) {
+        if (full(c)) return *reinterpret_cast<const uint4 *>(from + (long long)c * V);
+        float f[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = c * V + e >= lead && c * V + e < lead + p.h ? to_float<T>(from[c * V + e]) : 0.0f;
+        return pack<T>(f);   // exact: the values come from T
+    };
+    const auto load_h = [&](int c, float *h) {
+        const uint4 a = load_pack(x, c);
+        unpack<T>(a, h);
+        if (p.residual) {
+            float t[V];
+            unpack<T>(load_pack(residual, c), t);
+#pragma unroll
+            for (int e = 0; e < V; e += 2) {
+                const float2 s = unpair2(fma2(pair2(h[e], h[e + 1]), pair2(1.0f, 1.0f), pair2(t[e], t[e + 1])));
+                h[e] = s.x; h[e + 1] = s.y;
+            }
+        }
+    };
+    const auto load_gamma = [&](int c, float *g) {
+        if (!WHOLE) load_anywhere<G, V>(gamma, c * V - lead, p.h, g);
+        else if (sizeof(G) == 4) load_floats<V>(reinterpret_cast<const float *>(p.gamma) + c * V, g);
+        else unpack<typename std::conditional<sizeof(G) == 2, G, T>::type>(__ldg(reinterpret_cast<const uint4 *>(gamma + c * V)), g);
+    };
+    // u = h * gamma * smooth, over g
+    const auto weigh = [&](int c, const float *h, float *g) {
+#pragma unroll
+        for (int e = 0; e < V; e += 2) {
+            const float2 u = unpair2(mul2(pair2(h[e], h[e + 1]), pair2(g[e], g[e + 1])));
+            g[e] = u.x; g[e + 1] = u.y;
+        }
+    };
+    const auto smooth = [&](int c, float *u) {
+        float m[V];
+        if (WHOLE) load_floats<V>(p.smooth + c * V, m);
+        else load_anywhere<float, V>(p.smooth, c * V - lead, p.h, m);
+#pragma unroll
+        for (int e = 0; e < V; e += 2) {
+            const float2 t = unpair2(mul2(pair2(u[e], u[e + 1]), pair2(m[e], m[e + 1])));
+            u[e] = t.x; u[e + 1] = t.y;
+        }
+    };
     float h[NCH][V];
-    float sum = 0.0f;
-    uint32_t mag = 0;
-    for (int c0 = 0; c0 < packs; c0 += THREADS * NCH) {
+    f32x2 sum2 = 0;
+    float mag = 0.0f;
+    for (int c0 = threadIdx.x; c0 < packs; c0 += threads * NCH) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+            if (c0 + i * threads < packs) load_h(c0 + i * threads, h[i]);
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
-            const int c = c0 + i * THREADS + threadIdx.x;
+            const int c = c0 + i * threads;
             if (c >= packs) break;
-            load_floats<T, V>(p.x, row * p.ld_x + (long long)c * V, h[i]);
-            if (p.residual) {
-                float t[V];
-                load_floats<T, V>(p.residual, row * p.ld_residual + (long long)c * V, t);
+            float u[V];
+            load_gamma(c, u);
+            weigh(c, h[i], u);
+            if (p.smooth) smooth(c, u);
 #pragma unroll
-                for (int e = 0; e < V; ++e) h[i][e] = __fadd_rn(h[i][e], t[e]);
-            }
-            float g[V];
-            load_floats<G, V>(p.gamma, (long long)c * V, g);
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                float u = __fmul_rn(h[i][e], g[e]);
-                if (p.smooth) u = __fmul_rn(u, p.smooth[c * V + e]);
-                sum = __fmaf_rn(h[i][e], h[i][e], sum);
-                mag = max(mag, __float_as_uint(u) & 0x7fffffffu);
+            for (int e = 0; e < V; e += 2) {
+                const f32x2 v = pair2(h[i][e], h[i][e + 1]);
+                sum2 = fma2(v, v, sum2);
+                mag = max_mag(max_mag(mag, u[e]), u[e + 1]);
             }
         }
     }
-    block_reduce<THREADS>(sum, mag, red);
-    const float r = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, (float)p.h), p.eps)));
-    const float step = __fdiv_rn(__uint_as_float(mag), 127.0f);
+    const float2 parts = unpair2(sum2);
+    float sum = parts.x + parts.y;
+    block_reduce(sum, mag, red);
+    const float r = rms_scale(sum, p), step = __fdiv_rn(mag, 127.0f);
+    Quantiser quant;
+    quant.set(step);
     if (threadIdx.x == 0) p.scale[row] = step == 0.0f ? 0.0f : __fmul_rn(step, r);
-    const bool again = packs > THREADS * NCH;
-    for (int c0 = 0; c0 < packs; c0 += THREADS * NCH) {
+    T *residual_out = reinterpret_cast<T *>(p.residual_out) + row * p.ld_residual_out - lead;
+    T *normed_out = reinterpret_cast<T *>(p.normed_out) + row * p.ld_normed - lead;
+    int8_t *q_out = p.q + row * p.ld_q - lead;
+    const auto store_pack = [&](T *to, int c, const float *f) {
+        if (full(c)) {
+            *reinterpret_cast<uint4 *>(to + (long long)c * V) = pack<T>(f);
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (c * V + e >= lead && c * V + e < lead + p.h) to[c * V + e] = from_float<T>(f[e]);
+    };
+    const bool again = packs > threads * NCH;
+    for (int c0 = threadIdx.x; c0 < packs; c0 += threads * NCH) {
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
-            const int c = c0 + i * THREADS + threadIdx.x;
+            const int c = c0 + i * threads;
             if (c >= packs) break;
-            if (again) {
-                load_floats<T, V>(p.x, row * p.ld_x + (long long)c * V, h[i]);
-                if (p.residual) {
-                    float t[V];
-                    load_floats<T, V>(p.residual, row * p.ld_residual + (long long)c * V, t);
+            if (again) load_h(c, h[i]);
+            float u[V];
+            load_gamma(c, u);
+            weigh(c, h[i], u);
+            if (p.residual_out) store_pack(residual_out, c, h[i]);
+            if (p.normed_out) {
+                float y[V];
 #pragma unroll
-                    for (int e = 0; e < V; ++e) h[i][e] = __fadd_rn(h[i][e], t[e]);
+                for (int e = 0; e < V; e += 2) {
+                    const float2 t = unpair2(mul2(pair2(u[e], u[e + 1]), pair2(r, r)));
+                    y[e] = t.x; y[e + 1] = t.y;
                 }
+                store_pack(normed_out, c, y);
             }
-            float g[V], y[V];
-            Pack<int8_t, V> q;
-            load_floats<G, V>(p.gamma, (long long)c * V, g);
+            if (p.smooth) smooth(c, u);
+            uint32_t q[V / 4];
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                float u = __fmul_rn(h[i][e], g[e]);
-                y[e] = __fmul_rn(u, r);
-                if (p.smooth) u = __fmul_rn(u, p.smooth[c * V + e]);
-                q.v[e] = (int8_t)quantise(u, step);
+            for (int e = 0; e < V; e += 4) q[e / 4] = quant.four(u + e);
+            int8_t *to = q_out + (long long)c * V;
+            if (full(c)) {
+                if (V == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(q[0], q[V / 4 - 1]);
+                else *reinterpret_cast<uint32_t *>(to) = q[0];
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (c * V + e >= lead && c * V + e < lead + p.h) to[e] = (int8_t)(q[e / 4] >> (e % 4 * 8));
             }
-            *reinterpret_cast<Pack<int8_t, V> *>(p.q + row * p.ld_q + (long long)c * V) = q;
-            if (p.residual_out) store_floats<T, V>(p.residual_out, row * p.ld_residual_out + (long long)c * V, h[i]);
-            if (p.normed_out) store_floats<T, V>(p.normed_out, row * p.ld_normed + (long long)c * V, y);
         }
     }
 }
 
-template <typename T, typename G, int V>
-void launch_rows(const NormParams &p, cudaStream_t stream)
+// Any strides and addresses: one element at a time.
+template <typename T, typename G>
+__global__ void __launch_bounds__(256) norm_quant_any_kernel(const NormParams p)
 {
-    norm_quant_kernel<T, G, V, 4, 256><<<p.rows, 256, 0, stream>>>(p);
+    __shared__ float2 red[32];
+    const long long row = blockIdx.x;
+    const T *x = reinterpret_cast<const T *>(p.x) + row * p.ld_x, *residual = reinterpret_cast<const T *>(p.residual) + row * p.ld_residual;
+    const G *gamma = reinterpret_cast<const G *>(p.gamma);
+    const auto load = [&](int e) { return p.residual ? __fadd_rn(to_float<T>(x[e]), to_float<T>(residual[e])) : to_float<T>(x[e]); };
+    float sum = 0.0f, mag = 0.0f;
+    for (int e = threadIdx.x; e < p.h; e += 256) {
+        const float h = load(e);
+        float u = __fmul_rn(h, to_float<G>(gamma[e]));
+        if (p.smooth) u = __fmul_rn(u, p.smooth[e]);
+        sum = __fmaf_rn(h, h, sum);
+        mag = max_mag(mag, u);
+    }
+    block_reduce(sum, mag, red);
+    const float r = rms_scale(sum, p), step = __fdiv_rn(mag, 127.0f);
+    Quantiser quant;
+    quant.set(step);
+    if (threadIdx.x == 0) p.scale[row] = step == 0.0f ? 0.0f : __fmul_rn(step, r);
+    for (int e = threadIdx.x; e < p.h; e += 256) {
+        const float h = load(e);
+        float u = __fmul_rn(h, to_float<G>(gamma[e]));
+        if (p.residual_out) reinterpret_cast<T *>(p.residual_out)[row * p.ld_residual_out + e] = from_float<T>(h);
+        if (p.normed_out) reinterpret_cast<T *>(p.normed_out)[row * p.ld_normed + e] = from_float<T>(__fmul_rn(u, r));
+        if (p.smooth) u = __fmul_rn(u, p.smooth[e]);
+        p.q[row * p.ld_q + e] = (int8_t)quant.one(u);
+    }
+}
+
+template <typename T, typename G, bool WHOLE>
+void launch_packed(const NormParams &p, cudaStream_t stream)
+{
+    constexpr int V = 16 / (int)sizeof(T);
+    const int packs = (p.h + (WHOLE ? 0 : V - 1) + V - 1) / V;
+    const auto warps = [](int n) { return (n + 31) / 32 * 32; };
+    // Few rows: as many threads as a row has packs, for the shortest chain.  More: four packs a thread, for more rows on an SM.
+    if (packs <= 1024 && (p.rows <= 2 * 148 || packs <= 64)) norm_quant_kernel<T, G, 1, WHOLE, 1024, 1><<<p.rows, warps(packs), 0, stream>>>(p);
+    else if (packs <= 4 * 256) norm_quant_kernel<T, G, 4, WHOLE, 256, 3><<<p.rows, warps((packs + 3) / 4), 0, stream>>>(p);
+    else norm_quant_kernel<T, G, 4, WHOLE, 1024, 1><<<p.rows, packs >= 4096 ? 1024 : warps((packs + 3) / 4), 0, stream>>>(p);
 }
 
 template <typename T, typename G>
 void launch_typed(const NormParams &p, cudaStream_t stream)
 {
     constexpr int V = 16 / (int)sizeof(T);
-    // 16 bytes of T and V bytes of q at a time, where every row of every tensor starts on such a boundary
-    const auto fits = [](const void *base, long long ld, int bytes, int align) {
-        return !base || (((uintptr_t)base | (uintptr_t)(ld * bytes)) & (uintptr_t)(align - 1)) == 0;
+    // Packs need every tensor to begin on one (V elements of its own type) and its rows to be as far apart as x's, modulo a pack.
+    const auto fits = [&](const void *base, long long ld, int bytes) {
+        return !base || (((uintptr_t)base & (uintptr_t)(V * bytes < 16 ? V * bytes - 1 : 15)) == 0 && (ld - p.ld_x) % V == 0);
     };
-    const bool wide = p.h % V == 0 && fits(p.x, p.ld_x, sizeof(T), 16) && fits(p.residual, p.ld_residual, sizeof(T), 16) &&
-                      fits(p.residual_out, p.ld_residual_out, sizeof(T), 16) && fits(p.normed_out, p.ld_normed, sizeof(T), 16) &&
-                      fits(p.gamma, 0, 0, V * (int)sizeof(G)) && fits(p.smooth, 0, 0, 16) && fits(p.q, p.ld_q, 1, V);
-    if (wide) launch_rows<T, G, V>(p, stream);
-    else launch_rows<T, G, 1>(p, stream);
+    const bool packed = fits(p.x, p.ld_x, sizeof(T)) && fits(p.residual, p.ld_residual, sizeof(T)) && fits(p.residual_out, p.ld_residual_out, sizeof(T)) &&
+                        fits(p.normed_out, p.ld_normed, sizeof(T)) && fits(p.q, p.ld_q, 1) && fits(p.gamma, p.ld_x, sizeof(G)) &&
+                        fits(p.smooth, p.ld_x, 4);
+    if (!packed) norm_quant_any_kernel<T, G><<<p.rows, 256, 0, stream>>>(p);
+    else if (p.h % V == 0 && p.ld_x % V == 0) launch_packed<T, G, true>(p, stream);
+    else launch_packed<T, G, false>(p, stream);
 }
 
 }  // namespace
