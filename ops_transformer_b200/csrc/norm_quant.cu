@@ -28,7 +28,7 @@ struct NormParams {
     void *residual_out, *normed_out;
     long long ld_x, ld_residual, ld_q, ld_residual_out, ld_normed;
     int rows, h;
-    float eps;
+    float inv_h, eps;
 };
 
 template <typename T> __device__ __forceinline__ float to_float(T v);
@@ -87,11 +87,11 @@ template <> __device__ __forceinline__ uint4 pack<__nv_bfloat16>(const float *f)
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Largest magnitude; a NaN is larger than all numbers, so that it is not passed over.
-__device__ __forceinline__ float max_mag(float m, float v)
+// Largest magnitude of three; a NaN is larger than all numbers, so that it is not passed over.
+__device__ __forceinline__ float max_mag(float m, float a, float b)
 {
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(v)));
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(a), "f"(b));
     return r;
 }
 
@@ -155,9 +155,16 @@ struct Quantiser {
     }
 };
 
-__device__ __forceinline__ float rms_scale(float sum, const NormParams &p)
+__device__ __forceinline__ float rms_scale(float sum, const NormParams &p) { return rsqrtf(__fmaf_rn(sum, p.inv_h, p.eps)); }
+
+// m / 127, correctly rounded as in Quantiser::two; the rest of the range by division.
+__device__ __forceinline__ float step_of(float m)
 {
-    return __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, (float)p.h), p.eps)));
+    if (!(m > 1e-28f && m < 1e30f)) return __fdiv_rn(m, 127.0f);
+    const float r = 1.0f / 127.0f;
+    float q = __fmul_rn(m, r);
+    q = __fmaf_rn(__fmaf_rn(-q, 127.0f, m), r, q);
+    return __fmaf_rn(__fmaf_rn(-q, 127.0f, m), r, q);
 }
 
 // V elements from `at` on, which stands anywhere: 16-bit weights out of two aligned packs where these lie inside, else one by one.
@@ -195,17 +202,40 @@ __device__ __forceinline__ void load_floats(const float *g, float *f)
 // that do not fit are read again).  WHOLE: rows start on packs.  Else every row starts `lead` elements into one, the same in all tensors
 // (their rows are equally far apart, counted in elements modulo a pack), and only its first and last pack are handled one element at a
 // time.
-template <typename T, typename G, int NCH, bool WHOLE, int MAXT, int MINB>
+//
+// STREAM: the CTA takes every gridDim.x-th row (which fits).  While it works on one, the packs of the next are copied to shared memory,
+// each by the thread that will read it, so nothing but the thread's own copies is waited for and loads are under way all the time.
+template <typename T, typename G, int NCH, bool WHOLE, int MAXT, int MINB, bool STREAM>
 __global__ void __launch_bounds__(MAXT, MINB) norm_quant_kernel(const NormParams p)
 {
     constexpr int V = 16 / (int)sizeof(T);
-    __shared__ float2 red[32];
-    const long long row = blockIdx.x;
-    const int lead = WHOLE ? 0 : (int)((row * p.ld_x) & (V - 1));
-    const int packs = (lead + p.h + V - 1) / V, threads = blockDim.x;
+    extern __shared__ uint4 ahead[];   // STREAM: [2][NCH][threads]
+    __shared__ float2 red[2][32];
+    const int threads = blockDim.x;
+    const G *gamma = reinterpret_cast<const G *>(p.gamma);
+    const uint32_t mine = STREAM ? (uint32_t)__cvta_generic_to_shared(ahead) + threadIdx.x * 16 : 0;
+    const auto lead_of = [&](long long row) { return WHOLE ? 0 : (int)((row * p.ld_x) & (V - 1)); };
+    const auto fetch = [&](long long row) {
+        const int lead = lead_of(row);
+        const T *x = reinterpret_cast<const T *>(p.x) + row * p.ld_x - lead, *res = reinterpret_cast<const T *>(p.residual) + row * p.ld_residual - lead;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int c = threadIdx.x + i * threads;
+            if ((c + 1) * V <= lead + p.h && c * V >= lead) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine + i * threads * 16), "l"(x + (long long)c * V) : "memory");
+                if (p.residual)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine + (NCH + i) * threads * 16), "l"(res + (long long)c * V) : "memory");
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if (STREAM) fetch(blockIdx.x);
+    int parity = 0;
+    for (long long row = blockIdx.x; row < p.rows; row += STREAM ? (long long)gridDim.x : (long long)p.rows) {
+    const int lead = lead_of(row);
+    const int packs = (lead + p.h + V - 1) / V;
     const T *x = reinterpret_cast<const T *>(p.x) + row * p.ld_x - lead;
     const T *residual = reinterpret_cast<const T *>(p.residual) + row * p.ld_residual - lead;
-    const G *gamma = reinterpret_cast<const G *>(p.gamma);
     const auto full = [&](int c) { return WHOLE || (c * V >= lead && (c + 1) * V <= lead + p.h); };
     const auto load_pack = [&](const T *from, int c) {
         if (full(c)) return *reinterpret_cast<const uint4 *>(from + (long long)c * V);
@@ -214,12 +244,17 @@ __global__ void __launch_bounds__(MAXT, MINB) norm_quant_kernel(const NormParams
         for (int e = 0; e < V; ++e) f[e] = c * V + e >= lead && c * V + e < lead + p.h ? to_float<T>(from[c * V + e]) : 0.0f;
         return pack<T>(f);   // exact: the values come from T
     };
-    const auto load_h = [&](int c, float *h) {
-        const uint4 a = load_pack(x, c);
-        unpack<T>(a, h);
+    const auto load_h = [&](int c, int i, float *h) {
+        const auto get = [&](const T *from, int at) {
+            if (!STREAM || !full(c)) return load_pack(from, c);
+            uint4 u;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(mine + at * threads * 16) : "memory");
+            return u;
+        };
+        unpack<T>(get(x, i), h);
         if (p.residual) {
             float t[V];
-            unpack<T>(load_pack(residual, c), t);
+            unpack<T>(get(residual, NCH + i), t);
 #pragma unroll
             for (int e = 0; e < V; e += 2) {
                 const float2 s = unpair2(fma2(pair2(h[e], h[e + 1]), pair2(1.0f, 1.0f), pair2(t[e], t[e + 1])));
@@ -227,17 +262,16 @@ __global__ void __launch_bounds__(MAXT, MINB) norm_quant_kernel(const NormParams
             }
         }
     };
-    const auto load_gamma = [&](int c, float *g) {
+    // h * gamma in the place of h
+    const auto weigh = [&](int c, float *h) {
+        float g[V];
         if (!WHOLE) load_anywhere<G, V>(gamma, c * V - lead, p.h, g);
         else if (sizeof(G) == 4) load_floats<V>(reinterpret_cast<const float *>(p.gamma) + c * V, g);
         else unpack<typename std::conditional<sizeof(G) == 2, G, T>::type>(__ldg(reinterpret_cast<const uint4 *>(gamma + c * V)), g);
-    };
-    // u = h * gamma * smooth, over g
-    const auto weigh = [&](int c, const float *h, float *g) {
 #pragma unroll
         for (int e = 0; e < V; e += 2) {
             const float2 u = unpair2(mul2(pair2(h[e], h[e + 1]), pair2(g[e], g[e + 1])));
-            g[e] = u.x; g[e + 1] = u.y;
+            h[e] = u.x; h[e + 1] = u.y;
         }
     };
     const auto smooth = [&](int c, float *u) {
@@ -250,36 +284,7 @@ __global__ void __launch_bounds__(MAXT, MINB) norm_quant_kernel(const NormParams
             u[e] = t.x; u[e + 1] = t.y;
         }
     };
-    float h[NCH][V];
-    f32x2 sum2 = 0;
-    float mag = 0.0f;
-    for (int c0 = threadIdx.x; c0 < packs; c0 += threads * NCH) {
-#pragma unroll
-        for (int i = 0; i < NCH; ++i)
-            if (c0 + i * threads < packs) load_h(c0 + i * threads, h[i]);
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int c = c0 + i * threads;
-            if (c >= packs) break;
-            float u[V];
-            load_gamma(c, u);
-            weigh(c, h[i], u);
-            if (p.smooth) smooth(c, u);
-#pragma unroll
-            for (int e = 0; e < V; e += 2) {
-                const f32x2 v = pair2(h[i][e], h[i][e + 1]);
-                sum2 = fma2(v, v, sum2);
-                mag = max_mag(max_mag(mag, u[e]), u[e + 1]);
-            }
-        }
-    }
-    const float2 parts = unpair2(sum2);
-    float sum = parts.x + parts.y;
-    block_reduce(sum, mag, red);
-    const float r = rms_scale(sum, p), step = __fdiv_rn(mag, 127.0f);
-    Quantiser quant;
-    quant.set(step);
-    if (threadIdx.x == 0) p.scale[row] = step == 0.0f ? 0.0f : __fmul_rn(step, r);
+    const bool again = !STREAM && packs > threads * NCH;
     T *residual_out = reinterpret_cast<T *>(p.residual_out) + row * p.ld_residual_out - lead;
     T *normed_out = reinterpret_cast<T *>(p.normed_out) + row * p.ld_normed - lead;
     int8_t *q_out = p.q + row * p.ld_q - lead;
@@ -292,30 +297,66 @@ __global__ void __launch_bounds__(MAXT, MINB) norm_quant_kernel(const NormParams
         for (int e = 0; e < V; ++e)
             if (c * V + e >= lead && c * V + e < lead + p.h) to[c * V + e] = from_float<T>(f[e]);
     };
-    const bool again = packs > threads * NCH;
+    float u[NCH][V];
+    f32x2 sum2 = 0;
+    float mag = 0.0f;
+    if (STREAM) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    for (int c0 = threadIdx.x; c0 < packs; c0 += threads * NCH) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+            if (c0 + i * threads < packs) load_h(c0 + i * threads, i, u[i]);
+        if (STREAM && row + gridDim.x < p.rows) fetch(row + gridDim.x);   // the thread has read what this fills
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int c = c0 + i * threads;
+            if (c >= packs) break;
+#pragma unroll
+            for (int e = 0; e < V; e += 2) {
+                const f32x2 v = pair2(u[i][e], u[i][e + 1]);
+                sum2 = fma2(v, v, sum2);
+            }
+            // a row that is read again keeps its inputs, which residual_out may be, until then
+            if (p.residual_out && !again) store_pack(residual_out, c, u[i]);
+            weigh(c, u[i]);
+            float m[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) m[e] = u[i][e];
+            if (p.smooth) smooth(c, m);
+#pragma unroll
+            for (int e = 0; e < V; e += 2) mag = max_mag(mag, m[e], m[e + 1]);
+        }
+    }
+    const float2 parts = unpair2(sum2);
+    float sum = parts.x + parts.y;
+    block_reduce(sum, mag, red[parity]);
+    parity ^= 1;
+    const float r = rms_scale(sum, p), step = step_of(mag);
+    Quantiser quant;
+    quant.set(step);
+    if (threadIdx.x == 0) p.scale[row] = step == 0.0f ? 0.0f : __fmul_rn(step, r);
     for (int c0 = threadIdx.x; c0 < packs; c0 += threads * NCH) {
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             const int c = c0 + i * threads;
             if (c >= packs) break;
-            if (again) load_h(c, h[i]);
-            float u[V];
-            load_gamma(c, u);
-            weigh(c, h[i], u);
-            if (p.residual_out) store_pack(residual_out, c, h[i]);
+            if (again) {
+                load_h(c, i, u[i]);
+                if (p.residual_out) store_pack(residual_out, c, u[i]);
+                weigh(c, u[i]);
+            }
             if (p.normed_out) {
                 float y[V];
 #pragma unroll
                 for (int e = 0; e < V; e += 2) {
-                    const float2 t = unpair2(mul2(pair2(u[e], u[e + 1]), pair2(r, r)));
+                    const float2 t = unpair2(mul2(pair2(u[i][e], u[i][e + 1]), pair2(r, r)));
                     y[e] = t.x; y[e + 1] = t.y;
                 }
                 store_pack(normed_out, c, y);
             }
-            if (p.smooth) smooth(c, u);
+            if (p.smooth) smooth(c, u[i]);
             uint32_t q[V / 4];
 #pragma unroll
-            for (int e = 0; e < V; e += 4) q[e / 4] = quant.four(u + e);
+            for (int e = 0; e < V; e += 4) q[e / 4] = quant.four(u[i] + e);
             int8_t *to = q_out + (long long)c * V;
             if (full(c)) {
                 if (V == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(q[0], q[V / 4 - 1]);
@@ -326,6 +367,7 @@ __global__ void __launch_bounds__(MAXT, MINB) norm_quant_kernel(const NormParams
                     if (c * V + e >= lead && c * V + e < lead + p.h) to[e] = (int8_t)(q[e / 4] >> (e % 4 * 8));
             }
         }
+    }
     }
 }
 
@@ -344,10 +386,10 @@ __global__ void __launch_bounds__(256) norm_quant_any_kernel(const NormParams p)
         float u = __fmul_rn(h, to_float<G>(gamma[e]));
         if (p.smooth) u = __fmul_rn(u, p.smooth[e]);
         sum = __fmaf_rn(h, h, sum);
-        mag = max_mag(mag, u);
+        mag = max_mag(mag, u, u);
     }
     block_reduce(sum, mag, red);
-    const float r = rms_scale(sum, p), step = __fdiv_rn(mag, 127.0f);
+    const float r = rms_scale(sum, p), step = step_of(mag);
     Quantiser quant;
     quant.set(step);
     if (threadIdx.x == 0) p.scale[row] = step == 0.0f ? 0.0f : __fmul_rn(step, r);
@@ -367,10 +409,16 @@ void launch_packed(const NormParams &p, cudaStream_t stream)
     constexpr int V = 16 / (int)sizeof(T);
     const int packs = (p.h + (WHOLE ? 0 : V - 1) + V - 1) / V;
     const auto warps = [](int n) { return (n + 31) / 32 * 32; };
-    // Few rows: as many threads as a row has packs, for the shortest chain.  More: four packs a thread, for more rows on an SM.
-    if (packs <= 1024 && (p.rows <= 2 * 148 || packs <= 64)) norm_quant_kernel<T, G, 1, WHOLE, 1024, 1><<<p.rows, warps(packs), 0, stream>>>(p);
-    else if (packs <= 4 * 256) norm_quant_kernel<T, G, 4, WHOLE, 256, 3><<<p.rows, warps((packs + 3) / 4), 0, stream>>>(p);
-    else norm_quant_kernel<T, G, 4, WHOLE, 1024, 1><<<p.rows, packs >= 4096 ? 1024 : warps((packs + 3) / 4), 0, stream>>>(p);
+    // Few rows: as many threads as a row has packs, for the shortest chain.  More: four packs a thread, for more rows on an SM; from
+    // more rows than find a place on the SMs together on, the CTAs go through them with the next row's loads under way.
+    const int four = warps((packs + 3) / 4), smem = 2 * 4 * 16 * four;
+    const int fit = 1024 / four < 200 * 1024 / (smem + 1024) ? 1024 / four : 200 * 1024 / (smem + 1024), places = 148 * fit;
+    if (packs <= 4 * 256 && p.rows > places) {
+        const auto kernel = norm_quant_kernel<T, G, 4, WHOLE, 256, 3, true>;
+        kernel<<<places, four, smem, stream>>>(p);
+    } else if (packs <= 1024 && (p.rows <= 2 * 148 || packs <= 64)) norm_quant_kernel<T, G, 1, WHOLE, 1024, 1, false><<<p.rows, warps(packs), 0, stream>>>(p);
+    else if (packs <= 4 * 256) norm_quant_kernel<T, G, 4, WHOLE, 256, 3, false><<<p.rows, four, 0, stream>>>(p);
+    else norm_quant_kernel<T, G, 4, WHOLE, 1024, 1, false><<<p.rows, packs >= 4096 ? 1024 : four, 0, stream>>>(p);
 }
 
 template <typename T, typename G>
@@ -398,7 +446,7 @@ cudaError_t norm_quant_launch(const NormQuantProblem &n, cudaStream_t stream)
     p.x = n.x; p.residual = n.residual; p.gamma = n.gamma; p.smooth = n.smooth;
     p.q = n.q; p.scale = n.scale; p.residual_out = n.residual_out; p.normed_out = n.normed_out;
     p.ld_x = n.ld_x; p.ld_residual = n.ld_residual; p.ld_q = n.ld_q; p.ld_residual_out = n.ld_residual_out; p.ld_normed = n.ld_normed;
-    p.rows = (int)n.rows; p.h = (int)n.h; p.eps = n.eps;
+    p.rows = (int)n.rows; p.h = (int)n.h; p.inv_h = 1.0f / (float)n.h; p.eps = n.eps;
     const bool g32 = n.gamma_dtype == kF32;
     switch (n.dtype) {
         case kF32: launch_typed<float, float>(p, stream); break;
