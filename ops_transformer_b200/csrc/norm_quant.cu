@@ -40,51 +40,61 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// 16 bytes of T as floats, and back with one rounding each.
-template <typename T> __device__ __forceinline__ void unpack(const uint4 &u, float *f);
-template <> __device__ __forceinline__ void unpack<float>(const uint4 &u, float *f)
+// 16 bytes of T as pairs of floats, and back with one rounding each.  Values stay in pairs throughout: taken apart and put together
+// again, they cost as many register moves as arithmetic.
+template <typename T> __device__ __forceinline__ void unpack(const uint4 &u, f32x2 *f);
+template <> __device__ __forceinline__ void unpack<float>(const uint4 &u, f32x2 *f)
 {
-    f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+    f[0] = pair2(__uint_as_float(u.x), __uint_as_float(u.y));
+    f[1] = pair2(__uint_as_float(u.z), __uint_as_float(u.w));
 }
-template <> __device__ __forceinline__ void unpack<__half>(const uint4 &u, float *f)
+template <> __device__ __forceinline__ void unpack<__half>(const uint4 &u, f32x2 *f)
 {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 t = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-        f[2 * i] = t.x; f[2 * i + 1] = t.y;
+        f[i] = pair2(t.x, t.y);
     }
 }
-template <> __device__ __forceinline__ void unpack<__nv_bfloat16>(const uint4 &u, float *f)
+template <> __device__ __forceinline__ void unpack<__nv_bfloat16>(const uint4 &u, f32x2 *f)
 {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    for (int i = 0; i < 4; ++i) f[i] = pair2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
 }
-template <typename T> __device__ __forceinline__ uint4 pack(const float *f);
-template <> __device__ __forceinline__ uint4 pack<float>(const float *f)
+template <typename T> __device__ __forceinline__ uint4 pack(const f32x2 *f);
+template <> __device__ __forceinline__ uint4 pack<float>(const f32x2 *f)
 {
-    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    const float2 a = unpair2(f[0]), b = unpair2(f[1]);
+    return make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
 }
-template <> __device__ __forceinline__ uint4 pack<__half>(const float *f)
-{
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __half2 t = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t *>(&t);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-template <> __device__ __forceinline__ uint4 pack<__nv_bfloat16>(const float *f)
+template <> __device__ __forceinline__ uint4 pack<__half>(const f32x2 *f)
 {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 t = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        const float2 v = unpair2(f[i]);
+        const __half2 t = __floats2half2_rn(v.x, v.y);
         w[i] = *reinterpret_cast<const uint32_t *>(&t);
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <> __device__ __forceinline__ uint4 pack<__nv_bfloat16>(const f32x2 *f)
+{
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 v = unpair2(f[i]);
+        const __nv_bfloat162 t = __floats2bfloat162_rn(v.x, v.y);
+        w[i] = *reinterpret_cast<const uint32_t *>(&t);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ float element(const f32x2 *f, int e)
+{
+    const float2 v = unpair2(f[e / 2]);
+    return e % 2 ? v.y : v.x;
 }
 
 // Largest magnitude of three; a NaN is larger than all numbers, so that it is not passed over.
@@ -132,26 +142,22 @@ struct Quantiser {
     // faithful rounding of the quotient, and with an exact residual and a correctly rounded reciprocal the second one yields the
     // correctly rounded quotient (Markstein's theorem), at most 127 in magnitude.  Adding 1.5 * 2^23 rounds it to an integer, ties to
     // even, in the low bits.
-    __device__ __forceinline__ void two(f32x2 u, uint32_t &a, uint32_t &b) const
+    __device__ __forceinline__ f32x2 two(f32x2 u) const
     {
         const f32x2 r = pair2(rcp, rcp), ns = pair2(-step, -step);
         f32x2 q = mul2(u, r);
         q = fma2(fma2(q, ns, u), r, q);
         q = fma2(fma2(q, ns, u), r, q);
-        q = fma2(q, pair2(1.0f, 1.0f), pair2(12582912.0f, 12582912.0f));
-        a = (uint32_t)q;
-        b = (uint32_t)(q >> 32);
+        return fma2(q, pair2(1.0f, 1.0f), pair2(12582912.0f, 12582912.0f));
     }
-    __device__ __forceinline__ uint32_t four(const float *u) const
+    __device__ __forceinline__ uint32_t four(const f32x2 *u, bool by_rcp) const
     {
-        uint32_t a, b, c, d;
-        if (rcp != 0.0f) {
-            two(pair2(u[0], u[1]), a, b);
-            two(pair2(u[2], u[3]), c, d);
-        } else {
-            a = one(u[0]); b = one(u[1]); c = one(u[2]); d = one(u[3]);
+        if (by_rcp) {
+            const f32x2 a = two(u[0]), b = two(u[1]);
+            return __byte_perm(__byte_perm((uint32_t)a, (uint32_t)(a >> 32), 0x0040), __byte_perm((uint32_t)b, (uint32_t)(b >> 32), 0x0040), 0x5410);
         }
-        return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+        return __byte_perm(__byte_perm(one(element(u, 0)), one(element(u, 1)), 0x0040),
+                           __byte_perm(one(element(u, 2)), one(element(u, 3)), 0x0040), 0x5410);
     }
 };
 
@@ -169,39 +175,39 @@ __device__ __forceinline__ float step_of(float m)
 
 // V elements from `at` on, which stands anywhere: 16-bit weights out of two aligned packs where these lie inside, else one by one.
 template <typename G, int V>
-__device__ __forceinline__ void load_anywhere(const G *g, int at, int h, float *f)
+__device__ __forceinline__ void load_anywhere(const G *g, int at, int h, f32x2 *f)
 {
-    if (sizeof(G) == 2 && at >= 0) {
+    if constexpr (sizeof(G) == 2 && V == 8) {
         const int lo = at & ~7, shift = at & 7;
-        if (lo + 16 <= h) {
+        if (at >= 0 && lo + 16 <= h) {
             const uint4 a = __ldg(reinterpret_cast<const uint4 *>(g + lo)), b = __ldg(reinterpret_cast<const uint4 *>(g + lo + 8));
             uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
             if (shift & 4) { w[0] = w[2]; w[1] = w[3]; w[2] = w[4]; w[3] = w[5]; w[4] = w[6]; w[5] = w[7]; }
             if (shift & 2) { w[0] = w[1]; w[1] = w[2]; w[2] = w[3]; w[3] = w[4]; w[4] = w[5]; }
             const uint32_t bits = (shift & 1) * 16;
-            const uint4 u = make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
-                                       __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
-            if (sizeof(G) == 2 && V == 8) unpack<G>(u, f);
+            unpack<G>(make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                                 __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits)), f);
             return;
         }
     }
+    const auto one = [&](int e) { return e >= 0 && e < h ? to_float<G>(g[e]) : 0.0f; };
 #pragma unroll
-    for (int e = 0; e < V; ++e) f[e] = at + e >= 0 && at + e < h ? to_float<G>(g[at + e]) : 0.0f;
+    for (int e = 0; e < V; e += 2) f[e / 2] = pair2(one(at + e), one(at + e + 1));
 }
-template <int N>
-__device__ __forceinline__ void load_floats(const float *g, float *f)
+template <int V>
+__device__ __forceinline__ void load_fp32(const float *g, f32x2 *f)
 {
 #pragma unroll
-    for (int e = 0; e < N; e += 4) {
+    for (int e = 0; e < V; e += 4) {
         const float4 v = __ldg(reinterpret_cast<const float4 *>(g + e));
-        f[e] = v.x; f[e + 1] = v.y; f[e + 2] = v.z; f[e + 3] = v.w;
+        f[e / 2] = pair2(v.x, v.y);
+        f[e / 2 + 1] = pair2(v.z, v.w);
     }
 }
 
-// One CTA per row; a thread holds NCH packs of 16 bytes, blockDim.x apart, as fp32 sums h between the reduction and the stores (rows
-// that do not fit are read again).  WHOLE: rows start on packs.  Else every row starts `lead` elements into one, the same in all tensors
-// (their rows are equally far apart, counted in elements modulo a pack), and only its first and last pack are handled one element at a
-// time.
+// One CTA per row; a thread holds NCH packs of 16 bytes, blockDim.x apart, in fp32 between the reduction and the stores (rows that do
+// not fit are read again).  WHOLE: rows start on packs.  Else every row starts `lead` elements into one, the same in all tensors (their
+// rows are equally far apart, counted in elements modulo a pack), and only the stores of its first and last pack go one element at a time.
 //
 // STREAM: the CTA takes every gridDim.x-th row (which fits).  While it works on one, the packs of the next are copied to shared memory,
 // each by the thread that will read it, so nothing but the thread's own copies is waited for and loads are under way all the time.
@@ -215,13 +221,19 @@ __global__ void __launch_bounds__(MAXT, MINB) norm_quant_kernel(const NormParams
     const G *gamma = reinterpret_cast<const G *>(p.gamma);
     const uint32_t mine = STREAM ? (uint32_t)__cvta_generic_to_shared(ahead) + threadIdx.x * 16 : 0;
     const auto lead_of = [&](long long row) { return WHOLE ? 0 : (int)((row * p.ld_x) & (V - 1)); };
+    // Elements from the row's first pack on that lie inside x and residual: a row's first and last pack hold elements of its neighbours
+    // (or what is between the rows), which are read with it and dropped, but behind the tensor's end there may be nothing to read.
+    const auto room_of = [&](long long row, int lead) {
+        const long long behind = (p.rows - 1 - row) * (p.residual ? min(p.ld_x, p.ld_residual) : p.ld_x);
+        return lead + p.h + (int)min(behind, 1024ll);
+    };
     const auto fetch = [&](long long row) {
-        const int lead = lead_of(row);
+        const int lead = lead_of(row), room = room_of(row, lead);
         const T *x = reinterpret_cast<const T *>(p.x) + row * p.ld_x - lead, *res = reinterpret_cast<const T *>(p.residual) + row * p.ld_residual - lead;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             const int c = threadIdx.x + i * threads;
-            if ((c + 1) * V <= lead + p.h && c * V >= lead) {
+            if (WHOLE ? c * V < p.h : c * V < lead + p.h && (c + 1) * V <= room) {
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine + i * threads * 16), "l"(x + (long long)c * V) : "memory");
                 if (p.residual)
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine + (NCH + i) * threads * 16), "l"(res + (long long)c * V) : "memory");
@@ -232,142 +244,142 @@ __global__ void __launch_bounds__(MAXT, MINB) norm_quant_kernel(const NormParams
     if (STREAM) fetch(blockIdx.x);
     int parity = 0;
     for (long long row = blockIdx.x; row < p.rows; row += STREAM ? (long long)gridDim.x : (long long)p.rows) {
-    const int lead = lead_of(row);
-    const int packs = (lead + p.h + V - 1) / V;
-    const T *x = reinterpret_cast<const T *>(p.x) + row * p.ld_x - lead;
-    const T *residual = reinterpret_cast<const T *>(p.residual) + row * p.ld_residual - lead;
-    const auto full = [&](int c) { return WHOLE || (c * V >= lead && (c + 1) * V <= lead + p.h); };
-    const auto load_pack = [&](const T *from, int c) {
-        if (full(c)) return *reinterpret_cast<const uint4 *>(from + (long long)c * V);
-        float f[V];
+        const int lead = lead_of(row), end = lead + p.h, room = room_of(row, lead);
+        const int packs = (end + V - 1) / V;
+        const bool again = !STREAM && packs > threads * NCH;
+        const T *x = reinterpret_cast<const T *>(p.x) + row * p.ld_x - lead;
+        const T *residual = reinterpret_cast<const T *>(p.residual) + row * p.ld_residual - lead;
+        T *residual_out = reinterpret_cast<T *>(p.residual_out) + row * p.ld_residual_out - lead;
+        T *normed_out = reinterpret_cast<T *>(p.normed_out) + row * p.ld_normed - lead;
+        int8_t *q_out = p.q + row * p.ld_q - lead;
+        const auto full = [&](int c) { return WHOLE || (c * V >= lead && (c + 1) * V <= end); };
+        const auto get = [&](const T *from, int c, int at) {
+            if (!WHOLE && (c + 1) * V > room) {
+                const auto one = [&](int e) { return c * V + e >= lead && c * V + e < end ? to_float<T>(from[c * V + e]) : 0.0f; };
+                f32x2 f[V / 2];
 #pragma unroll
-        for (int e = 0; e < V; ++e) f[e] = c * V + e >= lead && c * V + e < lead + p.h ? to_float<T>(from[c * V + e]) : 0.0f;
-        return pack<T>(f);   // exact: the values come from T
-    };
-    const auto load_h = [&](int c, int i, float *h) {
-        const auto get = [&](const T *from, int at) {
-            if (!STREAM || !full(c)) return load_pack(from, c);
+                for (int e = 0; e < V; e += 2) f[e / 2] = pair2(one(e), one(e + 1));
+                return pack<T>(f);   // exact: the values come from T
+            }
             uint4 u;
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(mine + at * threads * 16) : "memory");
+            if (STREAM) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(mine + at * threads * 16) : "memory");
+            else u = *reinterpret_cast<const uint4 *>(from + (long long)c * V);
             return u;
         };
-        unpack<T>(get(x, i), h);
-        if (p.residual) {
-            float t[V];
-            unpack<T>(get(residual, NCH + i), t);
+        const auto load_h = [&](int c, int i, f32x2 *h) {
+            unpack<T>(get(x, c, i), h);
+            if (p.residual) {
+                f32x2 t[V / 2];
+                unpack<T>(get(residual, c, NCH + i), t);
 #pragma unroll
-            for (int e = 0; e < V; e += 2) {
-                const float2 s = unpair2(fma2(pair2(h[e], h[e + 1]), pair2(1.0f, 1.0f), pair2(t[e], t[e + 1])));
-                h[e] = s.x; h[e + 1] = s.y;
+                for (int e = 0; e < V / 2; ++e) h[e] = fma2(h[e], pair2(1.0f, 1.0f), t[e]);
             }
-        }
-    };
-    // h * gamma in the place of h
-    const auto weigh = [&](int c, float *h) {
-        float g[V];
-        if (!WHOLE) load_anywhere<G, V>(gamma, c * V - lead, p.h, g);
-        else if (sizeof(G) == 4) load_floats<V>(reinterpret_cast<const float *>(p.gamma) + c * V, g);
-        else unpack<typename std::conditional<sizeof(G) == 2, G, T>::type>(__ldg(reinterpret_cast<const uint4 *>(gamma + c * V)), g);
-#pragma unroll
-        for (int e = 0; e < V; e += 2) {
-            const float2 u = unpair2(mul2(pair2(h[e], h[e + 1]), pair2(g[e], g[e + 1])));
-            h[e] = u.x; h[e + 1] = u.y;
-        }
-    };
-    const auto smooth = [&](int c, float *u) {
-        float m[V];
-        if (WHOLE) load_floats<V>(p.smooth + c * V, m);
-        else load_anywhere<float, V>(p.smooth, c * V - lead, p.h, m);
-#pragma unroll
-        for (int e = 0; e < V; e += 2) {
-            const float2 t = unpair2(mul2(pair2(u[e], u[e + 1]), pair2(m[e], m[e + 1])));
-            u[e] = t.x; u[e + 1] = t.y;
-        }
-    };
-    const bool again = !STREAM && packs > threads * NCH;
-    T *residual_out = reinterpret_cast<T *>(p.residual_out) + row * p.ld_residual_out - lead;
-    T *normed_out = reinterpret_cast<T *>(p.normed_out) + row * p.ld_normed - lead;
-    int8_t *q_out = p.q + row * p.ld_q - lead;
-    const auto store_pack = [&](T *to, int c, const float *f) {
-        if (full(c)) {
-            *reinterpret_cast<uint4 *>(to + (long long)c * V) = pack<T>(f);
-            return;
-        }
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-            if (c * V + e >= lead && c * V + e < lead + p.h) to[c * V + e] = from_float<T>(f[e]);
-    };
-    float u[NCH][V];
-    f32x2 sum2 = 0;
-    float mag = 0.0f;
-    if (STREAM) asm volatile("cp.async.wait_group 0;" ::: "memory");
-    for (int c0 = threadIdx.x; c0 < packs; c0 += threads * NCH) {
-#pragma unroll
-        for (int i = 0; i < NCH; ++i)
-            if (c0 + i * threads < packs) load_h(c0 + i * threads, i, u[i]);
-        if (STREAM && row + gridDim.x < p.rows) fetch(row + gridDim.x);   // the thread has read what this fills
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int c = c0 + i * threads;
-            if (c >= packs) break;
-#pragma unroll
-            for (int e = 0; e < V; e += 2) {
-                const f32x2 v = pair2(u[i][e], u[i][e + 1]);
-                sum2 = fma2(v, v, sum2);
-            }
-            // a row that is read again keeps its inputs, which residual_out may be, until then
-            if (p.residual_out && !again) store_pack(residual_out, c, u[i]);
-            weigh(c, u[i]);
-            float m[V];
-#pragma unroll
-            for (int e = 0; e < V; ++e) m[e] = u[i][e];
-            if (p.smooth) smooth(c, m);
-#pragma unroll
-            for (int e = 0; e < V; e += 2) mag = max_mag(mag, m[e], m[e + 1]);
-        }
-    }
-    const float2 parts = unpair2(sum2);
-    float sum = parts.x + parts.y;
-    block_reduce(sum, mag, red[parity]);
-    parity ^= 1;
-    const float r = rms_scale(sum, p), step = step_of(mag);
-    Quantiser quant;
-    quant.set(step);
-    if (threadIdx.x == 0) p.scale[row] = step == 0.0f ? 0.0f : __fmul_rn(step, r);
-    for (int c0 = threadIdx.x; c0 < packs; c0 += threads * NCH) {
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int c = c0 + i * threads;
-            if (c >= packs) break;
-            if (again) {
-                load_h(c, i, u[i]);
-                if (p.residual_out) store_pack(residual_out, c, u[i]);
-                weigh(c, u[i]);
-            }
-            if (p.normed_out) {
-                float y[V];
+            if (!full(c)) {
 #pragma unroll
                 for (int e = 0; e < V; e += 2) {
-                    const float2 t = unpair2(mul2(pair2(u[i][e], u[i][e + 1]), pair2(r, r)));
-                    y[e] = t.x; y[e + 1] = t.y;
+                    const float2 v = unpair2(h[e / 2]);
+                    h[e / 2] = pair2(c * V + e >= lead && c * V + e < end ? v.x : 0.0f, c * V + e + 1 >= lead && c * V + e + 1 < end ? v.y : 0.0f);
                 }
-                store_pack(normed_out, c, y);
             }
-            if (p.smooth) smooth(c, u[i]);
-            uint32_t q[V / 4];
+        };
+        // h * gamma in the place of h
+        const auto weigh = [&](int c, f32x2 *h) {
+            f32x2 g[V / 2];
+            if constexpr (!WHOLE) load_anywhere<G, V>(gamma, c * V - lead, p.h, g);
+            else if constexpr (sizeof(G) == 4) load_fp32<V>(gamma + c * V, g);
+            else unpack<G>(__ldg(reinterpret_cast<const uint4 *>(gamma + c * V)), g);
 #pragma unroll
-            for (int e = 0; e < V; e += 4) q[e / 4] = quant.four(u[i] + e);
-            int8_t *to = q_out + (long long)c * V;
+            for (int e = 0; e < V / 2; ++e) h[e] = mul2(h[e], g[e]);
+        };
+        const auto smooth = [&](int c, const f32x2 *u, f32x2 *to) {
+            f32x2 m[V / 2];
+            if constexpr (WHOLE) load_fp32<V>(p.smooth + c * V, m);
+            else load_anywhere<float, V>(p.smooth, c * V - lead, p.h, m);
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) to[e] = mul2(u[e], m[e]);
+        };
+        const auto store = [&](T *to, int c, const f32x2 *f) {
             if (full(c)) {
-                if (V == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(q[0], q[V / 4 - 1]);
-                else *reinterpret_cast<uint32_t *>(to) = q[0];
-            } else {
+                *reinterpret_cast<uint4 *>(to + (long long)c * V) = pack<T>(f);
+                return;
+            }
 #pragma unroll
-                for (int e = 0; e < V; ++e)
-                    if (c * V + e >= lead && c * V + e < lead + p.h) to[e] = (int8_t)(q[e / 4] >> (e % 4 * 8));
+            for (int e = 0; e < V; ++e)
+                if (c * V + e >= lead && c * V + e < end) to[c * V + e] = from_float<T>(element(f, e));
+        };
+        f32x2 u[NCH][V / 2];
+        f32x2 sum2 = 0;
+        float mag = 0.0f;
+        if (STREAM) asm volatile("cp.async.wait_group 0;" ::: "memory");
+        for (int c0 = threadIdx.x; c0 < packs; c0 += threads * NCH) {
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) {
+                if (c0 + i * threads < packs) load_h(c0 + i * threads, i, u[i]);
+            }
+            if (STREAM && row + gridDim.x < p.rows) fetch(row + gridDim.x);   // the thread has read what this fills
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) {
+                const int c = c0 + i * threads;
+                if (c >= packs) break;
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) sum2 = fma2(u[i][e], u[i][e], sum2);
+                // a row that is read again keeps its inputs, which residual_out may be, until then
+                if (p.residual_out && !again) store(residual_out, c, u[i]);
+                weigh(c, u[i]);
+                f32x2 m[V / 2];
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) m[e] = u[i][e];
+                if (p.smooth) smooth(c, u[i], m);
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) {
+                    const float2 v = unpair2(m[e]);
+                    mag = max_mag(mag, v.x, v.y);
+                }
             }
         }
-    }
+        const float2 parts = unpair2(sum2);
+        float sum = parts.x + parts.y;
+        block_reduce(sum, mag, red[parity]);
+        parity ^= 1;
+        const float r = rms_scale(sum, p), step = step_of(mag);
+        Quantiser quant;
+        quant.set(step);
+        if (threadIdx.x == 0) p.scale[row] = step == 0.0f ? 0.0f : __fmul_rn(step, r);
+        const auto finish = [&](bool by_rcp) {
+            for (int c0 = threadIdx.x; c0 < packs; c0 += threads * NCH) {
+#pragma unroll
+                for (int i = 0; i < NCH; ++i) {
+                    const int c = c0 + i * threads;
+                    if (c >= packs) break;
+                    if (again) {
+                        load_h(c, i, u[i]);
+                        if (p.residual_out) store(residual_out, c, u[i]);
+                        weigh(c, u[i]);
+                    }
+                    if (p.normed_out) {
+                        f32x2 y[V / 2];
+#pragma unroll
+                        for (int e = 0; e < V / 2; ++e) y[e] = mul2(u[i][e], pair2(r, r));
+                        store(normed_out, c, y);
+                    }
+                    if (p.smooth) smooth(c, u[i], u[i]);
+                    uint32_t q[V / 4];
+#pragma unroll
+                    for (int e = 0; e < V / 4; ++e) q[e] = quant.four(u[i] + 2 * e, by_rcp);
+                    int8_t *to = q_out + (long long)c * V;
+                    if (full(c)) {
+                        if (V == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(q[0], q[V / 4 - 1]);
+                        else *reinterpret_cast<uint32_t *>(to) = q[0];
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < V; ++e)
+                            if (c * V + e >= lead && c * V + e < end) to[e] = (int8_t)(q[e / 4] >> (e % 4 * 8));
+                    }
+                }
+            }
+        };
+        if (quant.rcp != 0.0f) finish(true);
+        else finish(false);
     }
 }
 
@@ -414,7 +426,7 @@ void launch_packed(const NormParams &p, cudaStream_t stream)
     const int four = warps((packs + 3) / 4), smem = 2 * 4 * 16 * four;
     const int fit = 1024 / four < 200 * 1024 / (smem + 1024) ? 1024 / four : 200 * 1024 / (smem + 1024), places = 148 * fit;
     if (packs <= 4 * 256 && p.rows > places) {
-        const auto kernel = norm_quant_kernel<T, G, 4, WHOLE, 256, 3, true>;
+        const auto kernel = norm_quant_kernel<T, G, 4, WHOLE, 256, 4, true>;
         kernel<<<places, four, smem, stream>>>(p);
     } else if (packs <= 1024 && (p.rows <= 2 * 148 || packs <= 64)) norm_quant_kernel<T, G, 1, WHOLE, 1024, 1, false><<<p.rows, warps(packs), 0, stream>>>(p);
     else if (packs <= 4 * 256) norm_quant_kernel<T, G, 4, WHOLE, 256, 3, false><<<p.rows, four, 0, stream>>>(p);
