@@ -6,8 +6,13 @@
 // scores that are returned are computed (and with `renormalize` softmax needs no sum over all experts, since it cancels).
 //
 // One warp per row.  A group's experts lie in `sub` neighbouring lanes (sub * groups <= 32, sub a power of two), `per` consecutive ones
-// in each: lower experts are in lower lanes and lower registers, so the first of equal candidates has the lowest id, and a group is
-// ranked by shuffles among its lanes.  Candidates are compared as unsigned keys that order like their values; key 0 is no candidate.
+// in each: lower experts are in lower lanes and lower registers, and a group is ranked by shuffles among its lanes.  Candidates are
+// compared as unsigned keys that order like their values; key 0 is no candidate.
+//
+// The k-th largest of the lanes' maxima bounds the k-th largest key from below, and few keys reach it: those are gathered, one to a lane,
+// and each counts how many stand before it (larger, or equal with a lower id), which is its place in the result.  Taking the largest key
+// k times over instead, with the owner's registers searched every time, was 25 us for 16384 rows of 256; it is left for rows where more
+// than 32 keys reach the bound (many equal ones, or a large k).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -21,22 +26,45 @@ constexpr int kWarps = 4;
 
 struct RouteParams {
     const void *logits;
+    int dtype;
     long long ld;
     const float *bias;
     const int8_t *token_mask;
     int rows, experts, top_k;
     int groups, group_size, topk_group, sub, per;
+    bool whole;                // every lane's experts fill its registers and start on a boundary of their own size (at most 16 bytes)
+    bool renormalize, ids_i64;
     float scale;
     float *weights;
     void *ids;
 };
 
-template <typename T> __device__ __forceinline__ float load_logit(const void *p, long long at);
-template <> __device__ __forceinline__ float load_logit<float>(const void *p, long long at) { return __ldg(reinterpret_cast<const float *>(p) + at); }
-template <> __device__ __forceinline__ float load_logit<__half>(const void *p, long long at) { return __half2float(reinterpret_cast<const __half *>(p)[at]); }
-template <> __device__ __forceinline__ float load_logit<__nv_bfloat16>(const void *p, long long at) { return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[at]); }
-
 __device__ __forceinline__ float minus_inf() { return __int_as_float(0xff800000); }
+
+// R values of a lane with as wide loads as there are.
+template <typename T, int R>
+__device__ __forceinline__ void load_wide(const T *from, float (&l)[R])
+{
+    constexpr int BYTES = R * (int)sizeof(T), STEP = BYTES < 16 ? BYTES : 16, N = STEP / (int)sizeof(T);
+    struct alignas(STEP) Pack { T v[N]; };
+#pragma unroll
+    for (int i = 0; i < R; i += N) {
+        const Pack q = *reinterpret_cast<const Pack *>(from + i);
+#pragma unroll
+        for (int e = 0; e < N; ++e) l[i + e] = (float)q.v[e];
+    }
+}
+template <typename T, int R>
+__device__ __forceinline__ void load_logits(const RouteParams &p, long long at, int mine, float (&l)[R])
+{
+    const T *from = reinterpret_cast<const T *>(p.logits) + at;
+    if (p.whole) {
+        load_wide<T, R>(from, l);
+    } else {
+#pragma unroll
+        for (int i = 0; i < R; ++i) l[i] = i < mine ? (float)from[i] : minus_inf();
+    }
+}
 
 // Orders like v for all v above minus infinity; adding zero makes the two zeros equal.
 __device__ __forceinline__ uint32_t key_of(float v)
@@ -64,33 +92,42 @@ __device__ __forceinline__ float warp_max(float v)
     return v;
 }
 
-__device__ __forceinline__ float sigmoid(float l) { return __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-l))); }
+__device__ __forceinline__ float sigmoid(float l) { return __frcp_rn(__fadd_rn(1.0f, expf(-l))); }
 // exp(l - top); the largest logit gives 1 also where it is infinite.
 __device__ __forceinline__ float exp_below(float l, float top) { return l == top ? 1.0f : expf(__fsub_rn(l, top)); }
 
+__device__ __forceinline__ void put(const RouteParams &p, long long at, float w, int id)
+{
+    p.weights[at] = w;
+    if (p.ids_i64) reinterpret_cast<int64_t *>(p.ids)[at] = id;
+    else reinterpret_cast<int32_t *>(p.ids)[at] = id;
+}
+
 // SCORED: c is computed for every expert, else it is the logit.  R: experts per lane, at least p.per.
-template <typename T, typename I, int R, bool SIGMOID, bool SCORED, bool TOP2, bool RENORM>
+template <int R, bool SIGMOID, bool SCORED, bool TOP2>
 __global__ void __launch_bounds__(32 * kWarps) route_kernel(const RouteParams p)
 {
-    const int lane = threadIdx.x & 31;
-    const int row = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    __shared__ unsigned long long list_key[kWarps][32];   // key, then the id with its bits inverted: equal keys order by the lower id
+    __shared__ float list_logit[kWarps][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int row = blockIdx.x * kWarps + warp;
     if (row >= p.rows) return;
-    float *weights = p.weights + (long long)row * p.top_k;
-    I *ids = reinterpret_cast<I *>(p.ids) + (long long)row * p.top_k;
+    const long long out = (long long)row * p.top_k;
     if (p.token_mask && p.token_mask[row] == 0) {
-        if (lane < p.top_k) { weights[lane] = 0.0f; ids[lane] = (I)-1; }
+        if (lane < p.top_k) put(p, out + lane, 0.0f, -1);
         return;
     }
     const int group = lane / p.sub, inside = (lane % p.sub) * p.per;
     const int first = group * p.group_size + inside;
     const int mine = group < p.groups ? max(0, min(p.per, p.group_size - inside)) : 0;
     float l[R];
-    uint32_t key[R];
+    const long long at = (long long)row * p.ld + first;
+    if (p.dtype == kF32) load_logits<float, R>(p, at, mine, l);
+    else if (p.dtype == kBF16) load_logits<__nv_bfloat16, R>(p, at, mine, l);
+    else load_logits<__half, R>(p, at, mine, l);
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        l[i] = i < mine ? load_logit<T>(p.logits, (long long)row * p.ld + first + i) : minus_inf();
+    for (int i = 0; i < R; ++i)
         if (!(l[i] > minus_inf())) l[i] = minus_inf();   // NaN too
-    }
     float top = 0.0f, total = 1.0f;
     if (!SIGMOID) {
         top = l[0];
@@ -102,27 +139,39 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(const RouteParams p)
 #pragma unroll
             for (int i = 0; i < R; ++i) t += l[i] > minus_inf() ? (double)exp_below(l[i], top) : 0.0;
             total = (float)warp_sum(t);
-        } else if (!RENORM) {
+        } else if (!p.renormalize) {
             float t = 0.0f;
 #pragma unroll
             for (int i = 0; i < R; ++i) t += l[i] > minus_inf() ? exp_below(l[i], top) : 0.0f;
             total = warp_sum(t);
         }
     }
-    const auto score = [&](float v) { return SIGMOID ? sigmoid(v) : !SCORED && RENORM ? exp_below(v, top) : __fdiv_rn(exp_below(v, top), total); };
+    // without SCORED and with renormalisation the sum over all experts cancels: total stays 1
+    const auto score = [&](float v) { return SIGMOID ? sigmoid(v) : __fdiv_rn(exp_below(v, top), total); };
     float best = minus_inf(), second = minus_inf();
+    uint32_t key[R];
+    float bias[R];
+    if (SCORED && p.bias) {
+        if (p.whole) {
+            load_wide<float, R>(p.bias + first, bias);
+        } else {
+#pragma unroll
+            for (int i = 0; i < R; ++i) bias[i] = i < mine ? __ldg(p.bias + first + i) : 0.0f;
+        }
+    }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         float c = l[i];
-        if (SCORED && c > minus_inf()) {
+        if (SCORED) {
             c = score(c);
-            if (p.bias) c = __fadd_rn(c, __ldg(p.bias + first + i));
+            if (p.bias) c = __fadd_rn(c, bias[i]);
+            c = l[i] > minus_inf() && c > minus_inf() ? c : minus_inf();
         }
         key[i] = c > minus_inf() ? key_of(c) : 0u;
-        if (!(c > minus_inf())) c = minus_inf();
         if (TOP2) second = fmaxf(second, fminf(best, c));
         best = fmaxf(best, c);
     }
+    uint32_t top_key = best > minus_inf() ? key_of(best) : 0u;
     if (p.groups > 1) {
         for (int o = 1; o < p.sub; o <<= 1) {
             const float ob = __shfl_xor_sync(kAll, best, o);
@@ -136,78 +185,113 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(const RouteParams p)
             better += r > rank || (r == rank && g < group);
         }
         if (better >= p.topk_group) {
+            top_key = 0u;
 #pragma unroll
             for (int i = 0; i < R; ++i) key[i] = 0u;
         }
     }
-    // k rounds: the largest key of the warp, the first one of equal ones
+    // a bound that at least k keys reach, or all there are
+    uint32_t bound = 1u;
+    {
+        uint32_t rest = top_key;
+        for (int j = 0; j < p.top_k; ++j) {
+            const uint32_t m = __reduce_max_sync(kAll, rest);
+            if (m == 0u) { bound = 1u; break; }
+            bound = m;
+            if (rest == m) rest = 0u;
+        }
+    }
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) count += key[i] >= bound;
+    int before = count;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(kAll, before, o);
+        if (lane >= o) before += t;
+    }
+    const int found = __shfl_sync(kAll, before, 31);
+    before -= count;
     float chosen = 0.0f;
-    int id = -1;
-    for (int j = 0; j < p.top_k; ++j) {
-        uint32_t m = key[0];
+    int id = -1, place = lane;
+    if (found <= 32) {
+        list_key[warp][lane] = 0ull;
+        __syncwarp();
 #pragma unroll
-        for (int i = 1; i < R; ++i) m = max(m, key[i]);
-        const uint32_t warp_m = __reduce_max_sync(kAll, m);
-        if (warp_m == 0) break;
-        const int owner = __ffs(__ballot_sync(kAll, m == warp_m)) - 1;
-        float v = 0.0f;
-        int at = 0;
-        if (lane == owner) {
-            bool found = false;
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                if (!found && key[i] == warp_m) {
-                    found = true;
-                    at = first + i;
-                    v = l[i];
-                    key[i] = 0u;
-                }
+        for (int i = 0; i < R; ++i) {
+            if (key[i] >= bound) {
+                list_key[warp][before] = (unsigned long long)key[i] << 32 | (uint32_t)~(first + i);
+                list_logit[warp][before] = l[i];
+                ++before;
             }
         }
-        v = __shfl_sync(kAll, v, owner);
-        at = __shfl_sync(kAll, at, owner);
-        if (lane == j) { chosen = v; id = at; }
+        __syncwarp();
+        const unsigned long long own = list_key[warp][lane];
+        place = 0;
+        for (int q = 0; q < found; q += 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) place += list_key[warp][q + e] > own;
+        }
+        if (lane < found) {
+            chosen = list_logit[warp][lane];
+            id = ~(int)(uint32_t)own;
+        } else {
+            place = lane;   // at least `found`: a slot for which there is no expert
+        }
+    } else {
+        // k rounds: the largest key of the warp, the first one of equal ones
+        for (int j = 0; j < p.top_k; ++j) {
+            uint32_t m = key[0];
+#pragma unroll
+            for (int i = 1; i < R; ++i) m = max(m, key[i]);
+            const uint32_t warp_m = __reduce_max_sync(kAll, m);
+            const int owner = __ffs(__ballot_sync(kAll, m == warp_m)) - 1;
+            float v = 0.0f;
+            int it = 0;
+            if (lane == owner) {
+                bool done = false;
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    if (!done && key[i] == warp_m) {
+                        done = true;
+                        it = first + i;
+                        v = l[i];
+                        key[i] = 0u;
+                    }
+                }
+            }
+            v = __shfl_sync(kAll, v, owner);
+            it = __shfl_sync(kAll, it, owner);
+            if (lane == j) { chosen = v; id = it; }
+        }
     }
-    float w = id >= 0 ? score(chosen) : 0.0f;
-    if (RENORM) {
+    float w = place < p.top_k && id >= 0 ? score(chosen) : 0.0f;
+    if (p.renormalize) {
         const float sum = warp_sum(w);
         w = sum > 0.0f ? __fdiv_rn(w, sum) : 0.0f;
     }
-    if (lane < p.top_k) {
-        weights[lane] = __fmul_rn(w, p.scale);
-        ids[lane] = (I)id;
-    }
+    if (place < p.top_k) put(p, out + place, __fmul_rn(w, p.scale), id);
 }
 
-template <typename T, typename I, int R, bool SIGMOID, bool RENORM>
+template <int R, bool SIGMOID>
 void launch_scored(const RouteParams &p, bool scored, bool top2, cudaStream_t stream)
 {
     const unsigned grid = (unsigned)((p.rows + kWarps - 1) / kWarps);
-    if (!scored) route_kernel<T, I, R, SIGMOID, false, false, RENORM><<<grid, 32 * kWarps, 0, stream>>>(p);
-    else if (!top2) route_kernel<T, I, R, SIGMOID, true, false, RENORM><<<grid, 32 * kWarps, 0, stream>>>(p);
-    else route_kernel<T, I, R, SIGMOID, true, true, RENORM><<<grid, 32 * kWarps, 0, stream>>>(p);
+    if (!scored) route_kernel<R, SIGMOID, false, false><<<grid, 32 * kWarps, 0, stream>>>(p);
+    else if (!top2) route_kernel<R, SIGMOID, true, false><<<grid, 32 * kWarps, 0, stream>>>(p);
+    else route_kernel<R, SIGMOID, true, true><<<grid, 32 * kWarps, 0, stream>>>(p);
 }
 
-template <typename T, typename I, int R>
-void launch_rows(const RouteParams &p, const RouteTopKProblem &r, cudaStream_t stream)
+template <int R>
+void launch_rows(RouteParams &p, const RouteTopKProblem &r, cudaStream_t stream)
 {
+    const int bytes = R * (r.dtype == kF32 ? 4 : 2), step = bytes < 16 ? bytes : 16;
+    const long long pitch = r.ld * (r.dtype == kF32 ? 4 : 2);
+    p.whole = p.per == R && p.sub * R == p.group_size && p.sub * p.groups == 32 && (((uintptr_t)r.logits | (uintptr_t)pitch) & (uintptr_t)(step - 1)) == 0 &&
+              ((uintptr_t)r.bias & 15) == 0;
     const bool top2 = r.n_group > 1 && r.group_score == kGroupTop2, scored = r.bias || top2;
-    if (r.scoring == kScoreSigmoid) {
-        if (r.renormalize) launch_scored<T, I, R, true, true>(p, scored, top2, stream);
-        else launch_scored<T, I, R, true, false>(p, scored, top2, stream);
-    } else {
-        if (r.renormalize) launch_scored<T, I, R, false, true>(p, scored, top2, stream);
-        else launch_scored<T, I, R, false, false>(p, scored, top2, stream);
-    }
-}
-
-template <typename T, typename I>
-cudaError_t launch_typed(const RouteParams &p, const RouteTopKProblem &r, cudaStream_t stream)
-{
-    if (p.per <= 2) launch_rows<T, I, 2>(p, r, stream);
-    else if (p.per <= 8) launch_rows<T, I, 8>(p, r, stream);
-    else launch_rows<T, I, 64>(p, r, stream);
-    return cudaGetLastError();
+    if (r.scoring == kScoreSigmoid) launch_scored<R, true>(p, scored, top2, stream);
+    else launch_scored<R, false>(p, scored, top2, stream);
 }
 
 }  // namespace
@@ -216,19 +300,20 @@ cudaError_t route_top_k_launch(const RouteTopKProblem &r, cudaStream_t stream)
 {
     if (r.rows <= 0) return cudaSuccess;
     RouteParams p;
-    p.logits = r.logits; p.ld = r.ld; p.bias = r.bias; p.token_mask = r.token_mask;
+    p.logits = r.logits; p.dtype = r.dtype; p.ld = r.ld; p.bias = r.bias; p.token_mask = r.token_mask;
     p.rows = (int)r.rows; p.experts = r.experts; p.top_k = r.top_k;
     p.groups = r.n_group; p.group_size = r.experts / r.n_group; p.topk_group = r.topk_group;
     p.sub = 32;
     while (p.sub * p.groups > 32) p.sub >>= 1;
     p.per = (p.group_size + p.sub - 1) / p.sub;   // below 2 * 1024 / 32: more than half of the lanes have a group
+    p.renormalize = r.renormalize; p.ids_i64 = r.ids_i64;
     p.scale = r.scale; p.weights = r.weights; p.ids = r.ids;
-    switch (r.dtype) {
-        case kF32: return r.ids_i64 ? launch_typed<float, int64_t>(p, r, stream) : launch_typed<float, int32_t>(p, r, stream);
-        case kF16: return r.ids_i64 ? launch_typed<__half, int64_t>(p, r, stream) : launch_typed<__half, int32_t>(p, r, stream);
-        case kBF16: return r.ids_i64 ? launch_typed<__nv_bfloat16, int64_t>(p, r, stream) : launch_typed<__nv_bfloat16, int32_t>(p, r, stream);
-        default: return cudaErrorInvalidValue;
-    }
+    if (p.per <= 2) launch_rows<2>(p, r, stream);
+    else if (p.per <= 4) launch_rows<4>(p, r, stream);
+    else if (p.per <= 8) launch_rows<8>(p, r, stream);
+    else if (p.per <= 16) launch_rows<16>(p, r, stream);
+    else launch_rows<64>(p, r, stream);
+    return cudaGetLastError();
 }
 
 }  // namespace gmm
