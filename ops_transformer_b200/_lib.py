@@ -176,5 +176,16 @@ def describe_call(kinds: str, *items) -> bytes:
     return describe_call(kinds, *items)
 
 
+def native():
+    """(the description module, the address of gmmB200Call): what ``launch`` of the module takes."""
+    global _NATIVE
+    if _NATIVE is None:
+        _NATIVE = _describe_module(), C.cast(lib().gmmB200Call, C.c_void_p).value
+    return _NATIVE
+
+
+_NATIVE = None
+
+
 def last_error() -> str:
     return lib().aclGetRecentErrMsg().decode("utf-8", "replace")

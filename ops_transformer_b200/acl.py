@@ -435,19 +435,49 @@ def _float_bits(v: float) -> int:
     return struct.unpack("<I", struct.pack("<f", v))[0]
 
 
-def _block_call(op: int, name: str, words: bytes, tensors, workspace: Optional[torch.Tensor], stream,
-                options: Optional[LaunchOptions] = None) -> Optional[torch.Tensor]:
-    """``_call`` for operators whose tensors all have to be on the first one's GPU.  Elsewhere the arguments are checked and the call is
-    refused: these operators may need no workspace, whose place would tell."""
-    device = tensors[0].device
-    if device.type != "cuda" or any(t is not None and t.device != device for t in tensors):
+def _block_call(op: int, name: str, workspace: Optional[torch.Tensor], stream, kinds: str, *items) -> None:
+    """The call of an operator around the expert FFN, natively.  Its tensors all have to be on one GPU; elsewhere the arguments are
+    checked and the call is refused.  A call that needs no workspace (all but ``adapter_add`` and strided views) takes none."""
+    module, call = _lib.native()
+    x = items[0]
+    pooled = workspace is None and op == _lib.OP_ADAPTER_ADD
+    if not x.is_cuda:
+        done = False
+    else:
+        handle = _gpu_stream_handle(stream)
+        if pooled:
+            slot = _WS.slot(x.device, handle)
+            with slot.lock:   # the clear and the kernels of two calls must not interleave on the stream
+                done = module.launch(call, op | _lib.OP_POOLED, handle, slot.buf, kinds, *items)
+        else:
+            done = module.launch(call, op, handle, workspace, kinds, *items)
+    if done is None:
+        return
+    if done is False:
+        words = _lib.describe_call(kinds, *items)
         res = _lib.CallResult()
         rc = _lib.lib().gmmB200Call(op | _lib.OP_PLAN_ONLY, words, len(words) // 8, None, 0, None, None, C.byref(res))
         if rc != ACLNN_SUCCESS:
             raise AclnnError(rc, name + "GetWorkspaceSize")
         _lib.lib().aclDestroyAclOpExecutor(C.c_void_p(res.executor))
         raise ValueError(f"{name}: all tensors must be on one CUDA device")
-    return _call(op, name, words, device, workspace, stream, options)
+    rc, stage, need, executor = done
+    if rc != ACLNN_SUCCESS:
+        raise AclnnError(rc, name + ("GetWorkspaceSize" if stage == _lib.STAGE_PLAN else ""))
+    # planned only: the pool's buffer is too small or not for this call, or strided views need one
+    if workspace is not None:
+        _lib.lib().aclDestroyAclOpExecutor(C.c_void_p(executor))
+        raise ValueError(f"workspace of {workspace.numel()} bytes is smaller than the {need} required")
+    slot = _WS.slot(x.device, handle)
+    with slot.lock:
+        try:
+            workspace = _WS.lend(slot, x.device, stream, need)
+        except Exception:
+            _lib.lib().aclDestroyAclOpExecutor(C.c_void_p(executor))
+            raise
+        rc = getattr(_lib.lib(), name)(workspace.data_ptr(), need, C.c_void_p(executor), handle)
+    if rc != ACLNN_SUCCESS:
+        raise AclnnError(rc, name)
 
 
 def add_rms_norm_quant(x: torch.Tensor, gamma: torch.Tensor, *, residual: Optional[torch.Tensor] = None,
@@ -459,22 +489,23 @@ def add_rms_norm_quant(x: torch.Tensor, gamma: torch.Tensor, *, residual: Option
     as the W8A8 operators take their rows, ``h`` itself (None without a residual) and, with ``normed`` or a ``normed_out`` to write to,
     the normed rows in x's type.  ``smooth`` (fp32 [h]) multiplies what is quantised, not ``normed_out``.  ``residual_out`` may be
     ``residual`` or ``x``.  gmmB200AddRmsNormQuant (include/gmm_b200.h) has the formulas."""
+    empty = _lib.native()[0].empty
     if q is None:
-        q = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
+        q = empty(x, "b")
     if scale is None:
-        scale = x.new_empty(x.shape[:1], dtype=torch.float32)
+        scale = empty(x, "f", x.shape[0])
     if residual_out is None and residual is not None:
-        residual_out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        residual_out = empty(x, "=")
     if normed_out is None and normed:
-        normed_out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    words = _lib.describe_call("tttttttti", x, residual, gamma, smooth, q, scale, residual_out, normed_out, _float_bits(eps))
-    _block_call(_lib.OP_ADD_RMS_NORM_QUANT, "gmmB200AddRmsNormQuant", words, (x, residual, gamma, smooth, q, scale, residual_out, normed_out),
-                workspace, stream)
+        normed_out = empty(x, "=")
+    _block_call(_lib.OP_ADD_RMS_NORM_QUANT, "gmmB200AddRmsNormQuant", workspace, stream, "tttttttti", x, residual, gamma, smooth, q, scale,
+                residual_out, normed_out, _float_bits(eps))
     return q, scale, residual_out, normed_out
 
 
 _SCORING = {"softmax": 0, "sigmoid": 1}
 _GROUP_SCORE = {"max": 0, "top2": 1}
+_ID_LETTER = {torch.int32: "i", torch.int64: "l"}
 
 
 def route_top_k(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", bias: Optional[torch.Tensor] = None, n_group: int = 1,
@@ -488,16 +519,17 @@ def route_top_k(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", b
     what ``moe_init_routing_v3`` takes, int64 the expert-parallel layer.  gmmB200RouteTopK (include/gmm_b200.h) has the rules."""
     if scoring not in _SCORING or group_score not in _GROUP_SCORE:
         raise ValueError(f"unknown scoring {scoring!r} or group_score {group_score!r}")
-    shape = (logits.shape[0], top_k)
+    empty = _lib.native()[0].empty
     if weights is None:
-        weights = logits.new_empty(shape, dtype=torch.float32)
+        weights = empty(logits, "f", logits.shape[0], top_k)
     if ids is None:
-        ids = logits.new_empty(shape, dtype=ids_dtype)
+        letter = _ID_LETTER.get(ids_dtype)
+        shape = logits.shape[0], top_k
+        ids = empty(logits, letter, *shape) if letter else logits.new_empty(shape, dtype=ids_dtype)   # refused by the operator
     if token_mask is not None and token_mask.dtype == torch.bool:
         token_mask = token_mask.view(torch.int8)
-    words = _lib.describe_call("tttttiiiiii", logits, bias, token_mask, weights, ids, _SCORING[scoring], n_group, topk_group,
-                               _GROUP_SCORE[group_score], 1 if renormalize else 0, _float_bits(scale))
-    _block_call(_lib.OP_ROUTE_TOP_K, "gmmB200RouteTopK", words, (logits, bias, token_mask, weights, ids), workspace, stream)
+    _block_call(_lib.OP_ROUTE_TOP_K, "gmmB200RouteTopK", workspace, stream, "tttttiiiiii", logits, bias, token_mask, weights, ids,
+                _SCORING[scoring], n_group, topk_group, _GROUP_SCORE[group_score], 1 if renormalize else 0, _float_bits(scale))
     return weights, ids
 
 
@@ -509,7 +541,6 @@ def adapter_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.T
     ``x_scale`` (fp32 [rows]); a [adapters, rank, k], b [adapters, n, rank].  ``out`` may be ``base``.  gmmB200AdapterAdd
     (include/gmm_b200.h)."""
     if out is None:
-        out = torch.empty_like(base, memory_format=torch.contiguous_format)
-    words = _lib.describe_call("tttttttt", base, x, x_scale, a, b, adapter_ids, scaling, out)
-    _block_call(_lib.OP_ADAPTER_ADD, "gmmB200AdapterAdd", words, (base, x, x_scale, a, b, adapter_ids, scaling, out), workspace, stream)
+        out = _lib.native()[0].empty(base, "=")
+    _block_call(_lib.OP_ADAPTER_ADD, "gmmB200AdapterAdd", workspace, stream, "tttttttt", base, x, x_scale, a, b, adapter_ids, scaling, out)
     return out

@@ -8,13 +8,41 @@
 #include "aclnn/aclnn_base.h"
 #include "gmm_common.h"
 
+// Sizes of at most 8 dimensions, in place: a call describes up to ten tensors by three lists each, which as vectors were thirty
+// allocations.
+class Dims {
+public:
+    size_t size() const { return n_; }
+    int64_t operator[](size_t i) const { return v_[i]; }
+    int64_t &operator[](size_t i) { return v_[i]; }
+    const int64_t *begin() const { return v_; }
+    const int64_t *end() const { return v_ + n_; }
+    int64_t *begin() { return v_; }
+    int64_t *end() { return v_ + n_; }
+    void resize(size_t n) { n_ = n; }   // n <= 8; the values are set next
+    void assign(size_t n, int64_t v)
+    {
+        n_ = n;
+        for (int64_t &d : *this) d = v;
+    }
+    void assign(const int64_t *from, const int64_t *to)
+    {
+        n_ = 0;
+        while (from != to) v_[n_++] = *from++;
+    }
+
+private:
+    size_t n_ = 0;
+    int64_t v_[8];
+};
+
 struct aclTensor {
-    std::vector<int64_t> view_dims;
-    std::vector<int64_t> strides;   // elements
+    Dims view_dims;
+    Dims strides;                   // elements
     int64_t offset = 0;             // elements
     aclDataType dtype = ACL_DT_UNDEFINED;
     aclFormat format = ACL_FORMAT_ND;
-    std::vector<int64_t> storage_dims;
+    Dims storage_dims;
     void *data = nullptr;
 
     size_t rank() const { return view_dims.size(); }

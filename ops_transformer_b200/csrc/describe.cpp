@@ -2,8 +2,11 @@
 //
 // In Python the description of a call - address, type, format, sizes, strides and storage sizes of seven to ten tensors - cost
 // 7 us, more than the call's launches; here 0.6.
+//
+// launch() goes one step further for operators whose whole work is a few microseconds: it describes the tensors and makes the call.
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <ATen/ops/empty.h>
 
 #include <Python.h>
 #include <cstdint>
@@ -169,7 +172,102 @@ PyObject *describe_call(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     return packed(args + 1, n, [&](Py_ssize_t i) { return kinds[i]; });
 }
 
+// gmmB200CallResult and the type of gmmB200Call (include/gmm_b200.h), whose address the binding passes on.
+struct CallResult {
+    uint64_t workspace;
+    void *executor;
+    int32_t stage, reserved;
+};
+typedef int32_t (*CallFn)(int32_t, const int64_t *, uint64_t, void *, uint64_t, const void *, void *, CallResult *);
+constexpr int32_t kStageRun = 3;
+
+// launch(gmmB200Call, operator, stream, workspace or None, kinds, item, ...): the call itself.  None when it is enqueued; False, with
+// nothing done, when the tensors are not all on one CUDA device; else (status, stage, workspace size, executor).
+PyObject *launch(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    Py_ssize_t n = 0;
+    const char *kinds = nargs > 4 ? PyUnicode_AsUTF8AndSize(args[4], &n) : "";
+    if (!kinds) return nullptr;
+    if (nargs < 6 || n != nargs - 5) {
+        PyErr_SetString(PyExc_TypeError, "a function, an operator, a stream, a workspace, the kinds of the arguments and as many arguments are wanted");
+        return nullptr;
+    }
+    const CallFn fn = reinterpret_cast<CallFn>(PyLong_AsVoidPtr(args[0]));
+    const long op = PyLong_AsLong(args[1]);
+    void *stream = PyLong_AsVoidPtr(args[2]);
+    if (PyErr_Occurred()) return nullptr;
+    try {
+        PyObject *const *items = args + 5;
+        void *workspace = nullptr;
+        uint64_t bytes = 0;
+        int device = -1;
+        const auto elsewhere = [&](PyObject *o) {
+            if (o == Py_None || !THPVariable_Check(o)) return false;
+            const at::Tensor &t = THPVariable_Unpack(o);
+            if (!t.is_cuda()) return true;
+            if (device < 0) device = t.get_device();
+            return t.get_device() != device;
+        };
+        for (Py_ssize_t i = 0; i < n; ++i)
+            if (kinds[i] == 't' && elsewhere(items[i])) Py_RETURN_FALSE;
+        if (elsewhere(args[3])) Py_RETURN_FALSE;
+        if (args[3] != Py_None && THPVariable_Check(args[3])) {
+            const at::Tensor &t = THPVariable_Unpack(args[3]);
+            workspace = t.data_ptr();
+            bytes = t.nbytes();
+        }
+        std::vector<int64_t> w;
+        w.reserve(192);
+        for (Py_ssize_t i = 0; i < n; ++i)
+            if (!put_item(w, kinds[i], items[i])) return nullptr;
+        CallResult res = {};
+        int32_t rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = fn((int32_t)op, w.data(), w.size(), workspace, bytes, nullptr, stream, &res);
+        Py_END_ALLOW_THREADS
+        if (rc == 0 && res.stage == kStageRun) Py_RETURN_NONE;
+        return Py_BuildValue("(iiKN)", (int)rc, (int)res.stage, (unsigned long long)res.workspace, PyLong_FromVoidPtr(res.executor));
+    } catch (const std::exception &e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
+    }
+}
+
+// empty(tensor, letter of the type, size, ...): an uninitialised contiguous tensor on the tensor's device.  'b' int8, 'i' int32,
+// 'l' int64, 'f' float32, '=' the tensor's own type; without sizes it has the tensor's.
+PyObject *empty(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    if (nargs < 2 || nargs > 4 || !THPVariable_Check(args[0])) {
+        PyErr_SetString(PyExc_TypeError, "a tensor, a type and at most two sizes are wanted");
+        return nullptr;
+    }
+    const char *type = PyUnicode_AsUTF8(args[1]);
+    if (!type) return nullptr;
+    int64_t sizes[2] = {0, 0};
+    for (Py_ssize_t i = 2; i < nargs; ++i) {
+        PyObject *index = PyNumber_Index(args[i]);
+        sizes[i - 2] = index ? PyLong_AsLongLong(index) : -1;
+        Py_XDECREF(index);
+        if (PyErr_Occurred()) return nullptr;
+        if (sizes[i - 2] < 0) {
+            PyErr_SetString(PyExc_ValueError, "sizes must not be negative");
+            return nullptr;
+        }
+    }
+    try {
+        const at::Tensor &t = THPVariable_Unpack(args[0]);
+        const at::ScalarType dtype = *type == 'b' ? at::kChar : *type == 'i' ? at::kInt : *type == 'l' ? at::kLong : *type == 'f' ? at::kFloat : t.scalar_type();
+        const auto options = at::TensorOptions().dtype(dtype).device(t.device());
+        return THPVariable_Wrap(nargs == 2 ? at::empty(t.sizes(), options) : at::empty(at::IntArrayRef(sizes, (size_t)nargs - 2), options));
+    } catch (const std::exception &e) {   // out of memory
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
+    }
+}
+
 PyMethodDef methods[] = {
+    {"launch", (PyCFunction)(void (*)(void))launch, METH_FASTCALL, "Describes an operator's arguments and makes the call."},
+    {"empty", (PyCFunction)(void (*)(void))empty, METH_FASTCALL, "An uninitialised tensor beside another."},
     {"describe", (PyCFunction)(void (*)(void))describe, METH_FASTCALL, "Packed description of items by themselves."},
     {"describe_call", (PyCFunction)(void (*)(void))describe_call, METH_FASTCALL, "Packed description of an operator's arguments."},
     {nullptr, nullptr, 0, nullptr},

@@ -37,8 +37,8 @@ void bind_tensor(aclOpExecutor *e, const aclTensor *t, P *field, bool is_output,
     if (!t) { *field = nullptr; return; }
     if (t->contiguous() || contiguous_enough) { *field = (P)tensor_ptr(t); return; }
     StagedView v;
-    v.dims = t->view_dims;
-    v.strides = t->strides;
+    v.dims.assign(t->view_dims.begin(), t->view_dims.end());
+    v.strides.assign(t->strides.begin(), t->strides.end());
     v.elem = (int)dtype_size(t->dtype);
     v.data = tensor_ptr(t);
     v.ws_off = e->staged_bytes;
