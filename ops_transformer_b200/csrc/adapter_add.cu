@@ -338,10 +338,24 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(const Adapte
     if (tid == 0) carry = make_int2(0, 0);
     if (tid < 4) p.status[tid] = 0;
     __syncthreads();
-    for (int t0 = 0; t0 < p.rows; t0 += kPlanThreads) {
-        const int t = t0 + tid, id = t < p.rows ? adapter_of(p, t) : -2;
-        const unsigned same = __match_any_sync(0xffffffffu, id);
-        if (id != -2 && lane == __ffs(same) - 1) atomicAdd(&counts[id < 0 ? p.adapters : id], __popc(same));
+    // the first tokens' adapters stay in registers between the two passes; all loads of a batch are under way together
+    constexpr int KEEP = 8;
+    int ids[KEEP];
+    const auto fetch = [&](int t0) {
+#pragma unroll
+        for (int j = 0; j < KEEP; ++j) {
+            const int t = t0 + j * kPlanThreads + tid;
+            ids[j] = t < p.rows ? adapter_of(p, t) : -2;
+        }
+    };
+    for (int t0 = 0; t0 < p.rows; t0 += KEEP * kPlanThreads) {
+        fetch(t0);
+#pragma unroll
+        for (int j = 0; j < KEEP; ++j) {
+            if (t0 + j * kPlanThreads >= p.rows) break;
+            const unsigned same = __match_any_sync(0xffffffffu, ids[j]);
+            if (ids[j] != -2 && lane == __ffs(same) - 1) atomicAdd(&counts[ids[j] < 0 ? p.adapters : ids[j]], __popc(same));
+        }
     }
     __syncthreads();
     // running totals of tokens and tiles over the adapters
@@ -377,14 +391,19 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(const Adapte
         __syncthreads();
     }
     if (tid == 0) *p.n_tiles = carry.y;
-    for (int t0 = 0; t0 < p.rows; t0 += kPlanThreads) {
-        const int t = t0 + tid, id = t < p.rows ? adapter_of(p, t) : -2;
-        const unsigned same = __match_any_sync(0xffffffffu, id);
-        const int leader = __ffs(same) - 1;
-        int at = 0;
-        if (id != -2 && lane == leader) at = atomicAdd(&counts[id < 0 ? p.adapters : id], __popc(same));
-        at = __shfl_sync(0xffffffffu, at, leader);
-        if (id != -2) p.order[at + __popc(same & ((1u << lane) - 1u))] = t;
+    for (int t0 = 0; t0 < p.rows; t0 += KEEP * kPlanThreads) {
+        if (p.rows > KEEP * kPlanThreads) fetch(t0);
+#pragma unroll
+        for (int j = 0; j < KEEP; ++j) {
+            if (t0 + j * kPlanThreads >= p.rows) break;
+            const int id = ids[j];
+            const unsigned same = __match_any_sync(0xffffffffu, id);
+            const int leader = __ffs(same) - 1;
+            int at = 0;
+            if (id != -2 && lane == leader) at = atomicAdd(&counts[id < 0 ? p.adapters : id], __popc(same));
+            at = __shfl_sync(0xffffffffu, at, leader);
+            if (id != -2) p.order[at + __popc(same & ((1u << lane) - 1u))] = t0 + j * kPlanThreads + tid;
+        }
     }
 }
 
@@ -437,16 +456,20 @@ __global__ void __launch_bounds__(kShrinkThreads) adapter_shrink_kernel(const Ad
         constexpr int XB = I8 ? 1 : 2;
         const char *x = reinterpret_cast<const char *>(p.x);
         const char *a = reinterpret_cast<const char *>(p.a) + (long long)tile.adapter * p.rank * p.k * 2;
-        constexpr int XC = I8 ? 4 : 8;                        // copies per token row of a K block
-        constexpr int NX = (TN * XC + kShrinkThreads - 1) / kShrinkThreads, NA = 128 * 8 / kShrinkThreads;
+        // copies per token row of a K block, and rows apart of a thread's copies: a multiple of 8, so their places differ by that many rows
+        constexpr int XC = I8 ? 4 : 8, X_ROWS = kShrinkThreads / XC, A_ROWS = kShrinkThreads / 8;
+        constexpr int NX = (TN + X_ROWS - 1) / X_ROWS, NA = 128 / A_ROWS;
         const char *x_at[NX];
-        const int xc = tid % XC, ac = tid % 8;
-        const char *a_at = a + (long long)(tid / 8) * p.k * 2 + ac * 16;
-        const int a_step = (kShrinkThreads / 8) * p.k * 2;
+        const int xc = tid % XC, xr = tid / XC, ac = tid % 8, ar = tid / 8;
+        const uint32_t x_to = I8 ? (uint32_t)((TN + p.rank_pad) * 128 + xr * 64 + xc * 16) : swizzled(xr, xc * 16);
+        const uint32_t a_to = (uint32_t)(TN * 128) + swizzled(ar, ac * 16);
+        const char *a_at = a + (long long)ar * p.k * 2 + ac * 16;
+        const long long a_step = (long long)A_ROWS * p.k * 2;
+        const int na = FAST ? (p.rank - ar + A_ROWS - 1) / A_ROWS : 0;
         if (FAST) {
 #pragma unroll
             for (int i = 0; i < NX; ++i) {
-                const int r = tid / XC + i * (kShrinkThreads / XC);
+                const int r = xr + i * X_ROWS;
                 x_at[i] = r < tile.count ? x + (long long)rows[r] * p.ld_x * XB + xc * 16 : nullptr;
             }
         }
@@ -457,16 +480,14 @@ __global__ void __launch_bounds__(kShrinkThreads) adapter_shrink_kernel(const Ad
                 const int ax = min(max(have * XB - xc * 16, 0), 16), aa = min(max(have * 2 - ac * 16, 0), 16);
                 // a copy of no bytes names the row's start: its own place may lie beyond the tensor
                 const long long xo = ax > 0 ? (long long)kb * kBlockK * XB : -(long long)xc * 16;
-                const long long ao = aa > 0 ? (long long)kb * kBlockK * 2 : -(long long)ac * 16;
+                const char *from = a_at + (aa > 0 ? (long long)kb * kBlockK * 2 : -(long long)ac * 16);
 #pragma unroll
-                for (int i = 0; i < NX; ++i) {
-                    const int r = tid / XC + i * (kShrinkThreads / XC);
-                    if (x_at[i]) cp_async<16>(I8 ? s + (TN + p.rank_pad) * 128 + r * 64 + xc * 16 : s + swizzled(r, xc * 16), x_at[i] + xo, ax);
-                }
+                for (int i = 0; i < NX; ++i)
+                    if (x_at[i]) cp_async<16>(s + x_to + i * X_ROWS * (I8 ? 64 : 128), x_at[i] + xo, ax);
 #pragma unroll
                 for (int i = 0; i < NA; ++i) {
-                    const int r = tid / 8 + i * (kShrinkThreads / 8);
-                    if (r < p.rank) cp_async<16>(s + TN * 128 + swizzled(r, ac * 16), a_at + (long long)i * a_step + ao, aa);
+                    if (i < na) cp_async<16>(s + a_to + i * A_ROWS * 128, from, aa);
+                    from += a_step;
                 }
                 return;
             }
@@ -627,8 +648,10 @@ __global__ void __launch_bounds__(kExpandThreads) adapter_expand_kernel(const Ad
                 const char *from = b + (long long)n0 * p.rank * 2;
                 const uint32_t end = (uint32_t)(channels * p.rank * 2);
 #pragma unroll
-                for (int i = 0; i < NB; ++i)
-                    if (i < nb && b_from[i] >> 8 < end) cp_async<GB ? GB : 16>(s + b_to[i], from + (b_from[i] >> 8), (int)(b_from[i] & 255u));
+                for (int i = 0; i < NB; ++i) {
+                    if (i >= nb) break;
+                    if (b_from[i] >> 8 < end) cp_async<GB ? GB : 16>(s + b_to[i], from + (b_from[i] >> 8), (int)(b_from[i] & 255u));
+                }
 #pragma unroll
                 for (int i = 0; i < NR; ++i)
                     if (base_at_row[i] >= 0 && rc < channels)
