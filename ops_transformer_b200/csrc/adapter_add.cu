@@ -26,12 +26,12 @@
 namespace gmm {
 namespace {
 
-constexpr int kBlockK = 64;          // elements of a row per K block: 128 bytes, one swizzled row
+constexpr int kBlockK = 128;         // elements of a row per K block: two swizzled rows of 128 bytes
 constexpr int kChunkN = 128;         // channels per step of the second product
 constexpr int kSelfPlan = 256;       // most tokens for which every CTA finds its tile itself
 constexpr int kPlanThreads = 1024;
-constexpr int kShrinkThreads = 128, kExpandThreads = 256;
-constexpr int kShrinkStages = 4, kExpandStages = 2;
+constexpr int kShrinkThreads = 256, kExpandThreads = 256;
+constexpr int kShrinkStages = 3, kExpandStages = 2;
 constexpr long long kWaitLimitCycles = 1ll << 31;   // about a second
 
 struct AdapterParams {
@@ -133,7 +133,7 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16])
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8])
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t *v)
 {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
@@ -218,37 +218,38 @@ __device__ __forceinline__ uint32_t pack2(float a, float b)
     return (uint32_t)*reinterpret_cast<const uint16_t *>(&lo) | (uint32_t)*reinterpret_cast<const uint16_t *>(&hi) << 16;
 }
 
-// The int8 elements that this thread copied to `raw` (rows of 64), as T in the swizzled tile: exact in both types.
+// The int8 elements that this thread copied to `raw` (rows of kBlockK), as T in the swizzled tiles, `next` bytes apart: exact in both
+// types.
 template <typename T, int GRAIN, int THREADS>
-__device__ __forceinline__ void widen_rows_grain(uint32_t raw, uint32_t dst, int rows)
+__device__ __forceinline__ void widen_rows_grain(uint32_t raw, uint32_t dst, uint32_t next, int rows)
 {
-    constexpr int PER_ROW = 64 / GRAIN;
+    constexpr int PER_ROW = kBlockK / GRAIN;
     for (int i = threadIdx.x; i < rows * PER_ROW; i += THREADS) {
         const int r = i / PER_ROW, c = (i % PER_ROW) * GRAIN;
         if (GRAIN == 1) {
             uint16_t q;
-            asm volatile("ld.shared.u8 %0, [%1];" : "=h"(q) : "r"(raw + r * 64 + c) : "memory");
+            asm volatile("ld.shared.u8 %0, [%1];" : "=h"(q) : "r"(raw + r * kBlockK + c) : "memory");
             const T f = from_float<T>((float)(int8_t)q);
-            asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + swizzled(r, 2 * c)), "h"(*reinterpret_cast<const uint16_t *>(&f)) : "memory");
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + c / 64 * next + swizzled(r, 2 * c % 128)), "h"(*reinterpret_cast<const uint16_t *>(&f)) : "memory");
         } else {
 #pragma unroll
             for (int e = 0; e < GRAIN; e += 4) {
                 int q;
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(q) : "r"(raw + r * 64 + c + e) : "memory");
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(q) : "r"(raw + r * kBlockK + c + e) : "memory");
                 const uint32_t lo = pack2<T>((float)(int8_t)q, (float)(int8_t)(q >> 8));
                 const uint32_t hi = pack2<T>((float)(int8_t)(q >> 16), (float)(q >> 24));
-                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(dst + swizzled(r, 2 * (c + e))), "r"(lo), "r"(hi) : "memory");
+                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(dst + c / 64 * next + swizzled(r, 2 * (c + e) % 128)), "r"(lo), "r"(hi) : "memory");
             }
         }
     }
 }
 template <typename T, int THREADS>
-__device__ __forceinline__ void widen_rows(int grain, uint32_t raw, uint32_t dst, int rows)
+__device__ __forceinline__ void widen_rows(int grain, uint32_t raw, uint32_t dst, uint32_t next, int rows)
 {
-    if (grain == 16) widen_rows_grain<T, 16, THREADS>(raw, dst, rows);
-    else if (grain == 8) widen_rows_grain<T, 8, THREADS>(raw, dst, rows);
-    else if (grain == 4) widen_rows_grain<T, 4, THREADS>(raw, dst, rows);
-    else widen_rows_grain<T, 1, THREADS>(raw, dst, rows);
+    if (grain == 16) widen_rows_grain<T, 16, THREADS>(raw, dst, next, rows);
+    else if (grain == 8) widen_rows_grain<T, 8, THREADS>(raw, dst, next, rows);
+    else if (grain == 4) widen_rows_grain<T, 4, THREADS>(raw, dst, next, rows);
+    else widen_rows_grain<T, 1, THREADS>(raw, dst, next, rows);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -413,11 +414,15 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(const Adapte
 
 __host__ __device__ constexpr int align_up(int v, int a) { return (v + a - 1) / a * a; }
 __host__ __device__ inline int tmem_cols(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : 128; }
-// Bytes of a stage: the tokens' rows and the weights' (and the int8 rows as they come).
-__host__ __device__ inline int shrink_stage(int tn, int rank_pad, bool i8) { return (tn + rank_pad) * 128 + (i8 ? tn * 64 : 0); }
-// The first product reads 128 rows from the start of the tokens' tile, however few there are: what lies behind it decides nothing
-// but results that are not read.  The last stage needs that much room behind it.
-inline int shrink_smem(int tn, int rank_pad, bool i8) { return 1024 + kShrinkStages * align_up(shrink_stage(tn, rank_pad, i8), 1024) + 128 * 128; }
+// Bytes of a stage: two tiles of the tokens' rows, two of the weights' (and the int8 rows as they come).
+__host__ __device__ inline int shrink_stage(int tn, int rank_pad, bool i8) { return (tn + rank_pad) * 256 + (i8 ? tn * kBlockK : 0); }
+// The first product reads 128 rows from the start of a tile of tokens, however few there are: what lies behind it decides nothing but
+// results that are not read.  The last stage's second tile may need some room behind it.
+inline int shrink_smem(int tn, int rank_pad, bool i8)
+{
+    const int stage = align_up(shrink_stage(tn, rank_pad, i8), 1024), last = tn * 128 + 128 * 128;
+    return 1024 + (kShrinkStages - 1) * stage + (stage > last ? stage : last);
+}
 
 // Grid: (tiles, ksplit).  CTA y takes the K blocks [y * blocks / ksplit, (y + 1) * blocks / ksplit).
 // FAST: rows of x and a start on 16-byte boundaries.  A thread then copies the same 16 bytes of every K block, whose addresses it works
@@ -456,13 +461,15 @@ __global__ void __launch_bounds__(kShrinkThreads) adapter_shrink_kernel(const Ad
         constexpr int XB = I8 ? 1 : 2;
         const char *x = reinterpret_cast<const char *>(p.x);
         const char *a = reinterpret_cast<const char *>(p.a) + (long long)tile.adapter * p.rank * p.k * 2;
+        const uint32_t a_tile = TN * 256, raw_tile = (uint32_t)(TN + p.rank_pad) * 256;
         // copies per token row of a K block, and rows apart of a thread's copies: a multiple of 8, so their places differ by that many rows
-        constexpr int XC = I8 ? 4 : 8, X_ROWS = kShrinkThreads / XC, A_ROWS = kShrinkThreads / 8;
+        constexpr int XC = kBlockK * XB / 16, X_ROWS = kShrinkThreads / XC, AC = kBlockK * 2 / 16, A_ROWS = kShrinkThreads / AC;
+        static_assert(X_ROWS % 8 == 0 && A_ROWS % 8 == 0, "whole groups of swizzled rows");
         constexpr int NX = (TN + X_ROWS - 1) / X_ROWS, NA = 128 / A_ROWS;
         const char *x_at[NX];
-        const int xc = tid % XC, xr = tid / XC, ac = tid % 8, ar = tid / 8;
-        const uint32_t x_to = I8 ? (uint32_t)((TN + p.rank_pad) * 128 + xr * 64 + xc * 16) : swizzled(xr, xc * 16);
-        const uint32_t a_to = (uint32_t)(TN * 128) + swizzled(ar, ac * 16);
+        const int xc = tid % XC, xr = tid / XC, ac = tid % AC, ar = tid / AC;
+        const uint32_t x_to = I8 ? raw_tile + (uint32_t)(xr * kBlockK + xc * 16) : (uint32_t)(xc / 8 * TN * 128) + swizzled(xr, xc % 8 * 16);
+        const uint32_t a_to = a_tile + (uint32_t)(ac / 8 * p.rank_pad * 128) + swizzled(ar, ac % 8 * 16);
         const char *a_at = a + (long long)ar * p.k * 2 + ac * 16;
         const long long a_step = (long long)A_ROWS * p.k * 2;
         const int na = FAST ? (p.rank - ar + A_ROWS - 1) / A_ROWS : 0;
@@ -483,7 +490,7 @@ __global__ void __launch_bounds__(kShrinkThreads) adapter_shrink_kernel(const Ad
                 const char *from = a_at + (aa > 0 ? (long long)kb * kBlockK * 2 : -(long long)ac * 16);
 #pragma unroll
                 for (int i = 0; i < NX; ++i)
-                    if (x_at[i]) cp_async<16>(s + x_to + i * X_ROWS * (I8 ? 64 : 128), x_at[i] + xo, ax);
+                    if (x_at[i]) cp_async<16>(s + x_to + i * X_ROWS * (I8 ? kBlockK : 128), x_at[i] + xo, ax);
 #pragma unroll
                 for (int i = 0; i < NA; ++i) {
                     if (i < na) cp_async<16>(s + a_to + i * A_ROWS * 128, from, aa);
@@ -491,11 +498,18 @@ __global__ void __launch_bounds__(kShrinkThreads) adapter_shrink_kernel(const Ad
                 }
                 return;
             }
-            copy_rows<true, kShrinkThreads>(p.grain_a, s + TN * 128, p.rank, 128, have * 2,
-                                            [&](int r) { return a + ((long long)r * p.k + (long long)kb * kBlockK) * 2; });
-            const auto x_row = [&](int r) { return x + ((long long)rows[r] * p.ld_x + (long long)kb * kBlockK) * XB; };
-            if (I8) copy_rows<false, kShrinkThreads>(p.grain_x, s + (TN + p.rank_pad) * 128, tile.count, 64, have, x_row);
-            else copy_rows<true, kShrinkThreads>(p.grain_x, s, tile.count, 128, have * 2, x_row);
+            for (int at = 0; at < 2; ++at) {
+                const long long k0 = (long long)kb * kBlockK + at * 64;
+                if (at * 64 >= (have + 15) / 16 * 16) break;   // no K step reaches the second tile
+                copy_rows<true, kShrinkThreads>(p.grain_a, s + a_tile + (uint32_t)(at * p.rank_pad * 128), p.rank, 128, (have - at * 64) * 2,
+                                                [&](int r) { return a + ((long long)r * p.k + k0) * 2; });
+                if (!I8)
+                    copy_rows<true, kShrinkThreads>(p.grain_x, s + (uint32_t)(at * TN * 128), tile.count, 128, (have - at * 64) * 2,
+                                                    [&](int r) { return x + ((long long)rows[r] * p.ld_x + k0) * XB; });
+            }
+            if (I8)
+                copy_rows<false, kShrinkThreads>(p.grain_x, s + raw_tile, tile.count, kBlockK, have,
+                                                 [&](int r) { return x + (long long)rows[r] * p.ld_x + (long long)kb * kBlockK; });
         };
         for (int i = 0; i < kShrinkStages - 1; ++i) {
             if (kb0 + i < kb1) load(kb0 + i);
@@ -506,15 +520,16 @@ __global__ void __launch_bounds__(kShrinkThreads) adapter_shrink_kernel(const Ad
             const int i = kb - kb0, stage = i % kShrinkStages;
             const uint32_t s = smem0 + (uint32_t)stage * stage_bytes;
             cp_wait<kShrinkStages - 2>();
-            if (I8 && FAST) widen_rows_grain<T, 16, kShrinkThreads>(s + (TN + p.rank_pad) * 128, s, tile.count);
-            else if (I8) widen_rows<T, kShrinkThreads>(p.grain_x, s + (TN + p.rank_pad) * 128, s, tile.count);
+            if (I8 && FAST) widen_rows_grain<T, 16, kShrinkThreads>(s + raw_tile, s, TN * 128, tile.count);
+            else if (I8) widen_rows<T, kShrinkThreads>(p.grain_x, s + raw_tile, s, TN * 128, tile.count);
             fence_async_proxy();
             __syncthreads();
             if (tid == 0) {
                 tc_fence_after();
-                const uint64_t xd = operand_desc(s), ad = operand_desc(s + TN * 128);
+                const uint64_t xd = operand_desc(s), ad = operand_desc(s + a_tile);
                 const int steps = (min(kBlockK, p.k - kb * kBlockK) + 15) / 16;
-                for (int j = 0; j < steps; ++j) umma_f16(tmem_base, xd + j * 2, ad + j * 2, idesc, (i | j) != 0);
+                for (int j = 0; j < steps; ++j)
+                    umma_f16(tmem_base, xd + j / 4 * (TN * 128 / 16) + j % 4 * 2, ad + j / 4 * (p.rank_pad * 128 / 16) + j % 4 * 2, idesc, (i | j) != 0);
                 umma_commit(smem_u32(&bars[stage]));
             }
             // the stage that the block before this one was read from takes the next block
@@ -749,49 +764,58 @@ __global__ void __launch_bounds__(kExpandThreads) adapter_expand_kernel(const Ad
             }
         }
         const uint32_t idesc = instr_desc<T>(TN);
-        for (int c = c0; c < c1; ++c) {
-            const int i = c - c0;
-            const uint32_t s = stage0 + (uint32_t)(i % kExpandStages) * stage_bytes;
-            cp_wait<kExpandStages - 1>();
-            fence_async_proxy();
-            __syncthreads();
-            if (tid == 0) {
-                tc_fence_after();
-                uint32_t more = 0;
-                for (int j = 0; j < p.rank_pad / 16; ++j) {
-                    const uint64_t bd = operand_desc(s + (uint32_t)(j / 4) * kChunkN * 128) + (j % 4) * 2;
-                    umma_f16(tmem_base, bd, operand_desc(v_hi + (uint32_t)(j / 4) * TN * 128) + (j % 4) * 2, idesc, more);
-                    more = 1;
-                    umma_f16(tmem_base, bd, operand_desc(v_lo + (uint32_t)(j / 4) * TN * 128) + (j % 4) * 2, idesc, more);
-                }
-                umma_commit(smem_u32(&bar));
+        const auto multiply = [&](int c) {   // by one thread
+            const uint32_t s = stage0 + (uint32_t)((c - c0) % kExpandStages) * stage_bytes;
+            tc_fence_after();
+            uint32_t more = 0;
+            for (int j = 0; j < p.rank_pad / 16; ++j) {
+                const uint64_t bd = operand_desc(s + (uint32_t)(j / 4) * kChunkN * 128) + (j % 4) * 2;
+                umma_f16(tmem_base, bd, operand_desc(v_hi + (uint32_t)(j / 4) * TN * 128) + (j % 4) * 2, idesc, more);
+                more = 1;
+                umma_f16(tmem_base, bd, operand_desc(v_lo + (uint32_t)(j / 4) * TN * 128) + (j % 4) * 2, idesc, more);
             }
+            umma_commit(smem_u32(&bar));
+        };
+        cp_wait<kExpandStages - 1>();
+        fence_async_proxy();
+        __syncthreads();
+        if (tid == 0) multiply(c0);
+        // warp w: channels 32 (w % 4) + lane, half of the tokens
+        constexpr int HALF = TN / 2;
+        const int q = warp & 3, ch = q * 32 + lane, first = (warp >> 2) * HALF;
+        for (int c = c0; c < c1; ++c) {
+            const int i = c - c0, n = c * kChunkN + ch;
+            const uint32_t s = stage0 + (uint32_t)(i % kExpandStages) * stage_bytes;
             mbar_wait(smem_u32(&bar), i & 1, &gave_up, p.status, 910);
             tc_fence_after();
-            // warp w: channels 32 (w % 4) + lane, half of the tokens
-            const int q = warp & 3, ch = q * 32 + lane, n = c * kChunkN + ch;
-            constexpr int HALF = TN / 2;
-            const int first = (warp >> 2) * HALF;
-            for (int t0 = first; t0 < min(first + HALF, tile.count); t0 += 8) {
-                uint32_t d[8];
-                tmem_ld8(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)t0, d);
-                const uint32_t at = s + base_at + (uint32_t)(t0 * kChunkN * 2 + ch * 2);
-                uint16_t raw[8];
+            uint32_t d[HALF];
+            if (first < tile.count) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) asm volatile("ld.shared.u16 %0, [%1];" : "=h"(raw[e]) : "r"(at + e * kChunkN * 2) : "memory");
+                for (int t0 = 0; t0 < HALF; t0 += 8) tmem_ld8(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(first + t0), d + t0);
                 tmem_ld_wait();
+                const uint32_t at = s + base_at + (uint32_t)(first * kChunkN * 2 + ch * 2);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int slot = t0 + e;   // beyond the tile's tokens: values of no meaning that are not stored
-                    float f = __uint_as_float(d[e]);
-                    if (F16) f = __fmul_rn(f, unscale[slot]);
-                    const T o = from_float<T>(__fadd_rn(to_float(*reinterpret_cast<const T *>(&raw[e])), f));
-                    if (GB) asm volatile("st.shared.u16 [%0], %1;" ::"r"(at + e * kChunkN * 2), "h"(*reinterpret_cast<const uint16_t *>(&o)) : "memory");
-                    else if (slot < tile.count && n < p.n) out[(long long)rows[slot] * p.ld_out + n] = o;
+                for (int t0 = 0; t0 < HALF; t0 += 8) {
+                    if (first + t0 >= tile.count) break;
+                    uint16_t raw[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) asm volatile("ld.shared.u16 %0, [%1];" : "=h"(raw[e]) : "r"(at + (t0 + e) * kChunkN * 2) : "memory");
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int slot = first + t0 + e;   // beyond the tile's tokens: values of no meaning that are not stored
+                        float f = __uint_as_float(d[t0 + e]);
+                        if (F16) f = __fmul_rn(f, unscale[slot]);
+                        const T o = from_float<T>(__fadd_rn(to_float(*reinterpret_cast<const T *>(&raw[e])), f));
+                        if (GB) asm volatile("st.shared.u16 [%0], %1;" ::"r"(at + (t0 + e) * kChunkN * 2), "h"(*reinterpret_cast<const uint16_t *>(&o)) : "memory");
+                        else if (slot < tile.count && n < p.n) out[(long long)rows[slot] * p.ld_out + n] = o;
+                    }
                 }
             }
             tc_fence_before();
-            __syncthreads();
+            cp_wait<0>();           // the next chunk, for which a whole round was time
+            fence_async_proxy();
+            __syncthreads();        // this chunk's results are in place, its accumulators read, the next chunk there
+            if (tid == 0 && c + 1 < c1) multiply(c + 1);
             if (GB) {   // a thread stores the 16 bytes whose place it then fills again
 #pragma unroll
                 for (int i = 0; i < NR; ++i) {
@@ -818,7 +842,7 @@ __global__ void __launch_bounds__(kExpandThreads) adapter_expand_kernel(const Ad
 template <typename... KArgs>
 cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, int threads, int smem, cudaStream_t stream, bool dependent, KArgs... args)
 {
-    if (smem > 48 * 1024) {
+    if (smem > 44 * 1024) {   // with what the kernel has of its own it may pass 48 KB
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return e;
     }
