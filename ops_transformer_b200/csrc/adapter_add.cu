@@ -26,12 +26,14 @@
 namespace gmm {
 namespace {
 
-constexpr int kBlockK = 128;         // elements of a row per K block: two swizzled rows of 128 bytes
+constexpr int kBlockK = 128;         // elements of a row per K block
+constexpr int kBlockTiles = kBlockK / 64;   // swizzled rows of 128 bytes that these make
 constexpr int kChunkN = 128;         // channels per step of the second product
 constexpr int kSelfPlan = 256;       // most tokens for which every CTA finds its tile itself
 constexpr int kPlanThreads = 1024;
-constexpr int kShrinkThreads = 256, kExpandThreads = 256;
-constexpr int kShrinkStages = 3, kExpandStages = 2;
+constexpr int kWorkers = 256;        // threads of the first kernel that copy; one warp more issues the products
+__host__ __device__ constexpr int expand_workers(int tn) { return tn == 64 ? 512 : 256; }
+constexpr int kMaxStages = 6, kShrinkAhead = 2, kExpandStages = 2;
 constexpr long long kWaitLimitCycles = 1ll << 31;   // about a second
 
 struct AdapterParams {
@@ -43,12 +45,13 @@ struct AdapterParams {
     int rows, k, n, adapters, rank;
     int rank_pad;                   // rank, rounded up to the tensor cores' K step of 16
     int grain_x, grain_a, grain_b, grain_base, grain_out;   // bytes of a copy
-    int ksplit, nsplit;
+    int ksplit, nsplit, stages;
+    int parts;                      // tiles of the second kernel in one of the first
     int *status;                    // [4]
     int *n_tiles;
-    int4 *tiles;                    // adapter (-1: none), first entry in `order`, tokens
-    int *order;                     // [rows] tokens grouped by adapter
-    float *v;                       // [ksplit, rows, rank_pad]
+    int2 *tiles;                    // adapter (-1: none), tokens
+    int *order;                     // [tiles, tile_tokens] the tokens of every tile
+    float *v;                       // [ksplit, rows, rank_pad] partial sums
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -74,7 +77,12 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity)
         : "memory");
     return ok != 0;
 }
-// Bounded wait for the tensor cores.  When it runs out the status says so and later waits of the CTA return at once.
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// An arrival at `bar` once this thread's copies so far have landed.
+__device__ __forceinline__ void mbar_arrive_copies(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
+template <int THREADS>
+__device__ __forceinline__ void worker_sync() { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); }
+// Bounded wait for the tensor cores, or for the copies that they wait for.  When it runs out the status says so and later waits of the CTA return at once.
 __device__ __noinline__ void mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int *gave_up, int *status, int role)
 {
     const long long t0 = clock64();
@@ -122,16 +130,6 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint6
 __device__ __forceinline__ void umma_commit(uint32_t bar)
 {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16])
-{
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-        : "r"(taddr)
-        : "memory");
 }
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t *v)
 {
@@ -266,77 +264,57 @@ __device__ __forceinline__ int adapter_of(const AdapterParams &p, int t)
     return i >= 0 && i < p.adapters ? i : -1;
 }
 
-// Tile number blockIdx.x of at most TN tokens each, found by every CTA for itself; rows[slot] = token.  A token whose rank among the
-// tokens of its adapter is a multiple of TN begins a tile, and tiles are numbered by their first tokens.
+// The tile of at most TN tokens that begins with token blockIdx.x, found by every CTA for itself; rows[slot] = token.  A token begins one if
+// a multiple of TN tokens of its adapter come before it; the CTAs of the others have nothing to do.
 struct SelfPlan {
-    int ids[kSelfPlan];
-    int leaders[kSelfPlan / 32];
-    int adapter, from, count;
+    unsigned same[kSelfPlan / 32];   // the tokens of the first token's adapter
 };
-template <int TN, int THREADS>
+template <int TN>
 __device__ __forceinline__ Tile self_plan(const AdapterParams &p, SelfPlan &s, int *rows)
 {
-    constexpr int PER = kSelfPlan / THREADS;
-    const int tid = threadIdx.x;
-    for (int t = tid; t < kSelfPlan; t += THREADS) s.ids[t] = t < p.rows ? adapter_of(p, t) : -2;
-    if (tid == 0) { s.count = 0; s.from = -1; s.adapter = -1; }
-    __syncthreads();
-    int rank[PER];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const int t = j * THREADS + tid, id = s.ids[t];
-        int r = 0;
-        for (int o = 0; j * THREADS < p.rows && o < p.rows; o += 4) {
-            const int4 q = *reinterpret_cast<const int4 *>(&s.ids[o]);
-            r += (q.x == id && o < t) + (q.y == id && o + 1 < t) + (q.z == id && o + 2 < t) + (q.w == id && o + 3 < t);
-        }
-        rank[j] = r;
-        const unsigned b = __ballot_sync(0xffffffffu, id != -2 && r % TN == 0);
-        if ((tid & 31) == 0) s.leaders[t >> 5] = (int)b;
+    const int tid = threadIdx.x, x = blockIdx.x, id = adapter_of(p, x);
+    bool same = false;
+    if (tid < kSelfPlan) {
+        same = tid < p.rows && adapter_of(p, tid) == id;
+        const unsigned b = __ballot_sync(0xffffffffu, same);
+        if ((tid & 31) == 0) s.same[tid >> 5] = b;
     }
     __syncthreads();
+    int before = 0, all = 0, mine = 0;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const int t = j * THREADS + tid;
-        int before = 0;
-        for (int w = 0; w < (t >> 5); ++w) before += __popc(s.leaders[w]);
-        const unsigned mine = (unsigned)s.leaders[t >> 5];
-        before += __popc(mine & ((1u << (t & 31)) - 1u));
-        if ((mine >> (t & 31) & 1u) && before == (int)blockIdx.x) { s.adapter = s.ids[t]; s.from = rank[j]; }
+    for (int w = 0; w < kSelfPlan / 32; ++w) {
+        const unsigned b = s.same[w];
+        const auto below = [&](int t) { return __popc(t >= w * 32 + 32 ? b : t <= w * 32 ? 0u : b & ((1u << (t - w * 32)) - 1u)); };
+        all += __popc(b);
+        before += below(x);
+        mine += below(tid);
     }
+    if (before % TN != 0) return Tile{-1, 0};
+    if (same && mine >= before && mine < before + TN) rows[mine - before] = tid;
     __syncthreads();
-    if (s.from < 0) return Tile{-1, 0};
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const int t = j * THREADS + tid;
-        if (s.ids[t] == s.adapter && rank[j] >= s.from && rank[j] < s.from + TN) {
-            rows[rank[j] - s.from] = t;
-            atomicAdd(&s.count, 1);
-        }
-    }
-    __syncthreads();
-    return Tile{s.adapter, s.count};
+    return Tile{id, min(TN, all - before)};
 }
 
-// The same from the plan in the workspace.
-__device__ __forceinline__ Tile read_plan(const AdapterParams &p, int threads, int *rows)
+// The same from the plan in the workspace, whose tiles hold `parts` of them.
+template <int TN>
+__device__ __forceinline__ Tile read_plan(const AdapterParams &p, int parts, int threads, int *rows)
 {
-    if ((int)blockIdx.x >= __ldcg(p.n_tiles)) return Tile{-1, 0};
-    const int4 t = __ldcg(p.tiles + blockIdx.x);
-    for (int i = threadIdx.x; i < t.z; i += threads) rows[i] = __ldcg(p.order + t.y + i);
+    const int tiles = __ldcg(p.n_tiles), at = (int)blockIdx.x / parts, part = (int)blockIdx.x % parts;
+    const int2 t = __ldcg(p.tiles + at);   // with the rows, whose places do not hang on it, in one go
+    for (int i = threadIdx.x; i < TN; i += threads) rows[i] = __ldcg(p.order + (long long)blockIdx.x * TN + i);
     __syncthreads();
-    return Tile{t.x, t.z};
+    return at < tiles ? Tile{t.x, max(0, min(TN, t.y - part * TN))} : Tile{-1, 0};
 }
 
 // One CTA: counts the tokens of every adapter (the last counter: none), lays the tiles out and sorts the tokens.
 __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(const AdapterParams p, int tile_tokens)
 {
-    extern __shared__ int counts[];          // [adapters + 1] tokens, then the next place in `order`
-    __shared__ int2 carry, warp_sum[32];
+    extern __shared__ int counts[];          // [adapters + 1] tokens, then the next place in `order`, whose tiles are not packed
+    __shared__ int carry, warp_sum[32];
     const int tid = threadIdx.x, lane = tid & 31, n = p.adapters + 1;
     pdl_release();
     for (int i = tid; i < n; i += kPlanThreads) counts[i] = 0;
-    if (tid == 0) carry = make_int2(0, 0);
+    if (tid == 0) carry = 0;
     if (tid < 4) p.status[tid] = 0;
     __syncthreads();
     // the first tokens' adapters stay in registers between the two passes; all loads of a batch are under way together
@@ -359,39 +337,37 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(const Adapte
         }
     }
     __syncthreads();
-    // running totals of tokens and tiles over the adapters
+    // running totals of the tiles over the adapters
     for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
         const int i = i0 + tid, c = i < n ? counts[i] : 0, tiles = (c + tile_tokens - 1) / tile_tokens;
-        int2 s = make_int2(c, tiles);
+        int s = tiles;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int a = __shfl_up_sync(0xffffffffu, s.x, o), b = __shfl_up_sync(0xffffffffu, s.y, o);
-            if (lane >= o) { s.x += a; s.y += b; }
+            const int t = __shfl_up_sync(0xffffffffu, s, o);
+            if (lane >= o) s += t;
         }
         if (lane == 31) warp_sum[tid >> 5] = s;
         __syncthreads();
         if (tid < 32) {
-            int2 w = warp_sum[tid];
+            int w = warp_sum[tid];
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int a = __shfl_up_sync(0xffffffffu, w.x, o), b = __shfl_up_sync(0xffffffffu, w.y, o);
-                if (lane >= o) { w.x += a; w.y += b; }
+                const int t = __shfl_up_sync(0xffffffffu, w, o);
+                if (lane >= o) w += t;
             }
             warp_sum[tid] = w;
         }
         __syncthreads();
-        const int2 before = tid >= 32 ? warp_sum[(tid >> 5) - 1] : make_int2(0, 0);
-        const int start = carry.x + before.x + s.x - c, first = carry.y + before.y + s.y - tiles;
+        const int first = carry + (tid >= 32 ? warp_sum[(tid >> 5) - 1] : 0) + s - tiles;
         if (i < n) {
-            counts[i] = start;
-            for (int q = 0; q < tiles; ++q)
-                p.tiles[first + q] = make_int4(i < p.adapters ? i : -1, start + q * tile_tokens, min(tile_tokens, c - q * tile_tokens), 0);
+            counts[i] = first * tile_tokens;
+            for (int q = 0; q < tiles; ++q) p.tiles[first + q] = make_int2(i < p.adapters ? i : -1, min(tile_tokens, c - q * tile_tokens));
         }
         __syncthreads();
-        if (tid == kPlanThreads - 1) carry = make_int2(carry.x + warp_sum[31].x, carry.y + warp_sum[31].y);
+        if (tid == kPlanThreads - 1) carry += warp_sum[31];
         __syncthreads();
     }
-    if (tid == 0) *p.n_tiles = carry.y;
+    if (tid == 0) *p.n_tiles = carry;
     for (int t0 = 0; t0 < p.rows; t0 += KEEP * kPlanThreads) {
         if (p.rows > KEEP * kPlanThreads) fetch(t0);
 #pragma unroll
@@ -408,39 +384,299 @@ __global__ void __launch_bounds__(kPlanThreads) adapter_plan_kernel(const Adapte
     }
 }
 
+// Channels [n0, n1) of rows without an adapter, V elements a copy.
+template <typename T, int V, int THREADS>
+__device__ __forceinline__ void copy_base(const AdapterParams &p, const int *rows, int count, int n0, int n1)
+{
+    using Copy = typename std::conditional<V == 8, uint4, uint16_t>::type;
+    static_assert(V == 8 || V == 1, "");
+    constexpr int AHEAD = 4;   // copies in flight
+    const T *base = reinterpret_cast<const T *>(p.base);
+    T *out = reinterpret_cast<T *>(p.out);
+    const int across = (n1 - n0 + V - 1) / V, total = across * count;   // at most 64 rows of 65535
+    for (int i0 = threadIdx.x; i0 < total; i0 += THREADS * AHEAD) {
+        Copy v[AHEAD];
+        T *to[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int i = i0 + j * THREADS, r = i / across, c = n0 + (i - r * across) * V;
+            to[j] = nullptr;
+            if (i < total) {
+                v[j] = *reinterpret_cast<const Copy *>(base + (long long)rows[r] * p.ld_base + c);
+                to[j] = out + (long long)rows[r] * p.ld_out + c;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+            if (to[j]) *reinterpret_cast<Copy *>(to[j]) = v[j];
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// A few tokens per adapter: streams of weights, on the CUDA cores
+// ---------------------------------------------------------------------------------------------------------
+//
+// With up to four tokens a tile each weight takes part in four products at most, which costs fewer instructions than bringing it to the
+// tensor cores; the weights go straight from memory to registers, 16 bytes a lane.  128 tokens of 64 tenants, 2048 -> 7168, rank 32:
+// FEW_US us against 28 on the tensor cores.
+
+constexpr int kFew = 4;
+constexpr int kFewThreads = 256;
+constexpr int kFewExpandCtas = 2;   // that fit an SM by their registers
+
+template <typename T> __device__ __forceinline__ void unpack8(const uint4 &u, f32x2 (&f)[4]);
+template <> __device__ __forceinline__ void unpack8<__nv_bfloat16>(const uint4 &u, f32x2 (&f)[4])
+{
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = pair2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
+template <> __device__ __forceinline__ void unpack8<__half>(const uint4 &u, f32x2 (&f)[4])
+{
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 t = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        f[i] = pair2(t.x, t.y);
+    }
+}
+// Eight int8: a byte plus 128 in the low bits of 2^23 is the float 2^23 + 128 + q.
+__device__ __forceinline__ void unpack8(const uint2 &u, f32x2 (&f)[4])
+{
+    const uint32_t w[2] = {u.x ^ 0x80808080u, u.y ^ 0x80808080u};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float a = __uint_as_float(__byte_perm(w[i / 2], 0x4b000000u, i % 2 ? 0x7652 : 0x7650));
+        const float b = __uint_as_float(__byte_perm(w[i / 2], 0x4b000000u, i % 2 ? 0x7653 : 0x7651));
+        f[i] = pair2(__fsub_rn(a, 8388736.0f), __fsub_rn(b, 8388736.0f));
+    }
+}
+
+// fn(integral constant) for a tile of 1 to kFew tokens: with the count known to the compiler nothing stands between the loads, and all of
+// a step are under way together.
+template <typename Fn>
+__device__ __forceinline__ void for_count(int count, Fn fn)
+{
+    static_assert(kFew == 4, "");
+    if (count == 1) fn(std::integral_constant<int, 1>());
+    else if (count == 2) fn(std::integral_constant<int, 2>());
+    else if (count == 3) fn(std::integral_constant<int, 3>());
+    else fn(std::integral_constant<int, 4>());
+}
+
+// Grid: (tiles, ceil(rank / 8)); a warp takes one component of v, its lanes 8 elements of K each in turn.
+template <typename T, bool I8>
+__global__ void __launch_bounds__(kFewThreads) adapter_few_shrink_kernel(const AdapterParams p)
+{
+    __shared__ alignas(16) SelfPlan plan;
+    __shared__ int rows[kFew];
+    const int tid = threadIdx.x, lane = tid & 31, j = (int)blockIdx.y * (kFewThreads / 32) + (tid >> 5);
+    pdl_release();
+    if (tid < 4 && blockIdx.x == 0 && blockIdx.y == 0) p.status[tid] = 0;
+    const Tile tile = self_plan<kFew>(p, plan, rows);
+    if (tile.count == 0 || tile.adapter < 0 || j >= p.rank) return;
+    const uint4 *a = reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(p.a) + ((long long)tile.adapter * p.rank + j) * p.k);
+    for_count(tile.count, [&](auto tokens) {
+        constexpr int C = decltype(tokens)::value, AHEAD = 4;
+        using Pack = typename std::conditional<I8, uint2, uint4>::type;
+        const Pack *x[C];
+        f32x2 sum[C];
+#pragma unroll
+        for (int t = 0; t < C; ++t) {
+            x[t] = reinterpret_cast<const Pack *>(reinterpret_cast<const char *>(p.x) + (long long)rows[t] * p.ld_x * (I8 ? 1 : 2));
+            sum[t] = 0;
+        }
+        const int packs = p.k / 8;
+        for (int c0 = lane; c0 < packs; c0 += 32 * AHEAD) {
+            uint4 w[AHEAD];
+            Pack xs[AHEAD][C];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {   // beyond the end: zeros
+                const bool there = c0 + u * 32 < packs;
+                w[u] = there ? __ldg(a + c0 + u * 32) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < C; ++t) xs[u][t] = there ? __ldg(x[t] + c0 + u * 32) : Pack{};
+            }
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                if (c0 + u * 32 >= packs) break;
+                f32x2 f[4], g[4];
+                unpack8<T>(w[u], f);
+#pragma unroll
+                for (int t = 0; t < C; ++t) {
+                    if constexpr (I8) unpack8(xs[u][t], g);
+                    else unpack8<T>(xs[u][t], g);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[t] = fma2(f[e], g[e], sum[t]);
+                }
+            }
+        }
+        float v[C];
+#pragma unroll
+        for (int t = 0; t < C; ++t) {
+            const float2 both = unpair2(sum[t]);
+            v[t] = both.x + both.y;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+            for (int t = 0; t < C; ++t) v[t] += __shfl_xor_sync(0xffffffffu, v[t], o);
+        float mine = v[0];
+#pragma unroll
+        for (int t = 1; t < C; ++t) mine = lane == t ? v[t] : mine;
+        if (lane < C) {
+            const float by = p.scaling ? __ldg(p.scaling + tile.adapter) : 1.0f;
+            p.v[(long long)rows[lane] * p.rank_pad + j] = __fmul_rn(mine, I8 ? __fmul_rn(by, __ldg(p.x_scale + rows[lane])) : by);
+        }
+    });
+}
+
+// Grid: (tiles, nsplit), channels in units of kFewChannels.  LANES neighbouring lanes (the power of two that holds rank / 8) share a
+// channel's row of b, 8 components each, and add their sums up; of the tokens' results each then stores its share.
+constexpr int kFewChannels = 256;
+template <typename T, int LANES>
+__global__ void __launch_bounds__(kFewThreads) adapter_few_expand_kernel(const AdapterParams p)
+{
+    __shared__ alignas(16) SelfPlan plan;
+    __shared__ int rows[kFew];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const Tile tile = self_plan<kFew>(p, plan, rows);
+    const int units = (p.n + kFewChannels - 1) / kFewChannels;
+    const int n0 = (int)((long long)blockIdx.y * units / p.nsplit) * kFewChannels;
+    const int n1 = min((int)((long long)(blockIdx.y + 1) * units / p.nsplit) * kFewChannels, p.n);
+    if (tile.count == 0 || tile.adapter < 0) {
+        if (tile.count > 0 && p.out != p.base) {
+            if (p.grain_base == 16 && p.grain_out == 16 && p.n % 8 == 0) copy_base<T, 8, kFewThreads>(p, rows, tile.count, n0, n1);
+            else copy_base<T, 1, kFewThreads>(p, rows, tile.count, n0, n1);
+        }
+        if (tile.count > 0) pdl_wait();   // as every CTA with a tile: the grid must not end before the one in front of it
+        return;
+    }
+    constexpr int AHEAD = 4, ACROSS = 32 / LANES, STRIDE = kFewThreads / 32 * ACROSS;   // channels of a warp's step, of the CTA's
+    const int part = lane % LANES;
+    const bool mine = part * 8 < p.rank;
+    const T *b = reinterpret_cast<const T *>(p.b) + (long long)tile.adapter * p.n * p.rank + part * 8;
+    const T *base = reinterpret_cast<const T *>(p.base);
+    T *out = reinterpret_cast<T *>(p.out);
+    int c = n0 + warp * ACROSS + lane / LANES;
+    uint4 w[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+        w[u] = mine && c + u * STRIDE < n1 ? __ldg(reinterpret_cast<const uint4 *>(b + (long long)(c + u * STRIDE) * p.rank)) : make_uint4(0, 0, 0, 0);
+    pdl_wait();   // v is complete
+    for_count(tile.count, [&](auto tokens) {
+        constexpr int C = decltype(tokens)::value, OWN = (C + LANES - 1) / LANES;   // tokens that a lane stores: part, part + LANES, ...
+        f32x2 v[C][4];
+#pragma unroll
+        for (int t = 0; t < C; ++t) {
+            const float4 *from = reinterpret_cast<const float4 *>(p.v + (long long)rows[t] * p.rank_pad + part * 8);
+            const float4 q = mine ? __ldcg(from) : make_float4(0, 0, 0, 0), r = mine ? __ldcg(from + 1) : make_float4(0, 0, 0, 0);
+            v[t][0] = pair2(q.x, q.y); v[t][1] = pair2(q.z, q.w); v[t][2] = pair2(r.x, r.y); v[t][3] = pair2(r.z, r.w);
+        }
+        long long base_row[OWN], out_row[OWN];
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) {
+            const int t = part + i * LANES;
+            base_row[i] = t < C ? (long long)rows[t] * p.ld_base : -1;
+            out_row[i] = t < C ? (long long)rows[t] * p.ld_out : -1;
+        }
+        T add[AHEAD][OWN];   // base, fetched a step ahead like b
+        const auto fetch_base = [&](int c) {
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                for (int i = 0; i < OWN; ++i)
+                    if (base_row[i] >= 0 && c + u * STRIDE < n1) add[u][i] = base[base_row[i] + c + u * STRIDE];
+        };
+        fetch_base(c);
+        for (; c - lane / LANES < n1; c += AHEAD * STRIDE) {   // the same for all lanes of a warp
+            float to_add[AHEAD][OWN], sum[AHEAD][C];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                for (int i = 0; i < OWN; ++i) to_add[u][i] = to_float(add[u][i]);
+            fetch_base(c + AHEAD * STRIDE);
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int next = c + (u + AHEAD) * STRIDE;
+                f32x2 f[4];
+                unpack8<T>(w[u], f);
+                if (mine && next < n1) w[u] = __ldg(reinterpret_cast<const uint4 *>(b + (long long)next * p.rank));
+#pragma unroll
+                for (int t = 0; t < C; ++t) {
+                    f32x2 s2 = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s2 = fma2(f[e], v[t][e], s2);
+                    const float2 both = unpair2(s2);
+                    sum[u][t] = both.x + both.y;
+                }
+            }
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1)
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                    for (int t = 0; t < C; ++t) sum[u][t] += __shfl_xor_sync(0xffffffffu, sum[u][t], o);
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+#pragma unroll
+                for (int i = 0; i < OWN; ++i) {
+                    float s = sum[u][i * LANES];
+#pragma unroll
+                    for (int t = i * LANES + 1; t < C && t < (i + 1) * LANES; ++t) s = part == t - i * LANES ? sum[u][t] : s;
+                    if (out_row[i] >= 0 && c + u * STRIDE < n1) out[out_row[i] + c + u * STRIDE] = from_float<T>(__fadd_rn(to_add[u][i], s));
+                }
+            }
+        }
+    });
+}
+
 // ---------------------------------------------------------------------------------------------------------
 // v = scaling * x a^T
 // ---------------------------------------------------------------------------------------------------------
 
 __host__ __device__ constexpr int align_up(int v, int a) { return (v + a - 1) / a * a; }
 __host__ __device__ inline int tmem_cols(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : 128; }
-// Bytes of a stage: two tiles of the tokens' rows, two of the weights' (and the int8 rows as they come).
-__host__ __device__ inline int shrink_stage(int tn, int rank_pad, bool i8) { return (tn + rank_pad) * 256 + (i8 ? tn * kBlockK : 0); }
+// Bytes of a stage: the tokens' rows, the weights' (and the int8 rows as they come).
+__host__ __device__ inline int shrink_stage(int tn, int rank_pad, bool i8) { return (tn + rank_pad) * kBlockK * 2 + (i8 ? tn * kBlockK : 0); }
+// As many stages as fit a CTA of the large tiles alone on an SM, or one of two.
+inline int shrink_stages(int tn, int rank_pad, bool i8)
+{
+    const int n = (tn > 64 ? 216 : 108) * 1024 / align_up(shrink_stage(tn, rank_pad, i8), 1024);
+    return n < 3 ? 3 : n > kMaxStages ? kMaxStages : n;   // one that is read and kShrinkAhead under way
+}
 // The first product reads 128 rows from the start of a tile of tokens, however few there are: what lies behind it decides nothing but
-// results that are not read.  The last stage's second tile may need some room behind it.
+// results that are not read.  The last stage's last tile may need some room behind it.
 inline int shrink_smem(int tn, int rank_pad, bool i8)
 {
-    const int stage = align_up(shrink_stage(tn, rank_pad, i8), 1024), last = tn * 128 + 128 * 128;
-    return 1024 + (kShrinkStages - 1) * stage + (stage > last ? stage : last);
+    const int stage = align_up(shrink_stage(tn, rank_pad, i8), 1024), last = (kBlockTiles - 1) * tn * 128 + 128 * 128;
+    return 1024 + (shrink_stages(tn, rank_pad, i8) - 1) * stage + (stage > last ? stage : last);
 }
 
 // Grid: (tiles, ksplit).  CTA y takes the K blocks [y * blocks / ksplit, (y + 1) * blocks / ksplit).
 // FAST: rows of x and a start on 16-byte boundaries.  A thread then copies the same 16 bytes of every K block, whose addresses it works
 // out once; with the addresses of every copy worked out anew the kernel was bound by its instructions.
+// The products are issued by a warp of their own, which also orders them behind the copies (fence.proxy.async).  What bounds the kernel
+// is that thread: a product of 128 x 64 x 16 costs it 0.05 us, a block's barriers and fence 0.27; so blocks are 128 deep.
 template <typename T, bool I8, int TN, bool SELF, bool FAST>
-__global__ void __launch_bounds__(kShrinkThreads) adapter_shrink_kernel(const AdapterParams p)
+__global__ void __launch_bounds__(kWorkers + 32) adapter_shrink_kernel(const AdapterParams p)
 {
     extern __shared__ uint8_t smem_raw[];
     __shared__ alignas(16) SelfPlan plan;
-    __shared__ alignas(8) uint64_t bars[kShrinkStages];
+    __shared__ alignas(8) uint64_t full[kMaxStages], empty[kMaxStages], done;
     __shared__ uint32_t tmem_base;
     __shared__ int gave_up;
     __shared__ int rows[TN];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const bool issuer = tid >= kWorkers;
     const uint32_t cols = tmem_cols(p.rank_pad);
-    if (warp == 0) tmem_alloc(&tmem_base, cols);
+    if (issuer) tmem_alloc(&tmem_base, cols);
     if (tid == 0) {
-        for (int i = 0; i < kShrinkStages; ++i) mbar_init(smem_u32(&bars[i]), 1);
+        for (int i = 0; i < kMaxStages; ++i) {
+            mbar_init(smem_u32(&full[i]), kWorkers / 32);
+            mbar_init(smem_u32(&empty[i]), 1);
+        }
+        mbar_init(smem_u32(&done), 1);
         gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         if (SELF && blockIdx.x == 0 && blockIdx.y == 0)   // long before a wait can run out and record it
@@ -452,18 +688,46 @@ __global__ void __launch_bounds__(kShrinkThreads) adapter_shrink_kernel(const Ad
     __syncthreads();
     pdl_release();
     tc_fence_after();
-    const Tile tile = SELF ? self_plan<TN, kShrinkThreads>(p, plan, rows) : read_plan(p, kShrinkThreads, rows);
+    const Tile tile = SELF ? self_plan<TN>(p, plan, rows) : read_plan<TN>(p, 1, kWorkers + 32, rows);
     const int blocks = (p.k + kBlockK - 1) / kBlockK;
     const int kb0 = (int)((long long)blockIdx.y * blocks / p.ksplit), kb1 = (int)((long long)(blockIdx.y + 1) * blocks / p.ksplit);
-    if (tile.count > 0 && tile.adapter >= 0 && kb0 < kb1) {
-        const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
-        const uint32_t stage_bytes = align_up(shrink_stage(TN, p.rank_pad, I8), 1024);
+    const bool work = tile.count > 0 && tile.adapter >= 0;   // kb0 < kb1, since ksplit is at most blocks
+    const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t stage_bytes = align_up(shrink_stage(TN, p.rank_pad, I8), 1024), a_tile = TN * kBlockK * 2;
+    if (work && issuer) {
+        const uint32_t idesc = instr_desc<T>(p.rank_pad);
+        int stage = 0;
+        uint32_t phase = 0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            const uint32_t s = smem0 + (uint32_t)stage * stage_bytes;
+            mbar_wait(smem_u32(&full[stage]), phase, &gave_up, p.status, 900);
+            fence_async_proxy();
+            tc_fence_after();
+            if (lane == 0) {
+                const uint64_t xd = operand_desc(s), ad = operand_desc(s + a_tile);
+                const uint32_t x_next = TN * 128 / 16, a_next = (uint32_t)p.rank_pad * 128 / 16;
+                if (p.k - kb * kBlockK >= kBlockK) {
+#pragma unroll
+                    for (int j = 0; j < kBlockK / 16; ++j)
+                        umma_f16(tmem_base, xd + (j / 4 * x_next + j % 4 * 2), ad + (j / 4 * a_next + j % 4 * 2), idesc, j > 0 || kb > kb0);
+                } else {
+                    const int steps = (p.k - kb * kBlockK + 15) / 16;
+                    for (int j = 0; j < steps; ++j)
+                        umma_f16(tmem_base, xd + (j / 4 * x_next + j % 4 * 2), ad + (j / 4 * a_next + j % 4 * 2), idesc, j > 0 || kb > kb0);
+                }
+                umma_commit(smem_u32(&empty[stage]));
+                if (kb == kb1 - 1) umma_commit(smem_u32(&done));
+            }
+            __syncwarp();
+            if (++stage == p.stages) { stage = 0; phase ^= 1; }
+        }
+    } else if (work) {
         constexpr int XB = I8 ? 1 : 2;
         const char *x = reinterpret_cast<const char *>(p.x);
         const char *a = reinterpret_cast<const char *>(p.a) + (long long)tile.adapter * p.rank * p.k * 2;
-        const uint32_t a_tile = TN * 256, raw_tile = (uint32_t)(TN + p.rank_pad) * 256;
+        const uint32_t raw_tile = (uint32_t)(TN + p.rank_pad) * kBlockK * 2;
         // copies per token row of a K block, and rows apart of a thread's copies: a multiple of 8, so their places differ by that many rows
-        constexpr int XC = kBlockK * XB / 16, X_ROWS = kShrinkThreads / XC, AC = kBlockK * 2 / 16, A_ROWS = kShrinkThreads / AC;
+        constexpr int XC = kBlockK * XB / 16, X_ROWS = kWorkers / XC, AC = kBlockK * 2 / 16, A_ROWS = kWorkers / AC;
         static_assert(X_ROWS % 8 == 0 && A_ROWS % 8 == 0, "whole groups of swizzled rows");
         constexpr int NX = (TN + X_ROWS - 1) / X_ROWS, NA = 128 / A_ROWS;
         const char *x_at[NX];
@@ -480,10 +744,10 @@ __global__ void __launch_bounds__(kShrinkThreads) adapter_shrink_kernel(const Ad
                 x_at[i] = r < tile.count ? x + (long long)rows[r] * p.ld_x * XB + xc * 16 : nullptr;
             }
         }
-        const auto load = [&](int kb) {
-            const uint32_t s = smem0 + (uint32_t)((kb - kb0) % kShrinkStages) * stage_bytes;
+        const auto load = [&](int kb, int stage) {
+            const uint32_t s = smem0 + (uint32_t)stage * stage_bytes;
             const int have = min(kBlockK, p.k - kb * kBlockK);
-            if (FAST) {
+            if constexpr (FAST) {
                 const int ax = min(max(have * XB - xc * 16, 0), 16), aa = min(max(have * 2 - ac * 16, 0), 16);
                 // a copy of no bytes names the row's start: its own place may lie beyond the tensor
                 const long long xo = ax > 0 ? (long long)kb * kBlockK * XB : -(long long)xc * 16;
@@ -496,66 +760,64 @@ __global__ void __launch_bounds__(kShrinkThreads) adapter_shrink_kernel(const Ad
                     if (i < na) cp_async<16>(s + a_to + i * A_ROWS * 128, from, aa);
                     from += a_step;
                 }
-                return;
-            }
-            for (int at = 0; at < 2; ++at) {
+            } else {
+            for (int at = 0; at < kBlockTiles; ++at) {
                 const long long k0 = (long long)kb * kBlockK + at * 64;
-                if (at * 64 >= (have + 15) / 16 * 16) break;   // no K step reaches the second tile
-                copy_rows<true, kShrinkThreads>(p.grain_a, s + a_tile + (uint32_t)(at * p.rank_pad * 128), p.rank, 128, (have - at * 64) * 2,
-                                                [&](int r) { return a + ((long long)r * p.k + k0) * 2; });
+                if (at * 64 >= (have + 15) / 16 * 16) break;   // no K step reaches the tile
+                copy_rows<true, kWorkers>(p.grain_a, s + a_tile + (uint32_t)(at * p.rank_pad * 128), p.rank, 128, (have - at * 64) * 2,
+                                          [&](int r) { return a + ((long long)r * p.k + k0) * 2; });
                 if (!I8)
-                    copy_rows<true, kShrinkThreads>(p.grain_x, s + (uint32_t)(at * TN * 128), tile.count, 128, (have - at * 64) * 2,
-                                                    [&](int r) { return x + ((long long)rows[r] * p.ld_x + k0) * XB; });
+                    copy_rows<true, kWorkers>(p.grain_x, s + (uint32_t)(at * TN * 128), tile.count, 128, (have - at * 64) * 2,
+                                              [&](int r) { return x + ((long long)rows[r] * p.ld_x + k0) * XB; });
             }
             if (I8)
-                copy_rows<false, kShrinkThreads>(p.grain_x, s + raw_tile, tile.count, kBlockK, have,
-                                                 [&](int r) { return x + (long long)rows[r] * p.ld_x + (long long)kb * kBlockK; });
+                copy_rows<false, kWorkers>(p.grain_x, s + raw_tile, tile.count, kBlockK, have,
+                                           [&](int r) { return x + (long long)rows[r] * p.ld_x + (long long)kb * kBlockK; });
+            }
         };
-        for (int i = 0; i < kShrinkStages - 1; ++i) {
-            if (kb0 + i < kb1) load(kb0 + i);
-            cp_commit();
-        }
-        const uint32_t idesc = instr_desc<T>(p.rank_pad);
-        for (int kb = kb0; kb < kb1; ++kb) {
-            const int i = kb - kb0, stage = i % kShrinkStages;
+        // A warp's copies of block i have landed when those of the kShrinkAhead blocks behind it are all that its threads have under way;
+        // one lane says so (an arrival per thread, as copies make by themselves, takes as long as the block's copies).
+        const auto landed = [&](int stage) {
             const uint32_t s = smem0 + (uint32_t)stage * stage_bytes;
-            cp_wait<kShrinkStages - 2>();
-            if (I8 && FAST) widen_rows_grain<T, 16, kShrinkThreads>(s + raw_tile, s, TN * 128, tile.count);
-            else if (I8) widen_rows<T, kShrinkThreads>(p.grain_x, s + raw_tile, s, TN * 128, tile.count);
-            fence_async_proxy();
-            __syncthreads();
-            if (tid == 0) {
-                tc_fence_after();
-                const uint64_t xd = operand_desc(s), ad = operand_desc(s + a_tile);
-                const int steps = (min(kBlockK, p.k - kb * kBlockK) + 15) / 16;
-                for (int j = 0; j < steps; ++j)
-                    umma_f16(tmem_base, xd + j / 4 * (TN * 128 / 16) + j % 4 * 2, ad + j / 4 * (p.rank_pad * 128 / 16) + j % 4 * 2, idesc, (i | j) != 0);
-                umma_commit(smem_u32(&bars[stage]));
-            }
-            // the stage that the block before this one was read from takes the next block
-            if (kb + kShrinkStages - 1 < kb1) {
-                if (i > 0) mbar_wait(smem_u32(&bars[(i - 1) % kShrinkStages]), ((i - 1) / kShrinkStages) & 1, &gave_up, p.status, 900);
-                load(kb + kShrinkStages - 1);
+            if (I8 && FAST) widen_rows_grain<T, 16, kWorkers>(s + raw_tile, s, TN * 128, tile.count);
+            else if (I8) widen_rows<T, kWorkers>(p.grain_x, s + raw_tile, s, TN * 128, tile.count);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&full[stage]));
+        };
+        const int n = kb1 - kb0;
+        int stage = 0, behind = 0;
+        uint32_t phase = 1;   // a stage is free at first
+        for (int i = 0; i < n + kShrinkAhead; ++i) {
+            if (i < n) {
+                mbar_wait(smem_u32(&empty[stage]), phase, &gave_up, p.status, 901);
+                load(kb0 + i, stage);
+                if (++stage == p.stages) { stage = 0; phase ^= 1; }
             }
             cp_commit();
+            if (i >= kShrinkAhead) {
+                cp_wait<kShrinkAhead>();
+                landed(behind);
+                if (++behind == p.stages) behind = 0;
+            }
         }
-        const int last = kb1 - 1 - kb0;
-        mbar_wait(smem_u32(&bars[last % kShrinkStages]), (last / kShrinkStages) & 1, &gave_up, p.status, 901);
+    }
+    if (work) {
+        mbar_wait(smem_u32(&done), 0, &gave_up, p.status, 902);
         tc_fence_after();
-        const int slot = warp * 32 + lane;
-        if (warp * 32 < TN) {
+        const int quarter = warp % 4, half = p.rank_pad / 2, slot = quarter * 32 + lane;
+        if (!issuer && quarter * 32 < TN) {   // warp w: 32 tokens (w % 4) and half of the columns (w / 4)
             const bool live = slot < tile.count;
             const int row = live ? rows[slot] : 0;
             float f = p.scaling ? __ldg(p.scaling + tile.adapter) : 1.0f;
             if (I8 && live) f = __fmul_rn(f, __ldg(p.x_scale + row));
             float4 *v = reinterpret_cast<float4 *>(p.v + ((long long)blockIdx.y * p.rows + row) * p.rank_pad);
-            for (int c = 0; c < p.rank_pad; c += 16) {
-                uint32_t d[16];
-                tmem_ld16(tmem_base + ((uint32_t)(warp * 32) << 16) + (uint32_t)c, d);
+            for (int c = warp / 4 * half; c < (warp / 4 + 1) * half; c += 8) {
+                uint32_t d[8];
+                tmem_ld8(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)c, d);
                 tmem_ld_wait();
                 if (live) {
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4)
+                    for (int e = 0; e < 8; e += 4)
                         v[(c + e) / 4] = make_float4(__fmul_rn(__uint_as_float(d[e]), f), __fmul_rn(__uint_as_float(d[e + 1]), f),
                                                      __fmul_rn(__uint_as_float(d[e + 2]), f), __fmul_rn(__uint_as_float(d[e + 3]), f));
                 }
@@ -564,7 +826,10 @@ __global__ void __launch_bounds__(kShrinkThreads) adapter_shrink_kernel(const Ad
         tc_fence_before();
     }
     __syncthreads();
-    if (warp == 0) tmem_dealloc(tmem_base, cols);
+    if (issuer) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, cols);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -579,28 +844,35 @@ inline int expand_smem(int tn, int rank_pad) { return 1024 + rank_atoms(rank_pad
 // GB: 16 or 8 bytes of b a copy, with rows of base and out on 16-byte boundaries; addresses are worked out once, and results go back
 // through the chunk's base rows in shared memory, from which they are stored 16 bytes at a time.  0: any strides.
 template <typename T, int TN, bool SELF, int GB>
-__global__ void __launch_bounds__(kExpandThreads) adapter_expand_kernel(const AdapterParams p)
+__global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) adapter_expand_kernel(const AdapterParams p)
 {
     extern __shared__ uint8_t smem_raw[];
     __shared__ alignas(16) SelfPlan plan;
-    __shared__ alignas(8) uint64_t bar;
+    __shared__ alignas(8) uint64_t full[kExpandStages], acc_full[2], acc_empty[2], v_full;
     __shared__ uint32_t tmem_base;
     __shared__ int gave_up;
     __shared__ int rows[TN];
     __shared__ float unscale[TN];          // fp16: the power of two that v was divided by
     constexpr bool F16 = std::is_same<T, __half>::value;
-    constexpr uint32_t COLS = TN <= 32 ? 32 : TN;
+    constexpr uint32_t COLS = 2 * TN <= 32 ? 32 : 2 * TN;   // two buffers of accumulators
+    constexpr int WORKERS = expand_workers(TN), THREADS = WORKERS + 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (warp == 0) tmem_alloc(&tmem_base, COLS);
+    const bool issuer = tid >= WORKERS;
+    if (issuer) tmem_alloc(&tmem_base, COLS);
     if (tid == 0) {
-        mbar_init(smem_u32(&bar), 1);
+        for (int i = 0; i < kExpandStages; ++i) mbar_init(smem_u32(&full[i]), WORKERS);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&acc_full[i]), 1);
+            mbar_init(smem_u32(&acc_empty[i]), WORKERS / 32);
+        }
+        mbar_init(smem_u32(&v_full), WORKERS / 32);
         gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const Tile tile = SELF ? self_plan<TN, kExpandThreads>(p, plan, rows) : read_plan(p, kExpandThreads, rows);
+    const Tile tile = SELF ? self_plan<TN>(p, plan, rows) : read_plan<TN>(p, p.parts, THREADS, rows);
     const int chunks = (p.n + kChunkN - 1) / kChunkN;
     const int c0 = (int)((long long)blockIdx.y * chunks / p.nsplit), c1 = (int)((long long)(blockIdx.y + 1) * chunks / p.nsplit);
     const T *base = reinterpret_cast<const T *>(p.base);
@@ -608,26 +880,7 @@ __global__ void __launch_bounds__(kExpandThreads) adapter_expand_kernel(const Ad
     if (tile.count > 0 && tile.adapter < 0) {
         if (p.out != p.base) {
             pdl_wait();
-            const int n0 = c0 * kChunkN, width = min(c1 * kChunkN, p.n) - n0;
-            constexpr int V = GB ? 8 : 1, AHEAD = 4;     // elements a copy, copies in flight
-            using Copy = typename std::conditional<GB != 0, uint4, uint16_t>::type;
-            const int across = (width + V - 1) / V, total = across * tile.count;   // at most 64 rows of 65535
-            for (int i0 = tid; i0 < total; i0 += kExpandThreads * AHEAD) {
-                Copy v[AHEAD];
-                T *to[AHEAD];
-#pragma unroll
-                for (int j = 0; j < AHEAD; ++j) {
-                    const int i = i0 + j * kExpandThreads, r = i / across, c = n0 + (i - r * across) * V;
-                    to[j] = nullptr;
-                    if (i < total) {
-                        v[j] = *reinterpret_cast<const Copy *>(base + (long long)rows[r] * p.ld_base + c);
-                        to[j] = out + (long long)rows[r] * p.ld_out + c;
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < AHEAD; ++j)
-                    if (to[j]) *reinterpret_cast<Copy *>(to[j]) = v[j];
-            }
+            copy_base<T, GB ? 8 : 1, THREADS>(p, rows, tile.count, c0 * kChunkN, min(c1 * kChunkN, p.n));
         }
     } else if (tile.count > 0 && c0 < c1) {
         const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -636,22 +889,25 @@ __global__ void __launch_bounds__(kExpandThreads) adapter_expand_kernel(const Ad
         const uint32_t stage_bytes = expand_stage(TN, p.rank_pad), base_at = (uint32_t)(atoms * kChunkN * 128);
         const char *b = reinterpret_cast<const char *>(p.b) + (long long)tile.adapter * p.n * p.rank * 2;
         // b: the copies of a chunk, offset in its rows << 8 | bytes, and place in the tile
-        constexpr int NB = GB ? 256 / (2 * GB) : 1, NR = TN * 16 / kExpandThreads;
-        const int per_row = GB ? p.rank_pad * 2 / (GB ? GB : 1) : 1, nb = per_row * kChunkN / kExpandThreads;
+        constexpr int NB = GB ? 256 * kChunkN / ((GB ? GB : 1) * WORKERS) : 1, NR = TN * 16 / WORKERS;
+        const int per_row = GB ? p.rank_pad * 2 / (GB ? GB : 1) : 1, nb = (per_row * kChunkN + WORKERS - 1) / WORKERS;
         uint32_t b_from[NB], b_to[NB];
         long long base_at_row[NR], out_at_row[NR];
         const int rc = (tid % 16) * 8;
-        if (GB) {
+        if (GB && !issuer) {
+            const float across = 1.0f / (float)per_row;
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
-                const int idx = tid + i * kExpandThreads, r = idx / per_row, byte = (idx - r * per_row) * GB;
+                if (i >= nb) break;
+                const int idx = tid + i * WORKERS, r = (int)(((float)idx + 0.5f) * across), byte = (idx - r * per_row) * GB;   // exact for idx < 2^12
                 const int valid = min(max(p.rank * 2 - byte, 0), GB);
-                b_from[i] = (uint32_t)(r * p.rank * 2 + (valid ? byte : 0)) << 8 | (uint32_t)valid;
+                // one too many lies behind every chunk's end
+                b_from[i] = idx < per_row * kChunkN ? (uint32_t)(r * p.rank * 2 + (valid ? byte : 0)) << 8 | (uint32_t)valid : ~0u;
                 b_to[i] = (uint32_t)(byte / 128 * kChunkN * 128) + swizzled(r, byte % 128);
             }
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
-                const int r = tid / 16 + i * 16;
+                const int r = tid / 16 + i * (WORKERS / 16);
                 base_at_row[i] = r < tile.count ? (long long)rows[r] * p.ld_base + rc : -1;
                 out_at_row[i] = r < tile.count ? (long long)rows[r] * p.ld_out + rc : -1;
             }
@@ -659,7 +915,7 @@ __global__ void __launch_bounds__(kExpandThreads) adapter_expand_kernel(const Ad
         const auto load = [&](int c) {
             const uint32_t s = stage0 + (uint32_t)((c - c0) % kExpandStages) * stage_bytes;
             const int n0 = c * kChunkN, channels = min(kChunkN, p.n - n0);
-            if (GB) {
+            if constexpr (GB != 0) {
                 const char *from = b + (long long)n0 * p.rank * 2;
                 const uint32_t end = (uint32_t)(channels * p.rank * 2);
 #pragma unroll
@@ -670,132 +926,164 @@ __global__ void __launch_bounds__(kExpandThreads) adapter_expand_kernel(const Ad
 #pragma unroll
                 for (int i = 0; i < NR; ++i)
                     if (base_at_row[i] >= 0 && rc < channels)
-                        cp_async<16>(s + base_at + (uint32_t)((tid + i * kExpandThreads) * 16), base + base_at_row[i] + n0, 16);
-                return;
-            }
+                        cp_async<16>(s + base_at + (uint32_t)((tid + i * WORKERS) * 16), base + base_at_row[i] + n0, 16);
+            } else {
             for (int at = 0; at < atoms; ++at) {
                 const int left = p.rank_pad - at * 64;                       // a whole number of K steps, zero beyond the rank
                 const int width = left > 32 ? 128 : left > 16 ? 64 : 32;
-                copy_rows<true, kExpandThreads>(p.grain_b, s + (uint32_t)at * kChunkN * 128, channels, width, (p.rank - at * 64) * 2,
+                copy_rows<true, WORKERS>(p.grain_b, s + (uint32_t)at * kChunkN * 128, channels, width, (p.rank - at * 64) * 2,
                                                 [&](int r) { return b + ((long long)(n0 + r) * p.rank + at * 64) * 2; });
             }
-            copy_rows<false, kExpandThreads>(p.grain_base, s + base_at, tile.count, kChunkN * 2, channels * 2,
+            copy_rows<false, WORKERS>(p.grain_base, s + base_at, tile.count, kChunkN * 2, channels * 2,
                                              [&](int r) { return reinterpret_cast<const char *>(base + (long long)rows[r] * p.ld_base + n0); });
+            }
         };
-        for (int i = 0; i < kExpandStages; ++i) {
-            if (c0 + i < c1) load(c0 + i);
-            cp_commit();
-        }
-        pdl_wait();   // the partial sums are complete
-        {
-            constexpr int LANES = kExpandThreads / TN;    // per token
-            const int slot = tid / LANES, part = tid % LANES;
-            const bool live = slot < tile.count;
-            const int row = live ? rows[slot] : 0;
-            constexpr int CH = 16 / LANES;                // 8 components of v each, LANES apart
-            float f[CH][8];
+        if (issuer) {
+            pdl_wait();
+            const uint32_t idesc = instr_desc<T>(TN);
+            mbar_wait(smem_u32(&v_full), 0, &gave_up, p.status, 910);
+            for (int c = c0; c < c1; ++c) {
+                const int i = c - c0, buf = i & 1;
+                const uint32_t s = stage0 + (uint32_t)(i % kExpandStages) * stage_bytes, d = tmem_base + (uint32_t)(buf * TN);
+                mbar_wait(smem_u32(&full[i % kExpandStages]), (i / kExpandStages) & 1, &gave_up, p.status, 911);
+                if (i >= 2) mbar_wait(smem_u32(&acc_empty[buf]), (i / 2 - 1) & 1, &gave_up, p.status, 912);
+                fence_async_proxy();
+                tc_fence_after();
+                if (lane == 0) {
+                    uint32_t more = 0;
+                    for (int j = 0; j < p.rank_pad / 16; ++j) {
+                        const uint64_t bd = operand_desc(s + (uint32_t)(j / 4) * kChunkN * 128) + (j % 4) * 2;
+                        umma_f16(d, bd, operand_desc(v_hi + (uint32_t)(j / 4) * TN * 128) + (j % 4) * 2, idesc, more);
+                        more = 1;
+                        umma_f16(d, bd, operand_desc(v_lo + (uint32_t)(j / 4) * TN * 128) + (j % 4) * 2, idesc, more);
+                    }
+                    umma_commit(smem_u32(&acc_full[buf]));
+                }
+                __syncwarp();
+            }
+        } else {
+            // Copies through shared memory by whole 16 or 8 bytes announce themselves; others are waited for, a chunk ahead.
+            const auto announce = [&](int c) {
+                if (GB) mbar_arrive_copies(smem_u32(&full[(c - c0) % kExpandStages]));
+            };
+            const auto landed = [&](int c) {
+                if (GB) return;
+                cp_wait<0>();
+                mbar_arrive(smem_u32(&full[(c - c0) % kExpandStages]));
+            };
+            load(c0);
+            announce(c0);
+            if (GB && c0 + 1 < c1) {
+                load(c0 + 1);
+                announce(c0 + 1);
+            }
+            pdl_wait();   // v is complete
+            {
+                constexpr int LANES = WORKERS / TN, CH = 16 / LANES;   // threads of a token, and groups of 8 components of each
+                const int slot = tid / LANES, part = tid % LANES;
+                const bool live = slot < tile.count;
+                const int row = live ? rows[slot] : 0;
+                float f[CH][8];
 #pragma unroll
-            for (int h = 0; h < CH; ++h)
+                for (int h = 0; h < CH; ++h)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[h][e] = 0.0f;
-            const float4 *v = reinterpret_cast<const float4 *>(p.v + (long long)row * p.rank_pad);
-            const long long split = (long long)p.rows * p.rank_pad / 4;
-            if (live) {
-                constexpr int AHEAD = CH == 1 ? 8 : 4;    // partial sums that are fetched together
-                for (int s0 = 0; s0 < p.ksplit; s0 += AHEAD) {
+                    for (int e = 0; e < 8; ++e) f[h][e] = 0.0f;
+                const float4 *v = reinterpret_cast<const float4 *>(p.v + (long long)row * p.rank_pad);
+                const long long split = (long long)p.rows * p.rank_pad / 4;
+                if (live) {
+                    constexpr int AT_ONCE = 4;   // partial sums that are fetched together; they are added in the order of the splits
+                    for (int s0 = 0; s0 < p.ksplit; s0 += AT_ONCE) {
 #pragma unroll
-                    for (int h = 0; h < CH; ++h) {
-                        const int j = (part + h * LANES) * 8;
-                        if (j >= p.rank_pad) break;
-                        float4 q[AHEAD][2];
+                        for (int h = 0; h < CH; ++h) {
+                            const int j = (part + h * LANES) * 8;
+                            if (j >= p.rank_pad) break;
+                            float4 q[AT_ONCE][2];
 #pragma unroll
-                        for (int s = 0; s < AHEAD; ++s) {
-                            const bool there = s0 + s < p.ksplit;
-                            q[s][0] = there ? __ldcg(v + (s0 + s) * split + j / 4) : make_float4(0, 0, 0, 0);
-                            q[s][1] = there ? __ldcg(v + (s0 + s) * split + j / 4 + 1) : make_float4(0, 0, 0, 0);
-                        }
+                            for (int s = 0; s < AT_ONCE; ++s) {
+                                const bool there = s0 + s < p.ksplit;
+                                q[s][0] = there ? __ldcg(v + (s0 + s) * split + j / 4) : make_float4(0, 0, 0, 0);
+                                q[s][1] = there ? __ldcg(v + (s0 + s) * split + j / 4 + 1) : make_float4(0, 0, 0, 0);
+                            }
 #pragma unroll
-                        for (int s = 0; s < AHEAD; ++s) {
-                            f[h][0] += q[s][0].x; f[h][1] += q[s][0].y; f[h][2] += q[s][0].z; f[h][3] += q[s][0].w;
-                            f[h][4] += q[s][1].x; f[h][5] += q[s][1].y; f[h][6] += q[s][1].z; f[h][7] += q[s][1].w;
+                            for (int s = 0; s < AT_ONCE; ++s) {
+                                f[h][0] += q[s][0].x; f[h][1] += q[s][0].y; f[h][2] += q[s][0].z; f[h][3] += q[s][0].w;
+                                f[h][4] += q[s][1].x; f[h][5] += q[s][1].y; f[h][6] += q[s][1].z; f[h][7] += q[s][1].w;
+                            }
                         }
                     }
+#pragma unroll
+                    for (int h = 0; h < CH; ++h)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if ((part + h * LANES) * 8 + e >= p.rank) f[h][e] = 0.0f;   // the K steps end in zeros
+                }
+                float down = 1.0f;
+                if (F16) {
+                    uint32_t m = 0;
+#pragma unroll
+                    for (int h = 0; h < CH; ++h)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(f[h][e]) & 0x7fffffffu);
+#pragma unroll
+                    for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                    // 2^-e for a largest value in [2^e, 2^(e+1)); none for zero, for what no power of two can help, and at the ends of fp32
+                    const int e = (int)(m >> 23) - 127;
+                    const bool shift = m != 0 && e > -120 && e < 120;
+                    down = shift ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.0f;
+                    if (part == 0) unscale[slot] = shift ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.0f;
                 }
 #pragma unroll
-                for (int h = 0; h < CH; ++h)
+                for (int h = 0; h < CH; ++h) {
+                    const int j = (part + h * LANES) * 8;
+                    if (j >= p.rank_pad) break;
+                    float g[8];
+                    uint32_t hi[4], lo[4];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if ((part + h * LANES) * 8 + e >= p.rank) f[h][e] = 0.0f;
-            }
-            float down = 1.0f;
-            if (F16) {
-                uint32_t m = 0;
+                    for (int e = 0; e < 8; ++e) {
+                        f[h][e] = __fmul_rn(f[h][e], down);
+                        g[e] = __fsub_rn(f[h][e], to_float(from_float<T>(f[h][e])));
+                    }
 #pragma unroll
-                for (int h = 0; h < CH; ++h)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(f[h][e]) & 0x7fffffffu);
-#pragma unroll
-                for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-                // 2^-e for a largest value in [2^e, 2^(e+1)); none for zero, for what no power of two can help, and at the ends of fp32
-                const int e = (int)(m >> 23) - 127;
-                const bool shift = m != 0 && e > -120 && e < 120;
-                down = shift ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.0f;
-                if (part == 0) unscale[slot] = shift ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.0f;
-            }
-#pragma unroll
-            for (int h = 0; h < CH; ++h) {
-                const int j = (part + h * LANES) * 8;
-                if (j >= p.rank_pad) break;
-                float g[8];
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    f[h][e] = __fmul_rn(f[h][e], down);
-                    g[e] = __fsub_rn(f[h][e], to_float(from_float<T>(f[h][e])));
+                    for (int e = 0; e < 4; ++e) {
+                        hi[e] = pack2<T>(f[h][2 * e], f[h][2 * e + 1]);
+                        lo[e] = pack2<T>(g[2 * e], g[2 * e + 1]);
+                    }
+                    const uint32_t at = (uint32_t)(j / 64 * TN * 128) + swizzled(slot, (j % 64) * 2);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(v_hi + at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(v_lo + at), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&v_full));
+                if (F16) worker_sync<WORKERS>();   // unscale
+            }
+            cp_commit();
+            landed(c0);
+            if (!GB && c0 + 1 < c1) {
+                load(c0 + 1);
+                cp_commit();
+            }
+            // warp w: channels 32 (w % 4) + lane, its share of the tokens
+            constexpr int SHARE = TN * 128 / WORKERS;
+            const int q = warp & 3, ch = q * 32 + lane, first = (warp >> 2) * SHARE;
+            for (int c = c0; c < c1; ++c) {
+                const int i = c - c0, buf = i & 1, n = c * kChunkN + ch;
+                const uint32_t s = stage0 + (uint32_t)(i % kExpandStages) * stage_bytes;
+                if (c + 1 < c1) landed(c + 1);
+                mbar_wait(smem_u32(&full[i % kExpandStages]), (i / kExpandStages) & 1, &gave_up, p.status, 913);   // base, copied by others
+                mbar_wait(smem_u32(&acc_full[buf]), (i / 2) & 1, &gave_up, p.status, 914);
+                tc_fence_after();
+                uint32_t d[SHARE];
+                if (first < tile.count) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    hi[e] = pack2<T>(f[h][2 * e], f[h][2 * e + 1]);
-                    lo[e] = pack2<T>(g[2 * e], g[2 * e + 1]);
+                    for (int t0 = 0; t0 < SHARE; t0 += 8) tmem_ld8(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * TN + first + t0), d + t0);
+                    tmem_ld_wait();
                 }
-                const uint32_t at = (uint32_t)(j / 64 * TN * 128) + swizzled(slot, (j % 64) * 2);
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(v_hi + at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(v_lo + at), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
-            }
-        }
-        const uint32_t idesc = instr_desc<T>(TN);
-        const auto multiply = [&](int c) {   // by one thread
-            const uint32_t s = stage0 + (uint32_t)((c - c0) % kExpandStages) * stage_bytes;
-            tc_fence_after();
-            uint32_t more = 0;
-            for (int j = 0; j < p.rank_pad / 16; ++j) {
-                const uint64_t bd = operand_desc(s + (uint32_t)(j / 4) * kChunkN * 128) + (j % 4) * 2;
-                umma_f16(tmem_base, bd, operand_desc(v_hi + (uint32_t)(j / 4) * TN * 128) + (j % 4) * 2, idesc, more);
-                more = 1;
-                umma_f16(tmem_base, bd, operand_desc(v_lo + (uint32_t)(j / 4) * TN * 128) + (j % 4) * 2, idesc, more);
-            }
-            umma_commit(smem_u32(&bar));
-        };
-        cp_wait<kExpandStages - 1>();
-        fence_async_proxy();
-        __syncthreads();
-        if (tid == 0) multiply(c0);
-        // warp w: channels 32 (w % 4) + lane, half of the tokens
-        constexpr int HALF = TN / 2;
-        const int q = warp & 3, ch = q * 32 + lane, first = (warp >> 2) * HALF;
-        for (int c = c0; c < c1; ++c) {
-            const int i = c - c0, n = c * kChunkN + ch;
-            const uint32_t s = stage0 + (uint32_t)(i % kExpandStages) * stage_bytes;
-            mbar_wait(smem_u32(&bar), i & 1, &gave_up, p.status, 910);
-            tc_fence_after();
-            uint32_t d[HALF];
-            if (first < tile.count) {
-#pragma unroll
-                for (int t0 = 0; t0 < HALF; t0 += 8) tmem_ld8(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(first + t0), d + t0);
-                tmem_ld_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&acc_empty[buf]));
                 const uint32_t at = s + base_at + (uint32_t)(first * kChunkN * 2 + ch * 2);
 #pragma unroll
-                for (int t0 = 0; t0 < HALF; t0 += 8) {
+                for (int t0 = 0; t0 < SHARE; t0 += 8) {
                     if (first + t0 >= tile.count) break;
                     uint16_t raw[8];
 #pragma unroll
@@ -810,31 +1098,29 @@ __global__ void __launch_bounds__(kExpandThreads) adapter_expand_kernel(const Ad
                         else if (slot < tile.count && n < p.n) out[(long long)rows[slot] * p.ld_out + n] = o;
                     }
                 }
-            }
-            tc_fence_before();
-            cp_wait<0>();           // the next chunk, for which a whole round was time
-            fence_async_proxy();
-            __syncthreads();        // this chunk's results are in place, its accumulators read, the next chunk there
-            if (tid == 0 && c + 1 < c1) multiply(c + 1);
-            if (GB) {   // a thread stores the 16 bytes whose place it then fills again
+                worker_sync<WORKERS>();   // this chunk's results are in place, and its base rows have been read
+                if (GB) {   // a thread stores the 16 bytes whose place it then fills again
 #pragma unroll
-                for (int i = 0; i < NR; ++i) {
-                    if (out_at_row[i] >= 0 && c * kChunkN + rc < p.n) {
-                        uint4 o;
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(o.x), "=r"(o.y), "=r"(o.z), "=r"(o.w)
-                                     : "r"(s + base_at + (uint32_t)((tid + i * kExpandThreads) * 16)) : "memory");
-                        *reinterpret_cast<uint4 *>(out + out_at_row[i] + c * kChunkN) = o;
+                    for (int j = 0; j < NR; ++j) {
+                        if (out_at_row[j] >= 0 && c * kChunkN + rc < p.n) {
+                            uint4 o;
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(o.x), "=r"(o.y), "=r"(o.z), "=r"(o.w)
+                                         : "r"(s + base_at + (uint32_t)((tid + j * WORKERS) * 16)) : "memory");
+                            *reinterpret_cast<uint4 *>(out + out_at_row[j] + c * kChunkN) = o;
+                        }
                     }
                 }
+                if (c + kExpandStages < c1) {
+                    load(c + kExpandStages);
+                    announce(c + kExpandStages);
+                    cp_commit();
+                }
             }
-            if (c + kExpandStages < c1) load(c + kExpandStages);
-            cp_commit();
         }
-        cp_wait<0>();
     }
     pdl_wait();   // this grid must not end before the kernels in front of it: the stream goes on behind it alone
     __syncthreads();
-    if (warp == 0) tmem_dealloc(tmem_base, COLS);
+    if (issuer) tmem_dealloc(tmem_base, COLS);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -852,41 +1138,15 @@ cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, int threads, int 
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = dependent ? 1 : 0;
+    if (dependent) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 constexpr size_t align256(size_t v) { return (v + 255) / 256 * 256; }
-
-struct Shape {
-    int tile_tokens, tiles, ksplit, nsplit, rank_pad;
-    bool self;
-};
-
-// Tiles of 16 tokens while every CTA plans for itself, of 64 beyond.  `tiles` is the most there can be: full ones, and one that is not for
-// every adapter and for none.  K and N are split so that the CTAs find a place on the SMs together (about five of the small ones fit an SM,
-// two of the large), but no CTA gets less than two K blocks.
-Shape shape_of(const AdapterProblem &p)
-{
-    Shape s;
-    s.self = p.rows <= kSelfPlan;
-    s.tile_tokens = s.self ? 16 : 64;
-    const long long partial = p.adapters + 1 < p.rows ? p.adapters + 1 : p.rows;
-    s.tiles = (int)(p.rows / s.tile_tokens + partial);
-    if (s.tiles > p.rows) s.tiles = (int)p.rows;
-    s.rank_pad = align_up((int)p.rank, 16);
-    const int want = (s.self ? 4 : 2) * 148 / s.tiles;
-    const int blocks = (int)((p.k + kBlockK - 1) / kBlockK), chunks = (int)((p.n + kChunkN - 1) / kChunkN);
-    s.ksplit = want < blocks / 2 ? want : blocks / 2;
-    if (s.ksplit > 16) s.ksplit = 16;
-    if (s.ksplit < 1) s.ksplit = 1;
-    s.nsplit = want < chunks ? want : chunks;
-    if (s.nsplit < 1) s.nsplit = 1;
-    return s;
-}
 
 int grain_of(const void *base, long long pitch_bytes, int smallest)
 {
@@ -894,7 +1154,45 @@ int grain_of(const void *base, long long pitch_bytes, int smallest)
     return v % 16 == 0 ? 16 : v % 8 == 0 ? 8 : v % 4 == 0 ? 4 : smallest;
 }
 
-template <typename T, bool I8, int TN, bool SELF>
+struct Shape {
+    int tile_tokens, tiles, ksplit, nsplit, rank_pad;
+    bool self, few;
+};
+
+// Tiles of 4 tokens on the CUDA cores where adapters have no more on average, else of 16 while every CTA plans for itself, beyond of 64 or, where adapters have that many tokens on average and there are
+// enough of them for the SMs, of 128 (up to rank 64, for the sake of three stages): the first product reads 128 rows of the tokens' tile whether they are tokens or not.  `tiles` is the
+// most there can be: full ones, and one that is not for every adapter and for none.  K and N are split so that the CTAs find a place on the
+// SMs together (about four of the small ones fit an SM, two of the next, one of the large).
+Shape shape_of(const AdapterProblem &p, bool may_be_few = true)
+{
+    Shape s;
+    s.self = p.rows <= kSelfPlan;
+    const long long partial = p.adapters + 1 < p.rows ? p.adapters + 1 : p.rows;
+    // as many tokens as four per adapter, and rows that can be read 16 bytes at a time
+    const int xb = p.x_i8 ? 1 : 2;
+    s.few = may_be_few && s.self && (p.rows <= kFew || p.rows <= kFew * p.adapters) && grain_of(p.x, p.ld_x * xb, 1) >= 8 * xb && grain_of(p.a, p.k * 2, 1) == 16 &&
+            grain_of(p.b, p.rank * 2, 1) == 16;
+    s.tile_tokens = s.few ? kFew : s.self ? 16 : p.rows >= 2048 && p.rows >= 128 * p.adapters && p.rank <= 64 ? 128 : 64;
+    s.tiles = (int)(p.rows / s.tile_tokens + partial);
+    if (s.self || s.tiles > p.rows) s.tiles = (int)p.rows;   // any token may begin one
+    s.rank_pad = align_up((int)p.rank, 16);
+    const int places = (s.self ? 4 : s.tile_tokens == 64 ? 2 : 1) * 148;
+    const int likely = (int)(p.rows / s.tile_tokens + partial / 2) > 0 ? (int)(p.rows / s.tile_tokens + partial / 2) : 1;
+    const int blocks = (int)((p.k + kBlockK - 1) / kBlockK), chunks = (int)((p.n + kChunkN - 1) / kChunkN);
+    s.ksplit = 1;
+    while (s.ksplit < 8 && 2 * s.ksplit * likely <= places && 2 * s.ksplit <= blocks) s.ksplit *= 2;
+    const int want = 2 * 148 / (s.tile_tokens == 128 ? 2 * likely : likely);
+    s.nsplit = want < chunks ? want : chunks;
+    if (s.few) {
+        const int units = (int)((p.n + kFewChannels - 1) / kFewChannels), busy = (int)(p.rows < p.adapters ? p.rows : p.adapters);
+        s.ksplit = 1;
+        s.nsplit = kFewExpandCtas * 148 / busy < units ? kFewExpandCtas * 148 / busy : units;   // one wave: every CTA looks for its tile first
+    }
+    if (s.nsplit < 1) s.nsplit = 1;
+    return s;
+}
+
+template <typename T, bool I8, int TN, bool SELF>   // TN: tokens of the first kernel's tiles; the second one's have at most 64
 cudaError_t launch_tiles(const AdapterParams &p, const Shape &s, cudaStream_t stream)
 {
     cudaError_t e = cudaSuccess;
@@ -903,27 +1201,42 @@ cudaError_t launch_tiles(const AdapterParams &p, const Shape &s, cudaStream_t st
         if (e != cudaSuccess) return e;
     }
     const auto shrink = p.grain_x == 16 && p.grain_a == 16 ? adapter_shrink_kernel<T, I8, TN, SELF, true> : adapter_shrink_kernel<T, I8, TN, SELF, false>;
-    e = launch_kernel(shrink, dim3((unsigned)s.tiles, (unsigned)s.ksplit), kShrinkThreads, shrink_smem(TN, s.rank_pad, I8), stream, !SELF, p);
+    e = launch_kernel(shrink, dim3((unsigned)s.tiles, (unsigned)s.ksplit), kWorkers + 32, shrink_smem(TN, s.rank_pad, I8), stream, !SELF, p);
     if (e != cudaSuccess) return e;
     const bool rows16 = p.grain_base == 16 && p.grain_out == 16 && p.n % 8 == 0;
-    const auto expand = rows16 && p.grain_b == 16 ? adapter_expand_kernel<T, TN, SELF, 16>
-                        : rows16 && p.grain_b == 8 ? adapter_expand_kernel<T, TN, SELF, 8> : adapter_expand_kernel<T, TN, SELF, 0>;
-    return launch_kernel(expand, dim3((unsigned)s.tiles, (unsigned)s.nsplit), kExpandThreads, expand_smem(TN, s.rank_pad), stream, true, p);
+    constexpr int EN = TN < 64 ? TN : 64;
+    const auto expand = rows16 && p.grain_b == 16 ? adapter_expand_kernel<T, EN, SELF, 16>
+                        : rows16 && p.grain_b == 8 ? adapter_expand_kernel<T, EN, SELF, 8> : adapter_expand_kernel<T, EN, SELF, 0>;
+    return launch_kernel(expand, dim3((unsigned)(s.tiles * p.parts), (unsigned)s.nsplit), expand_workers(EN) + 32, expand_smem(EN, s.rank_pad), stream, true, p);
 }
 
 template <typename T, bool I8>
 cudaError_t launch_typed(const AdapterParams &p, const Shape &s, cudaStream_t stream)
 {
-    return s.self ? launch_tiles<T, I8, 16, true>(p, s, stream) : launch_tiles<T, I8, 64, false>(p, s, stream);
+    if (s.few) {
+        const cudaError_t e = launch_kernel(adapter_few_shrink_kernel<T, I8>, dim3((unsigned)s.tiles, (unsigned)((p.rank + 7) / 8)), kFewThreads, 0, stream, false, p);
+        if (e != cudaSuccess) return e;
+        const auto expand = p.rank <= 8 ? adapter_few_expand_kernel<T, 1> : p.rank <= 16 ? adapter_few_expand_kernel<T, 2>
+                            : p.rank <= 32 ? adapter_few_expand_kernel<T, 4> : p.rank <= 64 ? adapter_few_expand_kernel<T, 8> : adapter_few_expand_kernel<T, 16>;
+        return launch_kernel(expand, dim3((unsigned)s.tiles, (unsigned)s.nsplit), kFewThreads, 0, stream, true, p);
+    }
+    if (s.self) return launch_tiles<T, I8, 16, true>(p, s, stream);
+    return s.tile_tokens == 64 ? launch_tiles<T, I8, 64, false>(p, s, stream) : launch_tiles<T, I8, 128, false>(p, s, stream);
 }
 
 }  // namespace
 
 size_t adapter_workspace_bytes(const AdapterProblem &p)
 {
-    const Shape s = shape_of(p);
-    return 256 + (s.self ? 0 : 256 + align256((size_t)s.tiles * sizeof(int4)) + align256((size_t)p.rows * 4)) +
-           align256((size_t)s.ksplit * (size_t)p.rows * (size_t)s.rank_pad * 4);
+    // which kernels take the call hangs on the addresses that it is run with
+    size_t most = 0;
+    for (const bool few : {false, true}) {
+        const Shape s = shape_of(p, few);
+        const size_t bytes = 256 + (s.self ? 0 : 256 + align256((size_t)s.tiles * sizeof(int2)) + align256((size_t)s.tiles * s.tile_tokens * 4)) +
+                             align256((size_t)s.ksplit * (size_t)p.rows * (size_t)s.rank_pad * 4);
+        if (bytes > most) most = bytes;
+    }
+    return most;
 }
 
 cudaError_t adapter_launch(const AdapterProblem &a, void *workspace, size_t workspace_bytes, cudaStream_t stream)
@@ -943,17 +1256,18 @@ cudaError_t adapter_launch(const AdapterProblem &a, void *workspace, size_t work
     p.grain_b = grain_of(a.b, a.rank * 2, 2);
     p.grain_base = grain_of(a.base, a.ld_base * 2, 2);
     p.grain_out = grain_of(a.out, a.ld_out * 2, 2);
-    p.ksplit = s.ksplit; p.nsplit = s.nsplit;
+    p.ksplit = s.ksplit; p.nsplit = s.nsplit; p.parts = s.tile_tokens > 64 ? s.tile_tokens / 64 : 1;
     char *ws = static_cast<char *>(workspace);
     p.status = reinterpret_cast<int *>(ws);
     ws += 256;
     p.n_tiles = nullptr; p.tiles = nullptr; p.order = nullptr;
     if (!s.self) {
         p.n_tiles = reinterpret_cast<int *>(ws); ws += 256;
-        p.tiles = reinterpret_cast<int4 *>(ws); ws += align256((size_t)s.tiles * sizeof(int4));
-        p.order = reinterpret_cast<int *>(ws); ws += align256((size_t)a.rows * 4);
+        p.tiles = reinterpret_cast<int2 *>(ws); ws += align256((size_t)s.tiles * sizeof(int2));
+        p.order = reinterpret_cast<int *>(ws); ws += align256((size_t)s.tiles * s.tile_tokens * 4);
     }
     p.v = reinterpret_cast<float *>(ws);
+    p.stages = shrink_stages(s.tile_tokens, s.rank_pad, a.x_i8);
     if (a.dtype == kF16) return a.x_i8 ? launch_typed<__half, true>(p, s, stream) : launch_typed<__half, false>(p, s, stream);
     return a.x_i8 ? launch_typed<__nv_bfloat16, true>(p, s, stream) : launch_typed<__nv_bfloat16, false>(p, s, stream);
 }

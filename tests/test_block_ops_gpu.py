@@ -495,3 +495,23 @@ def test_tensors_elsewhere_are_refused():
         ops.add_rms_norm_quant(x, gamma)
     with pytest.raises(ValueError, match="CUDA device"):
         ops.route_top_k(x, 2, bias=torch.zeros(8))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("r", [8, 16, 24, 32, 64, 120, 128])
+@pytest.mark.parametrize("T,K,N,L", [(1, 8, 8, 1), (4, 264, 256, 1), (7, 2048, 1000, 64), (128, 1024, 2976, 64), (256, 520, 264, 300), (200, 256, 8, 50)])
+def test_adapter_few_tokens_of_many_adapters(T, K, N, L, r, dtype):
+    for x_i8 in (False, True):
+        c = adapter_case(T, K, N, L, r, dtype, x_i8, seed=T + r)
+        check_adapter(c, ops.adapter_add(**c))
+    # all tokens of one adapter, all without one
+    for i in (0, -1):
+        c["adapter_ids"] = torch.full_like(c["adapter_ids"], i)
+        check_adapter(c, ops.adapter_add(**c))
+
+
+@pytest.mark.parametrize("T,L,r", [(2048, 1, 64), (2500, 8, 16), (4100, 9, 40), (3000, 2, 128), (2048, 30, 8)])
+def test_adapter_large_tiles(T, L, r):
+    for x_i8 in (False, True):
+        c = adapter_case(T, 1032, 520, L, r, BF16, x_i8)
+        check_adapter(c, ops.adapter_add(**c))
