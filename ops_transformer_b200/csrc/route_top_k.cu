@@ -31,7 +31,7 @@ struct RouteParams {
     const float *bias;
     const int8_t *token_mask;
     int rows, experts, top_k;
-    int groups, group_size, topk_group, sub, per;
+    int groups, group_size, topk_group, sub, sub_log, per;
     bool whole;                // every lane's experts fill its registers and start on a boundary of their own size (at most 16 bytes)
     bool renormalize, ids_i64;
     float scale;
@@ -103,12 +103,126 @@ __device__ __forceinline__ void put(const RouteParams &p, long long at, float w,
     else reinterpret_cast<int32_t *>(p.ids)[at] = id;
 }
 
+// Sigmoid to within 3e-7 in five instructions; the exact one takes thirty.
+__device__ __forceinline__ float sigmoid_about(float l)
+{
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(l, -1.44269504f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(1.0f, e)));
+    return r;
+}
+
+// The choice by sigmoid scores plus a bias, from scores that are only about right.  Such a score is off by less than 6e-7 from the one that
+// the definition rounds (both count their own errors: 3e-7 here; exp, sum and quotient there), a sum with the bias by a unit of its last
+// place more.  Groups that differ by more than these errors together stay or go as with exact scores; and the k-th largest lane maximum,
+// less the errors, bounds the k-th largest exact choice from below.  So the few experts that reach it are the only ones whose exact score
+// is needed, and each has a lane of its own for that (16384 rows of 256 in eight groups: 17.1 -> 15.0 us).  False, with nothing written, where two groups are too close, where infinities are
+// about or more than 32 experts reach the bound: then every score is computed exactly.
+template <int R, bool TOP2>
+__device__ __forceinline__ bool route_about(const RouteParams &p, const float (&l)[R], const float (&bias)[R], int group, int first, long long out,
+                                            unsigned long long *list_key, float *list_logit, int *list_id)
+{
+    const int lane = threadIdx.x & 31;
+    float c[R], best = minus_inf(), second = minus_inf();
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        c[i] = sigmoid_about(l[i]);
+        if (p.bias) c[i] = __fadd_rn(c[i], bias[i]);
+        c[i] = l[i] > minus_inf() && c[i] > minus_inf() ? c[i] : minus_inf();   // NaN too
+        if (TOP2) second = fmaxf(second, fminf(best, c[i]));
+        best = fmaxf(best, c[i]);
+    }
+    float top = best;
+    bool stays = true;
+    if (p.groups > 1) {
+        for (int o = 1; o < p.sub; o <<= 1) {
+            const float ob = __shfl_xor_sync(kAll, best, o);
+            if (TOP2) second = fmaxf(fmaxf(second, __shfl_xor_sync(kAll, second, o)), fminf(best, ob));
+            best = fmaxf(best, ob);
+        }
+        const float rank = TOP2 && second > minus_inf() ? __fadd_rn(best, second) : best;
+        const float margin = 3e-6f + 1e-6f * fabsf(rank);
+        const float above = __fadd_rn(rank, margin), below = __fsub_rn(rank, margin);
+        int surely = 0, maybe = -1;   // groups that are, that may be better; it is no better than itself
+#pragma unroll 8
+        for (int g = 0; g < p.groups; ++g) {
+            const float r = __shfl_sync(kAll, rank, g << p.sub_log);
+            surely += r > above;
+            maybe += r > below;
+        }
+        stays = maybe < p.topk_group;
+        const bool gone = surely >= p.topk_group || !(rank > minus_inf());
+        // an infinite rank has no margin
+        if (__any_sync(kAll, group < p.groups && ((!stays && !gone) || rank > 1e30f))) return false;
+        stays = stays && !gone;
+    }
+    uint32_t rest = stays && top > minus_inf() ? key_of(top) : 0u, last = 0u;
+    bool all = false;   // fewer lanes than k have a candidate
+    for (int j = 0; j < p.top_k; ++j) {
+        const uint32_t m = __reduce_max_sync(kAll, rest);
+        if (m == 0u) { all = true; break; }
+        last = m;
+        if (rest == m) rest = 0u;
+    }
+    const float kth = __uint_as_float(last ^ (last & 0x80000000u ? 0x80000000u : 0xffffffffu));
+    if (last != 0u && !(fabsf(kth) < 1e30f)) return false;
+    // a lane whose group is gone compares with something that nothing reaches
+    const float lowest = -3.402823466e38f, bound = !stays ? __int_as_float(0x7fc00000) : all ? lowest : kth - (1.5e-6f + 4e-7f * fabsf(kth));
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) count += c[i] >= bound;
+    int before = count;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(kAll, before, o);
+        if (lane >= o) before += t;
+    }
+    const int found = __shfl_sync(kAll, before, 31);
+    if (found > 32) return false;
+    before -= count;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        if (c[i] >= bound) {
+            list_logit[before] = l[i];
+            list_id[before] = first + i;
+            ++before;
+        }
+    }
+    __syncwarp();
+    float exact = 0.0f;
+    int id = -1, place = lane;
+    unsigned long long own = 0ull;
+    if (lane < found) {
+        id = list_id[lane];
+        exact = sigmoid(list_logit[lane]);
+        const float choice = p.bias ? __fadd_rn(exact, __ldg(p.bias + id)) : exact;
+        own = (unsigned long long)key_of(choice) << 32 | (uint32_t)~id;
+    }
+    list_key[lane] = own;
+    __syncwarp();
+    if (lane < found) {
+        place = 0;
+        for (int q = 0; q < found; q += 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) place += list_key[q + e] > own;
+        }
+    }
+    float w = place < p.top_k && id >= 0 ? exact : 0.0f;
+    if (p.renormalize) {
+        const float sum = warp_sum(w);
+        w = sum > 0.0f ? __fdiv_rn(w, sum) : 0.0f;
+    }
+    if (place < p.top_k) put(p, out + place, __fmul_rn(w, p.scale), id);
+    return true;
+}
+
 // SCORED: c is computed for every expert, else it is the logit.  R: experts per lane, at least p.per.
 template <int R, bool SIGMOID, bool SCORED, bool TOP2>
 __global__ void __launch_bounds__(32 * kWarps) route_kernel(const RouteParams p)
 {
     __shared__ unsigned long long list_key[kWarps][32];   // key, then the id with its bits inverted: equal keys order by the lower id
     __shared__ float list_logit[kWarps][32];
+    __shared__ int list_id[kWarps][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int row = blockIdx.x * kWarps + warp;
     if (row >= p.rows) return;
@@ -117,7 +231,7 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(const RouteParams p)
         if (lane < p.top_k) put(p, out + lane, 0.0f, -1);
         return;
     }
-    const int group = lane / p.sub, inside = (lane % p.sub) * p.per;
+    const int group = lane >> p.sub_log, inside = (lane & (p.sub - 1)) * p.per;
     const int first = group * p.group_size + inside;
     const int mine = group < p.groups ? max(0, min(p.per, p.group_size - inside)) : 0;
     float l[R];
@@ -148,8 +262,6 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(const RouteParams p)
     }
     // without SCORED and with renormalisation the sum over all experts cancels: total stays 1
     const auto score = [&](float v) { return SIGMOID ? sigmoid(v) : __fdiv_rn(exp_below(v, top), total); };
-    float best = minus_inf(), second = minus_inf();
-    uint32_t key[R];
     float bias[R];
     if (SCORED && p.bias) {
         if (p.whole) {
@@ -159,6 +271,12 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(const RouteParams p)
             for (int i = 0; i < R; ++i) bias[i] = i < mine ? __ldg(p.bias + first + i) : 0.0f;
         }
     }
+    if constexpr (SIGMOID && SCORED) {
+        if (route_about<R, TOP2>(p, l, bias, group, first, out, list_key[warp], list_logit[warp], list_id[warp])) return;
+        __syncwarp();
+    }
+    float best = minus_inf(), second = minus_inf();
+    uint32_t key[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         float c = l[i];
@@ -304,7 +422,8 @@ cudaError_t route_top_k_launch(const RouteTopKProblem &r, cudaStream_t stream)
     p.rows = (int)r.rows; p.experts = r.experts; p.top_k = r.top_k;
     p.groups = r.n_group; p.group_size = r.experts / r.n_group; p.topk_group = r.topk_group;
     p.sub = 32;
-    while (p.sub * p.groups > 32) p.sub >>= 1;
+    p.sub_log = 5;
+    while (p.sub * p.groups > 32) { p.sub >>= 1; --p.sub_log; }
     p.per = (p.group_size + p.sub - 1) / p.sub;   // below 2 * 1024 / 32: more than half of the lanes have a group
     p.renormalize = r.renormalize; p.ids_i64 = r.ids_i64;
     p.scale = r.scale; p.weights = r.weights; p.ids = r.ids;

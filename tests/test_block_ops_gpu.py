@@ -515,3 +515,46 @@ def test_adapter_large_tiles(T, L, r):
     for x_i8 in (False, True):
         c = adapter_case(T, 1032, 520, L, r, BF16, x_i8)
         check_adapter(c, ops.adapter_add(**c))
+
+
+def test_route_choices_that_hang_on_the_last_bits():
+    """Sigmoid scores with a bias whose differences are of the size of their rounding: the choice is the one of scores that are rounded as
+    the definition says (torch's elementwise operations round the same), ties go to the lowest id."""
+    T, E = 512, 256
+    base = randn((T, 1), 1) * 2
+    for step in (0.0, 1e-7, 3e-7, 1e-6, 4e-6):
+        logits = base + step * torch.randint(-3, 4, (T, E), device=DEV, generator=gen(2))
+        for bias in (torch.zeros(E, device=DEV), torch.randint(-2, 3, (E,), device=DEV, generator=gen(3)) * 1e-7, torch.full((E,), 3.0, device=DEV)):
+            choice = 1.0 / (1.0 + torch.exp(-logits)) + bias
+            want = choice.sort(dim=1, descending=True, stable=True).indices[:, :8]
+            assert torch.equal(ops.route_top_k(logits, 8, scoring="sigmoid", bias=bias)[1].long(), want)
+            for score in ("max", "top2"):
+                best = choice.view(T, 8, 32).sort(dim=2, descending=True).values
+                rank = best[..., 0] if score == "max" else best[..., 0] + best[..., 1]
+                place = rank.argsort(dim=1, descending=True, stable=True).argsort(dim=1)
+                kept = torch.where((place < 3).repeat_interleave(32, 1), choice, -math.inf)
+                want = kept.sort(dim=1, descending=True, stable=True).indices[:, :8]
+                got = ops.route_top_k(logits, 8, scoring="sigmoid", bias=bias, n_group=8, topk_group=3, group_score=score)[1]
+                assert torch.equal(got.long(), want)
+
+
+@pytest.mark.parametrize("group_score", ["max", "top2"])
+def test_route_groups_with_special_biases(group_score):
+    T, E = 300, 64
+    logits = randn((T, E), 1)
+    logits[7, 8:24] = -math.inf
+    bias = randn((E,), 2, scale=0.1)
+    bias[3] = bias[9] = math.nan
+    bias[17] = -math.inf
+    bias[32:40] = math.nan       # a group without an expert
+    for scoring in ("sigmoid", "softmax"):
+        w, ids = route(logits, 5, scoring=scoring, bias=bias, n_group=8, topk_group=3, group_score=group_score)
+        assert not torch.isin(ids.long(), torch.tensor([3, 9, 17] + list(range(32, 40)), device=DEV)).any()
+        big = bias.nan_to_num(0.0, 0.0, 0.0)
+        big[20] = math.inf
+        _, ids = ops.route_top_k(logits, 5, scoring=scoring, bias=big, n_group=8, topk_group=3, group_score=group_score)
+        live = torch.arange(T, device=DEV) != 7
+        assert (ids[live, 0] == 20).all() and not (ids[7] == 20).any()
+        big[60] = math.inf       # two groups without bounds, one of which stays
+        _, ids = ops.route_top_k(logits, 5, scoring=scoring, bias=big, n_group=8, topk_group=1, group_score=group_score)
+        assert ((ids[live] >= 16) & (ids[live] < 24)).all()
