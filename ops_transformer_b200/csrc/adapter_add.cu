@@ -13,9 +13,8 @@
 // The operands are fetched with 16-byte asynchronous copies (8, 4 or 2 bytes where rows start on no such boundary), straight into the
 // 128-byte-swizzled layout that the tensor cores read; a row's tail is zero filled.
 //
-// Which tokens share an adapter is found on the device.  Up to kSelfPlan tokens every CTA ranks the tokens among those of their
-// adapter itself, beside its first loads; beyond, a one-CTA kernel counts and sorts them.  The order within an adapter does not matter:
-// every row's arithmetic is its own.
+// Which tokens share an adapter is found on the device: by a one-CTA kernel that counts and sorts them, or, where few tokens come to an
+// adapter, by every CTA for its own token.  The order within an adapter does not matter: every row's arithmetic is its own.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -29,7 +28,7 @@ namespace {
 constexpr int kBlockK = 128;         // elements of a row per K block
 constexpr int kBlockTiles = kBlockK / 64;   // swizzled rows of 128 bytes that these make
 constexpr int kChunkN = 128;         // channels per step of the second product
-constexpr int kSelfPlan = 256;       // most tokens for which every CTA finds its tile itself
+constexpr int kSelfPlan = 256;       // most tokens for which every CTA finds its tile itself, a thread for each
 constexpr int kPlanThreads = 1024;
 constexpr int kWorkers = 256;        // threads of the first kernel that copy; one warp more issues the products
 __host__ __device__ constexpr int expand_workers(int tn) { return tn == 64 ? 512 : 256; }
@@ -658,11 +657,10 @@ inline int shrink_smem(int tn, int rank_pad, bool i8)
 // out once; with the addresses of every copy worked out anew the kernel was bound by its instructions.
 // The products are issued by a warp of their own, which also orders them behind the copies (fence.proxy.async).  What bounds the kernel
 // is that thread: a product of 128 x 64 x 16 costs it 0.05 us, a block's barriers and fence 0.27; so blocks are 128 deep.
-template <typename T, bool I8, int TN, bool SELF, bool FAST>
+template <typename T, bool I8, int TN, bool FAST>
 __global__ void __launch_bounds__(kWorkers + 32) adapter_shrink_kernel(const AdapterParams p)
 {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ alignas(16) SelfPlan plan;
     __shared__ alignas(8) uint64_t full[kMaxStages], empty[kMaxStages], done;
     __shared__ uint32_t tmem_base;
     __shared__ int gave_up;
@@ -679,16 +677,14 @@ __global__ void __launch_bounds__(kWorkers + 32) adapter_shrink_kernel(const Ada
         mbar_init(smem_u32(&done), 1);
         gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        if (SELF && blockIdx.x == 0 && blockIdx.y == 0)   // long before a wait can run out and record it
-            for (int i = 0; i < 4; ++i) p.status[i] = 0;
     }
     tc_fence_before();
-    if (!SELF) pdl_wait();
+    pdl_wait();
     // Only now: the next kernel's CTAs wait for this grid with tensor memory in their hands, so every CTA of this one has its own first.
     __syncthreads();
     pdl_release();
     tc_fence_after();
-    const Tile tile = SELF ? self_plan<TN>(p, plan, rows) : read_plan<TN>(p, 1, kWorkers + 32, rows);
+    const Tile tile = read_plan<TN>(p, 1, kWorkers + 32, rows);
     const int blocks = (p.k + kBlockK - 1) / kBlockK;
     const int kb0 = (int)((long long)blockIdx.y * blocks / p.ksplit), kb1 = (int)((long long)(blockIdx.y + 1) * blocks / p.ksplit);
     const bool work = tile.count > 0 && tile.adapter >= 0;   // kb0 < kb1, since ksplit is at most blocks
@@ -843,11 +839,10 @@ inline int expand_smem(int tn, int rank_pad) { return 1024 + rank_atoms(rank_pad
 // Grid: (tiles, nsplit).  CTA y takes the channel chunks [y * chunks / nsplit, (y + 1) * chunks / nsplit).
 // GB: 16 or 8 bytes of b a copy, with rows of base and out on 16-byte boundaries; addresses are worked out once, and results go back
 // through the chunk's base rows in shared memory, from which they are stored 16 bytes at a time.  0: any strides.
-template <typename T, int TN, bool SELF, int GB>
+template <typename T, int TN, int GB>
 __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) adapter_expand_kernel(const AdapterParams p)
 {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ alignas(16) SelfPlan plan;
     __shared__ alignas(8) uint64_t full[kExpandStages], acc_full[2], acc_empty[2], v_full;
     __shared__ uint32_t tmem_base;
     __shared__ int gave_up;
@@ -872,7 +867,7 @@ __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) ada
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const Tile tile = SELF ? self_plan<TN>(p, plan, rows) : read_plan<TN>(p, p.parts, THREADS, rows);
+    const Tile tile = read_plan<TN>(p, p.parts, THREADS, rows);
     const int chunks = (p.n + kChunkN - 1) / kChunkN;
     const int c0 = (int)((long long)blockIdx.y * chunks / p.nsplit), c1 = (int)((long long)(blockIdx.y + 1) * chunks / p.nsplit);
     const T *base = reinterpret_cast<const T *>(p.base);
@@ -1156,57 +1151,54 @@ int grain_of(const void *base, long long pitch_bytes, int smallest)
 
 struct Shape {
     int tile_tokens, tiles, ksplit, nsplit, rank_pad;
-    bool self, few;
+    bool few;
 };
 
-// Tiles of 4 tokens on the CUDA cores where adapters have no more on average, else of 16 while every CTA plans for itself, beyond of 64 or, where adapters have that many tokens on average and there are
-// enough of them for the SMs, of 128 (up to rank 64, for the sake of three stages): the first product reads 128 rows of the tokens' tile whether they are tokens or not.  `tiles` is the
-// most there can be: full ones, and one that is not for every adapter and for none.  K and N are split so that the CTAs find a place on the
-// SMs together (about four of the small ones fit an SM, two of the next, one of the large).
+// Tiles of 4 tokens on the CUDA cores where adapters have no more on average, else of 16 or 64 or, where adapters have that many on average
+// and there are enough of them for the SMs, of 128 (up to rank 64, for the sake of three stages): the first product reads 128 rows of the
+// tokens' tile whether they are tokens or not.  `tiles` is the most there can be: full ones, and one that is not for every adapter and for
+// none; a tile on the CUDA cores may begin with any token.  K and N are split so that the CTAs find a place on the SMs together (four of
+// the first kernel's small ones fit an SM, two of the next, one of the large; two of the second's).
 Shape shape_of(const AdapterProblem &p, bool may_be_few = true)
 {
     Shape s;
-    s.self = p.rows <= kSelfPlan;
-    const long long partial = p.adapters + 1 < p.rows ? p.adapters + 1 : p.rows;
-    // as many tokens as four per adapter, and rows that can be read 16 bytes at a time
     const int xb = p.x_i8 ? 1 : 2;
-    s.few = may_be_few && s.self && (p.rows <= kFew || p.rows <= kFew * p.adapters) && grain_of(p.x, p.ld_x * xb, 1) >= 8 * xb && grain_of(p.a, p.k * 2, 1) == 16 &&
-            grain_of(p.b, p.rank * 2, 1) == 16;
-    s.tile_tokens = s.few ? kFew : s.self ? 16 : p.rows >= 2048 && p.rows >= 128 * p.adapters && p.rank <= 64 ? 128 : 64;
+    // rows that can be read 16 bytes at a time
+    s.few = may_be_few && p.rows <= kSelfPlan && (p.rows <= kFew || p.rows <= kFew * p.adapters) && grain_of(p.x, p.ld_x * xb, 1) >= 8 * xb &&
+            grain_of(p.a, p.k * 2, 1) == 16 && grain_of(p.b, p.rank * 2, 1) == 16;
+    const long long groups = p.adapters < p.rows ? p.adapters : p.rows, partial = p.adapters + 1 < p.rows ? p.adapters + 1 : p.rows;
+    s.tile_tokens = s.few ? kFew : p.rows >= 2048 && p.rows >= 128 * groups && p.rank <= 64 ? 128 : p.rows > 16 * groups ? 64 : 16;
     s.tiles = (int)(p.rows / s.tile_tokens + partial);
-    if (s.self || s.tiles > p.rows) s.tiles = (int)p.rows;   // any token may begin one
+    if (s.few || s.tiles > p.rows) s.tiles = (int)p.rows;
     s.rank_pad = align_up((int)p.rank, 16);
-    const int places = (s.self ? 4 : s.tile_tokens == 64 ? 2 : 1) * 148;
+    const int per_sm = s.tile_tokens == 16 ? 4 : s.tile_tokens == 64 ? 2 : 1;
     const int likely = (int)(p.rows / s.tile_tokens + partial / 2) > 0 ? (int)(p.rows / s.tile_tokens + partial / 2) : 1;
     const int blocks = (int)((p.k + kBlockK - 1) / kBlockK), chunks = (int)((p.n + kChunkN - 1) / kChunkN);
     s.ksplit = 1;
-    while (s.ksplit < 8 && 2 * s.ksplit * likely <= places && 2 * s.ksplit <= blocks) s.ksplit *= 2;
+    while (s.ksplit < 4 && 2 * s.ksplit * likely <= per_sm * 148 && 2 * s.ksplit <= blocks) s.ksplit *= 2;   // four sums are fetched at a time
     const int want = 2 * 148 / (s.tile_tokens == 128 ? 2 * likely : likely);
     s.nsplit = want < chunks ? want : chunks;
     if (s.few) {
-        const int units = (int)((p.n + kFewChannels - 1) / kFewChannels), busy = (int)(p.rows < p.adapters ? p.rows : p.adapters);
+        const int units = (int)((p.n + kFewChannels - 1) / kFewChannels), places = kFewExpandCtas * 148 / (int)groups;
         s.ksplit = 1;
-        s.nsplit = kFewExpandCtas * 148 / busy < units ? kFewExpandCtas * 148 / busy : units;   // one wave: every CTA looks for its tile first
+        s.nsplit = places < units ? places : units;   // one wave: every CTA looks for its tile first
     }
     if (s.nsplit < 1) s.nsplit = 1;
     return s;
 }
 
-template <typename T, bool I8, int TN, bool SELF>   // TN: tokens of the first kernel's tiles; the second one's have at most 64
+template <typename T, bool I8, int TN>   // TN: tokens of the first kernel's tiles; the second one's have at most 64
 cudaError_t launch_tiles(const AdapterParams &p, const Shape &s, cudaStream_t stream)
 {
-    cudaError_t e = cudaSuccess;
-    if (!SELF) {
-        e = launch_kernel(adapter_plan_kernel, dim3(1), kPlanThreads, (p.adapters + 1) * 4, stream, false, p, s.tile_tokens);
-        if (e != cudaSuccess) return e;
-    }
-    const auto shrink = p.grain_x == 16 && p.grain_a == 16 ? adapter_shrink_kernel<T, I8, TN, SELF, true> : adapter_shrink_kernel<T, I8, TN, SELF, false>;
-    e = launch_kernel(shrink, dim3((unsigned)s.tiles, (unsigned)s.ksplit), kWorkers + 32, shrink_smem(TN, s.rank_pad, I8), stream, !SELF, p);
+    cudaError_t e = launch_kernel(adapter_plan_kernel, dim3(1), kPlanThreads, (p.adapters + 1) * 4, stream, false, p, s.tile_tokens);
+    if (e != cudaSuccess) return e;
+    const auto shrink = p.grain_x == 16 && p.grain_a == 16 ? adapter_shrink_kernel<T, I8, TN, true> : adapter_shrink_kernel<T, I8, TN, false>;
+    e = launch_kernel(shrink, dim3((unsigned)s.tiles, (unsigned)s.ksplit), kWorkers + 32, shrink_smem(TN, s.rank_pad, I8), stream, true, p);
     if (e != cudaSuccess) return e;
     const bool rows16 = p.grain_base == 16 && p.grain_out == 16 && p.n % 8 == 0;
     constexpr int EN = TN < 64 ? TN : 64;
-    const auto expand = rows16 && p.grain_b == 16 ? adapter_expand_kernel<T, EN, SELF, 16>
-                        : rows16 && p.grain_b == 8 ? adapter_expand_kernel<T, EN, SELF, 8> : adapter_expand_kernel<T, EN, SELF, 0>;
+    const auto expand = rows16 && p.grain_b == 16 ? adapter_expand_kernel<T, EN, 16>
+                        : rows16 && p.grain_b == 8 ? adapter_expand_kernel<T, EN, 8> : adapter_expand_kernel<T, EN, 0>;
     return launch_kernel(expand, dim3((unsigned)(s.tiles * p.parts), (unsigned)s.nsplit), expand_workers(EN) + 32, expand_smem(EN, s.rank_pad), stream, true, p);
 }
 
@@ -1220,8 +1212,8 @@ cudaError_t launch_typed(const AdapterParams &p, const Shape &s, cudaStream_t st
                             : p.rank <= 32 ? adapter_few_expand_kernel<T, 4> : p.rank <= 64 ? adapter_few_expand_kernel<T, 8> : adapter_few_expand_kernel<T, 16>;
         return launch_kernel(expand, dim3((unsigned)s.tiles, (unsigned)s.nsplit), kFewThreads, 0, stream, true, p);
     }
-    if (s.self) return launch_tiles<T, I8, 16, true>(p, s, stream);
-    return s.tile_tokens == 64 ? launch_tiles<T, I8, 64, false>(p, s, stream) : launch_tiles<T, I8, 128, false>(p, s, stream);
+    return s.tile_tokens == 16 ? launch_tiles<T, I8, 16>(p, s, stream)
+           : s.tile_tokens == 64 ? launch_tiles<T, I8, 64>(p, s, stream) : launch_tiles<T, I8, 128>(p, s, stream);
 }
 
 }  // namespace
@@ -1232,7 +1224,7 @@ size_t adapter_workspace_bytes(const AdapterProblem &p)
     size_t most = 0;
     for (const bool few : {false, true}) {
         const Shape s = shape_of(p, few);
-        const size_t bytes = 256 + (s.self ? 0 : 256 + align256((size_t)s.tiles * sizeof(int2)) + align256((size_t)s.tiles * s.tile_tokens * 4)) +
+        const size_t bytes = 256 + (s.few ? 0 : 256 + align256((size_t)s.tiles * sizeof(int2)) + align256((size_t)s.tiles * s.tile_tokens * 4)) +
                              align256((size_t)s.ksplit * (size_t)p.rows * (size_t)s.rank_pad * 4);
         if (bytes > most) most = bytes;
     }
@@ -1261,7 +1253,7 @@ cudaError_t adapter_launch(const AdapterProblem &a, void *workspace, size_t work
     p.status = reinterpret_cast<int *>(ws);
     ws += 256;
     p.n_tiles = nullptr; p.tiles = nullptr; p.order = nullptr;
-    if (!s.self) {
+    if (!s.few) {
         p.n_tiles = reinterpret_cast<int *>(ws); ws += 256;
         p.tiles = reinterpret_cast<int2 *>(ws); ws += align256((size_t)s.tiles * sizeof(int2));
         p.order = reinterpret_cast<int *>(ws); ws += align256((size_t)s.tiles * s.tile_tokens * 4);
