@@ -757,18 +757,18 @@ __global__ void __launch_bounds__(kWorkers + 32) adapter_shrink_kernel(const Ada
                     from += a_step;
                 }
             } else {
-            for (int at = 0; at < kBlockTiles; ++at) {
-                const long long k0 = (long long)kb * kBlockK + at * 64;
-                if (at * 64 >= (have + 15) / 16 * 16) break;   // no K step reaches the tile
-                copy_rows<true, kWorkers>(p.grain_a, s + a_tile + (uint32_t)(at * p.rank_pad * 128), p.rank, 128, (have - at * 64) * 2,
-                                          [&](int r) { return a + ((long long)r * p.k + k0) * 2; });
-                if (!I8)
-                    copy_rows<true, kWorkers>(p.grain_x, s + (uint32_t)(at * TN * 128), tile.count, 128, (have - at * 64) * 2,
-                                              [&](int r) { return x + ((long long)rows[r] * p.ld_x + k0) * XB; });
-            }
-            if (I8)
-                copy_rows<false, kWorkers>(p.grain_x, s + raw_tile, tile.count, kBlockK, have,
-                                           [&](int r) { return x + (long long)rows[r] * p.ld_x + (long long)kb * kBlockK; });
+                for (int at = 0; at < kBlockTiles; ++at) {
+                    const long long k0 = (long long)kb * kBlockK + at * 64;
+                    if (at * 64 >= (have + 15) / 16 * 16) break;   // no K step reaches the tile
+                    copy_rows<true, kWorkers>(p.grain_a, s + a_tile + (uint32_t)(at * p.rank_pad * 128), p.rank, 128, (have - at * 64) * 2,
+                                              [&](int r) { return a + ((long long)r * p.k + k0) * 2; });
+                    if (!I8)
+                        copy_rows<true, kWorkers>(p.grain_x, s + (uint32_t)(at * TN * 128), tile.count, 128, (have - at * 64) * 2,
+                                                  [&](int r) { return x + ((long long)rows[r] * p.ld_x + k0) * XB; });
+                }
+                if (I8)
+                    copy_rows<false, kWorkers>(p.grain_x, s + raw_tile, tile.count, kBlockK, have,
+                                               [&](int r) { return x + (long long)rows[r] * p.ld_x + (long long)kb * kBlockK; });
             }
         };
         // A warp's copies of block i have landed when those of the kShrinkAhead blocks behind it are all that its threads have under way;
@@ -923,14 +923,14 @@ __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) ada
                     if (base_at_row[i] >= 0 && rc < channels)
                         cp_async<16>(s + base_at + (uint32_t)((tid + i * WORKERS) * 16), base + base_at_row[i] + n0, 16);
             } else {
-            for (int at = 0; at < atoms; ++at) {
-                const int left = p.rank_pad - at * 64;                       // a whole number of K steps, zero beyond the rank
-                const int width = left > 32 ? 128 : left > 16 ? 64 : 32;
-                copy_rows<true, WORKERS>(p.grain_b, s + (uint32_t)at * kChunkN * 128, channels, width, (p.rank - at * 64) * 2,
-                                                [&](int r) { return b + ((long long)(n0 + r) * p.rank + at * 64) * 2; });
-            }
-            copy_rows<false, WORKERS>(p.grain_base, s + base_at, tile.count, kChunkN * 2, channels * 2,
-                                             [&](int r) { return reinterpret_cast<const char *>(base + (long long)rows[r] * p.ld_base + n0); });
+                for (int at = 0; at < atoms; ++at) {
+                    const int left = p.rank_pad - at * 64;                       // a whole number of K steps, zero beyond the rank
+                    const int width = left > 32 ? 128 : left > 16 ? 64 : 32;
+                    copy_rows<true, WORKERS>(p.grain_b, s + (uint32_t)at * kChunkN * 128, channels, width, (p.rank - at * 64) * 2,
+                                                    [&](int r) { return b + ((long long)(n0 + r) * p.rank + at * 64) * 2; });
+                }
+                copy_rows<false, WORKERS>(p.grain_base, s + base_at, tile.count, kChunkN * 2, channels * 2,
+                                                 [&](int r) { return reinterpret_cast<const char *>(base + (long long)rows[r] * p.ld_base + n0); });
             }
         };
         if (issuer) {
@@ -1036,7 +1036,8 @@ __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) ada
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         f[h][e] = __fmul_rn(f[h][e], down);
-                        g[e] = __fsub_rn(f[h][e], to_float(from_float<T>(f[h][e])));
+                        const float first = to_float(from_float<T>(f[h][e]));
+                        g[e] = isinf(first) ? 0.0f : __fsub_rn(f[h][e], first);   // an infinity less itself is none
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -1175,7 +1176,7 @@ Shape shape_of(const AdapterProblem &p, bool may_be_few = true)
     const int likely = (int)(p.rows / s.tile_tokens + partial / 2) > 0 ? (int)(p.rows / s.tile_tokens + partial / 2) : 1;
     const int blocks = (int)((p.k + kBlockK - 1) / kBlockK), chunks = (int)((p.n + kChunkN - 1) / kChunkN);
     s.ksplit = 1;
-    while (s.ksplit < 4 && 2 * s.ksplit * likely <= per_sm * 148 && 2 * s.ksplit <= blocks) s.ksplit *= 2;   // four sums are fetched at a time
+    while (s.ksplit < (p.k % 8 ? 8 : 4) && 2 * s.ksplit * likely <= per_sm * 148 && 2 * s.ksplit <= blocks) s.ksplit *= 2;   // four sums are fetched at a time
     const int want = 2 * 148 / (s.tile_tokens == 128 ? 2 * likely : likely);
     s.nsplit = want < chunks ? want : chunks;
     if (s.few) {

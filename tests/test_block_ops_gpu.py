@@ -558,3 +558,20 @@ def test_route_groups_with_special_biases(group_score):
         big[60] = math.inf       # two groups without bounds, one of which stays
         _, ids = ops.route_top_k(logits, 5, scoring=scoring, bias=big, n_group=8, topk_group=1, group_score=group_score)
         assert ((ids[live] >= 16) & (ids[live] < 24)).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,r", [(40, 1), (40, 17), (8, 8)])
+def test_adapter_infinite_activations(T, r, dtype):
+    # one infinite element makes the row's first product infinite, and every result of the row with it, of the sign of b
+    c = adapter_case(T, 64, 200, 2, r, dtype, ids=torch.arange(T, device=DEV, dtype=torch.int32) % 2)
+    c["a"][:, :, 5] = 0.5
+    c["b"] = c["b"].abs() + 0.25
+    c["b"][:, 1::2] *= -1
+    clean = ops.adapter_add(**c)
+    c["x"][3, 5] = float("inf")
+    out = ops.adapter_add(**c)
+    want = torch.tensor([float("inf"), -float("inf")], device=DEV, dtype=dtype).repeat(100)
+    assert torch.equal(out[3], want)
+    others = torch.arange(T, device=DEV) != 3
+    assert torch.equal(out[others], clean[others])
