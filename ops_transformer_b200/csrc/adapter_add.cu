@@ -416,8 +416,9 @@ __device__ __forceinline__ void copy_base(const AdapterParams &p, const int *row
 // ---------------------------------------------------------------------------------------------------------
 //
 // With up to four tokens a tile each weight takes part in four products at most, which costs fewer instructions than bringing it to the
-// tensor cores; the weights go straight from memory to registers, 16 bytes a lane.  128 tokens of 64 tenants, 2048 -> 7168, rank 32:
-// FEW_US us against 28 on the tensor cores.
+// tensor cores; the weights go straight from memory to registers, 16 bytes a lane, and every CTA finds its own tile, so there are two
+// kernels and nothing in front of them.  One token, 2048 -> 4096, rank 16: 4.3 us, the two kernels' latency; 128 tokens of 64 adapters,
+// 2048 -> 7168, rank 32, int8: 19.5 us (28 on the tensor cores) for 42 MB, about as many instructions as bytes.
 
 constexpr int kFew = 4;
 constexpr int kFewThreads = 256;
@@ -451,6 +452,38 @@ __device__ __forceinline__ void unpack8(const uint2 &u, f32x2 (&f)[4])
     }
 }
 
+// 16 bytes at `at`, on any boundary of a 16-bit element, of which the first `valid` count and the others are zero: out of the two aligned
+// packs that hold them, where these lie in [begin, end), else element by element.
+__device__ __forceinline__ uint4 load_any(const char *at, int valid, const char *begin, const char *end)
+{
+    if (valid <= 0) return make_uint4(0, 0, 0, 0);
+    const int shift = (int)((uintptr_t)at & 15);
+    const bool two = shift + valid > 16;
+    const char *from = at - shift;
+    uint32_t out[4] = {};
+    if (from >= begin && from + (two ? 32 : 16) <= end) {
+        const uint4 lo = __ldg(reinterpret_cast<const uint4 *>(from));
+        const uint4 hi = two ? __ldg(reinterpret_cast<const uint4 *>(from) + 1) : make_uint4(0, 0, 0, 0);
+        uint32_t w[9] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w, 0};
+#pragma unroll
+        for (int by = 2; by > 0; by >>= 1)
+            if (shift & by * 4) {
+#pragma unroll
+                for (int i = 0; i + by < 9; ++i) w[i] = w[i + by];
+            }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int keep = valid - i * 4;
+            out[i] = __funnelshift_r(w[i], w[i + 1], shift % 4 * 8) & (keep >= 4 ? ~0u : keep <= 0 ? 0u : 0xffffu);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e * 2 < valid) out[e / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(at) + e) << (e % 2 * 16);
+    }
+    return make_uint4(out[0], out[1], out[2], out[3]);
+}
+
 // fn(integral constant) for a tile of 1 to kFew tokens: with the count known to the compiler nothing stands between the loads, and all of
 // a step are under way together.
 template <typename Fn>
@@ -473,7 +506,11 @@ __global__ void __launch_bounds__(kFewThreads) adapter_few_shrink_kernel(const A
     pdl_release();
     if (tid < 4 && blockIdx.x == 0 && blockIdx.y == 0) p.status[tid] = 0;
     const Tile tile = self_plan<kFew>(p, plan, rows);
-    if (tile.count == 0 || tile.adapter < 0 || j >= p.rank) return;
+    if (tile.count == 0 || tile.adapter < 0) return;
+    if (j >= p.rank) {   // the components that the next kernel reads with the last ones
+        if (lane < tile.count) p.v[(long long)rows[lane] * p.rank_pad + j] = 0.0f;
+        return;
+    }
     const uint4 *a = reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(p.a) + ((long long)tile.adapter * p.rank + j) * p.k);
     for_count(tile.count, [&](auto tokens) {
         constexpr int C = decltype(tokens)::value, AHEAD = 4;
@@ -531,9 +568,10 @@ __global__ void __launch_bounds__(kFewThreads) adapter_few_shrink_kernel(const A
 }
 
 // Grid: (tiles, nsplit), channels in units of kFewChannels.  LANES neighbouring lanes (the power of two that holds rank / 8) share a
-// channel's row of b, 8 components each, and add their sums up; of the tokens' results each then stores its share.
+// channel's row of b, 8 components each, and add their sums up; of the tokens' results each then stores its share.  ANY: rows of b on any
+// boundary.
 constexpr int kFewChannels = 256;
-template <typename T, int LANES>
+template <typename T, int LANES, bool ANY>
 __global__ void __launch_bounds__(kFewThreads) adapter_few_expand_kernel(const AdapterParams p)
 {
     __shared__ alignas(16) SelfPlan plan;
@@ -557,11 +595,17 @@ __global__ void __launch_bounds__(kFewThreads) adapter_few_expand_kernel(const A
     const T *b = reinterpret_cast<const T *>(p.b) + (long long)tile.adapter * p.n * p.rank + part * 8;
     const T *base = reinterpret_cast<const T *>(p.base);
     T *out = reinterpret_cast<T *>(p.out);
+    const char *b0 = reinterpret_cast<const char *>(p.b), *b1 = b0 + (long long)p.adapters * p.n * p.rank * 2;
+    const int have = min(16, (p.rank - part * 8) * 2);   // bytes of a channel's row
+    const auto at = [&](int c) { return reinterpret_cast<const char *>(b + (long long)c * p.rank); };
     int c = n0 + warp * ACROSS + lane / LANES;
     uint4 w[AHEAD];
+    const auto fetch = [&](int u, int c) {
+        if (ANY) w[u] = load_any(at(c), mine && c < n1 ? have : 0, b0, b1);
+        else w[u] = mine && c < n1 ? __ldg(reinterpret_cast<const uint4 *>(at(c))) : make_uint4(0, 0, 0, 0);
+    };
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u)
-        w[u] = mine && c + u * STRIDE < n1 ? __ldg(reinterpret_cast<const uint4 *>(b + (long long)(c + u * STRIDE) * p.rank)) : make_uint4(0, 0, 0, 0);
+    for (int u = 0; u < AHEAD; ++u) fetch(u, c + u * STRIDE);
     pdl_wait();   // v is complete
     for_count(tile.count, [&](auto tokens) {
         constexpr int C = decltype(tokens)::value, OWN = (C + LANES - 1) / LANES;   // tokens that a lane stores: part, part + LANES, ...
@@ -597,10 +641,9 @@ __global__ void __launch_bounds__(kFewThreads) adapter_few_expand_kernel(const A
             fetch_base(c + AHEAD * STRIDE);
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                const int next = c + (u + AHEAD) * STRIDE;
                 f32x2 f[4];
                 unpack8<T>(w[u], f);
-                if (mine && next < n1) w[u] = __ldg(reinterpret_cast<const uint4 *>(b + (long long)next * p.rank));
+                fetch(u, c + (u + AHEAD) * STRIDE);
 #pragma unroll
                 for (int t = 0; t < C; ++t) {
                     f32x2 s2 = 0;
@@ -772,7 +815,7 @@ __global__ void __launch_bounds__(kWorkers + 32) adapter_shrink_kernel(const Ada
             }
         };
         // A warp's copies of block i have landed when those of the kShrinkAhead blocks behind it are all that its threads have under way;
-        // one lane says so (an arrival per thread, as copies make by themselves, takes as long as the block's copies).
+        // one lane says so.
         const auto landed = [&](int stage) {
             const uint32_t s = smem0 + (uint32_t)stage * stage_bytes;
             if (I8 && FAST) widen_rows_grain<T, 16, kWorkers>(s + raw_tile, s, TN * 128, tile.count);
@@ -837,8 +880,9 @@ __host__ __device__ inline int expand_stage(int tn, int rank_pad) { return rank_
 inline int expand_smem(int tn, int rank_pad) { return 1024 + rank_atoms(rank_pad) * tn * 256 + kExpandStages * expand_stage(tn, rank_pad); }
 
 // Grid: (tiles, nsplit).  CTA y takes the channel chunks [y * chunks / nsplit, (y + 1) * chunks / nsplit).
-// GB: 16 or 8 bytes of b a copy, with rows of base and out on 16-byte boundaries; addresses are worked out once, and results go back
-// through the chunk's base rows in shared memory, from which they are stored 16 bytes at a time.  0: any strides.
+// GB 16: rows of b, base and out on 16-byte boundaries; addresses are worked out once, and results go back through the chunk's base rows in
+// shared memory, from which they are stored 16 bytes at a time.  2: the same with rows of b on any boundary, by way of registers (rank 61
+// beside 64, 3000 tokens: 44 us and 35; element by element, as with 0, 64).  0: any strides.
 template <typename T, int TN, int GB>
 __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) adapter_expand_kernel(const AdapterParams p)
 {
@@ -855,7 +899,7 @@ __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) ada
     const bool issuer = tid >= WORKERS;
     if (issuer) tmem_alloc(&tmem_base, COLS);
     if (tid == 0) {
-        for (int i = 0; i < kExpandStages; ++i) mbar_init(smem_u32(&full[i]), WORKERS);
+        for (int i = 0; i < kExpandStages; ++i) mbar_init(smem_u32(&full[i]), GB == 2 ? 2 * WORKERS : WORKERS);
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&acc_full[i]), 1);
             mbar_init(smem_u32(&acc_empty[i]), WORKERS / 32);
@@ -884,8 +928,8 @@ __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) ada
         const uint32_t stage_bytes = expand_stage(TN, p.rank_pad), base_at = (uint32_t)(atoms * kChunkN * 128);
         const char *b = reinterpret_cast<const char *>(p.b) + (long long)tile.adapter * p.n * p.rank * 2;
         // b: the copies of a chunk, offset in its rows << 8 | bytes, and place in the tile
-        constexpr int NB = GB ? 256 * kChunkN / ((GB ? GB : 1) * WORKERS) : 1, NR = TN * 16 / WORKERS;
-        const int per_row = GB ? p.rank_pad * 2 / (GB ? GB : 1) : 1, nb = (per_row * kChunkN + WORKERS - 1) / WORKERS;
+        constexpr int NB = 16 * kChunkN / WORKERS, NR = TN * 16 / WORKERS;
+        const int per_row = p.rank_pad / 8, nb = (per_row * kChunkN + WORKERS - 1) / WORKERS;
         uint32_t b_from[NB], b_to[NB];
         long long base_at_row[NR], out_at_row[NR];
         const int rc = (tid % 16) * 8;
@@ -894,8 +938,8 @@ __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) ada
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
                 if (i >= nb) break;
-                const int idx = tid + i * WORKERS, r = (int)(((float)idx + 0.5f) * across), byte = (idx - r * per_row) * GB;   // exact for idx < 2^12
-                const int valid = min(max(p.rank * 2 - byte, 0), GB);
+                const int idx = tid + i * WORKERS, r = (int)(((float)idx + 0.5f) * across), byte = (idx - r * per_row) * 16;   // exact for idx < 2^12
+                const int valid = min(max(p.rank * 2 - byte, 0), 16);
                 // one too many lies behind every chunk's end
                 b_from[i] = idx < per_row * kChunkN ? (uint32_t)(r * p.rank * 2 + (valid ? byte : 0)) << 8 | (uint32_t)valid : ~0u;
                 b_to[i] = (uint32_t)(byte / 128 * kChunkN * 128) + swizzled(r, byte % 128);
@@ -913,10 +957,15 @@ __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) ada
             if constexpr (GB != 0) {
                 const char *from = b + (long long)n0 * p.rank * 2;
                 const uint32_t end = (uint32_t)(channels * p.rank * 2);
+                const char *b0 = reinterpret_cast<const char *>(p.b), *b1 = b0 + (long long)p.adapters * p.n * p.rank * 2;
 #pragma unroll
                 for (int i = 0; i < NB; ++i) {
                     if (i >= nb) break;
-                    if (b_from[i] >> 8 < end) cp_async<GB ? GB : 16>(s + b_to[i], from + (b_from[i] >> 8), (int)(b_from[i] & 255u));
+                    if (b_from[i] >> 8 >= end) continue;
+                    if constexpr (GB == 2) {
+                        const uint4 w = load_any(from + (b_from[i] >> 8), (int)(b_from[i] & 255u), b0, b1);
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(s + b_to[i]), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+                    } else cp_async<16>(s + b_to[i], from + (b_from[i] >> 8), (int)(b_from[i] & 255u));
                 }
 #pragma unroll
                 for (int i = 0; i < NR; ++i)
@@ -957,9 +1006,10 @@ __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) ada
                 __syncwarp();
             }
         } else {
-            // Copies through shared memory by whole 16 or 8 bytes announce themselves; others are waited for, a chunk ahead.
+            // Copies through shared memory by whole 16 bytes announce themselves; others are waited for, a chunk ahead.
             const auto announce = [&](int c) {
                 if (GB) mbar_arrive_copies(smem_u32(&full[(c - c0) % kExpandStages]));
+                if (GB == 2) mbar_arrive(smem_u32(&full[(c - c0) % kExpandStages]));
             };
             const auto landed = [&](int c) {
                 if (GB) return;
@@ -1155,19 +1205,25 @@ struct Shape {
     bool few;
 };
 
-// Tiles of 4 tokens on the CUDA cores where adapters have no more on average, else of 16 or 64 or, where adapters have that many on average
-// and there are enough of them for the SMs, of 128 (up to rank 64, for the sake of three stages): the first product reads 128 rows of the
-// tokens' tile whether they are tokens or not.  `tiles` is the most there can be: full ones, and one that is not for every adapter and for
-// none; a tile on the CUDA cores may begin with any token.  K and N are split so that the CTAs find a place on the SMs together (four of
-// the first kernel's small ones fit an SM, two of the next, one of the large; two of the second's).
-Shape shape_of(const AdapterProblem &p, bool may_be_few = true)
+// On the CUDA cores, in tiles of 4 tokens: up to kSelfPlan tokens while all tiles together read no more than `limit` elements of weights.
+// They read them anew for every tile, at about 10 us per 10 million elements beyond the first 5; the tensor cores' way reads them once,
+// but takes a third kernel and some 0.3 us per adapter.  2048 -> 2048, rank 16: 16 tokens of 4 adapters 6.5 us and 10.6, 128 of 128 8.7
+// and 21; 4096 -> 4096, rank 64: 32 of 8 12.9 and 16.3, 64 of 8 18.0 and 17.9, 128 of 8 27 and 19, 128 of 128 40 and 40.
+//
+// Else tiles of 16 tokens, of 64 where adapters have more than 16 on average (2000 of 4 adapters 21 us, 31 with tiles of 16; 128 of 64 29,
+// 36 with tiles of 64) or, where they have 128 and there are enough tiles for the SMs, of 128 (4096 of 8 49.7, 51.9 with tiles of 64; up to
+// rank 64, for the sake of three stages): the first product reads 128 rows of the tokens' tile whether they are tokens or not.  `tiles` is
+// the most there can be: full ones, and one that is not for every adapter and for none; a tile on the CUDA cores may begin with any token.
+// K and N are split so that the CTAs find a place on the SMs together (four of the first kernel's small ones fit an SM, two of the next,
+// one of the large; two of the second's).  Rows that are not copied 16 bytes at a time take longer, so K is split further there (300
+// tokens, 1001 -> 3001: 22 us, 29 with four splits).
+Shape shape_of(const AdapterProblem &p, bool may_be_few)
 {
     Shape s;
-    const int xb = p.x_i8 ? 1 : 2;
-    // rows that can be read 16 bytes at a time
-    s.few = may_be_few && p.rows <= kSelfPlan && (p.rows <= kFew || p.rows <= kFew * p.adapters) && grain_of(p.x, p.ld_x * xb, 1) >= 8 * xb &&
-            grain_of(p.a, p.k * 2, 1) == 16 && grain_of(p.b, p.rank * 2, 1) == 16;
     const long long groups = p.adapters < p.rows ? p.adapters : p.rows, partial = p.adapters + 1 < p.rows ? p.adapters + 1 : p.rows;
+    const long long fours = p.rows / kFew + groups / 2 < p.rows ? p.rows / kFew + groups / 2 : p.rows;   // tiles of four, about
+    const long long limit = 5000000 + 400000 * groups < 35000000 ? 5000000 + 400000 * groups : 35000000;
+    s.few = may_be_few && p.rows <= kSelfPlan && fours * p.rank * (p.k + p.n) <= limit;
     s.tile_tokens = s.few ? kFew : p.rows >= 2048 && p.rows >= 128 * groups && p.rank <= 64 ? 128 : p.rows > 16 * groups ? 64 : 16;
     s.tiles = (int)(p.rows / s.tile_tokens + partial);
     if (s.few || s.tiles > p.rows) s.tiles = (int)p.rows;
@@ -1176,11 +1232,11 @@ Shape shape_of(const AdapterProblem &p, bool may_be_few = true)
     const int likely = (int)(p.rows / s.tile_tokens + partial / 2) > 0 ? (int)(p.rows / s.tile_tokens + partial / 2) : 1;
     const int blocks = (int)((p.k + kBlockK - 1) / kBlockK), chunks = (int)((p.n + kChunkN - 1) / kChunkN);
     s.ksplit = 1;
-    while (s.ksplit < (p.k % 8 ? 8 : 4) && 2 * s.ksplit * likely <= per_sm * 148 && 2 * s.ksplit <= blocks) s.ksplit *= 2;   // four sums are fetched at a time
+    while (s.ksplit < (p.k % 8 ? 8 : 4) && 2 * s.ksplit * likely <= per_sm * 148 && 2 * s.ksplit <= blocks) s.ksplit *= 2;
     const int want = 2 * 148 / (s.tile_tokens == 128 ? 2 * likely : likely);
     s.nsplit = want < chunks ? want : chunks;
     if (s.few) {
-        const int units = (int)((p.n + kFewChannels - 1) / kFewChannels), places = kFewExpandCtas * 148 / (int)groups;
+        const int units = (int)((p.n + kFewChannels - 1) / kFewChannels), places = kFewExpandCtas * 148 / (int)(fours > 0 ? fours : 1);
         s.ksplit = 1;
         s.nsplit = places < units ? places : units;   // one wave: every CTA looks for its tile first
     }
@@ -1199,8 +1255,16 @@ cudaError_t launch_tiles(const AdapterParams &p, const Shape &s, cudaStream_t st
     const bool rows16 = p.grain_base == 16 && p.grain_out == 16 && p.n % 8 == 0;
     constexpr int EN = TN < 64 ? TN : 64;
     const auto expand = rows16 && p.grain_b == 16 ? adapter_expand_kernel<T, EN, 16>
-                        : rows16 && p.grain_b == 8 ? adapter_expand_kernel<T, EN, 8> : adapter_expand_kernel<T, EN, 0>;
+                        : rows16 ? adapter_expand_kernel<T, EN, 2> : adapter_expand_kernel<T, EN, 0>;
     return launch_kernel(expand, dim3((unsigned)(s.tiles * p.parts), (unsigned)s.nsplit), expand_workers(EN) + 32, expand_smem(EN, s.rank_pad), stream, true, p);
+}
+
+template <typename T, bool ANY>
+cudaError_t launch_few_expand(const AdapterParams &p, const Shape &s, cudaStream_t stream)
+{
+    const auto expand = p.rank <= 8 ? adapter_few_expand_kernel<T, 1, ANY> : p.rank <= 16 ? adapter_few_expand_kernel<T, 2, ANY>
+                        : p.rank <= 32 ? adapter_few_expand_kernel<T, 4, ANY> : p.rank <= 64 ? adapter_few_expand_kernel<T, 8, ANY> : adapter_few_expand_kernel<T, 16, ANY>;
+    return launch_kernel(expand, dim3((unsigned)s.tiles, (unsigned)s.nsplit), kFewThreads, 0, stream, true, p);
 }
 
 template <typename T, bool I8>
@@ -1209,9 +1273,7 @@ cudaError_t launch_typed(const AdapterParams &p, const Shape &s, cudaStream_t st
     if (s.few) {
         const cudaError_t e = launch_kernel(adapter_few_shrink_kernel<T, I8>, dim3((unsigned)s.tiles, (unsigned)((p.rank + 7) / 8)), kFewThreads, 0, stream, false, p);
         if (e != cudaSuccess) return e;
-        const auto expand = p.rank <= 8 ? adapter_few_expand_kernel<T, 1> : p.rank <= 16 ? adapter_few_expand_kernel<T, 2>
-                            : p.rank <= 32 ? adapter_few_expand_kernel<T, 4> : p.rank <= 64 ? adapter_few_expand_kernel<T, 8> : adapter_few_expand_kernel<T, 16>;
-        return launch_kernel(expand, dim3((unsigned)s.tiles, (unsigned)s.nsplit), kFewThreads, 0, stream, true, p);
+        return p.grain_b == 16 ? launch_few_expand<T, false>(p, s, stream) : launch_few_expand<T, true>(p, s, stream);
     }
     return s.tile_tokens == 16 ? launch_tiles<T, I8, 16>(p, s, stream)
            : s.tile_tokens == 64 ? launch_tiles<T, I8, 64>(p, s, stream) : launch_tiles<T, I8, 128>(p, s, stream);
@@ -1236,7 +1298,7 @@ cudaError_t adapter_launch(const AdapterProblem &a, void *workspace, size_t work
 {
     if (a.rows <= 0) return cudaSuccess;
     if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < adapter_workspace_bytes(a)) return cudaErrorInvalidValue;
-    const Shape s = shape_of(a);
+    const Shape s = shape_of(a, grain_of(a.x, a.ld_x * (a.x_i8 ? 1 : 2), 1) >= (a.x_i8 ? 8 : 16) && grain_of(a.a, a.k * 2, 1) == 16);
     AdapterParams p;
     p.base = a.base; p.x = a.x; p.a = a.a; p.b = a.b;
     p.x_scale = a.x_scale; p.scaling = a.scaling; p.ids = a.ids; p.out = a.out;

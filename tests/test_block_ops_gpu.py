@@ -575,3 +575,32 @@ def test_adapter_infinite_activations(T, r, dtype):
     assert torch.equal(out[3], want)
     others = torch.arange(T, device=DEV) != 3
     assert torch.equal(out[others], clean[others])
+
+
+@pytest.mark.parametrize("x_i8", [False, True])
+@pytest.mark.parametrize("T,K,N,L,r", [(1, 1, 1, 1, 1), (1, 1001, 133, 1, 7), (5, 264, 200, 2, 31), (30, 77, 136, 4, 65), (9, 1500, 64, 3, 12),
+                                       (250, 17, 40, 20, 3), (16, 513, 96, 16, 127), (4, 6, 8, 1, 2), (70, 2047, 264, 9, 5)])
+def test_adapter_few_tokens_on_any_boundary(T, K, N, L, r, x_i8):
+    for dtype in (BF16, F16):
+        c = adapter_case(T, K, N, L, r, dtype, x_i8)
+        check_adapter(c, ops.adapter_add(**c))
+        # the same rows farther apart, from the second element on, with NaN around them; weights that begin at an odd place
+        wide = torch.full((T, K + 4), 99 if x_i8 else math.nan, device=DEV, dtype=c["x"].dtype)
+        wide[:, 1:K + 1] = c["x"]
+        moved = {}
+        for n in ("a", "b"):
+            store = torch.full((c[n].numel() + 2,), math.nan, device=DEV, dtype=dtype)
+            store[1:-1] = c[n].flatten()
+            moved[n] = store[1:-1].view(c[n].shape)
+        check_adapter(c, ops.adapter_add(**{**c, **moved, "x": wide[:, 1:K + 1]}))
+
+
+@pytest.mark.parametrize("T,L", [(300, 3), (1000, 60), (2100, 2)])
+@pytest.mark.parametrize("r", [1, 7, 30, 61, 67, 127])
+def test_adapter_ranks_on_any_boundary(T, L, r):
+    for dtype, N in ((BF16, 264), (F16, 1000)):
+        c = adapter_case(T, 520, N, L, r, dtype)
+        check_adapter(c, ops.adapter_add(**c))
+        store = torch.full((c["b"].numel() + 2,), math.nan, device=DEV, dtype=dtype)
+        store[1:-1] = c["b"].flatten()
+        check_adapter(c, ops.adapter_add(**{**c, "b": store[1:-1].view(c["b"].shape)}))
