@@ -299,13 +299,13 @@ __device__ __forceinline__ Tile self_plan(const AdapterParams &p, SelfPlan &s, i
     return Tile{id, min(TN, all - before)};
 }
 
-// The same from the plan in the workspace, whose tiles hold `parts` of them.
+// The same from the plan in the workspace, whose tiles hold `parts` of them: number `place`.
 template <int TN>
-__device__ __forceinline__ Tile read_plan(const AdapterParams &p, int parts, int threads, int *rows)
+__device__ __forceinline__ Tile read_plan(const AdapterParams &p, int place, int parts, int threads, int *rows)
 {
-    const int tiles = __ldcg(p.n_tiles), at = (int)blockIdx.x / parts, part = (int)blockIdx.x % parts;
+    const int tiles = __ldcg(p.n_tiles), at = place / parts, part = place % parts;
     const int2 t = __ldcg(p.tiles + at);   // with the rows, whose places do not hang on it, in one go
-    for (int i = threadIdx.x; i < TN; i += threads) rows[i] = __ldcg(p.order + (long long)blockIdx.x * TN + i);
+    for (int i = threadIdx.x; i < TN; i += threads) rows[i] = __ldcg(p.order + (long long)place * TN + i);
     __syncthreads();
     return at < tiles ? Tile{t.x, max(0, min(TN, t.y - part * TN))} : Tile{-1, 0};
 }
@@ -700,7 +700,8 @@ inline int shrink_smem(int tn, int rank_pad, bool i8)
     return 1024 + (shrink_stages(tn, rank_pad, i8) - 1) * stage + (stage > last ? stage : last);
 }
 
-// Grid: (tiles, ksplit).  CTA y takes the K blocks [y * blocks / ksplit, (y + 1) * blocks / ksplit).
+// Grid: tiles * ksplit, a tile's CTAs in a row: those of the places that no tile takes come last, so that they keep nobody waiting.  CTA s
+// of a tile takes the K blocks [s * blocks / ksplit, (s + 1) * blocks / ksplit).
 // FAST: rows of x and a start on 16-byte boundaries.  A thread then copies the same 16 bytes of every K block, whose addresses it works
 // out once; with the addresses of every copy worked out anew the kernel was bound by its instructions.
 // The products are issued by a warp of their own, which also orders them behind the copies (fence.proxy.async).  What bounds the kernel
@@ -732,9 +733,10 @@ __global__ void __launch_bounds__(kWorkers + 32) adapter_shrink_kernel(const Ada
     __syncthreads();
     pdl_release();
     tc_fence_after();
-    const Tile tile = read_plan<TN>(p, 1, kWorkers + 32, rows);
+    const int split = (int)(blockIdx.x % (unsigned)p.ksplit);
+    const Tile tile = read_plan<TN>(p, (int)(blockIdx.x / (unsigned)p.ksplit), 1, kWorkers + 32, rows);
     const int blocks = (p.k + kBlockK - 1) / kBlockK;
-    const int kb0 = (int)((long long)blockIdx.y * blocks / p.ksplit), kb1 = (int)((long long)(blockIdx.y + 1) * blocks / p.ksplit);
+    const int kb0 = (int)((long long)split * blocks / p.ksplit), kb1 = (int)((long long)(split + 1) * blocks / p.ksplit);
     const bool work = tile.count > 0 && tile.adapter >= 0;   // kb0 < kb1, since ksplit is at most blocks
     const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t stage_bytes = align_up(shrink_stage(TN, p.rank_pad, I8), 1024), a_tile = TN * kBlockK * 2;
@@ -854,7 +856,7 @@ __global__ void __launch_bounds__(kWorkers + 32) adapter_shrink_kernel(const Ada
             const int row = live ? rows[slot] : 0;
             float f = p.scaling ? __ldg(p.scaling + tile.adapter) : 1.0f;
             if (I8 && live) f = __fmul_rn(f, __ldg(p.x_scale + row));
-            float4 *v = reinterpret_cast<float4 *>(p.v + ((long long)blockIdx.y * p.rows + row) * p.rank_pad);
+            float4 *v = reinterpret_cast<float4 *>(p.v + ((long long)split * p.rows + row) * p.rank_pad);
             for (int c = warp / 4 * half; c < (warp / 4 + 1) * half; c += 8) {
                 uint32_t d[8];
                 tmem_ld8(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)c, d);
@@ -884,7 +886,7 @@ __host__ __device__ inline int rank_atoms(int rank_pad) { return rank_pad > 64 ?
 __host__ __device__ inline int expand_stage(int tn, int rank_pad) { return rank_atoms(rank_pad) * kChunkN * 128 + tn * kChunkN * 2; }
 inline int expand_smem(int tn, int rank_pad) { return 1024 + rank_atoms(rank_pad) * tn * 256 + kExpandStages * expand_stage(tn, rank_pad); }
 
-// Grid: (tiles, nsplit).  CTA y takes the channel chunks [y * chunks / nsplit, (y + 1) * chunks / nsplit).
+// Grid: tiles * nsplit, as above.  CTA s of a tile takes the channel chunks [s * chunks / nsplit, (s + 1) * chunks / nsplit).
 // GB 16: rows of b, base and out on 16-byte boundaries; addresses are worked out once, and results go back through the chunk's base rows in
 // shared memory, from which they are stored 16 bytes at a time.  2: the same with rows of b on any boundary, by way of registers (rank 61
 // beside 64, 3000 tokens: 44 us and 35; element by element, as with 0, 64).  0: any strides.
@@ -916,9 +918,10 @@ __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) ada
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const Tile tile = read_plan<TN>(p, p.parts, THREADS, rows);
+    const int split = (int)(blockIdx.x % (unsigned)p.nsplit);
+    const Tile tile = read_plan<TN>(p, (int)(blockIdx.x / (unsigned)p.nsplit), p.parts, THREADS, rows);
     const int chunks = (p.n + kChunkN - 1) / kChunkN;
-    const int c0 = (int)((long long)blockIdx.y * chunks / p.nsplit), c1 = (int)((long long)(blockIdx.y + 1) * chunks / p.nsplit);
+    const int c0 = (int)((long long)split * chunks / p.nsplit), c1 = (int)((long long)(split + 1) * chunks / p.nsplit);
     const T *base = reinterpret_cast<const T *>(p.base);
     T *out = reinterpret_cast<T *>(p.out);
     if (tile.count > 0 && tile.adapter < 0) {
@@ -1258,13 +1261,13 @@ cudaError_t launch_tiles(const AdapterParams &p, const Shape &s, cudaStream_t st
     cudaError_t e = launch_kernel(adapter_plan_kernel, dim3(1), kPlanThreads, (p.adapters + 1) * 4, stream, false, p, s.tile_tokens);
     if (e != cudaSuccess) return e;
     const auto shrink = p.grain_x == 16 && p.grain_a == 16 ? adapter_shrink_kernel<T, I8, TN, true> : adapter_shrink_kernel<T, I8, TN, false>;
-    e = launch_kernel(shrink, dim3((unsigned)s.tiles, (unsigned)s.ksplit), kWorkers + 32, shrink_smem(TN, s.rank_pad, I8), stream, true, p);
+    e = launch_kernel(shrink, dim3((unsigned)s.tiles * (unsigned)s.ksplit), kWorkers + 32, shrink_smem(TN, s.rank_pad, I8), stream, true, p);
     if (e != cudaSuccess) return e;
     const bool rows16 = p.grain_base == 16 && p.grain_out == 16 && p.n % 8 == 0;
     constexpr int EN = TN < 64 ? TN : 64;
     const auto expand = rows16 && p.grain_b == 16 ? adapter_expand_kernel<T, EN, 16>
                         : rows16 ? adapter_expand_kernel<T, EN, 2> : adapter_expand_kernel<T, EN, 0>;
-    return launch_kernel(expand, dim3((unsigned)(s.tiles * p.parts), (unsigned)s.nsplit), expand_workers(EN) + 32, expand_smem(EN, s.rank_pad), stream, true, p);
+    return launch_kernel(expand, dim3((unsigned)(s.tiles * p.parts) * (unsigned)s.nsplit), expand_workers(EN) + 32, expand_smem(EN, s.rank_pad), stream, true, p);
 }
 
 template <typename T, bool ANY>
