@@ -175,7 +175,8 @@ ACL_FUNC_VISIBILITY aclnnStatus gmmB200RouteTopK(void *workspace, uint64_t works
  *   a                 [adapters, rank, k], b [adapters, n, rank], both base's type; adapters in [1, 16384], rank in [1, 128], k and n in
  *                     [1, 65535]
  *   adapterIds        int32 [rows];   scaling  fp32 [adapters], optional (1 without it)
- * Tokens may come in any order; those of one adapter share its weights. */
+ * Tokens may come in any order; those of one adapter share its weights.  An infinity in b may give NaN where the formula gives an
+ * infinity (x a^T enters the second product in two 16-bit parts). */
 ACL_FUNC_VISIBILITY aclnnStatus gmmB200AdapterAddGetWorkspaceSize(
     const aclTensor *base, const aclTensor *x, const aclTensor *xScaleOptional, const aclTensor *a, const aclTensor *b,
     const aclTensor *adapterIds, const aclTensor *scalingOptional, aclTensor *out, uint64_t *workspaceSize, aclOpExecutor **executor);
