@@ -17,9 +17,9 @@
 // not matter: every row's arithmetic is its own.  A few tokens take two kernels on the CUDA cores instead, whose CTAs find their tiles
 // themselves.
 //
-// 4096 tokens of 8 adapters, 7168 -> 4096, rank 64, bf16: 50 us for 137 MB, which take 21 at the rate of a copy: the plan 5, the first
-// product 17 (its operands come at about 55 bytes per ns and SM, weights included, which every tile reads anew), the second 20 (4 for the
-// partial sums, then 5 TB/s).
+// 4096 tokens of 8 adapters, 7168 -> 4096, rank 64, bf16: 48 us for 137 MB, which take 21 at the rate of a copy: the plan 5, the first
+// product 17 (its operands come at about 55 bytes per ns and SM, weights included, which every tile reads anew), the second 20 (3 for the
+// partial sums, then 4 TB/s).  611 tokens of 13, 1424 -> 2976, rank 12: 16 us, the three kernels' latencies (3, 5 and 5).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -1215,7 +1215,8 @@ struct Shape {
     bool few;
 };
 
-// On the CUDA cores, in tiles of 4 tokens: up to kSelfPlan tokens while all tiles together read no more than `limit` elements of weights.
+// On the CUDA cores, in tiles of 4 tokens: up to kSelfPlan tokens while all tiles together read no more than `limit` elements of weights,
+// if rows of x and a start on packs (others, with two loads and a shift a pack: 200 tokens, 1500 -> 4096, 22 us, 16 on the tensor cores).
 // They read them anew for every tile, at about 10 us per 10 million elements beyond the first 5; the tensor cores' way reads them once,
 // but takes a third kernel and some 0.3 us per adapter.  2048 -> 2048, rank 16: 16 tokens of 4 adapters 6.5 us and 10.6, 128 of 128 8.7
 // and 21; 4096 -> 4096, rank 64: 32 of 8 12.9 and 16.3, 64 of 8 18.0 and 17.9, 128 of 8 27 and 19, 128 of 128 40 and 40.

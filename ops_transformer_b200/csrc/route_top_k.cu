@@ -15,7 +15,7 @@
 // than 32 keys reach the bound (many equal ones, or a large k).
 //
 // Bound by instructions: some 800 a row and warp for 256 experts in eight groups (16384 rows 15 us, where reading the logits takes 2.7),
-// 600 without groups and bias (11.3 us); 128 experts 9.6 us, 64 8.4.  Few rows cost a warp's chain: 2.6 us for 32 rows.
+// softmax without groups and bias 11.3 us, 128 experts 9.6 us, 64 8.4.  Few rows cost a warp's chain: 2.8 us for 16.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
