@@ -145,7 +145,14 @@ __device__ __forceinline__ bool route_about(const RouteParams &p, const float (&
             best = fmaxf(best, ob);
         }
         const float rank = TOP2 && second > minus_inf() ? __fadd_rn(best, second) : best;
-        const float margin = 3e-6f + 1e-6f * fabsf(rank);
+        // What two groups' ranks may be off by together.  The largest choices of groups that are close are of one size; the parts of a sum
+        // may be far larger than it, and another group's larger than this one's: there it goes by the largest parts of the row.
+        float size = fabsf(rank);
+        if (TOP2) {
+            const float parts = second > minus_inf() ? fabsf(best) + fabsf(second) : fabsf(best);
+            size = __uint_as_float(__reduce_max_sync(kAll, best > minus_inf() ? __float_as_uint(parts) : 0u));
+        }
+        const float margin = 3e-6f + 1e-6f * size;
         const float above = __fadd_rn(rank, margin), below = __fsub_rn(rank, margin);
         int surely = 0, maybe = -1;   // groups that are, that may be better; it is no better than itself
 #pragma unroll 8

@@ -604,3 +604,47 @@ def test_adapter_ranks_on_any_boundary(T, L, r):
         store = torch.full((c["b"].numel() + 2,), math.nan, device=DEV, dtype=dtype)
         store[1:-1] = c["b"].flatten()
         check_adapter(c, ops.adapter_add(**{**c, "b": store[1:-1].view(c["b"].shape)}))
+
+
+@pytest.mark.parametrize("size", [20.0, 50.0, 200.0, 1000.0, 3e4])
+def test_route_groups_whose_largest_choices_cancel(size):
+    """Groups are ranked by best + second, each rounded on the grid of its own size, which cancels out of the sum: two experts of a group with
+    biases of +size and -size.  Ranks then differ by a few units of that grid or are equal, and must order as the definition rounds them."""
+    T, G, E = 4096, 8, 64
+    near = randn((T, 1, 2), 1) + 2e-6 * randn((T, G, 2), 2)
+    logits = torch.full((T, G, E // G), -math.inf, device=DEV)
+    logits[:, :, 2], logits[:, :, 5] = near[..., 0], near[..., 1]
+    logits = logits.view(T, E)
+    bias = torch.zeros(G, E // G, device=DEV)
+    bias[:, 2], bias[:, 5] = size, -size
+    bias = bias.view(E)
+    choice = 1.0 / (1.0 + torch.exp(-logits)) + bias
+    choice = torch.where(logits > -math.inf, choice, -math.inf)
+    best = choice.view(T, G, -1).sort(dim=2, descending=True).values
+    rank = best[..., 0] + best[..., 1]
+    place = rank.argsort(dim=1, descending=True, stable=True).argsort(dim=1)
+    for kept in (1, 3):
+        left = torch.where((place < kept).repeat_interleave(E // G, 1), choice, -math.inf)
+        want = left.sort(dim=1, descending=True, stable=True).indices[:, :kept]
+        got = ops.route_top_k(logits, kept, scoring="sigmoid", bias=bias, n_group=G, topk_group=kept, group_score="top2")[1]
+        assert torch.equal(got.long(), want)
+
+
+def test_route_one_group_of_large_choices_among_small_ones():
+    """The error of another group's rank counts as much as a group's own: one whose two choices are large and cancel, among small ones."""
+    T, E = 4096, 32
+    near = torch.rand(T, 1, device=DEV, generator=gen(1)) - 0.5
+    logits = near + 3e-6 * randn((T, E), 2)
+    bias = torch.zeros(E, device=DEV)
+    logits[:, 8:16] = -math.inf
+    logits[:, [9, 14]] = near + 3e-6 * randn((T, 2), 3)
+    bias[9], bias[14] = 100.0, -100.0
+    choice = torch.where(logits > -math.inf, 1.0 / (1.0 + torch.exp(-logits)) + bias, -math.inf)
+    best = choice.view(T, 4, 8).sort(dim=2, descending=True).values
+    rank = best[..., 0] + best[..., 1]
+    place = rank.argsort(dim=1, descending=True, stable=True).argsort(dim=1)
+    left = torch.where((place < 2).repeat_interleave(8, 1), choice, -math.inf)
+    want = left.sort(dim=1, descending=True, stable=True).indices[:, :4]
+    got = ops.route_top_k(logits, 4, scoring="sigmoid", bias=bias, n_group=4, topk_group=2, group_score="top2")[1].long()
+    there = left.gather(1, want) > -math.inf
+    assert torch.equal(got, torch.where(there, want, -1))
