@@ -11,7 +11,6 @@ from __future__ import annotations
 import array
 import contextlib
 import ctypes as C
-import functools
 import struct
 import threading
 from typing import Optional, Sequence
@@ -430,9 +429,11 @@ def moe_init_routing_v3(x: torch.Tensor, expert_idx: torch.Tensor, *, expert_num
 # Operators around the expert FFN (include/gmm_b200.h)
 # ---------------------------------------------------------------------------------------------------------------------
 
-@functools.lru_cache(maxsize=64)
+_FLOAT, _WORD = struct.Struct("<f"), struct.Struct("<I")
+
+
 def _float_bits(v: float) -> int:
-    return struct.unpack("<I", struct.pack("<f", v))[0]
+    return _WORD.unpack(_FLOAT.pack(v))[0]
 
 
 def _block_call(op: int, name: str, workspace: Optional[torch.Tensor], stream, kinds: str, *items) -> None:

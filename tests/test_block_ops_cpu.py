@@ -145,3 +145,16 @@ def test_second_phase_takes_an_executor_once_and_of_its_own_operator():
     assert L.gmmB200AddRmsNormQuant(None, 0, ex, None) == INVALID
     assert L.gmmB200RouteTopK(None, 0, plan(), None) == INVALID
     assert L.gmmB200AdapterAdd(None, 0, None, None) == NULLPTR
+
+
+def test_numbers_are_read_anew_in_every_call():
+    """eps and scale may be anything that is a number; a tensor's value is the one that it has at the call."""
+    import struct
+    bits = lambda v: struct.unpack("<I", struct.pack("<f", v))[0]  # noqa: E731
+    t = torch.tensor(2.5)
+    assert acl._float_bits(t) == bits(2.5)
+    t.fill_(1.0)
+    assert acl._float_bits(t) == bits(1.0)
+    assert [acl._float_bits(v) for v in (0.0, -0.0, 0.0, 1, True, 1.0)] == [0, 1 << 31, 0] + [bits(1.0)] * 3
+    with pytest.raises(struct.error):
+        acl._float_bits("1")
