@@ -169,14 +169,15 @@ ACL_FUNC_VISIBILITY aclnnStatus gmmB200RouteTopK(void *workspace, uint64_t works
 
 /* Low-rank adapters of many requests on top of a projection that they share:
  *   out[t] = base[t] + scaling[i] * (x[t] a[i]^T) b[i]^T with i = adapterIds[t]; out[t] = base[t] where i names no adapter
- *   (negative, or at least `adapters`).  Sums are fp32, the result is rounded once.
+ *   (negative, or at least `adapters`).  Both sums are fp32, and so is x a^T between them (with fp16,
+ *   down to 2^-39 of the row's largest component); the result is rounded once.
  *   base, out         [rows, n] fp16 / bf16; out may be base itself;   rows may be 0
  *   x                 [rows, k] base's type, or int8 with xScale (fp32 [rows]): the rows of the W8A8 operators
  *   a                 [adapters, rank, k], b [adapters, n, rank], both base's type; adapters in [1, 16384], rank in [1, 128], k and n in
  *                     [1, 65535]
  *   adapterIds        int32 [rows];   scaling  fp32 [adapters], optional (1 without it)
  * Tokens may come in any order; those of one adapter share its weights.  An infinity in b may give NaN where the formula gives an
- * infinity (x a^T enters the second product in two 16-bit parts). */
+ * infinity (x a^T enters the second product in three 16-bit parts, some of them zero). */
 ACL_FUNC_VISIBILITY aclnnStatus gmmB200AdapterAddGetWorkspaceSize(
     const aclTensor *base, const aclTensor *x, const aclTensor *xScaleOptional, const aclTensor *a, const aclTensor *b,
     const aclTensor *adapterIds, const aclTensor *scalingOptional, aclTensor *out, uint64_t *workspaceSize, aclOpExecutor **executor);

@@ -8,8 +8,9 @@
 // Both products run on the tensor cores (tcgen05, fp32 accumulators in tensor memory) although few operations come with every byte:
 // they then cost no issue slots beside the loads.  The tokens are rows of the first product and columns of the second, so that tiles of
 // 16 tokens (few tokens) and of 64 share the code and the channels of a result row lie in neighbouring lanes.
-// v enters the second product as two 16-bit parts, v = hi + lo: one alone would add an error of 2^-8 (bf16) of v, as large as the
-// rounding of the result.  fp16 has no range to spare, so there every token's v is scaled by a power of two to below 2.
+// v enters the second product as three 16-bit parts, each the rounded rest of v less the ones before: all 24 bits of it, so the sums are
+// those of fp32 throughout.  fp16 has no range to spare, so there every token's v is scaled by a power of two to just below 2^15: parts
+// end at 2^-24, which is 2^-39 of the token's largest component.
 // The operands are fetched with 16-byte asynchronous copies (8, 4 or 2 bytes where rows start on no such boundary), straight into the
 // 128-byte-swizzled layout that the tensor cores read; a row's tail is zero filled.
 //
@@ -882,9 +883,10 @@ __global__ void __launch_bounds__(kWorkers + 32) adapter_shrink_kernel(const Ada
 // out = base + v b^T
 // ---------------------------------------------------------------------------------------------------------
 
+constexpr int kParts = 3;   // 16-bit parts of a component of v
 __host__ __device__ inline int rank_atoms(int rank_pad) { return rank_pad > 64 ? 2 : 1; }
 __host__ __device__ inline int expand_stage(int tn, int rank_pad) { return rank_atoms(rank_pad) * kChunkN * 128 + tn * kChunkN * 2; }
-inline int expand_smem(int tn, int rank_pad) { return 1024 + rank_atoms(rank_pad) * tn * 256 + kExpandStages * expand_stage(tn, rank_pad); }
+inline int expand_smem(int tn, int rank_pad) { return 1024 + kParts * rank_atoms(rank_pad) * tn * 128 + kExpandStages * expand_stage(tn, rank_pad); }
 
 // Grid: tiles * nsplit, as above.  CTA s of a tile takes the channel chunks [s * chunks / nsplit, (s + 1) * chunks / nsplit).
 // GB 16: rows of b, base and out on 16-byte boundaries; addresses are worked out once, and results go back through the chunk's base rows in
@@ -932,7 +934,7 @@ __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) ada
     } else if (tile.count > 0 && c0 < c1) {
         const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
         const int atoms = rank_atoms(p.rank_pad);
-        const uint32_t v_hi = smem0, v_lo = v_hi + (uint32_t)(atoms * TN * 128), stage0 = v_lo + (uint32_t)(atoms * TN * 128);
+        const uint32_t v_part = (uint32_t)(atoms * TN * 128), stage0 = smem0 + kParts * v_part;   // the parts of v, one behind the other
         const uint32_t stage_bytes = expand_stage(TN, p.rank_pad), base_at = (uint32_t)(atoms * kChunkN * 128);
         const char *b = reinterpret_cast<const char *>(p.b) + (long long)tile.adapter * p.n * p.rank * 2;
         // b: the copies of a chunk, offset in its rows << 8 | bytes, and place in the tile
@@ -1005,9 +1007,11 @@ __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) ada
                     uint32_t more = 0;
                     for (int j = 0; j < p.rank_pad / 16; ++j) {
                         const uint64_t bd = operand_desc(s + (uint32_t)(j / 4) * kChunkN * 128) + (j % 4) * 2;
-                        umma_f16(d, bd, operand_desc(v_hi + (uint32_t)(j / 4) * TN * 128) + (j % 4) * 2, idesc, more);
-                        more = 1;
-                        umma_f16(d, bd, operand_desc(v_lo + (uint32_t)(j / 4) * TN * 128) + (j % 4) * 2, idesc, more);
+#pragma unroll
+                        for (int part = 0; part < kParts; ++part) {
+                            umma_f16(d, bd, operand_desc(smem0 + part * v_part + (uint32_t)(j / 4) * TN * 128) + (j % 4) * 2, idesc, more);
+                            more = 1;
+                        }
                     }
                     umma_commit(smem_u32(&acc_full[buf]));
                 }
@@ -1076,35 +1080,39 @@ __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) ada
 #pragma unroll
                     for (int h = 0; h < CH; ++h)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(f[h][e]) & 0x7fffffffu);
+                        for (int e = 0; e < 8; ++e) {
+                            const uint32_t mag = __float_as_uint(f[h][e]) & 0x7fffffffu;
+                            m = max(m, mag < 0x7f800000u ? mag : 0u);   // infinities and NaN stay what they are
+                        }
 #pragma unroll
                     for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-                    // 2^-e for a largest value in [2^e, 2^(e+1)); none for zero, for what no power of two can help, and at the ends of fp32
+                    // 2^(14 - e) for a largest value in [2^e, 2^(e+1)); none where all are so small that no result sees them
                     const int e = (int)(m >> 23) - 127;
-                    const bool shift = m != 0 && e > -120 && e < 120;
-                    down = shift ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.0f;
-                    if (part == 0) unscale[slot] = shift ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.0f;
+                    const bool shift = e > -112;
+                    down = shift ? __uint_as_float((uint32_t)(127 + 14 - e) << 23) : 1.0f;
+                    if (part == 0) unscale[slot] = shift ? __uint_as_float((uint32_t)(127 - 14 + e) << 23) : 1.0f;
                 }
 #pragma unroll
                 for (int h = 0; h < CH; ++h) {
                     const int j = (part + h * LANES) * 8;
                     if (j >= p.rank_pad) break;
-                    float g[8];
-                    uint32_t hi[4], lo[4];
+                    if (F16) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        f[h][e] = __fmul_rn(f[h][e], down);
-                        const float first = to_float(from_float<T>(f[h][e]));
-                        g[e] = isinf(first) ? 0.0f : __fsub_rn(f[h][e], first);   // an infinity less itself is none
+                        for (int e = 0; e < 8; ++e) f[h][e] = __fmul_rn(f[h][e], down);
                     }
+                    uint32_t at = smem0 + (uint32_t)(j / 64 * TN * 128) + swizzled(slot, (j % 64) * 2);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        hi[e] = pack2<T>(f[h][2 * e], f[h][2 * e + 1]);
-                        lo[e] = pack2<T>(g[2 * e], g[2 * e + 1]);
+                    for (int q = 0; q < kParts; ++q, at += v_part) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = pack2<T>(f[h][2 * e], f[h][2 * e + 1]);
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {   // the rest, which is exact; an infinity less itself is none
+                            const float taken = to_float(from_float<T>(f[h][e]));
+                            f[h][e] = isinf(taken) ? 0.0f : __fsub_rn(f[h][e], taken);
+                        }
                     }
-                    const uint32_t at = (uint32_t)(j / 64 * TN * 128) + swizzled(slot, (j % 64) * 2);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(v_hi + at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(v_lo + at), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&v_full));

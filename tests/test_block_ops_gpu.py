@@ -648,3 +648,47 @@ def test_route_one_group_of_large_choices_among_small_ones():
     got = ops.route_top_k(logits, 4, scoring="sigmoid", bias=bias, n_group=4, topk_group=2, group_score="top2")[1].long()
     there = left.gather(1, want) > -math.inf
     assert torch.equal(got, torch.where(there, want, -1))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("r", [16, 61, 128])
+@pytest.mark.parametrize("T,K,L", [(300, 136, 3), (300, 137, 80), (2100, 64, 4)])
+def test_adapter_small_components_beside_large_ones(T, K, L, r, dtype):
+    """x a^T is held in fp32 on its way into the second product: an output whose b has weight only on components that are 2^-20 of the row's
+    largest is as exact as any other (fp16), and one in which large components nearly cancel too (bf16)."""
+    N = 264
+    ids = (torch.arange(T, device=DEV) % L).to(torch.int32)
+    c = adapter_case(T, K, N, L, r, dtype, ids=ids)
+    c["base"].zero_()
+    if dtype == F16:
+        c["a"].normal_(generator=gen(3))
+        c["a"][:, 0] *= 2.0 ** 7
+        c["a"][:, 1:] *= 2.0 ** -13
+        c["b"].normal_(generator=gen(4)).mul_(16)
+        c["b"][:, ::2, 0] = 0                       # every other channel hangs on the small components alone
+    else:
+        c["a"][:, 1:2] = c["a"][:, :1]
+        c["a"][:, 1, 3::7] *= 1 + 2.0 ** -7         # the two components differ by about 2^-9
+        c["b"][:, :, 1] = -c["b"][:, :, 0]
+        c["b"][:, :, 2:] *= 2.0 ** -9
+    check_adapter_fp32(c, ops.adapter_add(**c))
+
+
+def check_adapter_fp32(c, out):
+    """As check_adapter, without an allowance for fewer bits than fp32 has between the products: v of a row is off by its own sum's rounding, a
+    result by that times |b|, by the second sum's and by its own rounding."""
+    K, r, L = c["x"].shape[1], c["a"].shape[1], c["a"].shape[0]
+    want, tol = c["base"].double(), torch.zeros_like(c["base"], dtype=torch.float64)
+    for i in range(L):
+        at = (c["adapter_ids"] == i).nonzero()[:, 0]
+        x, a, b, s = c["x"][at].double(), c["a"][i].double(), c["b"][i].double(), c["scaling"][i].double()
+        v, mag = s * (x @ a.t()), s * (x.abs() @ a.abs().t())
+        want[at] += v @ b.t()
+        # K / 16 + 8 steps of the first sum (one unit of the partial sum each), rank / 16 + 8 of the second, which the largest product bounds
+        tol[at] = (mag @ b.abs().t()) * (K / 16 + 8) * 2 * U32 + (v.abs() @ b.abs().t()) * (r / 16 + 8) * 2 * U32
+    tol += want.abs() * HALF_ULP[out.dtype] * 1.001 + TINY[out.dtype]
+    # what passes the largest number of the type by more than its own error is an infinity
+    most = torch.finfo(out.dtype).max
+    over, fits = want.abs() - tol > most, want.abs() + tol < most
+    assert torch.equal(out[over].double(), want[over].sign() * math.inf) and out[fits].isfinite().all()
+    assert ((out.double() - want).abs() <= tol)[fits].all()
