@@ -41,7 +41,9 @@ ACL_FUNC_VISIBILITY aclnnStatus gmmB200CheckStatus(const void *workspace, uint64
  *                    limit: the warp that they wait for has two waits of its own per tile).
  *   testSkipKBlocks  test only: the copy-issuing warp leaves this many K blocks out of its last tile, so that the bounded wait
  *                    of the warp that consumes them runs out and the abort path (status record, clean exit) can be exercised
- *                    without touching memory the call does not own.  Results are then undefined.  0 = off. */
+ *                    without touching memory the call does not own.  Results are then undefined.  0 = off.
+ * gmmB200AdapterAdd takes waitLimitCycles and testSkipKBlocks (of its first product; its kernels for a few tokens have no waits); the
+ * operators without waits on the device take none. */
 typedef struct gmmB200LaunchOptions {
     uint32_t structSize;
     int32_t maxCtas;

@@ -39,7 +39,7 @@ constexpr int kPlanThreads = 1024;
 constexpr int kWorkers = 256;        // threads of the first kernel that copy; one warp more issues the products
 __host__ __device__ constexpr int expand_workers(int tn) { return tn == 64 ? 512 : 256; }
 constexpr int kMaxStages = 6, kShrinkAhead = 2, kExpandStages = 2;
-constexpr long long kWaitLimitCycles = 1ll << 31;   // about a second
+constexpr long long kWaitLimitCycles = 1ll << 31;   // of a call that names no other: about a second
 
 struct AdapterParams {
     const void *base, *x, *a, *b;
@@ -52,6 +52,8 @@ struct AdapterParams {
     int grain_x, grain_a, grain_b, grain_base, grain_out;   // bytes of a copy
     int ksplit, nsplit, stages;
     int parts;                      // tiles of the second kernel in one of the first
+    int skip_blocks;                // test only: K blocks of every tile whose arrival the first kernel leaves out
+    long long wait_limit;           // cycles
     int *status;                    // [4]
     int *n_tiles;
     int2 *tiles;                    // adapter (-1: none), tokens
@@ -87,13 +89,15 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarri
 __device__ __forceinline__ void mbar_arrive_copies(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
 template <int THREADS>
 __device__ __forceinline__ void worker_sync() { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); }
-// Bounded wait for the tensor cores, or for the copies that they wait for.  When it runs out the status says so and later waits of the CTA return at once.
-__device__ __noinline__ void mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int *gave_up, int *status, int role)
+// Bounded wait for the tensor cores, or for the copies that they wait for.  When it runs out the status says so and later waits of the CTA
+// return at once, except those that LAST stands for: behind one, nothing that the CTA has under way may be left.
+template <bool LAST>
+__device__ __noinline__ void mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int *gave_up, int *status, long long limit, int role)
 {
     const long long t0 = clock64();
     while (!mbar_try(bar, parity)) {
-        if (*gave_up) return;
-        if (clock64() - t0 > kWaitLimitCycles) {
+        if (!LAST && *gave_up) return;
+        if (clock64() - t0 > limit) {
             *gave_up = 1;
             if (atomicCAS(status, kStatusOk, kStatusWaitTimeout) == kStatusOk) {
                 status[1] = (int)(blockIdx.y * gridDim.x + blockIdx.x);
@@ -104,9 +108,10 @@ __device__ __noinline__ void mbar_wait_slow(uint32_t bar, uint32_t parity, volat
         }
     }
 }
-__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatile int *gave_up, int *status, int role)
+template <bool LAST = false>
+__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatile int *gave_up, const AdapterParams &p, int role)
 {
-    if (!mbar_try(bar, parity)) mbar_wait_slow(bar, parity, gave_up, status, role);
+    if (!mbar_try(bar, parity)) mbar_wait_slow<LAST>(bar, parity, gave_up, p.status, p.wait_limit, role);
 }
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -747,7 +752,7 @@ __global__ void __launch_bounds__(kWorkers + 32) adapter_shrink_kernel(const Ada
         uint32_t phase = 0;
         for (int kb = kb0; kb < kb1; ++kb) {
             const uint32_t s = smem0 + (uint32_t)stage * stage_bytes;
-            mbar_wait(smem_u32(&full[stage]), phase, &gave_up, p.status, 900);
+            mbar_wait(smem_u32(&full[stage]), phase, &gave_up, p, 900);
             fence_async_proxy();
             tc_fence_after();
             if (lane == 0) {
@@ -824,32 +829,32 @@ __global__ void __launch_bounds__(kWorkers + 32) adapter_shrink_kernel(const Ada
         };
         // A warp's copies of block i have landed when those of the kShrinkAhead blocks behind it are all that its threads have under way;
         // one lane says so.
-        const auto landed = [&](int stage) {
+        const auto landed = [&](int stage, bool say) {
             const uint32_t s = smem0 + (uint32_t)stage * stage_bytes;
             if (I8 && FAST) widen_rows_grain<T, 16, kWorkers>(s + raw_tile, s, TN * 128, tile.count);
             else if (I8) widen_rows<T, kWorkers>(p.grain_x, s + raw_tile, s, TN * 128, tile.count);
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&full[stage]));
+            if (lane == 0 && say) mbar_arrive(smem_u32(&full[stage]));
         };
         const int n = kb1 - kb0;
         int stage = 0, behind = 0;
         uint32_t phase = 1;   // a stage is free at first
         for (int i = 0; i < n + kShrinkAhead; ++i) {
             if (i < n) {
-                mbar_wait(smem_u32(&empty[stage]), phase, &gave_up, p.status, 901);
+                mbar_wait(smem_u32(&empty[stage]), phase, &gave_up, p, 901);
                 load(kb0 + i, stage);
                 if (++stage == p.stages) { stage = 0; phase ^= 1; }
             }
             cp_commit();
             if (i >= kShrinkAhead) {
                 cp_wait<kShrinkAhead>();
-                landed(behind);
+                landed(behind, i - kShrinkAhead < n - p.skip_blocks);
                 if (++behind == p.stages) behind = 0;
             }
         }
     }
     if (work) {
-        mbar_wait(smem_u32(&done), 0, &gave_up, p.status, 902);
+        mbar_wait<true>(smem_u32(&done), 0, &gave_up, p, 902);
         tc_fence_after();
         const int quarter = warp % 4, half = p.rank_pad / 2, slot = quarter * 32 + lane;
         if (!issuer && quarter * 32 < TN) {   // warp w: 32 tokens (w % 4) and half of the columns (w / 4)
@@ -995,12 +1000,12 @@ __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) ada
         if (issuer) {
             pdl_wait();
             const uint32_t idesc = instr_desc<T>(TN);
-            mbar_wait(smem_u32(&v_full), 0, &gave_up, p.status, 910);
+            mbar_wait(smem_u32(&v_full), 0, &gave_up, p, 910);
             for (int c = c0; c < c1; ++c) {
                 const int i = c - c0, buf = i & 1;
                 const uint32_t s = stage0 + (uint32_t)(i % kExpandStages) * stage_bytes, d = tmem_base + (uint32_t)(buf * TN);
-                mbar_wait(smem_u32(&full[i % kExpandStages]), (i / kExpandStages) & 1, &gave_up, p.status, 911);
-                if (i >= 2) mbar_wait(smem_u32(&acc_empty[buf]), (i / 2 - 1) & 1, &gave_up, p.status, 912);
+                mbar_wait(smem_u32(&full[i % kExpandStages]), (i / kExpandStages) & 1, &gave_up, p, 911);
+                if (i >= 2) mbar_wait(smem_u32(&acc_empty[buf]), (i / 2 - 1) & 1, &gave_up, p, 912);
                 fence_async_proxy();
                 tc_fence_after();
                 if (lane == 0) {
@@ -1017,6 +1022,8 @@ __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) ada
                 }
                 __syncwarp();
             }
+            // all products are done, also where the others have given up
+            mbar_wait<true>(smem_u32(&acc_full[(c1 - 1 - c0) & 1]), ((c1 - 1 - c0) / 2) & 1, &gave_up, p, 915);
         } else {
             // Copies through shared memory by whole 16 bytes announce themselves; others are waited for, a chunk ahead.
             const auto announce = [&](int c) {
@@ -1131,8 +1138,8 @@ __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) ada
                 const int i = c - c0, buf = i & 1, n = c * kChunkN + ch;
                 const uint32_t s = stage0 + (uint32_t)(i % kExpandStages) * stage_bytes;
                 if (c + 1 < c1) landed(c + 1);
-                mbar_wait(smem_u32(&full[i % kExpandStages]), (i / kExpandStages) & 1, &gave_up, p.status, 913);   // base, copied by others
-                mbar_wait(smem_u32(&acc_full[buf]), (i / 2) & 1, &gave_up, p.status, 914);
+                mbar_wait(smem_u32(&full[i % kExpandStages]), (i / kExpandStages) & 1, &gave_up, p, 913);   // base, copied by others
+                mbar_wait(smem_u32(&acc_full[buf]), (i / 2) & 1, &gave_up, p, 914);
                 tc_fence_after();
                 uint32_t d[SHARE];
                 if (first < tile.count) {
@@ -1178,6 +1185,7 @@ __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) ada
                     cp_commit();
                 }
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");   // none is left unless a wait ran out
         }
     }
     // This grid must not end before the kernels in front of it: the stream goes on behind it alone.  The CTAs without a tile leave their
@@ -1331,6 +1339,8 @@ cudaError_t adapter_launch(const AdapterProblem &a, void *workspace, size_t work
     p.grain_b = grain_of(a.b, a.rank * 2, 2);
     p.grain_base = grain_of(a.base, a.ld_base * 2, 2);
     p.grain_out = grain_of(a.out, a.ld_out * 2, 2);
+    p.wait_limit = a.opt.wait_limit_cycles > 0 ? a.opt.wait_limit_cycles : kWaitLimitCycles;
+    p.skip_blocks = a.opt.test_skip_k_blocks;
     p.ksplit = s.ksplit; p.nsplit = s.nsplit; p.parts = s.tile_tokens > 64 ? s.tile_tokens / 64 : 1;
     char *ws = static_cast<char *>(workspace);
     p.status = reinterpret_cast<int *>(ws);

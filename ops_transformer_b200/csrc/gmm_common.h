@@ -159,6 +159,7 @@ struct AdapterProblem {
     int64_t ld_base = 0, ld_x = 0, ld_out = 0;
     int dtype = kBF16;
     bool x_i8 = false;
+    LaunchOptions opt;                  // wait limit and test_skip_k_blocks
 };
 size_t adapter_workspace_bytes(const AdapterProblem &p);
 cudaError_t adapter_launch(const AdapterProblem &p, void *workspace, size_t workspace_bytes, cudaStream_t stream);

@@ -105,7 +105,7 @@ aclnnStatus run_executor(const char *op_name, void *workspace, uint64_t workspac
                 case aclOpExecutor::kInitRouting: ce = init_routing_launch(executor->routing, workspace, executor->plan.ws_bytes, cs); break;
                 case aclOpExecutor::kNormQuant: ce = norm_quant_launch(executor->norm, cs); break;
                 case aclOpExecutor::kRouteTopK: ce = route_top_k_launch(executor->route, cs); break;
-                case aclOpExecutor::kAdapterAdd: ce = adapter_launch(executor->adapter, workspace, executor->plan.ws_bytes, cs); break;
+                case aclOpExecutor::kAdapterAdd: executor->adapter.opt = executor->problem.opt; ce = adapter_launch(executor->adapter, workspace, executor->plan.ws_bytes, cs); break;
                 default: ce = launch(executor->problem, executor->plan, workspace, executor->plan.ws_bytes, cs);
             }
             for (StagedView &v : executor->staged)

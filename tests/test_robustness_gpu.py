@@ -319,3 +319,40 @@ def test_overlapping_group_ranges_stay_within_the_counters(oracle, monkeypatch, 
     ops.grouped_matmul_swiglu_quant(x, w, ws, xs, rising, output=q, output_scale=qs, workspace=wsb)
     ops.check_status(wsb)
     _check_swiglu_bits(oracle, [t.cpu().numpy() for t in (x, w, ws, xs)], rising.cpu().numpy(), q, qs)
+
+
+def _adapter_call(args, out, wsb, opts):
+    """adapter_add through gmmB200Call, with options."""
+    words = _lib.describe_call("tttttttt", *args, out)
+    res = _lib.CallResult()
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    rc = _lib.lib().gmmB200Call(_lib.OP_ADAPTER_ADD, words, len(words) // 8, wsb.data_ptr(), wsb.numel(), C.byref(opts) if opts else None, stream, C.byref(res))
+    assert rc == 0 and res.stage == _lib.STAGE_RUN, _lib.last_error()
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("tokens,adapters,k", [(300, 1, 512), (300, 60, 2048), (300, 2, 4100), (2100, 2, 512)])
+def test_adapter_wait_runs_out_and_the_workspace_stays_usable(tokens, adapters, k, int8):
+    import ops_transformer_b200 as ops
+    dev = _dev()
+    g = torch.Generator(dev).manual_seed(5)
+    normal = lambda *s: (torch.randn(s, device=dev, generator=g) / s[-1] ** 0.5).to(torch.bfloat16)  # noqa: E731
+    base, a, b = normal(tokens, 520), normal(adapters, 16, k), normal(adapters, 520, 16)
+    x = torch.randint(-127, 128, (tokens, k), device=dev, generator=g).to(torch.int8) if int8 else normal(tokens, k)
+    xs = torch.rand(tokens, device=dev, generator=g) if int8 else None
+    ids = (torch.arange(tokens, device=dev) % adapters).to(torch.int32)
+    args = base, x, xs, a, b, ids, None
+    want = ops.adapter_add(base, x, a, b, ids, x_scale=xs)
+    wsb = torch.zeros(8 << 20, dtype=torch.uint8, device=dev)
+    out = torch.zeros_like(base)
+    # ~1 ms wait bound; every tile's last K block is never announced
+    _adapter_call(args, out, wsb, ops.LaunchOptions(wait_limit_cycles=2_000_000, test_skip_k_blocks=1))
+    with pytest.raises(ops.AclnnError) as ei:
+        ops.check_status(wsb)
+    assert ei.value.status == _lib.ACLNN_ERR_RUNTIME_ERROR
+    code, _, role, _ = ei.value.record
+    assert code == 1 and 900 <= role < 920, ei.value.record
+    # the context is intact and the same workspace serves the next, ordinary call
+    _adapter_call(args, out, wsb, None)
+    ops.check_status(wsb)
+    assert torch.equal(out, want)
