@@ -436,11 +436,14 @@ def _float_bits(v: float) -> int:
     return _WORD.unpack(_FLOAT.pack(v))[0]
 
 
-def _block_call(op: int, name: str, workspace: Optional[torch.Tensor], stream, kinds: str, *items) -> None:
+def _block_call(op: int, name: str, workspace: Optional[torch.Tensor], stream, options: Optional[LaunchOptions], kinds: str,
+                *items) -> Optional[torch.Tensor]:
     """The call of an operator around the expert FFN, natively.  Its tensors all have to be on one GPU; elsewhere the arguments are
-    checked and the call is refused.  A call that needs no workspace (all but ``adapter_add`` and strided views) takes none."""
+    checked and the call is refused.  A call that needs no workspace (all but ``adapter_add`` and strided views) takes none.  Returns the
+    workspace that the call uses (None if none)."""
     module, call = _lib.native()
-    x = items[0]
+    x, buf = items[0], workspace
+    how = 0 if options is None else C.addressof(options)
     pooled = workspace is None and op == _lib.OP_ADAPTER_ADD
     if not x.is_cuda:
         done = False
@@ -449,11 +452,12 @@ def _block_call(op: int, name: str, workspace: Optional[torch.Tensor], stream, k
         if pooled:
             slot = _WS.slot(x.device, handle)
             with slot.lock:   # the clear and the kernels of two calls must not interleave on the stream
-                done = module.launch(call, op | _lib.OP_POOLED, handle, slot.buf, kinds, *items)
+                buf = slot.buf
+                done = module.launch(call, op | _lib.OP_POOLED, handle, buf, how, kinds, *items)
         else:
-            done = module.launch(call, op, handle, workspace, kinds, *items)
+            done = module.launch(call, op, handle, workspace, how, kinds, *items)
     if done is None:
-        return
+        return buf
     if done is False:
         words = _lib.describe_call(kinds, *items)
         res = _lib.CallResult()
@@ -464,7 +468,8 @@ def _block_call(op: int, name: str, workspace: Optional[torch.Tensor], stream, k
         raise ValueError(f"{name}: all tensors must be on one CUDA device")
     rc, stage, need, executor = done
     if rc != ACLNN_SUCCESS:
-        raise AclnnError(rc, name + ("GetWorkspaceSize" if stage == _lib.STAGE_PLAN else ""))
+        raise AclnnError(rc, name + ("GetWorkspaceSize" if stage == _lib.STAGE_PLAN else
+                                     ": gmmB200SetExecutorOptions" if stage == _lib.STAGE_OPTIONS else ""))
     # planned only: the pool's buffer is too small or not for this call, or strided views need one
     if workspace is not None:
         _lib.lib().aclDestroyAclOpExecutor(C.c_void_p(executor))
@@ -479,6 +484,7 @@ def _block_call(op: int, name: str, workspace: Optional[torch.Tensor], stream, k
         rc = getattr(_lib.lib(), name)(workspace.data_ptr(), need, C.c_void_p(executor), handle)
     if rc != ACLNN_SUCCESS:
         raise AclnnError(rc, name)
+    return workspace
 
 
 def add_rms_norm_quant(x: torch.Tensor, gamma: torch.Tensor, *, residual: Optional[torch.Tensor] = None,
@@ -499,7 +505,7 @@ def add_rms_norm_quant(x: torch.Tensor, gamma: torch.Tensor, *, residual: Option
         residual_out = empty(x, "=")
     if normed_out is None and normed:
         normed_out = empty(x, "=")
-    _block_call(_lib.OP_ADD_RMS_NORM_QUANT, "gmmB200AddRmsNormQuant", workspace, stream, "tttttttti", x, residual, gamma, smooth, q, scale,
+    _block_call(_lib.OP_ADD_RMS_NORM_QUANT, "gmmB200AddRmsNormQuant", workspace, stream, None, "tttttttti", x, residual, gamma, smooth, q, scale,
                 residual_out, normed_out, _float_bits(eps))
     return q, scale, residual_out, normed_out
 
@@ -529,19 +535,22 @@ def route_top_k(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", b
         ids = empty(logits, letter, *shape) if letter else logits.new_empty(shape, dtype=ids_dtype)   # refused by the operator
     if token_mask is not None and token_mask.dtype == torch.bool:
         token_mask = token_mask.view(torch.int8)
-    _block_call(_lib.OP_ROUTE_TOP_K, "gmmB200RouteTopK", workspace, stream, "tttttiiiiii", logits, bias, token_mask, weights, ids,
+    _block_call(_lib.OP_ROUTE_TOP_K, "gmmB200RouteTopK", workspace, stream, None, "tttttiiiiii", logits, bias, token_mask, weights, ids,
                 _SCORING[scoring], n_group, topk_group, _GROUP_SCORE[group_score], 1 if renormalize else 0, _float_bits(scale))
     return weights, ids
 
 
 def adapter_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter_ids: torch.Tensor, *,
                 x_scale: Optional[torch.Tensor] = None, scaling: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
-                stream=None, workspace: Optional[torch.Tensor] = None):
+                stream=None, workspace: Optional[torch.Tensor] = None, return_workspace: bool = False,
+                options: Optional[LaunchOptions] = None):
     """out [rows, n] = base + scaling[i] * (x a[i]^T) b[i]^T with the adapter i = adapter_ids[row] of every row (int32, negative: none):
     low-rank adapters of many requests beside one shared projection, whose result is ``base``.  ``x`` has base's type or is int8 with
-    ``x_scale`` (fp32 [rows]); a [adapters, rank, k], b [adapters, n, rank].  ``out`` may be ``base``.  gmmB200AdapterAdd
+    ``x_scale`` (fp32 [rows]); a [adapters, rank, k], b [adapters, n, rank].  ``out`` may be ``base``.  With
+    ``return_workspace`` (out, workspace), for ``check_status`` (no rows: None); ``options``: per-call ``LaunchOptions`` (wait bound).  gmmB200AdapterAdd
     (include/gmm_b200.h)."""
     if out is None:
         out = _lib.native()[0].empty(base, "=")
-    _block_call(_lib.OP_ADAPTER_ADD, "gmmB200AdapterAdd", workspace, stream, "tttttttt", base, x, x_scale, a, b, adapter_ids, scaling, out)
-    return out
+    workspace = _block_call(_lib.OP_ADAPTER_ADD, "gmmB200AdapterAdd", workspace, stream, options, "tttttttt", base, x, x_scale, a, b, adapter_ids,
+                            scaling, out)
+    return (out, workspace if base.shape[0] else None) if return_workspace else out

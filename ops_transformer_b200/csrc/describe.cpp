@@ -181,23 +181,25 @@ struct CallResult {
 typedef int32_t (*CallFn)(int32_t, const int64_t *, uint64_t, void *, uint64_t, const void *, void *, CallResult *);
 constexpr int32_t kStageRun = 3;
 
-// launch(gmmB200Call, operator, stream, workspace or None, kinds, item, ...): the call itself.  None when it is enqueued; False, with
-// nothing done, when the tensors are not all on one CUDA device; else (status, stage, workspace size, executor).
+// launch(gmmB200Call, operator, stream, workspace or None, address of the launch options or 0, kinds, item, ...): the call itself.  None
+// when it is enqueued; False, with nothing done, when the tensors are not all on one CUDA device; else (status, stage, workspace size,
+// executor).
 PyObject *launch(PyObject *, PyObject *const *args, Py_ssize_t nargs)
 {
     Py_ssize_t n = 0;
-    const char *kinds = nargs > 4 ? PyUnicode_AsUTF8AndSize(args[4], &n) : "";
+    const char *kinds = nargs > 5 ? PyUnicode_AsUTF8AndSize(args[5], &n) : "";
     if (!kinds) return nullptr;
-    if (nargs < 6 || n != nargs - 5) {
-        PyErr_SetString(PyExc_TypeError, "a function, an operator, a stream, a workspace, the kinds of the arguments and as many arguments are wanted");
+    if (nargs < 7 || n != nargs - 6) {
+        PyErr_SetString(PyExc_TypeError, "a function, an operator, a stream, a workspace, options, the kinds of the arguments and as many arguments are wanted");
         return nullptr;
     }
     const CallFn fn = reinterpret_cast<CallFn>(PyLong_AsVoidPtr(args[0]));
     const long op = PyLong_AsLong(args[1]);
     void *stream = PyLong_AsVoidPtr(args[2]);
+    const void *options = PyLong_AsVoidPtr(args[4]);
     if (PyErr_Occurred()) return nullptr;
     try {
-        PyObject *const *items = args + 5;
+        PyObject *const *items = args + 6;
         void *workspace = nullptr;
         uint64_t bytes = 0;
         int device = -1;
@@ -223,7 +225,7 @@ PyObject *launch(PyObject *, PyObject *const *args, Py_ssize_t nargs)
         CallResult res = {};
         int32_t rc;
         Py_BEGIN_ALLOW_THREADS
-        rc = fn((int32_t)op, w.data(), w.size(), workspace, bytes, nullptr, stream, &res);
+        rc = fn((int32_t)op, w.data(), w.size(), workspace, bytes, options, stream, &res);
         Py_END_ALLOW_THREADS
         if (rc == 0 && res.stage == kStageRun) Py_RETURN_NONE;
         return Py_BuildValue("(iiKN)", (int)rc, (int)res.stage, (unsigned long long)res.workspace, PyLong_FromVoidPtr(res.executor));

@@ -356,3 +356,29 @@ def test_adapter_wait_runs_out_and_the_workspace_stays_usable(tokens, adapters, 
     _adapter_call(args, out, wsb, None)
     ops.check_status(wsb)
     assert torch.equal(out, want)
+
+
+def test_adapter_wait_that_ran_out_is_seen_from_python():
+    import ops_transformer_b200 as ops
+    dev = _dev()
+    g = torch.Generator(dev).manual_seed(6)
+    normal = lambda *s: (torch.randn(s, device=dev, generator=g) / s[-1] ** 0.5).to(torch.bfloat16)  # noqa: E731
+    args = normal(400, 256), normal(400, 1024), normal(2, 16, 1024), normal(2, 256, 16), (torch.arange(400, device=dev) % 2).to(torch.int32)
+    want, wsb = ops.adapter_add(*args, return_workspace=True)
+    ops.check_status(wsb)
+    for own in (None, torch.zeros_like(wsb)):   # a pooled workspace and one of the caller's
+        short = ops.LaunchOptions(wait_limit_cycles=2_000_000, test_skip_k_blocks=1)
+        _, wsb = ops.adapter_add(*args, return_workspace=True, workspace=own, options=short)
+        assert own is None or wsb is own
+        with pytest.raises(ops.AclnnError) as ei:
+            ops.check_status(wsb)
+        assert ei.value.status == _lib.ACLNN_ERR_RUNTIME_ERROR and ei.value.record[0] == 1
+        got, wsb = ops.adapter_add(*args, return_workspace=True, workspace=own, options=ops.LaunchOptions(wait_limit_cycles=1 << 31))
+        ops.check_status(wsb)
+        assert torch.equal(got, want)
+    # the kernels for a few tokens keep a status as well, which is clean
+    _, wsb = ops.adapter_add(*(a[:4] if i != 2 and i != 3 else a for i, a in enumerate(args)), return_workspace=True)
+    ops.check_status(wsb)
+    assert ops.adapter_add(*(a[:0] if i != 2 and i != 3 else a for i, a in enumerate(args)), return_workspace=True)[1] is None
+    with pytest.raises(ops.AclnnError, match="SetExecutorOptions"):
+        ops.adapter_add(*args, options=ops.LaunchOptions(wait_limit_cycles=-1))
