@@ -128,8 +128,8 @@ ACL_FUNC_VISIBILITY aclnnStatus gmmB200GroupedMatmulW8A8(const void *x, const vo
 
 /* Three operators that stand around the expert FFN in a mixture-of-experts block, in the two-phase form of the aclnn operators (checks
  * and executor in the first call, which never touches the device; the second enqueues on `stream` and uses the executor up).  Absent
- * optional tensors are null.  Views whose rows are dense are read and written where they are, others through copies in the
- * workspace.  Lengths of zero are valid where stated and do nothing. */
+ * optional tensors are null.  Tensors begin on a boundary of their elements, a workspace on one of 16 bytes.  Views whose rows are dense
+ * are read and written where they are, others through copies in the workspace.  Lengths of zero are valid where stated and do nothing. */
 
 /* The norm in front of the experts, with the int8 rows and per-token scales that the W8A8 operators take:
  *   h = x + residual (fp32);  r = 1 / sqrt(mean(h^2) + eps);  u = h * gamma * smooth;  step = max|u| / 127

@@ -444,6 +444,8 @@ def _block_call(op: int, name: str, workspace: Optional[torch.Tensor], stream, o
     module, call = _lib.native()
     x, buf = items[0], workspace
     how = 0 if options is None else C.addressof(options)
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
     pooled = workspace is None and op == _lib.OP_ADAPTER_ADD
     if not x.is_cuda:
         done = False

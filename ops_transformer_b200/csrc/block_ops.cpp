@@ -14,6 +14,7 @@ constexpr int64_t kMaxRows = 0x7fffffffll / 2;
 
 // A tensor that may be absent, but not with elements and without an address, nor in a private format.
 bool usable(const aclTensor *t) { return !t || ((t->data || t->empty()) && !is_private_format(t->format)); }
+bool on_boundary(const aclTensor *t) { return !t || t->empty() || reinterpret_cast<uintptr_t>(tensor_ptr(t)) % dtype_size(t->dtype) == 0; }
 
 bool is_float(aclDataType t) { return t == ACL_FLOAT || t == ACL_FLOAT16 || t == ACL_BF16; }
 
@@ -32,9 +33,11 @@ struct NewExecutor {
 
 #define REQUIRE_NOT_NULL(t) GMM_REQUIRE((t) != nullptr, ACLNN_ERR_PARAM_NULLPTR, #t " must not be nullptr.")
 #define REQUIRE_RANK(t, r) GMM_REQUIRE((t)->rank() == (r), ACLNN_ERR_PARAM_INVALID, #t " dim num should be %d, but now is %zu.", (r), (t)->rank())
-#define REQUIRE_USABLE(...)                  \
-    for (const aclTensor *t_ : std::initializer_list<const aclTensor *>{__VA_ARGS__}) \
-    GMM_REQUIRE(usable(t_), ACLNN_ERR_PARAM_INVALID, "tensors must have an address and must not have a private format.")
+#define REQUIRE_USABLE(...)                                                                                                          \
+    for (const aclTensor *t_ : std::initializer_list<const aclTensor *>{__VA_ARGS__}) {                                               \
+        GMM_REQUIRE(usable(t_), ACLNN_ERR_PARAM_INVALID, "tensors must have an address and must not have a private format.");        \
+        GMM_REQUIRE(on_boundary(t_), ACLNN_ERR_PARAM_INVALID, "tensors must be aligned to their elements.");                         \
+    }
 #define REQUIRE_SHAPE1(t, a) \
     GMM_REQUIRE((t)->rank() == 1 && (t)->dim(0) == (a), ACLNN_ERR_PARAM_INVALID, #t " shape must be [%lld].", (long long)(a))
 #define REQUIRE_SHAPE2(t, a, b)                                                                                                     \

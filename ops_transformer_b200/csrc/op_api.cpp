@@ -86,11 +86,17 @@ aclnnStatus run_executor(const char *op_name, void *workspace, uint64_t workspac
         rc = fail(ACLNN_ERR_PARAM_INVALID, "%s: executor was built by %s.", op_name, executor->op_name);
     } else if (executor->kind != aclOpExecutor::kNoop) {
         const size_t need = executor->plan.ws_bytes + executor->staged_bytes;
+        // What is read and written there: packs by the operators around the expert FFN, whole elements in the copies of strided views.
+        size_t boundary = executor->kind >= aclOpExecutor::kNormQuant ? 16 : 1;
+        for (const StagedView &v : executor->staged)
+            if ((size_t)v.elem > boundary) boundary = (size_t)v.elem;
         if (workspace_size < need) {
             rc = fail(ACLNN_ERR_PARAM_INVALID, "%s: workspaceSize %llu is smaller than the %llu bytes required.", op_name,
                       (unsigned long long)workspace_size, (unsigned long long)need);
         } else if (need && !workspace) {
             rc = fail(ACLNN_ERR_PARAM_NULLPTR, "%s: workspace must not be nullptr.", op_name);
+        } else if (need && reinterpret_cast<uintptr_t>(workspace) % boundary) {
+            rc = fail(ACLNN_ERR_PARAM_INVALID, "%s: workspace must be aligned to %zu bytes.", op_name, boundary);
         } else {
             cudaStream_t cs = static_cast<cudaStream_t>(stream);
             char *tail = static_cast<char *>(workspace) + executor->plan.ws_bytes;

@@ -158,3 +158,63 @@ def test_numbers_are_read_anew_in_every_call():
     assert [acl._float_bits(v) for v in (0.0, -0.0, 0.0, 1, True, 1.0)] == [0, 1 << 31, 0] + [bits(1.0)] * 3
     with pytest.raises(struct.error):
         acl._float_bits("1")
+
+
+def _planned(op, words):
+    res = _lib.CallResult()
+    assert _lib.lib().gmmB200Call(op | _lib.OP_PLAN_ONLY, words, len(words) // 8, None, 0, None, None, C.byref(res)) == 0, _lib.last_error()
+    return C.c_void_p(res.executor), res.workspaceSize
+
+
+@pytest.mark.parametrize("shift", [1, 2, 4, 8])
+def test_workspaces_that_kernels_cannot_use_are_refused_before_anything_is_enqueued(shift):
+    """Copies of strided views and partial sums are read and written by whole elements and packs."""
+    apart = lambda *s, dtype=BF16: torch.empty(s[:-1] + (2 * s[-1],), dtype=dtype)[..., ::2]  # noqa: E731
+    x, gamma, q, scale = apart(4, 64), e(64), e(4, 64, dtype=I8), e(4, dtype=F32)
+    logits, weights, ids = apart(6, 32, dtype=F32), e(6, 4, dtype=F32), e(6, 4, dtype=I32)
+    base, ax, a, b = e(6, 48), apart(6, 64), e(3, 16, 64), e(3, 48, 16)
+    calls = [("gmmB200AddRmsNormQuant", _lib.OP_ADD_RMS_NORM_QUANT,
+              _lib.describe_call("tttttttti", x, None, gamma, None, q, scale, None, None, acl._float_bits(1e-6))),
+             ("gmmB200RouteTopK", _lib.OP_ROUTE_TOP_K, _lib.describe_call("tttttiiiiii", logits, None, None, weights, ids, 0, 1, 1, 0, 1, acl._float_bits(1.0))),
+             ("gmmB200AdapterAdd", _lib.OP_ADAPTER_ADD, _lib.describe_call("tttttttt", base, ax, None, a, b, e(6, dtype=I32), None, base))]
+    if shift < 4:   # the copy of the scales, for an operator whose workspace may begin on any boundary of 4 bytes
+        calls.append(("aclnnGroupedMatmulV4", _lib.OP_GMM["V4"], _lib.describe_call(
+            "tftttttiiiiil", e(4, 32, dtype=I8), (e(1, 32, 64, dtype=I8), 2, None), None, e(1, 64, dtype=F32), apart(4, dtype=F32),
+            e(1, dtype=torch.int64), e(4, 64), 3, 0, 0, 0, 0, None)))
+    for name, op, words in calls:
+        ex, need = _planned(op, words)
+        assert need > 0
+        room = torch.empty(need + 64, dtype=torch.uint8)
+        at = (room.data_ptr() + 15) // 16 * 16 + shift
+        assert getattr(_lib.lib(), name)(at, need, ex, None) == INVALID
+        assert "aligned" in _lib.last_error()
+
+
+def test_tensors_off_their_elements_boundaries_are_refused():
+    room = torch.empty(4096, dtype=torch.uint8)
+    at = (room.data_ptr() + 15) // 16 * 16 + 1
+    def moved(words, place):   # the tensor of `place` begins at an odd address
+        w = list((C.c_int64 * (len(words) // 8)).from_buffer_copy(words))
+        i = 0
+        for _ in range(place):
+            i += 1 if w[i] < 0 else 4 + 2 * w[i] + 1 + w[i + 4 + 2 * w[i]]
+        w[i + 1] = at
+        return (C.c_int64 * len(w))(*w), len(w)
+
+    res = _lib.CallResult()
+    for op, words, places in [
+            (_lib.OP_ADD_RMS_NORM_QUANT, _lib.describe_call("tttttttti", e(2, 8), e(2, 8), e(8), e(8, dtype=F32), e(2, 8, dtype=I8), e(2, dtype=F32), e(2, 8),
+                                                            e(2, 8), acl._float_bits(1e-6)), (0, 1, 2, 3, 5, 6, 7)),
+            (_lib.OP_ROUTE_TOP_K, _lib.describe_call("tttttiiiiii", e(2, 8), e(8, dtype=F32), None, e(2, 2, dtype=F32), e(2, 2, dtype=I32), 0, 1, 1, 0, 1,
+                                                     acl._float_bits(1.0)), (0, 1, 3, 4)),
+            (_lib.OP_ADAPTER_ADD, _lib.describe_call("tttttttt", e(2, 8), e(2, 8, dtype=I8), e(2, dtype=F32), e(1, 4, 8), e(1, 8, 4), e(2, dtype=I32),
+                                                     e(1, dtype=F32), e(2, 8)), (0, 2, 3, 4, 5, 6, 7))]:
+        for place in places:
+            w, n = moved(words, place)
+            assert _lib.lib().gmmB200Call(op | _lib.OP_PLAN_ONLY, w, n, None, 0, None, None, C.byref(res)) == INVALID, place
+            assert "aligned" in _lib.last_error()
+
+
+def test_a_workspace_in_pieces_is_refused():
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.adapter_add(e(6, 48), e(6, 64), e(3, 16, 64), e(3, 48, 16), e(6, dtype=I32), workspace=torch.empty(1, dtype=torch.uint8).expand(1 << 24))
