@@ -314,7 +314,8 @@ __global__ void __launch_bounds__(MAXT, MINB) norm_quant_kernel(const NormParams
         f32x2 sum2 = 0;
         float mag = 0.0f;
         if (STREAM) asm volatile("cp.async.wait_group 0;" ::: "memory");
-        for (int c0 = threadIdx.x; c0 < packs; c0 += threads * NCH) {
+        // A row that streams fits: one turn, which threads without a pack of it take too, since the next row may have one for them.
+        for (int c0 = threadIdx.x; c0 < packs || (STREAM && c0 < threads); c0 += threads * NCH) {
 #pragma unroll
             for (int i = 0; i < NCH; ++i) {
                 if (c0 + i * threads < packs) load_h(c0 + i * threads, i, u[i]);

@@ -692,3 +692,50 @@ def check_adapter_fp32(c, out):
     over, fits = want.abs() - tol > most, want.abs() + tol < most
     assert torch.equal(out[over].double(), want[over].sign() * math.inf) and out[fits].isfinite().all()
     assert ((out.double() - want).abs() <= tol)[fits].all()
+
+
+# More rows than find a place on the GPU together: a CTA goes through several, with the copies of the next under way.  Rows of one pack and of
+# four a thread, of one warp and of many, on pack boundaries and off them.
+NORM_MANY_ROWS = [(4096, 7168), (4096, 3500), (1500, 5001), (5000, 20), (2500, 1423), (6000, 1), (9500, 255), (2600, 2049), (1800, 4097)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("rows,h", NORM_MANY_ROWS)
+def test_norm_many_rows(rows, h, dtype):
+    x, res = randn((rows, h), 1, dtype), randn((rows, h), 2, dtype, 3.0)
+    gamma = randn((h,), 3, dtype, 0.2) + 1
+    smooth = torch.rand(h, device=DEV, generator=gen(4)) + 0.5
+    for residual, sm, normed in ((res, None, True), (None, smooth, False), (res, smooth, True), (None, None, False)):
+        got = ops.add_rms_norm_quant(x, gamma, residual=residual, smooth=sm, eps=1e-5, normed=normed)
+        check_norm(x, gamma, residual, sm, 1e-5, got)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,h", [(4096, 3584), (2500, 1423), (5000, 20)])
+def test_norm_many_rows_in_place(rows, h, dtype):
+    x, res, gamma = randn((rows, h), 1, dtype), randn((rows, h), 2, dtype), randn((h,), 3, dtype)
+    want = ops.add_rms_norm_quant(x, gamma, residual=res, normed=True)
+    check_norm(x, gamma, res, None, 1e-6, want)
+    for into in ("residual", "x"):
+        a, b = x.clone(), res.clone()
+        got = ops.add_rms_norm_quant(a, gamma, residual=b, residual_out=b if into == "residual" else a, normed_out=a if into == "residual" else None)
+        assert all(torch.equal(g, w) for g, w in zip(got[:3], want[:3]))
+        if into == "residual":
+            assert torch.equal(a, want[3])
+    alone = x.clone()
+    got = ops.add_rms_norm_quant(alone, gamma, normed_out=alone)
+    check_norm(x, gamma, None, None, 1e-6, got)
+
+
+@pytest.mark.parametrize("rows,h,pitch", [(5000, 100, 103), (5000, 100, 96), (2500, 1423, 1429), (1200, 7000, 7007), (3000, 1024, 2048)])
+def test_norm_many_rows_apart(rows, h, pitch):
+    """Rows that do not begin where the last one ends, behind one another or into one another; nothing lies behind the last one."""
+    for dtype in (BF16, F32):
+        at = lambda seed, p, n: randn(((rows - 1) * p + n,), seed, dtype).as_strided((rows, n), (p, 1))  # noqa: E731
+        x, res, gamma = at(1, pitch, h), at(2, pitch, h), randn((h,), 3, dtype)
+        check_norm(x, gamma, res, None, 1e-6, ops.add_rms_norm_quant(x, gamma, residual=res, normed=True))
+        if pitch >= h:   # outputs between the rows of which nothing may be written
+            out = torch.full((rows * pitch,), 7.0, dtype=dtype, device=DEV)
+            view = out[:(rows - 1) * pitch + h].as_strided((rows, h), (pitch, 1))
+            check_norm(x, gamma, res, None, 1e-6, ops.add_rms_norm_quant(x, gamma, residual=res, normed_out=view))
+            assert (out.view(rows, pitch)[:, h:] == 7.0).all()
