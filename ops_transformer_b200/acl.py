@@ -535,6 +535,8 @@ def route_top_k(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", b
         letter = _ID_LETTER.get(ids_dtype)
         shape = logits.shape[0], top_k
         ids = empty(logits, letter, *shape) if letter else logits.new_empty(shape, dtype=ids_dtype)   # refused by the operator
+    if weights.shape == ids.shape and weights.shape[-1:] != (top_k,):
+        raise ValueError(f"weights and ids must have top_k = {top_k} columns")
     if token_mask is not None and token_mask.dtype == torch.bool:
         token_mask = token_mask.view(torch.int8)
     _block_call(_lib.OP_ROUTE_TOP_K, "gmmB200RouteTopK", workspace, stream, None, "tttttiiiiii", logits, bias, token_mask, weights, ids,

@@ -218,3 +218,11 @@ def test_tensors_off_their_elements_boundaries_are_refused():
 def test_a_workspace_in_pieces_is_refused():
     with pytest.raises(ValueError, match="contiguous"):
         ops.adapter_add(e(6, 48), e(6, 64), e(3, 16, 64), e(3, 48, 16), e(6, dtype=I32), workspace=torch.empty(1, dtype=torch.uint8).expand(1 << 24))
+
+
+def test_route_outputs_of_another_width_are_refused():
+    for n in (3, 8):
+        with pytest.raises(ValueError, match="top_k"):
+            ops.route_top_k(e(6, 32, dtype=F32), 4, weights=e(6, n, dtype=F32), ids=e(6, n, dtype=I32))
+    assert route(top_k=4, weights=e(6, 4, dtype=F32), ids=e(6, 4, dtype=I32)) == 0
+    assert route(top_k=4, weights=e(6, 4, dtype=F32), ids=e(6, 8, dtype=I32)) == INVALID
