@@ -739,3 +739,172 @@ def test_norm_many_rows_apart(rows, h, pitch):
             view = out[:(rows - 1) * pitch + h].as_strided((rows, h), (pitch, 1))
             check_norm(x, gamma, res, None, 1e-6, ops.add_rms_norm_quant(x, gamma, residual=res, normed_out=view))
             assert (out.view(rows, pitch)[:, h:] == 7.0).all()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# adapter_add's two ways: a few tokens on the CUDA cores, tiles of 16, 64 or 128 tokens on the tensor cores
+# ---------------------------------------------------------------------------------------------------------------------
+
+def adapter_way(c):
+    """"few", or the tokens of a tile, for calls of these sizes (the way does not hang on the ids), from what one leaves in its workspace: behind
+    the status (256 bytes) the tiles' way keeps the number of tiles, in 256 bytes of their own; the other way keeps x a^T there."""
+    T, c = len(c["base"]), dict(c, adapter_ids=torch.zeros_like(c["adapter_ids"]))
+    need = ops.adapter_add(**c, return_workspace=True)[1].numel()
+    ws = torch.full((need,), 0x5a, dtype=torch.uint8, device=DEV)
+    ops.adapter_add(**c, workspace=ws)
+    ops.check_status(ws)
+    head = ws[256:512].cpu()
+    if not (head[4:] == 0x5a).all():
+        return "few"
+    return next(t for t in (16, 64, 128) if (T + t - 1) // t == int(head[:4].view(torch.int32)))
+
+
+# tokens, K, adapters, rank and the way that these sizes take; a K that is no multiple of 8 keeps few tokens off the CUDA cores
+ADAPTER_WAYS = [(60, 512, 3, 16, "few"), (60, 511, 3, 16, 64), (70, 511, 5, 16, 16), (300, 512, 60, 16, 16), (400, 512, 3, 16, 64), (400, 513, 3, 31, 64),
+                (300, 512, 3, 128, 64), (2100, 512, 2, 16, 128), (2300, 512, 4, 61, 128)]
+
+
+@pytest.mark.parametrize("T,K,L,r,way", ADAPTER_WAYS)
+def test_adapter_ways_are_the_ones_that_are_meant(T, K, L, r, way):
+    for dtype, x_i8 in ((BF16, False), (F16, True)):
+        c = adapter_case(T, K, 264, L, r, dtype, x_i8, ids=(torch.arange(T, device=DEV) % L).to(torch.int32))
+        assert adapter_way(c) == way
+        check_adapter(c, ops.adapter_add(**c))
+
+
+@pytest.mark.parametrize("T,K,L,r,way", ADAPTER_WAYS)
+def test_adapter_ways_nan_and_infinities_stay_in_their_rows(T, K, L, r, way):
+    for x_i8 in (False, True):
+        ids = (torch.arange(T, device=DEV) % (L + 1) - 1).to(torch.int32)
+        c = adapter_case(T, K, 264, L, r, x_i8=x_i8, ids=ids)
+        ops.adapter_add(**dict(c, x=torch.full_like(c["x"], 127) if x_i8 else torch.full_like(c["x"], math.nan)))   # NaN left behind on the chip
+        clean = ops.adapter_add(**c)
+        ids[7], ids[8], ids[9] = 0, 1, 1
+        if x_i8:
+            c["x_scale"][7], c["x_scale"][8] = math.nan, math.inf
+        else:
+            c["x"][7, 100], c["x"][8, 3] = math.nan, math.inf
+        c["base"][9, 5] = math.inf
+        out = ops.adapter_add(**c)
+        assert out[7].isnan().all() and not out[8].isfinite().any() and out[9, 5] == math.inf
+        keep = torch.ones(T, dtype=torch.bool, device=DEV)
+        keep[7:10] = False
+        assert torch.equal(out[keep], clean[keep])
+        check_adapter({n: (v[keep] if n in ("base", "x", "adapter_ids", "x_scale") and v is not None else v) for n, v in c.items()}, out[keep])
+        # weights of adapters that no token names
+        c = adapter_case(T, K, 264, L, r, x_i8=x_i8, ids=torch.full_like(ids, 1))
+        want = ops.adapter_add(**c)
+        c["a"][0], c["b"][0], c["scaling"][0] = math.nan, math.inf, math.nan
+        assert torch.equal(ops.adapter_add(**c), want)
+        check_adapter(dict(c, a=c["a"].nan_to_num(), b=c["b"].nan_to_num(), scaling=c["scaling"].nan_to_num()), want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,K,L,r,way", ADAPTER_WAYS)
+def test_adapter_ways_infinite_activations(T, K, L, r, way, dtype):
+    c = adapter_case(T, K, 200, L, r, dtype, ids=(torch.arange(T, device=DEV) % L).to(torch.int32))
+    c["a"][:, :, 5] = 0.5
+    c["b"] = c["b"].abs() + 0.25
+    c["b"][:, 1::2] *= -1
+    clean = ops.adapter_add(**c)
+    c["x"][3, 5] = math.inf
+    out = ops.adapter_add(**c)
+    assert torch.equal(out[3], torch.tensor([math.inf, -math.inf], device=DEV, dtype=dtype).repeat(100))
+    others = torch.arange(T, device=DEV) != 3
+    assert torch.equal(out[others], clean[others])
+
+
+@pytest.mark.parametrize("T,K,L,r,way", ADAPTER_WAYS)
+def test_adapter_ways_large_values_fp16(T, K, L, r, way):
+    c = adapter_case(T, K, 264, L, r, F16, ids=(torch.arange(T, device=DEV) % L).to(torch.int32))
+    c["a"].mul_(2000)
+    c["x"].mul_(40)
+    c["b"].mul_(1e-3)
+    check_adapter(c, ops.adapter_add(**c))
+
+
+@pytest.mark.parametrize("T,K,L,r,way", ADAPTER_WAYS)
+def test_adapter_ways_one_adapter_none_and_out_of_range(T, K, L, r, way):
+    for ids in (torch.full((T,), L - 1), torch.full((T,), -1), torch.full((T,), L), torch.arange(T) % (L + 4) - 2, torch.full((T,), 2 ** 31 - 1),
+                torch.full((T,), -2 ** 31)):
+        c = adapter_case(T, K, 264, L, r, ids=ids.to(torch.int32).to(DEV), scaling=False)
+        check_adapter(c, ops.adapter_add(**c))
+
+
+@pytest.mark.parametrize("T,K,L,r,way", ADAPTER_WAYS)
+def test_adapter_ways_in_place_and_strides(T, K, L, r, way):
+    for N in (264, 261):
+        c = adapter_case(T, K, N, L, r)
+        want = ops.adapter_add(**c)
+        check_adapter(c, want)
+        base = c["base"].clone()
+        assert ops.adapter_add(**dict(c, base=base), out=base) is base and torch.equal(base, want)
+        for off, pitch in ((0, 1024), (8, 1040), (3, 777)):
+            wide = lambda t: torch.full((T * pitch + 16,), 3.0, dtype=t.dtype, device=DEV)[off:off + T * pitch]  # noqa: E731
+            rows = lambda t, n: t.view(T, pitch)[:, :n]  # noqa: E731
+            x, base = rows(wide(c["x"]), K).copy_(c["x"]), wide(c["base"])
+            out = rows(base, N).copy_(c["base"])
+            assert ops.adapter_add(**dict(c, base=out, x=x), out=out) is out
+            check_adapter(c, out)
+            assert (base.view(T, pitch)[:, N:] == 3.0).all()
+
+
+@pytest.mark.parametrize("T,K,L,r,pitch", [(3, 63, 2, 8, 1 << 30), (300, 64, 2, 8, 1 << 23), (300, 64, 60, 8, 1 << 23)])
+def test_adapter_ways_offsets_beyond_32_bits(T, K, L, r, pitch):
+    c = adapter_case(T, K, 64, L, r, ids=(torch.arange(T, device=DEV) % (L + 1) - 1).to(torch.int32))
+    assert adapter_way(c) == (16 if L == 60 or T == 3 else 64)
+    big = torch.zeros((T - 1) * pitch + 64, dtype=BF16, device=DEV)
+    rows = lambda n: big.as_strided((T, n), (pitch, 1))  # noqa: E731
+    want = ops.adapter_add(**c)
+    check_adapter(c, want)
+    assert torch.equal(ops.adapter_add(**dict(c, x=rows(K).copy_(c["x"]))), want)
+    rows(64).copy_(c["base"])
+    assert torch.equal(ops.adapter_add(**dict(c, base=rows(64))), want)
+    assert torch.equal(ops.adapter_add(**dict(c, base=rows(64)), out=rows(64)), want)
+
+
+@pytest.mark.parametrize("T,K,L,r,way", ADAPTER_WAYS)
+def test_adapter_ways_streams_and_replays_with_other_ids(T, K, L, r, way):
+    c = adapter_case(T, K, 264, L, r)
+    want = ops.adapter_add(**c)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    got = ops.adapter_add(**c, stream=s)
+    s.synchronize()
+    assert torch.equal(got, want)
+    with torch.cuda.stream(s):
+        got = ops.adapter_add(**c)
+    s.synchronize()
+    assert torch.equal(got, want) and all(torch.equal(ops.adapter_add(**c), want) for _ in range(3))
+    torch.cuda.synchronize()
+    # which tokens share an adapter is found anew in every replay, for any distribution of them
+    live = dict(c, adapter_ids=c["adapter_ids"].clone())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.adapter_add(**live)
+    at = torch.arange(T, device=DEV)
+    for ids in (c["adapter_ids"], at % L, at * 0, at * 0 - 1, at * (L + 2) // T - 1, at % (L + 1) - 1, c["adapter_ids"].flip(0), at * 0 + L - 1):
+        live["adapter_ids"].copy_(ids)
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        fresh = dict(c, adapter_ids=ids.to(torch.int32))
+        assert torch.equal(got, ops.adapter_add(**fresh))
+        check_adapter(fresh, got)
+
+
+@pytest.mark.parametrize("T,L,r", [(8192, 5, 8), (8193, 3, 8), (16384, 40, 8), (20000, 1500, 4), (9000, 1024, 4), (3000, 16384, 2), (300, 12000, 4)])
+def test_adapter_many_tokens_and_many_adapters(T, L, r):
+    """More tokens than the plan keeps in registers, more adapters than it has threads, and than its counters fit the usual shared memory."""
+    for ids in (torch.randint(-1, L, (T,), device=DEV, generator=gen(1)), torch.arange(T, device=DEV) * L // T, torch.arange(T, device=DEV) % 2 * (L - 1)):
+        c = adapter_case(T, 72, 72, L, r, ids=ids.to(torch.int32))
+        # as check_adapter, without a loop over thousands of adapters
+        at = c["adapter_ids"].long().clamp_min(0)
+        x, a, b, s = c["x"].double(), c["a"].double()[at], c["b"].double()[at], c["scaling"].double()[at, None]
+        s = torch.where(c["adapter_ids"][:, None] < 0, 0.0, s)
+        delta = lambda x, a, b: s * torch.einsum("tr,tnr->tn", torch.einsum("tk,trk->tr", x, a), b)  # noqa: E731
+        want, mag = c["base"].double() + delta(x, a, b), delta(x.abs(), a.abs(), b.abs())
+        out = ops.adapter_add(**c)
+        tol = mag * (72 / 16 + r / 16 + 8) * 2 * U32 + want.abs() * HALF_ULP[BF16] * 1.001 + TINY[BF16]
+        assert ((out.double() - want).abs() <= tol).all()
+        assert torch.equal(out[c["adapter_ids"] < 0], c["base"][c["adapter_ids"] < 0])
