@@ -32,17 +32,19 @@ class Adapters:
 
 class QuantMoeBlock:
     """Weights of the experts: w_gate_up int8 [E, hidden, 2 * inter], w_down int8 [E, inter, hidden], scales fp32 per channel; of the shared
-    expert: the same with E = 1.  ``router`` bf16 [E, hidden], ``router_bias`` fp32 [E] or None.  Hidden states are bf16."""
+    expert: the same with E = 1.  ``router`` bf16 [E, hidden], ``router_bias`` fp32 [E] or None.  Hidden states are bf16.  Without
+    ``renormalize`` the chosen experts' weights are their scores as they are (times ``routed_scale``)."""
 
     def __init__(self, gamma, router, w_gate_up, s_gate_up, w_down, s_down, shared_gate_up, shared_s_gate_up, shared_down, shared_s_down, *,
                  top_k: int, router_bias=None, scoring: str = "softmax", n_group: int = 1, topk_group: int = 1, group_score: str = "max",
-                 routed_scale: float = 1.0, eps: float = 1e-6, adapters: Optional[Adapters] = None):
+                 routed_scale: float = 1.0, renormalize: bool = True, eps: float = 1e-6, adapters: Optional[Adapters] = None):
         self.gamma, self.router, self.router_bias = gamma, router.t(), router_bias
         self.w_gate_up, self.s_gate_up = w_gate_up, s_gate_up
         self.w_down, self.s_down = format_cast_nz(w_down), s_down      # the layout that the combining operator takes
         self.shared = shared_gate_up, shared_s_gate_up, shared_down, shared_s_down
         self.experts, self.top_k = router.shape[0], top_k
-        self.routing = dict(scoring=scoring, n_group=n_group, topk_group=topk_group, group_score=group_score, scale=routed_scale)
+        self.routing = dict(scoring=scoring, n_group=n_group, topk_group=topk_group, group_score=group_score, scale=routed_scale,
+                            renormalize=renormalize)
         self.eps, self.adapters = eps, adapters
 
     def __call__(self, x, residual, *, adapter_ids=None, token_mask=None):

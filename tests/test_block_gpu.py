@@ -113,3 +113,19 @@ def test_block_row_by_row(monkeypatch, tokens, hidden, inter, experts, top_k, ad
     # With two 16-bit roundings of 0.4 % below 8 % if all of it added up.
     off = (out.double() - want).norm(dim=1) / want.norm(dim=1)
     assert (off < 0.08).all()
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_block_weights_as_they_are(monkeypatch, scoring):
+    from ops_transformer_b200 import block as module
+    seen, kept = {}, {}
+    monkeypatch.setattr(module, "route_top_k", lambda logits, k, _f=module.route_top_k, **kw: seen.setdefault("r", (logits, *_f(logits, k, **kw)))[1:])
+    monkeypatch.setattr(module, "format_cast_nz", lambda w, _f=module.format_cast_nz: _f(kept.setdefault("w_down", w)))
+    b = random_block(512, 256, 8, 2, scoring=scoring, routed_scale=1.5, renormalize=False)
+    x, residual = (torch.randn(50, 512, device=DEV, generator=torch.Generator(DEV).manual_seed(i)).to(torch.bfloat16) for i in (1, 2))
+    out, _ = b(x, residual)
+    logits, weights, ids = seen["r"]
+    scores = (torch.softmax(logits.double(), 1) if scoring == "softmax" else torch.sigmoid(logits.double())).gather(1, ids.long())
+    assert torch.allclose(weights.double(), 1.5 * scores, rtol=1e-5, atol=0)
+    want = reference(b, x, residual, ids, 1.5 * scores, None, kept)
+    assert ((out.double() - want).norm(dim=1) / want.norm(dim=1) < 0.08).all()   # as in test_block_row_by_row
