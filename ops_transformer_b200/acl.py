@@ -528,6 +528,8 @@ def route_top_k(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", b
     what ``moe_init_routing_v3`` takes, int64 the expert-parallel layer.  gmmB200RouteTopK (include/gmm_b200.h) has the rules."""
     if scoring not in _SCORING or group_score not in _GROUP_SCORE:
         raise ValueError(f"unknown scoring {scoring!r} or group_score {group_score!r}")
+    if weights is not None and ids is not None and weights.shape == ids.shape and weights.shape[-1:] != (top_k,):
+        raise ValueError(f"weights and ids must have top_k = {top_k} columns")
     empty = _lib.native()[0].empty
     if weights is None:
         weights = empty(logits, "f", logits.shape[0], top_k)
@@ -535,8 +537,6 @@ def route_top_k(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", b
         letter = _ID_LETTER.get(ids_dtype)
         shape = logits.shape[0], top_k
         ids = empty(logits, letter, *shape) if letter else logits.new_empty(shape, dtype=ids_dtype)   # refused by the operator
-    if weights.shape == ids.shape and weights.shape[-1:] != (top_k,):
-        raise ValueError(f"weights and ids must have top_k = {top_k} columns")
     if token_mask is not None and token_mask.dtype == torch.bool:
         token_mask = token_mask.view(torch.int8)
     _block_call(_lib.OP_ROUTE_TOP_K, "gmmB200RouteTopK", workspace, stream, None, "tttttiiiiii", logits, bias, token_mask, weights, ids,
