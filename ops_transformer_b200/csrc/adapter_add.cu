@@ -18,9 +18,9 @@
 // not matter: every row's arithmetic is its own.  A few tokens take two kernels on the CUDA cores instead, whose CTAs find their tiles
 // themselves.
 //
-// 4096 tokens of 8 adapters, 7168 -> 4096, rank 64, bf16: 48 us for 137 MB, which take 21 at the rate of a copy: the plan 5, the first
-// product 17 (its operands come at about 55 bytes per ns and SM, weights included, which every tile reads anew), the second 20 (3 for the
-// partial sums, then 4 TB/s).  611 tokens of 13, 1424 -> 2976, rank 12: 16 us, the three kernels' latencies (3, 5 and 5).
+// 4096 tokens of 8 adapters, 7168 -> 4096, rank 64, bf16: 50 us for 137 MB, which take 21 at the rate of a copy: the plan 5, the first
+// product 17 (its operands come at about 55 bytes per ns and SM, weights included, which every tile reads anew), the second some 22 (3 for
+// the partial sums, then 4 TB/s; with two parts of v the three kernels took 48).  611 tokens of 13, 1424 -> 2976, rank 12: 16 us, the three kernels' latencies (3, 5 and 5).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -429,7 +429,8 @@ __device__ __forceinline__ void copy_base(const AdapterParams &p, const int *row
 // With up to four tokens a tile each weight takes part in four products at most, which costs fewer instructions than bringing it to the
 // tensor cores; the weights go straight from memory to registers, 16 bytes a lane, and every CTA finds its own tile, so there are two
 // kernels and nothing in front of them.  One token, 2048 -> 4096, rank 16: 4.3 us, the two kernels' latency; 128 tokens of 64 adapters,
-// 2048 -> 7168, rank 32, int8: 19.5 us (28 on the tensor cores) for 42 MB, about as many instructions as bytes.
+// 2048 -> 7168, rank 32, int8: 19.3 us (28 on the tensor cores) for 42 MB.  Neither the memory (at 6.4 us for these) nor the issue slots (46 % of
+// them used) bound that: with 74 and 107 registers a thread an SM has 20 and 14 warps at work on average, whose longest stall is for loads.
 
 constexpr int kFew = 4;
 constexpr int kFewThreads = 256;
@@ -1241,9 +1242,11 @@ struct Shape {
 // 36 with tiles of 64) or, where they have 128 and there are enough tiles for the SMs, of 128 (4096 of 8 49.7, 51.9 with tiles of 64; up to
 // rank 64, for the sake of three stages): the first product reads 128 rows of the tokens' tile whether they are tokens or not.  `tiles` is
 // the most there can be: full ones, and one that is not for every adapter and for none; a tile on the CUDA cores may begin with any token.
-// K and N are split so that the CTAs find a place on the SMs together (four of the first kernel's small ones fit an SM, two of the next,
-// one of the large; two of the second's).  Rows that are not copied 16 bytes at a time take longer, so K is split further there (300
-// tokens, 1001 -> 3001: 22 us, 29 with four splits).
+// K and N are split for four of the first kernel's small CTAs on an SM, two of the next size, one large, and two of the second kernel's.  By
+// their shared memory three small ones fit at rank 16, two at higher ranks (one with int8 rows of rank 128); of the next size two up to rank
+// 80 (48 with int8 rows), then one; of the second kernel's two up to rank 64, then one with tiles of 64.  What does not fit comes in a second
+// turn.  Rows that are not copied 16 bytes at a time take longer, so K is split further there (300 tokens, 1001 -> 3001: 22 us, 29 with four
+// splits).  The tensor cores' figures here were taken with two parts of v; the third adds 1 to 4 % to all of them.
 Shape shape_of(const AdapterProblem &p, bool may_be_few)
 {
     Shape s;
