@@ -5,6 +5,7 @@
 //
 // launch() goes one step further for operators whose whole work is a few microseconds: it describes the tensors and makes the call.
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
 
@@ -256,15 +257,12 @@ PyObject *empty(PyObject *, PyObject *const *args, Py_ssize_t nargs)
             return nullptr;
         }
     }
-    try {
+    HANDLE_TH_ERRORS   // what torch raises itself, OutOfMemoryError for instance
         const at::Tensor &t = THPVariable_Unpack(args[0]);
         const at::ScalarType dtype = *type == 'b' ? at::kChar : *type == 'i' ? at::kInt : *type == 'l' ? at::kLong : *type == 'f' ? at::kFloat : t.scalar_type();
         const auto options = at::TensorOptions().dtype(dtype).device(t.device());
         return THPVariable_Wrap(nargs == 2 ? at::empty(t.sizes(), options) : at::empty(at::IntArrayRef(sizes, (size_t)nargs - 2), options));
-    } catch (const std::exception &e) {   // out of memory
-        PyErr_SetString(PyExc_RuntimeError, e.what());
-        return nullptr;
-    }
+    END_HANDLE_TH_ERRORS
 }
 
 PyMethodDef methods[] = {

@@ -908,3 +908,12 @@ def test_adapter_many_tokens_and_many_adapters(T, L, r):
         tol = mag * (72 / 16 + r / 16 + 8) * 2 * U32 + want.abs() * HALF_ULP[BF16] * 1.001 + TINY[BF16]
         assert ((out.double() - want).abs() <= tol).all()
         assert torch.equal(out[c["adapter_ids"] < 0], c["base"][c["adapter_ids"] < 0])
+
+
+def test_results_that_do_not_fit_raise_what_torch_raises():
+    x = torch.zeros((1, 65528), dtype=BF16, device=DEV).expand(1 << 29, 65528)   # 32 TiB of results
+    with pytest.raises(torch.OutOfMemoryError):
+        ops.add_rms_norm_quant(x, x[0])
+    with pytest.raises(torch.OutOfMemoryError):
+        ops.route_top_k(torch.zeros((1, 64), device=DEV).expand(1 << 40, 64), 32)
+    assert torch.isfinite(ops.route_top_k(torch.zeros((2, 64), device=DEV), 2)[0]).all()
