@@ -271,11 +271,11 @@ def _own(s):
                                                  residual_scale=RESIDUAL_SCALE, block_scale=BLOCK_SCALE, smooth=s["smooth"], eps=EPS,
                                                  quant=case["quant"], normed=case["normed"])
         return (None, None, h, y) if q is None else (_values(q, scale), scale, h, y)
-    loss, counts, slope = ops.expert_balance(s["logits"], s["ids"], scoring=case["scoring"], coefficient=COEFFICIENT, token_mask=s["mask"],
-                                             cu_seqlens=s["cu"])
+    loss, counts, weight = ops.expert_balance(s["logits"], s["ids"], scoring=case["scoring"], coefficient=COEFFICIENT, token_mask=s["mask"],
+                                              cu_seqlens=s["cu"])
     if not case["grad"]:
         return loss, counts, None
-    return loss, counts, ops.expert_balance_grad(s["logits"], slope, scoring=case["scoring"], token_mask=s["mask"], cu_seqlens=s["cu"],
+    return loss, counts, ops.expert_balance_grad(s["logits"], counts, weight, scoring=case["scoring"], token_mask=s["mask"], cu_seqlens=s["cu"],
                                                  grad_loss=s["grad_loss"])
 
 
@@ -318,7 +318,7 @@ def exact(case, seed):
     parts = [torch.arange(a, b, device=l.device)[live[a:b]] for a, b in zip(cuts[:-1], cuts[1:])]
     parts = [at for at in parts if len(at)]
     l.requires_grad_(True)
-    loss = torch.zeros((), dtype=torch.float64, device=l.device) if parts else l.nan_to_num(neginf=0.0).sum() * 0
+    loss = l.nan_to_num(neginf=0.0).sum() * 0   # no token at all: no loss, and a gradient of zeros
     for at in parts:
         row = l[at]
         p = torch.softmax(row, 1) if case["scoring"] == "softmax" else torch.sigmoid(row) / torch.sigmoid(row).sum(1, keepdim=True)
