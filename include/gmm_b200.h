@@ -80,6 +80,11 @@ ACL_FUNC_VISIBILITY int32_t gmmB200StreamIsCapturing(aclrtStream stream);
  *   ADD_RMS_NORM_QUANT: x, residual, gamma, smooth, q, scale, residualOut, normedOut; eps (float)
  *   ROUTE_TOP_K: logits, bias, tokenMask, weights, ids; scoring, nGroup, topkGroup, groupScore, renormalize, scale (float)
  *   ADAPTER_ADD: base, x, xScale, a, b, adapterIds, scaling, out
+ *   QUANT_MATMUL: x, weight, scale, perTokenScale, bias, y
+ *   SANDWICH_NORM_QUANT: x, residual, gamma, postGamma, gate, smooth, q, scale, residualOut, normedOut; gateAct, residualScale,
+ *              blockScale, eps, postEps (floats)
+ *   EXPERT_BALANCE: logits, ids, tokenMask, cuSeqlens, loss, counts, weight; scoring, coefficient (float)
+ *   EXPERT_BALANCE_GRAD: logits, counts, weight, tokenMask, cuSeqlens, gradLoss, grad; scoring
  * If the workspace is too small, or a pooled one and the stream is being captured, the first phase's executor comes back (stage
  * PLANNED): the caller allocates result->workspaceSize bytes and makes the operator's second-phase call, or destroys the executor.  Otherwise stage says
  * how far the call came when its status is not ACLNN_SUCCESS. */
@@ -87,6 +92,7 @@ enum {
     GMM_B200_OP_GMM_V4 = 0, GMM_B200_OP_GMM_V5 = 1, GMM_B200_OP_GMM_WEIGHT_NZ = 2, GMM_B200_OP_SWIGLU_QUANT = 3,
     GMM_B200_OP_SWIGLU_QUANT_WEIGHT_NZ = 4, GMM_B200_OP_FINALIZE_ROUTING = 5, GMM_B200_OP_FINALIZE_ROUTING_V2 = 6,
     GMM_B200_OP_MOE_INIT_ROUTING_V3 = 7, GMM_B200_OP_ADD_RMS_NORM_QUANT = 8, GMM_B200_OP_ROUTE_TOP_K = 9, GMM_B200_OP_ADAPTER_ADD = 10,
+    GMM_B200_OP_QUANT_MATMUL = 11, GMM_B200_OP_SANDWICH_NORM_QUANT = 12, GMM_B200_OP_EXPERT_BALANCE = 13, GMM_B200_OP_EXPERT_BALANCE_GRAD = 14,
     GMM_B200_OP_POOLED = 0x100,   /* added to the operator: `workspace` comes from a pool and is not used if `stream` is being captured */
     GMM_B200_OP_PLAN_ONLY = 0x200 /* added to the operator: the first phase alone (stage PLANNED), whatever workspace is there */
 };
@@ -184,6 +190,84 @@ ACL_FUNC_VISIBILITY aclnnStatus gmmB200AdapterAddGetWorkspaceSize(
     const aclTensor *base, const aclTensor *x, const aclTensor *xScaleOptional, const aclTensor *a, const aclTensor *b,
     const aclTensor *adapterIds, const aclTensor *scalingOptional, aclTensor *out, uint64_t *workspaceSize, aclOpExecutor **executor);
 ACL_FUNC_VISIBILITY aclnnStatus gmmB200AdapterAdd(void *workspace, uint64_t workspaceSize, aclOpExecutor *executor, aclrtStream stream);
+
+/* What closes a mixture-of-experts block, in the same form and under the same rules as the three operators above: a dense W8A8 product,
+ * the norms on either side of the block's end, and the experts' load. */
+
+/* A matrix product of 8-bit integers with a scale for each token and each channel (no groups, no group list):
+ *   y[t, c] = ((sum_k x[t, k] weight[k, c]) * scale[c]) * perTokenScale[t] + bias[c]
+ * The sum is exact (int32), every step behind it is rounded in fp32, the result once more to y's type; with a 16-bit y and no bias these
+ * are the values of aclnnGroupedMatmulV4 with one group of all rows.
+ *   x                 int8 [m, k], m may be 0, k in [1, 65535]
+ *   weight            int8 [k, n], or the transposed view of a weight stored [n, k]; n in [1, 2^24]
+ *   scale             fp32 / fp16 / bf16 [n];   perTokenScale  fp32 [m], optional (1 without it);   bias  fp32 / fp16 / bf16 [n], optional
+ *   y                 fp32 / fp16 / bf16 [m, n]; shares no memory with the inputs
+ * x, weight and y may be views whose rows (of a transposed view: columns) are dense.  Addresses and distances of rows that are multiples
+ * of 16 bytes are read in place, others through a copy of the operand in the workspace.  gmmB200LaunchOptions: waitLimitCycles; a wait
+ * that runs out is reported by gmmB200CheckStatus. */
+ACL_FUNC_VISIBILITY aclnnStatus gmmB200QuantMatmulGetWorkspaceSize(
+    const aclTensor *x, const aclTensor *weight, const aclTensor *scale, const aclTensor *perTokenScaleOptional,
+    const aclTensor *biasOptional, aclTensor *y, uint64_t *workspaceSize, aclOpExecutor **executor);
+ACL_FUNC_VISIBILITY aclnnStatus gmmB200QuantMatmul(void *workspace, uint64_t workspaceSize, aclOpExecutor *executor, aclrtStream stream);
+
+/* The way from one block into the next: the norm behind a block, its gate, the scaled residual sum, and the norm in front of the next block
+ * with the int8 rows and per-token scales that the W8A8 operators take:
+ *   n = x * (1 / sqrt(mean(x^2) + postEps)) * postGamma       (n = x without postGamma)
+ *   s = residualScale * residual + blockScale * act(gate) * n   (act(gate) = 1 without gate);  residualOut = s
+ *   r = 1 / sqrt(mean(s^2) + eps);  normedOut = s * r * gamma
+ *   u = s * gamma * smooth;  step = max|u| / 127;  q = rint(u / step) within [-127, 127] (0 where step is 0 or not finite);  scale = step * r
+ * All in fp32; s is not rounded before it is normed; 16-bit outputs are rounded once.  A row that holds an infinity or a NaN gets a scale
+ * of NaN.
+ *   x                 [rows, h] residual's type or fp32 (what the finalize-routing operator returns);  h in [1, 65535], rows may be 0
+ *   residual          [rows, h] fp32 / fp16 / bf16
+ *   gamma, postGamma  [h] residual's type or fp32, both the same type; gamma is needed by q and normedOut
+ *   gate              residual's type: [h] or [1, h] (one for each channel), [rows, 1] (one for each token), [rows, h] or [1, 1]; optional
+ *   gateAct           0 the gate as it is, 1 its sigmoid, 2 its tanh
+ *   smooth            fp32 [h], optional
+ *   q                 int8 [rows, h], optional, together with scale  fp32 [rows]
+ *   residualOut, normedOut   [rows, h] residual's type, each optional; one of q, residualOut and normedOut is needed.  residualOut may be
+ *                     residual, or x where that has its type; normedOut may be x if residualOut is not
+ *   residualScale, blockScale finite; eps, postEps positive and finite */
+ACL_FUNC_VISIBILITY aclnnStatus gmmB200SandwichNormQuantGetWorkspaceSize(
+    const aclTensor *x, const aclTensor *residual, const aclTensor *gammaOptional, const aclTensor *postGammaOptional,
+    const aclTensor *gateOptional, const aclTensor *smoothOptional, int64_t gateAct, float residualScale, float blockScale, float eps,
+    float postEps, aclTensor *qOptional, aclTensor *scaleOptional, aclTensor *residualOutOptional, aclTensor *normedOutOptional,
+    uint64_t *workspaceSize, aclOpExecutor **executor);
+ACL_FUNC_VISIBILITY aclnnStatus gmmB200SandwichNormQuant(void *workspace, uint64_t workspaceSize, aclOpExecutor *executor, aclrtStream stream);
+
+/* How a router's choices load the experts, and the loss that evens them out:
+ *   p[t, e] = softmax(logits[t])[e], or sigmoid(logits[t, e]) / sum_j sigmoid(logits[t, j])
+ *   for every sequence s of T tokens:  counts[s, e] = its tokens' ids that are e;  share f = counts * experts / (top_k * T)
+ *   loss = coefficient * mean over the sequences with a token of sum_e f[s, e] * (mean of p[t, e] over the sequence's tokens)
+ * Balanced experts give `coefficient`.  weight[s] = coefficient * experts / (top_k * T^2 * sequences with a token), 0 without a token, is
+ * what the gradient needs beside the counts: a token's p[t, e] adds weight[s] * counts[s, e] * p[t, e] to the loss.  Sums over tokens are
+ * made in a fixed order.
+ *   logits            fp32 / fp16 / bf16 [rows, experts], experts in [1, 1024], rows may be 0 (the loss is 0 then).  An expert whose logit
+ *                     is NaN or minus infinity is not there (p = 0); those of plus infinity share the row's softmax.  A row whose
+ *                     scores are all 0 in fp32 has p = 0
+ *   ids               int32 / int64 [rows, top_k], top_k in [1, 1024]; ids that name no expert (-1) are not counted
+ *   tokenMask         int8 or bool [rows], optional: rows whose value is 0 hold no token
+ *   cuSeqlens         int32 [sequences + 1], optional, not falling: sequence s is the rows [cuSeqlens[s], cuSeqlens[s + 1]), at most 65535
+ *                     sequences; rows outside all of them hold no token, empty sequences count nowhere.  Without it all rows are one
+ *                     sequence.  The values are read on the device and cut to [0, rows]
+ *   scoring           0 softmax, 1 sigmoid;   coefficient  finite
+ *   loss              fp32, one element;  weight  fp32 [sequences];  counts  int64 [sequences, experts], or [experts] without cuSeqlens */
+ACL_FUNC_VISIBILITY aclnnStatus gmmB200ExpertBalanceGetWorkspaceSize(
+    const aclTensor *logits, const aclTensor *ids, const aclTensor *tokenMaskOptional, const aclTensor *cuSeqlensOptional, int64_t scoring,
+    float coefficient, aclTensor *loss, aclTensor *counts, aclTensor *weight, uint64_t *workspaceSize, aclOpExecutor **executor);
+ACL_FUNC_VISIBILITY aclnnStatus gmmB200ExpertBalance(void *workspace, uint64_t workspaceSize, aclOpExecutor *executor, aclrtStream stream);
+
+/* The gradient of that loss with respect to the logits (ids and counts have none), with c[e] = weight[s] * counts[s, e] of the row's sequence:
+ *   softmax  grad[t, e] = gradLoss * p[e] * (c[e] - sum_j p[j] c[j]);   sigmoid  the same times (1 - sigmoid(logits[t, e]))
+ * and 0 in rows without a token.
+ *   logits, tokenMask, cuSeqlens, scoring   as in the loss;   counts, weight   what it returned
+ *   gradLoss          fp32, one element, on the device, optional (1 without it)
+ *   grad              [rows, experts] logits' type; may be logits itself */
+ACL_FUNC_VISIBILITY aclnnStatus gmmB200ExpertBalanceGradGetWorkspaceSize(
+    const aclTensor *logits, const aclTensor *counts, const aclTensor *weight, const aclTensor *tokenMaskOptional,
+    const aclTensor *cuSeqlensOptional, const aclTensor *gradLossOptional, int64_t scoring, aclTensor *grad, uint64_t *workspaceSize,
+    aclOpExecutor **executor);
+ACL_FUNC_VISIBILITY aclnnStatus gmmB200ExpertBalanceGrad(void *workspace, uint64_t workspaceSize, aclOpExecutor *executor, aclrtStream stream);
 
 /* Buffers that other GPUs of the node can write into (CUDA IPC).  PeerAlloc/PeerFree own device memory of the calling
  * process; PeerExport fills a 64-byte handle that another process passes to PeerImport to obtain a device pointer to the

@@ -39,6 +39,8 @@ EXPORTED_SYMBOLS = [
     "gmmB200PeerAlloc", "gmmB200PeerFree", "gmmB200PeerExport", "gmmB200PeerImport", "gmmB200PeerRelease", "gmmB200EpDispatch", "gmmB200EpCount", "gmmB200EpRoute", "gmmB200EpInverseMap", "gmmB200EpCombine",
     "gmmB200AddRmsNormQuantGetWorkspaceSize", "gmmB200AddRmsNormQuant", "gmmB200RouteTopKGetWorkspaceSize", "gmmB200RouteTopK",
     "gmmB200AdapterAddGetWorkspaceSize", "gmmB200AdapterAdd",
+    "gmmB200QuantMatmulGetWorkspaceSize", "gmmB200QuantMatmul", "gmmB200SandwichNormQuantGetWorkspaceSize", "gmmB200SandwichNormQuant",
+    "gmmB200ExpertBalanceGetWorkspaceSize", "gmmB200ExpertBalance", "gmmB200ExpertBalanceGradGetWorkspaceSize", "gmmB200ExpertBalanceGrad",
 ]
 
 
@@ -58,6 +60,7 @@ class CallResult(C.Structure):
 
 OP_GMM, OP_SWIGLU_QUANT, OP_FINALIZE_ROUTING, OP_MOE_INIT_ROUTING = {"V4": 0, "V5": 1, "WeightNz": 2}, {"": 3, "WeightNZ": 4}, {"": 5, "V2": 6}, 7
 OP_ADD_RMS_NORM_QUANT, OP_ROUTE_TOP_K, OP_ADAPTER_ADD = 8, 9, 10
+OP_QUANT_MATMUL, OP_SANDWICH_NORM_QUANT, OP_EXPERT_BALANCE, OP_EXPERT_BALANCE_GRAD = 11, 12, 13, 14
 OP_POOLED, OP_PLAN_ONLY = 0x100, 0x200
 STAGE_PLAN, STAGE_OPTIONS, STAGE_PLANNED, STAGE_RUN = range(4)
 
@@ -128,6 +131,14 @@ def _load():
     L.gmmB200RouteTopK.argtypes = [p, u64, p, p]
     L.gmmB200AdapterAddGetWorkspaceSize.argtypes = [p] * 8 + [C.POINTER(u64), C.POINTER(p)]
     L.gmmB200AdapterAdd.argtypes = [p, u64, p, p]
+    L.gmmB200QuantMatmulGetWorkspaceSize.argtypes = [p] * 6 + [C.POINTER(u64), C.POINTER(p)]
+    L.gmmB200QuantMatmul.argtypes = [p, u64, p, p]
+    L.gmmB200SandwichNormQuantGetWorkspaceSize.argtypes = [p] * 6 + [i64] + [f32] * 4 + [p] * 4 + [C.POINTER(u64), C.POINTER(p)]
+    L.gmmB200SandwichNormQuant.argtypes = [p, u64, p, p]
+    L.gmmB200ExpertBalanceGetWorkspaceSize.argtypes = [p] * 4 + [i64, f32] + [p] * 3 + [C.POINTER(u64), C.POINTER(p)]
+    L.gmmB200ExpertBalance.argtypes = [p, u64, p, p]
+    L.gmmB200ExpertBalanceGradGetWorkspaceSize.argtypes = [p] * 6 + [i64, p, C.POINTER(u64), C.POINTER(p)]
+    L.gmmB200ExpertBalanceGrad.argtypes = [p, u64, p, p]
     L.gmmB200NoAllocScratchBytes.restype = u64
     L.gmmB200GroupedMatmulSwigluQuantNoAlloc.argtypes = [p, p, p, i32, p, p, i64, i64, i64, i64, i64, p, p, p]
     L.gmmB200NoAllocCheckStatus.argtypes = [p, C.POINTER(i32)]

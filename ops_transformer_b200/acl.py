@@ -436,17 +436,23 @@ def _float_bits(v: float) -> int:
     return _WORD.unpack(_FLOAT.pack(v))[0]
 
 
+_POOLED = frozenset((_lib.OP_ADAPTER_ADD, _lib.OP_QUANT_MATMUL, _lib.OP_EXPERT_BALANCE))
+
+
 def _block_call(op: int, name: str, workspace: Optional[torch.Tensor], stream, options: Optional[LaunchOptions], kinds: str,
                 *items) -> Optional[torch.Tensor]:
     """The call of an operator around the expert FFN, natively.  Its tensors all have to be on one GPU; elsewhere the arguments are
-    checked and the call is refused.  A call that needs no workspace (all but ``adapter_add`` and strided views) takes none.  Returns the
-    workspace that the call uses (None if none)."""
+    checked and the call is refused.  It runs on that GPU, whichever is the current one.  A call that needs no workspace (all but those of
+    ``_POOLED`` and strided views) takes none.  Returns the workspace that the call uses (None if none)."""
     module, call = _lib.native()
     x, buf = items[0], workspace
+    if x.is_cuda and x.get_device() != torch._C._cuda_getDevice():
+        with torch.cuda.device(x.device):
+            return _block_call(op, name, workspace, stream, options, kinds, *items)
     how = 0 if options is None else C.addressof(options)
     if workspace is not None and not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
-    pooled = workspace is None and op == _lib.OP_ADAPTER_ADD
+    pooled = workspace is None and op in _POOLED
     if not x.is_cuda:
         done = False
     else:
@@ -558,3 +564,121 @@ def adapter_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.T
     workspace = _block_call(_lib.OP_ADAPTER_ADD, "gmmB200AdapterAdd", workspace, stream, options, "tttttttt", base, x, x_scale, a, b, adapter_ids,
                             scaling, out)
     return (out, workspace if base.shape[0] else None) if return_workspace else out
+
+
+_FLOAT_LETTER = {torch.float32: "f", torch.float16: "h", torch.bfloat16: "w"}
+
+
+def quant_matmul(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, per_token_scale: Optional[torch.Tensor] = None, *,
+                 bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16, stream=None,
+                 workspace: Optional[torch.Tensor] = None, return_workspace: bool = False, options: Optional[LaunchOptions] = None):
+    """y [rows, n] = ((x @ weight) * scale) * per_token_scale + bias of int8 ``x`` [rows, k] and ``weight`` [k, n] (or the transposed view of
+    one stored [n, k]), with one scale a channel and, where given, one a token: the W8A8 product without groups.  ``scale`` and ``bias`` [n]
+    fp32 or 16-bit, ``per_token_scale`` fp32 [rows]; the result is ``out_dtype`` (bf16, fp16 or fp32) or ``out``.  With ``return_workspace``
+    (y, workspace), for ``check_status`` (no rows: None); ``options``: per-call ``LaunchOptions`` (wait bound).  gmmB200QuantMatmul
+    (include/gmm_b200.h)."""
+    if stream is not None:   # what a call returns belongs to the stream that writes it
+        with _on_stream(stream, x.device):
+            return quant_matmul(x, weight, scale, per_token_scale, bias=bias, out=out, out_dtype=out_dtype, workspace=workspace,
+                                return_workspace=return_workspace, options=options)
+    if out is None:
+        letter = _FLOAT_LETTER.get(out_dtype)
+        if letter and x.dim() == 2 and weight.dim() == 2:
+            out = _lib.native()[0].empty(x, letter, x.shape[0], weight.shape[1])
+        else:   # refused by the operator
+            out = x.new_empty((x.shape[0], weight.shape[-1]), dtype=out_dtype)
+    workspace = _block_call(_lib.OP_QUANT_MATMUL, "gmmB200QuantMatmul", workspace, None, options, "tttttt", x, weight, scale, per_token_scale, bias, out)
+    return (out, workspace if x.shape[0] else None) if return_workspace else out
+
+
+_GATE_ACT = {"none": 0, "sigmoid": 1, "tanh": 2}
+
+
+def sandwich_norm_quant(x: torch.Tensor, residual: torch.Tensor, gamma: Optional[torch.Tensor] = None, *,
+                        post_gamma: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, gate_act: str = "none",
+                        residual_scale: float = 1.0, block_scale: float = 1.0, smooth: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                        post_eps: Optional[float] = None, quant: bool = True, normed: bool = False, q: Optional[torch.Tensor] = None,
+                        scale: Optional[torch.Tensor] = None, residual_out: Optional[torch.Tensor] = None,
+                        normed_out: Optional[torch.Tensor] = None, stream=None, workspace: Optional[torch.Tensor] = None):
+    """(q int8 [rows, h], scale fp32 [rows], residual_out, normed_out): the way from a block's output ``x`` into the next block.  The residual
+    stream ``s = residual_scale * residual + block_scale * act(gate) * n`` with the block's output behind its norm, ``n = rms_norm(x) *
+    post_gamma`` (x itself without ``post_gamma``), and the norm of s with ``gamma`` in 8 bits with per-token scales (None without ``quant``)
+    and, with ``normed`` or a ``normed_out`` to write to, in residual's type.  ``x`` has residual's type or is fp32; ``gate`` is one for each
+    channel [h], each token [rows, 1] or each element, and goes through ``gate_act`` ("none", "sigmoid", "tanh"); ``smooth`` (fp32 [h])
+    multiplies what is quantised, not ``normed_out``; ``post_eps`` is ``eps`` unless given.  ``residual_out`` may be ``residual``.
+    gmmB200SandwichNormQuant (include/gmm_b200.h) has the formulas."""
+    if stream is not None:   # what a call returns belongs to the stream that writes it
+        with _on_stream(stream, x.device):
+            return sandwich_norm_quant(x, residual, gamma, post_gamma=post_gamma, gate=gate, gate_act=gate_act, residual_scale=residual_scale,
+                                       block_scale=block_scale, smooth=smooth, eps=eps, post_eps=post_eps, quant=quant, normed=normed, q=q,
+                                       scale=scale, residual_out=residual_out, normed_out=normed_out, workspace=workspace)
+    if gate_act not in _GATE_ACT:
+        raise ValueError(f"unknown gate_act {gate_act!r}")
+    empty = _lib.native()[0].empty
+    if quant or q is not None or scale is not None:
+        if q is None:
+            q = empty(x, "b")
+        if scale is None:
+            scale = empty(x, "f", x.shape[0])
+    if residual_out is None:
+        residual_out = empty(residual, "=")
+    if normed_out is None and normed:
+        normed_out = empty(residual, "=")
+    eps = _float_bits(eps)
+    _block_call(_lib.OP_SANDWICH_NORM_QUANT, "gmmB200SandwichNormQuant", workspace, None, None, "ttttttttttiiiii", x, residual, gamma, post_gamma,
+                gate, smooth, q, scale, residual_out, normed_out, _GATE_ACT[gate_act], _float_bits(residual_scale), _float_bits(block_scale), eps,
+                eps if post_eps is None else _float_bits(post_eps))
+    return q, scale, residual_out, normed_out
+
+
+def expert_balance(logits: torch.Tensor, ids: torch.Tensor, *, scoring: str = "softmax", coefficient: float = 1.0,
+                   token_mask: Optional[torch.Tensor] = None, cu_seqlens: Optional[torch.Tensor] = None, loss: Optional[torch.Tensor] = None,
+                   counts: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None, stream=None,
+                   workspace: Optional[torch.Tensor] = None):
+    """(loss, counts, weight): how the choices ``ids`` [rows, top_k] of ``route_top_k`` load the experts, and the loss that evens them out,
+    ``coefficient * experts / top_k * sum_e (share of the tokens' choices that are e) * (mean of the tokens' scores of e)``, the mean of it
+    over the sequences where ``cu_seqlens`` (int32 [sequences + 1]) names some.  ``loss`` is one fp32 number on the device, ``counts`` int64
+    [experts] or [sequences, experts], ``weight`` fp32 [sequences]: what ``expert_balance_grad`` takes.  ``scoring`` "softmax" or "sigmoid" (divided
+    by the row's sum); ``token_mask`` (bool or int8 [rows]): rows without a token; negative ids are not counted.  gmmB200ExpertBalance
+    (include/gmm_b200.h) has the formulas."""
+    if stream is not None:   # what a call returns belongs to the stream that writes it
+        with _on_stream(stream, logits.device):
+            return expert_balance(logits, ids, scoring=scoring, coefficient=coefficient, token_mask=token_mask, cu_seqlens=cu_seqlens, loss=loss,
+                                  counts=counts, weight=weight, workspace=workspace)
+    if scoring not in _SCORING:
+        raise ValueError(f"unknown scoring {scoring!r}")
+    empty = _lib.native()[0].empty
+    sequences = 1 if cu_seqlens is None else max(cu_seqlens.shape[0] - 1, 0)
+    if loss is None:
+        loss = empty(logits, "s")
+    if counts is None:
+        counts = empty(logits, "l", logits.shape[-1]) if cu_seqlens is None else empty(logits, "l", sequences, logits.shape[-1])
+    if weight is None:
+        weight = empty(logits, "f", sequences)
+    if token_mask is not None and token_mask.dtype == torch.bool:
+        token_mask = token_mask.view(torch.int8)
+    _block_call(_lib.OP_EXPERT_BALANCE, "gmmB200ExpertBalance", workspace, None, None, "tttttttii", logits, ids, token_mask, cu_seqlens, loss, counts,
+                weight, _SCORING[scoring], _float_bits(coefficient))
+    return loss, counts, weight
+
+
+def expert_balance_grad(logits: torch.Tensor, counts: torch.Tensor, weight: torch.Tensor, *, scoring: str = "softmax",
+                        token_mask: Optional[torch.Tensor] = None, cu_seqlens: Optional[torch.Tensor] = None,
+                        grad_loss: Optional[torch.Tensor] = None, grad: Optional[torch.Tensor] = None, stream=None,
+                        workspace: Optional[torch.Tensor] = None):
+    """The gradient of ``expert_balance``'s loss with respect to ``logits``, in their type, from the ``counts`` and ``weight`` that it returned and
+    the same ``scoring``, ``token_mask`` and ``cu_seqlens``; ``grad_loss`` (one fp32 number on the device) multiplies it.  ``logits.backward(grad)``
+    hands it on to a router that torch differentiates.  ``grad`` may be ``logits``.  gmmB200ExpertBalanceGrad (include/gmm_b200.h)."""
+    if stream is not None:   # what a call returns belongs to the stream that writes it
+        with _on_stream(stream, logits.device):
+            return expert_balance_grad(logits, counts, weight, scoring=scoring, token_mask=token_mask, cu_seqlens=cu_seqlens, grad_loss=grad_loss,
+                                       grad=grad, workspace=workspace)
+    if scoring not in _SCORING:
+        raise ValueError(f"unknown scoring {scoring!r}")
+    if grad is None:
+        grad = _lib.native()[0].empty(logits, "=")
+    if token_mask is not None and token_mask.dtype == torch.bool:
+        token_mask = token_mask.view(torch.int8)
+    _block_call(_lib.OP_EXPERT_BALANCE_GRAD, "gmmB200ExpertBalanceGrad", workspace, None, None, "ttttttti", logits, counts, weight,
+                token_mask, cu_seqlens, grad_loss, grad, _SCORING[scoring])
+    return grad

@@ -74,7 +74,8 @@ struct aclIntArray {
 };
 
 struct aclOpExecutor {
-    enum Kind { kNoop = 0, kGmm = 1, kInitRouting = 2, kNormQuant = 3, kRouteTopK = 4, kAdapterAdd = 5 } kind = kNoop;
+    enum Kind { kNoop = 0, kGmm = 1, kInitRouting = 2, kNormQuant = 3, kRouteTopK = 4, kAdapterAdd = 5,
+                kQuantMatmul = 6, kSandwichNorm = 7, kBalance = 8, kBalanceGrad = 9 } kind = kNoop;
     uint32_t magic = 0xac10e8ecu;
     bool consumed = false;
     const char *op_name = "";
@@ -84,6 +85,9 @@ struct aclOpExecutor {
     gmm::NormQuantProblem norm;
     gmm::RouteTopKProblem route;
     gmm::AdapterProblem adapter;
+    gmm::QuantMatmulProblem matmul;
+    gmm::SandwichNormProblem sandwich;
+    gmm::BalanceProblem balance;
     std::vector<gmm::StagedView> staged;   // non-contiguous views with a contiguous copy in the workspace tail
     size_t staged_bytes = 0;
 };

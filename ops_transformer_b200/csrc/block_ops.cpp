@@ -1,5 +1,5 @@
-// Host side of the operators around the expert FFN (include/gmm_b200.h): add_rms_norm_quant, route_top_k, adapter_add.  The first phase
-// checks and builds the executor; it is host only and never reads a tensor.  Nothing may leave an entry point as an exception.
+// Host side of the operators around the expert FFN (include/gmm_b200.h): add_rms_norm_quant, route_top_k, adapter_add, quant_matmul,
+// sandwich_norm_quant, expert_balance and its gradient.  The first phase checks and builds the executor; it is host only and never reads a tensor.  Nothing may leave an entry point as an exception.
 #include <cmath>
 #include <initializer_list>
 
@@ -10,6 +10,7 @@ namespace gmm {
 namespace {
 
 constexpr int64_t kMaxAxis = 65535;          // as for the inner axes of the grouped GEMM
+constexpr int64_t kMaxChannels = 1 << 24;    // of a dense product: a vocabulary
 constexpr int64_t kMaxRows = 0x7fffffffll / 2;
 
 // A tensor that may be absent, but not with elements and without an address, nor in a private format.
@@ -211,6 +212,250 @@ aclnnStatus adapter_phase1(const aclTensor *base, const aclTensor *x, const aclT
     return ne.hand_out(workspaceSize, executor);
 }
 
+// The weight of a dense product: rows along n, or along k in the transposed view of a weight stored [n, k]; any other view is copied.
+void bind_weight(aclOpExecutor *e, const aclTensor *w, QuantMatmulProblem *p)
+{
+    const int64_t k = w->dim(0), n = w->dim(1), sk = w->strides[0], sn = w->strides[1];
+    const bool by_n = (n == 1 || sn == 1) && (k == 1 || sk >= n), by_k = (k == 1 || sk == 1) && (n == 1 || sn >= k);
+    p->w_nk = !by_n && by_k;
+    p->ld_w = p->w_nk ? (n > 1 ? sn : k) : by_n && k > 1 ? sk : n;
+    bind_tensor(e, w, &p->w, false, by_n || by_k);
+}
+
+aclnnStatus matmul_phase1(const aclTensor *x, const aclTensor *weight, const aclTensor *scale, const aclTensor *perTokenScale,
+                          const aclTensor *bias, aclTensor *y, uint64_t *workspaceSize, aclOpExecutor **executor)
+{
+    REQUIRE_NOT_NULL(workspaceSize); REQUIRE_NOT_NULL(executor);
+    REQUIRE_NOT_NULL(x); REQUIRE_NOT_NULL(weight); REQUIRE_NOT_NULL(scale); REQUIRE_NOT_NULL(y);
+    REQUIRE_RANK(x, 2); REQUIRE_RANK(weight, 2);
+    const int64_t m = x->dim(0), k = x->dim(1), n = weight->dim(1);
+    GMM_REQUIRE(x->dtype == ACL_INT8 && weight->dtype == ACL_INT8, ACLNN_ERR_PARAM_INVALID, "x and weight dtype must be int8.");
+    GMM_REQUIRE(m >= 0 && m <= kMaxRows, ACLNN_ERR_PARAM_INVALID, "x must not have more than %lld rows.", (long long)kMaxRows);
+    GMM_REQUIRE(k >= 1 && k <= kMaxAxis, ACLNN_ERR_PARAM_INVALID, "k must be in [1, %lld], but is %lld.", (long long)kMaxAxis, (long long)k);
+    GMM_REQUIRE(n >= 1 && n <= kMaxChannels, ACLNN_ERR_PARAM_INVALID, "n must be in [1, %lld], but is %lld.", (long long)kMaxChannels, (long long)n);
+    REQUIRE_SHAPE2(weight, k, n);
+    REQUIRE_SHAPE1(scale, n);
+    GMM_REQUIRE(is_float(scale->dtype), ACLNN_ERR_PARAM_INVALID, "scale dtype must be float32, float16 or bfloat16.");
+    if (perTokenScale) {
+        REQUIRE_SHAPE1(perTokenScale, m);
+        GMM_REQUIRE(perTokenScale->dtype == ACL_FLOAT, ACLNN_ERR_PARAM_INVALID, "perTokenScale dtype must be float32.");
+    }
+    if (bias) {
+        REQUIRE_SHAPE1(bias, n);
+        GMM_REQUIRE(is_float(bias->dtype), ACLNN_ERR_PARAM_INVALID, "bias dtype must be float32, float16 or bfloat16.");
+    }
+    REQUIRE_SHAPE2(y, m, n);
+    GMM_REQUIRE(is_float(y->dtype), ACLNN_ERR_PARAM_INVALID, "y dtype must be float32, float16 or bfloat16.");
+    REQUIRE_USABLE(x, weight, scale, perTokenScale, bias, y);
+
+    NewExecutor ne("gmmB200QuantMatmul");
+    aclOpExecutor *e = ne.e;
+    GMM_REQUIRE(e != nullptr, ACLNN_ERR_INNER_CREATE_EXECUTOR, "cannot create executor.");
+    if (m > 0) {
+        QuantMatmulProblem &p = e->matmul;
+        bind_rows(e, x, &p.x, &p.ld_x, false);
+        bind_weight(e, weight, &p);
+        bind_tensor(e, scale, &p.scale, false);
+        bind_tensor(e, perTokenScale, &p.token_scale, false);
+        bind_tensor(e, bias, &p.bias, false);
+        bind_rows(e, y, &p.y, &p.ld_y, true);
+        p.scale_dtype = (int)scale->dtype; p.bias_dtype = bias ? (int)bias->dtype : kNone; p.y_dtype = (int)y->dtype;
+        p.m = m; p.k = k; p.n = n;
+        e->kind = aclOpExecutor::kQuantMatmul;
+        e->plan.ws_bytes = quant_matmul_workspace_bytes(p);
+    }
+    return ne.hand_out(workspaceSize, executor);
+}
+
+aclnnStatus sandwich_phase1(const aclTensor *x, const aclTensor *residual, const aclTensor *gamma, const aclTensor *postGamma,
+                            const aclTensor *gate, const aclTensor *smooth, int64_t gateAct, float residualScale, float blockScale, float eps,
+                            float postEps, aclTensor *q, aclTensor *scale, aclTensor *residualOut, aclTensor *normedOut,
+                            uint64_t *workspaceSize, aclOpExecutor **executor)
+{
+    REQUIRE_NOT_NULL(workspaceSize); REQUIRE_NOT_NULL(executor);
+    REQUIRE_NOT_NULL(x); REQUIRE_NOT_NULL(residual);
+    GMM_REQUIRE(q || residualOut || normedOut, ACLNN_ERR_PARAM_NULLPTR, "one of q, residualOut and normedOut is needed.");
+    GMM_REQUIRE((q == nullptr) == (scale == nullptr), ACLNN_ERR_PARAM_NULLPTR, "q and scale come together.");
+    GMM_REQUIRE(gamma || (!q && !normedOut), ACLNN_ERR_PARAM_NULLPTR, "q and normedOut need gamma.");
+    REQUIRE_RANK(residual, 2);
+    const int64_t rows = residual->dim(0), h = residual->dim(1);
+    const aclDataType type = residual->dtype;
+    GMM_REQUIRE(is_float(type), ACLNN_ERR_PARAM_INVALID, "residual dtype must be float32, float16 or bfloat16.");
+    GMM_REQUIRE(h >= 1 && h <= kMaxAxis, ACLNN_ERR_PARAM_INVALID, "residual's rows must have 1 to %lld elements, but have %lld.", (long long)kMaxAxis, (long long)h);
+    GMM_REQUIRE(rows >= 0 && rows <= kMaxRows, ACLNN_ERR_PARAM_INVALID, "residual must not have more than %lld rows.", (long long)kMaxRows);
+    REQUIRE_SHAPE2(x, rows, h);
+    GMM_REQUIRE(x->dtype == type || x->dtype == ACL_FLOAT, ACLNN_ERR_PARAM_INVALID, "x dtype must be residual's or float32.");
+    const aclDataType gamma_type = gamma ? gamma->dtype : postGamma ? postGamma->dtype : type;
+    GMM_REQUIRE(gamma_type == type || gamma_type == ACL_FLOAT, ACLNN_ERR_PARAM_INVALID, "gamma and postGamma dtype must be residual's or float32.");
+    for (const aclTensor *t : {gamma, postGamma})
+        GMM_REQUIRE(!t || (t->rank() == 1 && t->dim(0) == h && t->dtype == gamma_type), ACLNN_ERR_PARAM_INVALID,
+                    "gamma and postGamma must have shape [%lld] and the same dtype.", (long long)h);
+    if (smooth) {
+        REQUIRE_SHAPE1(smooth, h);
+        GMM_REQUIRE(smooth->dtype == ACL_FLOAT, ACLNN_ERR_PARAM_INVALID, "smooth dtype must be float32.");
+    }
+    if (gate) {
+        const bool shape = gate->rank() == 1 ? gate->dim(0) == h
+                           : gate->rank() == 2 && (gate->dim(0) == rows || gate->dim(0) == 1) && (gate->dim(1) == h || gate->dim(1) == 1);
+        GMM_REQUIRE(shape, ACLNN_ERR_PARAM_INVALID, "gate shape must be [%lld], or [%lld or 1, %lld or 1].", (long long)h, (long long)rows, (long long)h);
+        GMM_REQUIRE(gate->dtype == type, ACLNN_ERR_PARAM_INVALID, "gate dtype must be residual's.");
+    }
+    GMM_REQUIRE(gateAct >= kGateNone && gateAct <= kGateTanh, ACLNN_ERR_PARAM_INVALID, "gateAct must be 0 (none), 1 (sigmoid) or 2 (tanh).");
+    if (q) {
+        REQUIRE_SHAPE2(q, rows, h);
+        GMM_REQUIRE(q->dtype == ACL_INT8, ACLNN_ERR_PARAM_INVALID, "q dtype must be int8.");
+        REQUIRE_SHAPE1(scale, rows);
+        GMM_REQUIRE(scale->dtype == ACL_FLOAT, ACLNN_ERR_PARAM_INVALID, "scale dtype must be float32.");
+    }
+    for (const aclTensor *t : {residualOut, normedOut})
+        GMM_REQUIRE(!t || (t->rank() == 2 && t->dim(0) == rows && t->dim(1) == h && t->dtype == type), ACLNN_ERR_PARAM_INVALID,
+                    "residualOut and normedOut must have residual's shape and dtype.");
+    REQUIRE_USABLE(x, residual, gamma, postGamma, gate, smooth, q, scale, residualOut, normedOut);
+    GMM_REQUIRE(eps > 0.0f && std::isfinite(eps) && postEps > 0.0f && std::isfinite(postEps), ACLNN_ERR_PARAM_INVALID, "eps and postEps must be positive and finite.");
+    GMM_REQUIRE(std::isfinite(residualScale) && std::isfinite(blockScale), ACLNN_ERR_PARAM_INVALID, "residualScale and blockScale must be finite.");
+
+    NewExecutor ne("gmmB200SandwichNormQuant");
+    aclOpExecutor *e = ne.e;
+    GMM_REQUIRE(e != nullptr, ACLNN_ERR_INNER_CREATE_EXECUTOR, "cannot create executor.");
+    if (rows > 0) {
+        SandwichNormProblem &p = e->sandwich;
+        bind_rows(e, x, &p.x, &p.ld_x, false);
+        bind_rows(e, residual, &p.residual, &p.ld_residual, false);
+        bind_tensor(e, gamma, &p.gamma, false);
+        bind_tensor(e, postGamma, &p.post_gamma, false);
+        if (gate) {
+            const bool wide = gate->rank() == 1 || gate->dim(1) == h, tall = gate->rank() == 2 && gate->dim(0) == rows && rows > 1;
+            p.gate_step = wide && h > 1 ? 1 : 0;
+            if (gate->rank() == 2 && p.gate_step == 0) {   // a column: used where it is, however far its elements are apart
+                p.ld_gate = tall ? gate->strides[0] : 0;
+                bind_tensor(e, gate, &p.gate, false, true);
+            } else if (gate->rank() == 2) {
+                bind_rows(e, gate, &p.gate, &p.ld_gate, false);
+                if (!tall) p.ld_gate = 0;
+            } else {
+                bind_tensor(e, gate, &p.gate, false);
+            }
+        }
+        bind_tensor(e, smooth, &p.smooth, false);
+        bind_rows(e, q, &p.q, &p.ld_q, true);
+        bind_tensor(e, scale, &p.scale, true);
+        bind_rows(e, residualOut, &p.residual_out, &p.ld_residual_out, true);
+        bind_rows(e, normedOut, &p.normed_out, &p.ld_normed, true);
+        p.rows = rows; p.h = h;
+        p.dtype = (int)type; p.x_dtype = (int)x->dtype; p.gamma_dtype = (int)gamma_type;
+        p.gate_act = (int)gateAct;
+        p.residual_scale = residualScale; p.block_scale = blockScale; p.eps = eps; p.post_eps = postEps;
+        e->kind = aclOpExecutor::kSandwichNorm;
+    }
+    return ne.hand_out(workspaceSize, executor);
+}
+
+// What the balance loss and its gradient share.
+aclnnStatus check_balance(const aclTensor *logits, const aclTensor *tokenMask, const aclTensor *cuSeqlens, int64_t scoring, const aclTensor *counts,
+                          const aclTensor *weight, int64_t *sequences)
+{
+    REQUIRE_NOT_NULL(logits); REQUIRE_NOT_NULL(counts); REQUIRE_NOT_NULL(weight);
+    REQUIRE_RANK(logits, 2);
+    const int64_t rows = logits->dim(0), experts = logits->dim(1);
+    GMM_REQUIRE(is_float(logits->dtype), ACLNN_ERR_PARAM_INVALID, "logits dtype must be float32, float16 or bfloat16.");
+    GMM_REQUIRE(experts >= 1 && experts <= 1024, ACLNN_ERR_PARAM_INVALID, "logits must name 1 to 1024 experts, but name %lld.", (long long)experts);
+    GMM_REQUIRE(rows >= 0 && rows <= kMaxRows, ACLNN_ERR_PARAM_INVALID, "logits must not have more than %lld rows.", (long long)kMaxRows);
+    GMM_REQUIRE(scoring == kScoreSoftmax || scoring == kScoreSigmoid, ACLNN_ERR_PARAM_INVALID, "scoring must be 0 (softmax) or 1 (sigmoid).");
+    if (tokenMask) {
+        REQUIRE_SHAPE1(tokenMask, rows);
+        GMM_REQUIRE(tokenMask->dtype == ACL_INT8 || tokenMask->dtype == ACL_BOOL, ACLNN_ERR_PARAM_INVALID, "tokenMask dtype must be int8 or bool.");
+    }
+    *sequences = 1;
+    if (cuSeqlens) {
+        REQUIRE_RANK(cuSeqlens, 1);
+        GMM_REQUIRE(cuSeqlens->dtype == ACL_INT32, ACLNN_ERR_PARAM_INVALID, "cuSeqlens dtype must be int32.");
+        *sequences = cuSeqlens->dim(0) - 1;
+        GMM_REQUIRE(*sequences >= 1 && *sequences <= kMaxAxis, ACLNN_ERR_PARAM_INVALID, "cuSeqlens must name 1 to %lld sequences, but names %lld.",
+                    (long long)kMaxAxis, (long long)*sequences);
+        REQUIRE_SHAPE2(counts, *sequences, experts);
+    } else {
+        REQUIRE_SHAPE1(counts, experts);
+    }
+    GMM_REQUIRE(counts->dtype == ACL_INT64, ACLNN_ERR_PARAM_INVALID, "counts dtype must be int64.");
+    REQUIRE_SHAPE1(weight, *sequences);
+    GMM_REQUIRE(weight->dtype == ACL_FLOAT, ACLNN_ERR_PARAM_INVALID, "weight dtype must be float32.");
+    return ACLNN_SUCCESS;
+}
+
+void bind_balance(aclOpExecutor *e, const aclTensor *logits, const aclTensor *tokenMask, const aclTensor *cuSeqlens, int64_t scoring, int64_t sequences)
+{
+    BalanceProblem &p = e->balance;
+    bind_rows(e, logits, &p.logits, &p.ld, false);
+    p.dtype = (int)logits->dtype;
+    bind_tensor(e, tokenMask, &p.token_mask, false);
+    bind_tensor(e, cuSeqlens, &p.cu_seqlens, false);
+    p.rows = logits->dim(0); p.experts = (int)logits->dim(1); p.sequences = sequences;
+    p.scoring = (int)scoring;
+}
+
+aclnnStatus balance_phase1(const aclTensor *logits, const aclTensor *ids, const aclTensor *tokenMask, const aclTensor *cuSeqlens, int64_t scoring,
+                           float coefficient, aclTensor *loss, aclTensor *counts, aclTensor *weight, uint64_t *workspaceSize,
+                           aclOpExecutor **executor)
+{
+    REQUIRE_NOT_NULL(workspaceSize); REQUIRE_NOT_NULL(executor);
+    REQUIRE_NOT_NULL(ids); REQUIRE_NOT_NULL(loss);
+    int64_t sequences = 1;
+    const aclnnStatus rc = check_balance(logits, tokenMask, cuSeqlens, scoring, counts, weight, &sequences);
+    if (rc != ACLNN_SUCCESS) return rc;
+    REQUIRE_RANK(ids, 2);
+    GMM_REQUIRE(ids->dim(0) == logits->dim(0) && ids->dim(1) >= 1 && ids->dim(1) <= 1024, ACLNN_ERR_PARAM_INVALID,
+                "ids shape must be [%lld, 1 to 1024].", (long long)logits->dim(0));
+    GMM_REQUIRE(ids->dtype == ACL_INT32 || ids->dtype == ACL_INT64, ACLNN_ERR_PARAM_INVALID, "ids dtype must be int32 or int64.");
+    GMM_REQUIRE(loss->numel() == 1 && loss->dtype == ACL_FLOAT, ACLNN_ERR_PARAM_INVALID, "loss must be one float32 element.");
+    GMM_REQUIRE(std::isfinite(coefficient), ACLNN_ERR_PARAM_INVALID, "coefficient must be finite.");
+    REQUIRE_USABLE(logits, ids, tokenMask, cuSeqlens, loss, counts, weight);
+
+    NewExecutor ne("gmmB200ExpertBalance");
+    aclOpExecutor *e = ne.e;
+    GMM_REQUIRE(e != nullptr, ACLNN_ERR_INNER_CREATE_EXECUTOR, "cannot create executor.");
+    BalanceProblem &p = e->balance;
+    bind_balance(e, logits, tokenMask, cuSeqlens, scoring, sequences);
+    bind_tensor(e, ids, &p.ids, false);
+    bind_tensor(e, loss, &p.loss, true);
+    bind_tensor(e, counts, &p.counts, true);
+    bind_tensor(e, weight, &p.weight, true);
+    p.ids_i64 = ids->dtype == ACL_INT64;
+    p.top_k = (int)ids->dim(1);
+    p.coefficient = coefficient;
+    e->kind = aclOpExecutor::kBalance;   // without rows, too: the loss is 0 then
+    e->plan.ws_bytes = balance_workspace_bytes(p);
+    return ne.hand_out(workspaceSize, executor);
+}
+
+aclnnStatus balance_grad_phase1(const aclTensor *logits, const aclTensor *counts, const aclTensor *weight, const aclTensor *tokenMask,
+                                const aclTensor *cuSeqlens, const aclTensor *gradLoss, int64_t scoring, aclTensor *grad, uint64_t *workspaceSize,
+                                aclOpExecutor **executor)
+{
+    REQUIRE_NOT_NULL(workspaceSize); REQUIRE_NOT_NULL(executor);
+    REQUIRE_NOT_NULL(grad);
+    int64_t sequences = 1;
+    const aclnnStatus rc = check_balance(logits, tokenMask, cuSeqlens, scoring, counts, weight, &sequences);
+    if (rc != ACLNN_SUCCESS) return rc;
+    GMM_REQUIRE(!gradLoss || (gradLoss->numel() == 1 && gradLoss->dtype == ACL_FLOAT), ACLNN_ERR_PARAM_INVALID, "gradLoss must be one float32 element.");
+    REQUIRE_SHAPE2(grad, logits->dim(0), logits->dim(1));
+    GMM_REQUIRE(grad->dtype == logits->dtype, ACLNN_ERR_PARAM_INVALID, "grad dtype must be logits'.");
+    REQUIRE_USABLE(logits, counts, weight, tokenMask, cuSeqlens, gradLoss, grad);
+
+    NewExecutor ne("gmmB200ExpertBalanceGrad");
+    aclOpExecutor *e = ne.e;
+    GMM_REQUIRE(e != nullptr, ACLNN_ERR_INNER_CREATE_EXECUTOR, "cannot create executor.");
+    if (logits->dim(0) > 0) {
+        BalanceProblem &p = e->balance;
+        bind_balance(e, logits, tokenMask, cuSeqlens, scoring, sequences);
+        bind_tensor(e, counts, &p.counts, false);
+        bind_tensor(e, weight, &p.weight, false);
+        bind_tensor(e, gradLoss, &p.grad_loss, false);
+        bind_rows(e, grad, &p.grad, &p.ld_grad, true);
+        e->kind = aclOpExecutor::kBalanceGrad;
+    }
+    return ne.hand_out(workspaceSize, executor);
+}
+
 // A first phase whose allocations may fail.
 template <typename Fn>
 aclnnStatus guarded(const char *name, Fn fn)
@@ -273,6 +518,65 @@ aclnnStatus gmmB200AdapterAddGetWorkspaceSize(const aclTensor *base, const aclTe
 aclnnStatus gmmB200AdapterAdd(void *workspace, uint64_t workspaceSize, aclOpExecutor *executor, aclrtStream stream)
 {
     return run_executor("gmmB200AdapterAdd", workspace, workspaceSize, executor, stream);
+}
+
+aclnnStatus gmmB200QuantMatmulGetWorkspaceSize(const aclTensor *x, const aclTensor *weight, const aclTensor *scale,
+                                               const aclTensor *perTokenScaleOptional, const aclTensor *biasOptional, aclTensor *y,
+                                               uint64_t *workspaceSize, aclOpExecutor **executor)
+{
+    return guarded("gmmB200QuantMatmul", [&] { return matmul_phase1(x, weight, scale, perTokenScaleOptional, biasOptional, y, workspaceSize, executor); });
+}
+
+aclnnStatus gmmB200QuantMatmul(void *workspace, uint64_t workspaceSize, aclOpExecutor *executor, aclrtStream stream)
+{
+    return run_executor("gmmB200QuantMatmul", workspace, workspaceSize, executor, stream);
+}
+
+aclnnStatus gmmB200SandwichNormQuantGetWorkspaceSize(const aclTensor *x, const aclTensor *residual, const aclTensor *gammaOptional,
+                                                     const aclTensor *postGammaOptional, const aclTensor *gateOptional,
+                                                     const aclTensor *smoothOptional, int64_t gateAct, float residualScale, float blockScale,
+                                                     float eps, float postEps, aclTensor *qOptional, aclTensor *scaleOptional,
+                                                     aclTensor *residualOutOptional, aclTensor *normedOutOptional, uint64_t *workspaceSize,
+                                                     aclOpExecutor **executor)
+{
+    return guarded("gmmB200SandwichNormQuant", [&] {
+        return sandwich_phase1(x, residual, gammaOptional, postGammaOptional, gateOptional, smoothOptional, gateAct, residualScale, blockScale, eps,
+                               postEps, qOptional, scaleOptional, residualOutOptional, normedOutOptional, workspaceSize, executor);
+    });
+}
+
+aclnnStatus gmmB200SandwichNormQuant(void *workspace, uint64_t workspaceSize, aclOpExecutor *executor, aclrtStream stream)
+{
+    return run_executor("gmmB200SandwichNormQuant", workspace, workspaceSize, executor, stream);
+}
+
+aclnnStatus gmmB200ExpertBalanceGetWorkspaceSize(const aclTensor *logits, const aclTensor *ids, const aclTensor *tokenMaskOptional,
+                                                 const aclTensor *cuSeqlensOptional, int64_t scoring, float coefficient, aclTensor *loss,
+                                                 aclTensor *counts, aclTensor *weight, uint64_t *workspaceSize, aclOpExecutor **executor)
+{
+    return guarded("gmmB200ExpertBalance", [&] {
+        return balance_phase1(logits, ids, tokenMaskOptional, cuSeqlensOptional, scoring, coefficient, loss, counts, weight, workspaceSize, executor);
+    });
+}
+
+aclnnStatus gmmB200ExpertBalance(void *workspace, uint64_t workspaceSize, aclOpExecutor *executor, aclrtStream stream)
+{
+    return run_executor("gmmB200ExpertBalance", workspace, workspaceSize, executor, stream);
+}
+
+aclnnStatus gmmB200ExpertBalanceGradGetWorkspaceSize(const aclTensor *logits, const aclTensor *counts, const aclTensor *weight,
+                                                     const aclTensor *tokenMaskOptional, const aclTensor *cuSeqlensOptional,
+                                                     const aclTensor *gradLossOptional, int64_t scoring, aclTensor *grad, uint64_t *workspaceSize,
+                                                     aclOpExecutor **executor)
+{
+    return guarded("gmmB200ExpertBalanceGrad", [&] {
+        return balance_grad_phase1(logits, counts, weight, tokenMaskOptional, cuSeqlensOptional, gradLossOptional, scoring, grad, workspaceSize, executor);
+    });
+}
+
+aclnnStatus gmmB200ExpertBalanceGrad(void *workspace, uint64_t workspaceSize, aclOpExecutor *executor, aclrtStream stream)
+{
+    return run_executor("gmmB200ExpertBalanceGrad", workspace, workspaceSize, executor, stream);
 }
 
 }  // extern "C"

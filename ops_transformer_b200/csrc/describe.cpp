@@ -237,7 +237,8 @@ PyObject *launch(PyObject *, PyObject *const *args, Py_ssize_t nargs)
 }
 
 // empty(tensor, letter of the type, size, ...): an uninitialised contiguous tensor on the tensor's device.  'b' int8, 'i' int32,
-// 'l' int64, 'f' float32, '=' the tensor's own type; without sizes it has the tensor's.
+// 'l' int64, 'f' float32, 'h' float16, 'w' bfloat16, '=' the tensor's own type; without sizes it has the tensor's.  's': one float32
+// number, a tensor without dimensions.
 PyObject *empty(PyObject *, PyObject *const *args, Py_ssize_t nargs)
 {
     if (nargs < 2 || nargs > 4 || !THPVariable_Check(args[0])) {
@@ -259,8 +260,10 @@ PyObject *empty(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     }
     HANDLE_TH_ERRORS   // what torch raises itself, OutOfMemoryError for instance
         const at::Tensor &t = THPVariable_Unpack(args[0]);
-        const at::ScalarType dtype = *type == 'b' ? at::kChar : *type == 'i' ? at::kInt : *type == 'l' ? at::kLong : *type == 'f' ? at::kFloat : t.scalar_type();
+        const at::ScalarType dtype = *type == 'b' ? at::kChar : *type == 'i' ? at::kInt : *type == 'l' ? at::kLong : *type == 'f' || *type == 's' ? at::kFloat
+                                       : *type == 'h' ? at::kHalf : *type == 'w' ? at::kBFloat16 : t.scalar_type();
         const auto options = at::TensorOptions().dtype(dtype).device(t.device());
+        if (*type == 's') return THPVariable_Wrap(at::empty({}, options));
         return THPVariable_Wrap(nargs == 2 ? at::empty(t.sizes(), options) : at::empty(at::IntArrayRef(sizes, (size_t)nargs - 2), options));
     END_HANDLE_TH_ERRORS
 }

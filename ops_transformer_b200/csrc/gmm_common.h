@@ -164,6 +164,70 @@ struct AdapterProblem {
 size_t adapter_workspace_bytes(const AdapterProblem &p);
 cudaError_t adapter_launch(const AdapterProblem &p, void *workspace, size_t workspace_bytes, cudaStream_t stream);
 
+// quant_matmul (quant_matmul.cu): y = ((x w) * scale) * per_token_scale + bias.  Strides are in elements.
+struct QuantMatmulProblem {
+    const int8_t *x = nullptr;              // [m, k]
+    const int8_t *w = nullptr;              // [k, n], or [n, k] with w_nk
+    bool w_nk = false;
+    int64_t ld_x = 0, ld_w = 0, ld_y = 0;
+    const void *scale = nullptr;            // [n] f32 / f16 / bf16
+    int scale_dtype = kF32;
+    const float *token_scale = nullptr;     // [m], optional
+    const void *bias = nullptr;             // [n] f32 / f16 / bf16, optional
+    int bias_dtype = kNone;
+    void *y = nullptr;                      // [m, n] f32 / f16 / bf16
+    int y_dtype = kBF16;
+    int64_t m = 0, k = 0, n = 0;
+    LaunchOptions opt;
+};
+size_t quant_matmul_workspace_bytes(const QuantMatmulProblem &p);
+cudaError_t quant_matmul_launch(const QuantMatmulProblem &p, void *workspace, size_t workspace_bytes, cudaStream_t stream);
+
+// sandwich_norm_quant (sandwich_norm.cu).  Row strides are in elements; a missing tensor is null.
+enum : int { kGateNone = 0, kGateSigmoid = 1, kGateTanh = 2 };
+struct SandwichNormProblem {
+    const void *x = nullptr;                // [rows, h] x_dtype
+    const void *residual = nullptr;         // [rows, h] dtype
+    const void *gamma = nullptr, *post_gamma = nullptr;   // [h] gamma_dtype (dtype or fp32), both optional
+    const void *gate = nullptr;             // dtype, optional: element (row, column) at row * ld_gate + column * gate_step
+    const float *smooth = nullptr;          // [h], optional
+    int8_t *q = nullptr;                    // [rows, h], with scale
+    float *scale = nullptr;                 // [rows]
+    void *residual_out = nullptr, *normed_out = nullptr;   // [rows, h] dtype
+    int64_t rows = 0, h = 0;
+    int64_t ld_x = 0, ld_residual = 0, ld_gate = 0, ld_q = 0, ld_residual_out = 0, ld_normed = 0;
+    int gate_step = 0;                      // 1, or 0 for a gate that a row's elements share
+    int dtype = kBF16, x_dtype = kF32, gamma_dtype = kBF16;
+    int gate_act = kGateNone;
+    float residual_scale = 1.0f, block_scale = 1.0f, eps = 0.0f, post_eps = 0.0f;
+};
+cudaError_t sandwich_norm_launch(const SandwichNormProblem &p, cudaStream_t stream);
+
+// expert_balance and its gradient (expert_balance.cu).
+struct BalanceProblem {
+    const void *logits = nullptr;           // [rows, experts] f32 / f16 / bf16
+    int dtype = kF32;
+    int64_t ld = 0;
+    const int8_t *token_mask = nullptr;     // [rows], optional
+    const int *cu_seqlens = nullptr;        // [sequences + 1], optional: one sequence of all rows
+    int64_t rows = 0, sequences = 1;
+    int experts = 0, scoring = kScoreSoftmax;
+    // the loss
+    const void *ids = nullptr;              // [rows, top_k] int32 or int64
+    bool ids_i64 = false;
+    int top_k = 0;
+    float coefficient = 1.0f;
+    float *loss = nullptr, *weight = nullptr;   // [1], [sequences]
+    int64_t *counts = nullptr;              // [sequences, experts]
+    // the gradient, which reads counts and weight
+    const float *grad_loss = nullptr;       // [1], optional
+    void *grad = nullptr;                   // [rows, experts] dtype
+    int64_t ld_grad = 0;
+};
+size_t balance_workspace_bytes(const BalanceProblem &p);
+cudaError_t balance_launch(const BalanceProblem &p, void *workspace, size_t workspace_bytes, cudaStream_t stream);
+cudaError_t balance_grad_launch(const BalanceProblem &p, cudaStream_t stream);
+
 // A non-contiguous tensor view whose contiguous copy lives in the workspace (view_copy.cu).
 struct StagedView {
     std::vector<int64_t> dims, strides;  // strides in elements

@@ -112,6 +112,10 @@ aclnnStatus run_executor(const char *op_name, void *workspace, uint64_t workspac
                 case aclOpExecutor::kNormQuant: ce = norm_quant_launch(executor->norm, cs); break;
                 case aclOpExecutor::kRouteTopK: ce = route_top_k_launch(executor->route, cs); break;
                 case aclOpExecutor::kAdapterAdd: executor->adapter.opt = executor->problem.opt; ce = adapter_launch(executor->adapter, workspace, executor->plan.ws_bytes, cs); break;
+                case aclOpExecutor::kQuantMatmul: executor->matmul.opt = executor->problem.opt; ce = quant_matmul_launch(executor->matmul, workspace, executor->plan.ws_bytes, cs); break;
+                case aclOpExecutor::kSandwichNorm: ce = sandwich_norm_launch(executor->sandwich, cs); break;
+                case aclOpExecutor::kBalance: ce = balance_launch(executor->balance, workspace, executor->plan.ws_bytes, cs); break;
+                case aclOpExecutor::kBalanceGrad: ce = balance_grad_launch(executor->balance, cs); break;
                 default: ce = launch(executor->problem, executor->plan, workspace, executor->plan.ws_bytes, cs);
             }
             for (StagedView &v : executor->staged)
@@ -1219,6 +1223,44 @@ aclnnStatus plan_packed(int32_t op, WordReader &r, uint64_t *size, aclOpExecutor
             *run = gmmB200AdapterAdd;
             return gmmB200AdapterAddGetWorkspaceSize(base.get(), x.get(), x_scale.get(), a.get(), b.get(), ids.get(), scaling.get(), out.out(),
                                                      size, ex);
+        }
+        case GMM_B200_OP_QUANT_MATMUL: {
+            PackedTensor x, w, scale, token_scale, bias, y;
+            for (PackedTensor *t : {&x, &w, &scale, &token_scale, &bias, &y}) t->read(r);
+            if (!r.all_read()) return malformed();
+            *run = gmmB200QuantMatmul;
+            return gmmB200QuantMatmulGetWorkspaceSize(x.get(), w.get(), scale.get(), token_scale.get(), bias.get(), y.out(), size, ex);
+        }
+        case GMM_B200_OP_SANDWICH_NORM_QUANT: {
+            PackedTensor x, residual, gamma, post_gamma, gate, smooth, q, scale, residual_out, normed;
+            for (PackedTensor *t : {&x, &residual, &gamma, &post_gamma, &gate, &smooth, &q, &scale, &residual_out, &normed}) t->read(r);
+            const int64_t act = r.next();
+            const float residual_scale = float_of_bits(r.next()), block_scale = float_of_bits(r.next()), eps = float_of_bits(r.next()),
+                        post_eps = float_of_bits(r.next());
+            if (!r.all_read()) return malformed();
+            *run = gmmB200SandwichNormQuant;
+            return gmmB200SandwichNormQuantGetWorkspaceSize(x.get(), residual.get(), gamma.get(), post_gamma.get(), gate.get(), smooth.get(),
+                                                            act, residual_scale, block_scale, eps, post_eps, q.out(), scale.out(),
+                                                            residual_out.out(), normed.out(), size, ex);
+        }
+        case GMM_B200_OP_EXPERT_BALANCE: {
+            PackedTensor logits, ids, mask, cu, loss, counts, weight;
+            for (PackedTensor *t : {&logits, &ids, &mask, &cu, &loss, &counts, &weight}) t->read(r);
+            const int64_t scoring = r.next();
+            const float coefficient = float_of_bits(r.next());
+            if (!r.all_read()) return malformed();
+            *run = gmmB200ExpertBalance;
+            return gmmB200ExpertBalanceGetWorkspaceSize(logits.get(), ids.get(), mask.get(), cu.get(), scoring, coefficient, loss.out(),
+                                                        counts.out(), weight.out(), size, ex);
+        }
+        case GMM_B200_OP_EXPERT_BALANCE_GRAD: {
+            PackedTensor logits, counts, weight, mask, cu, grad_loss, grad;
+            for (PackedTensor *t : {&logits, &counts, &weight, &mask, &cu, &grad_loss, &grad}) t->read(r);
+            const int64_t scoring = r.next();
+            if (!r.all_read()) return malformed();
+            *run = gmmB200ExpertBalanceGrad;
+            return gmmB200ExpertBalanceGradGetWorkspaceSize(logits.get(), counts.get(), weight.get(), mask.get(), cu.get(), grad_loss.get(),
+                                                            scoring, grad.out(), size, ex);
         }
         default: return fail(ACLNN_ERR_PARAM_INVALID, "gmmB200Call: unknown operator %d.", op);
     }

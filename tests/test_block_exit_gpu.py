@@ -1,0 +1,653 @@
+"""quant_matmul, sandwich_norm_quant, expert_balance and its gradient on the GPU against plain implementations in 64 bits (and in fp32 where a
+result has to be bit-identical), at the sizes, strides, masks and special values where they can go wrong.
+
+Tolerances come from the operators' arithmetic: u = 2^-24 is half a unit in the last place of fp32, and a result in a 16-bit type may
+be off by half of one of its own units."""
+import math
+
+import pytest
+import torch
+
+import ops_transformer_b200 as ops
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+U32 = 2.0 ** -24
+HALF_ULP = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}   # of 24, 11 and 8 significant bits
+TINY = {torch.float32: 1e-38, torch.float16: 2.0 ** -25, torch.bfloat16: 1e-38}   # half a subnormal step, or nothing
+BF16, F16, F32, I8, I32, I64 = torch.bfloat16, torch.float16, torch.float32, torch.int8, torch.int32, torch.int64
+
+
+def gen(seed):
+    return torch.Generator(DEV).manual_seed(seed)
+
+
+def randn(shape, seed, dtype=F32, scale=1.0):
+    return (torch.randn(shape, device=DEV, generator=gen(seed)) * scale).to(dtype)
+
+
+def rand(shape, seed):
+    return torch.rand(shape, device=DEV, generator=gen(seed))
+
+
+def int8(shape, seed, lo=-128, hi=128):
+    return torch.randint(lo, hi, shape, device=DEV, generator=gen(seed)).to(I8)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# quant_matmul: every step is an exact sum or one rounding, so results are bit-identical to the same steps in torch
+# ---------------------------------------------------------------------------------------------------------------------
+
+def plain_matmul(x, w, scale, token, bias, dtype):
+    acc = x.double() @ w.double()   # exact: below 2^53
+    y = acc.float() * scale.float()
+    if token is not None:
+        y = y * token[:, None]
+    if bias is not None:
+        y = y + bias.float()
+    return y.to(dtype)
+
+
+def check_matmul(m, k, n, nk=False, dtype=BF16, bias=None, scale_dtype=F32, token=True, seed=0):
+    x = int8((m, k), seed + 1)
+    w = int8((n, k), seed + 2).t() if nk else int8((k, n), seed + 2)
+    scale = ((rand((n,), seed + 3) + 0.5) / 1024).to(scale_dtype)
+    per_token = (rand((m,), seed + 4) + 0.5) / 16 if token else None
+    b = randn((n,), seed + 5, bias) if bias else None
+    got = ops.quant_matmul(x, w, scale, per_token, bias=b, out_dtype=dtype)
+    assert got.shape == (m, n) and got.dtype == dtype
+    assert torch.equal(got, plain_matmul(x, w, scale, per_token, b, dtype))
+
+
+MATMUL_SIZES = [(1, 1, 1), (1, 16, 16), (1, 7168, 128), (2, 17, 33), (3, 128, 129), (5, 127, 255), (16, 768, 2048), (16, 2048, 160), (31, 1000, 1008),
+                (33, 4096, 384), (64, 512, 1536), (65, 2048, 2064), (100, 144, 7000), (128, 640, 129), (129, 1423, 300), (200, 16, 2000), (257, 1424, 2976),
+                (611, 1423, 2977), (700, 300, 512), (1025, 2048, 1040), (2000, 1000, 1999)]
+
+
+@pytest.mark.parametrize("nk", [False, True])
+@pytest.mark.parametrize("m,k,n", MATMUL_SIZES)
+def test_matmul_sizes(m, k, n, nk):
+    check_matmul(m, k, n, nk)
+    check_matmul(m, k, n, nk, dtype=F32, bias=F32, token=False, seed=10)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("bias", [None, F32, BF16, F16])
+@pytest.mark.parametrize("m,k,n", [(16, 1024, 1024), (7, 100, 77), (1500, 1536, 4096)])
+def test_matmul_types(m, k, n, bias, dtype):
+    for scale_dtype in (F32, BF16, F16):
+        check_matmul(m, k, n, nk=bias is None, dtype=dtype, bias=bias, scale_dtype=scale_dtype)
+
+
+def test_matmul_large():
+    check_matmul(4096, 2048, 4096)
+    check_matmul(1, 2048, 129280, nk=True, dtype=F32)     # a head
+    check_matmul(70, 512, 100003, dtype=F32)
+    check_matmul(70000, 64, 272, nk=True)
+    check_matmul(3, 65535, 48)
+
+
+def test_matmul_extreme_values():
+    """The largest sums that 65535 products make stay in int32; scales that leave the result's type."""
+    m, k, n = 4, 65535, 64
+    x, w = torch.full((m, k), -128, device=DEV, dtype=I8), torch.full((k, n), -128, device=DEV, dtype=I8)
+    one = torch.ones(n, device=DEV)
+    assert (ops.quant_matmul(x, w, one, out_dtype=F32) == 65535 * 16384).all()
+    w[:, 1::2] = 127
+    got = ops.quant_matmul(x, w, one, out_dtype=F32)
+    assert (got[:, ::2] == 65535.0 * 16384).all() and (got[:, 1::2] == -float(torch.tensor(65535 * 16256).float())).all()
+    scale = one.clone()
+    scale[:4] = torch.tensor([math.inf, math.nan, 0.0, 1e38], device=DEV)
+    got = ops.quant_matmul(x, w, scale, out_dtype=F16)
+    assert torch.equal(got, plain_matmul(x, w, scale, None, None, F16)) or (got[:, 0].isinf().all() and got[:, 1].isnan().all() and (got[:, 2] == 0).all() and got[:, 3].isinf().all())
+    token = torch.tensor([1.0, math.inf, math.nan, 0.0], device=DEV)
+    got = ops.quant_matmul(x, w, one, token, out_dtype=F32)
+    assert got[1].isinf().all() and got[2].isnan().all() and (got[3] == 0).all()
+
+
+def test_matmul_equals_one_group():
+    for m, k, n in ((1, 512, 256), (40, 2048, 4096), (300, 1024, 512)):
+        x, w = int8((m, k), 1), int8((k, n), 2)
+        scale, token = rand((n,), 3) / 256, rand((m,), 4)
+        for dtype in (BF16, F16):
+            one = ops.grouped_matmul_v4(x, w[None], scale[None], token, torch.full((1,), m, device=DEV, dtype=I64), out_dtype=dtype)
+            assert torch.equal(ops.quant_matmul(x, w, scale, token, out_dtype=dtype), one)
+
+
+@pytest.mark.parametrize("m", [5, 150, 1300])
+def test_matmul_strided_operands(m):
+    k, n = 400, 528
+    scale, token, bias = rand((n,), 1), rand((m,), 2), randn((n,), 3)
+    dense_x, dense_w = int8((m, k), 4), int8((k, n), 5)
+    want = plain_matmul(dense_x, dense_w, scale, token, bias, BF16)
+
+    def padded(t, left, right):   # the same values inside wider rows
+        wide = torch.full((t.shape[0], left + t.shape[1] + right), 77, device=DEV, dtype=t.dtype)
+        wide[:, left:left + t.shape[1]] = t
+        return wide[:, left:left + t.shape[1]]
+
+    xs = [padded(dense_x, 16, 32), padded(dense_x, 3, 0), padded(dense_x, 0, 5), dense_x.t().contiguous().t(), dense_x.repeat_interleave(2, 1)[:, ::2]]
+    ws = [padded(dense_w, 16, 32), padded(dense_w, 1, 2), dense_w.t().contiguous().t(), padded(dense_w.t(), 32, 16).t(), padded(dense_w.t(), 5, 2).t(),
+          dense_w.repeat_interleave(2, 1)[:, ::2]]
+    for x in xs:
+        assert torch.equal(ops.quant_matmul(x, dense_w, scale, token, bias=bias), want)
+    for w in ws:
+        assert torch.equal(ops.quant_matmul(dense_x, w, scale, token, bias=bias), want)
+    assert torch.equal(ops.quant_matmul(xs[1], ws[4], scale, token, bias=bias), want)
+    row = torch.ones(1, k, device=DEV, dtype=I8).expand(m, k)
+    assert torch.equal(ops.quant_matmul(row, dense_w, scale, token), plain_matmul(row, dense_w, scale, token, None, BF16))
+    # results into wider rows, on and off the boundaries of packs, and into columns apart; what lies between stays as it was
+    for left, right in ((8, 8), (1, 2), (0, 3)):
+        wide = torch.full((m, left + n + right), 5.0, device=DEV, dtype=BF16)
+        ops.quant_matmul(dense_x, dense_w, scale, token, bias=bias, out=wide[:, left:left + n])
+        assert torch.equal(wide[:, left:left + n], want) and (wide[:, :left] == 5).all() and (wide[:, left + n:] == 5).all()
+    apart = torch.full((m, 2 * n), 5.0, device=DEV, dtype=BF16)
+    ops.quant_matmul(dense_x, dense_w, scale, token, bias=bias, out=apart[:, ::2])
+    assert torch.equal(apart[:, ::2], want) and (apart[:, 1::2] == 5).all()
+
+
+def test_matmul_no_rows_and_rows_behind():
+    assert ops.quant_matmul(int8((0, 64), 1), int8((64, 48), 2), rand((48,), 3)).shape == (0, 48)
+    y, ws = ops.quant_matmul(int8((0, 64), 1), int8((64, 48), 2), rand((48,), 3), return_workspace=True)
+    assert ws is None
+    room = torch.full((70, 256), 9.0, device=DEV, dtype=BF16)
+    ops.quant_matmul(int8((33, 128), 1), int8((128, 256), 2), rand((256,), 3), out=room[:33])
+    assert (room[33:] == 9).all()
+
+
+def test_matmul_same_bits_every_time_and_status():
+    x, w, scale = int8((77, 3000), 1), int8((3000, 1111), 2), rand((1111,), 3)
+    first, ws = ops.quant_matmul(x, w, scale, out_dtype=F32, return_workspace=True)
+    ops.check_status(ws)
+    for _ in range(5):
+        assert torch.equal(ops.quant_matmul(x, w, scale, out_dtype=F32), first)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# sandwich_norm_quant
+# ---------------------------------------------------------------------------------------------------------------------
+
+def gate_of(gate, act):
+    return {"none": lambda g: g, "sigmoid": torch.sigmoid, "tanh": torch.tanh}[act](gate.double())
+
+
+def check_sandwich(x, residual, gamma, got, *, post_gamma=None, gate=None, gate_act="none", residual_scale=1.0, block_scale=1.0, smooth=None, eps=1e-6,
+                   post_eps=None, quant=True, normed=False):
+    q, scale, stream, y = got
+    dtype, h = residual.dtype, residual.shape[1]
+    post_eps = eps if post_eps is None else post_eps
+    f32 = lambda v: torch.tensor(v, dtype=F32).item()  # noqa: E731  (numbers travel as fp32)
+    # an fp32 sum of h squares by at most h / 32 + 10 steps in a row (each relative u, halved by the root), quotient, root, reciprocal
+    rel_r = (h / 32 + 16) * U32
+    n = x.double()
+    if post_gamma is not None:
+        n = n / (n.square().mean(1, keepdim=True) + f32(post_eps)).sqrt() * post_gamma.double()
+    if gate is not None:
+        n = n * gate_of(gate, gate_act)
+    n = n * f32(block_scale)
+    s = f32(residual_scale) * residual.double() + n
+    # n: the first norm, three products; a gate's exponential and quotient or hyperbolic tangent below 8 units
+    rel_n = (rel_r if post_gamma is not None else 0) + (4 + 16) * U32
+    off_s = n.abs() * rel_n + s.abs() * U32
+    if stream is not None:
+        assert stream.dtype == dtype
+        assert ((stream.double() - s).abs() <= s.abs() * HALF_ULP[dtype] + off_s * (1 + HALF_ULP[dtype]) + TINY[dtype]).all()
+    if gamma is None:
+        assert q is None and scale is None and y is None
+        return
+    r = 1 / (s.square().mean(1, keepdim=True) + f32(eps)).sqrt()
+    # the root mean square moves by no more than the 2-norm of what its elements move by
+    rel_r2 = rel_r + off_s.norm(dim=1, keepdim=True) / (s.norm(dim=1, keepdim=True) + 1e-30) * 1.01
+    g = gamma.double()
+    if normed:
+        want = s * r * g
+        assert ((y.double() - want).abs() <= want.abs() * (HALF_ULP[dtype] * (1 + 1e-3) + rel_r2 + 3 * U32) + off_s * r * g.abs() * 1.01 + TINY[dtype]).all()
+    else:
+        assert y is None
+    if not quant:
+        assert q is None and scale is None
+        return
+    m = smooth.double() if smooth is not None else 1
+    z, off_z = s * g * m, (off_s + 3 * U32 * s.abs()) * (g * m).abs() * 1.01
+    top = z.abs().amax(1, keepdim=True)
+    off_top = off_z.amax(1, keepdim=True)
+    exact = (top / 127 * r)[:, 0]
+    off_scale = (off_top / 127 * r)[:, 0] + exact * (rel_r2[:, 0] + 4 * U32)
+    assert ((scale.double() - exact).abs() <= off_scale * 1.01 + 1e-38).all()
+    # every element is the nearest step; the quotient's own error is what its parts make of it
+    t = torch.where(top > 0, z / (top / 127), torch.zeros_like(z))
+    off_t = torch.where(top > 0, (off_z + z.abs() * (off_top / (top + 1e-300) + 4 * U32)) / (top / 127), torch.zeros_like(z))
+    assert ((q.double() - t).abs() <= 0.5 + off_t * 1.01).all()
+    assert (q.abs().amax(1) == torch.where(top[:, 0] > 0, 127, 0)).all()
+
+
+def sandwich_inputs(rows, h, dtype, x_dtype, seed=0):
+    return dict(x=randn((rows, h), seed + 1, x_dtype, 3.0), residual=randn((rows, h), seed + 2, dtype), gamma=randn((h,), seed + 3, dtype, 0.2) + 1)
+
+
+def run_sandwich(x, residual, gamma, **kw):
+    got = ops.sandwich_norm_quant(x, residual, gamma, **kw)
+    kw.setdefault("normed", False)
+    check_sandwich(x, residual, gamma, got, **kw)
+    return got
+
+
+SANDWICH_SIZES = [(1, 1), (1, 8), (3, 7), (5, 16), (2, 255), (17, 256), (4, 1000), (1, 2048), (33, 1423), (150, 2048), (300, 1424), (7, 7168), (700, 7168), (1300, 1423),
+                  (3, 8200), (2, 16384), (700, 5001), (2, 20001), (1, 65535), (2, 65528), (640, 9000)]
+
+
+@pytest.mark.parametrize("dtype,x_dtype", [(BF16, F32), (BF16, BF16), (F16, F32), (F16, F16), (F32, F32)])
+@pytest.mark.parametrize("rows,h", SANDWICH_SIZES)
+def test_sandwich_sizes(rows, h, dtype, x_dtype):
+    t = sandwich_inputs(rows, h, dtype, x_dtype)
+    post, smooth = randn((h,), 4, dtype, 0.2) + 0.7, rand((h,), 5) + 0.5
+    run_sandwich(**t, post_gamma=post, normed=True, eps=1e-5)
+    run_sandwich(**t, gate=randn((h,), 6, dtype), smooth=smooth, residual_scale=0.75, block_scale=0.4)
+    run_sandwich(**t, post_gamma=post, gate=randn((rows, 1), 7, dtype), gate_act="sigmoid", quant=False, normed=True, post_eps=1e-3)
+    run_sandwich(**t, post_gamma=post, gate=randn((rows, h), 8, dtype), gate_act="tanh", smooth=smooth, normed=True, block_scale=-1.5)
+    run_sandwich(t["x"], t["residual"], None, post_gamma=post, quant=False)
+
+
+@pytest.mark.parametrize("act", ["none", "sigmoid", "tanh"])
+@pytest.mark.parametrize("rows,h", [(6, 520), (400, 1001)])
+def test_sandwich_gates(rows, h, act):
+    t = sandwich_inputs(rows, h, BF16, F32)
+    wide = randn((rows, 2 * h + 3), 9, BF16, 4.0)
+    for gate in (wide[0, :h], wide[:1, :h], wide[:, :1], wide[:, 5:6], wide[:, 3:3 + h], wide[:, :2 * h:2], wide[:1, 4:5], randn((h, rows), 3, BF16).t()):
+        run_sandwich(**t, post_gamma=t["gamma"], gate=gate, gate_act=act, normed=True)
+    # gates that saturate
+    gate = randn((h,), 10, BF16, 60.0)
+    gate[0], gate[1], gate[2] = 0, 1e4, -1e4
+    run_sandwich(**t, gate=gate, gate_act=act)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_sandwich_gammas_in_fp32(dtype):
+    for rows, h in ((9, 512), (700, 1000), (4, 333)):
+        t = sandwich_inputs(rows, h, dtype, F32)
+        t["gamma"] = randn((h,), 6)
+        run_sandwich(**t, post_gamma=randn((h,), 7), normed=True)
+
+
+@pytest.mark.parametrize("offset,pitch", [(0, 2 * 1024), (8, 1024 + 8), (1, 1024 + 3), (4, 1024 + 4)])
+@pytest.mark.parametrize("rows", [37, 700])
+def test_sandwich_strided_rows_and_offsets(offset, pitch, rows):
+    h = 1024
+    wide = lambda seed, dt=BF16: randn((rows * pitch + 64,), seed, dt)[offset:].as_strided((rows, h), (pitch, 1))  # noqa: E731
+    x, residual, gate = wide(1, F32), wide(2), wide(3)
+    gamma, post = randn((h + 8,), 3, BF16)[offset:offset + h], randn((h + 8,), 4, BF16)[offset:offset + h]
+    stream, normed = wide(4), wide(5)
+    q = torch.zeros(rows * pitch + 64, dtype=I8, device=DEV)[offset:].as_strided((rows, h), (pitch, 1))
+    got = ops.sandwich_norm_quant(x, residual, gamma, post_gamma=post, gate=gate, q=q, residual_out=stream, normed_out=normed)
+    assert got[0] is q and got[2] is stream and got[3] is normed
+    check_sandwich(x, residual, gamma, got, post_gamma=post, gate=gate, normed=True)
+    dense = [v.contiguous() for v in (x, residual, gate)]
+    for i, v in enumerate((randn((rows, 2 * h), 7, F32)[:, ::2], randn((h, rows), 8, BF16).t(), randn((1, h), 9, BF16).expand(rows, h))):
+        args = list(dense)
+        args[i] = v
+        run_sandwich(args[0], args[1], gamma, post_gamma=post, gate=args[2], normed=True)
+    # inputs whose rows are differently far apart
+    run_sandwich(dense[0], residual, gamma, post_gamma=post, gate=gate, normed=True)
+    run_sandwich(x, dense[1], gamma, post_gamma=post, gate=gate, normed=True)
+
+
+def test_sandwich_in_place():
+    for rows, h, dtype in ((40, 2048, BF16), (3, 40000, BF16), (5, 77, F32), (700, 1423, BF16), (800, 512, F16)):
+        t = sandwich_inputs(rows, h, dtype, dtype)
+        kw = dict(post_gamma=t["gamma"], gate=randn((rows, h), 5, dtype), gate_act="sigmoid", normed=True)
+        want = ops.sandwich_norm_quant(**t, **kw)
+        for into in ("residual", "x"):
+            a, b = t["x"].clone(), t["residual"].clone()
+            got = ops.sandwich_norm_quant(a, b, t["gamma"], residual_out=b if into == "residual" else a, normed_out=a if into == "residual" else None, **kw)
+            assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def test_sandwich_special_rows():
+    h = 1040
+    for dtype in (BF16, F32):
+        for rows in (9, 700):
+            t = sandwich_inputs(rows, h, dtype, F32)
+            x, residual = t["x"], t["residual"]
+            gamma = torch.ones(h, device=DEV, dtype=dtype)
+            x[1], residual[1] = 0, 0              # no step to divide by
+            x[2, 5] = math.inf
+            x[3, h - 1] = math.nan
+            residual[4, 7] = math.inf
+            x[5] = 0                              # nothing comes out of the block
+            residual[6] = 0
+            residual[7, 3] = 1e4                  # one value dwarfs the rest
+            q, scale, stream, y = got = ops.sandwich_norm_quant(x, residual, gamma, post_gamma=gamma, normed=True)
+            assert (q[1] == 0).all() and scale[1] == 0 and (y[1] == 0).all() and (stream[1] == 0).all()
+            assert all(scale[i].isnan() and (q[i] == 0).all() for i in (2, 3, 4))
+            good = torch.tensor([0, 5, 6, 7] + list(range(8, rows)), device=DEV)
+            check_sandwich(x[good], residual[good], gamma, [v[good] for v in got], post_gamma=gamma, normed=True)
+            # without the norm behind the block an infinity stays where it is
+            stream = ops.sandwich_norm_quant(x, residual, None, quant=False)[2]
+            assert stream[2, 5].isinf() and stream[2, :5].isfinite().all() and stream[3, h - 1].isnan() and stream[4, 7].isinf()
+    # gammas of zeros
+    t = sandwich_inputs(4, 64, BF16, F32)
+    q, scale, _, y = ops.sandwich_norm_quant(t["x"], t["residual"], torch.zeros_like(t["gamma"]), normed=True)
+    assert (q == 0).all() and (scale == 0).all() and (y == 0).all()
+    run_sandwich(**t, post_gamma=torch.zeros_like(t["gamma"]))
+
+
+def test_sandwich_no_rows_and_rows_behind():
+    q, scale, stream, y = ops.sandwich_norm_quant(randn((0, 64), 1), randn((0, 64), 2, BF16), randn((64,), 3, BF16), normed=True)
+    assert q.shape == stream.shape == y.shape == (0, 64) and scale.shape == (0,)
+    t = sandwich_inputs(700, 512, BF16, F32)
+    outs = dict(q=torch.full((710, 512), 7, device=DEV, dtype=I8), scale=torch.full((710,), 7.0, device=DEV), residual_out=torch.full((710, 512), 7.0, device=DEV, dtype=BF16),
+                normed_out=torch.full((710, 512), 7.0, device=DEV, dtype=BF16))
+    ops.sandwich_norm_quant(**t, **{k: v[:700] for k, v in outs.items()})
+    assert all((v[700:] == 7).all() for v in outs.values())
+
+
+def test_sandwich_agrees_with_add_rms_norm_quant():
+    """Without norm, gate and scales it is that operator, bit for bit."""
+    for rows, h, dtype in ((3, 2048, BF16), (700, 1423, F16), (500, 1024, F32), (2, 40000, BF16)):
+        x, residual, gamma, smooth = randn((rows, h), 1, dtype), randn((rows, h), 2, dtype), randn((h,), 3, dtype), rand((h,), 4)
+        a = ops.sandwich_norm_quant(x, residual, gamma, smooth=smooth, normed=True)
+        b = ops.add_rms_norm_quant(x, gamma, residual=residual, smooth=smooth, normed=True)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[2], b[2])
+        assert ((a[1] - b[1]).abs() <= b[1] * (h / 16 + 8) * U32).all()   # two orders of one sum
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# expert_balance
+# ---------------------------------------------------------------------------------------------------------------------
+
+def plain_balance(logits, ids, scoring, coefficient, mask=None, cu=None, upstream=1.0):
+    """(loss, counts, gradient, p, c, p's tokens' weights) in 64 bits, the gradient from the formula."""
+    l = logits.double()
+    t, E = l.shape
+    k = ids.shape[1]
+    gone = ~(l > -math.inf)
+    if scoring == "softmax":
+        top = l.masked_fill(gone, -math.inf).amax(1, keepdim=True)
+        e = torch.where(l == top, torch.ones_like(l), (l - top).exp()).masked_fill(gone, 0)
+        rest = torch.ones_like(l)
+    else:
+        e = torch.sigmoid(l).masked_fill(gone, 0)
+        rest = torch.sigmoid(-l).masked_fill(gone, 1)
+    total = e.sum(1, keepdim=True)
+    p = torch.where(total > 0, e / total, torch.zeros_like(e))
+    cuts = [0, t] if cu is None else cu.tolist()
+    row = torch.arange(t, device=DEV)
+    member = torch.stack([(row >= a) & (row < b) for a, b in zip(cuts[:-1], cuts[1:])])
+    if mask is not None:
+        member &= mask.bool()
+    n = member.sum(1)
+    chosen = torch.stack([(ids == j).sum(1) for j in range(E)], 1)
+    counts = (member.double() @ chosen.double()).long()
+    some = int((n > 0).sum())
+    weight = torch.where(n > 0, coefficient * E / (k * n.double().clamp(min=1) ** 2 * max(some, 1)), 0.0)
+    c = weight[:, None] * counts
+    loss = ((member.double() @ p) * c).sum()
+    of_row = member.double().t() @ c
+    grad = p * (of_row - (p * of_row).sum(1, keepdim=True)) * rest * upstream * member.any(0)[:, None]
+    return loss, counts, weight, grad, p, of_row
+
+
+def error_of_scores(logits, scoring):
+    # p: the argument of the exponential is off by u of its size, the exponential and the quotient by 4 units, the sum of the row's by
+    # E / 32 + 5, two products
+    finite = logits.double()[torch.isfinite(logits)]
+    span = float(finite.max() - finite.min()) if len(finite) and scoring == "softmax" else float(finite.abs().max()) if len(finite) else 0.0
+    return (span + 4 + logits.shape[1] / 32 + 5 + 3) * U32
+
+
+def check_grad(grad, logits, scoring, want, p, c, upstream):
+    assert grad.dtype == logits.dtype and grad.shape == logits.shape
+    # g = p (c - sum p c): p's own error, and that of a sum of E terms no larger than the largest c (and of c's own mean, taken off before)
+    rel_p, terms = error_of_scores(logits, scoring), logits.shape[1] / 32 + 12
+    size = p * (c - c.mean(1, keepdim=True)).abs().amax(1, keepdim=True) * abs(upstream)
+    bound = want.abs() * (rel_p + 8 * U32) + 2 * size * (rel_p + terms * U32)
+    assert ((grad.double() - want).abs() <= bound + want.abs() * HALF_ULP[grad.dtype] * 1.01 + TINY[grad.dtype]).all()
+
+
+def check_balance(logits, ids, scoring="softmax", coefficient=0.01, mask=None, cu=None, grad_loss=None):
+    t, E = logits.shape
+    kw = dict(scoring=scoring, token_mask=mask, cu_seqlens=cu)
+    loss, counts, weight = ops.expert_balance(logits, ids, coefficient=coefficient, **kw)
+    up = 1.0 if grad_loss is None else grad_loss.item()
+    f32 = torch.tensor(coefficient, dtype=F32).item()
+    want, want_counts, want_weight, want_grad, p, c = plain_balance(logits, ids, scoring, f32, mask, cu, up)
+    assert loss.shape == () and loss.dtype == F32 and weight.dtype == F32
+    assert torch.equal(counts, want_counts[0] if cu is None else want_counts)
+    assert ((weight.double() - want_weight).abs() <= want_weight.abs() * 2 * U32).all()
+    # a score's sum over tokens goes through rows / 8 / blocks of 8 warps (at most 64) and as many blocks (at most 37)
+    chain = t / 296 / 8 + 8 + 37 + 16
+    assert abs(loss.item() - want.item()) <= abs(want.item()) * (error_of_scores(logits, scoring) + (chain + 4) * U32) + 1e-38
+    grad = ops.expert_balance_grad(logits, counts, weight, grad_loss=grad_loss, **kw)
+    check_grad(grad, logits, scoring, want_grad, p, c, up)
+    return loss, counts, weight, grad
+
+
+def balance_inputs(t, E, k, dtype, seed=0):
+    logits = (randn((t, E), seed + 1) + randn((E,), seed + 2, scale=0.5)).to(dtype)
+    return logits, (logits.float() + randn((E,), seed + 3, scale=0.1)).topk(k, dim=1).indices
+
+
+BALANCE_SIZES = [(1, 1, 1), (1, 8, 2), (16, 64, 8), (17, 31, 3), (64, 256, 8), (65, 33, 4), (300, 100, 6), (512, 160, 8), (1000, 161, 8), (611, 512, 4), (300, 1024, 8),
+                 (77, 1000, 2), (3001, 155, 6), (5000, 256, 8), (16384, 64, 8), (9000, 8, 1), (2500, 257, 5)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("t,E,k", BALANCE_SIZES)
+def test_balance_sizes(t, E, k, dtype):
+    logits, ids = balance_inputs(t, E, k, dtype)
+    scale = torch.tensor(float(t) * 100, device=DEV)
+    for scoring in ("softmax", "sigmoid"):
+        check_balance(logits, ids.to(I32), scoring, grad_loss=scale)
+        mask = rand((t,), 5) < 0.7
+        check_balance(logits, torch.where(mask[:, None], ids, -1), scoring, mask=mask, grad_loss=scale)
+
+
+def cuts(t, n, seed, last=None):
+    c = torch.randint(0, t + 1, (n + 1,), device=DEV, generator=gen(seed)).sort().values.to(I32)
+    c[0] = 0
+    c[-1] = t if last is None else last
+    return c
+
+
+@pytest.mark.parametrize("t,E,k,n", [(1, 8, 2, 1), (40, 64, 4, 3), (40, 64, 4, 40), (700, 33, 3, 16), (5000, 256, 8, 5), (5000, 128, 8, 300), (16384, 256, 8, 16), (300, 16, 2, 2000)])
+def test_balance_sequences(t, E, k, n):
+    for dtype, scoring in ((F32, "softmax"), (BF16, "sigmoid")):
+        logits, ids = balance_inputs(t, E, k, dtype, seed=7)
+        check_balance(logits, ids, scoring, cu=cuts(t, n, 1), grad_loss=torch.tensor(100.0, device=DEV))
+        mask = rand((t,), 5) < 0.5
+        check_balance(logits, torch.where(mask[:, None], ids, -1).to(I32), scoring, mask=mask, cu=cuts(t, n, 2))
+
+
+def test_balance_of_one_sequence_is_that_of_all_rows():
+    logits, ids = balance_inputs(2000, 64, 4, F32)
+    cu = torch.tensor([0, 2000], device=DEV, dtype=I32)
+    a, b = ops.expert_balance(logits, ids), ops.expert_balance(logits, ids, cu_seqlens=cu)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1][0]) and torch.equal(a[2], b[2])
+    assert torch.equal(ops.expert_balance_grad(logits, *a[1:]), ops.expert_balance_grad(logits, *b[1:], cu_seqlens=cu))
+
+
+def test_balance_rows_outside_the_sequences():
+    """Rows in front of the first and behind the last sequence, and empty sequences at either end and between, as in a padded batch."""
+    logits, ids = balance_inputs(1000, 40, 4, F32)
+    for c in ([0, 0, 10, 10, 10, 700, 700], [5, 5, 300, 301], [1000, 1000, 1000], [0, 0], [999, 1000], [0, 1, 2, 3, 1000, 1000]):
+        cu = torch.tensor(c, device=DEV, dtype=I32)
+        *_, grad = check_balance(logits, ids, cu=cu)
+        assert (grad[:c[0]] == 0).all() and (grad[c[-1]:] == 0).all()
+    # offsets beyond the rows are cut to them
+    a = ops.expert_balance(logits, ids, cu_seqlens=torch.tensor([-5, 400, 2000], device=DEV, dtype=I32))
+    b = ops.expert_balance(logits, ids, cu_seqlens=torch.tensor([0, 400, 1000], device=DEV, dtype=I32))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_balance_no_rows_and_no_tokens():
+    for cu in (None, torch.zeros(4, device=DEV, dtype=I32)):
+        loss, counts, weight = ops.expert_balance(randn((0, 24), 1), torch.empty((0, 3), device=DEV, dtype=I32), cu_seqlens=cu)
+        assert loss == 0 and (counts == 0).all() and (weight == 0).all()
+        assert counts.shape == ((24,) if cu is None else (3, 24))
+    for t in (10, 500):
+        logits, ids = balance_inputs(t, 24, 3, BF16)
+        none = torch.zeros(t, device=DEV, dtype=torch.bool)
+        loss, counts, weight, grad = check_balance(logits, ids, mask=none)
+        assert loss == 0 and (counts == 0).all() and (weight == 0).all() and (grad == 0).all()
+
+
+def test_balance_special_logits_and_ids():
+    for t in (30, 3000):
+        for scoring in ("softmax", "sigmoid"):
+            logits, ids = balance_inputs(t, 72, 4, F32, seed=3)
+            logits[rand((t, 72), 1) < 0.1] = -math.inf
+            logits[1] = -math.inf               # no expert at all
+            logits[2] = math.nan
+            logits[3, 5], logits[3, 6] = math.nan, -math.inf
+            logits[4] = torch.finfo(F32).min    # a mask of the type's lowest value
+            logits[5, :40] = torch.finfo(F32).min
+            logits[6] *= 30
+            logits[7] -= 60
+            if scoring == "softmax":
+                logits[8, 3] = logits[8, 9] = math.inf
+            ids[9:12] = -1
+            ids[12] = 72                        # names no expert
+            ids[13] = 5                         # the same one in every slot
+            ids[14] = 1 << 40
+            # rows whose scores span the whole of fp32 have bounds of their own; here only that nothing is wrong beyond them
+            loss, counts, weight = ops.expert_balance(logits, ids, scoring=scoring, coefficient=0.01)
+            want = plain_balance(logits, ids, scoring, 0.01)
+            assert torch.equal(counts, want[1][0]) and abs(loss - want[0]) <= 1e-5 * want[0]
+            grad = ops.expert_balance_grad(logits, counts, weight, scoring=scoring)
+            assert grad.isfinite().all() and (grad[1] == 0).all() and (grad[2] == 0).all()
+            # Logits of up to 250 make exponentials that are 250 u off.  Where one score is all but 1 the gradient p (c - sum p c) is the small
+            # difference of two numbers of c's size, each of them rounded: its error goes by p times the largest |c - mean c|, as in
+            # check_balance, and not by the gradient, which vanishes with 1 - p (row 6: 1 - p is below u).
+            p, c = want[4:]
+            size = p * (c - c.mean(1, keepdim=True)).abs().amax(1, keepdim=True)
+            assert ((grad.double() - want[3]).abs() <= 2 * (size + want[3].abs()) * (250 + 4 + 8 + 72 / 32 + 12) * U32 + 1e-38).all()
+
+
+def test_balance_gradient_against_differences():
+    """(L(l + h v) - L(l - h v)) / 2h = <grad, v> + h^2 / 6 L'''; the counts stay, as the ids do."""
+    for scoring in ("softmax", "sigmoid"):
+        for cu in (None, torch.tensor([0, 30, 30, 90, 120], device=DEV, dtype=I32)):
+            logits, ids = balance_inputs(120, 24, 3, F32, seed=11)
+            mask = rand((120,), 6) < 0.9
+            kw = dict(scoring=scoring, token_mask=mask, cu_seqlens=cu)
+            _, counts, weight = ops.expert_balance(logits, ids, coefficient=1.0, **kw)
+            grad = ops.expert_balance_grad(logits, counts, weight, **kw).double()
+            for i in range(5):
+                v, h = randn((120, 24), 20 + i, torch.float64), 1e-4
+                up, down = (plain_balance(logits.double() + d * v, ids, scoring, 1.0, mask, cu)[0] for d in (h, -h))
+                # third derivatives of scores along v are below |v|^3 of a row, some 24 ** 1.5 of them: 1e-8 / 6 * 118 < 2e-7 a unit of loss;
+                # rounding 2^-53 / h = 1e-12; the gradient's own error 1e-6 of the sum of its terms
+                assert abs((up - down) / (2 * h) - (grad * v).sum()) <= 2e-7 * 3 + 1e-6 * (grad * v).abs().sum()
+
+
+def test_balance_strided_rows():
+    wide = randn((600, 3 * 64), 1, BF16)
+    ids = balance_inputs(600, 64, 4, BF16)[1]
+    for logits in (wide[:, 64:128], wide[:, 1:65], wide[:, 3:3 + 62], wide[:, :128:2], randn((64, 600), 2, BF16).t(), wide[:1, :64].expand(600, 64)):
+        _, counts, weight, grad = check_balance(logits, ids.clamp(max=logits.shape[1] - 1), grad_loss=torch.tensor(600.0, device=DEV))
+        room = torch.full((600, 200), 3.0, device=DEV, dtype=BF16)
+        for left in (0, 1, 8):
+            out = room[:, left:left + logits.shape[1]]
+            assert ops.expert_balance_grad(logits, counts, weight, grad_loss=torch.tensor(600.0, device=DEV), grad=out) is out
+            check_grad(out, logits, "softmax", *plain_balance(logits, ids.clamp(max=logits.shape[1] - 1), "softmax", 0.01, upstream=600.0)[3:], 600.0)
+            assert (room[:, :left] == 3).all()
+            assert (room[:, left + logits.shape[1]:] == 3).all()
+            room.fill_(3.0)
+    logits = wide[:, :64].contiguous()
+    _, counts, weight = ops.expert_balance(logits, ids.repeat_interleave(2, 1)[:, ::2])
+    want = ops.expert_balance_grad(logits, counts, weight)
+    assert torch.equal(ops.expert_balance_grad(logits, counts, weight, grad=logits), want) and torch.equal(logits, want)   # in place
+
+
+def test_balance_same_bits_every_time():
+    logits, ids = balance_inputs(12345, 256, 8, F32)
+    first = ops.expert_balance(logits, ids, cu_seqlens=cuts(12345, 7, 3))
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(first, ops.expert_balance(logits, ids, cu_seqlens=cuts(12345, 7, 3))))
+
+
+def test_balance_feeds_a_router_that_torch_differentiates():
+    """One step against the gradient lowers the loss of the same choices; the router's gradient is that of the formula."""
+    h, w = randn((400, 96), 1), randn((40, 96), 2, scale=0.1).requires_grad_(True)
+    logits = h @ w.t()
+    ids = ops.route_top_k(logits.detach(), 4)[1]
+    loss, counts, weight = ops.expert_balance(logits.detach(), ids, coefficient=1.0)
+    logits.backward(ops.expert_balance_grad(logits.detach(), counts, weight))
+    want = plain_balance(logits.detach(), ids, "softmax", 1.0)[3].t() @ h.double()
+    assert (w.grad.double() - want).norm() <= 1e-4 * want.norm()   # fp32 products of 400 terms
+    assert (counts == torch.bincount(ids.flatten().long(), minlength=40)).all()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# streams, graphs, threads
+# ---------------------------------------------------------------------------------------------------------------------
+
+def every_op(seed=0, rows=300):
+    x, w, scale, token = int8((rows, 512), seed + 1), int8((512, 640), 2), rand((640,), 3), rand((rows,), seed + 4)
+    t = sandwich_inputs(rows, 640, BF16, F32, seed)
+    logits, ids = balance_inputs(rows, 64, 4, F32, seed)
+    return dict(x=x, w=w, scale=scale, token=token, logits=logits, ids=ids, **{"n_" + k: v for k, v in t.items()})
+
+
+def run_every_op(s, stream=None):
+    y = ops.quant_matmul(s["x"], s["w"], s["scale"], s["token"], stream=stream)
+    normed = ops.sandwich_norm_quant(s["n_x"], s["n_residual"], s["n_gamma"], post_gamma=s["n_gamma"], normed=True, stream=stream)
+    loss, counts, weight = ops.expert_balance(s["logits"], s["ids"], stream=stream)
+    return (y, *normed, loss, counts, weight, ops.expert_balance_grad(s["logits"], counts, weight, stream=stream))
+
+
+def test_operators_on_another_stream():
+    s = every_op()
+    want = run_every_op(s)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    got = run_every_op(s, stream=side)
+    with torch.cuda.stream(side):
+        again = run_every_op(s)
+    side.synchronize()
+    assert all(torch.equal(a, b) and torch.equal(c, b) for a, b, c in zip(got, want, again))
+
+
+@pytest.mark.parametrize("rows", [3, 300])
+def test_operators_can_be_captured(rows):
+    """Two graphs that are replayed in turn, with calls outside between them, on inputs that change."""
+    states, graphs, outs = [every_op(i, rows) for i in (0, 50)], [], []
+    for s in states:
+        run_every_op(s)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(run_every_op(s))
+        graphs.append(g)
+    for i, fresh in ((0, 100), (1, 150), (0, 200), (1, 250)):
+        new = every_op(fresh, rows)
+        for k, v in states[i].items():
+            v.copy_(new[k])
+        graphs[i].replay()
+        want = run_every_op(new)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs[i], want))
+
+
+def test_operators_from_several_threads():
+    import threading
+    states = [every_op(10 * i, rows=100 + 50 * i) for i in range(4)]
+    want = [run_every_op(s) for s in states]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = run_every_op(states[i])
+            torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                failed.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
