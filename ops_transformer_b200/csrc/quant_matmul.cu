@@ -1,21 +1,142 @@
 // quant_matmul: y = ((x w) * scale) * per_token_scale + bias of int8 matrices, without groups.
+//
+// Orientation as in gmm_sm100.cu: weight channels are the M side of the MMA (128 per CTA, a TMEM lane each), tokens its N side, up to 256.
+// What a few tokens cost is the weights' way from memory, so K is split over the CTAs of a cluster until all SMs read: each accumulates its
+// part of K in TMEM, lays the int32 sums into its shared memory, and sums up every S-th token over the S CTAs' parts through distributed
+// shared memory.  Integer sums are exact in any order, so there is nothing to put in sequence and no workspace.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <cstdlib>
 
 #include "gmm_common.h"
 
 namespace gmm {
 namespace {
 
+constexpr int kChannels = 128, kBlockK = 128, kMaxTokens = 256;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kMaxStages = 10, kMaxSplit = 8;
+constexpr uint32_t kWeightStage = kChannels * kBlockK;
+constexpr long long kWaitLimitCycles = 1ll << 31, kDrainLimitCycles = 1ll << 24;   // about a second, a few milliseconds
+
 struct MatmulParams {
-    const int8_t *x, *w;
-    long long ld_x, ws_k, ws_n, ld_y;
     const void *scale, *bias;
     int scale_dtype, bias_dtype, y_dtype;
     const float *token_scale;
     void *y;
+    long long ld_y;
     int m, k, n;
+    int tile_tokens, token_tiles;   // tokens of a tile, a multiple of 32; tiles along them
+    int split, stages;
+    bool packs;                     // four results of a row can be stored at once
+    long long wait_limit;
+    int skip_blocks;                // test only: K blocks that the producer leaves out
+    int *status;
 };
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint64_t *bar, uint32_t count)
+{
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t *bar, uint32_t bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint64_t *bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// Bounded wait; false when it ran out, which the status says, or when another one of the CTA has.
+__device__ __noinline__ bool mbar_wait_slow(uint64_t *bar, uint32_t parity, volatile int *gave_up, const MatmulParams &p, int role)
+{
+    const long long t0 = clock64();
+    while (!mbar_try(bar, parity)) {
+        if (*gave_up) return false;
+        if (clock64() - t0 > p.wait_limit) {
+            *gave_up = 1;
+            if (atomicCAS(p.status, kStatusOk, kStatusWaitTimeout) == kStatusOk) {
+                p.status[1] = (int)blockIdx.x;
+                p.status[2] = role;
+                p.status[3] = (int)parity;
+            }
+            return false;
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volatile int *gave_up, const MatmulParams &p, int role)
+{
+    return mbar_try(bar, parity) || mbar_wait_slow(bar, parity, gave_up, p, role);
+}
+// One lane of a converged warp: copies and MMAs issued under this predicate cost a few cycles each, in a branch that one thread enters 150.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t r;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r != 0;
+}
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, int c0, int c1, uint64_t *bar)
+{
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"((uint64_t)map), "r"(c0), "r"(c1), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+// Operand descriptors, 128-byte swizzle: rows of 128 K-bytes in groups of 8 (tokens, weights stored [n, k]), or 128 channels of one K row,
+// 8 K rows 1024 bytes on (weights stored [k, n]).
+__device__ __forceinline__ uint64_t operand_desc(uint32_t saddr, uint32_t lbo_bytes)
+{
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(lbo_bytes >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int4 ld_cluster(uint32_t saddr, uint32_t rank)
+{
+    uint32_t at;
+    int4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(saddr), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
 
 __device__ __forceinline__ float load_as_float(const void *p, int dtype, long long i)
 {
@@ -23,49 +144,357 @@ __device__ __forceinline__ float load_as_float(const void *p, int dtype, long lo
     if (dtype == kF16) return __half2float(static_cast<const __half *>(p)[i]);
     return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
 }
-
-// One result per thread.
-__global__ void __launch_bounds__(256) quant_matmul_simple_kernel(const MatmulParams p)
+__device__ __forceinline__ uint32_t pack16(int dtype, float a, float b)
 {
-    const long long c = (long long)blockIdx.x * 32 + threadIdx.x % 32, t = (long long)blockIdx.y * 8 + threadIdx.x / 32;
-    if (c >= p.n || t >= p.m) return;
-    const int8_t *x = p.x + t * p.ld_x, *w = p.w + c * p.ws_n;
-    int acc = 0;
-    for (int k = 0; k < p.k; ++k) acc += (int)x[k] * (int)w[k * p.ws_k];
-    float v = __fmul_rn(__int2float_rn(acc), load_as_float(p.scale, p.scale_dtype, c));
-    if (p.token_scale) v = __fmul_rn(v, p.token_scale[t]);
-    if (p.bias) v = __fadd_rn(v, load_as_float(p.bias, p.bias_dtype, c));
-    const long long at = t * p.ld_y + c;
-    if (p.y_dtype == kF32) static_cast<float *>(p.y)[at] = v;
-    else if (p.y_dtype == kF16) static_cast<__half *>(p.y)[at] = __float2half_rn(v);
-    else static_cast<__nv_bfloat16 *>(p.y)[at] = __float2bfloat16_rn(v);
+    if (dtype == kF16) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// NK: the weight is stored [n, k].
+template <bool NK>
+__global__ void __launch_bounds__(kThreads) quant_matmul_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                                                               const MatmulParams p)
+{
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ alignas(8) uint64_t full[kMaxStages], empty[kMaxStages], done;
+    __shared__ uint32_t tmem_base;
+    __shared__ int gave_up;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const int rank = (int)(blockIdx.x % (unsigned)p.split), tile = (int)(blockIdx.x / (unsigned)p.split);
+    const int t0 = tile % p.token_tiles * p.tile_tokens, c0 = tile / p.token_tiles * kChannels;
+    const int blocks = (p.k + kBlockK - 1) / kBlockK;
+    const int kb0 = (int)((long long)rank * blocks / p.split), kb1 = (int)((long long)(rank + 1) * blocks / p.split);
+    uint32_t cols = 32;
+    while (cols < (uint32_t)p.tile_tokens) cols *= 2;
+    if (tid == 0) {
+        for (int i = 0; i < p.stages; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        mbar_init(&done, 1);
+        gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        // Block 0 is among the first to start, and a wait that runs out does so long after.
+        if (blockIdx.x == 0)
+            for (int i = 0; i < 4; ++i) p.status[i] = 0;
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t taddr = tmem_base, stage_bytes = kWeightStage + (uint32_t)p.tile_tokens * kBlockK;
+
+    if (warp == 0) {
+        const bool leader = elect_one();
+        int stage = 0;
+        uint32_t phase = 0;
+        for (int kb = kb0; kb < kb1 - p.skip_blocks; ++kb) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1u, &gave_up, p, 100 + stage))) break;
+            if (leader) {
+                const uint32_t s = smem0 + (uint32_t)stage * stage_bytes;
+                mbar_arrive_expect_tx(&full[stage], stage_bytes);
+                if (NK) tma_load(s, &map_w, kb * kBlockK, c0, &full[stage]);
+                else tma_load(s, &map_w, c0, kb * kBlockK, &full[stage]);
+                tma_load(s + kWeightStage, &map_x, kb * kBlockK, t0, &full[stage]);
+            }
+            __syncwarp();
+            if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+        }
+    } else if (warp == 1) {
+        // D = S32 (2 at bit 4), A = B = signed 8 bits (1 at bits 7 and 10), the major of A (the weights) at bit 15, N >> 3 at bit 17, M >> 4 at 24
+        const uint32_t idesc = 2u << 4 | 1u << 7 | 1u << 10 | (NK ? 0u : 1u) << 15 | (uint32_t)p.tile_tokens >> 3 << 17 | (kChannels >> 4) << 24;
+        const uint64_t w0 = operand_desc(smem0, NK ? 16 : kWeightStage), x0 = operand_desc(smem0 + kWeightStage, 16);
+        constexpr uint32_t kStepW = (NK ? 32 : 32 * kChannels) >> 4, kStepX = 32 >> 4;
+        const bool leader = elect_one();
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, &gave_up, p, 200 + stage));
+            if (!ok) break;
+            tc_fence_after();
+            if (leader) {
+                const uint32_t off = (uint32_t)stage * stage_bytes >> 4;
+#pragma unroll
+                for (int i = 0; i < kBlockK / 32; ++i)
+                    umma_i8(taddr, w0 + off + i * kStepW, x0 + off + i * kStepX, idesc, kb > kb0 || i > 0);
+                umma_commit(&empty[stage]);
+                if (kb + 1 == kb1) umma_commit(&done);
+            }
+            __syncwarp();
+            if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) {   // the MMAs that were issued write to TMEM, which this warp gives back
+            if (leader) umma_commit(&done);
+            __syncwarp();
+            const long long begin = clock64();
+            while (!mbar_try(&done, 0) && clock64() - begin < kDrainLimitCycles) {}
+        }
+    }
+    // This lane's channels, and the sums: TMEM lane = channel, column = token.
+    const int c = c0 + lane * 4, quarter = warp & 3;
+    float scale[4], bias[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        scale[i] = c + i < p.n ? load_as_float(p.scale, p.scale_dtype, c + i) : 0.0f;
+        bias[i] = p.bias && c + i < p.n ? load_as_float(p.bias, p.bias_dtype, c + i) : 0.0f;
+    }
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(&done, 0, &gave_up, p, 300 + warp));
+    tc_fence_after();
+    if (ok) {
+        // every copy has been read by an MMA and every MMA is done: the ring's memory is free
+        const int half = p.tile_tokens / 2;
+        for (int t = (warp >> 2) * half; t < ((warp >> 2) + 1) * half; t += 16) {
+            uint32_t v[16];
+            tmem_ld16(taddr + ((uint32_t)quarter << 21) + (uint32_t)t, v);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            const uint32_t to = smem0 + (uint32_t)t * (kChannels * 4) + (uint32_t)(quarter * 32 + lane) * 4;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + i * kChannels * 4), "r"(v[i]) : "memory");
+        }
+    }
+    tc_fence_before();
+    if (p.split > 1) cluster_sync();
+    else __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+    }
+    for (int t = rank + p.split * warp; t < p.tile_tokens && t0 + t < p.m; t += p.split * kWarps) {
+        const uint32_t at = smem0 + (uint32_t)t * (kChannels * 4) + (uint32_t)lane * 16;
+        int4 acc = make_int4(0, 0, 0, 0);
+        for (int r = 0; r < p.split; ++r) {
+            const int4 v = ld_cluster(at, (uint32_t)r);
+            acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+        }
+        const int sums[4] = {acc.x, acc.y, acc.z, acc.w};
+        const float token = p.token_scale ? p.token_scale[t0 + t] : 1.0f;
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] = __fmul_rn(__fmul_rn(__int2float_rn(sums[i]), scale[i]), token);
+            if (p.bias) v[i] = __fadd_rn(v[i], bias[i]);
+        }
+        const long long row = (long long)(t0 + t) * p.ld_y + c;
+        if (p.packs && c + 4 <= p.n) {
+            if (p.y_dtype == kF32) *reinterpret_cast<float4 *>(static_cast<float *>(p.y) + row) = make_float4(v[0], v[1], v[2], v[3]);
+            else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.y) + row) = make_uint2(pack16(p.y_dtype, v[0], v[1]), pack16(p.y_dtype, v[2], v[3]));
+            continue;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (c + i >= p.n) break;
+            if (p.y_dtype == kF32) static_cast<float *>(p.y)[row + i] = v[i];
+            else static_cast<uint16_t *>(p.y)[row + i] = (uint16_t)pack16(p.y_dtype, v[i], v[i]);
+        }
+    }
+    // A wait that ran out may have left copies in flight, which must not land in shared memory that is no longer this CTA's.
+    if (warp == 0 && *(volatile int *)&gave_up) {
+        const int issued = max(kb1 - kb0 - p.skip_blocks, 0);
+        for (int i = max(issued - p.stages, 0); i < issued; ++i) {
+            const long long begin = clock64();
+            while (!mbar_try(&full[i % p.stages], (uint32_t)(i / p.stages) & 1u) && clock64() - begin < kDrainLimitCycles) {}
+        }
+    }
+    if (p.split > 1) cluster_sync();   // the others have read this CTA's sums
+}
+
+// Rows on no 16-byte boundary, copied onto one: a thread makes 16 bytes of a row out of the two packs that hold them.  A pack that holds
+// a byte of the row lies in the row's own memory pages, whatever else is in it.
+struct PackParams {
+    const char *src[2];
+    char *dst[2];
+    long long ld[2], rows[2];
+    int width[2], pitch[2];             // bytes of a row, of its copy
+    long long first[3];                 // chunks of all rows of the first operand start at 0, of the second at first[1], end at first[2]
+};
+__global__ void __launch_bounds__(256) quant_matmul_pack_kernel(const PackParams p)
+{
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= p.first[2]) return;
+    const int o = i >= p.first[1];
+    const int per = p.pitch[o] / 16;
+    const long long row = (i - p.first[o]) / per;
+    const int at = (int)((i - p.first[o]) % per) * 16;
+    const char *src = p.src[o] + row * p.ld[o], *end = src + p.width[o];
+    const uintptr_t a = (uintptr_t)(src + at);
+    const uint4 *lo = reinterpret_cast<const uint4 *>(a & ~(uintptr_t)15);
+    const int shift = (int)(a & 15);
+    const uint4 u = *lo;
+    const uint4 v = reinterpret_cast<const char *>(lo + 1) < end ? lo[1] : make_uint4(0, 0, 0, 0);
+    const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+    uint32_t r[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t a0 = w[j], a1 = w[j + 1];
+        if (shift >= 12) { a0 = w[j + 3]; a1 = w[j + 4]; }
+        else if (shift >= 8) { a0 = w[j + 2]; a1 = w[j + 3]; }
+        else if (shift >= 4) { a0 = w[j + 1]; a1 = w[j + 2]; }
+        r[j] = __funnelshift_r(a0, a1, (uint32_t)(shift & 3) * 8);
+    }
+    const int left = p.width[o] - at;   // bytes of the row from here on
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int n = left - 4 * j;
+        if (n < 4) r[j] = n <= 0 ? 0u : r[j] & ((1u << 8 * n) - 1u);
+    }
+    *reinterpret_cast<uint4 *>(p.dst[o] + row * p.pitch[o] + at) = make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                  const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn()
+{
+    static EncodeTiledFn fn = []() -> EncodeTiledFn {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return nullptr;
+        return reinterpret_cast<EncodeTiledFn>(f);
+    }();
+    return fn;
+}
+bool encode(CUtensorMap *map, const void *base, long long inner, long long rows, long long pitch, int box_rows)
+{
+    const EncodeTiledFn fn = encode_fn();
+    const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};
+    const cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, ones[2] = {1, 1};
+    return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// A row of one element has no distance to the next one.
+long long pitch_of(long long ld, long long width, long long rows) { return rows > 1 ? ld : width; }
+// What a tensor map can describe: rows on packs that do not overlap.
+bool on_packs(const void *p, long long ld, long long width, long long rows) { return ((uintptr_t)p & 15) == 0 && (rows <= 1 || (ld % 16 == 0 && ld >= width)); }
+size_t round16(long long v) { return (size_t)(v + 15) / 16 * 16; }
+size_t align256(size_t v) { return (v + 255) / 256 * 256; }
+
+// The operands as the kernels read them, in place or in the workspace behind the status.
+struct Operands {
+    bool pack_x, pack_w;
+    long long w_rows, w_width;
+    size_t off_w, bytes;
+    explicit Operands(const QuantMatmulProblem &q)
+    {
+        w_rows = q.w_nk ? q.n : q.k;
+        w_width = q.w_nk ? q.k : q.n;
+        pack_x = !on_packs(q.x, q.ld_x, q.k, q.m);
+        pack_w = !on_packs(q.w, q.ld_w, w_width, w_rows);
+        off_w = 256 + (pack_x ? align256((size_t)q.m * round16(q.k)) : 0);
+        bytes = off_w + (pack_w ? align256((size_t)w_rows * round16(w_width)) : 0);
+    }
+};
+
+// Tiles and the split of K.
+struct Shape {
+    int tile_tokens, token_tiles, channel_tiles, split, stages;
+    size_t smem;
+};
+Shape shape_of(const QuantMatmulProblem &q)
+{
+    Shape s;
+    s.token_tiles = (int)((q.m + kMaxTokens - 1) / kMaxTokens);
+    s.tile_tokens = (int)(((q.m + s.token_tiles - 1) / s.token_tiles + 31) / 32 * 32);
+    s.channel_tiles = (int)((q.n + kChannels - 1) / kChannels);
+    const long long tiles = (long long)s.token_tiles * s.channel_tiles;
+    const int blocks = (int)((q.k + kBlockK - 1) / kBlockK);
+    int per_sm = s.tile_tokens <= 128 ? 2 : 1;
+    long long split = per_sm * 148 / tiles;
+    if (getenv("QM_PER_SM")) per_sm = atoi(getenv("QM_PER_SM"));
+    if (getenv("QM_SPLIT")) split = atoi(getenv("QM_SPLIT"));
+    s.split = (int)(split < 1 ? 1 : split > kMaxSplit ? kMaxSplit : split);
+    if (s.split > blocks) s.split = blocks;
+    const size_t stage = kWeightStage + (size_t)s.tile_tokens * kBlockK, room = (per_sm == 2 ? 111 : 222) * 1024;
+    const int each = (blocks + s.split - 1) / s.split;
+    s.stages = (int)(room / stage);
+    if (s.stages > kMaxStages) s.stages = kMaxStages;
+    if (s.stages > each) s.stages = each;
+    const size_t sums = (size_t)s.tile_tokens * kChannels * 4;
+    s.smem = 1024 + (s.stages * stage > sums ? s.stages * stage : sums);
+    return s;
+}
+
+template <bool NK>
+cudaError_t launch_split(const CUtensorMap &map_x, const CUtensorMap &map_w, const MatmulParams &p, const Shape &s, cudaStream_t stream)
+{
+    const auto kernel = quant_matmul_kernel<NK>;
+    static unsigned long long done_mask = 0;   // once per device; the attribute is idempotent, so a race only repeats the call
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!((done_mask >> (dev & 63)) & 1ull)) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
+        if (e != cudaSuccess) return e;
+        done_mask |= 1ull << (dev & 63);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((long long)s.token_tiles * s.channel_tiles * s.split));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = s.smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)s.split;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = s.split > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, map_x, map_w, p);
 }
 
 }  // namespace
 
-size_t quant_matmul_workspace_bytes(const QuantMatmulProblem &) { return 256; }
+size_t quant_matmul_workspace_bytes(const QuantMatmulProblem &q) { return Operands(q).bytes; }
 
-cudaError_t quant_matmul_launch(const QuantMatmulProblem &q, void *workspace, size_t workspace_bytes, cudaStream_t stream)
+cudaError_t quant_matmul_launch(const QuantMatmulProblem &given, void *workspace, size_t workspace_bytes, cudaStream_t stream)
 {
-    if (q.m <= 0) return cudaSuccess;
-    if (!workspace || workspace_bytes < quant_matmul_workspace_bytes(q)) return cudaErrorInvalidValue;
-    const cudaError_t e = cudaMemsetAsync(workspace, 0, 256, stream);
-    if (e != cudaSuccess) return e;
-    MatmulParams p;
-    p.x = q.x; p.w = q.w; p.ld_x = q.ld_x; p.ld_y = q.ld_y;
-    p.ws_k = q.w_nk ? 1 : q.ld_w; p.ws_n = q.w_nk ? q.ld_w : 1;
-    p.scale = q.scale; p.bias = q.bias; p.scale_dtype = q.scale_dtype; p.bias_dtype = q.bias_dtype; p.y_dtype = q.y_dtype;
-    p.token_scale = q.token_scale; p.y = q.y;
-    p.m = (int)q.m; p.k = (int)q.k; p.n = (int)q.n;
-    for (long long t0 = 0; t0 < q.m; t0 += 65535ll * 8) {   // a grid's second dimension
-        MatmulParams part = p;
-        part.x += t0 * p.ld_x;
-        if (p.token_scale) part.token_scale += t0;
-        part.y = static_cast<char *>(p.y) + t0 * p.ld_y * (p.y_dtype == kF32 ? 4 : 2);
-        part.m = (int)(q.m - t0 < 65535ll * 8 ? q.m - t0 : 65535ll * 8);
-        quant_matmul_simple_kernel<<<dim3((unsigned)((q.n + 31) / 32), (unsigned)((part.m + 7) / 8)), 256, 0, stream>>>(part);
+    if (given.m <= 0) return cudaSuccess;
+    const Operands at(given);
+    if (!workspace || workspace_bytes < at.bytes) return cudaErrorInvalidValue;
+    char *ws = static_cast<char *>(workspace);
+    QuantMatmulProblem q = given;
+    if (at.pack_x || at.pack_w) {
+        PackParams pp = {};
+        int n = 0;
+        const auto add = [&](const int8_t *&from, int64_t &ld, size_t off, long long rows, long long width) {
+            pp.src[n] = reinterpret_cast<const char *>(from);
+            pp.dst[n] = ws + off;
+            pp.ld[n] = pitch_of(ld, width, rows); pp.rows[n] = rows; pp.width[n] = (int)width; pp.pitch[n] = (int)round16(width);
+            from = reinterpret_cast<const int8_t *>(ws + off);
+            ld = pp.pitch[n];
+            pp.first[n + 1] = pp.first[n] + rows * (pp.pitch[n] / 16);
+            ++n;
+        };
+        if (at.pack_x) add(q.x, q.ld_x, 256, q.m, q.k);
+        if (at.pack_w) add(q.w, q.ld_w, at.off_w, at.w_rows, at.w_width);
+        if (n == 1) pp.first[2] = pp.first[1];
+        quant_matmul_pack_kernel<<<(unsigned)((pp.first[2] + 255) / 256), 256, 0, stream>>>(pp);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
     }
-    return cudaGetLastError();
+    const Shape s = shape_of(q);
+    CUtensorMap map_x, map_w;
+    // a single row may name any distance to the next one
+    if (!encode(&map_x, q.x, q.k, q.m, q.m > 1 ? q.ld_x : (long long)round16(q.k), s.tile_tokens) ||
+        !encode(&map_w, q.w, at.w_width, at.w_rows, at.w_rows > 1 ? q.ld_w : (long long)round16(at.w_width), 128))
+        return cudaErrorInvalidValue;
+    MatmulParams p;
+    p.scale = q.scale; p.bias = q.bias; p.scale_dtype = q.scale_dtype; p.bias_dtype = q.bias_dtype; p.y_dtype = q.y_dtype;
+    p.token_scale = q.token_scale; p.y = q.y; p.ld_y = q.ld_y;
+    p.m = (int)q.m; p.k = (int)q.k; p.n = (int)q.n;
+    p.tile_tokens = s.tile_tokens; p.token_tiles = s.token_tiles; p.split = s.split; p.stages = s.stages;
+    const int y_bytes = q.y_dtype == kF32 ? 4 : 2;
+    p.packs = (uintptr_t)q.y % (4 * y_bytes) == 0 && (q.m == 1 || q.ld_y % 4 == 0);
+    p.wait_limit = q.opt.wait_limit_cycles > 0 ? q.opt.wait_limit_cycles : kWaitLimitCycles;
+    p.skip_blocks = q.opt.test_skip_k_blocks;
+    p.status = reinterpret_cast<int *>(ws);
+    return q.w_nk ? launch_split<true>(map_x, map_w, p, s, stream) : launch_split<false>(map_x, map_w, p, s, stream);
 }
 
 }  // namespace gmm
