@@ -17,18 +17,21 @@ namespace {
 constexpr int kChannels = 128, kBlockK = 128, kMaxTokens = 256;
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxStages = 10, kMaxSplit = 8;
-constexpr uint32_t kWeightStage = kChannels * kBlockK;
+constexpr uint32_t kWeightStage = kChannels * kBlockK, kTokenBytes = kChannels * 4;   // of a K block's weights, of a token's sums
+template <int N> struct Int { static constexpr int value = N; };
 constexpr long long kWaitLimitCycles = 1ll << 31, kDrainLimitCycles = 1ll << 24;   // about a second, a few milliseconds
 
 struct MatmulParams {
     const void *scale, *bias;
-    int scale_dtype, bias_dtype, y_dtype;
+    int scale_dtype, bias_dtype;
     const float *token_scale;
     void *y;
     long long ld_y;
     int m, k, n;
     int tile_tokens, token_tiles;   // tokens of a tile, a multiple of 32; tiles along them
     int split, stages;
+    uint32_t parts_at;              // sums of the cluster's other CTAs: behind the ring, or in its place behind this CTA's own
+    bool apart;                     // behind the ring, this CTA's own among them
     bool packs;                     // four results of a row can be stored at once
     long long wait_limit;
     int skip_blocks;                // test only: K blocks that the producer leaves out
@@ -44,10 +47,21 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t *bar, uint32_t by
 {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
+// CLUSTER: for what other CTAs have sent.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_try(uint64_t *bar, uint32_t parity)
 {
     uint32_t ok;
-    asm volatile(
+    if (CLUSTER) asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    else asm volatile(
         "{\n"
         ".reg .pred p;\n"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
@@ -59,10 +73,11 @@ __device__ __forceinline__ bool mbar_try(uint64_t *bar, uint32_t parity)
     return ok != 0;
 }
 // Bounded wait; false when it ran out, which the status says, or when another one of the CTA has.
+template <bool CLUSTER>
 __device__ __noinline__ bool mbar_wait_slow(uint64_t *bar, uint32_t parity, volatile int *gave_up, const MatmulParams &p, int role)
 {
     const long long t0 = clock64();
-    while (!mbar_try(bar, parity)) {
+    while (!mbar_try<CLUSTER>(bar, parity)) {
         if (*gave_up) return false;
         if (clock64() - t0 > p.wait_limit) {
             *gave_up = 1;
@@ -76,9 +91,10 @@ __device__ __noinline__ bool mbar_wait_slow(uint64_t *bar, uint32_t parity, vola
     }
     return true;
 }
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volatile int *gave_up, const MatmulParams &p, int role)
 {
-    return mbar_try(bar, parity) || mbar_wait_slow(bar, parity, gave_up, p, role);
+    return mbar_try<CLUSTER>(bar, parity) || mbar_wait_slow<CLUSTER>(bar, parity, gave_up, p, role);
 }
 // One lane of a converged warp: copies and MMAs issued under this predicate cost a few cycles each, in a branch that one thread enters 150.
 __device__ __forceinline__ bool elect_one()
@@ -109,6 +125,7 @@ __device__ __forceinline__ void umma_commit(uint64_t *bar)
 {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16])
 {
     asm volatile(
@@ -125,86 +142,134 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t saddr, uint32_t lbo_by
 {
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(lbo_bytes >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
-__device__ __forceinline__ void cluster_sync()
+// The cluster's barrier in two parts, and bytes from this CTA's shared memory into another's, whose barrier counts them.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t in_cta(uint32_t saddr, uint32_t rank)
 {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+    return r;
 }
-__device__ __forceinline__ int4 ld_cluster(uint32_t saddr, uint32_t rank)
+__device__ __forceinline__ void copy_to_cta(uint32_t to, uint32_t from, uint32_t bytes, uint32_t bar)
 {
-    uint32_t at;
+    asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "r"(from), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void st_async(uint32_t to, uint32_t v, uint32_t bar)
+{
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(to), "r"(v), "r"(bar) : "memory");
+}
+__device__ __forceinline__ int4 ld_shared(uint32_t saddr)
+{
     int4 v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(saddr), "r"(rank));
-    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    asm volatile("ld.shared.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(saddr) : "memory");
     return v;
 }
-
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_release() { asm volatile("griddepcontrol.launch_dependents;"); }
 __device__ __forceinline__ float load_as_float(const void *p, int dtype, long long i)
 {
     if (dtype == kF32) return static_cast<const float *>(p)[i];
     if (dtype == kF16) return __half2float(static_cast<const __half *>(p)[i]);
     return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
 }
-__device__ __forceinline__ uint32_t pack16(int dtype, float a, float b)
+template <typename Y> __device__ __forceinline__ Y from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+__device__ __forceinline__ void store4(float *y, const float (&v)[4]) { *reinterpret_cast<float4 *>(y) = make_float4(v[0], v[1], v[2], v[3]); }
+template <typename Y>
+__device__ __forceinline__ void store4(Y *y, const float (&v)[4])
 {
-    if (dtype == kF16) {
-        const __half2 h = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t *>(&h);
-    }
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
+    Y h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = from_float<Y>(v[i]);
+    *reinterpret_cast<uint2 *>(y) = *reinterpret_cast<const uint2 *>(h);
 }
 
 // NK: the weight is stored [n, k].
-template <bool NK>
+template <bool NK, typename Y>
 __global__ void __launch_bounds__(kThreads) quant_matmul_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                                                                const MatmulParams p)
 {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ alignas(8) uint64_t full[kMaxStages], empty[kMaxStages], done;
+    __shared__ alignas(8) uint64_t full[kMaxStages], empty[kMaxStages], done, received;
     __shared__ uint32_t tmem_base;
     __shared__ int gave_up;
+    __shared__ alignas(16) float token_scales[kMaxTokens], scales[kChannels], biases[kChannels];
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const int rank = (int)(blockIdx.x % (unsigned)p.split), tile = (int)(blockIdx.x / (unsigned)p.split);
     const int t0 = tile % p.token_tiles * p.tile_tokens, c0 = tile / p.token_tiles * kChannels;
     const int blocks = (p.k + kBlockK - 1) / kBlockK;
     const int kb0 = (int)((long long)rank * blocks / p.split), kb1 = (int)((long long)(rank + 1) * blocks / p.split);
+    const int per = p.tile_tokens / p.split;   // tokens whose sums a CTA of the cluster makes
     uint32_t cols = 32;
     while (cols < (uint32_t)p.tile_tokens) cols *= 2;
-    if (tid == 0) {
+    const uint32_t stage_bytes = kWeightStage + (uint32_t)p.tile_tokens * kBlockK;
+    const int copies = max(kb1 - kb0 - p.skip_blocks, 0);
+    const auto copy_block = [&](int i, int stage) {
+        const uint32_t s = smem0 + (uint32_t)stage * stage_bytes;
+        mbar_arrive_expect_tx(&full[stage], stage_bytes);
+        if (NK) tma_load(s, &map_w, (kb0 + i) * kBlockK, c0, &full[stage]);
+        else tma_load(s, &map_w, c0, (kb0 + i) * kBlockK, &full[stage]);
+        tma_load(s + kWeightStage, &map_x, (kb0 + i) * kBlockK, t0, &full[stage]);
+    };
+    if (warp == 0 && lane == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_x) : "memory");
         for (int i = 0; i < p.stages; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
         mbar_init(&done, 1);
+        mbar_init(&received, 1);
         gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        // Block 0 is among the first to start, and a wait that runs out does so long after.
-        if (blockIdx.x == 0)
-            for (int i = 0; i < 4; ++i) p.status[i] = 0;
+        if (p.split > 1) mbar_arrive_expect_tx(&received, (uint32_t)(p.apart ? p.split : p.split - 1) * per * kTokenBytes);
     }
+    pdl_wait();
+    if (warp == 0) {
+        // the ring is filled before anything else: what follows runs beside the copies' way
+        __syncwarp();
+        const bool leader = elect_one();
+        for (int i = 0; i < min(copies, p.stages); ++i) {
+            if (leader) copy_block(i, i);
+            __syncwarp();
+        }
+    }
+    // What the sums are multiplied with is fetched beside the product and stored behind the barrier; behind the product, its way from memory
+    // would be waited for.
+    float mine[3] = {1.0f, 0.0f, 0.0f};
+    if (warp >= 4) {
+        const int i = tid - 128;
+        if (c0 + i < p.n) {
+            mine[0] = load_as_float(p.scale, p.scale_dtype, c0 + i);
+            if (p.bias) mine[1] = load_as_float(p.bias, p.bias_dtype, c0 + i);
+        }
+    }
+    // Block 0 is among the first to start, and a wait that runs out does so long after.
+    if (blockIdx.x == 0 && warp == 2 && lane < 4) p.status[lane] = 0;
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         tc_fence_before();
     }
     __syncthreads();
+    pdl_release();   // tensor memory is in hand: the next kernel's CTAs may come and wait
     tc_fence_after();
-    const uint32_t taddr = tmem_base, stage_bytes = kWeightStage + (uint32_t)p.tile_tokens * kBlockK;
+    const uint32_t taddr = tmem_base;
+    if (p.apart) cluster_arrive();   // this CTA can be sent to
 
     if (warp == 0) {
         const bool leader = elect_one();
         int stage = 0;
         uint32_t phase = 0;
-        for (int kb = kb0; kb < kb1 - p.skip_blocks; ++kb) {
-            if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1u, &gave_up, p, 100 + stage))) break;
-            if (leader) {
-                const uint32_t s = smem0 + (uint32_t)stage * stage_bytes;
-                mbar_arrive_expect_tx(&full[stage], stage_bytes);
-                if (NK) tma_load(s, &map_w, kb * kBlockK, c0, &full[stage]);
-                else tma_load(s, &map_w, c0, kb * kBlockK, &full[stage]);
-                tma_load(s + kWeightStage, &map_x, kb * kBlockK, t0, &full[stage]);
-            }
+        for (int i = p.stages; i < copies; ++i) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase, &gave_up, p, 100 + stage))) break;
+            if (leader) copy_block(i, stage);
             __syncwarp();
             if (++stage == p.stages) { stage = 0; phase ^= 1u; }
         }
@@ -239,72 +304,115 @@ __global__ void __launch_bounds__(kThreads) quant_matmul_kernel(const __grid_con
             while (!mbar_try(&done, 0) && clock64() - begin < kDrainLimitCycles) {}
         }
     }
-    // This lane's channels, and the sums: TMEM lane = channel, column = token.
-    const int c = c0 + lane * 4, quarter = warp & 3;
-    float scale[4], bias[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        scale[i] = c + i < p.n ? load_as_float(p.scale, p.scale_dtype, c + i) : 0.0f;
-        bias[i] = p.bias && c + i < p.n ? load_as_float(p.bias, p.bias_dtype, c + i) : 0.0f;
+    if (warp >= 4) {
+        scales[tid - 128] = mine[0];
+        biases[tid - 128] = mine[1];
+    } else if (warp >= 2) {
+        for (int t = tid - 64; t < p.tile_tokens; t += 64) token_scales[t] = p.token_scale && t0 + t < p.m ? p.token_scale[t0 + t] : 1.0f;
     }
-    const bool ok = __all_sync(0xffffffffu, mbar_wait(&done, 0, &gave_up, p, 300 + warp));
+    // The sums: TMEM lane = channel, column = token.  They go into shared memory by rows, at the ring's place (every copy has been read by an
+    // MMA and every MMA is done), and those that another CTA finishes from there in one piece; few go straight to it instead.
+    const int quarter = warp & 3, half = warp >> 2;
+    bool ok = __all_sync(0xffffffffu, mbar_wait(&done, 0, &gave_up, p, 300 + warp));
     tc_fence_after();
-    if (ok) {
-        // every copy has been read by an MMA and every MMA is done: the ring's memory is free
-        const int half = p.tile_tokens / 2;
-        for (int t = (warp >> 2) * half; t < ((warp >> 2) + 1) * half; t += 16) {
-            uint32_t v[16];
-            tmem_ld16(taddr + ((uint32_t)quarter << 21) + (uint32_t)t, v);
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            const uint32_t to = smem0 + (uint32_t)t * (kChannels * 4) + (uint32_t)(quarter * 32 + lane) * 4;
+    const uint32_t piece = (uint32_t)per * kTokenBytes, parts = smem0 + p.parts_at;
+    if (p.apart) cluster_wait();
+    const int begin = half * (p.tile_tokens / 2), end = ok ? begin + p.tile_tokens / 2 : begin;
+    for (int t = begin; t < end; t += 16) {
+        uint32_t v[16];
+        tmem_ld16(taddr + ((uint32_t)quarter << 21) + (uint32_t)t, v);
+        tmem_ld_wait();
+        const uint32_t to = (uint32_t)(quarter * 32 + lane) * 4;
+        if (!p.apart) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + i * kChannels * 4), "r"(v[i]) : "memory");
+            for (int i = 0; i < 16; ++i) asm volatile("st.shared.b32 [%0], %1;" ::"r"(smem0 + to + (uint32_t)(t + i) * kTokenBytes), "r"(v[i]) : "memory");
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const uint32_t owner = (uint32_t)((t + i) / per), at = parts + to + (uint32_t)(rank * per + (t + i) % per) * kTokenBytes;
+                const uint32_t there = in_cta(at, owner), bar = in_cta(smem_u32(&received), owner);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) st_async(there + j * kTokenBytes, v[i + j], bar);
+            }
         }
     }
     tc_fence_before();
-    if (p.split > 1) cluster_sync();
-    else __syncthreads();
+    if (p.split > 1 && !p.apart) {
+        fence_async_proxy();
+        cluster_arrive();   // what comes from the others stands in the ring's place, which every CTA of the cluster is done with then
+        cluster_wait();
+    }
+    __syncthreads();
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
     }
-    for (int t = rank + p.split * warp; t < p.tile_tokens && t0 + t < p.m; t += p.split * kWarps) {
-        const uint32_t at = smem0 + (uint32_t)t * (kChannels * 4) + (uint32_t)lane * 16;
-        int4 acc = make_int4(0, 0, 0, 0);
-        for (int r = 0; r < p.split; ++r) {
-            const int4 v = ld_cluster(at, (uint32_t)r);
-            acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+    if (p.split > 1) {
+        if (warp == 2 && ok && !p.apart) {
+            const bool leader = elect_one();
+            for (int i = 1; i < p.split; ++i) {
+                const int owner = (rank + i) % p.split;   // it has a place for every other CTA
+                if (leader)
+                    copy_to_cta(in_cta(parts + (uint32_t)(rank - (rank > owner)) * piece, owner), smem0 + (uint32_t)owner * piece, piece,
+                                in_cta(smem_u32(&received), owner));
+                __syncwarp();
+            }
         }
-        const int sums[4] = {acc.x, acc.y, acc.z, acc.w};
-        const float token = p.token_scale ? p.token_scale[t0 + t] : 1.0f;
-        float v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[i] = __fmul_rn(__fmul_rn(__int2float_rn(sums[i]), scale[i]), token);
-            if (p.bias) v[i] = __fadd_rn(v[i], bias[i]);
-        }
-        const long long row = (long long)(t0 + t) * p.ld_y + c;
-        if (p.packs && c + 4 <= p.n) {
-            if (p.y_dtype == kF32) *reinterpret_cast<float4 *>(static_cast<float *>(p.y) + row) = make_float4(v[0], v[1], v[2], v[3]);
-            else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.y) + row) = make_uint2(pack16(p.y_dtype, v[0], v[1]), pack16(p.y_dtype, v[2], v[3]));
-            continue;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (c + i >= p.n) break;
-            if (p.y_dtype == kF32) static_cast<float *>(p.y)[row + i] = v[i];
-            else static_cast<uint16_t *>(p.y)[row + i] = (uint16_t)pack16(p.y_dtype, v[i], v[i]);
-        }
+        ok = __all_sync(0xffffffffu, mbar_wait<true>(&received, 0, &gave_up, p, 400 + warp));
+        cluster_arrive();
     }
+    // A warp takes a token, a lane four channels.
+    const int c = c0 + lane * 4, first = rank * per, tokens = ok ? min(per, p.m - t0 - first) : 0;
+    const float4 sc = reinterpret_cast<const float4 *>(scales)[lane], bi = reinterpret_cast<const float4 *>(biases)[lane];
+    const float scale[4] = {sc.x, sc.y, sc.z, sc.w}, bias[4] = {bi.x, bi.y, bi.z, bi.w};
+    const auto finish = [&](auto together) {
+        constexpr int kTokens = decltype(together)::value;
+        for (int begin = warp; begin < tokens; begin += kTokens * kWarps) {
+            int acc[kTokens][4] = {};
+            for (int r = 0; r < p.split; ++r) {
+                const uint32_t part = p.apart ? parts + (uint32_t)r * piece : r == rank ? smem0 + (uint32_t)r * piece : parts + (uint32_t)(r - (r > rank)) * piece;
+                int4 v[kTokens];
+#pragma unroll
+                for (int j = 0; j < kTokens; ++j) v[j] = ld_shared(part + (uint32_t)min(begin + j * kWarps, tokens - 1) * kTokenBytes + (uint32_t)lane * 16);
+#pragma unroll
+                for (int j = 0; j < kTokens; ++j) {
+                    acc[j][0] += v[j].x; acc[j][1] += v[j].y; acc[j][2] += v[j].z; acc[j][3] += v[j].w;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kTokens; ++j) {
+                const int t = begin + j * kWarps;
+                if (t >= tokens) break;
+                const float token = token_scales[first + t];
+                float v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[i] = __fmul_rn(__fmul_rn(__int2float_rn(acc[j][i]), scale[i]), token);
+                    if (p.bias) v[i] = __fadd_rn(v[i], bias[i]);
+                }
+                Y *y = static_cast<Y *>(p.y) + (long long)(t0 + first + t) * p.ld_y + c;
+                if (p.packs && c + 4 <= p.n) {
+                    store4(y, v);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (c + i < p.n) y[i] = from_float<Y>(v[i]);
+                }
+            }
+        }
+    };
+    if (tokens <= kWarps) finish(Int<1>());
+    else if (p.split == 1) finish(Int<8>());
+    else finish(Int<4>());
     // A wait that ran out may have left copies in flight, which must not land in shared memory that is no longer this CTA's.
     if (warp == 0 && *(volatile int *)&gave_up) {
-        const int issued = max(kb1 - kb0 - p.skip_blocks, 0);
-        for (int i = max(issued - p.stages, 0); i < issued; ++i) {
+        for (int i = max(copies - p.stages, 0); i < copies; ++i) {
             const long long begin = clock64();
             while (!mbar_try(&full[i % p.stages], (uint32_t)(i / p.stages) & 1u) && clock64() - begin < kDrainLimitCycles) {}
         }
     }
-    if (p.split > 1) cluster_sync();   // the others have read this CTA's sums
+    // No CTA leaves before all of them have received, and so before what it has sent is read.
+    if (p.split > 1) cluster_wait();
 }
 
 // Rows on no 16-byte boundary, copied onto one: a thread makes 16 bytes of a row out of the two packs that hold them.  A pack that holds
@@ -396,12 +504,14 @@ struct Operands {
 // Tiles and the split of K.
 struct Shape {
     int tile_tokens, token_tiles, channel_tiles, split, stages;
-    size_t smem;
+    bool apart;
+    size_t parts_at, smem;
 };
 Shape shape_of(const QuantMatmulProblem &q)
 {
     Shape s;
-    s.token_tiles = (int)((q.m + kMaxTokens - 1) / kMaxTokens);
+    const int most = getenv("QM_MAXTOK") ? atoi(getenv("QM_MAXTOK")) : kMaxTokens;
+    s.token_tiles = (int)((q.m + most - 1) / most);
     s.tile_tokens = (int)(((q.m + s.token_tiles - 1) / s.token_tiles + 31) / 32 * 32);
     s.channel_tiles = (int)((q.n + kChannels - 1) / kChannels);
     const long long tiles = (long long)s.token_tiles * s.channel_tiles;
@@ -410,23 +520,30 @@ Shape shape_of(const QuantMatmulProblem &q)
     long long split = per_sm * 148 / tiles;
     if (getenv("QM_PER_SM")) per_sm = atoi(getenv("QM_PER_SM"));
     if (getenv("QM_SPLIT")) split = atoi(getenv("QM_SPLIT"));
-    s.split = (int)(split < 1 ? 1 : split > kMaxSplit ? kMaxSplit : split);
-    if (s.split > blocks) s.split = blocks;
-    const size_t stage = kWeightStage + (size_t)s.tile_tokens * kBlockK, room = (per_sm == 2 ? 111 : 222) * 1024;
+    s.split = 1;
+    while (2 * s.split <= split && s.split < kMaxSplit && 2 * s.split <= blocks) s.split *= 2;
+    const size_t stage = kWeightStage + (size_t)s.tile_tokens * kBlockK, room = (per_sm == 2 ? 109 : 220) * 1024;
+    const size_t sums = (size_t)s.tile_tokens * kTokenBytes;
+    const auto parts = [&] { return sums / s.split * (s.split - 1); };
+    while (s.split > 1 && sums + parts() > room) s.split /= 2;
+    s.apart = s.split > 1 && s.tile_tokens <= (getenv("QM_APART") ? atoi(getenv("QM_APART")) : 64);
     const int each = (blocks + s.split - 1) / s.split;
-    s.stages = (int)(room / stage);
+    s.stages = (int)((room - (s.apart ? sums : 0)) / stage);
     if (s.stages > kMaxStages) s.stages = kMaxStages;
     if (s.stages > each) s.stages = each;
-    const size_t sums = (size_t)s.tile_tokens * kChannels * 4;
-    s.smem = 1024 + (s.stages * stage > sums ? s.stages * stage : sums);
+    const size_t ring = s.stages * stage;
+    s.parts_at = s.apart ? ring : sums;
+    const size_t all = s.apart ? ring + sums : sums + parts();
+    s.smem = 1024 + (all > ring ? all : ring);
     return s;
 }
 
-template <bool NK>
-cudaError_t launch_split(const CUtensorMap &map_x, const CUtensorMap &map_w, const MatmulParams &p, const Shape &s, cudaStream_t stream)
+template <typename Y>
+cudaError_t launch_split(bool nk, const CUtensorMap &map_x, const CUtensorMap &map_w, const MatmulParams &p, const Shape &s, cudaStream_t stream)
 {
-    const auto kernel = quant_matmul_kernel<NK>;
-    static unsigned long long done_mask = 0;   // once per device; the attribute is idempotent, so a race only repeats the call
+    const auto kernel = nk ? quant_matmul_kernel<true, Y> : quant_matmul_kernel<false, Y>;
+    static unsigned long long done_masks[2] = {0, 0};   // once per device; the attribute is idempotent, so a race only repeats the call
+    unsigned long long &done_mask = done_masks[nk];
     int dev = 0;
     cudaGetDevice(&dev);
     if (!((done_mask >> (dev & 63)) & 1ull)) {
@@ -439,12 +556,14 @@ cudaError_t launch_split(const CUtensorMap &map_x, const CUtensorMap &map_w, con
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = s.smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)s.split;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)s.split;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = s.split > 1 ? 1 : 0;
+    cfg.numAttrs = s.split > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, map_x, map_w, p);
 }
 
@@ -485,16 +604,20 @@ cudaError_t quant_matmul_launch(const QuantMatmulProblem &given, void *workspace
         !encode(&map_w, q.w, at.w_width, at.w_rows, at.w_rows > 1 ? q.ld_w : (long long)round16(at.w_width), 128))
         return cudaErrorInvalidValue;
     MatmulParams p;
-    p.scale = q.scale; p.bias = q.bias; p.scale_dtype = q.scale_dtype; p.bias_dtype = q.bias_dtype; p.y_dtype = q.y_dtype;
+    p.scale = q.scale; p.bias = q.bias; p.scale_dtype = q.scale_dtype; p.bias_dtype = q.bias_dtype;
     p.token_scale = q.token_scale; p.y = q.y; p.ld_y = q.ld_y;
     p.m = (int)q.m; p.k = (int)q.k; p.n = (int)q.n;
-    p.tile_tokens = s.tile_tokens; p.token_tiles = s.token_tiles; p.split = s.split; p.stages = s.stages;
+    p.tile_tokens = s.tile_tokens; p.token_tiles = s.token_tiles; p.split = s.split; p.stages = s.stages; p.parts_at = (uint32_t)s.parts_at; p.apart = s.apart;
     const int y_bytes = q.y_dtype == kF32 ? 4 : 2;
     p.packs = (uintptr_t)q.y % (4 * y_bytes) == 0 && (q.m == 1 || q.ld_y % 4 == 0);
     p.wait_limit = q.opt.wait_limit_cycles > 0 ? q.opt.wait_limit_cycles : kWaitLimitCycles;
     p.skip_blocks = q.opt.test_skip_k_blocks;
     p.status = reinterpret_cast<int *>(ws);
-    return q.w_nk ? launch_split<true>(map_x, map_w, p, s, stream) : launch_split<false>(map_x, map_w, p, s, stream);
+    switch (q.y_dtype) {
+        case kF32: return launch_split<float>(q.w_nk, map_x, map_w, p, s, stream);
+        case kF16: return launch_split<__half>(q.w_nk, map_x, map_w, p, s, stream);
+        default: return launch_split<__nv_bfloat16>(q.w_nk, map_x, map_w, p, s, stream);
+    }
 }
 
 }  // namespace gmm
