@@ -45,9 +45,10 @@ struct Problem {
     const void *w_scale = nullptr;      // [E, N] f32 / bf16 / f16
     int w_scale_dtype = kF32;
     const float *x_scale = nullptr;     // [M] per-token scale (may be null for mode kModeInt32)
-    const void *bias = nullptr;         // [E, N] int32 or bf16, optional
+    int64_t ld_x = 0, ld_w = 0;         // bytes between rows of x and of the weight where they are not dense (the TMA path alone)
+    const void *bias = nullptr;         // [E, N] int32 or bf16, optional (grouped_matmul's kernels also fp32 and fp16)
     int bias_dtype = kNone;
-    const int64_t *group_list = nullptr;
+    const int64_t *group_list = nullptr;  // null: one group (gl_len 1) of all rows (the TMA path alone)
     int gl_len = 0;
     int gl_type = 0;                    // 0 = running total, 1 = per-group count
     int64_t M = 0, K = 0, N = 0, E = 0;

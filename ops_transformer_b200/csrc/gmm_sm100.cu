@@ -639,7 +639,7 @@ __device__ void build_schedule(Shared *sh, const KParams &p, int n_units)
 {
     const int tid = threadIdx.x, L = p.gl_len;
     for (int g = tid; g < L; g += (int)blockDim.x) {
-        const int v = (int)p.group_list[g];
+        const int v = p.group_list ? (int)p.group_list[g] : p.M;   // without a list one group has all rows
         int start = 0, rows = v;
         if (p.gl_type == 0) {
             const int prev = g ? (int)p.group_list[g - 1] : 0;
@@ -1515,6 +1515,7 @@ gmm_w8a8_sm100_kernel(const __grid_constant__ XMaps maps_x, const __grid_constan
                     bias_i[j] = 0;
                     if ((!PLAIN || COMBINE) && in) {
                         if (p.bias_dtype == kBF16) bias_f[j] = __uint_as_float((uint32_t)__ldg(reinterpret_cast<const uint16_t *>(p.bias) + col) << 16);
+                        else if (!COMBINE && (p.bias_dtype == kF32 || p.bias_dtype == kF16)) bias_f[j] = load_scale1(p.bias, p.bias_dtype, col);
                         else if (!COMBINE && p.bias_dtype == kI32) bias_i[j] = __ldg(reinterpret_cast<const int *>(p.bias) + col);
                     }
                 }
@@ -1716,7 +1717,7 @@ gmm_w8a8_sm100_kernel(const __grid_constant__ XMaps maps_x, const __grid_constan
                         }
                     }
                     if (!PLAIN) {
-                        if (p.bias_dtype == kBF16) {
+                        if (p.bias_dtype != kNone && p.bias_dtype != kI32) {
 #pragma unroll
                             for (int i = 0; i < N8; ++i)
 #pragma unroll
@@ -1972,7 +1973,8 @@ cudaError_t launch_layout(int layout, int epi, const Plan &plan, const KParams &
 // aligned base pointers and, for SwiGLU, a half width that keeps the second box aligned.
 bool sm100_shape_ok(const Problem &p)
 {
-    if (p.K % 16 != 0 || p.N % 16 != 0) return false;
+    if ((p.ld_x ? p.ld_x : p.K) % 16 != 0 || p.N % 16 != 0) return false;
+    if ((p.ld_w ? p.ld_w : p.w_layout == kBTransposed ? p.K : p.N) % 16 != 0) return false;
     if (p.mode == kModeSwigluQuant && p.N % 32 != 0) return false;
     if (p.w_layout == kBFractalNz && (p.N % 32 != 0 || (p.mode == kModeSwigluQuant && p.N % 64 != 0))) return false;
     if (p.gl_len > MAX_GROUPS || p.gl_len <= 0) return false;
@@ -1992,7 +1994,7 @@ cudaError_t sm100_encode_maps(const Problem &p, Plan &plan)
     // x: boxes of 32, 64 and 128 rows, of which the producer takes the one that covers a tile's share
     for (int i = 0; i < X_MAPS; ++i) {
         cuuint64_t dims[2] = {(cuuint64_t)p.K, (cuuint64_t)p.M};
-        cuuint64_t strides[1] = {(cuuint64_t)p.K};
+        cuuint64_t strides[1] = {(cuuint64_t)(p.ld_x ? p.ld_x : p.K)};
         cuuint32_t box[2] = {BK, 32u << i};
         cuuint32_t estr[2] = {1, 1};
         CUresult r = enc(&plan.map_x[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(p.x), dims, strides, box, estr,
@@ -2012,14 +2014,16 @@ cudaError_t sm100_encode_maps(const Problem &p, Plan &plan)
     }
     if (p.w_layout == kBTransposed) {  // [E, N, K]
         cuuint64_t dims[4] = {K, cols, halves, E};
-        cuuint64_t strides[3] = {K, K * cols, K * N};
+        const cuuint64_t ld = p.ld_w ? (cuuint64_t)p.ld_w : K;
+        cuuint64_t strides[3] = {ld, ld * cols, ld * N};
         cuuint32_t box[4] = {BK, box_ch, halves, 1};
         r = enc(&plan.map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<int8_t *>(p.w), dims, strides, box, estr,
                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     } else {  // [E, K, N]
         cuuint64_t dims[4] = {cols, K, halves, E};
-        cuuint64_t strides[3] = {N, cols, K * N};
+        const cuuint64_t ld = p.ld_w ? (cuuint64_t)p.ld_w : N;
+        cuuint64_t strides[3] = {ld, cols, K * ld};
         cuuint32_t box[4] = {box_ch, BK, halves, 1};
         r = enc(&plan.map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<int8_t *>(p.w), dims, strides, box, estr,
                 CU_TENSOR_MAP_INTERLEAVE_NONE, box_ch == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,

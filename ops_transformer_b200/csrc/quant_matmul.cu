@@ -7,7 +7,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include <cstdlib>
+#include <cmath>
 
 #include "gmm_common.h"
 
@@ -16,7 +16,7 @@ namespace {
 
 constexpr int kChannels = 128, kBlockK = 128, kMaxTokens = 256;
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kMaxStages = 10, kMaxSplit = 8;
+constexpr int kMaxStages = 10, kMaxSplit = 8, kSms = 148;
 constexpr uint32_t kWeightStage = kChannels * kBlockK, kTokenBytes = kChannels * 4;   // of a K block's weights, of a token's sums
 template <int N> struct Int { static constexpr int value = N; };
 constexpr long long kWaitLimitCycles = 1ll << 31, kDrainLimitCycles = 1ll << 24;   // about a second, a few milliseconds
@@ -506,36 +506,84 @@ struct Shape {
     int tile_tokens, token_tiles, channel_tiles, split, stages;
     bool apart;
     size_t parts_at, smem;
+    double us;                          // about what the kernel takes
 };
-Shape shape_of(const QuantMatmulProblem &q)
+
+// Between the values at 32, 64, 128 and 256 tokens.
+double at_tokens(const double (&v)[4], int tokens)
 {
+    const int i = tokens <= 64 ? 0 : tokens <= 128 ? 1 : 2;
+    return v[i] + (v[i + 1] - v[i]) * (tokens - (32 << i)) / (32 << i);
+}
+
+// Smaller tiles and K splits bring more CTAs to the weights, larger tiles read them less often, and a split has its sums sent around.  What
+// is best is where the estimate below is least: its parts were fitted to times of all ways over 165 sizes (1 to 4096 tokens, K and N of 256
+// to 8192), where the way that it picks takes 1 % longer than the best one on average and 14 % at most.  A K block takes 0.16 us at 32
+// tokens and 0.40 at 256 (what an SM gets from L2, 110 bytes per ns, bounds both), the end of a tile 0.4 to 2.9 us, a split 1.4 to 2.6.
+// Some of the measured times (us), tile tokens / split: 16 x 7168 -> 4096 32/1 14.1, 32/2 11.0, 32/4 9.4; 16 x 2048 -> 7168 32/1 6.5, 32/4
+// 7.2; 256 x 7168 -> 4096 256/2 17.8, 128/1 17.4, 128/2 13.3; 1024 x 2048 -> 2048 256/1 11.2, 128/1 8.5, 64/1 9.2, 128/2 16.2.
+Shape shape_with(const QuantMatmulProblem &q, int most_tokens, int split)
+{
+    static constexpr double kBlock[4] = {0.16, 0.22, 0.23, 0.40}, kEnd[4] = {0.42, 0.62, 1.16, 2.9}, kSplit[4] = {2.2, 1.4, 2.6, 2.5};
+    constexpr double kStart = 1.8, kSharedSm = 1.25, kSharedEnd = 0.55, kSharedSplit = 1.6, kBytesPerUs = 9.4e6;
     Shape s;
-    const int most = getenv("QM_MAXTOK") ? atoi(getenv("QM_MAXTOK")) : kMaxTokens;
-    s.token_tiles = (int)((q.m + most - 1) / most);
+    s.token_tiles = (int)((q.m + most_tokens - 1) / most_tokens);
     s.tile_tokens = (int)(((q.m + s.token_tiles - 1) / s.token_tiles + 31) / 32 * 32);
     s.channel_tiles = (int)((q.n + kChannels - 1) / kChannels);
-    const long long tiles = (long long)s.token_tiles * s.channel_tiles;
-    const int blocks = (int)((q.k + kBlockK - 1) / kBlockK);
-    int per_sm = s.tile_tokens <= 128 ? 2 : 1;
-    long long split = per_sm * 148 / tiles;
-    if (getenv("QM_PER_SM")) per_sm = atoi(getenv("QM_PER_SM"));
-    if (getenv("QM_SPLIT")) split = atoi(getenv("QM_SPLIT"));
-    s.split = 1;
-    while (2 * s.split <= split && s.split < kMaxSplit && 2 * s.split <= blocks) s.split *= 2;
-    const size_t stage = kWeightStage + (size_t)s.tile_tokens * kBlockK, room = (per_sm == 2 ? 109 : 220) * 1024;
-    const size_t sums = (size_t)s.tile_tokens * kTokenBytes;
-    const auto parts = [&] { return sums / s.split * (s.split - 1); };
-    while (s.split > 1 && sums + parts() > room) s.split /= 2;
-    s.apart = s.split > 1 && s.tile_tokens <= (getenv("QM_APART") ? atoi(getenv("QM_APART")) : 64);
-    const int each = (blocks + s.split - 1) / s.split;
+    s.split = split;
+    const int blocks = (int)((q.k + kBlockK - 1) / kBlockK), each = (blocks + split - 1) / split;
+    const double ctas = (double)s.token_tiles * s.channel_tiles * split;
+    // two CTAs on an SM where tiles are small, or of medium size and more than the SMs
+    const bool two = s.tile_tokens <= 64 || (s.tile_tokens <= 128 && ctas > kSms);
+    const size_t stage = kWeightStage + (size_t)s.tile_tokens * kBlockK, room = (two ? 109 : 220) * 1024;
+    const size_t sums = (size_t)s.tile_tokens * kTokenBytes, parts = sums / split * (split - 1);
+    s.apart = split > 1 && s.tile_tokens == 32;   // few sums go straight to their place, more (64 tokens: 10.4 us, 13.4 so) in one copy
     s.stages = (int)((room - (s.apart ? sums : 0)) / stage);
     if (s.stages > kMaxStages) s.stages = kMaxStages;
     if (s.stages > each) s.stages = each;
-    const size_t ring = s.stages * stage;
+    const size_t ring = s.stages * stage, all = s.apart ? ring + sums : split > 1 ? sums + parts : sums;
     s.parts_at = s.apart ? ring : sums;
-    const size_t all = s.apart ? ring + sums : sums + parts();
     s.smem = 1024 + (all > ring ? all : ring);
+    const double turns = std::ceil(ctas / kSms), shared = two && turns > 1 ? turns : 1;   // CTAs of the SM that has most
+    const double tile = two ? each * at_tokens(kBlock, s.tile_tokens) * (turns > 1 ? kSharedSm * turns : 1) : each * at_tokens(kBlock, s.tile_tokens) * turns;
+    const double end = at_tokens(kEnd, s.tile_tokens) * (two ? 1 + kSharedEnd * (shared - 1) : turns);
+    const double memory = ((double)q.m * q.k + (double)q.n * q.k + 2.0 * q.m * q.n) / kBytesPerUs + at_tokens(kEnd, s.tile_tokens);
+    s.us = kStart + (tile + end > memory ? tile + end : memory);
+    if (split > 1) s.us += at_tokens(kSplit, s.tile_tokens) * (split - 1) / split * (turns > 1 ? kSharedSplit : 1);
+    if (each * split >= blocks + split || split > blocks || all > room) s.us = HUGE_VAL;   // an empty part, or too little memory
     return s;
+}
+Shape shape_of(const QuantMatmulProblem &q)
+{
+    Shape best = shape_with(q, kMaxTokens, 1);
+    for (int tokens = kMaxTokens; tokens >= 32; tokens /= 2) {
+        if (tokens > 32 && tokens / 2 >= q.m) continue;   // the same tile as the next one's
+        for (int split = 1; split <= kMaxSplit; split *= 2) {
+            const Shape s = shape_with(q, tokens, split);
+            if (s.us < best.us) best = s;
+        }
+    }
+    return best;
+}
+
+// The persistent kernel of the grouped products takes large calls (4096 x 7168 -> 4096 78 us, 95 here): its CTA pairs have 256 channels for
+// the tokens that they read, and end a tile beside the next one's products.  About 9 us and, for every round of tiles over its units, a tile's
+// K blocks or its end (fitted to the same measurements); half a round at least for a last one that is not full.
+double grouped_us(const QuantMatmulProblem &q)
+{
+    const bool pairs = q.m > 128 && q.k >= 1536;
+    const double tiles = std::ceil(q.n / (pairs ? 256.0 : 128.0)) * std::ceil(q.m / 256.0), units = pairs ? kSms / 2 : kSms;
+    double rounds = tiles / units;
+    const double part = rounds - std::floor(rounds);
+    if (rounds < 1) rounds = 1;
+    else if (part > 0 && part < 0.5) rounds += 0.5 - part;
+    const double tile = std::ceil(q.k / 128.0) * 0.37 + 0.7;
+    return 9 + rounds * (tile > 3.4 ? tile : 3.4);
+}
+bool by_grouped(const QuantMatmulProblem &q, const Shape &s)
+{
+    const auto at4 = [](const void *p) { return ((uintptr_t)p & 3) == 0; };
+    return q.y_dtype != kF32 && q.n % 16 == 0 && ((uintptr_t)q.y & 15) == 0 && (q.m == 1 || q.ld_y == q.n) && at4(q.scale) && at4(q.bias) && grouped_us(q) < s.us;
 }
 
 template <typename Y>
@@ -598,6 +646,19 @@ cudaError_t quant_matmul_launch(const QuantMatmulProblem &given, void *workspace
         if (e != cudaSuccess) return e;
     }
     const Shape s = shape_of(q);
+    if (by_grouped(q, s)) {
+        Problem g;
+        g.x = q.x; g.w = q.w; g.w_scale = q.scale; g.w_scale_dtype = q.scale_dtype; g.x_scale = q.token_scale;
+        g.bias = q.bias; g.bias_dtype = q.bias ? q.bias_dtype : kNone;
+        g.gl_len = 1; g.M = q.m; g.K = q.k; g.N = q.n; g.E = 1;
+        g.ld_x = q.m > 1 ? q.ld_x : (int64_t)round16(q.k); g.ld_w = at.w_rows > 1 ? q.ld_w : (int64_t)round16(at.w_width);
+        g.w_layout = q.w_nk ? 1 : 0;
+        g.out_f16 = q.y_dtype == kF16; g.out0 = q.y;
+        g.opt = q.opt;
+        Plan plan;
+        make_plan(g, &plan);
+        if (plan.path == kPathSm100 && plan.ws_bytes <= 256) return launch(g, plan, workspace, 256, stream);
+    }
     CUtensorMap map_x, map_w;
     // a single row may name any distance to the next one
     if (!encode(&map_x, q.x, q.k, q.m, q.m > 1 ? q.ld_x : (long long)round16(q.k), s.tile_tokens) ||
