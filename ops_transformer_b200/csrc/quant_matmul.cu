@@ -19,6 +19,7 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxStages = 10, kMaxSplit = 8, kSms = 148;
 constexpr uint32_t kWeightStage = kChannels * kBlockK, kTokenBytes = kChannels * 4;   // of a K block's weights, of a token's sums
 template <int N> struct Int { static constexpr int value = N; };
+template <bool B> struct Flag { static constexpr bool value = B; };
 constexpr long long kWaitLimitCycles = 1ll << 31, kDrainLimitCycles = 1ll << 24;   // about a second, a few milliseconds
 
 struct MatmulParams {
@@ -159,10 +160,18 @@ __device__ __forceinline__ void st_async(uint32_t to, uint32_t v, uint32_t bar)
 {
     asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(to), "r"(v), "r"(bar) : "memory");
 }
+template <bool TOGETHER>   // four neighbours, or every 32nd
 __device__ __forceinline__ int4 ld_shared(uint32_t saddr)
 {
     int4 v;
-    asm volatile("ld.shared.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(saddr) : "memory");
+    if (TOGETHER) {
+        asm volatile("ld.shared.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(saddr) : "memory");
+    } else {
+        asm volatile("ld.shared.s32 %0, [%1];" : "=r"(v.x) : "r"(saddr) : "memory");
+        asm volatile("ld.shared.s32 %0, [%1];" : "=r"(v.y) : "r"(saddr + 128) : "memory");
+        asm volatile("ld.shared.s32 %0, [%1];" : "=r"(v.z) : "r"(saddr + 256) : "memory");
+        asm volatile("ld.shared.s32 %0, [%1];" : "=r"(v.w) : "r"(saddr + 384) : "memory");
+    }
     return v;
 }
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -242,7 +251,7 @@ __global__ void __launch_bounds__(kThreads) quant_matmul_kernel(const __grid_con
     }
     // What the sums are multiplied with is fetched beside the product and stored behind the barrier; behind the product, its way from memory
     // would be waited for.
-    float mine[3] = {1.0f, 0.0f, 0.0f};
+    float mine[2] = {0.0f, 0.0f};
     if (warp >= 4) {
         const int i = tid - 128;
         if (c0 + i < p.n) {
@@ -361,19 +370,25 @@ __global__ void __launch_bounds__(kThreads) quant_matmul_kernel(const __grid_con
         ok = __all_sync(0xffffffffu, mbar_wait<true>(&received, 0, &gave_up, p, 400 + warp));
         cluster_arrive();
     }
-    // A warp takes a token, a lane four channels.
-    const int c = c0 + lane * 4, first = rank * per, tokens = ok ? min(per, p.m - t0 - first) : 0;
-    const float4 sc = reinterpret_cast<const float4 *>(scales)[lane], bi = reinterpret_cast<const float4 *>(biases)[lane];
-    const float scale[4] = {sc.x, sc.y, sc.z, sc.w}, bias[4] = {bi.x, bi.y, bi.z, bi.w};
-    const auto finish = [&](auto together) {
+    // A warp takes a token, a lane four channels: neighbours that are stored at once, or where rows of y are on no such boundary every 32nd.
+    const int first = rank * per, tokens = ok ? min(per, p.m - t0 - first) : 0;
+    const auto finish = [&](auto together, auto packed) {
         constexpr int kTokens = decltype(together)::value;
+        constexpr bool PACKS = decltype(packed)::value;
+        const auto channel = [&](int i) { return PACKS ? lane * 4 + i : lane + 32 * i; };
+        float scale[4], bias[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            scale[i] = scales[channel(i)];
+            bias[i] = biases[channel(i)];
+        }
         for (int begin = warp; begin < tokens; begin += kTokens * kWarps) {
             int acc[kTokens][4] = {};
             for (int r = 0; r < p.split; ++r) {
                 const uint32_t part = p.apart ? parts + (uint32_t)r * piece : r == rank ? smem0 + (uint32_t)r * piece : parts + (uint32_t)(r - (r > rank)) * piece;
                 int4 v[kTokens];
 #pragma unroll
-                for (int j = 0; j < kTokens; ++j) v[j] = ld_shared(part + (uint32_t)min(begin + j * kWarps, tokens - 1) * kTokenBytes + (uint32_t)lane * 16);
+                for (int j = 0; j < kTokens; ++j) v[j] = ld_shared<PACKS>(part + (uint32_t)min(begin + j * kWarps, tokens - 1) * kTokenBytes + (uint32_t)channel(0) * 4);
 #pragma unroll
                 for (int j = 0; j < kTokens; ++j) {
                     acc[j][0] += v[j].x; acc[j][1] += v[j].y; acc[j][2] += v[j].z; acc[j][3] += v[j].w;
@@ -390,20 +405,21 @@ __global__ void __launch_bounds__(kThreads) quant_matmul_kernel(const __grid_con
                     v[i] = __fmul_rn(__fmul_rn(__int2float_rn(acc[j][i]), scale[i]), token);
                     if (p.bias) v[i] = __fadd_rn(v[i], bias[i]);
                 }
-                Y *y = static_cast<Y *>(p.y) + (long long)(t0 + first + t) * p.ld_y + c;
-                if (p.packs && c + 4 <= p.n) {
-                    store4(y, v);
+                Y *y = static_cast<Y *>(p.y) + (long long)(t0 + first + t) * p.ld_y + c0;
+                if (PACKS && c0 + channel(3) < p.n) {
+                    store4(y + channel(0), v);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (c + i < p.n) y[i] = from_float<Y>(v[i]);
+                        if (c0 + channel(i) < p.n) y[channel(i)] = from_float<Y>(v[i]);
                 }
             }
         }
     };
-    if (tokens <= kWarps) finish(Int<1>());
-    else if (p.split == 1) finish(Int<8>());
-    else finish(Int<4>());
+    if (!p.packs) finish(Int<4>(), Flag<false>());
+    else if (tokens <= kWarps) finish(Int<1>(), Flag<true>());
+    else if (p.split == 1) finish(Int<8>(), Flag<true>());
+    else finish(Int<4>(), Flag<true>());
     // A wait that ran out may have left copies in flight, which must not land in shared memory that is no longer this CTA's.
     if (warp == 0 && *(volatile int *)&gave_up) {
         for (int i = max(copies - p.stages, 0); i < copies; ++i) {
@@ -415,46 +431,63 @@ __global__ void __launch_bounds__(kThreads) quant_matmul_kernel(const __grid_con
     if (p.split > 1) cluster_wait();
 }
 
-// Rows on no 16-byte boundary, copied onto one: a thread makes 16 bytes of a row out of the two packs that hold them.  A pack that holds
-// a byte of the row lies in the row's own memory pages, whatever else is in it.
+// 16 bytes from byte `shift` of two packs on.
+__device__ __forceinline__ uint4 shifted(const uint4 &lo, const uint4 &hi, int shift)
+{
+    uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    if (shift & 8) { w[0] = w[2]; w[1] = w[3]; w[2] = w[4]; w[3] = w[5]; w[4] = w[6]; w[5] = w[7]; }
+    if (shift & 4) { w[0] = w[1]; w[1] = w[2]; w[2] = w[3]; w[3] = w[4]; w[4] = w[5]; }
+    const uint32_t bits = (uint32_t)(shift & 3) * 8;
+    return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+__device__ __forceinline__ uint4 first_bytes(const uint4 &v, int valid)
+{
+    uint32_t r[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int n = valid - 4 * j;
+        if (n < 4) r[j] = n <= 0 ? 0u : r[j] & ((1u << 8 * n) - 1u);
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+// Rows on no 16-byte boundary, which no tensor map can describe, copied onto one, with zeros up to the next: a warp takes 2 KB of a row.
+// 7168 x 4095 bytes take 8 us, 59 MB read and written.  (Rows shifted into place by the product's own idle warps, which a copy of the weights
+// as they lie in memory ran ahead of: 16 x 7168 -> 4095 15.5 us, 17.6 with the copy; 256 x 767 -> 2049 9.5 and 6.8, since every tile shifts its
+// weights anew at 0.8 us a K block.  Not kept: 160 lines for the few sizes where it wins.)
 struct PackParams {
-    const char *src[2];
-    char *dst[2];
-    long long ld[2], rows[2];
-    int width[2], pitch[2];             // bytes of a row, of its copy
-    long long first[3];                 // chunks of all rows of the first operand start at 0, of the second at first[1], end at first[2]
+    const int8_t *src[2];
+    int8_t *dst[2];
+    long long ld[2], units[2];          // distance of rows; pieces of 2 KB
+    int width[2], pitch[2], pieces[2];  // bytes of a row, of its copy; its pieces
 };
 __global__ void __launch_bounds__(256) quant_matmul_pack_kernel(const PackParams p)
 {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= p.first[2]) return;
-    const int o = i >= p.first[1];
-    const int per = p.pitch[o] / 16;
-    const long long row = (i - p.first[o]) / per;
-    const int at = (int)((i - p.first[o]) % per) * 16;
-    const char *src = p.src[o] + row * p.ld[o], *end = src + p.width[o];
-    const uintptr_t a = (uintptr_t)(src + at);
-    const uint4 *lo = reinterpret_cast<const uint4 *>(a & ~(uintptr_t)15);
-    const int shift = (int)(a & 15);
-    const uint4 u = *lo;
-    const uint4 v = reinterpret_cast<const char *>(lo + 1) < end ? lo[1] : make_uint4(0, 0, 0, 0);
-    const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-    uint32_t r[4];
+    pdl_wait();
+    pdl_release();
+    long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int o = unit >= p.units[0];
+    if (o) unit -= p.units[0];
+    if (unit >= p.units[o]) return;
+    const int width = o ? p.width[1] : p.width[0], pitch = o ? p.pitch[1] : p.pitch[0], pieces = o ? p.pieces[1] : p.pieces[0];
+    const long long row = pieces == 1 ? unit : unit / pieces;
+    const int first = (int)(unit - row * pieces) * 128 + (threadIdx.x & 31);
+    const int8_t *src = (o ? p.src[1] : p.src[0]) + row * (o ? p.ld[1] : p.ld[0]);
+    int8_t *dst = (o ? p.dst[1] : p.dst[0]) + row * pitch;
+    const int shift = (int)((uintptr_t)src & 15);
+    const uint4 *packs = reinterpret_cast<const uint4 *>((uintptr_t)src & ~(uintptr_t)15);
+    uint4 v[4][2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        uint32_t a0 = w[j], a1 = w[j + 1];
-        if (shift >= 12) { a0 = w[j + 3]; a1 = w[j + 4]; }
-        else if (shift >= 8) { a0 = w[j + 2]; a1 = w[j + 3]; }
-        else if (shift >= 4) { a0 = w[j + 1]; a1 = w[j + 2]; }
-        r[j] = __funnelshift_r(a0, a1, (uint32_t)(shift & 3) * 8);
+    for (int i = 0; i < 4; ++i) {
+        const int c = first + 32 * i;
+        v[i][0] = 16 * c < width ? packs[c] : make_uint4(0, 0, 0, 0);
+        v[i][1] = 16 * (c + 1) - shift < width ? packs[c + 1] : make_uint4(0, 0, 0, 0);
     }
-    const int left = p.width[o] - at;   // bytes of the row from here on
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int n = left - 4 * j;
-        if (n < 4) r[j] = n <= 0 ? 0u : r[j] & ((1u << 8 * n) - 1u);
+    for (int i = 0; i < 4; ++i) {
+        const int c = first + 32 * i;
+        if (16 * c < width) *reinterpret_cast<uint4 *>(dst + 16 * c) = first_bytes(shifted(v[i][0], v[i][1], shift), width - 16 * c);
     }
-    *reinterpret_cast<uint4 *>(p.dst[o] + row * p.pitch[o] + at) = make_uint4(r[0], r[1], r[2], r[3]);
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
@@ -478,28 +511,12 @@ bool encode(CUtensorMap *map, const void *base, long long inner, long long rows,
                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// A row of one element has no distance to the next one.
-long long pitch_of(long long ld, long long width, long long rows) { return rows > 1 ? ld : width; }
-// What a tensor map can describe: rows on packs that do not overlap.
+// What a tensor map can describe: rows on packs that do not overlap.  A single row has no distance to the next one.
 bool on_packs(const void *p, long long ld, long long width, long long rows) { return ((uintptr_t)p & 15) == 0 && (rows <= 1 || (ld % 16 == 0 && ld >= width)); }
 size_t round16(long long v) { return (size_t)(v + 15) / 16 * 16; }
 size_t align256(size_t v) { return (v + 255) / 256 * 256; }
-
-// The operands as the kernels read them, in place or in the workspace behind the status.
-struct Operands {
-    bool pack_x, pack_w;
-    long long w_rows, w_width;
-    size_t off_w, bytes;
-    explicit Operands(const QuantMatmulProblem &q)
-    {
-        w_rows = q.w_nk ? q.n : q.k;
-        w_width = q.w_nk ? q.k : q.n;
-        pack_x = !on_packs(q.x, q.ld_x, q.k, q.m);
-        pack_w = !on_packs(q.w, q.ld_w, w_width, w_rows);
-        off_w = 256 + (pack_x ? align256((size_t)q.m * round16(q.k)) : 0);
-        bytes = off_w + (pack_w ? align256((size_t)w_rows * round16(w_width)) : 0);
-    }
-};
+long long weight_rows(const QuantMatmulProblem &q) { return q.w_nk ? q.n : q.k; }
+long long weight_width(const QuantMatmulProblem &q) { return q.w_nk ? q.k : q.n; }
 
 // Tiles and the split of K.
 struct Shape {
@@ -580,14 +597,46 @@ double grouped_us(const QuantMatmulProblem &q)
     const double tile = std::ceil(q.k / 128.0) * 0.37 + 0.7;
     return 9 + rounds * (tile > 3.4 ? tile : 3.4);
 }
-bool by_grouped(const QuantMatmulProblem &q, const Shape &s)
+// The way that a call takes: the kernel above or the grouped one, and what is copied on 16-byte boundaries before.
+struct Way {
+    bool pack_x, pack_w, grouped;
+    Shape shape;
+    size_t off_w, bytes;                // workspace: status, copies
+    explicit Way(const QuantMatmulProblem &q)
+    {
+        pack_x = !on_packs(q.x, q.ld_x, q.k, q.m);
+        pack_w = !on_packs(q.w, q.ld_w, weight_width(q), weight_rows(q));
+        off_w = 256 + (pack_x ? align256((size_t)q.m * round16(q.k)) : 0);
+        bytes = off_w + (pack_w ? align256((size_t)weight_rows(q) * round16(weight_width(q))) : 0);
+        shape = shape_of(q);
+        const auto at4 = [](const void *p) { return ((uintptr_t)p & 3) == 0; };
+        grouped = q.y_dtype != kF32 && q.n % 16 == 0 && ((uintptr_t)q.y & 15) == 0 && (q.m == 1 || q.ld_y == q.n) && at4(q.scale) && at4(q.bias) &&
+                  grouped_us(q) < shape.us;
+    }
+};
+
+// A launch that may begin beside the end of the kernel before it, which it waits for on the device.
+template <typename... P, typename... A>
+cudaError_t launch_dependent(void (*kernel)(P...), unsigned blocks, unsigned threads, size_t smem, int cluster, cudaStream_t stream, const A &...args)
 {
-    const auto at4 = [](const void *p) { return ((uintptr_t)p & 3) == 0; };
-    return q.y_dtype != kF32 && q.n % 16 == 0 && ((uintptr_t)q.y & 15) == 0 && (q.m == 1 || q.ld_y == q.n) && at4(q.scale) && at4(q.bias) && grouped_us(q) < s.us;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 template <typename Y>
-cudaError_t launch_split(bool nk, const CUtensorMap &map_x, const CUtensorMap &map_w, const MatmulParams &p, const Shape &s, cudaStream_t stream)
+cudaError_t launch_typed(bool nk, const CUtensorMap &map_x, const CUtensorMap &map_w, const MatmulParams &p, const Shape &s, cudaStream_t stream)
 {
     const auto kernel = nk ? quant_matmul_kernel<true, Y> : quant_matmul_kernel<false, Y>;
     static unsigned long long done_masks[2] = {0, 0};   // once per device; the attribute is idempotent, so a race only repeats the call
@@ -599,85 +648,72 @@ cudaError_t launch_split(bool nk, const CUtensorMap &map_x, const CUtensorMap &m
         if (e != cudaSuccess) return e;
         done_mask |= 1ull << (dev & 63);
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((long long)s.token_tiles * s.channel_tiles * s.split));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = s.smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)s.split;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = s.split > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, map_x, map_w, p);
+    return launch_dependent(kernel, (unsigned)((long long)s.token_tiles * s.channel_tiles * s.split), kThreads, s.smem, s.split, stream, map_x, map_w, p);
+}
+cudaError_t launch_grouped(const QuantMatmulProblem &q, char *ws, cudaStream_t stream)
+{
+    Problem g;
+    g.x = q.x; g.w = q.w; g.w_scale = q.scale; g.w_scale_dtype = q.scale_dtype; g.x_scale = q.token_scale;
+    g.bias = q.bias; g.bias_dtype = q.bias ? q.bias_dtype : kNone;
+    g.gl_len = 1; g.M = q.m; g.K = q.k; g.N = q.n; g.E = 1;
+    g.ld_x = q.ld_x; g.ld_w = q.ld_w;
+    g.w_layout = q.w_nk ? 1 : 0;
+    g.out_f16 = q.y_dtype == kF16; g.out0 = q.y;
+    g.opt = q.opt;
+    Plan plan;
+    make_plan(g, &plan);
+    if (plan.path != kPathSm100 || plan.ws_bytes > 256) return cudaErrorInvalidValue;
+    return launch(g, plan, ws, 256, stream);
 }
 
 }  // namespace
 
-size_t quant_matmul_workspace_bytes(const QuantMatmulProblem &q) { return Operands(q).bytes; }
+size_t quant_matmul_workspace_bytes(const QuantMatmulProblem &q) { return Way(q).bytes; }
 
 cudaError_t quant_matmul_launch(const QuantMatmulProblem &given, void *workspace, size_t workspace_bytes, cudaStream_t stream)
 {
     if (given.m <= 0) return cudaSuccess;
-    const Operands at(given);
-    if (!workspace || workspace_bytes < at.bytes) return cudaErrorInvalidValue;
+    const Way way(given);
+    if (!workspace || workspace_bytes < way.bytes) return cudaErrorInvalidValue;
     char *ws = static_cast<char *>(workspace);
     QuantMatmulProblem q = given;
-    if (at.pack_x || at.pack_w) {
-        PackParams pp = {};
+    // a single row may name any distance to the next one
+    if (q.m == 1) q.ld_x = (int64_t)round16(q.k);
+    if (weight_rows(q) == 1) q.ld_w = (int64_t)round16(weight_width(q));
+    if (way.pack_x || way.pack_w) {
+        PackParams p = {};
         int n = 0;
         const auto add = [&](const int8_t *&from, int64_t &ld, size_t off, long long rows, long long width) {
-            pp.src[n] = reinterpret_cast<const char *>(from);
-            pp.dst[n] = ws + off;
-            pp.ld[n] = pitch_of(ld, width, rows); pp.rows[n] = rows; pp.width[n] = (int)width; pp.pitch[n] = (int)round16(width);
-            from = reinterpret_cast<const int8_t *>(ws + off);
-            ld = pp.pitch[n];
-            pp.first[n + 1] = pp.first[n] + rows * (pp.pitch[n] / 16);
-            ++n;
+            p.src[n] = from; p.dst[n] = reinterpret_cast<int8_t *>(ws + off);
+            p.ld[n] = ld; p.width[n] = (int)width; p.pitch[n] = (int)round16(width);
+            p.pieces[n] = (int)((width + 2047) / 2048); p.units[n] = rows * p.pieces[n];
+            from = p.dst[n];
+            ld = p.pitch[n++];
         };
-        if (at.pack_x) add(q.x, q.ld_x, 256, q.m, q.k);
-        if (at.pack_w) add(q.w, q.ld_w, at.off_w, at.w_rows, at.w_width);
-        if (n == 1) pp.first[2] = pp.first[1];
-        quant_matmul_pack_kernel<<<(unsigned)((pp.first[2] + 255) / 256), 256, 0, stream>>>(pp);
-        const cudaError_t e = cudaGetLastError();
+        if (way.pack_x) add(q.x, q.ld_x, 256, q.m, q.k);
+        if (way.pack_w) add(q.w, q.ld_w, way.off_w, weight_rows(q), weight_width(q));
+        const cudaError_t e = launch_dependent(quant_matmul_pack_kernel, (unsigned)((p.units[0] + p.units[1] + 7) / 8), 256, 0, 1, stream, p);
         if (e != cudaSuccess) return e;
     }
-    const Shape s = shape_of(q);
-    if (by_grouped(q, s)) {
-        Problem g;
-        g.x = q.x; g.w = q.w; g.w_scale = q.scale; g.w_scale_dtype = q.scale_dtype; g.x_scale = q.token_scale;
-        g.bias = q.bias; g.bias_dtype = q.bias ? q.bias_dtype : kNone;
-        g.gl_len = 1; g.M = q.m; g.K = q.k; g.N = q.n; g.E = 1;
-        g.ld_x = q.m > 1 ? q.ld_x : (int64_t)round16(q.k); g.ld_w = at.w_rows > 1 ? q.ld_w : (int64_t)round16(at.w_width);
-        g.w_layout = q.w_nk ? 1 : 0;
-        g.out_f16 = q.y_dtype == kF16; g.out0 = q.y;
-        g.opt = q.opt;
-        Plan plan;
-        make_plan(g, &plan);
-        if (plan.path == kPathSm100 && plan.ws_bytes <= 256) return launch(g, plan, workspace, 256, stream);
-    }
+    if (way.grouped) return launch_grouped(q, ws, stream);
+    const Shape &s = way.shape;
     CUtensorMap map_x, map_w;
-    // a single row may name any distance to the next one
-    if (!encode(&map_x, q.x, q.k, q.m, q.m > 1 ? q.ld_x : (long long)round16(q.k), s.tile_tokens) ||
-        !encode(&map_w, q.w, at.w_width, at.w_rows, at.w_rows > 1 ? q.ld_w : (long long)round16(at.w_width), 128))
-        return cudaErrorInvalidValue;
+    if (!encode(&map_x, q.x, q.k, q.m, q.ld_x, s.tile_tokens) || !encode(&map_w, q.w, weight_width(q), weight_rows(q), q.ld_w, 128)) return cudaErrorInvalidValue;
     MatmulParams p;
     p.scale = q.scale; p.bias = q.bias; p.scale_dtype = q.scale_dtype; p.bias_dtype = q.bias_dtype;
     p.token_scale = q.token_scale; p.y = q.y; p.ld_y = q.ld_y;
     p.m = (int)q.m; p.k = (int)q.k; p.n = (int)q.n;
-    p.tile_tokens = s.tile_tokens; p.token_tiles = s.token_tiles; p.split = s.split; p.stages = s.stages; p.parts_at = (uint32_t)s.parts_at; p.apart = s.apart;
+    p.tile_tokens = s.tile_tokens; p.token_tiles = s.token_tiles; p.split = s.split; p.stages = s.stages;
+    p.parts_at = (uint32_t)s.parts_at; p.apart = s.apart;
     const int y_bytes = q.y_dtype == kF32 ? 4 : 2;
     p.packs = (uintptr_t)q.y % (4 * y_bytes) == 0 && (q.m == 1 || q.ld_y % 4 == 0);
     p.wait_limit = q.opt.wait_limit_cycles > 0 ? q.opt.wait_limit_cycles : kWaitLimitCycles;
     p.skip_blocks = q.opt.test_skip_k_blocks;
     p.status = reinterpret_cast<int *>(ws);
     switch (q.y_dtype) {
-        case kF32: return launch_split<float>(q.w_nk, map_x, map_w, p, s, stream);
-        case kF16: return launch_split<__half>(q.w_nk, map_x, map_w, p, s, stream);
-        default: return launch_split<__nv_bfloat16>(q.w_nk, map_x, map_w, p, s, stream);
+        case kF32: return launch_typed<float>(q.w_nk, map_x, map_w, p, s, stream);
+        case kF16: return launch_typed<__half>(q.w_nk, map_x, map_w, p, s, stream);
+        default: return launch_typed<__nv_bfloat16>(q.w_nk, map_x, map_w, p, s, stream);
     }
 }
 
