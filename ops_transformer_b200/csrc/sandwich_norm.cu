@@ -93,9 +93,297 @@ __global__ void __launch_bounds__(256) sandwich_any_kernel(const SandwichParams 
     }
 }
 
+// V values of a vector over the channels from `at` on, as pairs.
+template <typename G, int V, bool WHOLE>
+__device__ __forceinline__ void load_channels(const void *vec, int at, int h, f32x2 *f)
+{
+    const G *g = static_cast<const G *>(vec);
+    if constexpr (!WHOLE) load_anywhere<G, V>(g, at, h, f);
+    else if constexpr (sizeof(G) == 4) load_fp32<V>(g + at, f);
+    else unpack<G>(__ldg(reinterpret_cast<const uint4 *>(g + at)), f);
+}
+
+// One CTA per row; a thread holds NCH packs of V elements (16 bytes of T), blockDim.x apart, in fp32 from the first look at x to the last
+// store.  WHOLE: rows start on packs.  Else every row starts `lead` elements into one, the same in all tensors, and only what lies in a row's
+// first and last pack is masked and stored one element at a time.
+//
+// STREAM: the CTA takes every gridDim.x-th row.  While it works on one, the packs of the next are copied to shared memory, each by the
+// thread that will read it, x as soon as it is in registers and the rest behind the first reduction.
+template <typename T, typename X, int NCH, bool WHOLE, int MAXT, int MINB, bool STREAM>
+__global__ void __launch_bounds__(MAXT, MINB) sandwich_kernel(const SandwichParams p)
+{
+    constexpr int V = 16 / (int)sizeof(T), XW = (int)sizeof(X) * V / 16;   // loads of a pack of x
+    extern __shared__ uint4 ahead[];    // STREAM: [(XW + 1 or 2) * NCH][threads]: x, residual, gate
+    __shared__ float2 red[4][32];
+    const int threads = blockDim.x;
+    const uint32_t mine = STREAM ? (uint32_t)__cvta_generic_to_shared(ahead) + threadIdx.x * 16 : 0;
+    const bool rows_gate = p.gate && p.ld_gate != 0 && p.gate_step != 0;
+    const auto lead_of = [&](long long row) { return WHOLE ? 0 : (int)((row * p.ld_x) & (V - 1)); };
+    // Elements from the row's first pack on that there are to read (see add_rms_norm_quant): a row's edge packs hold elements of its
+    // neighbours, which are read with it and dropped, but behind the last row's end there may be nothing.
+    const auto room_of = [&](long long row, int lead) {
+        long long ld = min(p.ld_x, p.ld_residual);
+        if (rows_gate) ld = min(ld, p.ld_gate);
+        return lead + p.h + (int)min((p.rows - 1 - row) * ld, 1024ll);
+    };
+    const auto slot = [&](int s) { return mine + (uint32_t)(s * threads) * 16; };
+    const auto copy = [&](int s, const void *from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot(s)), "l"(from) : "memory"); };
+    const auto there = [&](int c, int lead, int room) { return WHOLE ? c * V < p.h : c * V < lead + p.h && (c + 1) * V <= room; };
+    const auto fetch_x = [&](long long row) {
+        const int lead = lead_of(row), room = room_of(row, lead);
+        const X *x = static_cast<const X *>(p.x) + row * p.ld_x - lead;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int c = threadIdx.x + i * threads;
+            if (!there(c, lead, room)) continue;
+#pragma unroll
+            for (int j = 0; j < XW; ++j) copy(i * XW + j, reinterpret_cast<const uint4 *>(x + (long long)c * V) + j);
+        }
+    };
+    const auto fetch_rest = [&](long long row, int i) {
+        const int lead = lead_of(row), room = room_of(row, lead), c = threadIdx.x + i * threads;
+        if (!there(c, lead, room)) return;
+        copy(NCH * XW + i, static_cast<const T *>(p.residual) + row * p.ld_residual - lead + (long long)c * V);
+        if (rows_gate) copy(NCH * (XW + 1) + i, static_cast<const T *>(p.gate) + row * p.ld_gate - lead + (long long)c * V);
+    };
+    const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+    const auto await_older = [] { asm volatile("cp.async.wait_group 1;" ::: "memory"); };
+    if (STREAM) {
+        fetch_x(blockIdx.x);
+        commit();
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) fetch_rest(blockIdx.x, i);
+        commit();
+    }
+    int parity = 0;
+    for (long long row = blockIdx.x; row < p.rows; row += STREAM ? (long long)gridDim.x : (long long)p.rows) {
+        const long long next = row + gridDim.x;
+        const int lead = lead_of(row), end = lead + p.h, room = room_of(row, lead), packs = (end + V - 1) / V;
+        const X *x = static_cast<const X *>(p.x) + row * p.ld_x - lead;
+        const T *residual = static_cast<const T *>(p.residual) + row * p.ld_residual - lead, *gate = static_cast<const T *>(p.gate) + row * p.ld_gate - lead;
+        const auto full = [&](int c) { return WHOLE || (c * V >= lead && (c + 1) * V <= end); };
+        const auto inside = [&](int e) { return e >= lead && e < end; };
+        // a pack of a row of S: N loads of it, out of the slots from s on
+        const auto load = [&](auto type, const auto *from, int c, int s, f32x2 *f) {
+            typedef decltype(type) S;
+            constexpr int N = (int)sizeof(S) * V / 16;
+            if (!WHOLE && (c + 1) * V > room) {
+                const auto one = [&](int e) { return inside(e) ? to_float<S>(from[e]) : 0.0f; };
+#pragma unroll
+                for (int e = 0; e < V; e += 2) f[e / 2] = pair2(one(c * V + e), one(c * V + e + 1));
+                return;
+            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                uint4 u;
+                if (STREAM) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(slot(s + j)) : "memory");
+                else u = *(reinterpret_cast<const uint4 *>(from + (long long)c * V) + j);
+                unpack<S>(u, f + j * (V / 2 / N));
+            }
+        };
+        const auto mask = [&](int c, f32x2 *f) {
+            if (full(c)) return;
+#pragma unroll
+            for (int e = 0; e < V; e += 2) {
+                const float2 v = unpair2(f[e / 2]);
+                f[e / 2] = pair2(inside(c * V + e) ? v.x : 0.0f, inside(c * V + e + 1) ? v.y : 0.0f);
+            }
+        };
+        const auto gammas = [&](const void *g, int c, f32x2 *f) {
+            if (p.gamma32) load_channels<float, V, WHOLE>(g, c * V - lead, p.h, f);
+            else load_channels<T, V, WHOLE>(g, c * V - lead, p.h, f);
+        };
+        const auto store = [&](T *to, int c, const f32x2 *f) {
+            if (full(c)) {
+                *reinterpret_cast<uint4 *>(to + (long long)c * V) = pack<T>(f);
+                return;
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (inside(c * V + e)) to[c * V + e] = from_float<T>(element(f, e));
+        };
+
+        // the block's output, and the norm behind it
+        f32x2 u[NCH][V / 2];
+        if (STREAM) await_older();
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int c = threadIdx.x + i * threads;
+            if (c >= packs) break;
+            load(X(), x, c, i * XW, u[i]);
+            mask(c, u[i]);
+        }
+        if (STREAM) {
+            if (next < p.rows) fetch_x(next);   // the thread has read what this fills
+            commit();
+        }
+        float factor = p.block_scale;
+        if (p.post_gamma) {
+            f32x2 sum2 = 0;
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) {
+                if (threadIdx.x + i * threads >= packs) break;
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) sum2 = fma2(u[i][e], u[i][e], sum2);
+            }
+            const float2 parts = unpair2(sum2);
+            float sum = parts.x + parts.y, unused = 0.0f;
+            block_reduce(sum, unused, red[parity]);
+            factor = __fmul_rn(factor, rsqrtf(__fmaf_rn(sum, p.inv_h, p.post_eps)));
+        }
+        if (p.gate && p.gate_step == 0) factor = __fmul_rn(factor, gate_value(to_float<T>(static_cast<const T *>(p.gate)[row * p.ld_gate]), p.gate_act));
+
+        // the residual stream, and the sums of the next norm
+        if (STREAM) await_older();
+        f32x2 sum2 = 0;
+        float mag = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int c = threadIdx.x + i * threads;
+            if (c >= packs) break;
+            f32x2 f[V / 2];
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) u[i][e] = mul2(u[i][e], pair2(factor, factor));
+            if (p.post_gamma) {
+                gammas(p.post_gamma, c, f);
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) u[i][e] = mul2(u[i][e], f[e]);
+            }
+            if (p.gate && p.gate_step != 0) {
+                if (rows_gate) load(T(), gate, c, NCH * (XW + 1) + i, f);
+                else load_channels<T, V, WHOLE>(p.gate, c * V - lead, p.h, f);
+                if (p.gate_act != kGateNone) {
+#pragma unroll
+                    for (int e = 0; e < V / 2; ++e) {
+                        const float2 g = unpair2(f[e]);
+                        f[e] = pair2(gate_value(g.x, p.gate_act), gate_value(g.y, p.gate_act));
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) u[i][e] = mul2(u[i][e], f[e]);
+            }
+            load(T(), residual, c, NCH * XW + i, f);
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) u[i][e] = fma2(f[e], pair2(p.residual_scale, p.residual_scale), u[i][e]);
+            mask(c, u[i]);
+            if (p.residual_out) store(static_cast<T *>(p.residual_out) + row * p.ld_residual_out - lead, c, u[i]);
+            if (!p.gamma) continue;
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) sum2 = fma2(u[i][e], u[i][e], sum2);
+            gammas(p.gamma, c, f);
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) u[i][e] = mul2(u[i][e], f[e]);
+            if (!p.q) continue;
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) f[e] = u[i][e];
+            if (p.smooth) {
+                f32x2 m[V / 2];
+                load_channels<float, V, WHOLE>(p.smooth, c * V - lead, p.h, m);
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) f[e] = mul2(f[e], m[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) {
+                const float2 v = unpair2(f[e]);
+                mag = max_mag(mag, v.x, v.y);
+            }
+        }
+        if (STREAM) {
+#pragma unroll
+            for (int i = 0; i < NCH; ++i)
+                if (next < p.rows) fetch_rest(next, i);
+            commit();
+        }
+        if (p.gamma) {
+            const float2 parts = unpair2(sum2);
+            float sum = parts.x + parts.y;
+            block_reduce(sum, mag, red[2 + parity]);
+            const float r = rsqrtf(__fmaf_rn(sum, p.inv_h, p.eps)), step = step_of(mag);
+            Quantiser quant;
+            quant.set(step);
+            if (p.q && threadIdx.x == 0) p.scale[row] = step == 0.0f ? 0.0f : __fmul_rn(step, r);
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) {
+                const int c = threadIdx.x + i * threads;
+                if (c >= packs) break;
+                if (p.normed_out) {
+                    f32x2 y[V / 2];
+#pragma unroll
+                    for (int e = 0; e < V / 2; ++e) y[e] = mul2(u[i][e], pair2(r, r));
+                    store(static_cast<T *>(p.normed_out) + row * p.ld_normed - lead, c, y);
+                }
+                if (!p.q) continue;
+                if (p.smooth) {
+                    f32x2 m[V / 2];
+                    load_channels<float, V, WHOLE>(p.smooth, c * V - lead, p.h, m);
+#pragma unroll
+                    for (int e = 0; e < V / 2; ++e) u[i][e] = mul2(u[i][e], m[e]);
+                }
+                uint32_t q[V / 4];
+#pragma unroll
+                for (int e = 0; e < V / 4; ++e) q[e] = quant.four(u[i] + 2 * e, quant.rcp != 0.0f);
+                int8_t *to = p.q + row * p.ld_q - lead + (long long)c * V;
+                if (full(c)) {
+                    if (V == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(q[0], q[V / 4 - 1]);
+                    else *reinterpret_cast<uint32_t *>(to) = q[0];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if (inside(c * V + e)) to[e] = (int8_t)(q[e / 4] >> (e % 4 * 8));
+                }
+            }
+        }
+        parity ^= 1;
+    }
+}
+
+template <typename T, typename X, bool WHOLE>
+cudaError_t launch_packed(const SandwichParams &p, cudaStream_t stream)
+{
+    constexpr int V = 16 / (int)sizeof(T), XW = (int)sizeof(X) * V / 16;
+    const int packs = (p.h + (WHOLE ? 0 : V - 1) + V - 1) / V;
+    const auto warps = [](int n) { return (n + 31) / 32 * 32; };
+    // Few rows: as many threads as a row has packs, for the shortest chain.  More: four packs a thread, for more rows on an SM, and the next
+    // row's loads under way; the CTAs that find a place on the SMs together go through the rows.
+    const int four = warps((packs + 3) / 4);
+    if (packs <= 1024 && (p.rows <= 2 * 148 || packs <= 64)) {
+        sandwich_kernel<T, X, 1, WHOLE, 1024, 1, false><<<p.rows, warps(packs), 0, stream>>>(p);
+    } else if (packs <= 4 * 512) {
+        const int smem = (XW + (p.gate && p.ld_gate && p.gate_step ? 2 : 1)) * 4 * 16 * four;
+        const int fit = 1024 / four < 220 * 1024 / (smem + 2048) ? 1024 / four : 220 * 1024 / (smem + 2048);
+        const auto kernel = sandwich_kernel<T, X, 4, WHOLE, 512, 2, true>;
+        static unsigned long long done_mask = 0;   // once per device; the attribute is idempotent, so a race only repeats the call
+        int dev = 0;
+        cudaGetDevice(&dev);
+        if (!((done_mask >> (dev & 63)) & 1ull)) {
+            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * 4 * 16 * 512);
+            if (e != cudaSuccess) return e;
+            done_mask |= 1ull << (dev & 63);
+        }
+        kernel<<<p.rows < 148 * fit ? p.rows : 148 * fit, four, smem, stream>>>(p);
+    } else if (packs <= 4 * 1024) {
+        sandwich_kernel<T, X, 4, WHOLE, 1024, 1, false><<<p.rows, four, 0, stream>>>(p);
+    } else {
+        sandwich_any_kernel<T, X><<<p.rows, 256, 0, stream>>>(p);
+    }
+    return cudaGetLastError();
+}
+
 template <typename T, typename X>
 cudaError_t launch_typed(const SandwichParams &p, cudaStream_t stream)
 {
+    constexpr int V = 16 / (int)sizeof(T);
+    // Packs need every tensor to begin on one (V elements of its own type, at most 16 bytes) and its rows to be as far apart as x's, modulo
+    // a pack.
+    const auto fits = [&](const void *base, long long ld, int bytes) {
+        return !base || (((uintptr_t)base & (uintptr_t)(V * bytes < 16 ? V * bytes - 1 : 15)) == 0 && (ld - p.ld_x) % V == 0);
+    };
+    const bool rows_gate = p.gate && p.gate_step && p.ld_gate, channel_gate = p.gate && p.gate_step && !p.ld_gate;
+    const bool packed = fits(p.x, p.ld_x, sizeof(X)) && fits(p.residual, p.ld_residual, sizeof(T)) && fits(p.residual_out, p.ld_residual_out, sizeof(T)) &&
+                        fits(p.normed_out, p.ld_normed, sizeof(T)) && fits(p.q, p.ld_q, 1) && fits(p.gamma, p.ld_x, p.gamma32 ? 4 : sizeof(T)) &&
+                        fits(p.post_gamma, p.ld_x, p.gamma32 ? 4 : sizeof(T)) && fits(p.smooth, p.ld_x, 4) &&
+                        (!rows_gate || fits(p.gate, p.ld_gate, sizeof(T))) && (!channel_gate || fits(p.gate, p.ld_x, sizeof(T)));
+    if (packed) return p.h % V == 0 && p.ld_x % V == 0 ? launch_packed<T, X, true>(p, stream) : launch_packed<T, X, false>(p, stream);
     sandwich_any_kernel<T, X><<<p.rows, 256, 0, stream>>>(p);
     return cudaGetLastError();
 }
