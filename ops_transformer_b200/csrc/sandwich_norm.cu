@@ -337,6 +337,281 @@ __global__ void __launch_bounds__(MAXT, MINB) sandwich_kernel(const SandwichPara
     }
 }
 
+// Many rows that start on packs: one CTA per SM, in which groups of threads take a row each.  What multiplies the channels is laid out once
+// in shared memory, in fp32 and with everything folded in that a row does not change (the norm's weight, the activated gate, the block's
+// scale), so that a row's turn has no loads but its own.  Those come as one bulk copy a tensor, for the next row as soon as the group holds
+// this one in registers.  (With a 16-byte cp.async for each pack, the form of the other kernels, an SM takes in 16 bytes per ns however many
+// are under way: 4096 x 7168 in 80 us.)  A group's threads hold four packs each.
+constexpr int kGroupPacks = 2, kMaxGroups = 14, kMaxDepth = 3;    // of the 15 named barriers that are left
+constexpr long long kWaitLimitCycles = 1ll << 31;  // about a second
+__host__ __device__ constexpr int group_threads_most(int elem) { return 1024; }
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// Bounded: false when the copies have not come.
+__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity)
+{
+    uint32_t ok = 0;
+    const long long t0 = clock64();
+    while (true) {
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+            "selp.u32 %0, 1, 0, p;\n"
+            "}\n"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if (clock64() - t0 > kWaitLimitCycles) return false;
+    }
+}
+__device__ __forceinline__ void bulk_copy(void *to, const void *from, uint32_t bytes, uint64_t *bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(to)), "l"(from), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void group_sync(int group, int threads)
+{
+    if (threads > 32) asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(threads) : "memory");
+    else __syncwarp();
+}
+
+__device__ __forceinline__ void group_reduce(float &sum, float &mag, float2 *red, int group, int threads)
+{
+    uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(mag) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (threads > 32) {
+        const int lane = threadIdx.x & 31, warps = threads >> 5, warp = (int)(threadIdx.x >> 5) - group * warps;
+        red += group * warps;
+        if (lane == 0) red[warp] = make_float2(sum, __uint_as_float(m));
+        group_sync(group, threads);
+        const float2 v = lane < warps ? red[lane] : make_float2(0.0f, 0.0f);
+        sum = v.x;
+        m = __reduce_max_sync(0xffffffffu, __float_as_uint(v.y));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+    mag = __uint_as_float(m);
+}
+
+// EXACT: every thread of a group has all of its packs.  GATED: a gate for each element.
+template <typename T, typename X, bool EXACT, bool GATED>
+__global__ void __launch_bounds__(group_threads_most(sizeof(T)), 1) sandwich_rows_kernel(const SandwichParams p, int threads, int groups, int depth)
+{
+    constexpr int V = 16 / (int)sizeof(T), XW = (int)sizeof(X) * V / 16, N = kGroupPacks;
+    extern __shared__ uint4 smem[];     // the groups' rows (x, residual, gate); block's, next norm's and smoothing's factors [h]
+    __shared__ float2 red[4][32];
+    __shared__ alignas(8) uint64_t x_landed[kMaxGroups][kMaxDepth], rest_landed[kMaxGroups][kMaxDepth];
+    const bool channel_gate = !GATED && p.gate && p.gate_step != 0;
+    const int packs = p.h / V, row_packs = packs * (XW + (GATED ? 2 : 1));
+    float *by_block = reinterpret_cast<float *>(smem + (size_t)groups * depth * row_packs), *by_gamma = by_block + p.h, *by_smooth = by_gamma + (p.gamma ? p.h : 0);
+    const int group = (int)threadIdx.x / threads, tid = (int)threadIdx.x - group * threads;
+    uint4 *all = smem + (size_t)group * depth * row_packs;
+    const uint32_t bytes = (uint32_t)packs * 16;
+    const auto expect = [](uint64_t *bar, uint32_t n) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory"); };
+    // by one thread, when all of the group have read what is there
+    const auto fetch_x = [&](long long row, int at) {
+        expect(&x_landed[group][at], bytes * XW);
+        bulk_copy(all + at * row_packs, static_cast<const X *>(p.x) + row * p.ld_x, bytes * XW, &x_landed[group][at]);
+    };
+    const auto fetch_rest = [&](long long row, int at) {
+        uint4 *to = all + at * row_packs + packs * XW;
+        expect(&rest_landed[group][at], bytes * (GATED ? 2 : 1));
+        bulk_copy(to, static_cast<const T *>(p.residual) + row * p.ld_residual, bytes, &rest_landed[group][at]);
+        if (GATED) bulk_copy(to + packs, static_cast<const T *>(p.gate) + row * p.ld_gate, bytes, &rest_landed[group][at]);
+    };
+    const long long step = (long long)gridDim.x * groups;
+    long long row = (long long)blockIdx.x * groups + group;
+    if (tid == 0) {
+        for (int d = 0; d < depth; ++d) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&x_landed[group][d])) : "memory");
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&rest_landed[group][d])) : "memory");
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        for (int d = 0; d < depth && row + d * step < p.rows; ++d) {
+            fetch_x(row + d * step, d);
+            fetch_rest(row + d * step, d);
+        }
+    }
+    for (int e = threadIdx.x; e < p.h; e += blockDim.x) {
+        float f = p.block_scale;
+        if (p.post_gamma) f = __fmul_rn(f, load_gamma<T>(p.post_gamma, p.gamma32, e));
+        if (channel_gate) f = __fmul_rn(f, gate_value(to_float<T>(static_cast<const T *>(p.gate)[e]), p.gate_act));
+        const int at = (e % V / 4 * packs + e / V) * 4 + e % 4;   // four floats of every pack together, so that a warp reads no bank twice
+        by_block[at] = f;
+        if (p.gamma) by_gamma[at] = load_gamma<T>(p.gamma, p.gamma32, e);
+        if (p.smooth) by_smooth[at] = p.smooth[e];
+    }
+    const auto has = [&](int i) { return EXACT || tid + i * threads < packs; };
+    const auto factors = [&](const float *from, int c, f32x2 *f) {
+#pragma unroll
+        for (int e = 0; e < V; e += 4) unpack<float>(reinterpret_cast<const uint4 *>(from)[e / 4 * packs + c], f + e / 2);
+    };
+    __syncthreads();
+    uint32_t phase = 0;
+    int at = 0;     // the buffer that the row is in
+    for (int parity = 0; row < p.rows; row += step, parity ^= 1) {
+        const long long next = row + depth * step;   // what comes in its place
+        const uint4 *mine = all + at * row_packs;
+        const auto give_up = [&] {   // never while the GPU is well; what there is to see of it is a row of NaN
+            if (tid == 0 && p.q) p.scale[row] = __int_as_float(0x7fffffff);
+            if (tid == 0 && p.residual_out) static_cast<T *>(p.residual_out)[row * p.ld_residual_out] = from_float<T>(__int_as_float(0x7fffffff));
+        };
+        // the block's output, and the norm behind it
+        f32x2 u[N][V / 2];
+        if (!mbar_wait(&x_landed[group][at], phase)) return give_up();
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < XW; ++j) unpack<X>(has(i) ? mine[(tid + i * threads) * XW + j] : make_uint4(0, 0, 0, 0), u[i] + j * (V / 2 / XW));
+        float factor = 1.0f;
+        if (p.post_gamma) {
+            f32x2 sum2 = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) sum2 = fma2(u[i][e], u[i][e], sum2);
+            const float2 parts = unpair2(sum2);
+            float sum = parts.x + parts.y, unused = 0.0f;
+            group_reduce(sum, unused, red[parity], group, threads);
+            factor = rsqrtf(__fmaf_rn(sum, p.inv_h, p.post_eps));
+        } else {
+            group_sync(group, threads);
+        }
+        if (tid == 0 && next < p.rows) fetch_x(next, at);
+        if (p.gate && p.gate_step == 0) factor = __fmul_rn(factor, gate_value(to_float<T>(static_cast<const T *>(p.gate)[row * p.ld_gate]), p.gate_act));
+
+        // the residual stream, and the sums of the next norm
+        if (!mbar_wait(&rest_landed[group][at], phase)) return give_up();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (!has(i)) break;
+            const int c = tid + i * threads;
+            f32x2 f[V / 2], r[V / 2];
+            factors(by_block, c, f);
+            unpack<T>(mine[packs * XW + c], r);
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) u[i][e] = mul2(u[i][e], mul2(f[e], pair2(factor, factor)));
+            if (GATED) {
+                unpack<T>(mine[packs * (XW + 1) + c], f);
+                if (p.gate_act != kGateNone) {
+#pragma unroll
+                    for (int e = 0; e < V / 2; ++e) {
+                        const float2 g = unpair2(f[e]);
+                        f[e] = pair2(gate_value(g.x, p.gate_act), gate_value(g.y, p.gate_act));
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) u[i][e] = mul2(u[i][e], f[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) u[i][e] = fma2(r[e], pair2(p.residual_scale, p.residual_scale), u[i][e]);
+        }
+        if (p.residual_out) {
+            uint4 *to = reinterpret_cast<uint4 *>(static_cast<T *>(p.residual_out) + row * p.ld_residual_out) + tid;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (has(i)) to[i * threads] = pack<T>(u[i]);
+        }
+        f32x2 sum2 = 0;
+        float mag = 0.0f;
+        if (p.gamma) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (!has(i)) break;
+                f32x2 f[V / 2];
+                factors(by_gamma, tid + i * threads, f);
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) {
+                    sum2 = fma2(u[i][e], u[i][e], sum2);
+                    u[i][e] = mul2(u[i][e], f[e]);
+                }
+            }
+        }
+        if (p.q) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (!has(i)) break;
+                f32x2 f[V / 2];
+                if (p.smooth) factors(by_smooth, tid + i * threads, f);
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) {
+                    const float2 v = unpair2(p.smooth ? mul2(u[i][e], f[e]) : u[i][e]);
+                    mag = max_mag(mag, v.x, v.y);
+                }
+            }
+        }
+        const float2 parts = unpair2(sum2);
+        float sum = parts.x + parts.y;
+        if (p.gamma) group_reduce(sum, mag, red[2 + parity], group, threads);
+        else group_sync(group, threads);
+        if (tid == 0 && next < p.rows) fetch_rest(next, at);
+        if (++at == depth) { at = 0; phase ^= 1; }
+        if (!p.gamma) continue;
+        const float r = rsqrtf(__fmaf_rn(sum, p.inv_h, p.eps));
+        if (p.normed_out) {
+            uint4 *normed = reinterpret_cast<uint4 *>(static_cast<T *>(p.normed_out) + row * p.ld_normed) + tid;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (!has(i)) break;
+                f32x2 y[V / 2];
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) y[e] = mul2(u[i][e], pair2(r, r));
+                normed[i * threads] = pack<T>(y);
+            }
+        }
+        if (!p.q) continue;
+        const float of_row = step_of(mag);
+        Quantiser quant;
+        quant.set(of_row);
+        if (tid == 0) p.scale[row] = of_row == 0.0f ? 0.0f : __fmul_rn(of_row, r);
+        const auto finish = [&](bool by_rcp) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = tid + i * threads;
+                if (!has(i)) break;
+                if (p.smooth) {
+                    f32x2 f[V / 2];
+                    factors(by_smooth, c, f);
+#pragma unroll
+                    for (int e = 0; e < V / 2; ++e) u[i][e] = mul2(u[i][e], f[e]);
+                }
+                uint32_t q[V / 4];
+#pragma unroll
+                for (int e = 0; e < V / 4; ++e) q[e] = quant.four(u[i] + 2 * e, by_rcp);
+                int8_t *to = p.q + row * p.ld_q + c * V;
+                if (V == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(q[0], q[V / 4 - 1]);
+                else *reinterpret_cast<uint32_t *>(to) = q[0];
+            }
+        };
+        if (quant.rcp != 0.0f) finish(true);
+        else finish(false);
+    }
+}
+
+// Threads of a group and groups of a CTA; 0 where a row does not fit.
+struct Groups {
+    int threads, groups, depth, smem;
+};
+template <typename T, typename X>
+Groups groups_of(const SandwichParams &p)
+{
+    constexpr int V = 16 / (int)sizeof(T), XW = (int)sizeof(X) * V / 16;
+    const int packs = p.h / V, most = group_threads_most(sizeof(T)), room = 224 * 1024;
+    Groups g;
+    g.threads = ((packs + kGroupPacks - 1) / kGroupPacks + 31) / 32 * 32;
+    const int factors = 4 * p.h * (1 + (p.gamma != nullptr) + (p.smooth != nullptr));
+    const int row = (XW + (p.gate && p.ld_gate && p.gate_step ? 2 : 1)) * 16 * packs;
+    g.groups = most / g.threads;
+    if (g.groups > kMaxGroups) g.groups = kMaxGroups;
+    if (g.groups > (room - factors) / row) g.groups = room > factors ? (room - factors) / row : 0;
+    g.depth = g.groups > 0 ? (room - factors) / (g.groups * row) : 0;   // rows of a group that there is room for
+    if (g.depth > kMaxDepth) g.depth = kMaxDepth;
+    g.smem = factors + g.groups * g.depth * row;
+    return g;
+}
+
 template <typename T, typename X, bool WHOLE>
 cudaError_t launch_packed(const SandwichParams &p, cudaStream_t stream)
 {
@@ -348,20 +623,44 @@ cudaError_t launch_packed(const SandwichParams &p, cudaStream_t stream)
     const int four = warps((packs + 3) / 4);
     if (packs <= 1024 && (p.rows <= 2 * 148 || packs <= 64)) {
         sandwich_kernel<T, X, 1, WHOLE, 1024, 1, false><<<p.rows, warps(packs), 0, stream>>>(p);
+        return cudaGetLastError();
+    }
+    int dev = 0;
+    cudaGetDevice(&dev);
+    // once per device; the attribute is idempotent, so a race only repeats the call
+    static unsigned long long done_mask = 0;
+    const bool first = !((done_mask >> (dev & 63)) & 1ull);
+    if constexpr (WHOLE) {
+        const Groups g = groups_of<T, X>(p);
+        if (g.groups > 0) {
+            const bool exact = packs == kGroupPacks * g.threads, gated = p.gate && p.ld_gate && p.gate_step;
+            const auto kernel = exact ? gated ? sandwich_rows_kernel<T, X, true, true> : sandwich_rows_kernel<T, X, true, false>
+                                : gated ? sandwich_rows_kernel<T, X, false, true> : sandwich_rows_kernel<T, X, false, false>;
+            const unsigned long long bit = 1ull << (dev & 63);
+            static unsigned long long done[4] = {};   // as above
+            unsigned long long &mask = done[2 * exact + gated];
+            if (!(mask & bit)) {
+                const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
+                if (e != cudaSuccess) return e;
+                mask |= bit;
+            }
+            const int ctas = (p.rows + g.groups - 1) / g.groups;
+            kernel<<<ctas < 148 ? ctas : 148, g.threads * g.groups, g.smem, stream>>>(p, g.threads, g.groups, g.depth);
+            return cudaGetLastError();
+        }
     } else if (packs <= 4 * 512) {
         const int smem = (XW + (p.gate && p.ld_gate && p.gate_step ? 2 : 1)) * 4 * 16 * four;
         const int fit = 1024 / four < 220 * 1024 / (smem + 2048) ? 1024 / four : 220 * 1024 / (smem + 2048);
         const auto kernel = sandwich_kernel<T, X, 4, WHOLE, 512, 2, true>;
-        static unsigned long long done_mask = 0;   // once per device; the attribute is idempotent, so a race only repeats the call
-        int dev = 0;
-        cudaGetDevice(&dev);
-        if (!((done_mask >> (dev & 63)) & 1ull)) {
+        if (first) {
             const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * 4 * 16 * 512);
             if (e != cudaSuccess) return e;
             done_mask |= 1ull << (dev & 63);
         }
         kernel<<<p.rows < 148 * fit ? p.rows : 148 * fit, four, smem, stream>>>(p);
-    } else if (packs <= 4 * 1024) {
+        return cudaGetLastError();
+    }
+    if (packs <= 4 * 1024) {
         sandwich_kernel<T, X, 4, WHOLE, 1024, 1, false><<<p.rows, four, 0, stream>>>(p);
     } else {
         sandwich_any_kernel<T, X><<<p.rows, 256, 0, stream>>>(p);
