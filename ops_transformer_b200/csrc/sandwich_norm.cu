@@ -103,268 +103,222 @@ __device__ __forceinline__ void load_channels(const void *vec, int at, int h, f3
     else unpack<G>(__ldg(reinterpret_cast<const uint4 *>(g + at)), f);
 }
 
+template <typename T, int V, bool WHOLE>
+__device__ __forceinline__ void load_gammas(const void *vec, bool gamma32, int at, int h, f32x2 *f)
+{
+    if (gamma32) load_channels<float, V, WHOLE>(vec, at, h, f);
+    else load_channels<T, V, WHOLE>(vec, at, h, f);
+}
+
 // One CTA per row; a thread holds NCH packs of V elements (16 bytes of T), blockDim.x apart, in fp32 from the first look at x to the last
 // store.  WHOLE: rows start on packs.  Else every row starts `lead` elements into one, the same in all tensors, and only what lies in a row's
 // first and last pack is masked and stored one element at a time.
-//
-// STREAM: the CTA takes every gridDim.x-th row.  While it works on one, the packs of the next are copied to shared memory, each by the
-// thread that will read it, x as soon as it is in registers and the rest behind the first reduction.
-template <typename T, typename X, int NCH, bool WHOLE, int MAXT, int MINB, bool STREAM>
+template <typename T, typename X, int NCH, bool WHOLE, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) sandwich_kernel(const SandwichParams p)
 {
-    constexpr int V = 16 / (int)sizeof(T), XW = (int)sizeof(X) * V / 16;   // loads of a pack of x
-    extern __shared__ uint4 ahead[];    // STREAM: [(XW + 1 or 2) * NCH][threads]: x, residual, gate
-    __shared__ float2 red[4][32];
+    constexpr int V = 16 / (int)sizeof(T);
+    __shared__ float2 red[2][32];
     const int threads = blockDim.x;
-    const uint32_t mine = STREAM ? (uint32_t)__cvta_generic_to_shared(ahead) + threadIdx.x * 16 : 0;
     const bool rows_gate = p.gate && p.ld_gate != 0 && p.gate_step != 0;
-    const auto lead_of = [&](long long row) { return WHOLE ? 0 : (int)((row * p.ld_x) & (V - 1)); };
-    // Elements from the row's first pack on that there are to read (see add_rms_norm_quant): a row's edge packs hold elements of its
-    // neighbours, which are read with it and dropped, but behind the last row's end there may be nothing.
-    const auto room_of = [&](long long row, int lead) {
-        long long ld = min(p.ld_x, p.ld_residual);
-        if (rows_gate) ld = min(ld, p.ld_gate);
-        return lead + p.h + (int)min((p.rows - 1 - row) * ld, 1024ll);
+    const long long row = blockIdx.x;
+    const int lead = WHOLE ? 0 : (int)((row * p.ld_x) & (V - 1)), end = lead + p.h, packs = (end + V - 1) / V;
+    // Elements from the row's first pack on that there are to read: a row's edge packs hold elements of its neighbours, which are read with it
+    // and dropped, but behind the last row's end there may be nothing.
+    const long long apart = min(min(p.ld_x, p.ld_residual), rows_gate ? p.ld_gate : p.ld_x);
+    const int room = end + (int)min((p.rows - 1 - row) * apart, 1024ll);
+    const X *x = static_cast<const X *>(p.x) + row * p.ld_x - lead;
+    const T *residual = static_cast<const T *>(p.residual) + row * p.ld_residual - lead, *gate = static_cast<const T *>(p.gate) + row * p.ld_gate - lead;
+    const auto full = [&](int c) { return WHOLE || (c * V >= lead && (c + 1) * V <= end); };
+    const auto inside = [&](int e) { return e >= lead && e < end; };
+    const auto load = [&](auto type, const auto *from, int c, f32x2 *f) {   // a pack of a row
+        typedef decltype(type) S;
+        constexpr int N = (int)sizeof(S) * V / 16;
+        if (!WHOLE && (c + 1) * V > room) {
+            const auto one = [&](int e) { return inside(e) ? to_float<S>(from[e]) : 0.0f; };
+#pragma unroll
+            for (int e = 0; e < V; e += 2) f[e / 2] = pair2(one(c * V + e), one(c * V + e + 1));
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) unpack<S>(*(reinterpret_cast<const uint4 *>(from + (long long)c * V) + j), f + j * (V / 2 / N));
     };
-    const auto slot = [&](int s) { return mine + (uint32_t)(s * threads) * 16; };
-    const auto copy = [&](int s, const void *from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot(s)), "l"(from) : "memory"); };
-    const auto there = [&](int c, int lead, int room) { return WHOLE ? c * V < p.h : c * V < lead + p.h && (c + 1) * V <= room; };
-    const auto fetch_x = [&](long long row) {
-        const int lead = lead_of(row), room = room_of(row, lead);
-        const X *x = static_cast<const X *>(p.x) + row * p.ld_x - lead;
+    const auto mask = [&](int c, f32x2 *f) {
+        if (full(c)) return;
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int c = threadIdx.x + i * threads;
-            if (!there(c, lead, room)) continue;
-#pragma unroll
-            for (int j = 0; j < XW; ++j) copy(i * XW + j, reinterpret_cast<const uint4 *>(x + (long long)c * V) + j);
+        for (int e = 0; e < V; e += 2) {
+            const float2 v = unpair2(f[e / 2]);
+            f[e / 2] = pair2(inside(c * V + e) ? v.x : 0.0f, inside(c * V + e + 1) ? v.y : 0.0f);
         }
     };
-    const auto fetch_rest = [&](long long row, int i) {
-        const int lead = lead_of(row), room = room_of(row, lead), c = threadIdx.x + i * threads;
-        if (!there(c, lead, room)) return;
-        copy(NCH * XW + i, static_cast<const T *>(p.residual) + row * p.ld_residual - lead + (long long)c * V);
-        if (rows_gate) copy(NCH * (XW + 1) + i, static_cast<const T *>(p.gate) + row * p.ld_gate - lead + (long long)c * V);
-    };
-    const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
-    const auto await_older = [] { asm volatile("cp.async.wait_group 1;" ::: "memory"); };
-    if (STREAM) {
-        fetch_x(blockIdx.x);
-        commit();
+    const auto gammas = [&](const void *g, int c, f32x2 *f) { load_gammas<T, V, WHOLE>(g, p.gamma32, c * V - lead, p.h, f); };
+    const auto store = [&](T *to, int c, const f32x2 *f) {
+        if (full(c)) {
+            *reinterpret_cast<uint4 *>(to + (long long)c * V) = pack<T>(f);
+            return;
+        }
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) fetch_rest(blockIdx.x, i);
-        commit();
+        for (int e = 0; e < V; ++e)
+            if (inside(c * V + e)) to[c * V + e] = from_float<T>(element(f, e));
+    };
+
+    // the block's output, and the norm behind it
+    f32x2 u[NCH][V / 2];
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        const int c = threadIdx.x + i * threads;
+        if (c >= packs) break;
+        load(X(), x, c, u[i]);
+        mask(c, u[i]);
     }
-    int parity = 0;
-    for (long long row = blockIdx.x; row < p.rows; row += STREAM ? (long long)gridDim.x : (long long)p.rows) {
-        const long long next = row + gridDim.x;
-        const int lead = lead_of(row), end = lead + p.h, room = room_of(row, lead), packs = (end + V - 1) / V;
-        const X *x = static_cast<const X *>(p.x) + row * p.ld_x - lead;
-        const T *residual = static_cast<const T *>(p.residual) + row * p.ld_residual - lead, *gate = static_cast<const T *>(p.gate) + row * p.ld_gate - lead;
-        const auto full = [&](int c) { return WHOLE || (c * V >= lead && (c + 1) * V <= end); };
-        const auto inside = [&](int e) { return e >= lead && e < end; };
-        // a pack of a row of S: N loads of it, out of the slots from s on
-        const auto load = [&](auto type, const auto *from, int c, int s, f32x2 *f) {
-            typedef decltype(type) S;
-            constexpr int N = (int)sizeof(S) * V / 16;
-            if (!WHOLE && (c + 1) * V > room) {
-                const auto one = [&](int e) { return inside(e) ? to_float<S>(from[e]) : 0.0f; };
-#pragma unroll
-                for (int e = 0; e < V; e += 2) f[e / 2] = pair2(one(c * V + e), one(c * V + e + 1));
-                return;
-            }
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                uint4 u;
-                if (STREAM) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(slot(s + j)) : "memory");
-                else u = *(reinterpret_cast<const uint4 *>(from + (long long)c * V) + j);
-                unpack<S>(u, f + j * (V / 2 / N));
-            }
-        };
-        const auto mask = [&](int c, f32x2 *f) {
-            if (full(c)) return;
-#pragma unroll
-            for (int e = 0; e < V; e += 2) {
-                const float2 v = unpair2(f[e / 2]);
-                f[e / 2] = pair2(inside(c * V + e) ? v.x : 0.0f, inside(c * V + e + 1) ? v.y : 0.0f);
-            }
-        };
-        const auto gammas = [&](const void *g, int c, f32x2 *f) {
-            if (p.gamma32) load_channels<float, V, WHOLE>(g, c * V - lead, p.h, f);
-            else load_channels<T, V, WHOLE>(g, c * V - lead, p.h, f);
-        };
-        const auto store = [&](T *to, int c, const f32x2 *f) {
-            if (full(c)) {
-                *reinterpret_cast<uint4 *>(to + (long long)c * V) = pack<T>(f);
-                return;
-            }
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-                if (inside(c * V + e)) to[c * V + e] = from_float<T>(element(f, e));
-        };
-
-        // the block's output, and the norm behind it
-        f32x2 u[NCH][V / 2];
-        if (STREAM) await_older();
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int c = threadIdx.x + i * threads;
-            if (c >= packs) break;
-            load(X(), x, c, i * XW, u[i]);
-            mask(c, u[i]);
-        }
-        if (STREAM) {
-            if (next < p.rows) fetch_x(next);   // the thread has read what this fills
-            commit();
-        }
-        float factor = p.block_scale;
-        if (p.post_gamma) {
-            f32x2 sum2 = 0;
-#pragma unroll
-            for (int i = 0; i < NCH; ++i) {
-                if (threadIdx.x + i * threads >= packs) break;
-#pragma unroll
-                for (int e = 0; e < V / 2; ++e) sum2 = fma2(u[i][e], u[i][e], sum2);
-            }
-            const float2 parts = unpair2(sum2);
-            float sum = parts.x + parts.y, unused = 0.0f;
-            block_reduce(sum, unused, red[parity]);
-            factor = __fmul_rn(factor, rsqrtf(__fmaf_rn(sum, p.inv_h, p.post_eps)));
-        }
-        if (p.gate && p.gate_step == 0) factor = __fmul_rn(factor, gate_value(to_float<T>(static_cast<const T *>(p.gate)[row * p.ld_gate]), p.gate_act));
-
-        // the residual stream, and the sums of the next norm
-        if (STREAM) await_older();
+    float factor = p.block_scale;
+    if (p.post_gamma) {
         f32x2 sum2 = 0;
-        float mag = 0.0f;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
-            const int c = threadIdx.x + i * threads;
-            if (c >= packs) break;
-            f32x2 f[V / 2];
-#pragma unroll
-            for (int e = 0; e < V / 2; ++e) u[i][e] = mul2(u[i][e], pair2(factor, factor));
-            if (p.post_gamma) {
-                gammas(p.post_gamma, c, f);
-#pragma unroll
-                for (int e = 0; e < V / 2; ++e) u[i][e] = mul2(u[i][e], f[e]);
-            }
-            if (p.gate && p.gate_step != 0) {
-                if (rows_gate) load(T(), gate, c, NCH * (XW + 1) + i, f);
-                else load_channels<T, V, WHOLE>(p.gate, c * V - lead, p.h, f);
-                if (p.gate_act != kGateNone) {
-#pragma unroll
-                    for (int e = 0; e < V / 2; ++e) {
-                        const float2 g = unpair2(f[e]);
-                        f[e] = pair2(gate_value(g.x, p.gate_act), gate_value(g.y, p.gate_act));
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < V / 2; ++e) u[i][e] = mul2(u[i][e], f[e]);
-            }
-            load(T(), residual, c, NCH * XW + i, f);
-#pragma unroll
-            for (int e = 0; e < V / 2; ++e) u[i][e] = fma2(f[e], pair2(p.residual_scale, p.residual_scale), u[i][e]);
-            mask(c, u[i]);
-            if (p.residual_out) store(static_cast<T *>(p.residual_out) + row * p.ld_residual_out - lead, c, u[i]);
-            if (!p.gamma) continue;
+            if (threadIdx.x + i * threads >= packs) break;
 #pragma unroll
             for (int e = 0; e < V / 2; ++e) sum2 = fma2(u[i][e], u[i][e], sum2);
-            gammas(p.gamma, c, f);
+        }
+        const float2 parts = unpair2(sum2);
+        float sum = parts.x + parts.y, unused = 0.0f;
+        block_reduce(sum, unused, red[0]);
+        factor = __fmul_rn(factor, rsqrtf(__fmaf_rn(sum, p.inv_h, p.post_eps)));
+    }
+    if (p.gate && p.gate_step == 0) factor = __fmul_rn(factor, gate_value(to_float<T>(static_cast<const T *>(p.gate)[row * p.ld_gate]), p.gate_act));
+
+    // the residual stream, and the sums of the next norm
+    f32x2 sum2 = 0;
+    float mag = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) {
+        const int c = threadIdx.x + i * threads;
+        if (c >= packs) break;
+        f32x2 f[V / 2];
+#pragma unroll
+        for (int e = 0; e < V / 2; ++e) u[i][e] = mul2(u[i][e], pair2(factor, factor));
+        if (p.post_gamma) {
+            gammas(p.post_gamma, c, f);
 #pragma unroll
             for (int e = 0; e < V / 2; ++e) u[i][e] = mul2(u[i][e], f[e]);
-            if (!p.q) continue;
+        }
+        if (p.gate && p.gate_step != 0) {
+            if (rows_gate) load(T(), gate, c, f);
+            else load_channels<T, V, WHOLE>(p.gate, c * V - lead, p.h, f);
+            if (p.gate_act != kGateNone) {
 #pragma unroll
-            for (int e = 0; e < V / 2; ++e) f[e] = u[i][e];
+                for (int e = 0; e < V / 2; ++e) {
+                    const float2 g = unpair2(f[e]);
+                    f[e] = pair2(gate_value(g.x, p.gate_act), gate_value(g.y, p.gate_act));
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) u[i][e] = mul2(u[i][e], f[e]);
+        }
+        load(T(), residual, c, f);
+#pragma unroll
+        for (int e = 0; e < V / 2; ++e) u[i][e] = fma2(f[e], pair2(p.residual_scale, p.residual_scale), u[i][e]);
+        mask(c, u[i]);
+        if (p.residual_out) store(static_cast<T *>(p.residual_out) + row * p.ld_residual_out - lead, c, u[i]);
+        if (!p.gamma) continue;
+#pragma unroll
+        for (int e = 0; e < V / 2; ++e) sum2 = fma2(u[i][e], u[i][e], sum2);
+        gammas(p.gamma, c, f);
+#pragma unroll
+        for (int e = 0; e < V / 2; ++e) u[i][e] = mul2(u[i][e], f[e]);
+        if (!p.q) continue;
+#pragma unroll
+        for (int e = 0; e < V / 2; ++e) f[e] = u[i][e];
+        if (p.smooth) {
+            f32x2 m[V / 2];
+            load_channels<float, V, WHOLE>(p.smooth, c * V - lead, p.h, m);
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) f[e] = mul2(f[e], m[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < V / 2; ++e) {
+            const float2 v = unpair2(f[e]);
+            mag = max_mag(mag, v.x, v.y);
+        }
+    }
+    if (p.gamma) {
+        const float2 parts = unpair2(sum2);
+        float sum = parts.x + parts.y;
+        block_reduce(sum, mag, red[1]);
+        const float r = rsqrtf(__fmaf_rn(sum, p.inv_h, p.eps)), step = step_of(mag);
+        Quantiser quant;
+        quant.set(step);
+        if (p.q && threadIdx.x == 0) p.scale[row] = step == 0.0f ? 0.0f : __fmul_rn(step, r);
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int c = threadIdx.x + i * threads;
+            if (c >= packs) break;
+            if (p.normed_out) {
+                f32x2 y[V / 2];
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) y[e] = mul2(u[i][e], pair2(r, r));
+                store(static_cast<T *>(p.normed_out) + row * p.ld_normed - lead, c, y);
+            }
+            if (!p.q) continue;
             if (p.smooth) {
                 f32x2 m[V / 2];
                 load_channels<float, V, WHOLE>(p.smooth, c * V - lead, p.h, m);
 #pragma unroll
-                for (int e = 0; e < V / 2; ++e) f[e] = mul2(f[e], m[e]);
+                for (int e = 0; e < V / 2; ++e) u[i][e] = mul2(u[i][e], m[e]);
             }
+            uint32_t q[V / 4];
 #pragma unroll
-            for (int e = 0; e < V / 2; ++e) {
-                const float2 v = unpair2(f[e]);
-                mag = max_mag(mag, v.x, v.y);
-            }
-        }
-        if (STREAM) {
+            for (int e = 0; e < V / 4; ++e) q[e] = quant.four(u[i] + 2 * e, quant.rcp != 0.0f);
+            int8_t *to = p.q + row * p.ld_q - lead + (long long)c * V;
+            if (full(c)) {
+                if (V == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(q[0], q[V / 4 - 1]);
+                else *reinterpret_cast<uint32_t *>(to) = q[0];
+            } else {
 #pragma unroll
-            for (int i = 0; i < NCH; ++i)
-                if (next < p.rows) fetch_rest(next, i);
-            commit();
-        }
-        if (p.gamma) {
-            const float2 parts = unpair2(sum2);
-            float sum = parts.x + parts.y;
-            block_reduce(sum, mag, red[2 + parity]);
-            const float r = rsqrtf(__fmaf_rn(sum, p.inv_h, p.eps)), step = step_of(mag);
-            Quantiser quant;
-            quant.set(step);
-            if (p.q && threadIdx.x == 0) p.scale[row] = step == 0.0f ? 0.0f : __fmul_rn(step, r);
-#pragma unroll
-            for (int i = 0; i < NCH; ++i) {
-                const int c = threadIdx.x + i * threads;
-                if (c >= packs) break;
-                if (p.normed_out) {
-                    f32x2 y[V / 2];
-#pragma unroll
-                    for (int e = 0; e < V / 2; ++e) y[e] = mul2(u[i][e], pair2(r, r));
-                    store(static_cast<T *>(p.normed_out) + row * p.ld_normed - lead, c, y);
-                }
-                if (!p.q) continue;
-                if (p.smooth) {
-                    f32x2 m[V / 2];
-                    load_channels<float, V, WHOLE>(p.smooth, c * V - lead, p.h, m);
-#pragma unroll
-                    for (int e = 0; e < V / 2; ++e) u[i][e] = mul2(u[i][e], m[e]);
-                }
-                uint32_t q[V / 4];
-#pragma unroll
-                for (int e = 0; e < V / 4; ++e) q[e] = quant.four(u[i] + 2 * e, quant.rcp != 0.0f);
-                int8_t *to = p.q + row * p.ld_q - lead + (long long)c * V;
-                if (full(c)) {
-                    if (V == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(q[0], q[V / 4 - 1]);
-                    else *reinterpret_cast<uint32_t *>(to) = q[0];
-                } else {
-#pragma unroll
-                    for (int e = 0; e < V; ++e)
-                        if (inside(c * V + e)) to[e] = (int8_t)(q[e / 4] >> (e % 4 * 8));
-                }
+                for (int e = 0; e < V; ++e)
+                    if (inside(c * V + e)) to[e] = (int8_t)(q[e / 4] >> (e % 4 * 8));
             }
         }
-        parity ^= 1;
     }
 }
 
-// Many rows that start on packs: one CTA per SM, in which groups of threads take a row each.  What multiplies the channels is laid out once
-// in shared memory, in fp32 and with everything folded in that a row does not change (the norm's weight, the activated gate, the block's
-// scale), so that a row's turn has no loads but its own.  Those come as one bulk copy a tensor, for the next row as soon as the group holds
-// this one in registers.  (With a 16-byte cp.async for each pack, the form of the other kernels, an SM takes in 16 bytes per ns however many
-// are under way: 4096 x 7168 in 80 us.)  A group's threads hold four packs each.
+
+// Many rows: one CTA per SM, in which groups of threads take a row each.  What multiplies the channels is laid out once in shared memory, in
+// fp32 and with everything folded in that a row does not change (the norm's weight, the activated gate, the block's scale), so that a row's
+// turn has no loads but its own.  Those come as one bulk copy a tensor, for the next row as soon as the group holds this one in registers.
+// (With a 16-byte cp.async for each pack an SM takes in 16 bytes per ns however many are under way: 4096 x 7168 in 80 us.)  A group's
+// threads hold two packs each; four would leave too few rows in turn for the chain load, sum, load, sum, store of each.
+// 4096 x 7168, fp32 x, bf16 stream: 53.6 us with int8 rows (270 MB, 4.9 TB/s), 49.7 with bf16 rows and a gate (294 MB, 5.9 TB/s); 5001
+// channels, whose rows begin anywhere, 53.8.  Quantising costs what the difference is: max, step and rounding are the issue slots' work.
 constexpr int kGroupPacks = 2, kMaxGroups = 14, kMaxDepth = 3;    // of the 15 named barriers that are left
 constexpr long long kWaitLimitCycles = 1ll << 31;  // about a second
-__host__ __device__ constexpr int group_threads_most(int elem) { return 1024; }
+constexpr int kGroupThreads = 1024;
+// Packs that a row can touch, and floats of a vector of factors.
+template <int V, bool WHOLE> __host__ __device__ inline int most_packs(int h) { return WHOLE ? h / V : (h + 2 * V - 2) / V; }
+template <int V, bool WHOLE> __host__ __device__ inline int factor_floats(int h) { return WHOLE ? h : V * (most_packs<V, WHOLE>(h) + 2); }
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-// Bounded: false when the copies have not come.
-__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity)
+__device__ __forceinline__ bool mbar_try(uint64_t *bar, uint32_t parity)
 {
-    uint32_t ok = 0;
-    const long long t0 = clock64();
-    while (true) {
-        asm volatile(
-            "{\n"
-            ".reg .pred p;\n"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-            "selp.u32 %0, 1, 0, p;\n"
-            "}\n"
-            : "=r"(ok)
-            : "r"(smem_u32(bar)), "r"(parity)
-            : "memory");
-        if (ok) return true;
-        if (clock64() - t0 > kWaitLimitCycles) return false;
-    }
+    uint32_t ok;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok;
+}
+// Bounded: false when the copies have not come, and once that has been so, without waiting a second time.
+__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volatile int *late)
+{
+    if (mbar_try(bar, parity)) return true;
+    for (const long long t0 = clock64(); !*late && clock64() - t0 <= kWaitLimitCycles;)
+        if (mbar_try(bar, parity)) return true;
+    *late = 1;
+    return false;
 }
 __device__ __forceinline__ void bulk_copy(void *to, const void *from, uint32_t bytes, uint64_t *bar)
 {
@@ -395,31 +349,42 @@ __device__ __forceinline__ void group_reduce(float &sum, float &mag, float2 *red
     mag = __uint_as_float(m);
 }
 
-// EXACT: every thread of a group has all of its packs.  GATED: a gate for each element.
-template <typename T, typename X, bool EXACT, bool GATED>
-__global__ void __launch_bounds__(group_threads_most(sizeof(T)), 1) sandwich_rows_kernel(const SandwichParams p, int threads, int groups, int depth)
+// WHOLE as above; EXACT: every thread of a group has all of its packs; GATED: a gate for each element.
+template <typename T, typename X, bool WHOLE, bool EXACT, bool GATED>
+__global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const SandwichParams p, int threads, int groups, int depth)
 {
     constexpr int V = 16 / (int)sizeof(T), XW = (int)sizeof(X) * V / 16, N = kGroupPacks;
-    extern __shared__ uint4 smem[];     // the groups' rows (x, residual, gate); block's, next norm's and smoothing's factors [h]
+    extern __shared__ uint4 smem[];     // the groups' rows (x, residual, gate); block's, next norm's and smoothing's factors
     __shared__ float2 red[4][32];
     __shared__ alignas(8) uint64_t x_landed[kMaxGroups][kMaxDepth], rest_landed[kMaxGroups][kMaxDepth];
+    __shared__ volatile int late;   // a wait has run out, which none does while the GPU is well: what there is to see of it are rows of NaN
+    const float nan = __int_as_float(0x7fffffff);
+    if (threadIdx.x == 0) late = 0;
     const bool channel_gate = !GATED && p.gate && p.gate_step != 0;
-    const int packs = p.h / V, row_packs = packs * (XW + (GATED ? 2 : 1));
-    float *by_block = reinterpret_cast<float *>(smem + (size_t)groups * depth * row_packs), *by_gamma = by_block + p.h, *by_smooth = by_gamma + (p.gamma ? p.h : 0);
+    const int most = most_packs<V, WHOLE>(p.h), row_packs = most * (XW + (GATED ? 2 : 1)), plane = most + 2, vec = factor_floats<V, WHOLE>(p.h);
+    float *by_block = reinterpret_cast<float *>(smem + (size_t)groups * depth * row_packs), *by_gamma = by_block + vec, *by_smooth = by_gamma + (p.gamma ? vec : 0);
     const int group = (int)threadIdx.x / threads, tid = (int)threadIdx.x - group * threads;
     uint4 *all = smem + (size_t)group * depth * row_packs;
-    const uint32_t bytes = (uint32_t)packs * 16;
-    const auto expect = [](uint64_t *bar, uint32_t n) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory"); };
-    // by one thread, when all of the group have read what is there
+    const auto lead_of = [&](long long row) { return WHOLE ? 0 : (int)((row * p.ld_x) & (V - 1)); };
+    // A row from the pack on in which it begins, to the 16 bytes in which it ends (which lie in the row's own memory pages, whatever else is
+    // in them).  By one thread, when all of the group have read what is there.
+    const auto fetch = [&](const auto *from, long long row, long long ld, uint4 *to, uint64_t *bar) {
+        const int lead = lead_of(row);
+        bulk_copy(to, from + row * ld - lead, ((lead + p.h) * (uint32_t)sizeof(*from) + 15) / 16 * 16, bar);
+    };
+    const auto expect = [&](uint64_t *bar, long long row, int bytes, int n) {   // n rows of elements of so many bytes
+        const uint32_t all = ((lead_of(row) + p.h) * (uint32_t)bytes + 15) / 16 * 16 * n;
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(all) : "memory");
+    };
     const auto fetch_x = [&](long long row, int at) {
-        expect(&x_landed[group][at], bytes * XW);
-        bulk_copy(all + at * row_packs, static_cast<const X *>(p.x) + row * p.ld_x, bytes * XW, &x_landed[group][at]);
+        expect(&x_landed[group][at], row, sizeof(X), 1);
+        fetch(static_cast<const X *>(p.x), row, p.ld_x, all + at * row_packs, &x_landed[group][at]);
     };
     const auto fetch_rest = [&](long long row, int at) {
-        uint4 *to = all + at * row_packs + packs * XW;
-        expect(&rest_landed[group][at], bytes * (GATED ? 2 : 1));
-        bulk_copy(to, static_cast<const T *>(p.residual) + row * p.ld_residual, bytes, &rest_landed[group][at]);
-        if (GATED) bulk_copy(to + packs, static_cast<const T *>(p.gate) + row * p.ld_gate, bytes, &rest_landed[group][at]);
+        uint4 *to = all + at * row_packs + most * XW;
+        expect(&rest_landed[group][at], row, sizeof(T), GATED ? 2 : 1);
+        fetch(static_cast<const T *>(p.residual), row, p.ld_residual, to, &rest_landed[group][at]);
+        if (GATED) fetch(static_cast<const T *>(p.gate), row, p.ld_gate, to + most, &rest_landed[group][at]);
     };
     const long long step = (long long)gridDim.x * groups;
     long long row = (long long)blockIdx.x * groups + group;
@@ -434,37 +399,94 @@ __global__ void __launch_bounds__(group_threads_most(sizeof(T)), 1) sandwich_row
             fetch_rest(row + d * step, d);
         }
     }
-    for (int e = threadIdx.x; e < p.h; e += blockDim.x) {
-        float f = p.block_scale;
-        if (p.post_gamma) f = __fmul_rn(f, load_gamma<T>(p.post_gamma, p.gamma32, e));
-        if (channel_gate) f = __fmul_rn(f, gate_value(to_float<T>(static_cast<const T *>(p.gate)[e]), p.gate_act));
-        const int at = (e % V / 4 * packs + e / V) * 4 + e % 4;   // four floats of every pack together, so that a warp reads no bank twice
-        by_block[at] = f;
-        if (p.gamma) by_gamma[at] = load_gamma<T>(p.gamma, p.gamma32, e);
-        if (p.smooth) by_smooth[at] = p.smooth[e];
-    }
-    const auto has = [&](int i) { return EXACT || tid + i * threads < packs; };
-    const auto factors = [&](const float *from, int c, f32x2 *f) {
+    // The factors, so that a warp reads no bank twice.  WHOLE: four floats of every pack together.  Else, since a pack begins at any channel,
+    // every V-th channel together, a zero before and behind, for the packs that reach beyond a row's ends.
+    const auto place = [&](float *to, int c, const f32x2 *f) {
+        if constexpr (WHOLE) {
 #pragma unroll
-        for (int e = 0; e < V; e += 4) unpack<float>(reinterpret_cast<const uint4 *>(from)[e / 4 * packs + c], f + e / 2);
+            for (int e = 0; e < V; e += 4) {
+                const float2 u = unpair2(f[e / 2]), v = unpair2(f[e / 2 + 1]);
+                reinterpret_cast<float4 *>(to)[e / 4 * most + c] = make_float4(u.x, u.y, v.x, v.y);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) to[e * plane + c + 1] = element(f, e);
+        }
     };
+    for (int c = (int)threadIdx.x - (WHOLE ? 0 : 1); c < (WHOLE ? most : plane - 1); c += blockDim.x) {
+        f32x2 post[V / 2], g[V / 2], gamma[V / 2], smooth[V / 2];
+#pragma unroll
+        for (int e = 0; e < V / 2; ++e) post[e] = g[e] = pair2(1.0f, 1.0f);
+        if (p.post_gamma) load_gammas<T, V, WHOLE>(p.post_gamma, p.gamma32, c * V, p.h, post);
+        if (channel_gate) load_channels<T, V, WHOLE>(p.gate, c * V, p.h, g);
+        if (p.gamma) load_gammas<T, V, WHOLE>(p.gamma, p.gamma32, c * V, p.h, gamma);
+        if (p.smooth) load_channels<float, V, WHOLE>(p.smooth, c * V, p.h, smooth);
+        if (p.gamma) place(by_gamma, c, gamma);
+        if (p.smooth) place(by_smooth, c, smooth);
+        if (channel_gate && p.gate_act != kGateNone) {
+#pragma unroll
+            for (int e = 0; e < V / 2; ++e) {
+                const float2 v = unpair2(g[e]);
+                g[e] = pair2(gate_value(v.x, p.gate_act), gate_value(v.y, p.gate_act));
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < V / 2; ++e) {
+            post[e] = mul2(mul2(post[e], pair2(p.block_scale, p.block_scale)), g[e]);
+            const float2 v = unpair2(post[e]);
+            if (!WHOLE) post[e] = pair2((unsigned)(c * V + 2 * e) < (unsigned)p.h ? v.x : 0.0f, (unsigned)(c * V + 2 * e + 1) < (unsigned)p.h ? v.y : 0.0f);
+        }
+        place(by_block, c, post);
+    }
     __syncthreads();
     uint32_t phase = 0;
     int at = 0;     // the buffer that the row is in
     for (int parity = 0; row < p.rows; row += step, parity ^= 1) {
         const long long next = row + depth * step;   // what comes in its place
         const uint4 *mine = all + at * row_packs;
-        const auto give_up = [&] {   // never while the GPU is well; what there is to see of it is a row of NaN
-            if (tid == 0 && p.q) p.scale[row] = __int_as_float(0x7fffffff);
-            if (tid == 0 && p.residual_out) static_cast<T *>(p.residual_out)[row * p.ld_residual_out] = from_float<T>(__int_as_float(0x7fffffff));
+        const int lead = lead_of(row), packs = WHOLE ? most : (lead + p.h + V - 1) / V;
+        const auto has = [&](int i) { return EXACT || tid + i * threads < packs; };
+        const auto full = [&](int c) { return WHOLE || (c * V >= lead && (c + 1) * V <= lead + p.h); };
+        const auto inside = [&](int e) { return e >= lead && e < lead + p.h; };
+        const auto mask = [&](int c, f32x2 *f) {
+            if (full(c)) return;
+#pragma unroll
+            for (int e = 0; e < V; e += 2) {
+                const float2 v = unpair2(f[e / 2]);
+                f[e / 2] = pair2(inside(c * V + e) ? v.x : 0.0f, inside(c * V + e + 1) ? v.y : 0.0f);
+            }
         };
+        const auto factors = [&](const float *from, int c, f32x2 *f) {
+            if constexpr (WHOLE) {
+#pragma unroll
+                for (int e = 0; e < V; e += 4) unpack<float>(reinterpret_cast<const uint4 *>(from)[e / 4 * most + c], f + e / 2);
+            } else {
+                const auto one = [&](int j) { return from[((j - lead) & (V - 1)) * plane + c + 1 - (j < lead)]; };
+#pragma unroll
+                for (int e = 0; e < V; e += 2) f[e / 2] = pair2(one(e), one(e + 1));
+            }
+        };
+        const auto store = [&](T *to, int c, const f32x2 *f) {
+            if (full(c)) {
+                *reinterpret_cast<uint4 *>(to + c * V) = pack<T>(f);
+                return;
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (inside(c * V + e)) to[c * V + e] = from_float<T>(element(f, e));
+        };
+
         // the block's output, and the norm behind it
         f32x2 u[N][V / 2];
-        if (!mbar_wait(&x_landed[group][at], phase)) return give_up();
+        const bool x_here = mbar_wait(&x_landed[group][at], phase, &late);
 #pragma unroll
-        for (int i = 0; i < N; ++i)
+        for (int i = 0; i < N; ++i) {
+            const int c = tid + i * threads;
 #pragma unroll
-            for (int j = 0; j < XW; ++j) unpack<X>(has(i) ? mine[(tid + i * threads) * XW + j] : make_uint4(0, 0, 0, 0), u[i] + j * (V / 2 / XW));
+            for (int j = 0; j < XW; ++j) unpack<X>(has(i) ? mine[c * XW + j] : make_uint4(0, 0, 0, 0), u[i] + j * (V / 2 / XW));
+            if (has(i)) mask(c, u[i]);
+        }
+        if (!x_here) u[0][0] = pair2(nan, nan);
         float factor = 1.0f;
         if (p.post_gamma) {
             f32x2 sum2 = 0;
@@ -475,26 +497,26 @@ __global__ void __launch_bounds__(group_threads_most(sizeof(T)), 1) sandwich_row
             const float2 parts = unpair2(sum2);
             float sum = parts.x + parts.y, unused = 0.0f;
             group_reduce(sum, unused, red[parity], group, threads);
-            factor = rsqrtf(__fmaf_rn(sum, p.inv_h, p.post_eps));
+            factor = __fmul_rn(factor, rsqrtf(__fmaf_rn(sum, p.inv_h, p.post_eps)));
         } else {
             group_sync(group, threads);
         }
-        if (tid == 0 && next < p.rows) fetch_x(next, at);
+        if (tid == 0 && next < p.rows && !late) fetch_x(next, at);
         if (p.gate && p.gate_step == 0) factor = __fmul_rn(factor, gate_value(to_float<T>(static_cast<const T *>(p.gate)[row * p.ld_gate]), p.gate_act));
 
         // the residual stream, and the sums of the next norm
-        if (!mbar_wait(&rest_landed[group][at], phase)) return give_up();
+        const bool rest_here = mbar_wait(&rest_landed[group][at], phase, &late);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             if (!has(i)) break;
             const int c = tid + i * threads;
             f32x2 f[V / 2], r[V / 2];
             factors(by_block, c, f);
-            unpack<T>(mine[packs * XW + c], r);
+            unpack<T>(mine[most * XW + c], r);
 #pragma unroll
             for (int e = 0; e < V / 2; ++e) u[i][e] = mul2(u[i][e], mul2(f[e], pair2(factor, factor)));
             if (GATED) {
-                unpack<T>(mine[packs * (XW + 1) + c], f);
+                unpack<T>(mine[most * (XW + 1) + c], f);
                 if (p.gate_act != kGateNone) {
 #pragma unroll
                     for (int e = 0; e < V / 2; ++e) {
@@ -507,12 +529,13 @@ __global__ void __launch_bounds__(group_threads_most(sizeof(T)), 1) sandwich_row
             }
 #pragma unroll
             for (int e = 0; e < V / 2; ++e) u[i][e] = fma2(r[e], pair2(p.residual_scale, p.residual_scale), u[i][e]);
+            mask(c, u[i]);
         }
+        if (!rest_here) u[0][0] = pair2(nan, nan);
         if (p.residual_out) {
-            uint4 *to = reinterpret_cast<uint4 *>(static_cast<T *>(p.residual_out) + row * p.ld_residual_out) + tid;
 #pragma unroll
             for (int i = 0; i < N; ++i)
-                if (has(i)) to[i * threads] = pack<T>(u[i]);
+                if (has(i)) store(static_cast<T *>(p.residual_out) + row * p.ld_residual_out - lead, tid + i * threads, u[i]);
         }
         f32x2 sum2 = 0;
         float mag = 0.0f;
@@ -546,19 +569,18 @@ __global__ void __launch_bounds__(group_threads_most(sizeof(T)), 1) sandwich_row
         float sum = parts.x + parts.y;
         if (p.gamma) group_reduce(sum, mag, red[2 + parity], group, threads);
         else group_sync(group, threads);
-        if (tid == 0 && next < p.rows) fetch_rest(next, at);
+        if (tid == 0 && next < p.rows && !late) fetch_rest(next, at);
         if (++at == depth) { at = 0; phase ^= 1; }
         if (!p.gamma) continue;
         const float r = rsqrtf(__fmaf_rn(sum, p.inv_h, p.eps));
         if (p.normed_out) {
-            uint4 *normed = reinterpret_cast<uint4 *>(static_cast<T *>(p.normed_out) + row * p.ld_normed) + tid;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 if (!has(i)) break;
                 f32x2 y[V / 2];
 #pragma unroll
                 for (int e = 0; e < V / 2; ++e) y[e] = mul2(u[i][e], pair2(r, r));
-                normed[i * threads] = pack<T>(y);
+                store(static_cast<T *>(p.normed_out) + row * p.ld_normed - lead, tid + i * threads, y);
             }
         }
         if (!p.q) continue;
@@ -580,9 +602,15 @@ __global__ void __launch_bounds__(group_threads_most(sizeof(T)), 1) sandwich_row
                 uint32_t q[V / 4];
 #pragma unroll
                 for (int e = 0; e < V / 4; ++e) q[e] = quant.four(u[i] + 2 * e, by_rcp);
-                int8_t *to = p.q + row * p.ld_q + c * V;
-                if (V == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(q[0], q[V / 4 - 1]);
-                else *reinterpret_cast<uint32_t *>(to) = q[0];
+                int8_t *to = p.q + row * p.ld_q - lead + c * V;
+                if (full(c)) {
+                    if (V == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(q[0], q[V / 4 - 1]);
+                    else *reinterpret_cast<uint32_t *>(to) = q[0];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if (inside(c * V + e)) to[e] = (int8_t)(q[e / 4] >> (e % 4 * 8));
+                }
             }
         };
         if (quant.rcp != 0.0f) finish(true);
@@ -594,16 +622,16 @@ __global__ void __launch_bounds__(group_threads_most(sizeof(T)), 1) sandwich_row
 struct Groups {
     int threads, groups, depth, smem;
 };
-template <typename T, typename X>
+template <typename T, typename X, bool WHOLE>
 Groups groups_of(const SandwichParams &p)
 {
     constexpr int V = 16 / (int)sizeof(T), XW = (int)sizeof(X) * V / 16;
-    const int packs = p.h / V, most = group_threads_most(sizeof(T)), room = 224 * 1024;
+    const int packs = most_packs<V, WHOLE>(p.h), room = 224 * 1024;
     Groups g;
     g.threads = ((packs + kGroupPacks - 1) / kGroupPacks + 31) / 32 * 32;
-    const int factors = 4 * p.h * (1 + (p.gamma != nullptr) + (p.smooth != nullptr));
+    const int factors = 4 * factor_floats<V, WHOLE>(p.h) * (1 + (p.gamma != nullptr) + (p.smooth != nullptr));
     const int row = (XW + (p.gate && p.ld_gate && p.gate_step ? 2 : 1)) * 16 * packs;
-    g.groups = most / g.threads;
+    g.groups = kGroupThreads / g.threads;
     if (g.groups > kMaxGroups) g.groups = kMaxGroups;
     if (g.groups > (room - factors) / row) g.groups = room > factors ? (room - factors) / row : 0;
     g.depth = g.groups > 0 ? (room - factors) / (g.groups * row) : 0;   // rows of a group that there is room for
@@ -612,59 +640,50 @@ Groups groups_of(const SandwichParams &p)
     return g;
 }
 
+template <typename T, typename X, bool WHOLE, bool EXACT, bool GATED>
+cudaError_t launch_rows(const SandwichParams &p, const Groups &g, cudaStream_t stream)
+{
+    const auto kernel = sandwich_rows_kernel<T, X, WHOLE, EXACT, GATED>;
+    static unsigned long long done_mask = 0;   // once per device; the attribute is idempotent, so a race only repeats the call
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!((done_mask >> (dev & 63)) & 1ull)) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
+        if (e != cudaSuccess) return e;
+        done_mask |= 1ull << (dev & 63);
+    }
+    const int ctas = (p.rows + g.groups - 1) / g.groups;
+    kernel<<<ctas < 148 ? ctas : 148, g.threads * g.groups, g.smem, stream>>>(p, g.threads, g.groups, g.depth);
+    return cudaGetLastError();
+}
+
 template <typename T, typename X, bool WHOLE>
 cudaError_t launch_packed(const SandwichParams &p, cudaStream_t stream)
 {
-    constexpr int V = 16 / (int)sizeof(T), XW = (int)sizeof(X) * V / 16;
-    const int packs = (p.h + (WHOLE ? 0 : V - 1) + V - 1) / V;
+    constexpr int V = 16 / (int)sizeof(T);
+    const int packs = most_packs<V, WHOLE>(p.h);
     const auto warps = [](int n) { return (n + 31) / 32 * 32; };
-    // Few rows: as many threads as a row has packs, for the shortest chain.  More: four packs a thread, for more rows on an SM, and the next
-    // row's loads under way; the CTAs that find a place on the SMs together go through the rows.
-    const int four = warps((packs + 3) / 4);
-    if (packs <= 1024 && (p.rows <= 2 * 148 || packs <= 64)) {
-        sandwich_kernel<T, X, 1, WHOLE, 1024, 1, false><<<p.rows, warps(packs), 0, stream>>>(p);
+    // Few rows: as many threads as a row has packs, for the shortest chain.  The kernel of many rows has the factors to lay out first and
+    // gains where every SM has rows enough in turn, later for short rows, of which an SM holds more CTAs (this one / that one, us, bf16 and
+    // an fp32 x: 148 x 7168 6.0 / 8.1, 200 x 7168 9.6 / 8.2, 1184 x 4096 14.8 / 15.6, 2368 x 4096 25.8 / 22.8, 4096 x 2048 19.6 / 22.5,
+    // 16384 x 2048 64.5 / 57.6, 16384 x 1424 49.8 / 47.3, 16384 x 768 26.8 / 32.0).
+    const long long work = (long long)p.rows * packs;
+    if (packs <= 256 && (packs <= 128 || work <= 148 * 8192)) {
+        sandwich_kernel<T, X, 1, WHOLE, 256, 8><<<p.rows, warps(packs), 0, stream>>>(p);
         return cudaGetLastError();
     }
-    int dev = 0;
-    cudaGetDevice(&dev);
-    // once per device; the attribute is idempotent, so a race only repeats the call
-    static unsigned long long done_mask = 0;
-    const bool first = !((done_mask >> (dev & 63)) & 1ull);
-    if constexpr (WHOLE) {
-        const Groups g = groups_of<T, X>(p);
-        if (g.groups > 0) {
-            const bool exact = packs == kGroupPacks * g.threads, gated = p.gate && p.ld_gate && p.gate_step;
-            const auto kernel = exact ? gated ? sandwich_rows_kernel<T, X, true, true> : sandwich_rows_kernel<T, X, true, false>
-                                : gated ? sandwich_rows_kernel<T, X, false, true> : sandwich_rows_kernel<T, X, false, false>;
-            const unsigned long long bit = 1ull << (dev & 63);
-            static unsigned long long done[4] = {};   // as above
-            unsigned long long &mask = done[2 * exact + gated];
-            if (!(mask & bit)) {
-                const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
-                if (e != cudaSuccess) return e;
-                mask |= bit;
-            }
-            const int ctas = (p.rows + g.groups - 1) / g.groups;
-            kernel<<<ctas < 148 ? ctas : 148, g.threads * g.groups, g.smem, stream>>>(p, g.threads, g.groups, g.depth);
-            return cudaGetLastError();
-        }
-    } else if (packs <= 4 * 512) {
-        const int smem = (XW + (p.gate && p.ld_gate && p.gate_step ? 2 : 1)) * 4 * 16 * four;
-        const int fit = 1024 / four < 220 * 1024 / (smem + 2048) ? 1024 / four : 220 * 1024 / (smem + 2048);
-        const auto kernel = sandwich_kernel<T, X, 4, WHOLE, 512, 2, true>;
-        if (first) {
-            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * 4 * 16 * 512);
-            if (e != cudaSuccess) return e;
-            done_mask |= 1ull << (dev & 63);
-        }
-        kernel<<<p.rows < 148 * fit ? p.rows : 148 * fit, four, smem, stream>>>(p);
+    if (packs <= 1024 && (p.rows <= 148 || (packs <= 512 && work <= 148 * 4096))) {
+        sandwich_kernel<T, X, 1, WHOLE, 1024, 1><<<p.rows, warps(packs), 0, stream>>>(p);
         return cudaGetLastError();
     }
-    if (packs <= 4 * 1024) {
-        sandwich_kernel<T, X, 4, WHOLE, 1024, 1, false><<<p.rows, four, 0, stream>>>(p);
-    } else {
-        sandwich_any_kernel<T, X><<<p.rows, 256, 0, stream>>>(p);
+    const Groups g = groups_of<T, X, WHOLE>(p);
+    if (g.groups > 0) {
+        const bool gated = p.gate && p.ld_gate && p.gate_step;
+        if (WHOLE && packs == kGroupPacks * g.threads) return gated ? launch_rows<T, X, WHOLE, WHOLE, true>(p, g, stream) : launch_rows<T, X, WHOLE, WHOLE, false>(p, g, stream);
+        return gated ? launch_rows<T, X, WHOLE, false, true>(p, g, stream) : launch_rows<T, X, WHOLE, false, false>(p, g, stream);
     }
+    if (packs <= 4 * 1024) sandwich_kernel<T, X, 4, WHOLE, 1024, 1><<<p.rows, warps((packs + 3) / 4), 0, stream>>>(p);
+    else sandwich_any_kernel<T, X><<<p.rows, 256, 0, stream>>>(p);
     return cudaGetLastError();
 }
 
