@@ -18,7 +18,7 @@ DESCRIBE_SOURCE = os.path.join(CSRC, "describe.cpp")
 
 SOURCES = ["gmm_sm100.cu", "gmm_simt.cu", "gmm_noalloc.cu", "ep_peer.cu", "moe_init_routing.cu", "norm_quant.cu", "route_top_k.cu",
            "adapter_add.cu", "quant_matmul.cu", "sandwich_norm.cu", "expert_balance.cu", "view_copy.cu", "acl_shim.cpp", "op_api.cpp", "block_ops.cpp"]
-HEADERS = ["gmm_common.h", "norm_common.h", "acl_shim.h", "op_api.h"]
+HEADERS = ["gmm_common.h", "norm_common.h", "dependent.h", "acl_shim.h", "op_api.h"]
 
 # -fmad=false: the epilogues reproduce the reference's separately rounded fp32 steps, so the compiler must not
 # fuse a multiply and an add.  No fast-math.

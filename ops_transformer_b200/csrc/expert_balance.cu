@@ -10,12 +10,19 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
+#include "dependent.h"
 #include "gmm_common.h"
+#include "norm_common.h"
 
 namespace gmm {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kGradThreads = 256, kGradWarps = kGradThreads / 32;
+// Threads of a block of rows, at most: for 8, 16 and 32 values a lane, as many as there are registers for.
+constexpr int threads_of(int per) { return per <= 8 ? 1024 : per <= 16 ? 512 : 256; }
+inline int warps_of(int experts) { return threads_of(experts <= 256 ? 8 : experts <= 512 ? 16 : 32) / 32; }
 
 struct BalanceParams {
     const void *logits;
@@ -31,8 +38,8 @@ struct BalanceParams {
     const float *grad_loss;
     void *grad;
     long long ld_grad;
-    // workspace of the loss: what a block of rows adds to a sequence stands in the piece `block + sequence`, which is another one for every
-    // block and sequence that meet, since both only grow on the way through the rows
+    // workspace of the loss: what a block of rows adds to a sequence is the piece `block + sequence`, which is another one for every block
+    // and sequence that meet, since both only grow on the way through the rows
     int chunk, blocks;                  // rows of a block, blocks
     int *ticket;
     int *piece_tokens;                  // [blocks + sequences]
@@ -42,17 +49,39 @@ struct BalanceParams {
     double *seq_dots;                   // [sequences, ceil(experts / 32)]
 };
 
-template <typename T> __device__ __forceinline__ float to_float(T v);
-template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
 constexpr float kInf = __builtin_huge_valf();
 
+__device__ __forceinline__ double warp_sum(double v)
+{
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b)
+{
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^v and 1 / v to 2 units in the last place; what is below the normal numbers is 0.
+__device__ __forceinline__ float exp2_of(float v)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float rcp_of(float v)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float warp_max(float v)      // passes NaN over
+{
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
 __device__ __forceinline__ float warp_sum(float v)
 {
 #pragma unroll
@@ -60,73 +89,146 @@ __device__ __forceinline__ float warp_sum(float v)
     return v;
 }
 
+// Rows whose loads a warp has under way: at most four, and no more than there are registers for.
+__host__ __device__ constexpr int rows_ahead(int per, int bytes, int registers)
+{
+    const int n = registers * 4 / (per * bytes);
+    return n > 4 ? 4 : n < 1 ? 1 : n;
+}
+
 // The expert of a lane's i-th value: V neighbours at a time.
 template <int V>
 __device__ __forceinline__ int expert_of(int i, int lane) { return (i / V * 32 + lane) * V + i % V; }
 
-// A row's logits; minus infinity where there is no expert.  V: values of one 16-byte load, or 1.
+// A row as it is in memory, for the loads of the next one to be under way while this one is worked on; minus infinity where there is no
+// expert.  V: values of one 16-byte load, or 1.
 template <typename T, int PER, int V>
-__device__ __forceinline__ void load_row(const T *row, int experts, int lane, float (&l)[PER])
-{
+struct RawRow {
+    static constexpr int N = PER / V;
+    typename std::conditional<(V > 1), uint4, T>::type raw[N];
+    __device__ __forceinline__ RawRow()
+    {
+        constexpr uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
 #pragma unroll
-    for (int i = 0; i < PER; i += V) {
-        const int e = expert_of<V>(i, lane);
-        if constexpr (V > 1) {
-            uint4 u = make_uint4(0, 0, 0, 0);
-            if (e < experts) u = *reinterpret_cast<const uint4 *>(row + e);
-            const T *t = reinterpret_cast<const T *>(&u);
-#pragma unroll
-            for (int j = 0; j < V; ++j) l[i + j] = e < experts ? to_float<T>(t[j]) : -kInf;
-        } else {
-            l[i] = e < experts ? to_float<T>(row[e]) : -kInf;
+        for (int i = 0; i < N; ++i) {
+            if constexpr (V > 1) raw[i] = make_uint4(none, none, none, none);
+            else raw[i] = from_float<T>(-kInf);
         }
     }
-}
-
-// p in the place of a row's logits, and for the sigmoid's gradient 1 - sigmoid.  An expert whose logit is NaN or minus infinity is not
-// there; a row without one is all zeros.
-template <bool SIGMOID, int PER>
-__device__ __forceinline__ void scores(float (&l)[PER], float (&rest)[PER])
-{
-    float total = 0.0f;
-    if constexpr (SIGMOID) {
+    __device__ __forceinline__ void load(const T *row, int experts, int lane)
+    {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const float t = expf(-fabsf(l[i])), big = __fdividef(1.0f, 1.0f + t), small = __fmul_rn(t, big);   // of |l| and -|l|
-            const bool there = l[i] > -kInf;
-            rest[i] = !there ? 0.0f : l[i] >= 0.0f ? small : big;
-            l[i] = !there ? 0.0f : l[i] >= 0.0f ? big : small;
-            total += l[i];
+        for (int i = 0; i < N; ++i) {
+            const int e = expert_of<V>(i * V, lane);
+            if (e >= experts) continue;
+            if constexpr (V > 1) raw[i] = *reinterpret_cast<const uint4 *>(row + e);
+            else raw[i] = row[e];
+        }
+    }
+    __device__ __forceinline__ void values(f32x2 (&l)[PER / 2]) const
+    {
+        if constexpr (V > 1) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) unpack<T>(raw[i], l + i * (V / 2));
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; i += 2) l[i / 2] = pair2(to_float<T>(raw[i]), to_float<T>(raw[i + 1]));
+        }
+    }
+};
+
+// e, of which p = e * inv, of a row's logits, and for the sigmoid's gradient rest = 1 - sigmoid.  An expert whose logit is NaN or minus
+// infinity is not there; a row without one is all zeros.
+//
+// The plain way takes the exponential's argument from one fma (off by a unit of its size, as the difference itself would be; an error that
+// the whole row has in common goes out with inv) and passes every infinity through to the right result.  What it cannot do shows in its
+// total, and is done again element by element: a logit of NaN, a row whose largest logit is so far out that the fma's constant term is
+// off by more than a little, or one whose sigmoids all but vanish, of which p is what softmax makes of it (to 2^-60).  Below sigmoids of
+// e^-700, which 64 bits hardly hold, there is nothing.
+template <bool SIGMOID, int PER>
+__device__ __forceinline__ void scores(const f32x2 (&l)[PER / 2], f32x2 (&e)[PER / 2], f32x2 (&rest)[PER / 2], float &inv)
+{
+    constexpr float kLog2e = 1.4426950408889634f;
+    float top = -kInf;
+    f32x2 total2 = 0;
+    if constexpr (SIGMOID) {
+        const f32x2 scale = pair2(-kLog2e, -kLog2e), one = pair2(1.0f, 1.0f);
+#pragma unroll
+        for (int i = 0; i < PER / 2; ++i) {
+            const float2 x = unpair2(mul2(l[i], scale));
+            const f32x2 t = pair2(exp2_of(x.x), exp2_of(x.y));
+            const float2 v = unpair2(add2(t, one));
+            e[i] = pair2(rcp_of(v.x), rcp_of(v.y));
+            const float2 r = unpair2(mul2(t, e[i]));
+            rest[i] = pair2(fminf(r.x, 1.0f), fminf(r.y, 1.0f));    // of infinity times 0, too
+            total2 = add2(total2, e[i]);
         }
     } else {
-        float top = -kInf;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) top = fmaxf(top, l[i]);   // passes NaN over
+        for (int i = 0; i < PER / 2; ++i) {
+            const float2 v = unpair2(l[i]);
+            top = fmaxf(top, fmaxf(v.x, v.y));
+        }
+        top = warp_max(top);
+        const float shift = __fmul_rn(top, -kLog2e);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            l[i] = !(l[i] > -kInf) ? 0.0f : l[i] == top ? 1.0f : expf(l[i] - top);
-            total += l[i];
+        for (int i = 0; i < PER / 2; ++i) {
+            const float2 x = unpair2(fma2(l[i], pair2(kLog2e, kLog2e), pair2(shift, shift)));
+            e[i] = pair2(exp2_of(x.x), exp2_of(x.y));
+            total2 = add2(total2, e[i]);
         }
     }
-    total = warp_sum(total);
-    const float inv = total > 0.0f ? __frcp_rn(total) : 0.0f;
+    const float2 parts = unpair2(total2);
+    float total = warp_sum(parts.x + parts.y);
+    if (!(total >= 1e-20f) || (!SIGMOID && !(fabsf(top) <= 0x1p20f))) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) l[i] = __fmul_rn(l[i], inv);
+        for (int i = 0; i < PER / 2; ++i) {
+            const float2 v = unpair2(l[i]);
+            top = fmaxf(top, fmaxf(v.x, v.y));
+        }
+        top = warp_max(top);
+        const bool soft = !SIGMOID || (top < -60.0f && top > -700.0f);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER / 2; ++i) {
+            const float2 v = unpair2(l[i]);
+            float of[2] = {v.x, v.y}, r[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float x = of[j];
+                if (soft) {
+                    of[j] = x == top ? 1.0f : expf(x - top);
+                    r[j] = 1.0f;
+                } else {
+                    const float t = expf(-fabsf(x)), big = __fdividef(1.0f, 1.0f + t), small = __fmul_rn(t, big);   // of |x| and -|x|
+                    of[j] = x >= 0.0f ? big : small;
+                    r[j] = x >= 0.0f ? small : big;
+                }
+                if (!(x > -kInf)) of[j] = r[j] = 0.0f;
+                sum += of[j];
+            }
+            e[i] = pair2(of[0], of[1]);
+            rest[i] = pair2(r[0], r[1]);
+        }
+        total = warp_sum(sum);
+    }
+    inv = total > 0.0f ? rcp_of(total) : 0.0f;
 }
 
 // Rows of sequence s, cut to those that there are.
 __device__ __forceinline__ int seq_begin(const BalanceParams &p, int s) { return p.cu ? min(max(p.cu[s], 0), p.rows) : 0; }
 __device__ __forceinline__ int seq_end(const BalanceParams &p, int s) { return p.cu ? min(max(p.cu[s + 1], 0), p.rows) : p.rows; }
-// The first sequence that ends behind `row`.
-__device__ __forceinline__ int seq_of(const BalanceParams &p, int row)
+// The first sequence that ends behind `row`; by a warp, 32 ends at a time.
+__device__ __forceinline__ int seq_of(const BalanceParams &p, int row, int lane)
 {
+    if (!p.cu) return row < p.rows ? 0 : 1;
     int lo = 0, hi = p.sequences;
     while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (seq_end(p, mid) > row) hi = mid;
-        else lo = mid + 1;
+        const int width = (int)(((long long)hi - lo + 31) / 32);
+        const long long probe = lo + (lane + 1ll) * width - 1;
+        const int before = __popc(__ballot_sync(0xffffffffu, probe < hi && seq_end(p, (int)probe) <= row));
+        lo = min(lo + before * width, hi);
+        hi = min(hi, lo + width - 1);
     }
     return lo;
 }
@@ -136,102 +238,237 @@ __device__ __forceinline__ float weight_of(const BalanceParams &p, int tokens, i
     return tokens > 0 ? (float)((double)p.coefficient * p.experts / ((double)p.top_k * tokens * tokens * sequences)) : 0.0f;
 }
 
-// What the rows of a block add to the sequences that they belong to.  ALL: one block holds all rows of the one sequence, and finishes.
-template <typename T, bool SIGMOID, int PER, int V, bool ALL>
-__global__ void __launch_bounds__(kThreads) balance_rows_kernel(const BalanceParams p)
+// The sequence and the block of rows that a piece belongs to: the sequence is the first whose last piece is not before it.
+__device__ __forceinline__ int seq_of_piece(const BalanceParams &p, int piece, int lane)
 {
-    extern __shared__ float sums[];     // [warps][experts], then the counts [experts]
-    __shared__ int warp_tokens[kWarps];
-    __shared__ double warp_dots[kWarps];
-    int *counts = reinterpret_cast<int *>(sums + kWarps * p.experts);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, block = blockIdx.x;
-    if (!ALL && block == 0 && tid == 0) *p.ticket = 0;
-    const int row0 = block * p.chunk, row1 = min(row0 + p.chunk, p.rows);
-    for (int s = ALL ? 0 : seq_of(p, row0); s < p.sequences; ++s) {
-        const int begin = max(seq_begin(p, s), row0), end = min(seq_end(p, s), row1);
-        if (!ALL && seq_begin(p, s) >= row1) break;
-        if (!ALL && begin >= end) continue;
-        for (int e = tid; e < p.experts; e += kThreads) counts[e] = 0;
-        __syncthreads();
-        float sum[PER] = {};
-        int tokens = 0;
-        for (int row = begin + warp; row < end; row += kWarps) {
-            if (p.mask && p.mask[row] == 0) continue;
-            ++tokens;
-            float l[PER], rest[PER];
-            load_row<T, PER, V>(static_cast<const T *>(p.logits) + row * p.ld, p.experts, lane, l);
-            scores<SIGMOID, PER>(l, rest);
+    if (!p.cu) return piece < p.blocks ? 0 : 1;
+    int lo = 0, hi = p.sequences;
+    while (lo < hi) {
+        const int width = (hi - lo + 31) / 32, probe = lo + (lane + 1) * width - 1;
+        const bool before = probe < hi && probe + max(seq_end(p, probe) - 1, 0) / p.chunk < piece;
+        lo = min(lo + __popc(__ballot_sync(0xffffffffu, before)) * width, hi);
+        hi = min(hi, lo + width - 1);
+    }
+    return lo;
+}
+
+// What a block of rows adds to a sequence: one piece, which a CTA makes.  A warp takes up to `ahead` rows at a time, whose loads it issues
+// together.  ALL: the rows are all those of the only sequence, and the CTA finishes.
+template <typename T, bool SIGMOID, int PER, int V, bool ALL>
+__global__ void __launch_bounds__(threads_of(PER), 1) balance_rows_kernel(const BalanceParams p)
+{
+    constexpr int R = rows_ahead(PER, sizeof(T), PER <= 8 ? 32 : 64);
+    extern __shared__ float4 smem[];    // sums [warps][experts], then the counts [experts]
+    __shared__ int warp_tokens[32];
+    __shared__ double warp_dots[32];
+    float *sums = reinterpret_cast<float *>(smem);
+    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = threads >> 5, piece = blockIdx.x;
+    int *counts = reinterpret_cast<int *>(sums + warps * p.experts);
+    for (int e = tid; e < p.experts; e += threads) counts[e] = 0;
+    dependent_wait();
+    dependent_release();
+    if (!ALL && piece == 0 && tid == 0) *p.ticket = 0;
+    const int s = ALL ? 0 : seq_of_piece(p, piece, lane);
+    if (s >= p.sequences) return;
+    const int begin = ALL ? 0 : max(seq_begin(p, s), (piece - s) * p.chunk), end = ALL ? p.rows : min(seq_end(p, s), (piece - s + 1) * p.chunk);
+    if (!ALL && begin >= end) return;
+    f32x2 sum[PER / 2] = {};
+    int tokens = 0;
+    RawRow<T, PER, V> rows[R];
+    __syncthreads();    // the counts are zero
+    for (int row0 = begin + warp; row0 < end; row0 += R * warps) {
+        bool token[R];
+        int ids[R];
+        const auto id_of = [&](int row, int j) {
+            const long long i = (long long)row * p.top_k + j, id = p.ids_i64 ? static_cast<const long long *>(p.ids)[i] : (long long)static_cast<const int *>(p.ids)[i];
+            return id >= 0 && id < p.experts ? (int)id : -1;
+        };
 #pragma unroll
-            for (int i = 0; i < PER; ++i) sum[i] += l[i];
+        for (int r = 0; r < R; ++r) {   // of a row that the mask leaves out, too, so that no load waits for another
+            const int row = row0 + r * warps;
+            token[r] = false;
+            if (row >= end) continue;
+            rows[r].load(static_cast<const T *>(p.logits) + row * p.ld, p.experts, lane);
+            ids[r] = lane < p.top_k ? id_of(row, lane) : -1;
+            token[r] = !p.mask || p.mask[row] != 0;
         }
-        const long long id0 = (long long)begin * p.top_k;
-        const long long pairs = (long long)(end - begin) * p.top_k;
-        for (long long i = tid; i < pairs; i += kThreads) {
-            if (p.mask && p.mask[begin + i / p.top_k] == 0) continue;
-            const long long id = p.ids_i64 ? static_cast<const long long *>(p.ids)[id0 + i] : static_cast<const int *>(p.ids)[id0 + i];
-            if (id >= 0 && id < p.experts) atomicAdd(counts + id, 1);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (!token[r]) continue;
+            ++tokens;
+            int id = ids[r];
+            for (int j = lane;;) {
+                if (id >= 0) atomicAdd(counts + id, 1);
+                if ((j += 32) >= p.top_k) break;
+                id = id_of(row0 + r * warps, j);
+            }
+            f32x2 l[PER / 2], e[PER / 2], rest[PER / 2];
+            float inv;
+            rows[r].values(l);
+            scores<SIGMOID, PER>(l, e, rest, inv);
+#pragma unroll
+            for (int i = 0; i < PER / 2; ++i) sum[i] = fma2(e[i], pair2(inv, inv), sum[i]);
         }
-        if (lane == 0) warp_tokens[warp] = tokens;
+    }
+    if (lane == 0) warp_tokens[warp] = tokens;
+    if constexpr (V > 1) {
+#pragma unroll
+        for (int i = 0; i < PER; i += 4) {
+            const int e = expert_of<V>(i, lane);
+            if (e < p.experts)
+                *reinterpret_cast<float4 *>(sums + warp * p.experts + e) = make_float4(element(sum, i), element(sum, i + 1), element(sum, i + 2), element(sum, i + 3));
+        }
+    } else {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int e = expert_of<V>(i, lane);
-            if (e < p.experts) sums[warp * p.experts + e] = sum[i];
+            if (e < p.experts) sums[warp * p.experts + e] = element(sum, i);
         }
-        __syncthreads();
-        tokens = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) tokens += warp_tokens[w];
-        double dot = 0.0;
-        for (int e = tid; e < p.experts; e += kThreads) {
-            float total = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) total += sums[w * p.experts + e];
-            if (ALL) {
-                p.counts[e] = counts[e];
-                dot += (double)total * counts[e];
-            } else {
-                p.piece_sums[(long long)(block + s) * p.experts + e] = total;
-                p.piece_counts[(long long)(block + s) * p.experts + e] = counts[e];
-            }
-        }
+    }
+    __syncthreads();
+    double dot = 0.0;
+    for (int e = tid; e < p.experts; e += threads) {
+        float total = 0.0f;
+#pragma unroll 8
+        for (int w = 0; w < warps; ++w) total += sums[w * p.experts + e];
         if (ALL) {
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-            if (lane == 0) warp_dots[warp] = dot;
-            __syncthreads();
-            if (tid == 0) {
-                dot = 0.0;
-                for (int w = 0; w < kWarps; ++w) dot += warp_dots[w];
-                const float weight = weight_of(p, tokens, 1);
-                p.weight[0] = weight;
-                *p.loss = (float)(dot * weight);
-            }
-            return;
+            p.counts[e] = counts[e];
+            dot += (double)total * counts[e];
+        } else {
+            p.piece_sums[(long long)piece * p.experts + e] = total;
+            p.piece_counts[(long long)piece * p.experts + e] = counts[e];
         }
-        if (tid == 0) p.piece_tokens[block + s] = tokens;
+    }
+    if (ALL) {
+        dot = warp_sum(dot);
+        if (lane == 0) warp_dots[warp] = dot;
         __syncthreads();
+    }
+    if (warp != 0) return;
+    tokens = (int)__reduce_add_sync(0xffffffffu, lane < warps ? warp_tokens[lane] : 0);
+    if (ALL) {
+        dot = warp_sum(lane < warps ? warp_dots[lane] : 0.0);
+        const float weight = weight_of(p, tokens, 1);
+        if (lane == 0) p.weight[0] = weight;
+        if (lane == 0) *p.loss = (float)(dot * weight);
+    } else if (lane == 0) {
+        p.piece_tokens[piece] = tokens;
     }
 }
 
-// The pieces of a sequence, 32 experts a block; the block that comes last makes the loss of all.
-__global__ void __launch_bounds__(kThreads) balance_finish_kernel(const BalanceParams p)
+// The sums of a warp's share of a sequence's pieces, for the expert of each lane; N of them under way.
+template <int N>
+__device__ __forceinline__ void sum_pieces(const BalanceParams &p, int s, int first, int step, int e, float &sum, int &count, int &tokens)
 {
-    __shared__ float sums[kWarps][32];
-    __shared__ int counts[kWarps][32], tokens_of[kWarps];
-    __shared__ double warp_dots[kWarps];
+    const int begin = seq_begin(p, s), end = seq_end(p, s);
+    if (begin >= end) return;
+    const int behind = (end - 1) / p.chunk + 1;
+    for (int b = begin / p.chunk + first; b < behind; b += N * step) {
+        float some_sum[N];
+        int some_count[N], some_tokens[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const long long piece = b + i * step + s;
+            const bool there = b + i * step < behind;
+            some_sum[i] = there && e < p.experts ? p.piece_sums[piece * p.experts + e] : 0.0f;
+            some_count[i] = there && e < p.experts ? p.piece_counts[piece * p.experts + e] : 0;
+            some_tokens[i] = there ? p.piece_tokens[piece] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            sum += some_sum[i];
+            count += some_count[i];
+            tokens += some_tokens[i];
+        }
+    }
+}
+
+// Few sequences: one cluster adds up their pieces, a CTA an eighth of the experts, and its first CTA makes the loss of what they put into
+// its shared memory.  (Through memory and a ticket, as below, that last step costs 2.7 us instead of a half.)
+constexpr int kFewSequences = 64, kFinishCtas = 8;
+__global__ void __launch_bounds__(1024, 1) balance_finish_few_kernel(const BalanceParams p)
+{
+    __shared__ float sums[32][32];
+    __shared__ int counts[32][32], tokens_of[kFewSequences];
+    __shared__ double dots[kFewSequences], all_dots[kFinishCtas][kFewSequences], warp_dots[2];
+    __shared__ int some;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = blockIdx.x;
+    const int groups = (p.experts + 32 * kFinishCtas - 1) / (32 * kFinishCtas);     // of 32 experts, a CTA's share
+    int each = 1;   // warps of a sequence
+    while (each * 2 * p.sequences <= 32) each *= 2;
+    dependent_wait();
+    dependent_release();
+    if (tid < p.sequences) dots[tid] = 0.0;
+    if (tid == 0) some = 0;
+    const int part = warp & (each - 1);
+    for (int g = 0; g < groups; ++g) {
+        const int e = (rank * groups + g) * 32 + lane;
+        for (int s0 = 0; s0 < p.sequences; s0 += 32 / each) {
+            const int s = s0 + warp / each;
+            float sum = 0.0f;
+            int count = 0, tokens = 0;
+            if (s < p.sequences) sum_pieces<5>(p, s, part, each, e, sum, count, tokens);
+            sums[warp][lane] = sum;
+            counts[warp][lane] = count;
+            if (g == 0) {
+                __syncthreads();
+                if (lane == 0 && part == 0 && s < p.sequences) tokens_of[s] = 0;
+                __syncthreads();
+                if (lane == 0 && tokens) atomicAdd(tokens_of + s, tokens);
+            }
+            __syncthreads();
+            if (part == 0 && s < p.sequences) {
+                sum = 0.0f;
+                count = 0;
+#pragma unroll 8
+                for (int w = warp; w < warp + each; ++w) {
+                    sum += sums[w][lane];
+                    count += counts[w][lane];
+                }
+                if (e < p.experts) p.counts[(long long)s * p.experts + e] = count;
+                const double dot = warp_sum((double)sum * count);
+                if (lane == 0) dots[s] += dot;
+            }
+            __syncthreads();
+        }
+    }
+    if (tid < p.sequences) {
+        uint32_t to;
+        asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"((uint32_t)__cvta_generic_to_shared(&all_dots[rank][tid])));
+        asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(dots[tid]) : "memory");
+        if (tokens_of[tid] > 0) atomicAdd(&some, 1);
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (rank != 0 || warp >= 2) return;
+    double loss = 0.0;
+    if (tid < p.sequences) {
+        const float weight = weight_of(p, tokens_of[tid], some);
+        p.weight[tid] = weight;
+#pragma unroll
+        for (int r = 0; r < kFinishCtas; ++r) loss += all_dots[r][tid];
+        loss *= weight;
+    }
+    loss = warp_sum(loss);
+    if (lane == 0) warp_dots[warp] = loss;
+    asm volatile("bar.sync 1, 64;" ::: "memory");
+    if (tid == 0) *p.loss = (float)(warp_dots[0] + warp_dots[1]);
+}
+
+// Any number of sequences: the pieces of one, 32 experts a block; the block that comes last makes the loss of all.
+__global__ void __launch_bounds__(1024) balance_finish_kernel(const BalanceParams p)
+{
+    __shared__ float sums[32][32];
+    __shared__ int counts[32][32], tokens_of[32];
+    __shared__ double warp_dots[32];
     __shared__ int last, some;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, s = blockIdx.y, parts = gridDim.x;
-    const int e = blockIdx.x * 32 + lane, begin = seq_begin(p, s), end = seq_end(p, s);
-    const int first = begin / p.chunk, behind = begin < end ? (end - 1) / p.chunk + 1 : first;
+    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = threads >> 5, s = blockIdx.x, parts = gridDim.y;
+    const int e = blockIdx.y * 32 + lane;
+    dependent_wait();
+    dependent_release();
     float sum = 0.0f;
     int count = 0, tokens = 0;
-    for (int b = first + warp; b < behind; b += kWarps) {
-        if (e < p.experts) {
-            sum += p.piece_sums[(long long)(b + s) * p.experts + e];
-            count += p.piece_counts[(long long)(b + s) * p.experts + e];
-        }
-        tokens += p.piece_tokens[b + s];
-    }
+    sum_pieces<4>(p, s, warp, warps, e, sum, count, tokens);
     sums[warp][lane] = sum;
     counts[warp][lane] = count;
     if (lane == 0) tokens_of[warp] = tokens;
@@ -239,20 +476,18 @@ __global__ void __launch_bounds__(kThreads) balance_finish_kernel(const BalanceP
     __syncthreads();
     if (warp == 0) {
         sum = 0.0f;
-        count = tokens = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        count = 0;
+#pragma unroll 8
+        for (int w = 0; w < warps; ++w) {
             sum += sums[w][lane];
             count += counts[w][lane];
-            tokens += tokens_of[w];
         }
+        tokens = (int)__reduce_add_sync(0xffffffffu, lane < warps ? tokens_of[lane] : 0);
         if (e < p.experts) p.counts[(long long)s * p.experts + e] = count;
-        double dot = (double)sum * count;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        const double dot = warp_sum((double)sum * count);
         if (lane == 0) {
-            p.seq_dots[(long long)s * parts + blockIdx.x] = dot;
-            if (blockIdx.x == 0) p.seq_tokens[s] = tokens;
+            p.seq_dots[(long long)s * parts + blockIdx.y] = dot;
+            if (blockIdx.y == 0) p.seq_tokens[s] = tokens;
             __threadfence();
             last = atomicAdd(p.ticket, 1) == p.sequences * parts - 1;
         }
@@ -260,72 +495,102 @@ __global__ void __launch_bounds__(kThreads) balance_finish_kernel(const BalanceP
     __syncthreads();
     if (!last) return;
     __threadfence();
+    double loss = 0.0;
+    const auto dot_of = [&](int i) {
+        double dot = 0.0;
+#pragma unroll 8
+        for (int j = 0; j < parts; ++j) dot += __ldcg(p.seq_dots + (long long)i * parts + j);
+        return dot;
+    };
+    const double dot = tid < p.sequences ? dot_of(tid) : 0.0;   // of most calls all, under way with the tokens
     int mine = 0;
-    for (int i = tid; i < p.sequences; i += kThreads) mine += __ldcg(p.seq_tokens + i) > 0;
+    for (int i = tid; i < p.sequences; i += threads) mine += __ldcg(p.seq_tokens + i) > 0;
     if (mine) atomicAdd(&some, mine);
     __syncthreads();
-    double loss = 0.0;
-    for (int i = tid; i < p.sequences; i += kThreads) {
+    for (int i = tid; i < p.sequences; i += threads) {
         const float weight = weight_of(p, __ldcg(p.seq_tokens + i), some);
         p.weight[i] = weight;
-        double dot = 0.0;
-        for (int j = 0; j < parts; ++j) dot += __ldcg(p.seq_dots + (long long)i * parts + j);
-        loss += dot * weight;
+        loss += (i == tid ? dot : dot_of(i)) * weight;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
+    loss = warp_sum(loss);
     if (lane == 0) warp_dots[warp] = loss;
     __syncthreads();
-    if (tid == 0) {
-        loss = 0.0;
-        for (int w = 0; w < kWarps; ++w) loss += warp_dots[w];
-        *p.loss = (float)loss;
+    if (warp == 0) {
+        loss = warp_sum(lane < warps ? warp_dots[lane] : 0.0);
+        if (lane == 0) *p.loss = (float)loss;
     }
 }
 
 template <typename T, bool SIGMOID, int PER, int V>
-__global__ void __launch_bounds__(kThreads) balance_grad_kernel(const BalanceParams p)
+__global__ void __launch_bounds__(kGradThreads) balance_grad_kernel(const BalanceParams p)
 {
-    const int lane = threadIdx.x & 31, row0 = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * p.chunk, row1 = min(row0 + p.chunk, p.rows);
+    constexpr int R = rows_ahead(PER, sizeof(T), 16);
+    const int lane = threadIdx.x & 31, row0 = (blockIdx.x * kGradWarps + (threadIdx.x >> 5)) * p.chunk, row1 = min(row0 + p.chunk, p.rows);
+    dependent_wait();
+    dependent_release();
     if (row0 >= row1) return;
     const float grad_loss = p.grad_loss ? *p.grad_loss : 1.0f;
-    int s = seq_of(p, row0), known = -1;
-    float load[PER], factor = 0.0f;
-    for (int row = row0; row < row1; ++row) {
-        while (s < p.sequences && seq_end(p, s) <= row) ++s;
-        const bool token = s < p.sequences && row >= seq_begin(p, s) && !(p.mask && p.mask[row] == 0);
-        float l[PER] = {};
+    int s = seq_of(p, row0, lane), known = -1, begin = 0, end = 0;
+    f32x2 load[PER / 2];
+    float factor = 0.0f;
+    RawRow<T, PER, V> rows[R];
+    for (int batch = row0; batch < row1; batch += R) {
+    int8_t mask[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        if (batch + r >= row1) break;
+        rows[r].load(static_cast<const T *>(p.logits) + (batch + r) * p.ld, p.experts, lane);
+        mask[r] = p.mask ? p.mask[batch + r] : 1;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int row = batch + r;
+        if (row >= row1) break;
+        while (row >= end && s < p.sequences) {
+            begin = seq_begin(p, s);
+            end = seq_end(p, s);
+            if (row >= end) ++s;
+        }
+        const bool token = row >= begin && row < end && mask[r] != 0;
+        f32x2 g[PER / 2] = {};
         if (token) {
             if (known != s) {
                 // Counts less a whole number near their mean: the difference from the row's mean of them, which is what the gradient is made
                 // of, does not lose its places to what they all have in common.
                 known = s;
                 const long long *counts = p.counts + (long long)s * p.experts;
+                factor = __fmul_rn(p.weight[s], grad_loss);
+                long long count[PER];
+#pragma unroll
+                for (int i = 0; i < PER; i += V > 1 ? 2 : 1) {
+                    const int e = expert_of<V>(i, lane);
+                    if constexpr (V > 1) {
+                        const longlong2 two = e < p.experts ? *reinterpret_cast<const longlong2 *>(counts + e) : make_longlong2(0, 0);
+                        count[i] = two.x;
+                        count[i + 1] = two.y;
+                    } else {
+                        count[i] = e < p.experts ? counts[e] : 0;
+                    }
+                }
                 float total = 0.0f;
 #pragma unroll
-                for (int i = 0; i < PER; ++i) {
-                    const int e = expert_of<V>(i, lane);
-                    if (e < p.experts) total += (float)counts[e];
-                }
+                for (int i = 0; i < PER; ++i) total += (float)count[i];
                 const long long base = (long long)(warp_sum(total) / (float)p.experts);
 #pragma unroll
-                for (int i = 0; i < PER; ++i) {
-                    const int e = expert_of<V>(i, lane);
-                    load[i] = e < p.experts ? (float)(counts[e] - base) : 0.0f;
-                }
-                factor = __fmul_rn(p.weight[s], grad_loss);
+                for (int i = 0; i < PER; i += 2) load[i / 2] = pair2((float)(count[i] - base), (float)(count[i + 1] - base));
             }
-            float rest[PER];
-            load_row<T, PER, V>(static_cast<const T *>(p.logits) + row * p.ld, p.experts, lane, l);
-            scores<SIGMOID, PER>(l, rest);
-            float mean = 0.0f;
+            f32x2 l[PER / 2], e[PER / 2], rest[PER / 2], mean2 = 0;
+            float inv;
+            rows[r].values(l);
+            scores<SIGMOID, PER>(l, e, rest, inv);
 #pragma unroll
-            for (int i = 0; i < PER; ++i) mean = __fmaf_rn(l[i], load[i], mean);
-            mean = warp_sum(mean);
+            for (int i = 0; i < PER / 2; ++i) mean2 = fma2(e[i], load[i], mean2);
+            const float2 parts = unpair2(mean2);
+            const float mean = -__fmul_rn(warp_sum(parts.x + parts.y), inv), scale = __fmul_rn(inv, factor);
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                l[i] = __fmul_rn(__fmul_rn(l[i], load[i] - mean), factor);
-                if (SIGMOID) l[i] = __fmul_rn(l[i], rest[i]);
+            for (int i = 0; i < PER / 2; ++i) {
+                g[i] = mul2(mul2(e[i], pair2(scale, scale)), add2(load[i], pair2(mean, mean)));
+                if (SIGMOID) g[i] = mul2(g[i], rest[i]);
             }
         }
         T *to = static_cast<T *>(p.grad) + row * p.ld_grad;
@@ -333,26 +598,15 @@ __global__ void __launch_bounds__(kThreads) balance_grad_kernel(const BalancePar
         for (int i = 0; i < PER; i += V) {
             const int e = expert_of<V>(i, lane);
             if (e >= p.experts) continue;
-            if constexpr (V > 1) {
-                uint4 u;
-                T *t = reinterpret_cast<T *>(&u);
-#pragma unroll
-                for (int j = 0; j < V; ++j) t[j] = from_float<T>(l[i + j]);
-                *reinterpret_cast<uint4 *>(to + e) = u;
-            } else {
-                to[e] = from_float<T>(l[i]);
-            }
+            if constexpr (V > 1) *reinterpret_cast<uint4 *>(to + e) = pack<T>(g + i / 2);
+            else to[e] = from_float<T>(element(g, i));
         }
+    }
     }
 }
 
-constexpr int kAllRows = 64;    // most rows that one block takes by itself
-
-int chunk_of(int64_t rows)      // rows of a block: two blocks an SM, at least one row a warp
-{
-    const int64_t each = (rows + 2 * 148 - 1) / (2 * 148);
-    return (int)((each + kWarps - 1) / kWarps * kWarps);
-}
+#include <cstdlib>
+static const int kAllRows = getenv("BAL_ALL") ? atoi(getenv("BAL_ALL")) : 64;    // most rows that one block takes by itself
 
 size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
@@ -372,8 +626,9 @@ cudaError_t dispatch_width(int experts, bool packs, Fn fn)
         return fn(Type<T>(), Flag<SIGMOID>(), Int<32>(), Int<V>());
     }
     if (experts <= 64) return fn(Type<T>(), Flag<SIGMOID>(), Int<2>(), Int<1>());
-    if (experts <= 160) return fn(Type<T>(), Flag<SIGMOID>(), Int<5>(), Int<1>());
+    if (experts <= 192) return fn(Type<T>(), Flag<SIGMOID>(), Int<6>(), Int<1>());
     if (experts <= 256) return fn(Type<T>(), Flag<SIGMOID>(), Int<8>(), Int<1>());
+    if (experts <= 512) return fn(Type<T>(), Flag<SIGMOID>(), Int<16>(), Int<1>());
     return fn(Type<T>(), Flag<SIGMOID>(), Int<32>(), Int<1>());
 }
 template <typename Fn>
@@ -407,10 +662,16 @@ BalanceParams params_of(const BalanceProblem &b)
 
 struct Layout {
     size_t tokens, counts, sums, seq_tokens, seq_dots, bytes;
-    int chunk, blocks;
+    int chunk, blocks, warps;
     explicit Layout(const BalanceProblem &b)
     {
-        chunk = b.rows > 0 ? chunk_of(b.rows) : kWarps;
+        // One piece for each CTA that there is room for at once, in smaller CTAs where there are many sequences, each of which has a piece
+        // that it shares with none; at least a row for each warp.
+        const int most = warps_of(b.experts);
+        const auto at_once = [&] { return 148 * (most / warps); };
+        for (warps = most; warps > 4 && at_once() < 2 * b.sequences;) warps /= 2;
+        const int64_t wanted = at_once() >= 2 * b.sequences ? at_once() - b.sequences + 1 : at_once() / 2, each = (b.rows + wanted - 1) / wanted;
+        chunk = (int)(each < warps ? warps : each);
         blocks = (int)((b.rows + chunk - 1) / chunk);
         const size_t pieces = (size_t)blocks + (size_t)b.sequences, parts = ((size_t)b.experts + 31) / 32;
         tokens = 256;
@@ -432,9 +693,9 @@ cudaError_t balance_launch(const BalanceProblem &b, void *workspace, size_t work
 {
     BalanceParams p = params_of(b);
     const bool all = one_block(b);
-    const int smem = (kWarps + 1) * b.experts * 4;
-    int blocks = 1;
+    int blocks = 1, warps = warps_of(b.experts);
     if (all) {
+        if (warps > b.rows) warps = b.rows < 4 ? 4 : (int)b.rows;
         p.chunk = kAllRows;
     } else {
         const Layout at(b);
@@ -447,18 +708,21 @@ cudaError_t balance_launch(const BalanceProblem &b, void *workspace, size_t work
         p.piece_sums = reinterpret_cast<float *>(ws + at.sums);
         p.seq_tokens = reinterpret_cast<int *>(ws + at.seq_tokens);
         p.seq_dots = reinterpret_cast<double *>(ws + at.seq_dots);
-        blocks = at.blocks > 0 ? at.blocks : 1;   // no rows: the ticket is cleared all the same
+        warps = at.warps;
+        blocks = at.blocks + (int)b.sequences - (at.blocks > 0);    // no rows: the ticket is cleared all the same
     }
     cudaError_t e = dispatch(b, in_packs(b.logits, b.ld, b), [&](auto type, auto sigmoid, auto per, auto v) {
         typedef typename decltype(type)::type T;
         const auto kernel = all ? balance_rows_kernel<T, decltype(sigmoid)::value, decltype(per)::value, decltype(v)::value, true>
                                 : balance_rows_kernel<T, decltype(sigmoid)::value, decltype(per)::value, decltype(v)::value, false>;
-        kernel<<<blocks, kThreads, smem, stream>>>(p);
-        return cudaGetLastError();
+        return launch_dependent(kernel, dim3(blocks), warps * 32, (size_t)(warps + 1) * b.experts * 4, 1, stream, p);
     });
     if (e != cudaSuccess || all) return e;
-    balance_finish_kernel<<<dim3((unsigned)(b.experts + 31) / 32, (unsigned)b.sequences), kThreads, 0, stream>>>(p);
-    return cudaGetLastError();
+    if (b.sequences <= kFewSequences) return launch_dependent(balance_finish_few_kernel, dim3(kFinishCtas), 1024, 0, kFinishCtas, stream, p);
+    // four pieces a warp, of the most that a sequence has on average
+    const int64_t finish_warps = (p.blocks / b.sequences + 1 + 3) / 4;
+    return launch_dependent(balance_finish_kernel, dim3((unsigned)b.sequences, (unsigned)(b.experts + 31) / 32),
+                            (unsigned)(finish_warps < 4 ? 128 : finish_warps > 32 ? 1024 : finish_warps * 32), 0, 1, stream, p);
 }
 
 cudaError_t balance_grad_launch(const BalanceProblem &b, cudaStream_t stream)
@@ -466,13 +730,13 @@ cudaError_t balance_grad_launch(const BalanceProblem &b, cudaStream_t stream)
     if (b.rows <= 0) return cudaSuccess;
     BalanceParams p = params_of(b);
     // rows of a warp: four blocks an SM
-    const int64_t warps = 4 * 148 * kWarps;
+    const int64_t warps = 4 * 148 * kGradWarps;
     p.chunk = (int)((b.rows + warps - 1) / warps);
-    const int64_t blocks = (b.rows + (int64_t)p.chunk * kWarps - 1) / ((int64_t)p.chunk * kWarps);
-    return dispatch(b, in_packs(b.logits, b.ld, b) && in_packs(b.grad, b.ld_grad, b), [&](auto type, auto sigmoid, auto per, auto v) {
+    const int64_t blocks = (b.rows + (int64_t)p.chunk * kGradWarps - 1) / ((int64_t)p.chunk * kGradWarps);
+    return dispatch(b, in_packs(b.logits, b.ld, b) && in_packs(b.grad, b.ld_grad, b) && !((uintptr_t)b.counts & 15), [&](auto type, auto sigmoid, auto per, auto v) {
         typedef typename decltype(type)::type T;
-        balance_grad_kernel<T, decltype(sigmoid)::value, decltype(per)::value, decltype(v)::value><<<(unsigned)blocks, kThreads, 0, stream>>>(p);
-        return cudaGetLastError();
+        return launch_dependent(balance_grad_kernel<T, decltype(sigmoid)::value, decltype(per)::value, decltype(v)::value>, dim3((unsigned)blocks),
+                                kGradThreads, 0, 1, stream, p);
     });
 }
 

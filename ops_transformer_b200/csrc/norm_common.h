@@ -1,4 +1,4 @@
-// What the kernels that norm and quantise rows share: packs of values as pairs of floats, the reduction over a block, the int8 step and
+// What the kernels that work on rows share: packs of values as pairs of floats, the reduction over a block, the int8 step and
 // its quotients.
 #pragma once
 #include <cuda_bf16.h>

@@ -9,6 +9,7 @@
 
 #include <cmath>
 
+#include "dependent.h"
 #include "gmm_common.h"
 
 namespace gmm {
@@ -175,8 +176,6 @@ __device__ __forceinline__ int4 ld_shared(uint32_t saddr)
     return v;
 }
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void pdl_release() { asm volatile("griddepcontrol.launch_dependents;"); }
 __device__ __forceinline__ float load_as_float(const void *p, int dtype, long long i)
 {
     if (dtype == kF32) return static_cast<const float *>(p)[i];
@@ -239,7 +238,7 @@ __global__ void __launch_bounds__(kThreads) quant_matmul_kernel(const __grid_con
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         if (p.split > 1) mbar_arrive_expect_tx(&received, (uint32_t)(p.apart ? p.split : p.split - 1) * per * kTokenBytes);
     }
-    pdl_wait();
+    dependent_wait();
     if (warp == 0) {
         // the ring is filled before anything else: what follows runs beside the copies' way
         __syncwarp();
@@ -267,7 +266,7 @@ __global__ void __launch_bounds__(kThreads) quant_matmul_kernel(const __grid_con
         tc_fence_before();
     }
     __syncthreads();
-    pdl_release();   // tensor memory is in hand: the next kernel's CTAs may come and wait
+    dependent_release();   // tensor memory is in hand: the next kernel's CTAs may come and wait
     tc_fence_after();
     const uint32_t taddr = tmem_base;
     if (p.apart) cluster_arrive();   // this CTA can be sent to
@@ -463,8 +462,8 @@ struct PackParams {
 };
 __global__ void __launch_bounds__(256) quant_matmul_pack_kernel(const PackParams p)
 {
-    pdl_wait();
-    pdl_release();
+    dependent_wait();
+    dependent_release();
     long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int o = unit >= p.units[0];
     if (o) unit -= p.units[0];
@@ -614,26 +613,6 @@ struct Way {
                   grouped_us(q) < shape.us;
     }
 };
-
-// A launch that may begin beside the end of the kernel before it, which it waits for on the device.
-template <typename... P, typename... A>
-cudaError_t launch_dependent(void (*kernel)(P...), unsigned blocks, unsigned threads, size_t smem, int cluster, cudaStream_t stream, const A &...args)
-{
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(blocks);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)cluster;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
 
 template <typename Y>
 cudaError_t launch_typed(bool nk, const CUtensorMap &map_x, const CUtensorMap &map_w, const MatmulParams &p, const Shape &s, cudaStream_t stream)
