@@ -46,7 +46,7 @@ struct BalanceParams {
     int *piece_counts;                  // [blocks + sequences, experts]
     float *piece_sums;                  // the same
     int *seq_tokens;                    // [sequences]
-    double *seq_dots;                   // [sequences, ceil(experts / 32)]
+    double *seq_dots;                   // the same
 };
 
 constexpr float kInf = __builtin_huge_valf();
@@ -90,9 +90,9 @@ __device__ __forceinline__ float warp_sum(float v)
 }
 
 // Rows whose loads a warp has under way: at most four, and no more than there are registers for.
-__host__ __device__ constexpr int rows_ahead(int per, int bytes, int registers)
+template <typename T, int PER, int V> __host__ __device__ constexpr int rows_ahead(int registers)
 {
-    const int n = registers * 4 / (per * bytes);
+    const int n = registers * 4 / (PER * (V > 1 ? (int)sizeof(T) : 4));
     return n > 4 ? 4 : n < 1 ? 1 : n;
 }
 
@@ -257,7 +257,7 @@ __device__ __forceinline__ int seq_of_piece(const BalanceParams &p, int piece, i
 template <typename T, bool SIGMOID, int PER, int V, bool ALL>
 __global__ void __launch_bounds__(threads_of(PER), 1) balance_rows_kernel(const BalanceParams p)
 {
-    constexpr int R = rows_ahead(PER, sizeof(T), PER <= 8 ? 32 : 64);
+    constexpr int R = rows_ahead<T, PER, V>(PER <= 8 ? 16 : 32);
     extern __shared__ float4 smem[];    // sums [warps][experts], then the counts [experts]
     __shared__ int warp_tokens[32];
     __shared__ double warp_dots[32];
@@ -385,228 +385,211 @@ __device__ __forceinline__ void sum_pieces(const BalanceParams &p, int s, int fi
 
 // Few sequences: one cluster adds up their pieces, a CTA an eighth of the experts, and its first CTA makes the loss of what they put into
 // its shared memory.  (Through memory and a ticket, as below, that last step costs 2.7 us instead of a half.)
-constexpr int kFewSequences = 64, kFinishCtas = 8;
+constexpr int kFewSequences = 32, kFinishCtas = 8, kMostGroups = 1024 / (32 * kFinishCtas);
 __global__ void __launch_bounds__(1024, 1) balance_finish_few_kernel(const BalanceParams p)
 {
     __shared__ float sums[32][32];
     __shared__ int counts[32][32], tokens_of[kFewSequences];
-    __shared__ double dots[kFewSequences], all_dots[kFinishCtas][kFewSequences], warp_dots[2];
-    __shared__ int some;
+    __shared__ double dots[kFewSequences * kMostGroups], all_dots[kFinishCtas][kFewSequences];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = blockIdx.x;
-    const int groups = (p.experts + 32 * kFinishCtas - 1) / (32 * kFinishCtas);     // of 32 experts, a CTA's share
-    int each = 1;   // warps of a sequence
-    while (each * 2 * p.sequences <= 32) each *= 2;
+    // A CTA's items are a sequence and 32 experts each, for a power of two of warps.
+    const int groups = (p.experts + 32 * kFinishCtas - 1) / (32 * kFinishCtas), items = p.sequences * groups;
+    int each = 1;
+    while (each * 2 * items <= 32) each *= 2;
+    const int part = warp & (each - 1);
+    if (tid < kFewSequences) tokens_of[tid] = 0;
     dependent_wait();
     dependent_release();
-    if (tid < p.sequences) dots[tid] = 0.0;
-    if (tid == 0) some = 0;
-    const int part = warp & (each - 1);
-    for (int g = 0; g < groups; ++g) {
-        const int e = (rank * groups + g) * 32 + lane;
-        for (int s0 = 0; s0 < p.sequences; s0 += 32 / each) {
-            const int s = s0 + warp / each;
-            float sum = 0.0f;
-            int count = 0, tokens = 0;
-            if (s < p.sequences) sum_pieces<5>(p, s, part, each, e, sum, count, tokens);
-            sums[warp][lane] = sum;
-            counts[warp][lane] = count;
-            if (g == 0) {
-                __syncthreads();
-                if (lane == 0 && part == 0 && s < p.sequences) tokens_of[s] = 0;
-                __syncthreads();
-                if (lane == 0 && tokens) atomicAdd(tokens_of + s, tokens);
-            }
-            __syncthreads();
-            if (part == 0 && s < p.sequences) {
-                sum = 0.0f;
-                count = 0;
+    for (int item0 = 0; item0 < items; item0 += 32 / each) {
+        const int item = item0 + warp / each, s = item / groups, g = item - s * groups, e = (rank * groups + g) * 32 + lane;
+        float sum = 0.0f;
+        int count = 0, tokens = 0;
+        if (item < items) sum_pieces<5>(p, s, part, each, e, sum, count, tokens);
+        sums[warp][lane] = sum;
+        counts[warp][lane] = count;
+        __syncthreads();
+        if (item < items && g == 0 && lane == 0) atomicAdd(tokens_of + s, tokens);
+        if (item < items && part == 0) {
+            sum = 0.0f;
+            count = 0;
 #pragma unroll 8
-                for (int w = warp; w < warp + each; ++w) {
-                    sum += sums[w][lane];
-                    count += counts[w][lane];
-                }
-                if (e < p.experts) p.counts[(long long)s * p.experts + e] = count;
-                const double dot = warp_sum((double)sum * count);
-                if (lane == 0) dots[s] += dot;
+            for (int w = warp; w < warp + each; ++w) {
+                sum += sums[w][lane];
+                count += counts[w][lane];
             }
-            __syncthreads();
+            if (e < p.experts) p.counts[(long long)s * p.experts + e] = count;
+            const double dot = warp_sum((double)sum * count);
+            if (lane == 0) dots[item] = dot;
         }
+        __syncthreads();
     }
     if (tid < p.sequences) {
+        double dot = 0.0;
+        for (int g = 0; g < groups; ++g) dot += dots[tid * groups + g];
         uint32_t to;
         asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"((uint32_t)__cvta_generic_to_shared(&all_dots[rank][tid])));
-        asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(dots[tid]) : "memory");
-        if (tokens_of[tid] > 0) atomicAdd(&some, 1);
+        asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(dot) : "memory");
     }
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (rank != 0 || warp >= 2) return;
+    if (rank != 0 || warp != 0) return;
+    const int mine = lane < p.sequences ? tokens_of[lane] : 0;
+    const float weight = weight_of(p, mine, __popc(__ballot_sync(0xffffffffu, mine > 0)));
     double loss = 0.0;
-    if (tid < p.sequences) {
-        const float weight = weight_of(p, tokens_of[tid], some);
-        p.weight[tid] = weight;
+    if (lane < p.sequences) {
+        p.weight[lane] = weight;
 #pragma unroll
-        for (int r = 0; r < kFinishCtas; ++r) loss += all_dots[r][tid];
-        loss *= weight;
+        for (int r = 0; r < kFinishCtas; ++r) loss += all_dots[r][lane];
     }
-    loss = warp_sum(loss);
-    if (lane == 0) warp_dots[warp] = loss;
-    asm volatile("bar.sync 1, 64;" ::: "memory");
-    if (tid == 0) *p.loss = (float)(warp_dots[0] + warp_dots[1]);
+    loss = warp_sum(loss * weight);
+    if (lane == 0) *p.loss = (float)loss;
 }
 
-// Any number of sequences: the pieces of one, 32 experts a block; the block that comes last makes the loss of all.
-__global__ void __launch_bounds__(1024) balance_finish_kernel(const BalanceParams p)
+// Any number of sequences: a CTA adds up the pieces of one, which are few where sequences are many; the one that comes last makes the loss
+// of all.
+constexpr int kFinishThreads = 256;
+__global__ void __launch_bounds__(kFinishThreads) balance_finish_many_kernel(const BalanceParams p)
 {
-    __shared__ float sums[32][32];
-    __shared__ int counts[32][32], tokens_of[32];
-    __shared__ double warp_dots[32];
+    __shared__ double warp_dots[kFinishThreads / 32];
     __shared__ int last, some;
-    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = threads >> 5, s = blockIdx.x, parts = gridDim.y;
-    const int e = blockIdx.y * 32 + lane;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, s = blockIdx.x;
     dependent_wait();
     dependent_release();
-    float sum = 0.0f;
-    int count = 0, tokens = 0;
-    sum_pieces<4>(p, s, warp, warps, e, sum, count, tokens);
-    sums[warp][lane] = sum;
-    counts[warp][lane] = count;
-    if (lane == 0) tokens_of[warp] = tokens;
-    if (tid == 0) some = 0;
+    int tokens = 0;
+    double dot = 0.0;
+    for (int e = tid; e < p.experts; e += kFinishThreads) {
+        float sum = 0.0f;
+        int count = 0;
+        tokens = 0;
+        sum_pieces<4>(p, s, 0, 1, e, sum, count, tokens);
+        p.counts[(long long)s * p.experts + e] = count;
+        dot += (double)sum * count;
+    }
+    dot = warp_sum(dot);
+    if (lane == 0) warp_dots[warp] = dot;
     __syncthreads();
     if (warp == 0) {
-        sum = 0.0f;
-        count = 0;
-#pragma unroll 8
-        for (int w = 0; w < warps; ++w) {
-            sum += sums[w][lane];
-            count += counts[w][lane];
-        }
-        tokens = (int)__reduce_add_sync(0xffffffffu, lane < warps ? tokens_of[lane] : 0);
-        if (e < p.experts) p.counts[(long long)s * p.experts + e] = count;
-        const double dot = warp_sum((double)sum * count);
+        dot = warp_sum(lane < kFinishThreads / 32 ? warp_dots[lane] : 0.0);
         if (lane == 0) {
-            p.seq_dots[(long long)s * parts + blockIdx.y] = dot;
-            if (blockIdx.y == 0) p.seq_tokens[s] = tokens;
+            p.seq_dots[s] = dot;
+            p.seq_tokens[s] = tokens;
+            some = 0;
             __threadfence();
-            last = atomicAdd(p.ticket, 1) == p.sequences * parts - 1;
+            last = atomicAdd(p.ticket, 1) == p.sequences - 1;
         }
     }
     __syncthreads();
     if (!last) return;
     __threadfence();
     double loss = 0.0;
-    const auto dot_of = [&](int i) {
-        double dot = 0.0;
-#pragma unroll 8
-        for (int j = 0; j < parts; ++j) dot += __ldcg(p.seq_dots + (long long)i * parts + j);
-        return dot;
-    };
-    const double dot = tid < p.sequences ? dot_of(tid) : 0.0;   // of most calls all, under way with the tokens
     int mine = 0;
-    for (int i = tid; i < p.sequences; i += threads) mine += __ldcg(p.seq_tokens + i) > 0;
+    for (int i = tid; i < p.sequences; i += kFinishThreads) mine += __ldcg(p.seq_tokens + i) > 0;
     if (mine) atomicAdd(&some, mine);
     __syncthreads();
-    for (int i = tid; i < p.sequences; i += threads) {
+    for (int i = tid; i < p.sequences; i += kFinishThreads) {
         const float weight = weight_of(p, __ldcg(p.seq_tokens + i), some);
         p.weight[i] = weight;
-        loss += (i == tid ? dot : dot_of(i)) * weight;
+        loss += __ldcg(p.seq_dots + i) * weight;
     }
     loss = warp_sum(loss);
     if (lane == 0) warp_dots[warp] = loss;
     __syncthreads();
     if (warp == 0) {
-        loss = warp_sum(lane < warps ? warp_dots[lane] : 0.0);
+        loss = warp_sum(lane < kFinishThreads / 32 ? warp_dots[lane] : 0.0);
         if (lane == 0) *p.loss = (float)loss;
     }
 }
 
 template <typename T, bool SIGMOID, int PER, int V>
-__global__ void __launch_bounds__(kGradThreads) balance_grad_kernel(const BalanceParams p)
+__global__ void __launch_bounds__(kGradThreads, PER <= 8 ? 4 : 2) balance_grad_kernel(const BalanceParams p)
 {
-    constexpr int R = rows_ahead(PER, sizeof(T), 16);
+    constexpr int R = rows_ahead<T, PER, V>(PER <= 8 ? 16 : 32);
     const int lane = threadIdx.x & 31, row0 = (blockIdx.x * kGradWarps + (threadIdx.x >> 5)) * p.chunk, row1 = min(row0 + p.chunk, p.rows);
     dependent_wait();
     dependent_release();
     if (row0 >= row1) return;
+    RawRow<T, PER, V> rows[R];
+    int8_t mask[R];
+    const auto fetch = [&](int batch) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (batch + r >= row1) break;
+            rows[r].load(static_cast<const T *>(p.logits) + (batch + r) * p.ld, p.experts, lane);
+            mask[r] = p.mask ? p.mask[batch + r] : 1;
+        }
+    };
+    fetch(row0);
     const float grad_loss = p.grad_loss ? *p.grad_loss : 1.0f;
     int s = seq_of(p, row0, lane), known = -1, begin = 0, end = 0;
     f32x2 load[PER / 2];
     float factor = 0.0f;
-    RawRow<T, PER, V> rows[R];
     for (int batch = row0; batch < row1; batch += R) {
-    int8_t mask[R];
+        if (batch > row0) fetch(batch);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        if (batch + r >= row1) break;
-        rows[r].load(static_cast<const T *>(p.logits) + (batch + r) * p.ld, p.experts, lane);
-        mask[r] = p.mask ? p.mask[batch + r] : 1;
-    }
+        for (int r = 0; r < R; ++r) {
+            const int row = batch + r;
+            if (row >= row1) break;
+            while (row >= end && s < p.sequences) {
+                begin = seq_begin(p, s);
+                end = seq_end(p, s);
+                if (row >= end) ++s;
+            }
+            const bool token = row >= begin && row < end && mask[r] != 0;
+            f32x2 g[PER / 2] = {};
+            if (token) {
+                if (known != s) {
+                    // Counts less a whole number near their mean: the difference from the row's mean of them, which is what the gradient is made
+                    // of, does not lose its places to what they all have in common.
+                    known = s;
+                    const long long *counts = p.counts + (long long)s * p.experts;
+                    factor = __fmul_rn(p.weight[s], grad_loss);
+                    long long count[PER];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int row = batch + r;
-        if (row >= row1) break;
-        while (row >= end && s < p.sequences) {
-            begin = seq_begin(p, s);
-            end = seq_end(p, s);
-            if (row >= end) ++s;
-        }
-        const bool token = row >= begin && row < end && mask[r] != 0;
-        f32x2 g[PER / 2] = {};
-        if (token) {
-            if (known != s) {
-                // Counts less a whole number near their mean: the difference from the row's mean of them, which is what the gradient is made
-                // of, does not lose its places to what they all have in common.
-                known = s;
-                const long long *counts = p.counts + (long long)s * p.experts;
-                factor = __fmul_rn(p.weight[s], grad_loss);
-                long long count[PER];
-#pragma unroll
-                for (int i = 0; i < PER; i += V > 1 ? 2 : 1) {
-                    const int e = expert_of<V>(i, lane);
-                    if constexpr (V > 1) {
-                        const longlong2 two = e < p.experts ? *reinterpret_cast<const longlong2 *>(counts + e) : make_longlong2(0, 0);
-                        count[i] = two.x;
-                        count[i + 1] = two.y;
-                    } else {
-                        count[i] = e < p.experts ? counts[e] : 0;
+                    for (int i = 0; i < PER; i += V > 1 ? 2 : 1) {
+                        const int e = expert_of<V>(i, lane);
+                        if constexpr (V > 1) {
+                            const longlong2 two = e < p.experts ? *reinterpret_cast<const longlong2 *>(counts + e) : make_longlong2(0, 0);
+                            count[i] = two.x;
+                            count[i + 1] = two.y;
+                        } else {
+                            count[i] = e < p.experts ? counts[e] : 0;
+                        }
                     }
+                    float total = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < PER; ++i) total += (float)count[i];
+                    const long long base = (long long)(warp_sum(total) / (float)p.experts);
+#pragma unroll
+                    for (int i = 0; i < PER; i += 2) load[i / 2] = pair2((float)(count[i] - base), (float)(count[i + 1] - base));
                 }
-                float total = 0.0f;
+                f32x2 l[PER / 2], e[PER / 2], rest[PER / 2], mean2 = 0;
+                float inv;
+                rows[r].values(l);
+                scores<SIGMOID, PER>(l, e, rest, inv);
 #pragma unroll
-                for (int i = 0; i < PER; ++i) total += (float)count[i];
-                const long long base = (long long)(warp_sum(total) / (float)p.experts);
+                for (int i = 0; i < PER / 2; ++i) mean2 = fma2(e[i], load[i], mean2);
+                const float2 parts = unpair2(mean2);
+                const float mean = -__fmul_rn(warp_sum(parts.x + parts.y), inv), scale = __fmul_rn(inv, factor);
 #pragma unroll
-                for (int i = 0; i < PER; i += 2) load[i / 2] = pair2((float)(count[i] - base), (float)(count[i + 1] - base));
+                for (int i = 0; i < PER / 2; ++i) {
+                    g[i] = mul2(mul2(e[i], pair2(scale, scale)), add2(load[i], pair2(mean, mean)));
+                    if (SIGMOID) g[i] = mul2(g[i], rest[i]);
+                }
             }
-            f32x2 l[PER / 2], e[PER / 2], rest[PER / 2], mean2 = 0;
-            float inv;
-            rows[r].values(l);
-            scores<SIGMOID, PER>(l, e, rest, inv);
+            T *to = static_cast<T *>(p.grad) + row * p.ld_grad;
 #pragma unroll
-            for (int i = 0; i < PER / 2; ++i) mean2 = fma2(e[i], load[i], mean2);
-            const float2 parts = unpair2(mean2);
-            const float mean = -__fmul_rn(warp_sum(parts.x + parts.y), inv), scale = __fmul_rn(inv, factor);
-#pragma unroll
-            for (int i = 0; i < PER / 2; ++i) {
-                g[i] = mul2(mul2(e[i], pair2(scale, scale)), add2(load[i], pair2(mean, mean)));
-                if (SIGMOID) g[i] = mul2(g[i], rest[i]);
+            for (int i = 0; i < PER; i += V) {
+                const int e = expert_of<V>(i, lane);
+                if (e >= p.experts) continue;
+                if constexpr (V > 1) *reinterpret_cast<uint4 *>(to + e) = pack<T>(g + i / 2);
+                else to[e] = from_float<T>(element(g, i));
             }
         }
-        T *to = static_cast<T *>(p.grad) + row * p.ld_grad;
-#pragma unroll
-        for (int i = 0; i < PER; i += V) {
-            const int e = expert_of<V>(i, lane);
-            if (e >= p.experts) continue;
-            if constexpr (V > 1) *reinterpret_cast<uint4 *>(to + e) = pack<T>(g + i / 2);
-            else to[e] = from_float<T>(element(g, i));
-        }
-    }
     }
 }
 
-#include <cstdlib>
-static const int kAllRows = getenv("BAL_ALL") ? atoi(getenv("BAL_ALL")) : 64;    // most rows that one block takes by itself
+// Most rows that one CTA takes by itself (256 experts, bf16: 64 rows 4.1 us against 6.5 with more CTAs and a second kernel, 128 5.5, 192 6.6).
+constexpr int kAllRows = 128;
 
 size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
@@ -673,13 +656,13 @@ struct Layout {
         const int64_t wanted = at_once() >= 2 * b.sequences ? at_once() - b.sequences + 1 : at_once() / 2, each = (b.rows + wanted - 1) / wanted;
         chunk = (int)(each < warps ? warps : each);
         blocks = (int)((b.rows + chunk - 1) / chunk);
-        const size_t pieces = (size_t)blocks + (size_t)b.sequences, parts = ((size_t)b.experts + 31) / 32;
+        const size_t pieces = (size_t)blocks + (size_t)b.sequences;
         tokens = 256;
         counts = tokens + align256(pieces * 4);
         sums = counts + align256(pieces * b.experts * 4);
         seq_tokens = sums + align256(pieces * b.experts * 4);
         seq_dots = seq_tokens + align256((size_t)b.sequences * 4);
-        bytes = seq_dots + align256((size_t)b.sequences * parts * 8);
+        bytes = seq_dots + align256((size_t)b.sequences * 8);
     }
 };
 
@@ -719,10 +702,7 @@ cudaError_t balance_launch(const BalanceProblem &b, void *workspace, size_t work
     });
     if (e != cudaSuccess || all) return e;
     if (b.sequences <= kFewSequences) return launch_dependent(balance_finish_few_kernel, dim3(kFinishCtas), 1024, 0, kFinishCtas, stream, p);
-    // four pieces a warp, of the most that a sequence has on average
-    const int64_t finish_warps = (p.blocks / b.sequences + 1 + 3) / 4;
-    return launch_dependent(balance_finish_kernel, dim3((unsigned)b.sequences, (unsigned)(b.experts + 31) / 32),
-                            (unsigned)(finish_warps < 4 ? 128 : finish_warps > 32 ? 1024 : finish_warps * 32), 0, 1, stream, p);
+    return launch_dependent(balance_finish_many_kernel, dim3((unsigned)b.sequences), kFinishThreads, 0, 1, stream, p);
 }
 
 cudaError_t balance_grad_launch(const BalanceProblem &b, cudaStream_t stream)

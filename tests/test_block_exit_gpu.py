@@ -415,8 +415,9 @@ def check_balance(logits, ids, scoring="softmax", coefficient=0.01, mask=None, c
     assert loss.shape == () and loss.dtype == F32 and weight.dtype == F32
     assert torch.equal(counts, want_counts[0] if cu is None else want_counts)
     assert ((weight.double() - want_weight).abs() <= want_weight.abs() * 2 * U32).all()
-    # a score's sum over tokens goes through rows / 8 / blocks of 8 warps (at most 64) and as many blocks (at most 37)
-    chain = t / 296 / 8 + 8 + 37 + 16
+    # additions that a score's sum over tokens goes through: a warp's rows (of 32 warps on 148 SMs), the 32 warps, a warp's share of at most
+    # 148 + 1 pieces, the 32 warps
+    chain = t / 148 / 32 + 1 + 32 + 149 / 32 + 1 + 32
     assert abs(loss.item() - want.item()) <= abs(want.item()) * (error_of_scores(logits, scoring) + (chain + 4) * U32) + 1e-38
     grad = ops.expert_balance_grad(logits, counts, weight, grad_loss=grad_loss, **kw)
     check_grad(grad, logits, scoring, want_grad, p, c, up)
