@@ -655,8 +655,6 @@ def expert_balance(logits: torch.Tensor, ids: torch.Tensor, *, scoring: str = "s
         counts = empty(logits, "l", logits.shape[-1]) if cu_seqlens is None else empty(logits, "l", sequences, logits.shape[-1])
     if weight is None:
         weight = empty(logits, "f", sequences)
-    if token_mask is not None and token_mask.dtype == torch.bool:
-        token_mask = token_mask.view(torch.int8)
     _block_call(_lib.OP_EXPERT_BALANCE, "gmmB200ExpertBalance", workspace, None, None, "tttttttii", logits, ids, token_mask, cu_seqlens, loss, counts,
                 weight, _SCORING[scoring], _float_bits(coefficient))
     return loss, counts, weight
@@ -677,8 +675,6 @@ def expert_balance_grad(logits: torch.Tensor, counts: torch.Tensor, weight: torc
         raise ValueError(f"unknown scoring {scoring!r}")
     if grad is None:
         grad = _lib.native()[0].empty(logits, "=")
-    if token_mask is not None and token_mask.dtype == torch.bool:
-        token_mask = token_mask.view(torch.int8)
     _block_call(_lib.OP_EXPERT_BALANCE_GRAD, "gmmB200ExpertBalanceGrad", workspace, None, None, "ttttttti", logits, counts, weight,
                 token_mask, cu_seqlens, grad_loss, grad, _SCORING[scoring])
     return grad

@@ -4,8 +4,11 @@
   2. router projection (a matrix product of torch) and ``route_top_k``
   3. ``moe_init_routing_v3``: the int8 rows and their scales grouped by expert, without another quantisation
   4. ``grouped_matmul_swiglu_quant`` over the experts' rows, and over all rows for the shared expert
-  5. ``grouped_matmul_v4``: the shared expert's down projection, with ``adapter_add`` for the requests that bring an adapter to it
+  5. ``quant_matmul``: the shared expert's down projection, with ``adapter_add`` for the requests that bring an adapter to it
   6. ``grouped_matmul_finalize_routing``: the experts' down projection, weighted and added onto the shared expert's rows
+  7. where the next block's weights are at hand, ``sandwich_norm_quant``: what this block puts out, through its own norm, gate and residual
+     sum, into the int8 rows that the next one begins with at step 3
+  8. on request, ``expert_balance``: how the step's tokens load the experts, and the loss that evens them out
 
 Nothing is read back to the host, so a step can be captured in a CUDA graph; padded rows of such a batch are named by ``token_mask``.
 ``python -m ops_transformer_b200.block`` runs a small one.
@@ -13,12 +16,12 @@ Nothing is read back to the host, so a step can be captured in a CUDA graph; pad
 from __future__ import annotations
 
 import dataclasses
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
-from .acl import (adapter_add, add_rms_norm_quant, format_cast_nz, grouped_matmul_finalize_routing, grouped_matmul_swiglu_quant,
-                  grouped_matmul_v4, moe_init_routing_v3, route_top_k)
+from .acl import (adapter_add, add_rms_norm_quant, expert_balance, format_cast_nz, grouped_matmul_finalize_routing,
+                  grouped_matmul_swiglu_quant, moe_init_routing_v3, quant_matmul, route_top_k, sandwich_norm_quant)
 
 
 @dataclasses.dataclass
@@ -28,6 +31,33 @@ class Adapters:
     a: torch.Tensor
     b: torch.Tensor
     scaling: Optional[torch.Tensor] = None
+
+
+class Entered(NamedTuple):
+    """What a block begins with once its norm is done: int8 rows, their scales, the residual stream and the rows in 16 bits."""
+    rows: torch.Tensor
+    scales: torch.Tensor
+    stream: torch.Tensor
+    normed: torch.Tensor
+
+
+@dataclasses.dataclass
+class BlockExit:
+    """The way from a block's output into the next block: ``gamma`` of the next block's norm, and the optional parts of
+    ``sandwich_norm_quant`` that the model has (the block's own norm, its gate, the scales of the residual sum)."""
+    gamma: torch.Tensor
+    post_gamma: Optional[torch.Tensor] = None
+    gate: Optional[torch.Tensor] = None
+    gate_act: str = "none"
+    residual_scale: float = 1.0
+    block_scale: float = 1.0
+    eps: float = 1e-6
+    post_eps: Optional[float] = None
+
+    def __call__(self, out, stream) -> Entered:
+        return Entered(*sandwich_norm_quant(out, stream, self.gamma, post_gamma=self.post_gamma, gate=self.gate, gate_act=self.gate_act,
+                                            residual_scale=self.residual_scale, block_scale=self.block_scale, eps=self.eps,
+                                            post_eps=self.post_eps, normed=True))
 
 
 class QuantMoeBlock:
@@ -47,13 +77,22 @@ class QuantMoeBlock:
                             renormalize=renormalize)
         self.eps, self.adapters = eps, adapters
 
-    def __call__(self, x, residual, *, adapter_ids=None, token_mask=None):
-        """(the block's output fp32 [tokens, hidden], the new residual stream) for the layer's hidden states ``x`` and ``residual``.
-        ``adapter_ids`` (int32 [tokens]): the adapter of every token, negative for none.  ``token_mask``: rows without a token, which take
-        part in no expert."""
-        tokens, E = x.shape[0], self.experts
-        rows, scales, stream, normed = add_rms_norm_quant(x, self.gamma, residual=residual, eps=self.eps, normed=True)
-        weights, ids = route_top_k(normed @ self.router, self.top_k, bias=self.router_bias, token_mask=token_mask, **self.routing)
+    def __call__(self, x, residual=None, *, adapter_ids=None, token_mask=None, leave: Optional[BlockExit] = None,
+                 balance: Optional[float] = None):
+        """(the block's output fp32 [tokens, hidden], the new residual stream) for the layer's hidden states ``x`` and ``residual``.  ``x`` may
+        be what the block before left as ``Entered``, without a residual; with ``leave`` that is what this one returns for the next, in
+        the place of the two.  ``adapter_ids`` (int32 [tokens]): the adapter of every token, negative for none.  ``token_mask``: rows without a
+        token, which take part in no expert.  With ``balance``, a coefficient, the load of the experts follows: ``expert_balance``'s
+        (loss, counts, weight)."""
+        if isinstance(x, Entered):
+            if residual is not None:
+                raise ValueError("rows that have entered the block bring their residual stream")
+            rows, scales, stream, normed = x
+        else:
+            rows, scales, stream, normed = add_rms_norm_quant(x, self.gamma, residual=residual, eps=self.eps, normed=True)
+        tokens, E = rows.shape[0], self.experts
+        logits = normed @ self.router
+        weights, ids = route_top_k(logits, self.top_k, bias=self.router_bias, token_mask=token_mask, **self.routing)
 
         pairs = tokens * self.top_k
         # pairs without an expert leave rows behind, which must name a pair all the same
@@ -64,15 +103,19 @@ class QuantMoeBlock:
         act, act_scales = grouped_matmul_swiglu_quant(ex, self.w_gate_up, self.s_gate_up, ex_scales, counts.cumsum(0))
 
         gate_up, s_gate_up, down, s_down = self.shared
-        every = torch.full((1,), tokens, dtype=torch.int64, device=x.device)
+        every = torch.full((1,), tokens, dtype=torch.int64, device=rows.device)
         shared_act, shared_scales = grouped_matmul_swiglu_quant(rows, gate_up, s_gate_up, scales, every)
-        shared = grouped_matmul_v4(shared_act, down, s_down, shared_scales, every)
+        shared = quant_matmul(shared_act, down[0], s_down[0], shared_scales)
         if self.adapters is not None and adapter_ids is not None:
             adapter_add(shared, shared_act, self.adapters.a, self.adapters.b, adapter_ids, x_scale=shared_scales, scaling=self.adapters.scaling,
                         out=shared)
         out = grouped_matmul_finalize_routing(act, self.w_down, self.s_down, counts, pair_of_row // self.top_k, tokens, pertoken_scale=act_scales,
                                               logit=weights.view(-1)[pair_of_row], shared_input=shared)
-        return out, stream
+        result = (out, stream) if leave is None else leave(out, stream)
+        if balance is None:
+            return result
+        load = expert_balance(logits, ids, scoring=self.routing["scoring"], coefficient=balance, token_mask=token_mask)
+        return (*result, load) if leave is None else (result, load)
 
 
 def random_block(hidden: int, inter: int, experts: int, top_k: int, *, adapters: int = 0, rank: int = 16, seed: int = 0, device="cuda", **routing):
@@ -91,17 +134,23 @@ def random_block(hidden: int, inter: int, experts: int, top_k: int, *, adapters:
 
 def main():
     tokens, hidden, adapters = 128, 2048, 8
-    block = random_block(hidden, 768, 64, 8, adapters=adapters, scoring="sigmoid", n_group=8, topk_group=4, group_score="top2",
-                         router_bias=torch.zeros(64, device="cuda"), routed_scale=2.5)
+    first, second = (random_block(hidden, 768, 64, 8, adapters=adapters, scoring="sigmoid", n_group=8, topk_group=4, group_score="top2",
+                                  router_bias=torch.zeros(64, device="cuda"), routed_scale=2.5, seed=seed) for seed in (0, 1))
+    between = BlockExit(second.gamma, post_gamma=torch.ones_like(second.gamma))
     g = torch.Generator("cuda").manual_seed(1)
     x, residual = (torch.randn(tokens, hidden, device="cuda", generator=g).to(torch.bfloat16) for _ in range(2))
     adapter_ids = (torch.arange(tokens, device="cuda") % (adapters + 1) - 1).to(torch.int32)
     mask = torch.arange(tokens, device="cuda") < 120
-    out, stream = block(x, residual, adapter_ids=adapter_ids, token_mask=mask)
+
+    def step():
+        entered, load = first(x, residual, adapter_ids=adapter_ids, token_mask=mask, leave=between, balance=0.01)
+        return *second(entered, adapter_ids=adapter_ids, token_mask=mask), load
+
+    step()
     start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        out, stream = block(x, residual, adapter_ids=adapter_ids, token_mask=mask)
+        out, stream, (loss, counts, _) = step()
     for _ in range(3):
         graph.replay()
     start.record()
@@ -109,8 +158,9 @@ def main():
         graph.replay()
     end.record()
     torch.cuda.synchronize()
-    print(f"{tokens} tokens of {hidden}, 64 experts (top 8) and {adapters} adapters: {start.elapsed_time(end) / 20 * 1e3:.1f} us a step, "
-          f"rms of the output {out.square().mean().sqrt().item():.3f}, finite {bool(out.isfinite().all())}")
+    print(f"two blocks, {tokens} tokens of {hidden}, 64 experts (top 8) and {adapters} adapters: {start.elapsed_time(end) / 20 * 1e3:.1f} us a step, "
+          f"rms of the output {out.square().mean().sqrt().item():.3f}, finite {bool(out.isfinite().all())}, "
+          f"busiest expert of the first {int(counts.max())} of {int(counts.sum())} choices, balance loss {loss.item():.4f}")
 
 
 if __name__ == "__main__":

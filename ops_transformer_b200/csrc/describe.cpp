@@ -24,6 +24,7 @@ int acl_dtype(at::ScalarType t)
         case at::kChar: return 2;
         case at::kInt: return 3;
         case at::kLong: return 9;
+        case at::kBool: return 12;
         case at::kBFloat16: return 27;
         default: return -1;
     }

@@ -652,3 +652,106 @@ def test_operators_from_several_threads():
     for t in threads:
         t.join()
     assert not failed
+
+
+@pytest.mark.parametrize("m,k,n", [(16, 1024, 256), (256, 512, 18944), (600, 384, 640)])
+def test_matmul_reports_a_wait_that_runs_out(m, k, n):
+    """The producer leaves out the last K block of every CTA and the others wait for about 1 ms: the call ends, says so in its status, and the next
+    one on the same workspace is right.  Cluster of several CTAs, and one CTA a tile."""
+    x, w, scale = int8((m, k), 1), int8((k, n), 2), rand((n,), 3) + 0.5
+    want = plain_matmul(x, w, scale, None, None, BF16)
+    y, ws = ops.quant_matmul(x, w, scale, return_workspace=True)
+    ops.check_status(ws)
+    assert torch.equal(y, want)
+    ws = torch.zeros(ws.numel(), dtype=torch.uint8, device=DEV)
+    ops.quant_matmul(x, w, scale, out=torch.empty_like(y), workspace=ws, options=ops.LaunchOptions(wait_limit_cycles=2_000_000, test_skip_k_blocks=1))
+    with pytest.raises(ops.AclnnError):
+        ops.check_status(ws)
+    again = ops.quant_matmul(x, w, scale, out=torch.zeros_like(y), workspace=ws)
+    ops.check_status(ws)
+    assert torch.equal(again, want)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# all of them as a decoder layer runs them: block, exit, next block, load
+# ---------------------------------------------------------------------------------------------------------------------
+
+def chain(tokens, hidden=512, inter=256, experts=8, top_k=2, scoring="softmax"):
+    from ops_transformer_b200.block import BlockExit, random_block
+    first, second = (random_block(hidden, inter, experts, top_k, adapters=2, scoring=scoring, seed=s) for s in (0, 1))
+    leave = BlockExit(second.gamma, post_gamma=randn((hidden,), 5, BF16, 0.1) + 1, gate=randn((hidden,), 6, BF16), gate_act="sigmoid", residual_scale=0.75,
+                      block_scale=1.25)
+    return first, second, leave
+
+
+@pytest.mark.parametrize("tokens,scoring", [(1, "softmax"), (40, "sigmoid"), (300, "softmax")])
+def test_blocks_in_a_row(monkeypatch, tokens, scoring):
+    from ops_transformer_b200 import block as module
+    first, second, leave = chain(tokens, scoring=scoring)
+    x, residual = randn((tokens, 512), 1, BF16), randn((tokens, 512), 2, BF16)
+    adapter_ids, mask = (torch.arange(tokens, device=DEV) % 3 - 1).to(I32), torch.arange(tokens, device=DEV) % 5 != 3
+    kw = dict(adapter_ids=adapter_ids, token_mask=mask)
+    out, stream = first(x, residual, **kw)
+    routed = []
+    with monkeypatch.context() as m:
+        m.setattr(module, "route_top_k", lambda logits, k, _f=module.route_top_k, **kw: routed.append((logits, *_f(logits, k, **kw))) or routed[-1][1:])
+        entered, (loss, counts, weight) = first(x, residual, leave=leave, balance=0.01, **kw)
+        got, got_stream, load = second(entered, balance=0.02, **kw)
+    # the way out, from `out` as another run of the block gives it: its rows are added up in no fixed order, a few units of fp32 of their
+    # size, below 2^-16 of the largest value, which the norms pass on about as large
+    n = out.double() * (out.double().square().mean(1, keepdim=True) + 1e-6).rsqrt() * leave.post_gamma.double()
+    s = 0.75 * stream.double() + 1.25 * torch.sigmoid(leave.gate.double()) * n
+    u = s * (s.square().mean(1, keepdim=True) + 1e-6).rsqrt() * second.gamma.double()
+    near = 2.0 ** -15 * s.abs().amax(1, keepdim=True)
+    assert ((entered.stream.double() - s).abs() <= s.abs() * 2.0 ** -8 + near).all()
+    near = 2.0 ** -14 * u.abs().amax(1, keepdim=True)
+    assert ((entered.normed.double() - u).abs() <= u.abs() * 2.0 ** -8 * 1.01 + near).all()
+    assert ((entered.rows * entered.scales.double()[:, None] - u).abs() <= entered.scales.double()[:, None] * 0.501 + near).all()
+    # the next block takes the rows as its own norm would have left them
+    want = second(module.Entered(*entered), **kw)
+    assert torch.equal(got_stream, entered.stream) and torch.equal(want[1], entered.stream)
+    assert (got - want[0]).abs().max() < 64 * U32 * math.sqrt(512)
+    for (logits, _, ids), (loss, counts, weight), coefficient in ((routed[0], (loss, counts, weight), 0.01), (routed[1], load, 0.02)):
+        f32 = torch.tensor(coefficient, dtype=F32).item()
+        want = plain_balance(logits, ids, scoring, f32, mask)
+        assert torch.equal(counts, want[1][0]) and int(counts.sum()) == int(mask.sum()) * 2
+        assert abs(loss.item() - want[0].item()) <= abs(want[0].item()) * (error_of_scores(logits, scoring) + 80 * U32)
+
+
+def test_blocks_in_a_row_can_be_captured():
+    first, second, leave = chain(24)
+    x, residual = randn((24, 512), 1, BF16), randn((24, 512), 2, BF16)
+    mask = torch.arange(24, device=DEV) < 20
+
+    def step():
+        entered, load = first(x, residual, token_mask=mask, leave=leave, balance=0.01)
+        return *second(entered, token_mask=mask), *load
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    x.copy_(randn((24, 512), 3, BF16))
+    mask[:4] = False
+    graph.replay()
+    got = [o.clone() for o in outs]
+    want = step()
+    # rows are added into the first block's result in no fixed order, which an int8 row of the second may round to its other neighbour
+    assert torch.equal(got[3], want[3]) and torch.equal(got[4], want[4]) and torch.equal(got[2], want[2])
+    assert ((got[1].double() - want[1].double()).abs() <= want[1].double().abs() * 2.0 ** -7 + 2.0 ** -15).all()
+    assert (got[0] - want[0]).norm() <= 0.01 * want[0].norm()
+
+
+def test_block_takes_one_residual_stream():
+    first, second, leave = chain(4)
+    entered = first(randn((4, 512), 1, BF16), randn((4, 512), 2, BF16), leave=leave)
+    with pytest.raises(ValueError, match="residual"):
+        second(entered, randn((4, 512), 2, BF16))
+
+
+def test_shared_expert_as_the_grouped_product_gives_it():
+    """The block's shared expert goes through quant_matmul; its rows are those of the grouped product with one group."""
+    for m, k, n in ((1, 256, 512), (40, 512, 1024), (300, 256, 768)):
+        x, w, scale, token = int8((m, k), 1), int8((1, k, n), 2), rand((1, n), 3) * 0.01, rand((m,), 4)
+        group = torch.full((1,), m, dtype=I64, device=DEV)
+        assert torch.equal(ops.quant_matmul(x, w[0], scale[0], token), ops.grouped_matmul_v4(x, w, scale, token, group))
