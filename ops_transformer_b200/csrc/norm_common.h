@@ -149,14 +149,17 @@ __device__ __forceinline__ float step_of(float m)
     return __fmaf_rn(__fmaf_rn(-q, 127.0f, m), r, q);
 }
 
+// 16 bytes.  LATE: not to be read before a wait for the kernel before, behind which the compiler would let a load of constants go.
+template <bool LATE, typename P> __device__ __forceinline__ P load16(const P *p) { return LATE ? *p : __ldg(p); }
+
 // V elements from `at` on, which stands anywhere: 16-bit weights out of two aligned packs where these lie inside, else one by one.
-template <typename G, int V>
+template <typename G, int V, bool LATE = false>
 __device__ __forceinline__ void load_anywhere(const G *g, int at, int h, f32x2 *f)
 {
     if constexpr (sizeof(G) == 2 && V == 8) {
         const int lo = at & ~7, shift = at & 7;
         if (at >= 0 && lo + 16 <= h) {
-            const uint4 a = __ldg(reinterpret_cast<const uint4 *>(g + lo)), b = __ldg(reinterpret_cast<const uint4 *>(g + lo + 8));
+            const uint4 a = load16<LATE>(reinterpret_cast<const uint4 *>(g + lo)), b = load16<LATE>(reinterpret_cast<const uint4 *>(g + lo + 8));
             uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
             if (shift & 4) { w[0] = w[2]; w[1] = w[3]; w[2] = w[4]; w[3] = w[5]; w[4] = w[6]; w[5] = w[7]; }
             if (shift & 2) { w[0] = w[1]; w[1] = w[2]; w[2] = w[3]; w[3] = w[4]; w[4] = w[5]; }
@@ -170,12 +173,12 @@ __device__ __forceinline__ void load_anywhere(const G *g, int at, int h, f32x2 *
 #pragma unroll
     for (int e = 0; e < V; e += 2) f[e / 2] = pair2(one(at + e), one(at + e + 1));
 }
-template <int V>
+template <int V, bool LATE = false>
 __device__ __forceinline__ void load_fp32(const float *g, f32x2 *f)
 {
 #pragma unroll
     for (int e = 0; e < V; e += 4) {
-        const float4 v = __ldg(reinterpret_cast<const float4 *>(g + e));
+        const float4 v = load16<LATE>(reinterpret_cast<const float4 *>(g + e));
         f[e / 2] = pair2(v.x, v.y);
         f[e / 2 + 1] = pair2(v.z, v.w);
     }

@@ -8,6 +8,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "dependent.h"
 #include "gmm_common.h"
 #include "norm_common.h"
 
@@ -45,6 +46,8 @@ template <typename T, typename X>
 __global__ void __launch_bounds__(256) sandwich_any_kernel(const SandwichParams p)
 {
     __shared__ float2 red[2][32];
+    dependent_wait();
+    dependent_release();
     const long long row = blockIdx.x;
     const X *x = static_cast<const X *>(p.x) + row * p.ld_x;
     const T *residual = static_cast<const T *>(p.residual) + row * p.ld_residual, *gate = static_cast<const T *>(p.gate) + row * p.ld_gate;
@@ -98,9 +101,9 @@ template <typename G, int V, bool WHOLE>
 __device__ __forceinline__ void load_channels(const void *vec, int at, int h, f32x2 *f)
 {
     const G *g = static_cast<const G *>(vec);
-    if constexpr (!WHOLE) load_anywhere<G, V>(g, at, h, f);
-    else if constexpr (sizeof(G) == 4) load_fp32<V>(g + at, f);
-    else unpack<G>(__ldg(reinterpret_cast<const uint4 *>(g + at)), f);
+    if constexpr (!WHOLE) load_anywhere<G, V, true>(g, at, h, f);
+    else if constexpr (sizeof(G) == 4) load_fp32<V, true>(g + at, f);
+    else unpack<G>(load16<true>(reinterpret_cast<const uint4 *>(g + at)), f);
 }
 
 template <typename T, int V, bool WHOLE>
@@ -118,6 +121,8 @@ __global__ void __launch_bounds__(MAXT, MINB) sandwich_kernel(const SandwichPara
 {
     constexpr int V = 16 / (int)sizeof(T);
     __shared__ float2 red[2][32];
+    dependent_wait();
+    dependent_release();
     const int threads = blockDim.x;
     const bool rows_gate = p.gate && p.ld_gate != 0 && p.gate_step != 0;
     const long long row = blockIdx.x;
@@ -287,8 +292,8 @@ __global__ void __launch_bounds__(MAXT, MINB) sandwich_kernel(const SandwichPara
 // turn has no loads but its own.  Those come as one bulk copy a tensor, for the next row as soon as the group holds this one in registers.
 // (With a 16-byte cp.async for each pack an SM takes in 16 bytes per ns however many are under way: 4096 x 7168 in 80 us.)  A group's
 // threads hold two packs each; four would leave too few rows in turn for the chain load, sum, load, sum, store of each.
-// 4096 x 7168, fp32 x, bf16 stream: 53.6 us with int8 rows (270 MB, 4.9 TB/s), 49.7 with bf16 rows and a gate (294 MB, 5.9 TB/s); 5001
-// channels, whose rows begin anywhere, 53.8.  Quantising costs what the difference is: max, step and rounding are the issue slots' work.
+// 4096 x 7168, fp32 x, bf16 stream: 53.3 us with int8 rows (270 MB, 5.1 TB/s), 49.0 with bf16 rows and a gate (294 MB, 6.0 TB/s); 5001
+// channels, whose rows begin anywhere, 52.7.  Quantising costs what the difference is: max, step and rounding are the issue slots' work.
 constexpr int kGroupPacks = 2, kMaxGroups = 14, kMaxDepth = 3;    // of the 15 named barriers that are left
 constexpr long long kWaitLimitCycles = 1ll << 31;  // about a second
 constexpr int kGroupThreads = 1024;
@@ -394,6 +399,10 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&rest_landed[group][d])) : "memory");
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    dependent_wait();
+    dependent_release();
+    if (tid == 0) {
         for (int d = 0; d < depth && row + d * step < p.rows; ++d) {
             fetch_x(row + d * step, d);
             fetch_rest(row + d * step, d);
@@ -653,8 +662,7 @@ cudaError_t launch_rows(const SandwichParams &p, const Groups &g, cudaStream_t s
         done_mask |= 1ull << (dev & 63);
     }
     const int ctas = (p.rows + g.groups - 1) / g.groups;
-    kernel<<<ctas < 148 ? ctas : 148, g.threads * g.groups, g.smem, stream>>>(p, g.threads, g.groups, g.depth);
-    return cudaGetLastError();
+    return launch_dependent(kernel, dim3(ctas < 148 ? ctas : 148), g.threads * g.groups, g.smem, 1, stream, p, g.threads, g.groups, g.depth);
 }
 
 template <typename T, typename X, bool WHOLE>
@@ -668,23 +676,18 @@ cudaError_t launch_packed(const SandwichParams &p, cudaStream_t stream)
     // an fp32 x: 148 x 7168 6.0 / 8.1, 200 x 7168 9.6 / 8.2, 1184 x 4096 14.8 / 15.6, 2368 x 4096 25.8 / 22.8, 4096 x 2048 19.6 / 22.5,
     // 16384 x 2048 64.5 / 57.6, 16384 x 1424 49.8 / 47.3, 16384 x 768 26.8 / 32.0).
     const long long work = (long long)p.rows * packs;
-    if (packs <= 256 && (packs <= 128 || work <= 148 * 8192)) {
-        sandwich_kernel<T, X, 1, WHOLE, 256, 8><<<p.rows, warps(packs), 0, stream>>>(p);
-        return cudaGetLastError();
-    }
-    if (packs <= 1024 && (p.rows <= 148 || (packs <= 512 && work <= 148 * 4096))) {
-        sandwich_kernel<T, X, 1, WHOLE, 1024, 1><<<p.rows, warps(packs), 0, stream>>>(p);
-        return cudaGetLastError();
-    }
+    if (packs <= 256 && (packs <= 128 || work <= 148 * 8192))
+        return launch_dependent(sandwich_kernel<T, X, 1, WHOLE, 256, 8>, dim3(p.rows), warps(packs), 0, 1, stream, p);
+    if (packs <= 1024 && (p.rows <= 148 || (packs <= 512 && work <= 148 * 4096)))
+        return launch_dependent(sandwich_kernel<T, X, 1, WHOLE, 1024, 1>, dim3(p.rows), warps(packs), 0, 1, stream, p);
     const Groups g = groups_of<T, X, WHOLE>(p);
     if (g.groups > 0) {
         const bool gated = p.gate && p.ld_gate && p.gate_step;
         if (WHOLE && packs == kGroupPacks * g.threads) return gated ? launch_rows<T, X, WHOLE, WHOLE, true>(p, g, stream) : launch_rows<T, X, WHOLE, WHOLE, false>(p, g, stream);
         return gated ? launch_rows<T, X, WHOLE, false, true>(p, g, stream) : launch_rows<T, X, WHOLE, false, false>(p, g, stream);
     }
-    if (packs <= 4 * 1024) sandwich_kernel<T, X, 4, WHOLE, 1024, 1><<<p.rows, warps((packs + 3) / 4), 0, stream>>>(p);
-    else sandwich_any_kernel<T, X><<<p.rows, 256, 0, stream>>>(p);
-    return cudaGetLastError();
+    if (packs <= 4 * 1024) return launch_dependent(sandwich_kernel<T, X, 4, WHOLE, 1024, 1>, dim3(p.rows), warps((packs + 3) / 4), 0, 1, stream, p);
+    return launch_dependent(sandwich_any_kernel<T, X>, dim3(p.rows), 256, 0, 1, stream, p);
 }
 
 template <typename T, typename X>
@@ -702,8 +705,7 @@ cudaError_t launch_typed(const SandwichParams &p, cudaStream_t stream)
                         fits(p.post_gamma, p.ld_x, p.gamma32 ? 4 : sizeof(T)) && fits(p.smooth, p.ld_x, 4) &&
                         (!rows_gate || fits(p.gate, p.ld_gate, sizeof(T))) && (!channel_gate || fits(p.gate, p.ld_x, sizeof(T)));
     if (packed) return p.h % V == 0 && p.ld_x % V == 0 ? launch_packed<T, X, true>(p, stream) : launch_packed<T, X, false>(p, stream);
-    sandwich_any_kernel<T, X><<<p.rows, 256, 0, stream>>>(p);
-    return cudaGetLastError();
+    return launch_dependent(sandwich_any_kernel<T, X>, dim3(p.rows), 256, 0, 1, stream, p);
 }
 
 }  // namespace
