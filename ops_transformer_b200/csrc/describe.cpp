@@ -8,6 +8,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
+#include <ATen/ops/empty_native.h>
 
 #include <Python.h>
 #include <cstdint>
@@ -263,9 +264,10 @@ PyObject *empty(PyObject *, PyObject *const *args, Py_ssize_t nargs)
         const at::Tensor &t = THPVariable_Unpack(args[0]);
         const at::ScalarType dtype = *type == 'b' ? at::kChar : *type == 'i' ? at::kInt : *type == 'l' ? at::kLong : *type == 'f' || *type == 's' ? at::kFloat
                                        : *type == 'h' ? at::kHalf : *type == 'w' ? at::kBFloat16 : t.scalar_type();
-        const auto options = at::TensorOptions().dtype(dtype).device(t.device());
-        if (*type == 's') return THPVariable_Wrap(at::empty({}, options));
-        return THPVariable_Wrap(nargs == 2 ? at::empty(t.sizes(), options) : at::empty(at::IntArrayRef(sizes, (size_t)nargs - 2), options));
+        const auto shape = *type == 's' ? at::IntArrayRef() : nargs == 2 ? t.sizes() : at::IntArrayRef(sizes, (size_t)nargs - 2);
+        // on the GPU without the dispatcher, which costs as much as the allocation
+        return THPVariable_Wrap(t.is_cuda() ? at::native::empty_cuda(shape, dtype, std::nullopt, t.device())
+                                            : at::empty(shape, at::TensorOptions().dtype(dtype).device(t.device())));
     END_HANDLE_TH_ERRORS
 }
 
