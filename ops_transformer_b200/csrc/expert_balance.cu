@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(threads_of(PER), 1) balance_rows_kernel(const 
 
 // The sums of a warp's share of a sequence's pieces, for the expert of each lane; N of them under way.
 template <int N>
-__device__ __forceinline__ void sum_pieces(const BalanceParams &p, int s, int first, int step, int e, float &sum, int &count, int &tokens)
+__device__ __forceinline__ void sum_pieces(const BalanceParams &p, int s, int first, int step, int e, float &sum, long long &count, int &tokens)
 {
     const int begin = seq_begin(p, s), end = seq_end(p, s);
     if (begin >= end) return;
@@ -389,7 +389,8 @@ constexpr int kFewSequences = 32, kFinishCtas = 8, kMostGroups = 1024 / (32 * kF
 __global__ void __launch_bounds__(1024, 1) balance_finish_few_kernel(const BalanceParams p)
 {
     __shared__ float sums[32][32];
-    __shared__ int counts[32][32], tokens_of[kFewSequences];
+    __shared__ long long counts[32][32];
+    __shared__ int tokens_of[kFewSequences];
     __shared__ double dots[kFewSequences * kMostGroups], all_dots[kFinishCtas][kFewSequences];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = blockIdx.x;
     // A CTA's items are a sequence and 32 experts each, for a power of two of warps.
@@ -403,7 +404,8 @@ __global__ void __launch_bounds__(1024, 1) balance_finish_few_kernel(const Balan
     for (int item0 = 0; item0 < items; item0 += 32 / each) {
         const int item = item0 + warp / each, s = item / groups, g = item - s * groups, e = (rank * groups + g) * 32 + lane;
         float sum = 0.0f;
-        int count = 0, tokens = 0;
+        long long count = 0;
+        int tokens = 0;
         if (item < items) sum_pieces<5>(p, s, part, each, e, sum, count, tokens);
         sums[warp][lane] = sum;
         counts[warp][lane] = count;
@@ -459,7 +461,7 @@ __global__ void __launch_bounds__(kFinishThreads) balance_finish_many_kernel(con
     double dot = 0.0;
     for (int e = tid; e < p.experts; e += kFinishThreads) {
         float sum = 0.0f;
-        int count = 0;
+        long long count = 0;
         tokens = 0;
         sum_pieces<4>(p, s, 0, 1, e, sum, count, tokens);
         p.counts[(long long)s * p.experts + e] = count;

@@ -249,6 +249,53 @@ def test_sandwich_sizes(rows, h, dtype, x_dtype):
     run_sandwich(t["x"], t["residual"], None, post_gamma=post, quant=False)
 
 
+@pytest.mark.parametrize("dtype,x_dtype", [(BF16, F32), (F16, F16), (F32, F32)])
+@pytest.mark.parametrize("rows,h", [(149, 7168), (200, 5001), (2500, 2047), (5000, 2048), (7000, 1431), (450, 8200), (150, 16384), (150, 33000)])
+def test_sandwich_many_rows(rows, h, dtype, x_dtype):
+    """Groups of threads with rows in turn, at every start of a row; what is too long for them."""
+    t = sandwich_inputs(rows, h, dtype, x_dtype)
+    post, smooth = randn((h,), 4, dtype, 0.2) + 0.7, rand((h,), 5) + 0.5
+    run_sandwich(**t, post_gamma=post)
+    run_sandwich(**t, gate=randn((h,), 6, dtype), gate_act="tanh", smooth=smooth, normed=True, residual_scale=0.75, block_scale=0.4)
+    run_sandwich(**t, post_gamma=post, gate=randn((rows, h), 8, dtype), gate_act="sigmoid", smooth=smooth, normed=True)
+    run_sandwich(**t, gate=randn((rows, 1), 7, dtype), quant=False, normed=True)
+    run_sandwich(t["x"], t["residual"], None, post_gamma=post, quant=False)
+    want = ops.sandwich_norm_quant(**t, post_gamma=post, normed=True)
+    for into in ("residual", "x") if x_dtype == dtype else ("residual",):
+        mine = {k: v.clone() for k, v in t.items()}
+        got = ops.sandwich_norm_quant(**mine, post_gamma=post, normed=True, residual_out=mine[into])
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[2] is mine[into]
+
+
+@pytest.mark.parametrize("offset,pitch", [(0, 2 * 5000), (8, 5008), (1, 5003), (4, 5004)])
+def test_sandwich_many_strided_rows(offset, pitch):
+    rows, h = 333, 5000
+    wide = lambda seed, dt=BF16: randn((rows * pitch + 64,), seed, dt)[offset:].as_strided((rows, h), (pitch, 1))  # noqa: E731
+    x, residual, gate, stream, normed = wide(1, F32), wide(2), wide(3), wide(4), wide(5)
+    gamma, post = randn((h + 8,), 3, BF16)[offset:offset + h], randn((h + 8,), 4, BF16)[offset:offset + h]
+    room = torch.full((rows * pitch + 64,), 5, dtype=I8, device=DEV)
+    q = room[offset:].as_strided((rows, h), (pitch, 1))
+    before = [v.as_strided((rows * pitch,), (1,)).clone() for v in (stream, normed)]
+    got = ops.sandwich_norm_quant(x, residual, gamma, post_gamma=post, gate=gate, q=q, residual_out=stream, normed_out=normed)
+    check_sandwich(x, residual, gamma, got, post_gamma=post, gate=gate, normed=True)
+    gap = torch.arange(rows * pitch, device=DEV) % pitch >= h   # between the rows nothing is written
+    for was, now in zip(before, (stream, normed)):
+        assert torch.equal(was[gap], now.as_strided((rows * pitch,), (1,))[gap])
+    assert (room[offset:offset + rows * pitch][gap] == 5).all() and (room[:offset] == 5).all()
+
+
+def test_sandwich_many_special_rows():
+    for h in (7168, 5003):
+        t = sandwich_inputs(400, h, BF16, F32)
+        gamma = torch.ones(h, device=DEV, dtype=BF16)
+        t["x"][1], t["residual"][1] = 0, 0
+        t["x"][2, 5], t["x"][3, h - 1], t["residual"][399, 0] = math.inf, math.nan, -math.inf
+        q, scale, stream, y = got = ops.sandwich_norm_quant(t["x"], t["residual"], gamma, post_gamma=gamma, normed=True)
+        assert (q[1] == 0).all() and scale[1] == 0 and (y[1] == 0).all() and all(scale[i].isnan() and (q[i] == 0).all() for i in (2, 3, 399))
+        good = torch.tensor([0] + list(range(4, 399)), device=DEV)
+        check_sandwich(t["x"][good], t["residual"][good], gamma, [v[good] for v in got], post_gamma=gamma, normed=True)
+
+
 @pytest.mark.parametrize("act", ["none", "sigmoid", "tanh"])
 @pytest.mark.parametrize("rows,h", [(6, 520), (400, 1001)])
 def test_sandwich_gates(rows, h, act):
@@ -451,7 +498,8 @@ def cuts(t, n, seed, last=None):
     return c
 
 
-@pytest.mark.parametrize("t,E,k,n", [(1, 8, 2, 1), (40, 64, 4, 3), (40, 64, 4, 40), (700, 33, 3, 16), (5000, 256, 8, 5), (5000, 128, 8, 300), (16384, 256, 8, 16), (300, 16, 2, 2000)])
+@pytest.mark.parametrize("t,E,k,n", [(1, 8, 2, 1), (40, 64, 4, 3), (40, 64, 4, 40), (700, 33, 3, 16), (5000, 256, 8, 5), (5000, 128, 8, 300), (16384, 256, 8, 16), (300, 16, 2, 2000), (2000, 1000, 3, 20), (900, 600, 2, 32),
+                                     (900, 8, 2, 33)])
 def test_balance_sequences(t, E, k, n):
     for dtype, scoring in ((F32, "softmax"), (BF16, "sigmoid")):
         logits, ids = balance_inputs(t, E, k, dtype, seed=7)
@@ -523,6 +571,32 @@ def test_balance_special_logits_and_ids():
             p, c = want[4:]
             size = p * (c - c.mean(1, keepdim=True)).abs().amax(1, keepdim=True)
             assert ((grad.double() - want[3]).abs() <= 2 * (size + want[3].abs()) * (250 + 4 + 8 + 72 / 32 + 12) * U32 + 1e-38).all()
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E", [72, 71])
+def test_balance_logits_far_out(scoring, E):
+    """Rows whose logits are all far from zero, on both sides of what the plain way of forming scores takes."""
+    base = randn((40, E), 1)
+    for shift in ([-700, -300, -104, -90, -61, -59, -47, -45, -20, 30, 88, 89, 104] if scoring == "sigmoid" else
+                  [-3e5, -700, -90, 90, 1e5, 2.0 ** 20 - 8, 2.0 ** 20, 2.0 ** 21, 2.0 ** 22]):
+        logits = base + shift
+        ids = logits.topk(3, dim=1).indices
+        loss, counts, weight = ops.expert_balance(logits, ids, scoring=scoring)
+        grad = ops.expert_balance_grad(logits, counts, weight, scoring=scoring, grad_loss=torch.tensor(1e3, device=DEV))
+        want, want_counts, _, want_grad, p, c = plain_balance(logits, ids, scoring, 1.0, upstream=1e3)
+        if scoring == "sigmoid" and shift == -700:      # around the border below which there is no score
+            assert loss.isfinite() and grad.isfinite().all()
+            continue
+        # softmax depends on differences alone, which fp32 forms exactly this near to one another; sigmoids on the logits themselves
+        rel = (float(logits.abs().max() if scoring == "sigmoid" else (logits.max() - logits.min())) + 4 + E / 32 + 8) * U32
+        assert torch.equal(counts, want_counts[0]) and abs(loss.item() - want.item()) <= abs(want.item()) * (rel + 60 * U32)
+        size = p * (c - c.mean(1, keepdim=True)).abs().amax(1, keepdim=True) * 1e3
+        assert ((grad.double() - want_grad).abs() <= want_grad.abs() * (rel + 8 * U32) + 2 * size * (rel + (E / 32 + 12) * U32) + 1e-38).all()
+    huge = torch.full((3, E), -3e38, device=DEV)
+    huge[0, 3], huge[1, :2], huge[2, 1] = 3e38, 1e30, -1e38
+    grad = ops.expert_balance_grad(huge, *ops.expert_balance(huge, torch.tensor([[3], [0], [1]], device=DEV), scoring=scoring)[1:], scoring=scoring)
+    assert grad.isfinite().all()
 
 
 def test_balance_gradient_against_differences():
