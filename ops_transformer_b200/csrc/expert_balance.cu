@@ -5,8 +5,9 @@
 //   d loss / d l[e] = weight * p[e] * (c[e] - sum_j p[j] c[j])   (sigmoid: times 1 - sigmoid(l[e]))
 //
 // The loss needs the counts of all tokens, so its gradient reads the logits a second time and forms p anew: 1 KB a row from memory against
-// the same to write p and read it back.  A warp holds a row, a lane its share of the experts; sums over tokens are made in a fixed order
-// (a lane's rows one after the other, then the warps, then the blocks), so that a call gives the same bits every time.
+// the same to write p and read it back.  A group of 8, 16 or 32 lanes holds a row, a lane 16 of its experts or so: fewer lanes make fewer
+// steps of sums and maxima across them, and of all that a row costs once.  Sums over tokens are made in a fixed order (a lane's rows one
+// after the other, then the groups, then the pieces), so that a call gives the same bits every time.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -20,9 +21,12 @@ namespace gmm {
 namespace {
 
 constexpr int kGradThreads = 256, kGradWarps = kGradThreads / 32;
-// Threads of a block of rows, at most: for 8, 16 and 32 values a lane, as many as there are registers for.
-constexpr int threads_of(int per) { return per <= 8 ? 1024 : per <= 16 ? 512 : 256; }
-inline int warps_of(int experts) { return threads_of(experts <= 256 ? 8 : experts <= 512 ? 16 : 32) / 32; }
+// Lanes of a row and values of a lane by the number of experts, and the threads of a block of rows, at most: as many as there are registers
+// for.
+constexpr int lanes_of(int experts) { return experts <= 128 ? 8 : experts <= 256 ? 16 : 32; }
+constexpr int values_of(int experts) { return experts <= 64 ? 8 : experts <= 512 ? 16 : 32; }
+constexpr int threads_of(int values) { return values <= 8 ? 1024 : values <= 16 ? 512 : 256; }
+inline int warps_of(int experts) { return threads_of(values_of(experts)) / 32; }
 
 struct BalanceParams {
     const void *logits;
@@ -76,16 +80,23 @@ __device__ __forceinline__ float rcp_of(float v)
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-__device__ __forceinline__ float warp_max(float v)      // passes NaN over
+// Over groups of G lanes; the maximum passes NaN over.
+template <int G>
+__device__ __forceinline__ float group_max(float v)
 {
-    float r;
-    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-    return r;
+    if constexpr (G == 32) {
+        asm volatile("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(v));
+    } else {
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    }
+    return v;
 }
-__device__ __forceinline__ float warp_sum(float v)
+template <int G>
+__device__ __forceinline__ float group_sum(float v)
 {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 
@@ -96,13 +107,13 @@ template <typename T, int PER, int V> __host__ __device__ constexpr int rows_ahe
     return n > 4 ? 4 : n < 1 ? 1 : n;
 }
 
-// The expert of a lane's i-th value: V neighbours at a time.
-template <int V>
-__device__ __forceinline__ int expert_of(int i, int lane) { return (i / V * 32 + lane) * V + i % V; }
+// The expert of the i-th value of a group's lane: V neighbours at a time.
+template <int G, int V>
+__device__ __forceinline__ int expert_of(int i, int lane) { return (i / V * G + lane) * V + i % V; }
 
 // A row as it is in memory, for the loads of the next one to be under way while this one is worked on; minus infinity where there is no
 // expert.  V: values of one 16-byte load, or 1.
-template <typename T, int PER, int V>
+template <typename T, int G, int PER, int V>
 struct RawRow {
     static constexpr int N = PER / V;
     typename std::conditional<(V > 1), uint4, T>::type raw[N];
@@ -119,20 +130,25 @@ struct RawRow {
     {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int e = expert_of<V>(i * V, lane);
+            const int e = expert_of<G, V>(i * V, lane);
             if (e >= experts) continue;
             if constexpr (V > 1) raw[i] = *reinterpret_cast<const uint4 *>(row + e);
             else raw[i] = row[e];
         }
     }
-    __device__ __forceinline__ void values(f32x2 (&l)[PER / 2]) const
+    // Zeros where there is no token, so that nothing in its place is worked on.
+    __device__ __forceinline__ void values(bool token, f32x2 (&l)[PER / 2]) const
     {
         if constexpr (V > 1) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) unpack<T>(raw[i], l + i * (V / 2));
+            for (int i = 0; i < N; ++i) {
+                uint4 u = raw[i];
+                if (!token) u = make_uint4(0, 0, 0, 0);
+                unpack<T>(u, l + i * (V / 2));
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < PER; i += 2) l[i / 2] = pair2(to_float<T>(raw[i]), to_float<T>(raw[i + 1]));
+            for (int i = 0; i < PER; i += 2) l[i / 2] = token ? pair2(to_float<T>(raw[i]), to_float<T>(raw[i + 1])) : 0;
         }
     }
 };
@@ -145,7 +161,7 @@ struct RawRow {
 // total, and is done again element by element: a logit of NaN, a row whose largest logit is so far out that the fma's constant term is
 // off by more than a little, or one whose sigmoids all but vanish, of which p is what softmax makes of it (to 2^-60).  Below sigmoids of
 // e^-700, which 64 bits hardly hold, there is nothing.
-template <bool SIGMOID, int PER>
+template <bool SIGMOID, int G, int PER>
 __device__ __forceinline__ void scores(const f32x2 (&l)[PER / 2], f32x2 (&e)[PER / 2], f32x2 (&rest)[PER / 2], float &inv)
 {
     constexpr float kLog2e = 1.4426950408889634f;
@@ -169,7 +185,7 @@ __device__ __forceinline__ void scores(const f32x2 (&l)[PER / 2], f32x2 (&e)[PER
             const float2 v = unpair2(l[i]);
             top = fmaxf(top, fmaxf(v.x, v.y));
         }
-        top = warp_max(top);
+        top = group_max<G>(top);
         const float shift = __fmul_rn(top, -kLog2e);
 #pragma unroll
         for (int i = 0; i < PER / 2; ++i) {
@@ -179,14 +195,15 @@ __device__ __forceinline__ void scores(const f32x2 (&l)[PER / 2], f32x2 (&e)[PER
         }
     }
     const float2 parts = unpair2(total2);
-    float total = warp_sum(parts.x + parts.y);
-    if (!(total >= 1e-20f) || (!SIGMOID && !(fabsf(top) <= 0x1p20f))) {
+    float total = group_sum<G>(parts.x + parts.y);
+    const bool again = !(total >= 1e-20f) || (!SIGMOID && !(fabsf(top) <= 0x1p20f));
+    if (__any_sync(0xffffffffu, again)) {
 #pragma unroll
         for (int i = 0; i < PER / 2; ++i) {
             const float2 v = unpair2(l[i]);
             top = fmaxf(top, fmaxf(v.x, v.y));
         }
-        top = warp_max(top);
+        top = group_max<G>(top);
         const bool soft = !SIGMOID || (top < -60.0f && top > -700.0f);
         float sum = 0.0f;
 #pragma unroll
@@ -207,10 +224,13 @@ __device__ __forceinline__ void scores(const f32x2 (&l)[PER / 2], f32x2 (&e)[PER
                 if (!(x > -kInf)) of[j] = r[j] = 0.0f;
                 sum += of[j];
             }
-            e[i] = pair2(of[0], of[1]);
-            rest[i] = pair2(r[0], r[1]);
+            if (again) {
+                e[i] = pair2(of[0], of[1]);
+                rest[i] = pair2(r[0], r[1]);
+            }
         }
-        total = warp_sum(sum);
+        sum = group_sum<G>(sum);
+        if (again) total = sum;
     }
     inv = total > 0.0f ? rcp_of(total) : 0.0f;
 }
@@ -252,18 +272,19 @@ __device__ __forceinline__ int seq_of_piece(const BalanceParams &p, int piece, i
     return lo;
 }
 
-// What a block of rows adds to a sequence: one piece, which a CTA makes.  A warp takes up to `ahead` rows at a time, whose loads it issues
-// together.  ALL: the rows are all those of the only sequence, and the CTA finishes.
-template <typename T, bool SIGMOID, int PER, int V, bool ALL>
+// What a block of rows adds to a sequence: one piece, which a CTA makes.  A warp takes a row for each of its groups of G lanes at a time, and
+// has the loads of R times as many under way.  ALL: the rows are all those of the only sequence, and the CTA finishes.
+template <typename T, bool SIGMOID, int G, int PER, int V, bool ALL>
 __global__ void __launch_bounds__(threads_of(PER), 1) balance_rows_kernel(const BalanceParams p)
 {
-    constexpr int R = rows_ahead<T, PER, V>(PER <= 8 ? 16 : 32);
-    extern __shared__ float4 smem[];    // sums [warps][experts], then the counts [experts]
+    constexpr int R = rows_ahead<T, PER, V>(PER <= 8 ? 8 : 16), GROUPS = 32 / G;
+    extern __shared__ float4 smem[];    // sums [warps][GROUPS][experts], then the counts [experts]
     __shared__ int warp_tokens[32];
     __shared__ double warp_dots[32];
     float *sums = reinterpret_cast<float *>(smem);
     const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = threads >> 5, piece = blockIdx.x;
-    int *counts = reinterpret_cast<int *>(sums + warps * p.experts);
+    const int group = lane / G, mine = lane % G, step = warps * GROUPS;
+    int *counts = reinterpret_cast<int *>(sums + step * p.experts);
     for (int e = tid; e < p.experts; e += threads) counts[e] = 0;
     dependent_wait();
     dependent_release();
@@ -274,55 +295,62 @@ __global__ void __launch_bounds__(threads_of(PER), 1) balance_rows_kernel(const 
     if (!ALL && begin >= end) return;
     f32x2 sum[PER / 2] = {};
     int tokens = 0;
-    RawRow<T, PER, V> rows[R];
-    __syncthreads();    // the counts are zero
-    for (int row0 = begin + warp; row0 < end; row0 += R * warps) {
-        bool token[R];
-        int ids[R];
-        const auto id_of = [&](int row, int j) {
-            const long long i = (long long)row * p.top_k + j, id = p.ids_i64 ? static_cast<const long long *>(p.ids)[i] : (long long)static_cast<const int *>(p.ids)[i];
-            return id >= 0 && id < p.experts ? (int)id : -1;
-        };
+    RawRow<T, G, PER, V> rows[R];
+    int2 ids[R];    // as they are in memory, and the mask too: a look at one would hold up the loads behind it
+    int8_t mask[R];
+    const auto load_id = [&](int row, int j) {
+        const long long i = (long long)row * p.top_k + j;
+        return p.ids_i64 ? static_cast<const int2 *>(p.ids)[i] : make_int2(static_cast<const int *>(p.ids)[i], 0);
+    };
+    const auto count_id = [&](const int2 &v) {
+        if ((unsigned)v.x < (unsigned)p.experts && v.y == 0) atomicAdd(counts + v.x, 1);
+    };
+    const auto fetch = [&](int r, int row) {    // of a row that the mask leaves out, too, so that no load waits for another
+        mask[r] = 0;
+        if (row >= end) return;
+        rows[r].load(static_cast<const T *>(p.logits) + row * p.ld, p.experts, mine);
+        if (mine < p.top_k) ids[r] = load_id(row, mine);
+        mask[r] = 1;
+        if (p.mask) mask[r] = p.mask[row];
+    };
 #pragma unroll
-        for (int r = 0; r < R; ++r) {   // of a row that the mask leaves out, too, so that no load waits for another
-            const int row = row0 + r * warps;
-            token[r] = false;
-            if (row >= end) continue;
-            rows[r].load(static_cast<const T *>(p.logits) + row * p.ld, p.experts, lane);
-            ids[r] = lane < p.top_k ? id_of(row, lane) : -1;
-            token[r] = !p.mask || p.mask[row] != 0;
-        }
+    for (int r = 0; r < R; ++r) fetch(r, begin + warp * GROUPS + group + r * step);
+    __syncthreads();    // the counts are zero
+    for (int row0 = begin + warp * GROUPS; row0 < end; row0 += R * step) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if (!token[r]) continue;
-            ++tokens;
-            int id = ids[r];
-            for (int j = lane;;) {
-                if (id >= 0) atomicAdd(counts + id, 1);
-                if ((j += 32) >= p.top_k) break;
-                id = id_of(row0 + r * warps, j);
-            }
+            const int row = row0 + group + r * step;
+            const bool token = mask[r] != 0;
             f32x2 l[PER / 2], e[PER / 2], rest[PER / 2];
+            rows[r].values(token, l);
+            if (token) {
+                tokens += mine == 0;
+                if (mine < p.top_k) count_id(ids[r]);
+                for (int j = mine + G; j < p.top_k; j += G) count_id(load_id(row, j));
+            }
+            fetch(r, row + R * step);
+            if (!__any_sync(0xffffffffu, token)) continue;
             float inv;
-            rows[r].values(l);
-            scores<SIGMOID, PER>(l, e, rest, inv);
+            scores<SIGMOID, G, PER>(l, e, rest, inv);
+            if (!token) inv = 0.0f;
 #pragma unroll
             for (int i = 0; i < PER / 2; ++i) sum[i] = fma2(e[i], pair2(inv, inv), sum[i]);
         }
     }
+    tokens = (int)__reduce_add_sync(0xffffffffu, tokens);
     if (lane == 0) warp_tokens[warp] = tokens;
+    float *to = sums + (warp * GROUPS + group) * p.experts;
     if constexpr (V > 1) {
 #pragma unroll
         for (int i = 0; i < PER; i += 4) {
-            const int e = expert_of<V>(i, lane);
-            if (e < p.experts)
-                *reinterpret_cast<float4 *>(sums + warp * p.experts + e) = make_float4(element(sum, i), element(sum, i + 1), element(sum, i + 2), element(sum, i + 3));
+            const int e = expert_of<G, V>(i, mine);
+            if (e < p.experts) *reinterpret_cast<float4 *>(to + e) = make_float4(element(sum, i), element(sum, i + 1), element(sum, i + 2), element(sum, i + 3));
         }
     } else {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int e = expert_of<V>(i, lane);
-            if (e < p.experts) sums[warp * p.experts + e] = element(sum, i);
+            const int e = expert_of<G, V>(i, mine);
+            if (e < p.experts) to[e] = element(sum, i);
         }
     }
     __syncthreads();
@@ -330,7 +358,7 @@ __global__ void __launch_bounds__(threads_of(PER), 1) balance_rows_kernel(const 
     for (int e = tid; e < p.experts; e += threads) {
         float total = 0.0f;
 #pragma unroll 8
-        for (int w = 0; w < warps; ++w) total += sums[w * p.experts + e];
+        for (int w = 0; w < step; ++w) total += sums[w * p.experts + e];
         if (ALL) {
             p.counts[e] = counts[e];
             dot += (double)total * counts[e];
@@ -502,90 +530,82 @@ __global__ void __launch_bounds__(kFinishThreads) balance_finish_many_kernel(con
     }
 }
 
+// A warp holds a row: its loads are the longest part of it, and more warps hide more of them than a row's fewer instructions in fewer lanes
+// would gain (4096 x 256 4.0 us, with 16 lanes a row 4.1; 16384 x 256 in fp32 9.2 and 10.4).
 template <typename T, bool SIGMOID, int PER, int V>
 __global__ void __launch_bounds__(kGradThreads, PER <= 8 ? 4 : 2) balance_grad_kernel(const BalanceParams p)
 {
-    constexpr int R = rows_ahead<T, PER, V>(PER <= 8 ? 16 : 32);
     const int lane = threadIdx.x & 31, row0 = (blockIdx.x * kGradWarps + (threadIdx.x >> 5)) * p.chunk, row1 = min(row0 + p.chunk, p.rows);
     dependent_wait();
     dependent_release();
     if (row0 >= row1) return;
-    RawRow<T, PER, V> rows[R];
-    int8_t mask[R];
-    const auto fetch = [&](int batch) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            if (batch + r >= row1) break;
-            rows[r].load(static_cast<const T *>(p.logits) + (batch + r) * p.ld, p.experts, lane);
-            mask[r] = p.mask ? p.mask[batch + r] : 1;
-        }
+    RawRow<T, 32, PER, V> here;
+    int8_t mask = 1;
+    const auto fetch = [&](int row) {
+        here.load(static_cast<const T *>(p.logits) + row * p.ld, p.experts, lane);
+        if (p.mask) mask = p.mask[row];
     };
     fetch(row0);
     const float grad_loss = p.grad_loss ? *p.grad_loss : 1.0f;
     int s = seq_of(p, row0, lane), known = -1, begin = 0, end = 0;
     f32x2 load[PER / 2];
     float factor = 0.0f;
-    for (int batch = row0; batch < row1; batch += R) {
-        if (batch > row0) fetch(batch);
+    for (int row = row0; row < row1; ++row) {
+        while (row >= end && s < p.sequences) {
+            begin = seq_begin(p, s);
+            end = seq_end(p, s);
+            if (row >= end) ++s;
+        }
+        const bool token = row >= begin && row < end && mask != 0;
+        f32x2 l[PER / 2], g[PER / 2] = {};
+        here.values(true, l);
+        if (row + 1 < row1) fetch(row + 1);
+        if (token) {
+            if (known != s) {
+                // Counts less a whole number near their mean: the difference from the row's mean of them, which is what the gradient is made
+                // of, does not lose its places to what they all have in common.
+                known = s;
+                const long long *counts = p.counts + (long long)s * p.experts;
+                factor = __fmul_rn(p.weight[s], grad_loss);
+                long long count[PER];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int row = batch + r;
-            if (row >= row1) break;
-            while (row >= end && s < p.sequences) {
-                begin = seq_begin(p, s);
-                end = seq_end(p, s);
-                if (row >= end) ++s;
-            }
-            const bool token = row >= begin && row < end && mask[r] != 0;
-            f32x2 g[PER / 2] = {};
-            if (token) {
-                if (known != s) {
-                    // Counts less a whole number near their mean: the difference from the row's mean of them, which is what the gradient is made
-                    // of, does not lose its places to what they all have in common.
-                    known = s;
-                    const long long *counts = p.counts + (long long)s * p.experts;
-                    factor = __fmul_rn(p.weight[s], grad_loss);
-                    long long count[PER];
-#pragma unroll
-                    for (int i = 0; i < PER; i += V > 1 ? 2 : 1) {
-                        const int e = expert_of<V>(i, lane);
-                        if constexpr (V > 1) {
-                            const longlong2 two = e < p.experts ? *reinterpret_cast<const longlong2 *>(counts + e) : make_longlong2(0, 0);
-                            count[i] = two.x;
-                            count[i + 1] = two.y;
-                        } else {
-                            count[i] = e < p.experts ? counts[e] : 0;
-                        }
+                for (int i = 0; i < PER; i += V > 1 ? 2 : 1) {
+                    const int e = expert_of<32, V>(i, lane);
+                    if constexpr (V > 1) {
+                        const longlong2 two = e < p.experts ? *reinterpret_cast<const longlong2 *>(counts + e) : make_longlong2(0, 0);
+                        count[i] = two.x;
+                        count[i + 1] = two.y;
+                    } else {
+                        count[i] = e < p.experts ? counts[e] : 0;
                     }
-                    float total = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < PER; ++i) total += (float)count[i];
-                    const long long base = (long long)(warp_sum(total) / (float)p.experts);
-#pragma unroll
-                    for (int i = 0; i < PER; i += 2) load[i / 2] = pair2((float)(count[i] - base), (float)(count[i + 1] - base));
                 }
-                f32x2 l[PER / 2], e[PER / 2], rest[PER / 2], mean2 = 0;
-                float inv;
-                rows[r].values(l);
-                scores<SIGMOID, PER>(l, e, rest, inv);
+                float total = 0.0f;
 #pragma unroll
-                for (int i = 0; i < PER / 2; ++i) mean2 = fma2(e[i], load[i], mean2);
-                const float2 parts = unpair2(mean2);
-                const float mean = -__fmul_rn(warp_sum(parts.x + parts.y), inv), scale = __fmul_rn(inv, factor);
+                for (int i = 0; i < PER; ++i) total += (float)count[i];
+                const long long base = (long long)(group_sum<32>(total) / (float)p.experts);
 #pragma unroll
-                for (int i = 0; i < PER / 2; ++i) {
-                    g[i] = mul2(mul2(e[i], pair2(scale, scale)), add2(load[i], pair2(mean, mean)));
-                    if (SIGMOID) g[i] = mul2(g[i], rest[i]);
-                }
+                for (int i = 0; i < PER; i += 2) load[i / 2] = pair2((float)(count[i] - base), (float)(count[i + 1] - base));
             }
-            T *to = static_cast<T *>(p.grad) + row * p.ld_grad;
+            f32x2 e[PER / 2], rest[PER / 2], mean2 = 0;
+            float inv;
+            scores<SIGMOID, 32, PER>(l, e, rest, inv);
 #pragma unroll
-            for (int i = 0; i < PER; i += V) {
-                const int e = expert_of<V>(i, lane);
-                if (e >= p.experts) continue;
-                if constexpr (V > 1) *reinterpret_cast<uint4 *>(to + e) = pack<T>(g + i / 2);
-                else to[e] = from_float<T>(element(g, i));
+            for (int i = 0; i < PER / 2; ++i) mean2 = fma2(e[i], load[i], mean2);
+            const float2 parts = unpair2(mean2);
+            const float mean = -__fmul_rn(group_sum<32>(parts.x + parts.y), inv), scale = __fmul_rn(inv, factor);
+#pragma unroll
+            for (int i = 0; i < PER / 2; ++i) {
+                g[i] = mul2(mul2(e[i], pair2(scale, scale)), add2(load[i], pair2(mean, mean)));
+                if (SIGMOID) g[i] = mul2(g[i], rest[i]);
             }
+        }
+        T *to = static_cast<T *>(p.grad) + row * p.ld_grad;
+#pragma unroll
+        for (int i = 0; i < PER; i += V) {
+            const int e = expert_of<32, V>(i, lane);
+            if (e >= p.experts) continue;
+            if constexpr (V > 1) *reinterpret_cast<uint4 *>(to + e) = pack<T>(g + i / 2);
+            else to[e] = from_float<T>(element(g, i));
         }
     }
 }
@@ -600,30 +620,28 @@ template <int N> struct Int { static constexpr int value = N; };
 template <bool B> struct Flag { static constexpr bool value = B; };
 template <typename T> struct Type { typedef T type; };
 
-template <typename T, bool SIGMOID, typename Fn>
-cudaError_t dispatch_width(int experts, bool packs, Fn fn)
+template <typename T, bool SIGMOID, int V, typename Fn>
+cudaError_t dispatch_width(int experts, Fn fn)
 {
-    constexpr int V = 16 / (int)sizeof(T);
-    if (packs) {
-        if (experts <= 32 * V) return fn(Type<T>(), Flag<SIGMOID>(), Int<V>(), Int<V>());
-        if (experts <= 64 * V) return fn(Type<T>(), Flag<SIGMOID>(), Int<2 * V>(), Int<V>());
-        if (experts <= 512) return fn(Type<T>(), Flag<SIGMOID>(), Int<16>(), Int<V>());
-        return fn(Type<T>(), Flag<SIGMOID>(), Int<32>(), Int<V>());
-    }
-    if (experts <= 64) return fn(Type<T>(), Flag<SIGMOID>(), Int<2>(), Int<1>());
-    if (experts <= 192) return fn(Type<T>(), Flag<SIGMOID>(), Int<6>(), Int<1>());
-    if (experts <= 256) return fn(Type<T>(), Flag<SIGMOID>(), Int<8>(), Int<1>());
-    if (experts <= 512) return fn(Type<T>(), Flag<SIGMOID>(), Int<16>(), Int<1>());
-    return fn(Type<T>(), Flag<SIGMOID>(), Int<32>(), Int<1>());
+    if (experts <= 64) return fn(Type<T>(), Flag<SIGMOID>(), Int<lanes_of(64)>(), Int<values_of(64)>(), Int<V>());
+    if (experts <= 128) return fn(Type<T>(), Flag<SIGMOID>(), Int<lanes_of(128)>(), Int<values_of(128)>(), Int<V>());
+    if (experts <= 256) return fn(Type<T>(), Flag<SIGMOID>(), Int<lanes_of(256)>(), Int<values_of(256)>(), Int<V>());
+    if (experts <= 512) return fn(Type<T>(), Flag<SIGMOID>(), Int<lanes_of(512)>(), Int<values_of(512)>(), Int<V>());
+    return fn(Type<T>(), Flag<SIGMOID>(), Int<lanes_of(1024)>(), Int<values_of(1024)>(), Int<V>());
+}
+template <typename T, bool SIGMOID, typename Fn>
+cudaError_t dispatch_packs(int experts, bool packs, Fn fn)
+{
+    return packs ? dispatch_width<T, SIGMOID, 16 / (int)sizeof(T)>(experts, fn) : dispatch_width<T, SIGMOID, 1>(experts, fn);
 }
 template <typename Fn>
 cudaError_t dispatch(const BalanceProblem &b, bool packs, Fn fn)
 {
     const bool sigmoid = b.scoring == kScoreSigmoid;
     switch (b.dtype) {
-        case kF32: return sigmoid ? dispatch_width<float, true>(b.experts, packs, fn) : dispatch_width<float, false>(b.experts, packs, fn);
-        case kF16: return sigmoid ? dispatch_width<__half, true>(b.experts, packs, fn) : dispatch_width<__half, false>(b.experts, packs, fn);
-        case kBF16: return sigmoid ? dispatch_width<__nv_bfloat16, true>(b.experts, packs, fn) : dispatch_width<__nv_bfloat16, false>(b.experts, packs, fn);
+        case kF32: return sigmoid ? dispatch_packs<float, true>(b.experts, packs, fn) : dispatch_packs<float, false>(b.experts, packs, fn);
+        case kF16: return sigmoid ? dispatch_packs<__half, true>(b.experts, packs, fn) : dispatch_packs<__half, false>(b.experts, packs, fn);
+        case kBF16: return sigmoid ? dispatch_packs<__nv_bfloat16, true>(b.experts, packs, fn) : dispatch_packs<__nv_bfloat16, false>(b.experts, packs, fn);
         default: return cudaErrorInvalidValue;
     }
 }
@@ -651,12 +669,13 @@ struct Layout {
     explicit Layout(const BalanceProblem &b)
     {
         // One piece for each CTA that there is room for at once, in smaller CTAs where there are many sequences, each of which has a piece
-        // that it shares with none; at least a row for each warp.
+        // that it shares with none; at least a row for each group of lanes.
         const int most = warps_of(b.experts);
         const auto at_once = [&] { return 148 * (most / warps); };
         for (warps = most; warps > 4 && at_once() < 2 * b.sequences;) warps /= 2;
+        const int at_least = warps * (32 / lanes_of(b.experts));
         const int64_t wanted = at_once() >= 2 * b.sequences ? at_once() - b.sequences + 1 : at_once() / 2, each = (b.rows + wanted - 1) / wanted;
-        chunk = (int)(each < warps ? warps : each);
+        chunk = (int)(each < at_least ? at_least : each);
         blocks = (int)((b.rows + chunk - 1) / chunk);
         const size_t pieces = (size_t)blocks + (size_t)b.sequences;
         tokens = 256;
@@ -678,9 +697,10 @@ cudaError_t balance_launch(const BalanceProblem &b, void *workspace, size_t work
 {
     BalanceParams p = params_of(b);
     const bool all = one_block(b);
+    const int groups = 32 / lanes_of(b.experts);
     int blocks = 1, warps = warps_of(b.experts);
     if (all) {
-        if (warps > b.rows) warps = b.rows < 4 ? 4 : (int)b.rows;
+        if (warps * groups > b.rows) warps = b.rows <= 4 * groups ? 4 : (int)(b.rows + groups - 1) / groups;
         p.chunk = kAllRows;
     } else {
         const Layout at(b);
@@ -696,11 +716,11 @@ cudaError_t balance_launch(const BalanceProblem &b, void *workspace, size_t work
         warps = at.warps;
         blocks = at.blocks + (int)b.sequences - (at.blocks > 0);    // no rows: the ticket is cleared all the same
     }
-    cudaError_t e = dispatch(b, in_packs(b.logits, b.ld, b), [&](auto type, auto sigmoid, auto per, auto v) {
+    cudaError_t e = dispatch(b, in_packs(b.logits, b.ld, b), [&](auto type, auto sigmoid, auto lanes, auto per, auto v) {
         typedef typename decltype(type)::type T;
-        const auto kernel = all ? balance_rows_kernel<T, decltype(sigmoid)::value, decltype(per)::value, decltype(v)::value, true>
-                                : balance_rows_kernel<T, decltype(sigmoid)::value, decltype(per)::value, decltype(v)::value, false>;
-        return launch_dependent(kernel, dim3(blocks), warps * 32, (size_t)(warps + 1) * b.experts * 4, 1, stream, p);
+        const auto kernel = all ? balance_rows_kernel<T, decltype(sigmoid)::value, decltype(lanes)::value, decltype(per)::value, decltype(v)::value, true>
+                                : balance_rows_kernel<T, decltype(sigmoid)::value, decltype(lanes)::value, decltype(per)::value, decltype(v)::value, false>;
+        return launch_dependent(kernel, dim3(blocks), warps * 32, (size_t)(warps * groups + 1) * b.experts * 4, 1, stream, p);
     });
     if (e != cudaSuccess || all) return e;
     if (b.sequences <= kFewSequences) return launch_dependent(balance_finish_few_kernel, dim3(kFinishCtas), 1024, 0, kFinishCtas, stream, p);
@@ -711,13 +731,14 @@ cudaError_t balance_grad_launch(const BalanceProblem &b, cudaStream_t stream)
 {
     if (b.rows <= 0) return cudaSuccess;
     BalanceParams p = params_of(b);
-    // rows of a warp: four blocks an SM
-    const int64_t warps = 4 * 148 * kGradWarps;
+    // rows of a warp: as many blocks as an SM holds
+    const int64_t warps = (b.experts <= 256 ? 4 : 2) * 148 * kGradWarps;
     p.chunk = (int)((b.rows + warps - 1) / warps);
     const int64_t blocks = (b.rows + (int64_t)p.chunk * kGradWarps - 1) / ((int64_t)p.chunk * kGradWarps);
-    return dispatch(b, in_packs(b.logits, b.ld, b) && in_packs(b.grad, b.ld_grad, b) && !((uintptr_t)b.counts & 15), [&](auto type, auto sigmoid, auto per, auto v) {
+    return dispatch(b, in_packs(b.logits, b.ld, b) && in_packs(b.grad, b.ld_grad, b) && !((uintptr_t)b.counts & 15), [&](auto type, auto sigmoid, auto lanes, auto per, auto v) {
         typedef typename decltype(type)::type T;
-        return launch_dependent(balance_grad_kernel<T, decltype(sigmoid)::value, decltype(per)::value, decltype(v)::value>, dim3((unsigned)blocks),
+        constexpr int values = decltype(lanes)::value < 32 ? 8 : decltype(per)::value;   // of a lane where a warp holds a row
+        return launch_dependent(balance_grad_kernel<T, decltype(sigmoid)::value, values, decltype(v)::value>, dim3((unsigned)blocks),
                                 kGradThreads, 0, 1, stream, p);
     });
 }
