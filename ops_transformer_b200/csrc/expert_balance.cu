@@ -610,9 +610,6 @@ __global__ void __launch_bounds__(kGradThreads, PER <= 8 ? 4 : 2) balance_grad_k
     }
 }
 
-// Most rows that one CTA takes by itself (256 experts, bf16: 64 rows 4.1 us against 6.5 with more CTAs and a second kernel, 128 5.5, 192 6.6).
-constexpr int kAllRows = 128;
-
 size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
 // fn(kernel traits) for the type, the scoring and the way that rows are loaded.
@@ -687,7 +684,9 @@ struct Layout {
     }
 };
 
-bool one_block(const BalanceProblem &b) { return !b.cu_seqlens && b.rows <= kAllRows; }
+// One CTA takes all rows by itself while that is no longer than many and a second kernel behind them, which are 6.2 to 6.8 us (bf16; 16 rows of
+// 64 experts 2.2 us, 128 3.6, 512 5.6; of 256 experts 32 2.9, 128 5.0, 192 6.3; of 1024 32 5.1, 64 7.9).
+bool one_block(const BalanceProblem &b) { return !b.cu_seqlens && b.rows * (b.experts < 64 ? 64 : b.experts) <= 40 * 1024; }
 
 }  // namespace
 
@@ -701,7 +700,7 @@ cudaError_t balance_launch(const BalanceProblem &b, void *workspace, size_t work
     int blocks = 1, warps = warps_of(b.experts);
     if (all) {
         if (warps * groups > b.rows) warps = b.rows <= 4 * groups ? 4 : (int)(b.rows + groups - 1) / groups;
-        p.chunk = kAllRows;
+        p.chunk = (int)b.rows;
     } else {
         const Layout at(b);
         if (!workspace || workspace_bytes < at.bytes) return cudaErrorInvalidValue;
