@@ -24,7 +24,7 @@ HEADERS = ["gmm_common.h", "norm_common.h", "dependent.h", "acl_shim.h", "op_api
 # fuse a multiply and an add.  No fast-math.
 NVCC_FLAGS = [
     "-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-fmad=false",
-    "-Xcompiler", "-fPIC,-fvisibility=hidden,-Wall", "-shared", "-cudart", "static",
+    "-Xcompiler", "-fPIC,-fvisibility=hidden,-Wall", "-shared", "-cudart", "static", "-t", "0",   # files side by side
 ]
 
 

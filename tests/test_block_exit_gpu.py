@@ -829,3 +829,79 @@ def test_shared_expert_as_the_grouped_product_gives_it():
         x, w, scale, token = int8((m, k), 1), int8((1, k, n), 2), rand((1, n), 3) * 0.01, rand((m,), 4)
         group = torch.full((1,), m, dtype=I64, device=DEV)
         assert torch.equal(ops.quant_matmul(x, w[0], scale[0], token), ops.grouped_matmul_v4(x, w, scale, token, group))
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# sizes and arguments at the edge of what is allowed
+# ---------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("m,k,n,nk", [(600_000, 128, 4096, False), (300_000, 8192, 160, True), (300_001, 7170, 20, False)])
+def test_matmul_beyond_32_bits(m, k, n, nk):
+    """Rows of the result, or of x, behind the 2^31st element: as a call of their own gives them."""
+    x = torch.zeros((m, k), dtype=I8, device=DEV)
+    x[-300:] = int8((300, k), 1)
+    w = int8((n, k), 2).t() if nk else int8((k, n), 2)
+    scale, token, bias = rand((n,), 3), rand((m,), 4), rand((n,), 5)
+    got = ops.quant_matmul(x, w, scale, token, bias=bias)
+    assert torch.equal(got[-300:], ops.quant_matmul(x[-300:].clone(), w, scale, token[-300:].clone(), bias=bias))
+    assert (got[:1000] == bias.to(BF16)).all() and (got[m // 2:m // 2 + 1000] == bias.to(BF16)).all()
+
+
+@pytest.mark.parametrize("rows,h", [(310_000, 7168), (310_001, 7001), (40_000, 65535), (9_000_000, 256)])
+def test_sandwich_beyond_32_bits(rows, h):
+    x, residual = (torch.zeros((rows, h), dtype=F16, device=DEV) for _ in range(2))
+    t = sandwich_inputs(200, h, F16, F16)
+    x[-200:], residual[-200:] = t["x"], t["residual"]
+    got = ops.sandwich_norm_quant(x, residual, t["gamma"], post_gamma=t["gamma"], normed=True)
+    check_sandwich(t["x"], t["residual"], t["gamma"], [v[-200:] for v in got], post_gamma=t["gamma"], normed=True)
+    assert all((v[:1000] == 0).all() and (v[rows // 2:rows // 2 + 1000] == 0).all() for v in got)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_balance_beyond_32_bits(scoring):
+    """The same 4096 tokens 1100 times over: their loss is that of them once, and a gradient the 1100th part."""
+    times, E = 1100, 512
+    logits, ids = balance_inputs(4096, E, 8, BF16)
+    loss, counts, weight = ops.expert_balance(logits, ids, scoring=scoring)
+    grad = ops.expert_balance_grad(logits, counts, weight, scoring=scoring, grad_loss=torch.tensor(4096.0, device=DEV))
+    many, many_ids = logits.repeat(times, 1), ids.repeat(times, 1)
+    assert many.numel() > 1 << 31
+    got = ops.expert_balance(many, many_ids, scoring=scoring)
+    assert torch.equal(got[1], counts * times)
+    # sums of 4.5 million scores: a warp's rows, its groups, the pieces
+    assert abs(got[0].item() / loss.item() - 1) <= (4096 * times / 148 / 16 + 80) * U32
+    g = ops.expert_balance_grad(many, got[1], got[2], scoring=scoring, grad_loss=torch.tensor(4096.0 * times, device=DEV))
+    for part in (g[:4096], g[-4096:]):
+        # the same steps with factors that are rounded apart: half a unit of bf16 each, and single ones of fp32
+        assert ((part.double() - grad.double()).abs() <= grad.double().abs() * 2.0 ** -7 + 1e-30).all()
+
+
+def test_balance_arguments_of_other_strides_and_places():
+    logits, ids = balance_inputs(700, 64, 4, F32)
+    mask = rand((1400,), 1) < 0.6
+    cu = torch.tensor([0, 9, 100, 9, 350, 9, 700, 9], device=DEV, dtype=I32)
+    for kw in (dict(token_mask=mask[::2]), dict(cu_seqlens=cu[::2]), dict(token_mask=mask[::2].to(I8), cu_seqlens=cu[::2])):
+        dense = {k: v.contiguous() for k, v in kw.items()}
+        want = ops.expert_balance(logits, ids, **dense)
+        want_grad = ops.expert_balance_grad(logits, *want[1:], **dense)
+        n = 3 if "cu_seqlens" in kw else 1
+        room = torch.full((9,), 7.0, device=DEV)
+        counts = torch.full((n, 2 * 64) if n > 1 else (2 * 64,), 5, device=DEV, dtype=I64)[..., ::2]
+        weight = torch.full((2 * n,), 3.0, device=DEV)
+        loss, c, w = ops.expert_balance(logits, ids, loss=room[4], counts=counts, weight=weight[::2], **kw)
+        assert torch.equal(loss, want[0]) and room[4] == want[0] and (room[:4] == 7).all() and (room[5:] == 7).all()
+        assert torch.equal(c, want[1]) and torch.equal(w, want[2]) and (weight[1::2] == 3).all()
+        assert torch.equal(ops.expert_balance_grad(logits, c, w, grad_loss=torch.ones(3, device=DEV)[1], **kw), want_grad)
+        # counts on no 16-byte boundary
+        off = torch.zeros(want[1].numel() + 1, dtype=I64, device=DEV)[1:].view_as(want[1]).copy_(want[1])
+        # (other lanes have the experts then: two sums of 64 terms a row in another order, 6 additions each, and what is formed from them)
+        assert (ops.expert_balance_grad(logits, off, w.clone(), **dense) - want_grad).abs().max() <= 2 * (6 + 6 + 4) * U32 * want_grad.abs().max()
+
+
+def test_sandwich_normed_rows_in_place_of_x():
+    for rows, h in ((20, 512), (400, 5001), (300, 7168), (3, 40000)):
+        t = sandwich_inputs(rows, h, BF16, BF16)
+        want = ops.sandwich_norm_quant(**t, post_gamma=t["gamma"], normed=True)
+        x = t["x"].clone()
+        got = ops.sandwich_norm_quant(x, t["residual"], t["gamma"], post_gamma=t["gamma"], normed_out=x)
+        assert got[3] is x and all(torch.equal(a, b) for a, b in zip(got, want))
