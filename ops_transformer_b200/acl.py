@@ -113,6 +113,11 @@ class _Workspace:
                     del self._slots[next(iter(self._slots))]
         return s
 
+    def slot_of(self, index: int, handle: int) -> _Slot:
+        """The same by a GPU's number."""
+        s = self._slots.get(("cuda", index, handle, 0)) if handle != _STREAM_PER_THREAD else None
+        return s if s is not None else self.slot(torch.device("cuda", index), handle)
+
     def lend(self, slot: _Slot, device: torch.device, stream, nbytes: int) -> torch.Tensor:
         """A workspace of at least ``nbytes`` for the call that is about to be enqueued with the slot's lock held."""
         return (self.for_capture if device.type == "cuda" and _capturing(stream) else self.grown)(slot, device, stream, nbytes)
@@ -436,6 +441,7 @@ def _float_bits(v: float) -> int:
     return _WORD.unpack(_FLOAT.pack(v))[0]
 
 
+_current_device, _raw_stream = (getattr(torch._C, name, None) for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"))
 _POOLED = frozenset((_lib.OP_ADAPTER_ADD, _lib.OP_QUANT_MATMUL, _lib.OP_EXPERT_BALANCE))
 
 
@@ -446,6 +452,17 @@ def _block_call(op: int, name: str, workspace: Optional[torch.Tensor], stream, o
     ``_POOLED`` and strided views) takes none.  Returns the workspace that the call uses (None if none)."""
     module, call = _lib.native()
     x, buf = items[0], workspace
+    if workspace is None and stream is None and options is None and x.get_device() >= 0 and x.get_device() == _current_device():
+        # what most calls are, with as little on the way as can be: their kernels are often shorter
+        handle = _raw_stream(x.get_device())
+        if op not in _POOLED:
+            done = module.launch(call, op, handle, None, 0, kinds, *items)
+        else:
+            slot = _WS.slot_of(x.get_device(), handle)
+            with slot.lock:   # the clear and the kernels of two calls must not interleave on the stream
+                buf = slot.buf
+                done = module.launch(call, op | _lib.OP_POOLED, handle, buf, 0, kinds, *items)
+        return buf if done is None else _block_rest(op, name, workspace, stream, handle, kinds, items, done)
     if x.is_cuda and x.get_device() != torch._C._cuda_getDevice():
         with torch.cuda.device(x.device):
             return _block_call(op, name, workspace, stream, options, kinds, *items)
@@ -453,6 +470,7 @@ def _block_call(op: int, name: str, workspace: Optional[torch.Tensor], stream, o
     if workspace is not None and not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
     pooled = workspace is None and op in _POOLED
+    handle = None
     if not x.is_cuda:
         done = False
     else:
@@ -464,8 +482,12 @@ def _block_call(op: int, name: str, workspace: Optional[torch.Tensor], stream, o
                 done = module.launch(call, op | _lib.OP_POOLED, handle, buf, how, kinds, *items)
         else:
             done = module.launch(call, op, handle, workspace, how, kinds, *items)
-    if done is None:
-        return buf
+    return buf if done is None else _block_rest(op, name, workspace, stream, handle, kinds, items, done)
+
+
+def _block_rest(op: int, name: str, workspace, stream, handle, kinds: str, items, done) -> Optional[torch.Tensor]:
+    """What a call that was not enqueued at once still needs: its refusal, or a workspace."""
+    x = items[0]
     if done is False:
         words = _lib.describe_call(kinds, *items)
         res = _lib.CallResult()
