@@ -8,6 +8,10 @@
 // the same to write p and read it back.  A group of 8, 16 or 32 lanes holds a row, a lane 16 of its experts or so: fewer lanes make fewer
 // steps of sums and maxima across them, and of all that a row costs once.  Sums over tokens are made in a fixed order (a lane's rows one
 // after the other, then the groups, then the pieces), so that a call gives the same bits every time.
+//
+// Measured, us (forward, gradient): 16 x 64 bf16 2.2, 2.0; 4096 x 256 bf16 7.2, 3.8; 16384 x 256 fp32 in 16 sequences 12.7, 9.1; 65536 x 256 bf16
+// 17.0, 17.7 (2 TB/s and 3.8).  Loads' latency bounds the large ones: with no scores and no ids to work on 65536 rows take 12.0, each of the
+// two adds about 4.6, and half the instructions (16 lanes a row for 32) changed nothing.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -499,7 +499,8 @@ def cuts(t, n, seed, last=None):
 
 
 @pytest.mark.parametrize("t,E,k,n", [(1, 8, 2, 1), (40, 64, 4, 3), (40, 64, 4, 40), (700, 33, 3, 16), (5000, 256, 8, 5), (5000, 128, 8, 300), (16384, 256, 8, 16), (300, 16, 2, 2000), (2000, 1000, 3, 20), (900, 600, 2, 32),
-                                     (900, 8, 2, 33)])
+                                     (900, 8, 2, 33), (19, 172, 4, 19), (150, 256, 8, 32), (600, 64, 8, 7), (40, 1024, 8, 16), (40, 1024, 8, 17), (320, 121, 5, 3),
+                                     (80, 512, 4, 32), (1, 64, 4, 32)])
 def test_balance_sequences(t, E, k, n):
     for dtype, scoring in ((F32, "softmax"), (BF16, "sigmoid")):
         logits, ids = balance_inputs(t, E, k, dtype, seed=7)
@@ -514,6 +515,15 @@ def test_balance_of_one_sequence_is_that_of_all_rows():
     a, b = ops.expert_balance(logits, ids), ops.expert_balance(logits, ids, cu_seqlens=cu)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1][0]) and torch.equal(a[2], b[2])
     assert torch.equal(ops.expert_balance_grad(logits, *a[1:]), ops.expert_balance_grad(logits, *b[1:], cu_seqlens=cu))
+
+
+def test_balance_few_rows_outside_and_between():
+    """Sequences that begin and end inside and on the borders of what a group of lanes holds, empty ones among them, rows before and behind."""
+    for rows, E in ((97, 64), (160, 256), (33, 1000)):
+        logits, ids = balance_inputs(rows, E, 4, F32)
+        for cu in ([0, rows], [5, 5, 6, 6, rows - 3], [0, 0, 0, rows, rows], [rows, rows], [0, 0], [1, 2, 3, 4, 5, 6, 7, 8, 16, 24, 25, 32], list(range(0, 33)),
+                   [0, 8, 16, 32], [31, 32, 33]):
+            check_balance(logits, ids, cu=torch.tensor(cu, device=DEV, dtype=I32), mask=rand((rows,), 3) < 0.8)
 
 
 def test_balance_rows_outside_the_sequences():
