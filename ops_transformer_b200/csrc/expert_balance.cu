@@ -9,7 +9,7 @@
 // steps of sums and maxima across them, and of all that a row costs once.  Sums over tokens are made in a fixed order (a lane's rows one
 // after the other, then the groups, then the pieces), so that a call gives the same bits every time.
 //
-// Measured, us (forward, gradient): 16 x 64 bf16 2.2, 2.0; 4096 x 256 bf16 7.2, 3.8; 16384 x 256 fp32 in 16 sequences 12.7, 9.1; 65536 x 256 bf16
+// Measured, us (forward, gradient): 16 x 64 bf16 2.2, 2.0; 256 x 256 bf16 4.0, 2.3; 4096 x 256 bf16 7.2, 3.8; 16384 x 256 fp32 in 16 sequences 12.7, 9.1; 65536 x 256 bf16
 // 17.0, 17.7 (2 TB/s and 3.8).  Loads' latency bounds the large ones: with no scores and no ids to work on 65536 rows take 12.0, each of the
 // two adds about 4.6, and half the instructions (16 lanes a row for 32) changed nothing.
 #include <cuda_bf16.h>
@@ -24,6 +24,7 @@
 namespace gmm {
 namespace {
 
+constexpr int kMostCtas = 8;    // of a cluster that takes all rows
 constexpr int kGradThreads = 256, kGradWarps = kGradThreads / 32;
 // Lanes of a row and values of a lane by the number of experts, and the threads of a block of rows, at most: as many as there are registers
 // for.
@@ -276,14 +277,27 @@ __device__ __forceinline__ int seq_of_piece(const BalanceParams &p, int piece, i
     return lo;
 }
 
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_first_cta(const void *p)
+{
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)));
+    return r;
+}
+
 // What a block of rows adds to a sequence: one piece, which a CTA makes.  A warp takes a row for each of its groups of G lanes at a time, and
-// has the loads of R times as many under way.  ALL: the rows are all those of the only sequence, and the CTA finishes.
+// has the loads of R times as many under way.  ALL: the CTAs, one or a cluster, hold all rows of the only sequence; the first one adds up what
+// the others put into its shared memory, and finishes.
 template <typename T, bool SIGMOID, int G, int PER, int V, bool ALL>
 __global__ void __launch_bounds__(threads_of(PER), 1) balance_rows_kernel(const BalanceParams p)
 {
     constexpr int R = rows_ahead<T, PER, V>(PER <= 8 ? 8 : 16), GROUPS = 32 / G;
     extern __shared__ float4 smem[];    // sums [warps][GROUPS][experts], then the counts [experts]
-    __shared__ int warp_tokens[32];
+    __shared__ int warp_tokens[32], cta_tokens[kMostCtas];
     __shared__ double warp_dots[32];
     float *sums = reinterpret_cast<float *>(smem);
     const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = threads >> 5, piece = blockIdx.x;
@@ -295,7 +309,8 @@ __global__ void __launch_bounds__(threads_of(PER), 1) balance_rows_kernel(const 
     if (!ALL && piece == 0 && tid == 0) *p.ticket = 0;
     const int s = ALL ? 0 : seq_of_piece(p, piece, lane);
     if (s >= p.sequences) return;
-    const int begin = ALL ? 0 : max(seq_begin(p, s), (piece - s) * p.chunk), end = ALL ? p.rows : min(seq_end(p, s), (piece - s + 1) * p.chunk);
+    const int begin = ALL ? piece * p.chunk : max(seq_begin(p, s), (piece - s) * p.chunk);
+    const int end = min(ALL ? p.rows : seq_end(p, s), (piece - s + 1) * p.chunk);
     if (!ALL && begin >= end) return;
     f32x2 sum[PER / 2] = {};
     int tokens = 0;
@@ -358,34 +373,67 @@ __global__ void __launch_bounds__(threads_of(PER), 1) balance_rows_kernel(const 
         }
     }
     __syncthreads();
-    double dot = 0.0;
-    for (int e = tid; e < p.experts; e += threads) {
+    const auto total_of = [&](int e) {
         float total = 0.0f;
 #pragma unroll 8
         for (int w = 0; w < step; ++w) total += sums[w * p.experts + e];
-        if (ALL) {
-            p.counts[e] = counts[e];
-            dot += (double)total * counts[e];
-        } else {
-            p.piece_sums[(long long)piece * p.experts + e] = total;
+        return total;
+    };
+    tokens = (int)__reduce_add_sync(0xffffffffu, lane < warps ? warp_tokens[lane] : 0);
+    if constexpr (!ALL) {
+        for (int e = tid; e < p.experts; e += threads) {
+            p.piece_sums[(long long)piece * p.experts + e] = total_of(e);
             p.piece_counts[(long long)piece * p.experts + e] = counts[e];
         }
+        if (tid == 0) p.piece_tokens[piece] = tokens;
+        return;
     }
-    if (ALL) {
-        dot = warp_sum(dot);
-        if (lane == 0) warp_dots[warp] = dot;
-        __syncthreads();
+    const int ctas = gridDim.x;
+    double dot = 0.0;
+    if (ctas == 1) {
+        for (int e = tid; e < p.experts; e += threads) {
+            p.counts[e] = counts[e];
+            dot += (double)total_of(e) * counts[e];
+        }
+    } else {
+        constexpr int N = PER / 8;      // experts of a thread, of as many threads as there can be
+        float total[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) total[i] = tid + i * threads < p.experts ? total_of(tid + i * threads) : 0.0f;
+        cluster_sync();     // the first CTA has done with its sums, whose place the parts take
+        const uint32_t parts = in_first_cta(sums);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int e = tid + i * threads;
+            if (e < p.experts)
+                asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(parts + (uint32_t)(piece * p.experts + e) * 8), "r"(__float_as_uint(total[i])), "r"(counts[e]) : "memory");
+        }
+        if (tid == 0) asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(in_first_cta(cta_tokens + piece)), "r"(tokens) : "memory");
+        cluster_sync();
+        if (piece != 0) return;
+        const uint2 *here = reinterpret_cast<const uint2 *>(sums);
+        for (int e = tid; e < p.experts; e += threads) {
+            float sum = 0.0f;
+            int count = 0;
+#pragma unroll 8
+            for (int c = 0; c < ctas; ++c) {
+                const uint2 v = here[c * p.experts + e];
+                sum += __uint_as_float(v.x);
+                count += (int)v.y;
+            }
+            p.counts[e] = count;
+            dot += (double)sum * count;
+        }
+        tokens = (int)__reduce_add_sync(0xffffffffu, lane < ctas ? cta_tokens[lane] : 0);
     }
+    dot = warp_sum(dot);
+    if (lane == 0) warp_dots[warp] = dot;
+    __syncthreads();
     if (warp != 0) return;
-    tokens = (int)__reduce_add_sync(0xffffffffu, lane < warps ? warp_tokens[lane] : 0);
-    if (ALL) {
-        dot = warp_sum(lane < warps ? warp_dots[lane] : 0.0);
-        const float weight = weight_of(p, tokens, 1);
-        if (lane == 0) p.weight[0] = weight;
-        if (lane == 0) *p.loss = (float)(dot * weight);
-    } else if (lane == 0) {
-        p.piece_tokens[piece] = tokens;
-    }
+    dot = warp_sum(lane < warps ? warp_dots[lane] : 0.0);
+    const float weight = weight_of(p, tokens, 1);
+    if (lane == 0) p.weight[0] = weight;
+    if (lane == 0) *p.loss = (float)(dot * weight);
 }
 
 // The sums of a warp's share of a sequence's pieces, for the expert of each lane; N of them under way.
@@ -460,12 +508,9 @@ __global__ void __launch_bounds__(1024, 1) balance_finish_few_kernel(const Balan
     if (tid < p.sequences) {
         double dot = 0.0;
         for (int g = 0; g < groups; ++g) dot += dots[tid * groups + g];
-        uint32_t to;
-        asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"((uint32_t)__cvta_generic_to_shared(&all_dots[rank][tid])));
-        asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(dot) : "memory");
+        asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(in_first_cta(&all_dots[rank][tid])), "d"(dot) : "memory");
     }
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_sync();
     if (rank != 0 || warp != 0) return;
     const int mine = lane < p.sequences ? tokens_of[lane] : 0;
     const float weight = weight_of(p, mine, __popc(__ballot_sync(0xffffffffu, mine > 0)));
@@ -688,23 +733,30 @@ struct Layout {
     }
 };
 
-// One CTA takes all rows by itself while that is no longer than many and a second kernel behind them, which are 6.2 to 6.8 us (bf16; 16 rows of
-// 64 experts 2.2 us, 128 3.6, 512 5.6; of 256 experts 32 2.9, 128 5.0, 192 6.3; of 1024 32 5.1, 64 7.9).
-bool one_block(const BalanceProblem &b) { return !b.cu_seqlens && b.rows * (b.experts < 64 ? 64 : b.experts) <= 40 * 1024; }
+// CTAs that take all rows by themselves, one up to 12 K scores and a cluster up to 256 K; 0: more of them, and a second kernel behind them.
+// (one CTA / a cluster / two kernels, us, bf16: 48 x 256 3.5, 3.5, 6.4; 128 x 256 5.2, 3.7, 6.4; 1024 x 256 24, 6.4, 6.8; 2048 x 256 46, 9.3, 7.1;
+// 128 x 64 3.7, 4.1, 6.8; 4096 x 64 27, 6.8, 7.4; 512 x 512 22, 6.6, 6.9; with four CTAs 16 x 1024 3.9, 4.3, 6.5; 128 x 1024 13, 7.1, 7.1)
+int ctas_of_all(const BalanceProblem &b)
+{
+    const int64_t scores = b.rows * (b.experts < 64 ? 64 : b.experts);
+    const int most = b.experts <= 512 ? kMostCtas : kMostCtas / 2;      // whose parts fit where the first one's sums were
+    return b.cu_seqlens ? 0 : scores <= 12 * 1024 ? 1 : scores <= 32 * 1024 * most ? most : 0;
+}
 
 }  // namespace
 
-size_t balance_workspace_bytes(const BalanceProblem &b) { return one_block(b) ? 0 : Layout(b).bytes; }
+size_t balance_workspace_bytes(const BalanceProblem &b) { return ctas_of_all(b) ? 0 : Layout(b).bytes; }
 
 cudaError_t balance_launch(const BalanceProblem &b, void *workspace, size_t workspace_bytes, cudaStream_t stream)
 {
     BalanceParams p = params_of(b);
-    const bool all = one_block(b);
+    const int all = ctas_of_all(b);
     const int groups = 32 / lanes_of(b.experts);
     int blocks = 1, warps = warps_of(b.experts);
     if (all) {
-        if (warps * groups > b.rows) warps = b.rows <= 4 * groups ? 4 : (int)(b.rows + groups - 1) / groups;
-        p.chunk = (int)b.rows;
+        if (all == 1 && warps * groups > b.rows) warps = b.rows <= 4 * groups ? 4 : (int)(b.rows + groups - 1) / groups;
+        blocks = all;
+        p.chunk = (int)((b.rows + all - 1) / all);
     } else {
         const Layout at(b);
         if (!workspace || workspace_bytes < at.bytes) return cudaErrorInvalidValue;
@@ -723,7 +775,7 @@ cudaError_t balance_launch(const BalanceProblem &b, void *workspace, size_t work
         typedef typename decltype(type)::type T;
         const auto kernel = all ? balance_rows_kernel<T, decltype(sigmoid)::value, decltype(lanes)::value, decltype(per)::value, decltype(v)::value, true>
                                 : balance_rows_kernel<T, decltype(sigmoid)::value, decltype(lanes)::value, decltype(per)::value, decltype(v)::value, false>;
-        return launch_dependent(kernel, dim3(blocks), warps * 32, (size_t)(warps * groups + 1) * b.experts * 4, 1, stream, p);
+        return launch_dependent(kernel, dim3(blocks), warps * 32, (size_t)(warps * groups + 1) * b.experts * 4, all > 1 ? all : 1, stream, p);
     });
     if (e != cudaSuccess || all) return e;
     if (b.sequences <= kFewSequences) return launch_dependent(balance_finish_few_kernel, dim3(kFinishCtas), 1024, 0, kFinishCtas, stream, p);

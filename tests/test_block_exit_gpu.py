@@ -477,7 +477,7 @@ def balance_inputs(t, E, k, dtype, seed=0):
 
 
 BALANCE_SIZES = [(1, 1, 1), (1, 8, 2), (16, 64, 8), (17, 31, 3), (64, 256, 8), (65, 33, 4), (300, 100, 6), (512, 160, 8), (1000, 161, 8), (611, 512, 4), (300, 1024, 8),
-                 (77, 1000, 2), (3001, 155, 6), (5000, 256, 8), (16384, 64, 8), (9000, 8, 1), (2500, 257, 5)]
+                 (77, 1000, 2), (48, 256, 8), (49, 256, 8), (1024, 256, 8), (1025, 256, 8), (500, 512, 8), (4000, 40, 5), (129, 1024, 4), (3001, 155, 6), (5000, 256, 8), (16384, 64, 8), (9000, 8, 1), (2500, 257, 5)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
