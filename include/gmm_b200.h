@@ -244,7 +244,7 @@ ACL_FUNC_VISIBILITY aclnnStatus gmmB200SandwichNormQuant(void *workspace, uint64
  * made in a fixed order.
  *   logits            fp32 / fp16 / bf16 [rows, experts], experts in [1, 1024], rows may be 0 (the loss is 0 then).  An expert whose logit
  *                     is NaN or minus infinity is not there (p = 0); those of plus infinity share the row's softmax.  A row whose
- *                     scores are all 0 in fp32 has p = 0
+ *                     sigmoids are all below e^-700 has p = 0
  *   ids               int32 / int64 [rows, top_k], top_k in [1, 1024]; ids that name no expert (-1) are not counted
  *   tokenMask         int8 or bool [rows], optional: rows whose value is 0 hold no token
  *   cuSeqlens         int32 [sequences + 1], optional, not falling: sequence s is the rows [cuSeqlens[s], cuSeqlens[s + 1]), at most 65535
