@@ -96,6 +96,107 @@ __global__ void __launch_bounds__(256) sandwich_any_kernel(const SandwichParams 
     }
 }
 
+// The same for few rows, in batches of loads that wait for nothing between them.
+template <typename T, typename X>
+__global__ void __launch_bounds__(1024, 1) sandwich_any_few_kernel(const SandwichParams p)
+{
+    constexpr int N = 4;    // elements of a batch
+    __shared__ float2 red[2][32];
+    dependent_wait();
+    dependent_release();
+    const long long row = blockIdx.x;
+    const int threads = blockDim.x;
+    const X *x = static_cast<const X *>(p.x) + row * p.ld_x;
+    const T *residual = static_cast<const T *>(p.residual) + row * p.ld_residual, *gate = static_cast<const T *>(p.gate) + row * p.ld_gate;
+    float norm = 1.0f;
+    if (p.post_gamma) {
+        float sum = 0.0f, unused = 0.0f;
+        for (int e0 = threadIdx.x; e0 < p.h; e0 += N * threads) {
+            float v[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = e0 + i * threads < p.h ? to_float<X>(x[e0 + i * threads]) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum = __fmaf_rn(v[i], v[i], sum);
+        }
+        block_reduce(sum, unused, red[0]);
+        norm = rsqrtf(__fmaf_rn(sum, p.inv_h, p.post_eps));
+    }
+    // A batch of the stream and of what multiplies it behind the norm; all loads come before the first conversion.
+    float s[N], g[N], m[N];
+    const auto load = [&](int e0) {
+        const auto at = [&](int i) { return min(e0 + i * threads, p.h - 1); };   // what is beyond the row is loaded for nothing
+        X xs[N];
+        T rs[N], gates[N], post[N], next[N];
+        float post32[N], next32[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) xs[i] = x[at(i)];
+#pragma unroll
+        for (int i = 0; i < N; ++i) rs[i] = residual[at(i)];
+        const auto load_gammas = [&](const void *from, T (&v)[N], float (&v32)[N]) {
+            if (!from) return;
+            if (p.gamma32) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) v32[i] = static_cast<const float *>(from)[at(i)];
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[i] = static_cast<const T *>(from)[at(i)];
+            }
+        };
+        load_gammas(p.post_gamma, post, post32);
+        load_gammas(p.gamma, next, next32);
+        if (p.gate) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) gates[i] = gate[at(i) * p.gate_step];
+        }
+        if (p.smooth) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) m[i] = p.smooth[at(i)];
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float n = to_float<X>(xs[i]);
+            if (p.post_gamma) n = __fmul_rn(__fmul_rn(n, norm), p.gamma32 ? post32[i] : to_float<T>(post[i]));
+            if (p.gate) n = __fmul_rn(n, gate_value(to_float<T>(gates[i]), p.gate_act));
+            s[i] = __fmaf_rn(p.residual_scale, to_float<T>(rs[i]), __fmul_rn(p.block_scale, n));
+            g[i] = p.gamma32 ? next32[i] : to_float<T>(next[i]);
+        }
+    };
+    float r = 0.0f, step = 0.0f;
+    if (p.gamma) {
+        float sum = 0.0f, mag = 0.0f;
+        for (int e0 = threadIdx.x; e0 < p.h; e0 += N * threads) {
+            load(e0);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (e0 + i * threads >= p.h) break;
+                sum = __fmaf_rn(s[i], s[i], sum);
+                const float u = p.smooth ? __fmul_rn(__fmul_rn(s[i], g[i]), m[i]) : __fmul_rn(s[i], g[i]);
+                if (p.q) mag = max_mag(mag, u, u);
+            }
+        }
+        block_reduce(sum, mag, red[1]);
+        r = rsqrtf(__fmaf_rn(sum, p.inv_h, p.eps));
+        step = step_of(mag);
+    }
+    Quantiser quant;
+    quant.set(step);
+    if (p.q && threadIdx.x == 0) p.scale[row] = step == 0.0f ? 0.0f : __fmul_rn(step, r);
+    for (int e0 = threadIdx.x; e0 < p.h; e0 += N * threads) {
+        load(e0);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int e = e0 + i * threads;
+            if (e >= p.h) break;
+            if (p.residual_out) static_cast<T *>(p.residual_out)[row * p.ld_residual_out + e] = from_float<T>(s[i]);
+            if (!p.gamma) continue;
+            float u = __fmul_rn(s[i], g[i]);
+            if (p.normed_out) static_cast<T *>(p.normed_out)[row * p.ld_normed + e] = from_float<T>(__fmul_rn(u, r));
+            if (p.smooth) u = __fmul_rn(u, m[i]);
+            if (p.q) p.q[row * p.ld_q + e] = (int8_t)quant.one(u);
+        }
+    }
+}
+
 // V values of a vector over the channels from `at` on, as pairs.
 template <typename G, int V, bool WHOLE>
 __device__ __forceinline__ void load_channels(const void *vec, int at, int h, f32x2 *f)
@@ -115,7 +216,8 @@ __device__ __forceinline__ void load_gammas(const void *vec, bool gamma32, int a
 
 // One CTA per row; a thread holds NCH packs of V elements (16 bytes of T), blockDim.x apart, in fp32 from the first look at x to the last
 // store.  WHOLE: rows start on packs.  Else every row starts `lead` elements into one, the same in all tensors, and only what lies in a row's
-// first and last pack is masked and stored one element at a time.
+// first and last pack is masked and stored one element at a time.  Its time is a row's chain of load, sum, load, sum and store (16 x 2048 2.7 us,
+// 128 x 7168 4.9, 600 x 16384 with four packs a thread 24).
 template <typename T, typename X, int NCH, bool WHOLE, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) sandwich_kernel(const SandwichParams p)
 {
@@ -665,6 +767,16 @@ cudaError_t launch_rows(const SandwichParams &p, const Groups &g, cudaStream_t s
     return launch_dependent(kernel, dim3(ctas < 148 ? ctas : 148), g.threads * g.groups, g.smem, 1, stream, p, g.threads, g.groups, g.depth);
 }
 
+template <typename T, typename X>
+cudaError_t launch_any(const SandwichParams &p, cudaStream_t stream)
+{
+    // Few rows: up to 1024 threads with eight elements or more each.  Many: small CTAs, of which an SM holds more (128 rows of 7168 on no pack
+    // 9.8 us against 17.5 with those, 16 of 40000 33 and 107, 300 of 40000 142 and 183, but 4096 of 7168 173 and 130).
+    const int wanted = (p.h + 7) / 8, most = p.rows <= 148 ? 1024 : 256, threads = wanted > most ? most : (wanted + 31) / 32 * 32;
+    if (p.rows <= 4 * 148) return launch_dependent(sandwich_any_few_kernel<T, X>, dim3(p.rows), threads, 0, 1, stream, p);
+    return launch_dependent(sandwich_any_kernel<T, X>, dim3(p.rows), 256, 0, 1, stream, p);
+}
+
 template <typename T, typename X, bool WHOLE>
 cudaError_t launch_packed(const SandwichParams &p, cudaStream_t stream)
 {
@@ -687,7 +799,7 @@ cudaError_t launch_packed(const SandwichParams &p, cudaStream_t stream)
         return gated ? launch_rows<T, X, WHOLE, false, true>(p, g, stream) : launch_rows<T, X, WHOLE, false, false>(p, g, stream);
     }
     if (packs <= 4 * 1024) return launch_dependent(sandwich_kernel<T, X, 4, WHOLE, 1024, 1>, dim3(p.rows), warps((packs + 3) / 4), 0, 1, stream, p);
-    return launch_dependent(sandwich_any_kernel<T, X>, dim3(p.rows), 256, 0, 1, stream, p);
+    return launch_any<T, X>(p, stream);
 }
 
 template <typename T, typename X>
@@ -705,7 +817,7 @@ cudaError_t launch_typed(const SandwichParams &p, cudaStream_t stream)
                         fits(p.post_gamma, p.ld_x, p.gamma32 ? 4 : sizeof(T)) && fits(p.smooth, p.ld_x, 4) &&
                         (!rows_gate || fits(p.gate, p.ld_gate, sizeof(T))) && (!channel_gate || fits(p.gate, p.ld_x, sizeof(T)));
     if (packed) return p.h % V == 0 && p.ld_x % V == 0 ? launch_packed<T, X, true>(p, stream) : launch_packed<T, X, false>(p, stream);
-    return launch_dependent(sandwich_any_kernel<T, X>, dim3(p.rows), 256, 0, 1, stream, p);
+    return launch_any<T, X>(p, stream);
 }
 
 }  // namespace
