@@ -277,10 +277,13 @@ __device__ __forceinline__ int seq_of_piece(const BalanceParams &p, int piece, i
     return lo;
 }
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync()
 {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    __syncwarp();           // a warp's lanes come from branches of their own
+    cluster_arrive();
+    cluster_wait();
 }
 __device__ __forceinline__ uint32_t in_first_cta(const void *p)
 {
@@ -478,6 +481,7 @@ __global__ void __launch_bounds__(1024, 1) balance_finish_few_kernel(const Balan
     int each = 1;
     while (each * 2 * items <= 32) each *= 2;
     const int part = warp & (each - 1);
+    cluster_arrive();       // this CTA is there, and can be sent to
     if (tid < kFewSequences) tokens_of[tid] = 0;
     dependent_wait();
     dependent_release();
@@ -505,6 +509,7 @@ __global__ void __launch_bounds__(1024, 1) balance_finish_few_kernel(const Balan
         }
         __syncthreads();
     }
+    cluster_wait();         // until the first CTA is there
     if (tid < p.sequences) {
         double dot = 0.0;
         for (int g = 0; g < groups; ++g) dot += dots[tid * groups + g];

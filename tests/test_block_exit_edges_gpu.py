@@ -1,0 +1,51 @@
+"""The operators of a block's exit where kernels wait: for other CTAs of a cluster, for copies that do not come, beside other work on the GPU."""
+import pytest
+import torch
+
+import ops_transformer_b200 as ops
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+BF16, F16, F32, I8, I32, I64 = torch.bfloat16, torch.float16, torch.float32, torch.int8, torch.int32, torch.int64
+
+
+def gen(seed):
+    return torch.Generator(DEV).manual_seed(seed)
+
+
+def randn(shape, seed, dtype=F32, scale=1.0):
+    return (torch.randn(shape, device=DEV, generator=gen(seed)) * scale).to(dtype)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# expert_balance: the cluster whose CTAs send one another their parts of the loss
+# ---------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,experts,sequences", [(3000, 64, None), (700, 256, 1), (900, 40, 7), (2000, 1000, 32), (40, 1024, 16)])
+def test_balance_clusters_beside_other_work(rows, experts, sequences):
+    """Calls among products of another stream, whose CTAs keep the SMs busy while those of a cluster come: the same bits each time, and the loss
+    that the counts and the scores' sums give."""
+    logits = randn((rows, experts), 1)
+    ids = (logits + randn((experts,), 2)).topk(4, 1).indices
+    cu = None if sequences is None else torch.linspace(0, rows, sequences + 1, device=DEV).to(I32)
+    first = ops.expert_balance(logits, ids, cu_seqlens=cu)
+    bounds = [0, rows] if cu is None else cu.tolist()
+    p, want = logits.double().softmax(1), 0.0
+    for a, b in zip(bounds[:-1], bounds[1:]):
+        want += experts / (4 * (b - a) ** 2) * (torch.bincount(ids[a:b].flatten(), minlength=experts) * p[a:b].sum(0)).sum().item() / (len(bounds) - 1)
+    # a score: its exponent's argument and size (logits within 10), the row's sum of E / 32 + 5 steps; over tokens at most rows / 148 + 80 additions
+    assert abs(first[0].item() - want) <= want * (10 + experts / 32 + 12 + rows / 148 + 80) * 2.0 ** -24
+    a = randn((2048, 2048), 3, BF16)
+    torch.cuda.synchronize()
+    busy, side = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for _ in range(30):
+        with torch.cuda.stream(busy):
+            b = a @ a
+        with torch.cuda.stream(side):
+            got += [ops.expert_balance(logits, ids, cu_seqlens=cu) for _ in range(3)]
+    torch.cuda.synchronize()
+    assert b.isfinite().all()
+    for again in got:
+        assert all(torch.equal(x, y) for x, y in zip(again, first))
