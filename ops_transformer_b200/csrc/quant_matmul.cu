@@ -44,6 +44,7 @@ struct MatmulParams {
     long long wait_limit;
     int skip_blocks;                // test only: K blocks that the producer leaves out
     int *status;
+    bool clear_status;              // else it has been, before the launch
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -264,8 +265,8 @@ __global__ void __launch_bounds__(kThreads) quant_matmul_kernel(const __grid_con
             if (p.bias) mine[1] = load_as_float(p.bias, p.bias_dtype, c0 + i);
         }
     }
-    // Block 0 is among the first to start, and a wait that runs out does so long after.
-    if (blockIdx.x == 0 && warp == 2 && lane < 4) p.status[lane] = 0;
+    // Block 0 is among the first to start, and a wait of the default limit runs out about a second after.
+    if (p.clear_status && blockIdx.x == 0 && warp == 2 && lane < 4) p.status[lane] = 0;
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -662,6 +663,12 @@ cudaError_t quant_matmul_launch(const QuantMatmulProblem &given, void *workspace
     if (!workspace || workspace_bytes < way.bytes) return cudaErrorInvalidValue;
     char *ws = static_cast<char *>(workspace);
     QuantMatmulProblem q = given;
+    // A caller's limit may be short: nothing but the stream orders another block's record behind the clearing then.
+    const bool clear_status = q.opt.wait_limit_cycles <= 0;
+    if (!clear_status && !way.grouped) {
+        const cudaError_t e = cudaMemsetAsync(ws, 0, 16, stream);
+        if (e != cudaSuccess) return e;
+    }
     // a single row may name any distance to the next one
     if (q.m == 1) q.ld_x = (int64_t)round16(q.k);
     if (weight_rows(q) == 1) q.ld_w = (int64_t)round16(weight_width(q));
@@ -695,6 +702,7 @@ cudaError_t quant_matmul_launch(const QuantMatmulProblem &given, void *workspace
     p.wait_limit = q.opt.wait_limit_cycles > 0 ? q.opt.wait_limit_cycles : kWaitLimitCycles;
     p.skip_blocks = q.opt.test_skip_k_blocks;
     p.status = reinterpret_cast<int *>(ws);
+    p.clear_status = clear_status;
     switch (q.y_dtype) {
         case kF32: return launch_typed<float>(q.w_nk, map_x, map_w, p, s, stream);
         case kF16: return launch_typed<__half>(q.w_nk, map_x, map_w, p, s, stream);

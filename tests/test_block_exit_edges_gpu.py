@@ -49,3 +49,28 @@ def test_balance_clusters_beside_other_work(rows, experts, sequences):
     assert b.isfinite().all()
     for again in got:
         assert all(torch.equal(x, y) for x, y in zip(again, first))
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# waits that run out
+# ---------------------------------------------------------------------------------------------------------------------
+
+def int8(shape, seed):
+    return torch.randint(-128, 128, shape, device=DEV, generator=gen(seed)).to(I8)
+
+
+@pytest.mark.parametrize("m,k,n", [(16, 4096, 2048), (256, 512, 18944), (3, 100, 77)])
+def test_matmul_records_of_limited_waits(m, k, n):
+    """A workspace that holds anything, a limit of the caller's: the record is that of this call, whatever order its CTAs come in."""
+    x, w, scale = int8((m, k), 1), int8((k, n), 2), torch.rand(n, device=DEV, generator=gen(3)) + 0.5
+    want, ws = ops.quant_matmul(x, w, scale, return_workspace=True)
+    for fill in (0, 1, 2, 255):
+        mine = torch.full((ws.numel(),), fill, dtype=torch.uint8, device=DEV)
+        ops.quant_matmul(x, w, scale, workspace=mine, options=ops.LaunchOptions(wait_limit_cycles=2_000_000, test_skip_k_blocks=1))
+        with pytest.raises(ops.AclnnError) as info:
+            ops.check_status(mine)
+        code, cta, role, parity = info.value.record
+        assert code == 1 and cta >= 0 and 200 <= role < 500 and parity in (0, 1)
+        got = ops.quant_matmul(x, w, scale, workspace=mine, options=ops.LaunchOptions(wait_limit_cycles=1 << 31))
+        ops.check_status(mine)
+        assert torch.equal(got, want)
