@@ -105,6 +105,12 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volati
 {
     return mbar_try<CLUSTER>(bar, parity) || mbar_wait_slow<CLUSTER>(bar, parity, gave_up, p, role);
 }
+// Behind a wait that ran out: what is under way has to land before this CTA's memory is another's.
+__device__ __forceinline__ void drain(uint64_t *bar, uint32_t parity)
+{
+    const long long begin = clock64();
+    while (!mbar_try(bar, parity) && clock64() - begin < kDrainLimitCycles) {}
+}
 // One lane of a converged warp: copies and MMAs issued under this predicate cost a few cycles each, in a branch that one thread enters 150.
 __device__ __forceinline__ bool elect_one()
 {
@@ -225,6 +231,7 @@ __global__ void __launch_bounds__(kThreads) quant_matmul_kernel(const __grid_con
     while (cols < (uint32_t)p.tile_tokens) cols *= 2;
     const uint32_t stage_bytes = kWeightStage + (uint32_t)p.tile_tokens * kBlockK;
     const int copies = max(kb1 - kb0 - p.skip_blocks, 0);
+    int issued = min(copies, p.stages);        // by warp 0
     const auto copy_block = [&](int i, int stage) {
         const uint32_t s = smem0 + (uint32_t)stage * stage_bytes;
         mbar_arrive_expect_tx(&full[stage], stage_bytes);
@@ -250,7 +257,7 @@ __global__ void __launch_bounds__(kThreads) quant_matmul_kernel(const __grid_con
         // the ring is filled before anything else: what follows runs beside the copies' way
         __syncwarp();
         const bool leader = elect_one();
-        for (int i = 0; i < min(copies, p.stages); ++i) {
+        for (int i = 0; i < issued; ++i) {
             if (leader) copy_block(i, i);
             __syncwarp();
         }
@@ -282,9 +289,9 @@ __global__ void __launch_bounds__(kThreads) quant_matmul_kernel(const __grid_con
         const bool leader = elect_one();
         int stage = 0;
         uint32_t phase = 0;
-        for (int i = p.stages; i < copies; ++i) {
+        for (; issued < copies; ++issued) {
             if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase, &gave_up, p, 100 + stage))) break;
-            if (leader) copy_block(i, stage);
+            if (leader) copy_block(issued, stage);
             __syncwarp();
             if (++stage == p.stages) { stage = 0; phase ^= 1u; }
         }
@@ -312,12 +319,8 @@ __global__ void __launch_bounds__(kThreads) quant_matmul_kernel(const __grid_con
             __syncwarp();
             if (++stage == p.stages) { stage = 0; phase ^= 1u; }
         }
-        if (!ok) {   // the MMAs that were issued write to TMEM, which this warp gives back
-            if (leader) umma_commit(&done);
-            __syncwarp();
-            const long long begin = clock64();
-            while (!mbar_try(&done, 0) && clock64() - begin < kDrainLimitCycles) {}
-        }
+        if (!ok && leader) umma_commit(&done);   // of the MMAs that were issued
+        __syncwarp();
     }
     if (warp >= 4) {
         scales[tid - 128] = mine[0];
@@ -328,7 +331,8 @@ __global__ void __launch_bounds__(kThreads) quant_matmul_kernel(const __grid_con
     // The sums: TMEM lane = channel, column = token.  They go into shared memory by rows, at the ring's place (every copy has been read by an
     // MMA and every MMA is done), and those that another CTA finishes from there in one piece; few go straight to it instead.
     const int quarter = warp & 3, half = warp >> 2;
-    bool ok = __all_sync(0xffffffffu, mbar_wait(&done, 0, &gave_up, p, 300 + warp));
+    bool ok = __all_sync(0xffffffffu, mbar_wait(&done, 0, &gave_up, p, 300 + warp) && !*(volatile int *)&gave_up);
+    if (!ok) drain(&done, 0);   // MMAs write to TMEM, which is given back below, and read the ring
     tc_fence_after();
     const uint32_t piece = (uint32_t)per * kTokenBytes, parts = smem0 + p.parts_at;
     if (p.apart) cluster_wait();
@@ -373,7 +377,10 @@ __global__ void __launch_bounds__(kThreads) quant_matmul_kernel(const __grid_con
                 __syncwarp();
             }
         }
-        ok = __all_sync(0xffffffffu, mbar_wait<true>(&received, 0, &gave_up, p, 400 + warp));
+        const bool all = __all_sync(0xffffffffu, mbar_wait<true>(&received, 0, &gave_up, p, 400 + warp));
+        if (!all) drain(&received, 0);
+        ok = ok && all;
+        __syncwarp();
         cluster_arrive();
     }
     // A warp takes a token, a lane four channels: neighbours that are stored at once, or where rows of y are on no such boundary every 32nd.
@@ -428,12 +435,10 @@ __global__ void __launch_bounds__(kThreads) quant_matmul_kernel(const __grid_con
     else finish(Int<4>(), Flag<true>());
     // A wait that ran out may have left copies in flight, which must not land in shared memory that is no longer this CTA's.
     if (warp == 0 && *(volatile int *)&gave_up) {
-        for (int i = max(copies - p.stages, 0); i < copies; ++i) {
-            const long long begin = clock64();
-            while (!mbar_try(&full[i % p.stages], (uint32_t)(i / p.stages) & 1u) && clock64() - begin < kDrainLimitCycles) {}
-        }
+        for (int i = max(issued - p.stages, 0); i < issued; ++i) drain(&full[i % p.stages], (uint32_t)(i / p.stages) & 1u);
     }
     // No CTA leaves before all of them have received, and so before what it has sent is read.
+    __syncwarp();
     if (p.split > 1) cluster_wait();
 }
 

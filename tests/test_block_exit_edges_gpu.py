@@ -74,3 +74,33 @@ def test_matmul_records_of_limited_waits(m, k, n):
         got = ops.quant_matmul(x, w, scale, workspace=mine, options=ops.LaunchOptions(wait_limit_cycles=1 << 31))
         ops.check_status(mine)
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("m,k,n,nk", [(16, 7168, 4096, True), (64, 4096, 512, False), (256, 7168, 1024, True), (300, 1000, 640, False), (5, 128, 100, True)])
+def test_matmul_leaves_nothing_under_way_when_a_wait_runs_out(m, k, n, nk):
+    """Waits that give up while copies, products and sums of other CTAs are still on their way: the kernel ends only when these have landed, and what
+    runs next, in the same places of the GPU, is right.  With K blocks left out the call says that it failed; rows that it does not finish stay."""
+    x, scale, token = int8((m, k), 1), torch.rand(n, device=DEV, generator=gen(3)) + 0.5, torch.rand(m, device=DEV, generator=gen(4)) + 0.5
+    w = int8((n, k), 2).t() if nk else int8((k, n), 2)
+    want = (x.double() @ w.double()).float() * scale * token[:, None]
+    got, ws = ops.quant_matmul(x, w, scale, token, out_dtype=F32, return_workspace=True)
+    ops.check_status(ws)
+    assert torch.equal(got, want)
+    mine = torch.zeros(ws.numel(), dtype=torch.uint8, device=DEV)
+    for limit in (100, 1000, 3000, 10_000, 100_000):
+        for skip in (0, 1):
+            room = torch.full((m, n), 7.0, device=DEV)
+            ops.quant_matmul(x, w, scale, token, out=room, workspace=mine, options=ops.LaunchOptions(wait_limit_cycles=limit, test_skip_k_blocks=skip))
+            again = [ops.quant_matmul(x, w, scale, token, out_dtype=F32) for _ in range(3)]
+            assert all(torch.equal(a, want) for a in again)
+            if skip:
+                with pytest.raises(ops.AclnnError) as info:
+                    ops.check_status(mine)
+                assert info.value.record[0] == 1
+                assert (room == 7).all()   # every CTA misses a block of its own
+            else:
+                try:
+                    ops.check_status(mine)
+                except ops.AclnnError:
+                    continue
+                assert torch.equal(room, want)
