@@ -42,8 +42,9 @@ ACL_FUNC_VISIBILITY aclnnStatus gmmB200CheckStatus(const void *workspace, uint64
  *   testSkipKBlocks  test only: the copy-issuing warp leaves this many K blocks out of its last tile, so that the bounded wait
  *                    of the warp that consumes them runs out and the abort path (status record, clean exit) can be exercised
  *                    without touching memory the call does not own.  Results are then undefined.  0 = off.
- * gmmB200AdapterAdd takes waitLimitCycles and testSkipKBlocks (of its first product; its kernels for a few tokens have no waits); the
- * operators without waits on the device take none. */
+ * gmmB200AdapterAdd takes waitLimitCycles and testSkipKBlocks (of its first product; its kernels for a few tokens have no waits),
+ * gmmB200SandwichNormQuant waitLimitCycles and testSkipKBlocks (as many rows at the end that are not fetched; its kernel for many rows
+ * alone has waits); the operators without waits on the device take none. */
 typedef struct gmmB200LaunchOptions {
     uint32_t structSize;
     int32_t maxCtas;
@@ -227,7 +228,9 @@ ACL_FUNC_VISIBILITY aclnnStatus gmmB200QuantMatmul(void *workspace, uint64_t wor
  *   q                 int8 [rows, h], optional, together with scale  fp32 [rows]
  *   residualOut, normedOut   [rows, h] residual's type, each optional; one of q, residualOut and normedOut is needed.  residualOut may be
  *                     residual, or x where that has its type; normedOut may be x if residualOut is not
- *   residualScale, blockScale finite; eps, postEps positive and finite */
+ *   residualScale, blockScale finite; eps, postEps positive and finite
+ * Calls of many rows wait on the device for copies.  Rows whose copies have not come when a wait runs out are NaN (int8 rows 0 with a scale of
+ * NaN), and gmmB200CheckStatus reports it, as for the other operators; gmmB200LaunchOptions: waitLimitCycles. */
 ACL_FUNC_VISIBILITY aclnnStatus gmmB200SandwichNormQuantGetWorkspaceSize(
     const aclTensor *x, const aclTensor *residual, const aclTensor *gammaOptional, const aclTensor *postGammaOptional,
     const aclTensor *gateOptional, const aclTensor *smoothOptional, int64_t gateAct, float residualScale, float blockScale, float eps,

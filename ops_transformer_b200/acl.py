@@ -442,7 +442,7 @@ def _float_bits(v: float) -> int:
 
 
 _current_device, _raw_stream = (getattr(torch._C, name, None) for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"))
-_POOLED = frozenset((_lib.OP_ADAPTER_ADD, _lib.OP_QUANT_MATMUL, _lib.OP_EXPERT_BALANCE))
+_POOLED = frozenset((_lib.OP_ADAPTER_ADD, _lib.OP_QUANT_MATMUL, _lib.OP_SANDWICH_NORM_QUANT, _lib.OP_EXPERT_BALANCE))
 
 
 def _block_call(op: int, name: str, workspace: Optional[torch.Tensor], stream, options: Optional[LaunchOptions], kinds: str,
@@ -621,19 +621,22 @@ def sandwich_norm_quant(x: torch.Tensor, residual: torch.Tensor, gamma: Optional
                         residual_scale: float = 1.0, block_scale: float = 1.0, smooth: Optional[torch.Tensor] = None, eps: float = 1e-6,
                         post_eps: Optional[float] = None, quant: bool = True, normed: bool = False, q: Optional[torch.Tensor] = None,
                         scale: Optional[torch.Tensor] = None, residual_out: Optional[torch.Tensor] = None,
-                        normed_out: Optional[torch.Tensor] = None, stream=None, workspace: Optional[torch.Tensor] = None):
+                        normed_out: Optional[torch.Tensor] = None, stream=None, workspace: Optional[torch.Tensor] = None,
+                        return_workspace: bool = False, options: Optional[LaunchOptions] = None):
     """(q int8 [rows, h], scale fp32 [rows], residual_out, normed_out): the way from a block's output ``x`` into the next block.  The residual
     stream ``s = residual_scale * residual + block_scale * act(gate) * n`` with the block's output behind its norm, ``n = rms_norm(x) *
     post_gamma`` (x itself without ``post_gamma``), and the norm of s with ``gamma`` in 8 bits with per-token scales (None without ``quant``)
     and, with ``normed`` or a ``normed_out`` to write to, in residual's type.  ``x`` has residual's type or is fp32; ``gate`` is one for each
     channel [h], each token [rows, 1] or each element, and goes through ``gate_act`` ("none", "sigmoid", "tanh"); ``smooth`` (fp32 [h])
     multiplies what is quantised, not ``normed_out``; ``post_eps`` is ``eps`` unless given.  ``residual_out`` may be ``residual``.
-    gmmB200SandwichNormQuant (include/gmm_b200.h) has the formulas."""
+    With ``return_workspace`` the workspace follows, for ``check_status`` (no rows: None); ``options``: per-call
+    ``LaunchOptions`` (wait bound).  gmmB200SandwichNormQuant (include/gmm_b200.h) has the formulas."""
     if stream is not None:   # what a call returns belongs to the stream that writes it
         with _on_stream(stream, x.device):
             return sandwich_norm_quant(x, residual, gamma, post_gamma=post_gamma, gate=gate, gate_act=gate_act, residual_scale=residual_scale,
                                        block_scale=block_scale, smooth=smooth, eps=eps, post_eps=post_eps, quant=quant, normed=normed, q=q,
-                                       scale=scale, residual_out=residual_out, normed_out=normed_out, workspace=workspace)
+                                       scale=scale, residual_out=residual_out, normed_out=normed_out, workspace=workspace,
+                                       return_workspace=return_workspace, options=options)
     if gate_act not in _GATE_ACT:
         raise ValueError(f"unknown gate_act {gate_act!r}")
     empty = _lib.native()[0].empty
@@ -647,9 +650,11 @@ def sandwich_norm_quant(x: torch.Tensor, residual: torch.Tensor, gamma: Optional
     if normed_out is None and normed:
         normed_out = empty(residual, "=")
     eps = _float_bits(eps)
-    _block_call(_lib.OP_SANDWICH_NORM_QUANT, "gmmB200SandwichNormQuant", workspace, None, None, "ttttttttttiiiii", x, residual, gamma, post_gamma,
-                gate, smooth, q, scale, residual_out, normed_out, _GATE_ACT[gate_act], _float_bits(residual_scale), _float_bits(block_scale), eps,
-                eps if post_eps is None else _float_bits(post_eps))
+    workspace = _block_call(_lib.OP_SANDWICH_NORM_QUANT, "gmmB200SandwichNormQuant", workspace, None, options, "ttttttttttiiiii", x, residual, gamma,
+                            post_gamma, gate, smooth, q, scale, residual_out, normed_out, _GATE_ACT[gate_act], _float_bits(residual_scale),
+                            _float_bits(block_scale), eps, eps if post_eps is None else _float_bits(post_eps))
+    if return_workspace:
+        return q, scale, residual_out, normed_out, workspace if residual.shape[0] else None
     return q, scale, residual_out, normed_out
 
 

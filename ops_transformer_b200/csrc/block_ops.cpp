@@ -346,6 +346,7 @@ aclnnStatus sandwich_phase1(const aclTensor *x, const aclTensor *residual, const
         p.gate_act = (int)gateAct;
         p.residual_scale = residualScale; p.block_scale = blockScale; p.eps = eps; p.post_eps = postEps;
         e->kind = aclOpExecutor::kSandwichNorm;
+        e->plan.ws_bytes = kSandwichNormWorkspace;
     }
     return ne.hand_out(workspaceSize, executor);
 }

@@ -201,8 +201,10 @@ struct SandwichNormProblem {
     int dtype = kBF16, x_dtype = kF32, gamma_dtype = kBF16;
     int gate_act = kGateNone;
     float residual_scale = 1.0f, block_scale = 1.0f, eps = 0.0f, post_eps = 0.0f;
+    LaunchOptions opt;                      // wait limit; test_skip_k_blocks: rows at the end whose copies are left out
 };
-cudaError_t sandwich_norm_launch(const SandwichNormProblem &p, cudaStream_t stream);
+constexpr size_t kSandwichNormWorkspace = 256;   // the status record
+cudaError_t sandwich_norm_launch(const SandwichNormProblem &p, void *workspace, size_t workspace_bytes, cudaStream_t stream);
 
 // expert_balance and its gradient (expert_balance.cu).
 struct BalanceProblem {

@@ -113,7 +113,7 @@ aclnnStatus run_executor(const char *op_name, void *workspace, uint64_t workspac
                 case aclOpExecutor::kRouteTopK: ce = route_top_k_launch(executor->route, cs); break;
                 case aclOpExecutor::kAdapterAdd: executor->adapter.opt = executor->problem.opt; ce = adapter_launch(executor->adapter, workspace, executor->plan.ws_bytes, cs); break;
                 case aclOpExecutor::kQuantMatmul: executor->matmul.opt = executor->problem.opt; ce = quant_matmul_launch(executor->matmul, workspace, executor->plan.ws_bytes, cs); break;
-                case aclOpExecutor::kSandwichNorm: ce = sandwich_norm_launch(executor->sandwich, cs); break;
+                case aclOpExecutor::kSandwichNorm: executor->sandwich.opt = executor->problem.opt; ce = sandwich_norm_launch(executor->sandwich, workspace, executor->plan.ws_bytes, cs); break;
                 case aclOpExecutor::kBalance: ce = balance_launch(executor->balance, workspace, executor->plan.ws_bytes, cs); break;
                 case aclOpExecutor::kBalanceGrad: ce = balance_grad_launch(executor->balance, cs); break;
                 default: ce = launch(executor->problem, executor->plan, workspace, executor->plan.ws_bytes, cs);

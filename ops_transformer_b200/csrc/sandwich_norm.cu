@@ -25,6 +25,11 @@ struct SandwichParams {
     int rows, h, gate_step, gate_act;
     bool gamma32;
     float inv_h, residual_scale, block_scale, eps, post_eps;
+    // of the kernel with waits
+    int fetched;                // rows whose copies are made: all but in a test
+    bool clear_status;          // else it has been, before the launch
+    long long wait_limit;
+    int *status;
 };
 
 // The division's error is within 2 units, expf's within 1, and an exponential that overflows gives 0.
@@ -40,6 +45,12 @@ __device__ __forceinline__ float load_gamma(const void *g, bool f32, int e)
     return f32 ? static_cast<const float *>(g)[e] : to_float<T>(static_cast<const T *>(g)[e]);
 }
 
+// The status record, by a call's first block.  That is among the first to start, and a wait of the default limit runs out about a second after.
+__device__ __forceinline__ void clear_status(const SandwichParams &p)
+{
+    if (p.clear_status && blockIdx.x == 0 && threadIdx.x < 4) p.status[threadIdx.x] = 0;
+}
+
 // Any strides, addresses and lengths: one element at a time, the inputs read anew in each of up to three passes.  Every thread stores only
 // elements that it alone reads, behind its last look at them, so that outputs may be inputs.
 template <typename T, typename X>
@@ -48,6 +59,7 @@ __global__ void __launch_bounds__(256) sandwich_any_kernel(const SandwichParams 
     __shared__ float2 red[2][32];
     dependent_wait();
     dependent_release();
+    clear_status(p);
     const long long row = blockIdx.x;
     const X *x = static_cast<const X *>(p.x) + row * p.ld_x;
     const T *residual = static_cast<const T *>(p.residual) + row * p.ld_residual, *gate = static_cast<const T *>(p.gate) + row * p.ld_gate;
@@ -104,6 +116,7 @@ __global__ void __launch_bounds__(1024, 1) sandwich_any_few_kernel(const Sandwic
     __shared__ float2 red[2][32];
     dependent_wait();
     dependent_release();
+    clear_status(p);
     const long long row = blockIdx.x;
     const int threads = blockDim.x;
     const X *x = static_cast<const X *>(p.x) + row * p.ld_x;
@@ -225,6 +238,7 @@ __global__ void __launch_bounds__(MAXT, MINB) sandwich_kernel(const SandwichPara
     __shared__ float2 red[2][32];
     dependent_wait();
     dependent_release();
+    clear_status(p);
     const int threads = blockDim.x;
     const bool rows_gate = p.gate && p.ld_gate != 0 && p.gate_step != 0;
     const long long row = blockIdx.x;
@@ -397,7 +411,7 @@ __global__ void __launch_bounds__(MAXT, MINB) sandwich_kernel(const SandwichPara
 // 4096 x 7168, fp32 x, bf16 stream: 53.3 us with int8 rows (270 MB, 5.1 TB/s), 49.0 with bf16 rows and a gate (294 MB, 6.0 TB/s); 5001
 // channels, whose rows begin anywhere, 52.7.  Quantising costs what the difference is: max, step and rounding are the issue slots' work.
 constexpr int kGroupPacks = 2, kMaxGroups = 14, kMaxDepth = 3;    // of the 15 named barriers that are left
-constexpr long long kWaitLimitCycles = 1ll << 31;  // about a second
+constexpr long long kWaitLimitCycles = 1ll << 31, kDrainLimitCycles = 1ll << 24;   // about a second, a few milliseconds
 constexpr int kGroupThreads = 1024;
 // Packs that a row can touch, and floats of a vector of factors.
 template <int V, bool WHOLE> __host__ __device__ inline int most_packs(int h) { return WHOLE ? h / V : (h + 2 * V - 2) / V; }
@@ -418,14 +432,27 @@ __device__ __forceinline__ bool mbar_try(uint64_t *bar, uint32_t parity)
         : "memory");
     return ok;
 }
-// Bounded: false when the copies have not come, and once that has been so, without waiting a second time.
-__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volatile int *late)
+// Bounded: false when the copies have not come, which the status says, or when another wait of the CTA has run out.
+__device__ __noinline__ bool mbar_wait_slow(uint64_t *bar, uint32_t parity, volatile int *late, int *status, long long limit, int role)
 {
-    if (mbar_try(bar, parity)) return true;
-    for (const long long t0 = clock64(); !*late && clock64() - t0 <= kWaitLimitCycles;)
-        if (mbar_try(bar, parity)) return true;
-    *late = 1;
-    return false;
+    const long long t0 = clock64();
+    while (!mbar_try(bar, parity)) {
+        if (*late) return false;
+        if (clock64() - t0 > limit) {
+            *late = 1;
+            if (atomicCAS(status, kStatusOk, kStatusWaitTimeout) == kStatusOk) {
+                status[1] = (int)blockIdx.x;
+                status[2] = role;
+                status[3] = (int)parity;
+            }
+            return false;
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volatile int *late, const SandwichParams &p, int role)
+{
+    return mbar_try(bar, parity) || mbar_wait_slow(bar, parity, late, p.status, p.wait_limit, role);
 }
 __device__ __forceinline__ void bulk_copy(void *to, const void *from, uint32_t bytes, uint64_t *bar)
 {
@@ -464,7 +491,8 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
     extern __shared__ uint4 smem[];     // the groups' rows (x, residual, gate); block's, next norm's and smoothing's factors
     __shared__ float2 red[4][32];
     __shared__ alignas(8) uint64_t x_landed[kMaxGroups][kMaxDepth], rest_landed[kMaxGroups][kMaxDepth];
-    __shared__ volatile int late;   // a wait has run out, which none does while the GPU is well: what there is to see of it are rows of NaN
+    __shared__ volatile int late;   // a wait has run out: from then on nothing is fetched, and what has not come is NaN
+    __shared__ int issued[2][kMaxGroups];   // x and the rest, by a group's first thread
     const float nan = __int_as_float(0x7fffffff);
     if (threadIdx.x == 0) late = 0;
     const bool channel_gate = !GATED && p.gate && p.gate_step != 0;
@@ -484,10 +512,12 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(all) : "memory");
     };
     const auto fetch_x = [&](long long row, int at) {
+        ++issued[0][group];
         expect(&x_landed[group][at], row, sizeof(X), 1);
         fetch(static_cast<const X *>(p.x), row, p.ld_x, all + at * row_packs, &x_landed[group][at]);
     };
     const auto fetch_rest = [&](long long row, int at) {
+        ++issued[1][group];
         uint4 *to = all + at * row_packs + most * XW;
         expect(&rest_landed[group][at], row, sizeof(T), GATED ? 2 : 1);
         fetch(static_cast<const T *>(p.residual), row, p.ld_residual, to, &rest_landed[group][at]);
@@ -496,6 +526,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
     const long long step = (long long)gridDim.x * groups;
     long long row = (long long)blockIdx.x * groups + group;
     if (tid == 0) {
+        issued[0][group] = issued[1][group] = 0;
         for (int d = 0; d < depth; ++d) {
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&x_landed[group][d])) : "memory");
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&rest_landed[group][d])) : "memory");
@@ -504,8 +535,9 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
     }
     dependent_wait();
     dependent_release();
+    clear_status(p);
     if (tid == 0) {
-        for (int d = 0; d < depth && row + d * step < p.rows; ++d) {
+        for (int d = 0; d < depth && row + d * step < p.fetched; ++d) {
             fetch_x(row + d * step, d);
             fetch_rest(row + d * step, d);
         }
@@ -552,6 +584,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
     __syncthreads();
     uint32_t phase = 0;
     int at = 0;     // the buffer that the row is in
+    bool gone = false;      // for good: behind a row that was not fetched a barrier's parity says nothing
     for (int parity = 0; row < p.rows; row += step, parity ^= 1) {
         const long long next = row + depth * step;   // what comes in its place
         const uint4 *mine = all + at * row_packs;
@@ -589,7 +622,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
 
         // the block's output, and the norm behind it
         f32x2 u[N][V / 2];
-        const bool x_here = mbar_wait(&x_landed[group][at], phase, &late);
+        gone = gone || !mbar_wait(&x_landed[group][at], phase, &late, p, 1000);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = tid + i * threads;
@@ -597,7 +630,13 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
             for (int j = 0; j < XW; ++j) unpack<X>(has(i) ? mine[c * XW + j] : make_uint4(0, 0, 0, 0), u[i] + j * (V / 2 / XW));
             if (has(i)) mask(c, u[i]);
         }
-        if (!x_here) u[0][0] = pair2(nan, nan);
+        const auto spoil = [&] {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) u[i][e] = pair2(nan, nan);
+        };
+        if (gone) spoil();
         float factor = 1.0f;
         if (p.post_gamma) {
             f32x2 sum2 = 0;
@@ -612,11 +651,11 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
         } else {
             group_sync(group, threads);
         }
-        if (tid == 0 && next < p.rows && !late) fetch_x(next, at);
+        if (tid == 0 && next < p.fetched && !late) fetch_x(next, at);
         if (p.gate && p.gate_step == 0) factor = __fmul_rn(factor, gate_value(to_float<T>(static_cast<const T *>(p.gate)[row * p.ld_gate]), p.gate_act));
 
         // the residual stream, and the sums of the next norm
-        const bool rest_here = mbar_wait(&rest_landed[group][at], phase, &late);
+        gone = gone || !mbar_wait(&rest_landed[group][at], phase, &late, p, 1001);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             if (!has(i)) break;
@@ -642,7 +681,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
             for (int e = 0; e < V / 2; ++e) u[i][e] = fma2(r[e], pair2(p.residual_scale, p.residual_scale), u[i][e]);
             mask(c, u[i]);
         }
-        if (!rest_here) u[0][0] = pair2(nan, nan);
+        if (gone) spoil();
         if (p.residual_out) {
 #pragma unroll
             for (int i = 0; i < N; ++i)
@@ -680,7 +719,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
         float sum = parts.x + parts.y;
         if (p.gamma) group_reduce(sum, mag, red[2 + parity], group, threads);
         else group_sync(group, threads);
-        if (tid == 0 && next < p.rows && !late) fetch_rest(next, at);
+        if (tid == 0 && next < p.fetched && !late) fetch_rest(next, at);
         if (++at == depth) { at = 0; phase ^= 1; }
         if (!p.gamma) continue;
         const float r = rsqrtf(__fmaf_rn(sum, p.inv_h, p.eps));
@@ -726,6 +765,15 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
         };
         if (quant.rcp != 0.0f) finish(true);
         else finish(false);
+    }
+    // Copies that were not waited for must not land in shared memory that is no longer this CTA's.
+    if (tid == 0 && late) {
+        const auto drain = [&](uint64_t *bars, int n) {
+            for (int i = max(n - depth, 0); i < n; ++i)
+                for (const long long t0 = clock64(); !mbar_try(bars + i % depth, (uint32_t)(i / depth) & 1u) && clock64() - t0 < kDrainLimitCycles;) {}
+        };
+        drain(x_landed[group], issued[0][group]);
+        drain(rest_landed[group], issued[1][group]);
     }
 }
 
@@ -822,9 +870,10 @@ cudaError_t launch_typed(const SandwichParams &p, cudaStream_t stream)
 
 }  // namespace
 
-cudaError_t sandwich_norm_launch(const SandwichNormProblem &n, cudaStream_t stream)
+cudaError_t sandwich_norm_launch(const SandwichNormProblem &n, void *workspace, size_t workspace_bytes, cudaStream_t stream)
 {
     if (n.rows <= 0) return cudaSuccess;
+    if (!workspace || workspace_bytes < kSandwichNormWorkspace) return cudaErrorInvalidValue;
     SandwichParams p;
     p.x = n.x; p.residual = n.residual; p.gamma = n.gamma; p.post_gamma = n.post_gamma; p.gate = n.gate; p.smooth = n.smooth;
     p.q = n.q; p.scale = n.scale; p.residual_out = n.residual_out; p.normed_out = n.normed_out;
@@ -833,6 +882,15 @@ cudaError_t sandwich_norm_launch(const SandwichNormProblem &n, cudaStream_t stre
     p.rows = (int)n.rows; p.h = (int)n.h; p.gate_step = n.gate_step; p.gate_act = n.gate_act;
     p.gamma32 = n.gamma_dtype == kF32;
     p.inv_h = 1.0f / (float)n.h; p.residual_scale = n.residual_scale; p.block_scale = n.block_scale; p.eps = n.eps; p.post_eps = n.post_eps;
+    p.status = static_cast<int *>(workspace);
+    p.wait_limit = n.opt.wait_limit_cycles > 0 ? n.opt.wait_limit_cycles : kWaitLimitCycles;
+    p.fetched = p.rows > n.opt.test_skip_k_blocks ? p.rows - n.opt.test_skip_k_blocks : 0;
+    // A caller's limit may be short: nothing but the stream orders another block's record behind the clearing then.
+    p.clear_status = n.opt.wait_limit_cycles <= 0;
+    if (!p.clear_status) {
+        const cudaError_t e = cudaMemsetAsync(workspace, 0, 16, stream);
+        if (e != cudaSuccess) return e;
+    }
     switch (n.dtype) {
         case kF32: return launch_typed<float, float>(p, stream);
         case kF16: return n.x_dtype == kF32 ? launch_typed<__half, float>(p, stream) : launch_typed<__half, __half>(p, stream);

@@ -104,3 +104,113 @@ def test_matmul_leaves_nothing_under_way_when_a_wait_runs_out(m, k, n, nk):
                 except ops.AclnnError:
                     continue
                 assert torch.equal(room, want)
+
+
+def sandwich_inputs(rows, h, x_dtype=F32, dtype=BF16):
+    return dict(x=randn((rows, h), 1, x_dtype, 3.0), residual=randn((rows, h), 2, dtype), gamma=randn((h,), 3, dtype, 0.2) + 1)
+
+
+def right_or_nan(got, want):
+    """Whether every element is the right one, or NaN."""
+    return ((got == want) | got.isnan()).all()
+
+
+SANDWICH_WAITS = [(4096, 7168, F32, BF16, dict(post_gamma=True, gate="channel", normed=True)), (3000, 5001, F32, F16, dict(post_gamma=True, normed=True)),
+                  (4000, 2100, BF16, BF16, dict(gate="full", normed=True)), (600, 9000, F32, F32, dict(post_gamma=True, gate="token")),
+                  (600, 7000, F32, F32, dict(post_gamma=True, gate="token")),
+                  (2500, 7168, F16, F16, dict(post_gamma=True, smooth=True)), (2000, 6000, F32, BF16, dict(stream_only=True)),
+                  (2000, 6001, BF16, BF16, dict(stream_only=True, post_gamma=True))]
+
+
+def in_turn(h, dtype):
+    """Whether rows of that length fit a group of threads with two packs each, as the kernel with waits takes them: up to 1024 threads.  (9000 values
+    of fp32 are 2250 packs, for 1125.)"""
+    v = 16 // dtype.itemsize
+    packs = h // v if h % v == 0 else (h + 2 * v - 2) // v
+    return (packs + 1) // 2 <= 1024
+
+
+def sandwich_call(rows, h, x_dtype, dtype, how):
+    t = sandwich_inputs(rows, h, x_dtype, dtype)
+    kw = dict(normed=how.get("normed", False))
+    if how.get("post_gamma"):
+        kw["post_gamma"] = randn((h,), 4, dtype, 0.2) + 0.7
+    if "gate" in how:
+        kw["gate"] = randn({"channel": (h,), "token": (rows, 1), "full": (rows, h)}[how["gate"]], 5, dtype)
+        kw["gate_act"] = "sigmoid"
+    if how.get("smooth"):
+        kw["smooth"] = torch.rand(h, device=DEV, generator=gen(6)) + 0.5
+    if how.get("stream_only"):
+        kw["quant"] = False
+        t["gamma"] = None
+    return lambda **more: ops.sandwich_norm_quant(**t, **kw, **more)
+
+
+@pytest.mark.parametrize("rows,h,x_dtype,dtype,how", SANDWICH_WAITS)
+def test_sandwich_reports_a_wait_that_runs_out(rows, h, x_dtype, dtype, how):
+    """Rows at the end are not fetched and waits last about 1 ms: the call ends, says so, and what it could not work on is NaN through and through;
+    the next one on the same workspace is right."""
+    call = sandwich_call(rows, h, x_dtype, dtype, how)
+    want = call()
+    for skip in (1, rows // 2, rows):
+        for fill in (0, 255):
+            mine = torch.full((256,), fill, dtype=torch.uint8, device=DEV)
+            *got, ws = call(workspace=mine, return_workspace=True, options=ops.LaunchOptions(wait_limit_cycles=2_000_000, test_skip_k_blocks=skip))
+            assert ws is mine
+            if not in_turn(h, dtype):
+                ops.check_status(mine)
+                assert all(a is b if a is None else torch.equal(a, b) for a, b in zip(got, want))
+                continue
+            with pytest.raises(ops.AclnnError) as info:
+                ops.check_status(mine)
+            code, cta, role, parity = info.value.record
+            assert code == 1 and 0 <= cta < 148 and role in (1000, 1001) and parity in (0, 1)
+            q, scale, stream, normed = got
+            lost = stream.isnan().all(1)
+            assert lost[rows - skip:].all() and torch.equal(stream[~lost], want[2][~lost])
+            if scale is not None:
+                assert scale[lost].isnan().all() and (q[lost] == 0).all()
+                assert torch.equal(scale[~lost], want[1][~lost]) and torch.equal(q[~lost], want[0][~lost])
+            if normed is not None:
+                assert normed[lost].isnan().all() and torch.equal(normed[~lost], want[3][~lost])
+            *again, ws = call(workspace=mine, return_workspace=True)
+            ops.check_status(ws)
+            assert all(a is b if a is None else torch.equal(a, b) for a, b in zip(again, want))
+
+
+@pytest.mark.parametrize("rows,h,x_dtype,dtype,how", SANDWICH_WAITS)
+def test_sandwich_leaves_nothing_under_way_when_a_wait_runs_out(rows, h, x_dtype, dtype, how):
+    """Waits that give up while rows are on their way: these land before the kernel ends, and what runs next in its place is right."""
+    call = sandwich_call(rows, h, x_dtype, dtype, how)
+    want = call()
+    mine = torch.empty(256, dtype=torch.uint8, device=DEV)
+    for limit in (100, 1000, 3000, 10_000, 100_000):
+        got = call(workspace=mine, options=ops.LaunchOptions(wait_limit_cycles=limit))
+        again = [call() for _ in range(2)]
+        for a in again:
+            assert all(x is y if x is None else torch.equal(x, y) for x, y in zip(a, want))
+        assert right_or_nan(got[2], want[2])
+        if got[3] is not None:
+            assert right_or_nan(got[3], want[3])
+        if got[1] is not None:
+            assert right_or_nan(got[1], want[1]) and ((got[0] == want[0]) | (got[0] == 0)).all()
+        try:
+            ops.check_status(mine)
+        except ops.AclnnError:
+            continue
+        assert all(x is y if x is None else torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_sandwich_status_of_calls_without_waits():
+    """Few rows and rows on no pack have kernels without waits, and a clean record."""
+    for rows, h, offset in ((1, 8, 0), (16, 2048, 0), (9, 40000, 0), (700, 1000, 1)):
+        t = sandwich_inputs(rows, h)
+        t["x"] = randn((rows * h + 8,), 7)[offset:offset + rows * h].view(rows, h)
+        for options in (None, ops.LaunchOptions(wait_limit_cycles=1000)):
+            mine = torch.full((256,), 255, dtype=torch.uint8, device=DEV)
+            *got, ws = ops.sandwich_norm_quant(**t, workspace=mine, return_workspace=True, options=options)
+            assert ws is mine
+            ops.check_status(ws)
+            assert all(a is b if a is None else torch.equal(a, b) for a, b in zip(got, ops.sandwich_norm_quant(**t)))
+    t = sandwich_inputs(0, 64)
+    assert ops.sandwich_norm_quant(**t, return_workspace=True)[4] is None
