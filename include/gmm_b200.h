@@ -44,7 +44,7 @@ ACL_FUNC_VISIBILITY aclnnStatus gmmB200CheckStatus(const void *workspace, uint64
  *                    without touching memory the call does not own.  Results are then undefined.  0 = off.
  * gmmB200AdapterAdd takes waitLimitCycles and testSkipKBlocks (of its first product; its kernels for a few tokens have no waits),
  * gmmB200SandwichNormQuant waitLimitCycles and testSkipKBlocks (as many rows at the end that are not fetched; its kernel for many rows
- * alone has waits); the operators without waits on the device take none. */
+ * alone has waits), gmmB200QuantMatmul all but maxCtas; the operators without waits on the device take none. */
 typedef struct gmmB200LaunchOptions {
     uint32_t structSize;
     int32_t maxCtas;
@@ -204,8 +204,8 @@ ACL_FUNC_VISIBILITY aclnnStatus gmmB200AdapterAdd(void *workspace, uint64_t work
  *   scale             fp32 / fp16 / bf16 [n];   perTokenScale  fp32 [m], optional (1 without it);   bias  fp32 / fp16 / bf16 [n], optional
  *   y                 fp32 / fp16 / bf16 [m, n]; shares no memory with the inputs
  * x, weight and y may be views whose rows (of a transposed view: columns) are dense.  Addresses and distances of rows that are multiples
- * of 16 bytes are read in place, others through a copy of the operand in the workspace.  gmmB200LaunchOptions: waitLimitCycles; a wait
- * that runs out is reported by gmmB200CheckStatus. */
+ * of 16 bytes are read in place, others through a copy of the operand in the workspace.  gmmB200LaunchOptions: waitLimitCycles, startEvent and
+ * stopEvent (around the product, not the copy); a wait that runs out is reported by gmmB200CheckStatus. */
 ACL_FUNC_VISIBILITY aclnnStatus gmmB200QuantMatmulGetWorkspaceSize(
     const aclTensor *x, const aclTensor *weight, const aclTensor *scale, const aclTensor *perTokenScaleOptional,
     const aclTensor *biasOptional, aclTensor *y, uint64_t *workspaceSize, aclOpExecutor **executor);

@@ -597,8 +597,8 @@ def quant_matmul(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, per
     """y [rows, n] = ((x @ weight) * scale) * per_token_scale + bias of int8 ``x`` [rows, k] and ``weight`` [k, n] (or the transposed view of
     one stored [n, k]), with one scale a channel and, where given, one a token: the W8A8 product without groups.  ``scale`` and ``bias`` [n]
     fp32 or 16-bit, ``per_token_scale`` fp32 [rows]; the result is ``out_dtype`` (bf16, fp16 or fp32) or ``out``.  With ``return_workspace``
-    (y, workspace), for ``check_status`` (no rows: None); ``options``: per-call ``LaunchOptions`` (wait bound).  gmmB200QuantMatmul
-    (include/gmm_b200.h)."""
+    (y, workspace), for ``check_status`` (no rows: None); ``options``: per-call ``LaunchOptions`` (wait bound, timing events).
+    gmmB200QuantMatmul (include/gmm_b200.h)."""
     if stream is not None:   # what a call returns belongs to the stream that writes it
         with _on_stream(stream, x.device):
             return quant_matmul(x, weight, scale, per_token_scale, bias=bias, out=out, out_dtype=out_dtype, workspace=workspace,

@@ -651,6 +651,7 @@ cudaError_t launch_grouped(const QuantMatmulProblem &q, char *ws, cudaStream_t s
     g.w_layout = q.w_nk ? 1 : 0;
     g.out_f16 = q.y_dtype == kF16; g.out0 = q.y;
     g.opt = q.opt;
+    g.opt.max_ctas = 0;   // which the kernels above could not follow
     Plan plan;
     make_plan(g, &plan);
     if (plan.path != kPathSm100 || plan.ws_bytes > 256) return cudaErrorInvalidValue;
@@ -708,11 +709,12 @@ cudaError_t quant_matmul_launch(const QuantMatmulProblem &given, void *workspace
     p.skip_blocks = q.opt.test_skip_k_blocks;
     p.status = reinterpret_cast<int *>(ws);
     p.clear_status = clear_status;
-    switch (q.y_dtype) {
-        case kF32: return launch_typed<float>(q.w_nk, map_x, map_w, p, s, stream);
-        case kF16: return launch_typed<__half>(q.w_nk, map_x, map_w, p, s, stream);
-        default: return launch_typed<__nv_bfloat16>(q.w_nk, map_x, map_w, p, s, stream);
-    }
+    if (q.opt.ev_start) cudaEventRecord(q.opt.ev_start, stream);
+    const cudaError_t e = q.y_dtype == kF32 ? launch_typed<float>(q.w_nk, map_x, map_w, p, s, stream)
+                        : q.y_dtype == kF16 ? launch_typed<__half>(q.w_nk, map_x, map_w, p, s, stream)
+                                            : launch_typed<__nv_bfloat16>(q.w_nk, map_x, map_w, p, s, stream);
+    if (q.opt.ev_stop) cudaEventRecord(q.opt.ev_stop, stream);
+    return e;
 }
 
 }  // namespace gmm

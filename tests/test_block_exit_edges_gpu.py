@@ -214,3 +214,27 @@ def test_sandwich_status_of_calls_without_waits():
             assert all(a is b if a is None else torch.equal(a, b) for a, b in zip(got, ops.sandwich_norm_quant(**t)))
     t = sandwich_inputs(0, 64)
     assert ops.sandwich_norm_quant(**t, return_workspace=True)[4] is None
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# launch options
+# ---------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("m,k,n", [(16, 768, 2048), (100, 1000, 640), (4096, 2048, 4096), (3000, 1001, 4096)])
+def test_matmul_options_do_not_hang_on_the_size(m, k, n):
+    """Events are recorded around the product whatever kernel takes the call, and a cap on the CTAs is followed by none."""
+    x, w, scale = int8((m, k), 1), int8((k, n), 2), torch.rand(n, device=DEV, generator=gen(3)) + 0.5
+    want = ops.quant_matmul(x, w, scale)
+    took = {}
+    for cap in (0, 2):
+        for _ in range(3):
+            start, stop = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            start.record()   # creates it; what the two say until they are recorded anew is about 10 ms
+            torch.cuda._sleep(20_000_000)
+            stop.record()
+            torch.cuda.synchronize()
+            got = ops.quant_matmul(x, w, scale, options=ops.LaunchOptions(max_ctas=cap, start_event=start.cuda_event, stop_event=stop.cuda_event))
+            stop.synchronize()
+            took[cap] = min(took.get(cap, 1e9), start.elapsed_time(stop))
+            assert torch.equal(got, want)
+    assert 0 < took[0] < 1 and took[2] < 4 * took[0] + 0.01   # two CTAs of 148 would take 70 times as long for the large ones
