@@ -46,9 +46,15 @@ __device__ __forceinline__ float load_gamma(const void *g, bool f32, int e)
 }
 
 // The status record, by a call's first block.  That is among the first to start, and a wait of the default limit runs out about a second after.
+// (A store under a predicate: behind a branch it costs the kernel of many rows registers, 4096 x 7168 54.4 us for 53.4.)
 __device__ __forceinline__ void clear_status(const SandwichParams &p)
 {
-    if (p.clear_status && blockIdx.x == 0 && threadIdx.x < 4) p.status[threadIdx.x] = 0;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.eq.u32 p, %1, 0;\n"
+        "@p st.global.v4.b32 [%0], {%2, %2, %2, %2};\n"
+        "}\n" ::"l"(p.status), "r"(blockIdx.x | threadIdx.x | !p.clear_status), "r"(0));
 }
 
 // Any strides, addresses and lengths: one element at a time, the inputs read anew in each of up to three passes.  Every thread stores only
@@ -59,7 +65,6 @@ __global__ void __launch_bounds__(256) sandwich_any_kernel(const SandwichParams 
     __shared__ float2 red[2][32];
     dependent_wait();
     dependent_release();
-    clear_status(p);
     const long long row = blockIdx.x;
     const X *x = static_cast<const X *>(p.x) + row * p.ld_x;
     const T *residual = static_cast<const T *>(p.residual) + row * p.ld_residual, *gate = static_cast<const T *>(p.gate) + row * p.ld_gate;
@@ -96,7 +101,10 @@ __global__ void __launch_bounds__(256) sandwich_any_kernel(const SandwichParams 
     }
     Quantiser quant;
     quant.set(step);
-    if (p.q && threadIdx.x == 0) p.scale[row] = step == 0.0f ? 0.0f : __fmul_rn(step, r);
+    if (threadIdx.x == 0) {
+        if (p.q) p.scale[row] = step == 0.0f ? 0.0f : __fmul_rn(step, r);
+        if (row == 0 && p.clear_status) *reinterpret_cast<int4 *>(p.status) = make_int4(0, 0, 0, 0);
+    }
     for (int e = threadIdx.x; e < p.h; e += 256) {
         const float s = stream_at(e);
         if (p.residual_out) static_cast<T *>(p.residual_out)[row * p.ld_residual_out + e] = from_float<T>(s);
@@ -411,7 +419,7 @@ __global__ void __launch_bounds__(MAXT, MINB) sandwich_kernel(const SandwichPara
 // 4096 x 7168, fp32 x, bf16 stream: 53.3 us with int8 rows (270 MB, 5.1 TB/s), 49.0 with bf16 rows and a gate (294 MB, 6.0 TB/s); 5001
 // channels, whose rows begin anywhere, 52.7.  Quantising costs what the difference is: max, step and rounding are the issue slots' work.
 constexpr int kGroupPacks = 2, kMaxGroups = 14, kMaxDepth = 3;    // of the 15 named barriers that are left
-constexpr long long kWaitLimitCycles = 1ll << 31, kDrainLimitCycles = 1ll << 24;   // about a second, a few milliseconds
+constexpr long long kWaitLimitCycles = 1ll << 31, kDrainLimitCycles = 1ll << 20;   // about a second, half a millisecond
 constexpr int kGroupThreads = 1024;
 // Packs that a row can touch, and floats of a vector of factors.
 template <int V, bool WHOLE> __host__ __device__ inline int most_packs(int h) { return WHOLE ? h / V : (h + 2 * V - 2) / V; }
@@ -432,27 +440,25 @@ __device__ __forceinline__ bool mbar_try(uint64_t *bar, uint32_t parity)
         : "memory");
     return ok;
 }
-// Bounded: false when the copies have not come, which the status says, or when another wait of the CTA has run out.
-__device__ __noinline__ bool mbar_wait_slow(uint64_t *bar, uint32_t parity, volatile int *late, int *status, long long limit, int role)
+// What a wait that has run out leaves behind.
+__device__ __noinline__ void gave_up(volatile int *late, int *status, int role, uint32_t parity)
 {
-    const long long t0 = clock64();
-    while (!mbar_try(bar, parity)) {
-        if (*late) return false;
-        if (clock64() - t0 > limit) {
-            *late = 1;
-            if (atomicCAS(status, kStatusOk, kStatusWaitTimeout) == kStatusOk) {
-                status[1] = (int)blockIdx.x;
-                status[2] = role;
-                status[3] = (int)parity;
-            }
-            return false;
-        }
+    *late = 1;
+    if (atomicCAS(status, kStatusOk, kStatusWaitTimeout) == kStatusOk) {
+        status[1] = (int)blockIdx.x;
+        status[2] = role;
+        status[3] = (int)parity;
     }
-    return true;
 }
+// Bounded: false when the copies have not come, which the status says, or when another wait of the CTA has run out.
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volatile int *late, const SandwichParams &p, int role)
 {
-    return mbar_try(bar, parity) || mbar_wait_slow(bar, parity, late, p.status, p.wait_limit, role);
+    if (mbar_try(bar, parity)) return true;
+    for (const long long t0 = clock64(); !*late;) {
+        if (mbar_try(bar, parity)) return true;
+        if (clock64() - t0 > p.wait_limit) gave_up(late, p.status, role, parity);
+    }
+    return false;
 }
 __device__ __forceinline__ void bulk_copy(void *to, const void *from, uint32_t bytes, uint64_t *bar)
 {
@@ -492,7 +498,6 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
     __shared__ float2 red[4][32];
     __shared__ alignas(8) uint64_t x_landed[kMaxGroups][kMaxDepth], rest_landed[kMaxGroups][kMaxDepth];
     __shared__ volatile int late;   // a wait has run out: from then on nothing is fetched, and what has not come is NaN
-    __shared__ int issued[2][kMaxGroups];   // x and the rest, by a group's first thread
     const float nan = __int_as_float(0x7fffffff);
     if (threadIdx.x == 0) late = 0;
     const bool channel_gate = !GATED && p.gate && p.gate_step != 0;
@@ -512,12 +517,10 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(all) : "memory");
     };
     const auto fetch_x = [&](long long row, int at) {
-        ++issued[0][group];
         expect(&x_landed[group][at], row, sizeof(X), 1);
         fetch(static_cast<const X *>(p.x), row, p.ld_x, all + at * row_packs, &x_landed[group][at]);
     };
     const auto fetch_rest = [&](long long row, int at) {
-        ++issued[1][group];
         uint4 *to = all + at * row_packs + most * XW;
         expect(&rest_landed[group][at], row, sizeof(T), GATED ? 2 : 1);
         fetch(static_cast<const T *>(p.residual), row, p.ld_residual, to, &rest_landed[group][at]);
@@ -526,7 +529,6 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
     const long long step = (long long)gridDim.x * groups;
     long long row = (long long)blockIdx.x * groups + group;
     if (tid == 0) {
-        issued[0][group] = issued[1][group] = 0;
         for (int d = 0; d < depth; ++d) {
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&x_landed[group][d])) : "memory");
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&rest_landed[group][d])) : "memory");
@@ -535,7 +537,6 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
     }
     dependent_wait();
     dependent_release();
-    clear_status(p);
     if (tid == 0) {
         for (int d = 0; d < depth && row + d * step < p.fetched; ++d) {
             fetch_x(row + d * step, d);
@@ -581,6 +582,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
         }
         place(by_block, c, post);
     }
+    clear_status(p);
     __syncthreads();
     uint32_t phase = 0;
     int at = 0;     // the buffer that the row is in
@@ -630,13 +632,6 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
             for (int j = 0; j < XW; ++j) unpack<X>(has(i) ? mine[c * XW + j] : make_uint4(0, 0, 0, 0), u[i] + j * (V / 2 / XW));
             if (has(i)) mask(c, u[i]);
         }
-        const auto spoil = [&] {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-#pragma unroll
-                for (int e = 0; e < V / 2; ++e) u[i][e] = pair2(nan, nan);
-        };
-        if (gone) spoil();
         float factor = 1.0f;
         if (p.post_gamma) {
             f32x2 sum2 = 0;
@@ -645,7 +640,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
 #pragma unroll
                 for (int e = 0; e < V / 2; ++e) sum2 = fma2(u[i][e], u[i][e], sum2);
             const float2 parts = unpair2(sum2);
-            float sum = parts.x + parts.y, unused = 0.0f;
+            float sum = gone ? nan : parts.x + parts.y, unused = 0.0f;
             group_reduce(sum, unused, red[parity], group, threads);
             factor = __fmul_rn(factor, rsqrtf(__fmaf_rn(sum, p.inv_h, p.post_eps)));
         } else {
@@ -656,6 +651,7 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
 
         // the residual stream, and the sums of the next norm
         gone = gone || !mbar_wait(&rest_landed[group][at], phase, &late, p, 1001);
+        if (gone) factor = nan;     // and so all that follows
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             if (!has(i)) break;
@@ -681,7 +677,6 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
             for (int e = 0; e < V / 2; ++e) u[i][e] = fma2(r[e], pair2(p.residual_scale, p.residual_scale), u[i][e]);
             mask(c, u[i]);
         }
-        if (gone) spoil();
         if (p.residual_out) {
 #pragma unroll
             for (int i = 0; i < N; ++i)
@@ -766,14 +761,13 @@ __global__ void __launch_bounds__(kGroupThreads, 1) sandwich_rows_kernel(const S
         if (quant.rcp != 0.0f) finish(true);
         else finish(false);
     }
-    // Copies that were not waited for must not land in shared memory that is no longer this CTA's.
+    // Copies that were not waited for must not land in shared memory that is no longer this CTA's.  One of a barrier's two parities is the past
+    // phase's, and no wait; the other one comes with the copies, or not at all where none are under way.
     if (tid == 0 && late) {
-        const auto drain = [&](uint64_t *bars, int n) {
-            for (int i = max(n - depth, 0); i < n; ++i)
-                for (const long long t0 = clock64(); !mbar_try(bars + i % depth, (uint32_t)(i / depth) & 1u) && clock64() - t0 < kDrainLimitCycles;) {}
-        };
-        drain(x_landed[group], issued[0][group]);
-        drain(rest_landed[group], issued[1][group]);
+        for (int i = 0; i < 4 * depth; ++i) {
+            uint64_t *bar = (i & 2 ? rest_landed : x_landed)[group] + i / 4;
+            for (const long long t0 = clock64(); !mbar_try(bar, i & 1) && clock64() - t0 < kDrainLimitCycles;) {}
+        }
     }
 }
 
