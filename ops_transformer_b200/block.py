@@ -79,17 +79,19 @@ class QuantMoeBlock:
 
     def __call__(self, x, residual=None, *, adapter_ids=None, token_mask=None, leave: Optional[BlockExit] = None,
                  balance: Optional[float] = None):
-        """(the block's output fp32 [tokens, hidden], the new residual stream) for the layer's hidden states ``x`` and ``residual``.  ``x`` may
-        be what the block before left as ``Entered``, without a residual; with ``leave`` that is what this one returns for the next, in
-        the place of the two.  ``adapter_ids`` (int32 [tokens]): the adapter of every token, negative for none.  ``token_mask``: rows without a
-        token, which take part in no expert.  With ``balance``, a coefficient, the load of the experts follows: ``expert_balance``'s
-        (loss, counts, weight)."""
+        """(the block's output fp32 [tokens, hidden], the new residual stream) for the layer's hidden states ``x`` and ``residual``; without a
+        residual the stream is ``x`` itself, as in a model's first layer.  ``x`` may be what the block before left as ``Entered``, without a
+        residual; with ``leave`` that is what this one returns for the next, in the place of the two.  ``adapter_ids`` (int32 [tokens]): the
+        adapter of every token, negative for none.  ``token_mask``: rows without a token, which take part in no expert.  With ``balance``, a
+        coefficient, the load of the experts follows: ``expert_balance``'s (loss, counts, weight)."""
         if isinstance(x, Entered):
             if residual is not None:
                 raise ValueError("rows that have entered the block bring their residual stream")
             rows, scales, stream, normed = x
         else:
             rows, scales, stream, normed = add_rms_norm_quant(x, self.gamma, residual=residual, eps=self.eps, normed=True)
+            if residual is None:
+                stream = x
         tokens, E = rows.shape[0], self.experts
         logits = normed @ self.router
         weights, ids = route_top_k(logits, self.top_k, bias=self.router_bias, token_mask=token_mask, **self.routing)
