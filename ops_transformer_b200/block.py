@@ -44,7 +44,8 @@ class Entered(NamedTuple):
 @dataclasses.dataclass
 class BlockExit:
     """The way from a block's output into the next block: ``gamma`` of the next block's norm, and the optional parts of
-    ``sandwich_norm_quant`` that the model has (the block's own norm, its gate, the scales of the residual sum)."""
+    ``sandwich_norm_quant`` that the model has (the block's own norm, its gate, the scales of the residual sum, the scales that the next block's
+    int8 weights were smoothed with)."""
     gamma: torch.Tensor
     post_gamma: Optional[torch.Tensor] = None
     gate: Optional[torch.Tensor] = None
@@ -53,11 +54,12 @@ class BlockExit:
     block_scale: float = 1.0
     eps: float = 1e-6
     post_eps: Optional[float] = None
+    smooth: Optional[torch.Tensor] = None
 
     def __call__(self, out, stream) -> Entered:
         return Entered(*sandwich_norm_quant(out, stream, self.gamma, post_gamma=self.post_gamma, gate=self.gate, gate_act=self.gate_act,
                                             residual_scale=self.residual_scale, block_scale=self.block_scale, eps=self.eps,
-                                            post_eps=self.post_eps, normed=True))
+                                            post_eps=self.post_eps, smooth=self.smooth, normed=True))
 
 
 class QuantMoeBlock:

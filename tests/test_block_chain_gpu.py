@@ -36,3 +36,21 @@ def test_first_block_has_no_residual(tokens):
     assert ((entered.stream.double() - other.stream.double()).abs() <= other.stream.double().abs() * 2.0 ** -7 + 2.0 ** -15 * other.stream.double().abs().amax(1, keepdim=True)).all()
     out, stream = second(entered)
     assert torch.equal(stream, entered.stream) and out.isfinite().all()
+
+
+@pytest.mark.parametrize("tokens", [3, 300])
+def test_way_into_a_block_with_smoothed_weights(tokens):
+    """The smoothing scales multiply what is quantised, and neither the stream nor the rows that the router reads."""
+    first, second = (random_block(512, 256, 8, 2, seed=s) for s in (0, 1))
+    x, residual = randn((tokens, 512), 1, BF16), randn((tokens, 512), 2, BF16)
+    out, stream = first(x, residual)
+    smooth = 2.0 ** torch.randint(-1, 2, (512,), device=DEV, generator=torch.Generator(DEV).manual_seed(3)).float()
+    plain, smoothed = BlockExit(second.gamma)(out, stream), BlockExit(second.gamma, smooth=smooth)(out, stream)
+    assert torch.equal(plain.stream, smoothed.stream) and torch.equal(plain.normed, smoothed.normed)
+    s = 1.0 * stream.double() + out.double()
+    u = s * (s.square().mean(1, keepdim=True) + 1e-6).rsqrt() * second.gamma.double() * smooth.double()
+    top = u.abs().amax(1, keepdim=True)
+    # half a step of 127, and a hundred units of fp32 for the norm (512 / 32 + 16 additions) and its products
+    assert ((smoothed.rows * smoothed.scales.double()[:, None] - u).abs() <= top / 127 * 0.5 + top * 100 * U32).all()
+    assert not torch.equal(plain.rows, smoothed.rows)
+    assert second(smoothed)[1] is smoothed.stream
