@@ -666,7 +666,8 @@ def expert_balance(logits: torch.Tensor, ids: torch.Tensor, *, scoring: str = "s
     ``coefficient * experts / top_k * sum_e (share of the tokens' choices that are e) * (mean of the tokens' scores of e)``, the mean of it
     over the sequences where ``cu_seqlens`` (int32 [sequences + 1]) names some.  ``loss`` is one fp32 number on the device, ``counts`` int64
     [experts] or [sequences, experts], ``weight`` fp32 [sequences]: what ``expert_balance_grad`` takes.  ``scoring`` "softmax" or "sigmoid" (divided
-    by the row's sum); ``token_mask`` (bool or int8 [rows]): rows without a token; negative ids are not counted.  gmmB200ExpertBalance
+    by the row's sum); ``token_mask`` (bool or int8 [rows]): rows without a token; negative ids are not counted.  The loss has no autograd history,
+    also where ``logits`` have one: added to another loss it brings no gradient, which is ``expert_balance_grad``'s.  gmmB200ExpertBalance
     (include/gmm_b200.h) has the formulas."""
     if stream is not None:   # what a call returns belongs to the stream that writes it
         with _on_stream(stream, logits.device):

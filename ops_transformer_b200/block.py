@@ -20,7 +20,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from .acl import (adapter_add, add_rms_norm_quant, expert_balance, format_cast_nz, grouped_matmul_finalize_routing,
+from .acl import (adapter_add, add_rms_norm_quant, expert_balance, expert_balance_grad, format_cast_nz, grouped_matmul_finalize_routing,
                   grouped_matmul_swiglu_quant, moe_init_routing_v3, quant_matmul, route_top_k, sandwich_norm_quant)
 
 
@@ -39,6 +39,23 @@ class Entered(NamedTuple):
     scales: torch.Tensor
     stream: torch.Tensor
     normed: torch.Tensor
+
+
+class Load(tuple):
+    """(loss, counts, weight) of ``expert_balance`` for the tokens of one call of a block, with what the gradient takes beside them.  ``loss`` is a
+    number without an autograd history; what trains the router is ``load.logits.backward(load.grad())``, whose logits have one if the block's
+    router requires gradients."""
+
+    def __new__(cls, result, logits, scoring, token_mask):
+        self = super().__new__(cls, result)
+        self.logits, self.scoring, self.token_mask = logits, scoring, token_mask
+        return self
+
+    loss, counts, weight = (property(lambda self, i=i: self[i]) for i in range(3))
+
+    def grad(self, grad_loss=None):
+        """The gradient of ``loss``, times ``grad_loss`` (one fp32 number on the device), with respect to ``logits``."""
+        return expert_balance_grad(self.logits, self.counts, self.weight, scoring=self.scoring, token_mask=self.token_mask, grad_loss=grad_loss)
 
 
 @dataclasses.dataclass
@@ -85,7 +102,7 @@ class QuantMoeBlock:
         residual the stream is ``x`` itself, as in a model's first layer.  ``x`` may be what the block before left as ``Entered``, without a
         residual; with ``leave`` that is what this one returns for the next, in the place of the two.  ``adapter_ids`` (int32 [tokens]): the
         adapter of every token, negative for none.  ``token_mask``: rows without a token, which take part in no expert.  With ``balance``, a
-        coefficient, the load of the experts follows: ``expert_balance``'s (loss, counts, weight)."""
+        coefficient, the load of the experts follows: ``expert_balance``'s (loss, counts, weight) as a ``Load``."""
         if isinstance(x, Entered):
             if residual is not None:
                 raise ValueError("rows that have entered the block bring their residual stream")
@@ -118,7 +135,8 @@ class QuantMoeBlock:
         result = (out, stream) if leave is None else leave(out, stream)
         if balance is None:
             return result
-        load = expert_balance(logits, ids, scoring=self.routing["scoring"], coefficient=balance, token_mask=token_mask)
+        scoring = self.routing["scoring"]
+        load = Load(expert_balance(logits, ids, scoring=scoring, coefficient=balance, token_mask=token_mask), logits, scoring, token_mask)
         return (*result, load) if leave is None else (result, load)
 
 

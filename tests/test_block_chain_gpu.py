@@ -54,3 +54,58 @@ def test_way_into_a_block_with_smoothed_weights(tokens):
     assert ((smoothed.rows * smoothed.scales.double()[:, None] - u).abs() <= top / 127 * 0.5 + top * 100 * U32).all()
     assert not torch.equal(plain.rows, smoothed.rows)
     assert second(smoothed)[1] is smoothed.stream
+
+
+@pytest.mark.parametrize("tokens,scoring", [(1, "softmax"), (50, "sigmoid"), (700, "softmax")])
+@pytest.mark.parametrize("last", [True, False])
+def test_a_router_is_trained_by_the_load_of_its_block(tokens, scoring, last):
+    """The block hands out what the balance loss is differentiated with: the router's gradient is the formula's."""
+    block, after = (random_block(512, 256, 16, 2, seed=s, scoring=scoring) for s in (0, 1))
+    router = block.router.t().detach().clone().requires_grad_(True)
+    block.router = router.t()
+    x, residual = randn((tokens, 512), 1, BF16), randn((tokens, 512), 2, BF16)
+    mask = torch.arange(tokens, device=DEV) % 4 != 3
+    *_, load = block(x, residual, token_mask=mask, balance=0.01, leave=None if last else BlockExit(after.gamma))
+    loss, counts, weight = load
+    assert loss is load.loss and counts is load.counts and weight is load.weight and not loss.requires_grad
+    scale = torch.tensor(1000.0, device=DEV)
+    grad = load.grad(scale)
+    load.logits.backward(grad)
+
+    normed = ops.add_rms_norm_quant(x, block.gamma, residual=residual, normed=True)[3]
+    logits = load.logits.detach().double().requires_grad_(True)
+    assert torch.equal(load.logits, normed @ block.router)
+    p = logits.softmax(1) if scoring == "softmax" else logits.sigmoid() / logits.sigmoid().sum(1, keepdim=True)
+    n = int(mask.sum())
+    want = 0.01 * 16 / (2 * n * n) * (counts * (p * mask[:, None]).sum(0)).sum()
+    (1000.0 * want).backward()
+    # p's errors are some units of fp32 (logits of about 3), a sum over `tokens` of them
+    assert abs(loss.item() - want.item()) <= want.item() * (tokens + 100) * U32
+    # every element within half a unit of bf16 of its own, and some units of fp32 of the largest of its row's products before they cancel
+    size = (p * 0.01 * 16 / (2 * n * n) * counts.max() * 1000).detach()
+    assert ((grad.double() - logits.grad).abs() <= logits.grad.abs() * 2.0 ** -8 + size * 100 * U32).all()
+    # the product with `normed` in bf16, fp32 sums of up to 700 terms, one rounding
+    want_router = grad.double().t() @ normed.double()
+    assert (router.grad.double() - want_router).norm() <= want_router.norm() * 2.0 ** -7
+    assert (grad[~mask] == 0).all()
+
+
+def test_load_of_a_captured_block():
+    """Loss, counts and gradient of a replay are those of its inputs."""
+    block = random_block(512, 256, 16, 2)
+    x, residual = randn((24, 512), 1, BF16), randn((24, 512), 2, BF16)
+    mask = torch.arange(24, device=DEV) < 20
+
+    def step():
+        out, stream, load = block(x, residual, token_mask=mask, balance=0.01)
+        return (*load, load.grad())
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in (3, 4):
+        x.copy_(randn((24, 512), seed, BF16))
+        mask[:seed] = False
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
