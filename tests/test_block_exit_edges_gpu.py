@@ -238,3 +238,30 @@ def test_matmul_options_do_not_hang_on_the_size(m, k, n):
             took[cap] = min(took.get(cap, 1e9), start.elapsed_time(stop))
             assert torch.equal(got, want)
     assert 0 < took[0] < 1 and took[2] < 4 * took[0] + 0.01   # two CTAs of 148 would take 70 times as long for the large ones
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# scales and biases that leave the result's type, element by element
+# ---------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("m,k,n", [(4, 65535, 64), (40, 2048, 512), (3, 100, 77), (1500, 1536, 4096)])
+@pytest.mark.parametrize("special", ["scale", "token", "bias", "all"])
+def test_matmul_extreme_scales_element_by_element(m, k, n, dtype, special):
+    """Overflow, infinities, NaN and zeros in scales and bias: every element as the same steps in fp32 give it, with its sign."""
+    x, w = int8((m, k), 1), int8((k, n), 2)
+    x[0], w[:, 0] = -128, -128
+    x[1], w[:, 1] = 127, 127
+    scale, token, bias = torch.ones(n, device=DEV), torch.ones(m, device=DEV), torch.zeros(n, device=DEV)
+    odd = torch.tensor([float("inf"), -float("inf"), float("nan"), 0.0, -0.0, 1e38, -3e38, 1e-38], device=DEV)
+    if special in ("scale", "all"):
+        scale[:64] = odd.repeat(8)
+    if special in ("token", "all"):
+        token[:min(m, 8)] = odd[:min(m, 8)]
+    if special in ("bias", "all"):
+        bias[8:72 if n >= 72 else n] = odd.repeat(8)[:min(64, n - 8)]
+    got = ops.quant_matmul(x, w, scale, token, bias=bias, out_dtype=dtype)
+    want = ((x.double() @ w.double()).float() * scale * token[:, None] + bias).to(dtype)
+    torch.testing.assert_close(got, want, rtol=0, atol=0, equal_nan=True)
+    if special == "scale":   # the same without what the calls need not have
+        torch.testing.assert_close(ops.quant_matmul(x, w, scale, out_dtype=dtype), ((x.double() @ w.double()).float() * scale).to(dtype), rtol=0, atol=0, equal_nan=True)
