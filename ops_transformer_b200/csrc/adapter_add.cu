@@ -40,6 +40,7 @@ constexpr int kWorkers = 256;        // threads of the first kernel that copy; o
 __host__ __device__ constexpr int expand_workers(int tn) { return tn == 64 ? 512 : 256; }
 constexpr int kMaxStages = 6, kShrinkAhead = 2, kExpandStages = 2;
 constexpr long long kWaitLimitCycles = 1ll << 31;   // of a call that names no other: about a second
+constexpr long long kDrainLimitCycles = 1ll << 24;  // at least, of waits for what is under way: a few milliseconds
 
 struct AdapterParams {
     const void *base, *x, *a, *b;
@@ -90,11 +91,12 @@ __device__ __forceinline__ void mbar_arrive_copies(uint32_t bar) { asm volatile(
 template <int THREADS>
 __device__ __forceinline__ void worker_sync() { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); }
 // Bounded wait for the tensor cores, or for the copies that they wait for.  When it runs out the status says so and later waits of the CTA
-// return at once, except those that LAST stands for: behind one, nothing that the CTA has under way may be left.
+// return at once, except those that LAST stands for: behind one, nothing that the CTA has under way may be left, however short the limit.
 template <bool LAST>
 __device__ __noinline__ void mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int *gave_up, int *status, long long limit, int role)
 {
     const long long t0 = clock64();
+    if (LAST && limit < kDrainLimitCycles) limit = kDrainLimitCycles;
     while (!mbar_try(bar, parity)) {
         if (!LAST && *gave_up) return;
         if (clock64() - t0 > limit) {
@@ -902,7 +904,7 @@ template <typename T, int TN, int GB>
 __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) adapter_expand_kernel(const AdapterParams p)
 {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ alignas(8) uint64_t full[kExpandStages], acc_full[2], acc_empty[2], v_full;
+    __shared__ alignas(8) uint64_t full[kExpandStages], acc_full[2], acc_empty[2], v_full, done;
     __shared__ uint32_t tmem_base;
     __shared__ int gave_up;
     __shared__ int rows[TN];
@@ -920,6 +922,7 @@ __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) ada
             mbar_init(smem_u32(&acc_empty[i]), WORKERS / 32);
         }
         mbar_init(smem_u32(&v_full), WORKERS / 32);
+        mbar_init(smem_u32(&done), 1);
         gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -1023,8 +1026,10 @@ __global__ void __launch_bounds__(expand_workers(TN) + 32, TN == 64 ? 2 : 1) ada
                 }
                 __syncwarp();
             }
-            // all products are done, also where the others have given up
-            mbar_wait<true>(smem_u32(&acc_full[(c1 - 1 - c0) & 1]), ((c1 - 1 - c0) / 2) & 1, &gave_up, p, 915);
+            // All products are done, also where the others have given up: then a buffer's barrier may be two products behind, with the same parity.
+            if (lane == 0) umma_commit(smem_u32(&done));
+            __syncwarp();
+            mbar_wait<true>(smem_u32(&done), 0, &gave_up, p, 915);
         } else {
             // Copies through shared memory by whole 16 bytes announce themselves; others are waited for, a chunk ahead.
             const auto announce = [&](int c) {

@@ -265,3 +265,30 @@ def test_matmul_extreme_scales_element_by_element(m, k, n, dtype, special):
     torch.testing.assert_close(got, want, rtol=0, atol=0, equal_nan=True)
     if special == "scale":   # the same without what the calls need not have
         torch.testing.assert_close(ops.quant_matmul(x, w, scale, out_dtype=dtype), ((x.double() @ w.double()).float() * scale).to(dtype), rtol=0, atol=0, equal_nan=True)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# adapter_add: limits that are shorter than what is under way takes
+# ---------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("is_int8", [False, True])
+@pytest.mark.parametrize("tokens,adapters,k,n,rank", [(300, 2, 4096, 4096, 16), (300, 60, 2048, 520, 16), (2100, 2, 512, 3000, 64), (300, 2, 1001, 3001, 61)])
+def test_adapter_leaves_nothing_under_way_when_a_wait_runs_out(tokens, adapters, k, n, rank, is_int8):
+    """The kernels end only when their products have, and what runs next in the same tensor memory is right."""
+    base, a, b = randn((tokens, n), 1, BF16), randn((adapters, rank, k), 2, BF16, k ** -0.5), randn((adapters, n, rank), 3, BF16, rank ** -0.5)
+    x = int8((tokens, k), 4) if is_int8 else randn((tokens, k), 4, BF16)
+    kw = dict(x_scale=torch.rand(tokens, device=DEV, generator=gen(5)) / 64 if is_int8 else None)
+    ids = (torch.arange(tokens, device=DEV) % adapters).to(I32)
+    want, ws = ops.adapter_add(base, x, a, b, ids, return_workspace=True, **kw)
+    ops.check_status(ws)
+    mine = torch.zeros(ws.numel(), dtype=torch.uint8, device=DEV)
+    for limit in (100, 1000, 3000, 10_000, 100_000):
+        got = ops.adapter_add(base, x, a, b, ids, workspace=mine, options=ops.LaunchOptions(wait_limit_cycles=limit), **kw)
+        again = [ops.adapter_add(base, x, a, b, ids, **kw) for _ in range(2)]
+        assert all(torch.equal(t, want) for t in again)
+        try:
+            ops.check_status(mine)
+        except ops.AclnnError as error:
+            assert error.record[0] == 1
+            continue
+        assert torch.equal(got, want)
