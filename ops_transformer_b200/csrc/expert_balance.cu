@@ -9,9 +9,10 @@
 // steps of sums and maxima across them, and of all that a row costs once.  Sums over tokens are made in a fixed order (a lane's rows one
 // after the other, then the groups, then the pieces), so that a call gives the same bits every time.
 //
-// Measured, us (forward, gradient): 16 x 64 bf16 2.2, 2.0; 256 x 256 bf16 4.0, 2.3; 4096 x 256 bf16 7.2, 3.8; 16384 x 256 fp32 in 16 sequences 12.7, 9.1; 65536 x 256 bf16
-// 17.0, 17.7 (2 TB/s and 3.8).  Loads' latency bounds the large ones: with no scores and no ids to work on 65536 rows take 12.0, each of the
-// two adds about 4.6, and half the instructions (16 lanes a row for 32) changed nothing.
+// Measured, us (forward, gradient): 16 x 64 bf16 2.2, 2.0; 256 x 256 bf16 4.0, 2.3; 4096 x 256 bf16 7.3, 3.8; 4096 x 1024 bf16 13.3, 8.7; 16384 x 256 fp32 in 16
+// sequences 12.7, 9.1; 65536 x 256 bf16 17.5, 17.7 (2 TB/s and 3.8).  Loads' latency bounds the large ones: with no scores and no ids to work
+// on 65536 rows take 12.0, each of the two adds about 4.6, and half the instructions (16 lanes a row for 32) changed nothing.  Rows on their
+// way are held in registers, of which one or two rows a group are all that there is room for; by way of shared memory was not tried.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -585,7 +586,8 @@ __global__ void __launch_bounds__(kFinishThreads) balance_finish_many_kernel(con
 }
 
 // A warp holds a row: its loads are the longest part of it, and more warps hide more of them than a row's fewer instructions in fewer lanes
-// would gain (4096 x 256 4.0 us, with 16 lanes a row 4.1; 16384 x 256 in fp32 9.2 and 10.4).
+// would gain (4096 x 256 4.0 us, with 16 lanes a row 4.1; 16384 x 256 in fp32 9.2 and 10.4).  Above 512 experts a lane's 32 values do not fit
+// its 128 registers, and 0.1 to 0.6 KB a thread go through local memory: 4096 x 512 in bf16 5.0, x 1024 8.7, x 513, on no pack, 9.7.
 template <typename T, bool SIGMOID, int PER, int V>
 __global__ void __launch_bounds__(kGradThreads, PER <= 8 ? 4 : 2) balance_grad_kernel(const BalanceParams p)
 {

@@ -7,9 +7,11 @@
 // sums are exact in any order, so there is nothing to put in sequence and no workspace for it.
 //
 // Measured, us: 16 x 768 -> 2048 3.7, 16 x 7168 -> 4096 9.7 (29 MB, 3.0 TB/s: a third of it is the launch, the first bytes' way and the
-// sums'), 128 tokens of it 11.3, 256 13.3, 1024 25.3, 1024 x 2048 -> 2048 8.5, 611 x 1424 -> 2976 9.1.  From about 2000 tokens of 7168 on the
-// persistent kernel of the grouped product (two SMs a tile, epilogue beside the next tile's MMAs) is faster, and takes the call: 4096 tokens
-// 78 against 95, of the 77 that the tensor cores take at twice the 16-bit rate.
+// sums'), 128 tokens of it 11.4, 256 13.8, 1024 26.0, 1024 x 2048 -> 2048 8.8, 611 x 1424 -> 2976 8.4.  A CTA has one tile, so that the first
+// bytes' way, the K blocks and the end follow one another: with hundreds of tokens, of which memory and tensor cores want a third to a fifth
+// of that time, that is what it goes to.  From about 2000 tokens of 7168 on the persistent kernel of the grouped product (two SMs a tile,
+// epilogue beside the next tile's MMAs) is faster, and takes the call: 4096 tokens 78 against 95, of the 77 that the tensor cores take at
+// twice the 16-bit rate.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -546,8 +548,11 @@ double at_tokens(const double (&v)[4], int tokens)
 
 // Smaller tiles and K splits bring more CTAs to the weights, larger tiles read them less often, and a split has its sums sent around.  What
 // is best is where the estimate below is least: its parts were fitted to times of all ways over 165 sizes (1 to 4096 tokens, K and N of 256
-// to 8192), where the way that it picks takes 1 % longer than the best one on average and 14 % at most.  A K block takes 0.16 us at 32
-// tokens and 0.40 at 256 (what an SM gets from L2, 110 bytes per ns, bounds both), the end of a tile 0.4 to 2.9 us, a split 1.4 to 2.6.
+// to 8192; in replayed graphs, with as many sets of operands in turn as make 300 MB and twelve at most, so that weights of more than 10 MB
+// come from memory and smaller ones from L2), where the way that it picks takes 1 % longer than the best one on average and 14 % at most.
+// It ranks ways and is no forecast: one memory rate for both places and no share of the launch make it up to a quarter too low (16 x 7168
+// -> 4096 with 32/4 7.0 for 9.4).  A K block takes 0.16 us at 32 tokens and 0.40 at 256 (what an SM gets from L2, 110 bytes per ns, bounds
+// both), the end of a tile 0.4 to 2.9 us, a split 1.4 to 2.6.
 // Some of the measured times (us), tile tokens / split: 16 x 7168 -> 4096 32/1 14.1, 32/2 11.0, 32/4 9.4; 16 x 2048 -> 7168 32/1 6.5, 32/4
 // 7.2; 256 x 7168 -> 4096 256/2 17.8, 128/1 17.4, 128/2 13.3; 1024 x 2048 -> 2048 256/1 11.2, 128/1 8.5, 64/1 9.2, 128/2 16.2.
 Shape shape_with(const QuantMatmulProblem &q, int most_tokens, int split)
@@ -561,7 +566,9 @@ Shape shape_with(const QuantMatmulProblem &q, int most_tokens, int split)
     s.split = split;
     const int blocks = (int)((q.k + kBlockK - 1) / kBlockK), each = (blocks + split - 1) / split;
     const double ctas = (double)s.token_tiles * s.channel_tiles * split;
-    // two CTAs on an SM where tiles are small, or of medium size and more than the SMs
+    // room for two CTAs on an SM where tiles are small, or of medium size and more than the SMs.  Small ones leave it where the grid is smaller
+    // than the SMs, too, since calls in a row overlap in it (32 tokens, 7168 -> 4096, 32/4 9.6 us, with a ring over all of the memory 10.1; 4096
+    // -> 4096 7.7 and 8.3; over 368 such pairs of times the two are equal on average).
     const bool two = s.tile_tokens <= 64 || (s.tile_tokens <= 128 && ctas > kSms);
     const size_t stage = kWeightStage + (size_t)s.tile_tokens * kBlockK, room = (two ? 109 : 220) * 1024;
     const size_t sums = (size_t)s.tile_tokens * kTokenBytes, parts = sums / split * (split - 1);

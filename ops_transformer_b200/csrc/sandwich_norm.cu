@@ -238,7 +238,7 @@ __device__ __forceinline__ void load_gammas(const void *vec, bool gamma32, int a
 // One CTA per row; a thread holds NCH packs of V elements (16 bytes of T), blockDim.x apart, in fp32 from the first look at x to the last
 // store.  WHOLE: rows start on packs.  Else every row starts `lead` elements into one, the same in all tensors, and only what lies in a row's
 // first and last pack is masked and stored one element at a time.  Its time is a row's chain of load, sum, load, sum and store (16 x 2048 2.7 us,
-// 128 x 7168 4.9, 600 x 16384 with four packs a thread 24).
+// 128 x 7168 4.9); the second loads stand behind the first sum, although none of them needs it.
 template <typename T, typename X, int NCH, bool WHOLE, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) sandwich_kernel(const SandwichParams p)
 {
@@ -416,8 +416,9 @@ __global__ void __launch_bounds__(MAXT, MINB) sandwich_kernel(const SandwichPara
 // turn has no loads but its own.  Those come as one bulk copy a tensor, for the next row as soon as the group holds this one in registers.
 // (With a 16-byte cp.async for each pack an SM takes in 16 bytes per ns however many are under way: 4096 x 7168 in 80 us.)  A group's
 // threads hold two packs each; four would leave too few rows in turn for the chain load, sum, load, sum, store of each.
-// 4096 x 7168, fp32 x, bf16 stream: 53.3 us with int8 rows (270 MB, 5.1 TB/s), 49.0 with bf16 rows and a gate (294 MB, 6.0 TB/s); 5001
-// channels, whose rows begin anywhere, 52.7.  Quantising costs what the difference is: max, step and rounding are the issue slots' work.
+// 4096 x 7168, fp32 x, bf16 stream: 53.4 us with int8 rows (264 MB, 4.9 TB/s), 48.1 with bf16 rows and a gate (294 MB, 6.1 TB/s).  Quantising
+// costs what the difference is: max, step and rounding are the issue slots' work.  5001 channels, whose rows begin anywhere, take 52.6 and 5008
+// take 42.9: eight single reads of a factor for two wide ones, and rows' ends element by element.  600 x 16384 24.3.
 constexpr int kGroupPacks = 2, kMaxGroups = 14, kMaxDepth = 3;    // of the 15 named barriers that are left
 constexpr long long kWaitLimitCycles = 1ll << 31, kDrainLimitCycles = 1ll << 20;   // about a second, half a millisecond
 constexpr int kGroupThreads = 1024;
