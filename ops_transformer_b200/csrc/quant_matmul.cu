@@ -8,8 +8,8 @@
 //
 // Measured, us: 16 x 768 -> 2048 3.7, 16 x 7168 -> 4096 9.7 (29 MB, 3.0 TB/s: a third of it is the launch, the first bytes' way and the
 // sums'), 128 tokens of it 11.4, 256 13.8, 1024 26.0, 1024 x 2048 -> 2048 8.8, 611 x 1424 -> 2976 8.4.  A CTA has one tile, so that the first
-// bytes' way, the K blocks and the end follow one another: with hundreds of tokens, of which memory and tensor cores want a third to a fifth
-// of that time, that is what it goes to.  From about 2000 tokens of 7168 on the persistent kernel of the grouped product (two SMs a tile,
+// bytes' way, the K blocks and the end follow one another: with 100 to 600 tokens memory or the tensor cores would take a fifth to three
+// fifths of these times.  From about 2000 tokens of 7168 on the persistent kernel of the grouped product (two SMs a tile,
 // epilogue beside the next tile's MMAs) is faster, and takes the call: 4096 tokens 78 against 95, of the 77 that the tensor cores take at
 // twice the 16-bit rate.
 #include <cuda_bf16.h>

@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(MAXT, MINB) sandwich_kernel(const SandwichPara
 // costs what the difference is: max, step and rounding are the issue slots' work.  5001 channels, whose rows begin anywhere, take 52.6 and 5008
 // take 42.9: eight single reads of a factor for two wide ones, and rows' ends element by element.  600 x 16384 24.3.
 constexpr int kGroupPacks = 2, kMaxGroups = 14, kMaxDepth = 3;    // of the 15 named barriers that are left
-constexpr long long kWaitLimitCycles = 1ll << 31, kDrainLimitCycles = 1ll << 20;   // about a second, half a millisecond
+constexpr long long kWaitLimitCycles = 1ll << 31, kDrainLimitCycles = 1ll << 22;   // about a second, two milliseconds
 constexpr int kGroupThreads = 1024;
 // Packs that a row can touch, and floats of a vector of factors.
 template <int V, bool WHOLE> __host__ __device__ inline int most_packs(int h) { return WHOLE ? h / V : (h + 2 * V - 2) / V; }
